@@ -76,6 +76,14 @@ extern "C" {
 #define RELUX_POOL_FLAG_REFERENCE_COMPAT 1   /* keep what RELUX_ATTN_REFERENCE_FAITHFUL needs: the chunk boundaries of every
                                                 Append (GQA), a float32 copy of every appended row (MLA) */
 
+/* 8-bit cache (GQA pools with page_tokens = 64 and head_dim = 128): of every cached row, per kv head, 128 whole numbers of
+ * [-127, 127] and one float32 scale, 264 bytes of K and V a token and kv head instead of 512.  With a the largest magnitude of the row's
+ * 128 values, scale = a / 127 and number = value * (127 / a) to the nearest, even on a tie, each operation rounded to float32; a row with
+ * a < 1e-36 is stored as zeros, one that holds an infinity or a NaN reads back as NaN in every place.  Rows are quantised as they are
+ * appended, attention takes number * scale for the value, relux_pool_read_rows, relux_seq_save_file and relux_gqa_read_kv give it.
+ * All calls of a GQA pool take such a pool in RELUX_ATTN_FAST; the two reference modes and relux_gqa_decode_noalloc refuse it. */
+#define RELUX_POOL_FLAG_CACHE_INT8 2
+
 typedef void* relux_device_t;
 typedef void* relux_pool_t;
 typedef void* relux_event_t;
@@ -133,7 +141,7 @@ int32_t relux_cuda_flush_l2(relux_device_t dev);
  *   GQA: KVCache / NewKVCacheSized   internal/transformer/kvcache.go:34-49, 66-93
  *   MLA: MLACache / NewMLACache      internal/transformer/mla_cache.go:21-59
  *   storage: internal/alloc/alloc.go:95-117,168-188 (64 MiB power-of-two freelist buckets)
- * Storage is bf16.  One pool serves num_layers layers and up to max_seqs sequences; a sequence
+ * Storage is bf16 (or 8-bit: RELUX_POOL_FLAG_CACHE_INT8).  One pool serves num_layers layers and up to max_seqs sequences; a sequence
  * owns a page table of up to max_pages_per_seq physical page ids shared by all layers, and a
  * length per layer (the reference keeps one cursor per layer: kvcache.go:44-49).
  * MLA page  : [page_tokens][dC + dHR] (latent row followed by the rotated shared key).
@@ -201,6 +209,23 @@ typedef struct relux_read_rows_args {
   int32_t reserved[4];
 } relux_read_rows_args;
 int32_t relux_pool_read_rows(relux_pool_t pool, const relux_read_rows_args* args);
+
+/* Cached K and V rows of a batch of sequences, copied to dense device memory as float32 or bf16: tokens tok0[i] .. tok0[i] +
+ * n_tokens[i] - 1 of every named sequence, one sequence behind the other, on one layer or on all.  An 8-bit cache's rows are number *
+ * scale, rounded once; a bf16 cache's are its bits.  Asynchronous on the handle's stream.  KVCache.View (kvcache.go:363-380) for
+ * a batch, without the way through host memory. */
+typedef struct relux_read_kv_args {
+  int32_t layer;             /* < 0: every layer, results [num_layers][sum of n_tokens][...] */
+  int32_t n_seqs;
+  const int32_t* seq_ids;    /* host [n_seqs]; NULL = 0..n_seqs-1 */
+  const int32_t* tok0;       /* host [n_seqs]; NULL = 0 */
+  const int32_t* n_tokens;   /* host [n_seqs]; rows past a sequence's length are returned as stored */
+  int32_t dtype;             /* RELUX_DTYPE_* of k and v */
+  int32_t reserved[3];
+  void* k;                   /* device [sum of n_tokens][num_kv_heads][head_dim] */
+  void* v;
+} relux_read_kv_args;
+int32_t relux_gqa_read_kv(relux_pool_t pool, const relux_read_kv_args* args);
 
 /* Tuning knobs of relux_pool_tune. */
 #define RELUX_TUNE_MLA_GENERIC 0        /* RELUX_MLA_GENERIC: 1 = MLA decode on the CUDA-core kernels                      */
@@ -324,6 +349,38 @@ int32_t relux_gqa_step(relux_pool_t pool, const relux_append_args* append, const
  * extra_tokens = q_tokens.  Commit the accepted prefix with relux_seq_set_len afterwards. */
 int32_t relux_gqa_verify(relux_pool_t pool, const relux_attn_args* attn, const relux_append_args* draft_kv);
 int32_t relux_mla_verify(relux_pool_t pool, const relux_attn_args* attn, const relux_append_args* draft_kv);
+
+/* Verify of drafted TREES in one call: several continuations of every sequence at once, where relux_gqa_verify takes one.  Node j of a
+ * tree continues node parents[j] < j, or (-1) the cached rows.  The call writes the nodes' K / V rows past the cursors (draft_kv: advance
+ * = 0, n_new = nodes of every sequence, NULL = q_tokens of each; packed, as in relux_gqa_append), then query token j of a sequence
+ * attends to all its cached rows, to itself and to its ancestors.  attn->causal is not read, attn->extra_tokens must be 0; q and out are
+ * [n_seqs][q_tokens][...], and rows past a sequence's nodes come out as zeros.  Positions for RoPE are the caller's: cached length plus depth.
+ * An infinity or a NaN in a row past the cursor (a node's, or what an older draft has left) reaches the outputs of the queries that see it
+ * and no others; where it is among a node's values, all of the output of that head becomes NaN.
+ * Shapes: GQA pools (bf16 or 8-bit) with page_tokens = 64 and head_dim = 128, num_heads / num_kv_heads <= 32, up to 64 nodes,
+ * RELUX_ATTN_FAST; others are refused.  Commit what was accepted with relux_gqa_tree_commit.  No counterpart in the reference, whose
+ * speculative decoder drafts one chain (speculative.go:189-207). */
+typedef struct relux_tree_args {
+  const int32_t* parents;    /* host [n_trees][q_tokens]; entries past a sequence's nodes are not read */
+  int32_t n_trees;           /* n_seqs, or 1: the same tree for every sequence (its first nodes where a sequence has fewer) */
+  int32_t reserved[3];
+} relux_tree_args;
+int32_t relux_gqa_tree_verify(relux_pool_t pool, const relux_attn_args* attn, const relux_append_args* draft_kv, const relux_tree_args* tree);
+
+/* Commits the accepted path of a tree: the rows of nodes path[i][0] < path[i][1] < ... of sequence i, which relux_gqa_tree_verify wrote
+ * past its cursor, move to the places behind the cursor, in that order, and its length grows by path_len[i] (0: nothing happens to it).
+ * One layer or all.  Lengths are the device's, as in an append.  That the path is one of the tree's is the caller's word.  No counterpart in
+ * the reference: its speculative decoder never removes rejected draft rows from the cache (speculative.go:136-156). */
+typedef struct relux_tree_commit_args {
+  int32_t layer;             /* < 0: every layer */
+  int32_t n_seqs;
+  const int32_t* seq_ids;    /* host [n_seqs]; NULL = 0..n_seqs-1 */
+  const int32_t* path;       /* host [n_seqs][path_stride] */
+  const int32_t* path_len;   /* host [n_seqs], up to 64 */
+  int32_t path_stride;
+  int32_t reserved[3];
+} relux_tree_commit_args;
+int32_t relux_gqa_tree_commit(relux_pool_t pool, const relux_tree_commit_args* args);
 
 /* One MLA attention layer step, device-resident end to end: MLA.forwardCached (mla.go:272-397) for a batch of
  * independent sequences.  x [n_seqs][q_tokens][d_model] float32 (host or device) is projected with the reference's

@@ -167,17 +167,17 @@ class PinnedArray:
 
 
 class Pool:
-    """Paged bf16 KV pool on one device (see relux_pool_create in include/relux_cuda.h)."""
+    """Paged KV pool on one device, bf16 or (cache_int8, grouped-query pools) 8-bit (see relux_pool_create in include/relux_cuda.h)."""
 
     def __init__(self, dev, kind, num_layers, num_pages, page_tokens=64, max_seqs=1, max_pages_per_seq=None, dC=0, dHR=0,
-                 num_kv_heads=0, head_dim=0, reference_compat=False):
+                 num_kv_heads=0, head_dim=0, reference_compat=False, cache_int8=False):
         self.dev = dev
         self.lib = dev.lib
         if max_pages_per_seq is None:
             max_pages_per_seq = num_pages
         prm = L.PoolParams(kind=kind, num_layers=num_layers, num_pages=num_pages, page_tokens=page_tokens, max_seqs=max_seqs,
                            max_pages_per_seq=max_pages_per_seq, mla_dc=dC, mla_dhr=dHR, gqa_num_kv_heads=num_kv_heads,
-                           gqa_head_dim=head_dim, flags=L.POOL_FLAG_REFERENCE_COMPAT if reference_compat else 0)
+                           gqa_head_dim=head_dim, flags=(L.POOL_FLAG_REFERENCE_COMPAT if reference_compat else 0) | (L.POOL_FLAG_CACHE_INT8 if cache_int8 else 0))
         self.prm = prm
         self.kind = kind
         h = C.c_void_p()
@@ -235,6 +235,24 @@ class Pool:
         args = L.ReadRowsArgs(layer=layer, seq_id=seq, tok0=tok0, n_tokens=n, dst_a=a.ctypes.data, dst_b=b.ctypes.data)
         L.check(self.lib.relux_pool_read_rows(self.h, C.byref(args)))
         return a, b
+
+    def read_kv(self, layer, n_seqs, k, v, tok0, n_tokens, seq_ids=None, dtype=None):
+        """Cached rows of a batch into dense device memory (relux_gqa_read_kv): tokens tok0[i] .. tok0[i] + n_tokens[i] - 1 of every sequence, as
+        k and v [sum of n_tokens, num_kv_heads, head_dim], on every layer where layer < 0.  k, v: device buffers, or addresses with dtype."""
+        for a in (k, v):
+            if not isinstance(a, (DeviceBuffer, int)):
+                raise TypeError("read_kv: k and v must be device memory (read_rows gives host arrays)")
+        ids, t0, n = (None if x is None else np.ascontiguousarray(x, dtype=np.int32) for x in (seq_ids, tok0, n_tokens))
+        for x in (ids, t0, n):
+            if x is not None and x.size != n_seqs:
+                raise ValueError("read_kv: an array of %d entries for %d sequences" % (x.size, n_seqs))
+        if isinstance(k, DeviceBuffer) and n is not None:
+            need = int(n.sum()) * self.prm.gqa_num_kv_heads * self.prm.gqa_head_dim * (4 if _dtype_flag(k, dtype) == L.DTYPE_F32 else 2)
+            need *= self.prm.num_layers if layer < 0 else 1
+            if min(b.nbytes for b in (k, v) if isinstance(b, DeviceBuffer)) < need:
+                raise ValueError("read_kv: %d bytes needed" % need)
+        L.check(L.packed["gqa_read_kv"](self.h, L.pack_read_kv(layer, n_seqs, _ptr(ids) or 0, _ptr(t0) or 0, _ptr(n) or 0, _dtype_flag(k, dtype),
+                                                               _ptr(k) or 0, _ptr(v) or 0)))
 
     def wait_output(self, calls_back=0):
         """Blocks until the host output of a pipelined attention call has landed (0: the latest call, 1: the one before)."""
@@ -371,6 +389,34 @@ class Pool:
         at, self._keep2 = self._pack_attn(layer, n_seqs, q, q_rope, out, num_heads, head_dim, scale, q_tokens, q_tokens, True, mode, w_uk,
                                           w_uv, seq_ids, L.LAYOUT_TOKEN_MAJOR, L.LAYOUT_TOKEN_MAJOR, q_dtype, out_dtype, pipelined)
         L.check(self._fn("verify")(self.h, at, ap))
+
+    def tree_verify(self, layer, n_seqs, q, out, draft_k, draft_v, num_heads, head_dim, scale, parents, n_nodes=None, mode=L.ATTN_FAST,
+                    seq_ids=None, kv_layout=L.LAYOUT_TOKEN_MAJOR, q_layout=L.LAYOUT_TOKEN_MAJOR, out_layout=L.LAYOUT_TOKEN_MAJOR, q_dtype=None,
+                    out_dtype=None, kv_dtype=None, pipelined=False):
+        """Verify of drafted trees (relux_gqa_tree_verify): parents [q_tokens] (one tree for all) or [n_seqs, q_tokens], node j's parent or -1; q and
+        out [n_seqs, q_tokens, H, D]; draft_k, draft_v the nodes' rows, n_nodes[i] of sequence i (None: q_tokens each), packed."""
+        par = np.ascontiguousarray(parents, dtype=np.int32)
+        if par.ndim == 1:
+            par = par[None]
+        if par.ndim != 2 or par.shape[0] not in (1, n_seqs):
+            raise ValueError("tree_verify: parents of shape %s for %d sequences" % (par.shape, n_seqs))
+        if n_nodes is not None and np.size(n_nodes) != n_seqs:
+            raise ValueError("tree_verify: %d numbers of nodes for %d sequences" % (np.size(n_nodes), n_seqs))
+        ap, self._keep = self._pack_append(layer, draft_k, draft_v, n_seqs, seq_ids, np.full(n_seqs, par.shape[1], np.int32) if n_nodes is None else n_nodes,
+                                           kv_layout, False, kv_dtype, pipelined)
+        at, self._keep2 = self._pack_attn(layer, n_seqs, q, None, out, num_heads, head_dim, scale, par.shape[1], 0, True, mode, None, None, seq_ids,
+                                          q_layout, out_layout, q_dtype, out_dtype, pipelined)
+        L.check(L.packed["gqa_tree_verify"](self.h, at, ap, L.pack_tree(_ptr(par), par.shape[0])))
+
+    def tree_commit(self, layer, path, path_len, seq_ids=None):
+        """Commits the accepted path of every sequence's tree (relux_gqa_tree_commit): path [n_seqs, any], node numbers in rising order, path_len
+        [n_seqs] of them valid; layer < 0: every layer."""
+        path = np.ascontiguousarray(path, dtype=np.int32)
+        n = np.ascontiguousarray(path_len, dtype=np.int32)
+        ids = None if seq_ids is None else np.ascontiguousarray(seq_ids, dtype=np.int32)
+        if path.ndim != 2 or path.shape[0] != n.size or (ids is not None and ids.size != n.size):
+            raise ValueError("tree_commit: path of shape %s, %d lengths" % (path.shape, n.size))
+        L.check(L.packed["gqa_tree_commit"](self.h, L.pack_tree_commit(layer, n.size, _ptr(ids) or 0, _ptr(path) or 0, _ptr(n) or 0, path.shape[1])))
 
     def step(self, layer, n_seqs, new_a, new_b, q, out, num_heads, head_dim, scale, q_rope=None, w_uk=None, w_uv=None, n_new=None,
              mode=L.ATTN_FAST, seq_ids=None, kv_layout=L.LAYOUT_TOKEN_MAJOR, q_dtype=None, out_dtype=None, kv_dtype=None, pipelined=False):

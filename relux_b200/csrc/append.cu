@@ -7,6 +7,7 @@
 // loads, then all their stores (a row at a time, the dependent latencies of every row added up: 43 us for 8 x 2048 rows of 4 KB
 // each way, now 32; 16 us for 4 x 1000 latent rows, now 7).
 #include "common.cuh"
+#include "gqa_int8_parts.cuh"
 #include "internal.h"
 
 namespace relux {
@@ -169,6 +170,46 @@ __global__ void gqa_append_kernel(AppendGeom g, uint16_t* __restrict__ k_base, u
   advance_lengths_by_last_block(g);
 }
 
+// The same rows into an 8-bit cache (gqa_int8_parts.cuh): 16 lanes quantise a kv head's row, of K or of V.
+template <bool kF32>
+__global__ void gqa_append_int8_kernel(AppendGeom g, uint8_t* k_base, uint8_t* v_base, float* scales, const void* ksrc, const void* vsrc, int Hkv,
+                                       int head_major) {
+  chain_release();
+  chain_wait();
+  using Src = typename std::conditional<kF32, float, uint16_t>::type;
+  constexpr int D = kGqaD;
+  const int i = blockIdx.x;
+  const int seq = g.seq_ids ? g.seq_ids[i] : i;
+  const int r0 = g.row_off ? g.row_off[i] : i * g.rows_each;
+  const int nrows = g.row_off ? g.row_off[i + 1] - r0 : g.rows_each;
+  const int base_len = load_chained(g.len + seq);
+  const int c = (threadIdx.x & 15) * 8;
+  constexpr int kN = kAhead;
+  for (int r = blockIdx.y * kN; r < nrows; r += gridDim.y * kN) {
+    int32_t pg[kN], tok[kN];
+    pages_of_rows<kN>(g, seq, base_len, r, nrows, pg, tok);
+    for (int u = threadIdx.x >> 4; u < 2 * Hkv; u += blockDim.x >> 4) {   // two a warp: all of its lanes or none
+      const int which = u >= Hkv, h = u - which * Hkv;
+      float x[kN][8];
+#pragma unroll
+      for (int q = 0; q < kN; q++) {
+        const size_t src_off = head_major ? ((size_t)r0 * Hkv * D + ((size_t)h * nrows + r + q) * D + c) : (((size_t)(r0 + r + q) * Hkv + h) * D + c);
+        if (pg[q] >= 0) load8(x[q], reinterpret_cast<const Src*>(which ? vsrc : ksrc) + src_off);
+      }
+#pragma unroll
+      for (int q = 0; q < kN; q++) {
+        if (pg[q] < 0) continue;   // the same for the whole block
+        const Int8Row row = int8_quantise(x[q], row_top(x[q]));
+        const size_t head = (size_t)pg[q] * Hkv + h;
+        *reinterpret_cast<uint2*>((which ? v_base : k_base) + (head * kGqaPageTok + tok[q]) * D + c) = row.codes;
+        if (c == 0) scales[(head * 2 + which) * kGqaPageTok + tok[q]] = row.scale;
+      }
+    }
+  }
+  fence_chained_writes();
+  advance_lengths_by_last_block(g);
+}
+
 // New lengths travel as kernel arguments: no staging copy and its engine switch in front of the launch.
 constexpr int kSetLenMax = 256;
 struct SetLenParams {
@@ -226,11 +267,13 @@ int32_t launch_mla_append(Pool* p, const SeqBatch& sb, int layer, const void* ck
 int32_t launch_gqa_append(Pool* p, const SeqBatch& sb, int layer, const void* k, const void* v, int dtype, int layout,
                           int advance) {
   AppendGeom g = make_geom(p, sb, layer, advance);
-  uint16_t* kb = p->storage + (size_t)layer * p->layer_elems;
-  uint16_t* vb = kb + p->page_elems * p->prm.num_pages;
+  uint16_t *kb = (uint16_t*)p->rows_at(layer, 0), *vb = (uint16_t*)p->rows_at(layer, 1);
   dim3 grid(sb.n_seqs, row_slices(sb));
   int threads = 256;
   int hm = layout == RELUX_LAYOUT_HEAD_MAJOR;
+  if (p->int8)
+    return launch_append(p, dtype == RELUX_DTYPE_F32 ? gqa_append_int8_kernel<true> : gqa_append_int8_kernel<false>, grid, threads, g, (uint8_t*)kb,
+                         (uint8_t*)vb, p->scales_at(layer), k, v, p->prm.gqa_num_kv_heads, hm);
   return launch_append(p, dtype == RELUX_DTYPE_F32 ? gqa_append_kernel<true> : gqa_append_kernel<false>, grid, threads, g, kb, vb, k, v,
                        p->prm.gqa_num_kv_heads, p->prm.gqa_head_dim, hm);
 }
@@ -283,6 +326,12 @@ __global__ void gather_rows_kernel(const uint16_t* __restrict__ layer_base, cons
 
 int32_t launch_gather_rows(Pool* p, int layer, int seq, int tok0, int n, uint16_t* d_a, uint16_t* d_b) {
   const relux_pool_params& prm = p->prm;
+  if (p->int8) {
+    SeqBatch sb;
+    sb.n_seqs = 1;
+    sb.seq = {seq};
+    return launch_read_kv(p, sb, layer, 1, &tok0, &n, RELUX_DTYPE_BF16, d_a, d_b);
+  }
   const uint16_t* base = p->storage + (size_t)layer * p->layer_elems;
   gather_rows_kernel<<<n, 128, 0, p->dev->stream>>>(base, p->d_table, prm.max_pages_per_seq, seq, tok0, n, prm.num_pages,
                                                     prm.page_tokens, prm.kind, prm.mla_dc, prm.mla_dhr, prm.gqa_num_kv_heads,

@@ -264,7 +264,7 @@ int32_t launch_gqa_prefill_sm100(Pool* p, const SeqBatch& sb, const relux_attn_a
 
 bool gqa_prompt_wants_bf16(const Pool* p, const relux_attn_args& a) {
   const int g = a.num_heads / std::max(1, p->prm.gqa_num_kv_heads);
-  return g >= 1 && a.q_tokens > std::max(1, 32 / g) && !p->tune.get(RELUX_TUNE_GQA_PROMPT_SLICES) && gqa_prefill_eligible(p, a);
+  return !p->int8 && g >= 1 && a.q_tokens > std::max(1, 32 / g) && !p->tune.get(RELUX_TUNE_GQA_PROMPT_SLICES) && gqa_prefill_eligible(p, a);
 }
 
 int32_t launch_gqa_decode_fast(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out) {
@@ -279,7 +279,7 @@ int32_t launch_gqa_decode_fast(Pool* p, const SeqBatch& sb, const relux_attn_arg
   // the kernel holds (num_heads / num_kv_heads) * q_tokens <= 32 query rows per kv head; longer multi-token calls
   // (a prompt) are cut into groups of tokens that run as the z slices of one grid
   const int per_group = std::max(1, 32 / g);
-  if (a.q_tokens <= per_group) return launch_gqa_stream(p, sb, a, d_q, d_out, false, nullptr);
+  if (a.q_tokens <= per_group || p->int8) return launch_gqa_stream(p, sb, a, d_q, d_out, false, nullptr);
   // a prompt: 128 query rows per CTA on the tcgen05 prefill kernel; the grid slices of the decode kernel serve the
   // group sizes that do not tile 128 rows, and stay selectable as a tuning knob
   if (a.q_dtype == RELUX_DTYPE_BF16 && gqa_prompt_wants_bf16(p, a)) return launch_gqa_prefill_sm100(p, sb, a, (const uint16_t*)d_q, (float*)d_out);
@@ -327,6 +327,7 @@ extern "C" __attribute__((visibility("default"))) int32_t relux_gqa_decode_noall
   const relux_pool_params& prm = p->prm;
   if (!a) { set_error("nil argument struct"); return RELUX_ERR_INVALID_ARG; }
   if (prm.kind != RELUX_POOL_GQA) { set_error("relux_gqa_decode_noalloc needs a GQA pool"); return RELUX_ERR_INVALID_ARG; }
+  if (p->int8) { set_error("relux_gqa_decode_noalloc: the pool holds 8-bit rows; use relux_gqa_decode"); return RELUX_ERR_UNSUPPORTED; }
   if (a->layer < 0 || a->layer >= prm.num_layers) { set_error("layerIdx=%d out of range [0, %d)", a->layer, prm.num_layers); return RELUX_ERR_INVALID_ARG; }
   if (!a->q || !a->out || a->q_tokens <= 0 || a->extra_tokens < 0 || a->num_heads <= 0 || a->head_dim != prm.gqa_head_dim ||
       a->num_heads % prm.gqa_num_kv_heads != 0) {

@@ -1,0 +1,293 @@
+// Rows of the 8-bit grouped-query cache, and per-warp attention over one 64-token page of them (gqa_stream_kernel.cuh, gqa_int8.cu,
+// gqa_tree_sm100.cu).
+//
+// A row of a kv head, 128 values x of K or of V, is 128 codes c (int8) and a float32 scale s:
+//   a = max |x|,  s = a / 127,  c = x * (127 / a) to the nearest whole number, even where two are as near
+// with every operation rounded to float32.  |c| <= 127: x * (127 / a) is at most 127 (1 + 2^-23).  A row with a < 1e-36, whose 127 / a might not be
+// finite, is s = 0, c = 0.  A row that holds an infinity or a NaN is s = NaN, c = 0: a code is always a number, so a row that no query sees adds
+// exactly nothing to a tensor-core product, whatever it held (0 * c, where bf16 rows have 0 * NaN).
+// Whole numbers and not an 8-bit float: the same bytes, and a fourth of the error (half a step of 1 / 127 of the row's largest value against 2^-4 of each
+// value); both are exact in binary16 and bfloat16.
+//
+// A page of a kv head is 64 rows of 128 bytes of K codes, the same of V, and 2 x 64 scales.  Both kinds of rows arrive by TMA with the 128-byte swizzle and
+// are read 16 bytes a thread without bank conflicts, straight into the B fragments of mma.sync m16n8k16: what a fragment wants side by side are
+// four consecutive K indices of one column, and the order of the indices is the reader's own as long as A has the same.
+//   K: thread (n, c) = (lane / 4, lane % 4) takes bytes 32 c .. 32 c + 31 of token n of a block of eight; K slice ks is its word ks.
+//   V: thread (n, c) takes bytes 16 n .. 16 n + 15 of tokens 2c, 2c + 1, 2c + 8, 2c + 9; output block j's column n is dim 16 n + j.
+// Codes become binary16 for the scores (two instructions for two codes; queries are brought to binary16 with a power of two per row, which keeps
+// 11 bits of a float32 query where bf16 keeps 8), and bfloat16 for the values: P carries s^v, whose range binary16 does not have.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "gqa_parts.cuh"
+
+namespace relux {
+
+constexpr int kInt8StageBytes = 2 * kGqaPageTok * kGqaD;                      // K codes, V codes
+constexpr int kInt8ScaleBytes = 2 * kGqaPageTok * (int)sizeof(float);         // K scales, V scales
+constexpr float kInt8Tiny = 1e-36f;
+
+// Untiled bulk copy global -> shared (multiples of 16 bytes), completion on an mbarrier of this CTA.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// ---- a row's values, eight a lane ----
+__device__ __forceinline__ void load8(float (&x)[8], const float* src) {
+  const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load8(float (&x)[8], const uint16_t* src) {
+  const uint4 a = *reinterpret_cast<const uint4*>(src);
+  x[0] = bf16_lo(a.x); x[1] = bf16_hi(a.x); x[2] = bf16_lo(a.y); x[3] = bf16_hi(a.y);
+  x[4] = bf16_lo(a.z); x[5] = bf16_hi(a.z); x[6] = bf16_lo(a.w); x[7] = bf16_hi(a.w);
+}
+// Largest magnitude of a row, as bits (larger for an infinity or a NaN than for any number), by the 16 lanes that hold it; the warp is converged.
+__device__ __forceinline__ uint32_t row_top(const float (&x)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return top;
+}
+struct Int8Row {
+  uint2 codes;   // this lane's eight
+  float scale;
+};
+__device__ __forceinline__ Int8Row int8_quantise(const float (&x)[8], uint32_t top) {
+  Int8Row r{{0u, 0u}, 0.f};
+  const float a = __uint_as_float(top);
+  if (top >= 0x7F800000u) {
+    r.scale = __uint_as_float(0x7FC00000u);
+  } else if (a >= kInt8Tiny) {
+    const float inv = __fdiv_rn(127.f, a);
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      int c[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) c[i] = __float2int_rn(__fmul_rn(x[4 * h + i], inv));
+      w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    }
+    r.codes = make_uint2(w[0], w[1]);
+    r.scale = __fdiv_rn(a, 127.f);
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Int8Row int8_row(const T* src) {
+  float x[8];
+  load8(x, src);
+  return int8_quantise(x, row_top(x));
+}
+
+// ---- codes -> matrix operands ----
+// Four codes -> two pairs of binary16: 1024 + (c + 128) is the byte below the exponent of 1024; 1152 is taken off again.
+__device__ __forceinline__ void int8x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+// Two codes in the even bytes under 0x43 -> bfloat16: 128 + the code's low seven bits, less 128, or 256 where its sign bit is set.
+__device__ __forceinline__ uint32_t int8x2_to_bf16(uint32_t t) {
+  const uint32_t a = t & 0xFF7FFF7Fu, s = t & 0xFF80FF80u;
+  const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&s));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// ---- queries ----
+// Row of queries in shared memory: 128 binary16 values, the row's factor (what a score of theirs is multiplied by, softmax scale and log2 e included),
+// and what the row sees of the new rows.  By 16 lanes of a converged warp, eight dims each.
+__device__ __forceinline__ void int8_put_query(uint16_t* row, int ch, bool there, const void* q, size_t off, bool q_bf16, float scale_log2) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) x[i] = 0.f;
+  if (there) {
+    if (q_bf16) load8(x, reinterpret_cast<const uint16_t*>(q) + off);
+    else load8(x, reinterpret_cast<const float*>(q) + off);
+  }
+  const int k = min(141 - (int)(row_top(x) >> 23), 126);   // the largest value comes to [2^14, 2^15); a row of zeros or of subnormal numbers does not
+  const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+  if (!there) return;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const __half2 h = __floats2half2_rn(x[2 * i] * up, x[2 * i + 1] * up);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(row + ch) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (ch == 0) *reinterpret_cast<float*>(row + kGqaD) = scale_log2 * down;
+}
+// 16 such rows -> A fragments in the order of K's bytes, and the factors of this lane's two rows.
+__device__ __forceinline__ void int8_load_q(uint32_t (&qa)[8][4], float (&q_scale)[2], const uint16_t* qs, int lane) {
+#pragma unroll
+  for (int hf = 0; hf < 2; hf++) {
+    const uint16_t* row = qs + ((lane >> 2) + 8 * hf) * kGqaQStride;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + 32 * (lane & 3) + 8 * i);
+      qa[2 * i][hf] = w.x;
+      qa[2 * i][2 + hf] = w.y;
+      qa[2 * i + 1][hf] = w.z;
+      qa[2 * i + 1][2 + hf] = w.w;
+    }
+    q_scale[hf] = *reinterpret_cast<const float*>(row + kGqaD);
+  }
+}
+
+// D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// gqa_consume_page for a page of codes.
+template <bool kTree>
+__device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_t (&qa)[8][4], const float (&q_scale)[2], const uint8_t* page,
+                                                  const float* scales, int tb, int tok0, int T, int S, int g, int causal, int lane, int row0,
+                                                  const TreeRows& tree) {
+  const int n = lane >> 2, c = lane & 3;
+  float sacc[2][4], sodd[2][4];   // even and odd K slices: two chains of dependent MMAs a block
+#pragma unroll
+  for (int nt = 0; nt < 2; nt++) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) sacc[nt][e] = sodd[nt][e] = 0.f;
+    const uint32_t row = tb + nt * 8 + n;
+    const uint4 k0 = *reinterpret_cast<const uint4*>(page + swz128(row, 2 * c)), k1 = *reinterpret_cast<const uint4*>(page + swz128(row, 2 * c + 1));
+    const uint32_t w[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) {
+      uint32_t b0, b1;
+      int8x4_to_f16(w[ks], b0, b1);
+      mma_f16_16816(ks & 1 ? sodd[nt] : sacc[nt], qa[ks], b0, b1);
+    }
+  }
+  // the values' codes, while the scores are on their way
+  const uint8_t* vt = page + kGqaPageTok * kGqaD;
+  uint4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const uint4*>(vt + swz128(tb + 2 * c + (i & 1) + (i >> 1) * 8, n));
+  float sv[2][2];
+#pragma unroll
+  for (int nt = 0; nt < 2; nt++) {
+    const float2 sk = *reinterpret_cast<const float2*>(scales + tb + nt * 8 + 2 * c);
+    const float2 s2 = *reinterpret_cast<const float2*>(scales + kGqaPageTok + tb + nt * 8 + 2 * c);
+    sv[nt][0] = s2.x;
+    sv[nt][1] = s2.y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) sacc[nt][e] = (sacc[nt][e] + sodd[nt][e]) * (e & 1 ? sk.y : sk.x);
+  }
+  uint32_t hidden = 0;   // bit 4 hf + 2 nt + e
+  const bool need_mask = tok0 + 16 > (kTree ? tree.len0 : T - (causal ? S : 0));
+  if (need_mask) {
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++) {
+      const int limit = causal ? (T - S + (row0 + hf * 8 + n) / g) : (T - 1);   // last visible token
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int tok = tok0 + nt * 8 + 2 * c + e;
+          if (kTree ? tree.hides(hf, tok) : tok > limit || tok >= T) {
+            hidden |= 1u << (4 * hf + 2 * nt + e);
+            sacc[nt][hf * 2 + e] = -INFINITY;
+          }
+        }
+    }
+  }
+  float mx[2];
+  bool grow = false;
+#pragma unroll
+  for (int hf = 0; hf < 2; hf++) {
+    float x = fmaxf(fmaxf(sacc[0][hf * 2], sacc[0][hf * 2 + 1]), fmaxf(sacc[1][hf * 2], sacc[1][hf * 2 + 1]));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    mx[hf] = x * q_scale[hf];
+    grow |= mx[hf] > st.m[0][hf];
+  }
+  if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++) {
+      const float m_new = fmaxf(st.m[0][hf], mx[hf]);
+      const float alpha = (m_new == -INFINITY) ? 0.f : gqa_ex2(st.m[0][hf] - m_new);
+      st.m[0][hf] = m_new;
+      st.l[0][hf] *= alpha;
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        st.o[0][j][hf * 2] *= alpha;
+        st.o[0][j][hf * 2 + 1] *= alpha;
+      }
+    }
+  }
+  // P times the values' scales, rounded to bf16 (2^-8 of each at most, as the bf16 cache's P)
+  uint32_t pa[4];
+#pragma unroll
+  for (int hf = 0; hf < 2; hf++) {
+    const float neg_m = (st.m[0][hf] == -INFINITY) ? 0.f : -st.m[0][hf];
+    float ps = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      float p0 = gqa_ex2(fmaf(sacc[nt][hf * 2], q_scale[hf], neg_m));
+      float p1 = gqa_ex2(fmaf(sacc[nt][hf * 2 + 1], q_scale[hf], neg_m));
+      ps += p0 + p1;
+      p0 *= sv[nt][0];
+      p1 *= sv[nt][1];
+      if (need_mask) {   // the scale of a hidden row may be NaN
+        if (hidden >> (4 * hf + 2 * nt) & 1u) p0 = 0.f;
+        if (hidden >> (4 * hf + 2 * nt + 1) & 1u) p1 = 0.f;
+      }
+      pa[nt * 2 + hf] = round_bf16x2(p0, p1);
+    }
+    st.l[0][hf] += ps;
+  }
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = w == 0 ? v[i].x : w == 1 ? v[i].y : w == 2 ? v[i].z : v[i].w;
+    const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[0], x[1], 0x7362);
+    const uint32_t b01 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t sel = j & 1 ? 0x4342 : 0x4140;
+      mma_bf16_16816(st.o[0][4 * w + j], pa, int8x2_to_bf16(__byte_perm(j < 2 ? a01 : a23, 0x43434343u, sel)),
+                     int8x2_to_bf16(__byte_perm(j < 2 ? b01 : b23, 0x43434343u, sel)));
+    }
+  }
+}
+
+// gqa_store_state: output block j's column 2c + e is dim 16 (2c + e) + j.
+__device__ __forceinline__ void int8_store_state(const GqaState<1>& st, float* dst0, int rows, int lane, bool alive) {
+#pragma unroll
+  for (int hf = 0; hf < 2; hf++) {
+    float l = st.l[0][hf];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const int row = hf * 8 + (lane >> 2);
+    if (row >= rows) continue;
+    float* dst = dst0 + row * kGqaStateStride;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<float4*>(dst + 16 * (2 * (lane & 3) + e) + j) =
+            make_float4(st.o[0][j][hf * 2 + e], st.o[0][j + 1][hf * 2 + e], st.o[0][j + 2][hf * 2 + e], st.o[0][j + 3][hf * 2 + e]);
+    if ((lane & 3) == 0) {
+      dst[kGqaD] = alive ? st.m[0][hf] : -INFINITY;
+      dst[kGqaD + 1] = alive ? l : 0.f;
+    }
+  }
+}
+
+}  // namespace relux

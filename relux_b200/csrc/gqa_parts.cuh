@@ -57,11 +57,39 @@ __device__ __forceinline__ void gqa_load_q(uint32_t (&qa)[MT][8][4], const uint1
     }
 }
 
+__device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr));
+  return w;
+}
+// Not zero where one of two bf16 values is an infinity or a NaN (its exponent is all ones: one more carries into the sign's place).
+__device__ __forceinline__ uint32_t bf16x2_not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+// The pair with zeros for such values.
+__device__ __forceinline__ uint32_t bf16x2_finite(uint32_t w) {
+  const uint32_t bad = bf16x2_not_finite(w);
+  return w & ~((bad >> 15) * 0xFFFFu);
+}
+
+// The new rows of a call that are the nodes of a drafted tree: of the rows from len0 on, query row hf (of this lane's two) sees node j where bit j of
+// see[hf] is set.
+constexpr int kTreeNodes = 64;
+struct TreeRows {
+  uint64_t see[2];
+  int len0;
+  __device__ __forceinline__ bool hides(int hf, int tok) const {
+    const int j = tok - len0;
+    return j >= 0 && (j >= kTreeNodes || !(see[hf] >> j & 1u));
+  }
+};
+// Where a row of queries in shared memory keeps it.
+__device__ __forceinline__ uint64_t row_tree(const uint16_t* q_row) { return *reinterpret_cast<const uint64_t*>(q_row + kGqaD + 4); }
+
 // Adds this warp's 16 tokens (tb .. tb + 15 of the page, logical tokens tok0 ..) to its state.  T: visible tokens; row r
-// (counted from row0 of the fragment) belongs to query token r / g of S, which with the causal mask sees tokens up to T - S + r / g.
-template <int MT>
+// (counted from row0 of the fragment) belongs to query token r / g of S, which with the causal mask sees tokens up to T - S + r / g;
+// kTree: it sees what `tree` says.
+template <int MT, bool kTree = false>
 __device__ __forceinline__ void gqa_consume_page(GqaState<MT>& st, const uint32_t (&qa)[MT][8][4], uint32_t kt, int tb, int tok0, int T, int S,
-                                                 int g, int causal, float scale_log2, int lane, int row0 = 0) {
+                                                 int g, int causal, float scale_log2, int lane, int row0 = 0, const TreeRows& tree = {}) {
   const uint32_t vt = kt + 16384;
   // two accumulators per 8-token column block (even and odd K slices): the MMAs of one block depend on each other, and
   // the chain's latency, not the issue rate, is what a page costs a warp
@@ -86,7 +114,7 @@ __device__ __forceinline__ void gqa_consume_page(GqaState<MT>& st, const uint32_
     }
   }
   // mask the tail of the sequence and the causal part of the draft
-  const bool need_mask = (tok0 + 16 > T - (causal ? S : 0));
+  const bool need_mask = tok0 + 16 > (kTree ? tree.len0 : T - (causal ? S : 0));
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -105,7 +133,7 @@ __device__ __forceinline__ void gqa_consume_page(GqaState<MT>& st, const uint32_
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const int tok = tok0 + nt * 8 + 2 * (lane & 3) + e;
-            if (tok > limit || tok >= T) sacc[mt][nt][hf * 2 + e] = -INFINITY;
+            if (kTree ? tree.hides(hf, tok) : tok > limit || tok >= T) sacc[mt][nt][hf * 2 + e] = -INFINITY;
           }
       }
   }
@@ -156,6 +184,30 @@ __device__ __forceinline__ void gqa_consume_page(GqaState<MT>& st, const uint32_
       }
       st.l[mt][hf] += ps;
     }
+  // A product with P = 0 does not hide an infinity or a NaN among the values.  kTree: where the warp's tokens are not all seen by all, such values
+  // count as zeros, and a row that sees a token with one becomes NaN as a whole.
+  bool clean = false;
+  if (kTree && need_mask) {
+    uint32_t bad = 0;   // of this lane's half token: any of its 64 values
+    const uint32_t row = tb + (lane >> 1);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint4 w = lds_v4(vt + (lane & 1) * 8192 + swz128(row, i));
+      bad |= bf16x2_not_finite(w.x) | bf16x2_not_finite(w.y) | bf16x2_not_finite(w.z) | bf16x2_not_finite(w.w);
+    }
+    const uint32_t tokens = __ballot_sync(0xffffffffu, bad != 0);   // bits 2 t and 2 t + 1 of token t
+    clean = tokens != 0;
+    if (clean) {
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+          for (int t = 0; t < 16; t++)
+            if ((tokens >> (2 * t) & 3u) && !tree.hides(hf, tok0 + t))
+#pragma unroll
+              for (int nt = 0; nt < 16; nt++) st.o[mt][nt][hf * 2] = st.o[mt][nt][hf * 2 + 1] = __uint_as_float(0x7FC00000u);
+    }
+  }
   // O += P V
 #pragma unroll
   for (int n2 = 0; n2 < 8; n2++) {
@@ -164,6 +216,12 @@ __device__ __forceinline__ void gqa_consume_page(GqaState<MT>& st, const uint32_
     const uint32_t chunk = n2 * 2 + (m >> 1);  // 16 chunks of 8 dims
     uint32_t b0, b1, b2, b3;
     ldmatrix_x4_trans(b0, b1, b2, b3, vt + (chunk >> 3) * 8192 + swz128(row, chunk & 7));
+    if (kTree && clean) {
+      b0 = bf16x2_finite(b0);
+      b1 = bf16x2_finite(b1);
+      b2 = bf16x2_finite(b2);
+      b3 = bf16x2_finite(b3);
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
       mma_bf16_16816(st.o[mt][2 * n2], pa[mt], b0, b1);

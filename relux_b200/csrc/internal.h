@@ -118,7 +118,14 @@ struct Pool {
   int row_elems_a = 0;  // MLA: dC + dHR (one fused row); GQA: head_dim
   size_t page_elems = 0;    // elements per page per tensor (MLA: P*(dC+dHR); GQA: Hkv*P*D for K, same for V)
   size_t layer_elems = 0;   // elements per layer (GQA: K then V)
-  uint16_t* storage = nullptr;  // bf16 bits
+  uint16_t* storage = nullptr;  // bf16 bits; with int8 a byte an element: codes
+  bool int8 = false;            // RELUX_POOL_FLAG_CACHE_INT8
+  float* scales = nullptr;      // int8: [num_layers][num_pages][Hkv][K, V][page_tokens]
+  size_t elem_bytes() const { return int8 ? 1 : sizeof(uint16_t); }
+  // GQA: K (which = 0) or V rows of a layer; the scales of an int8 layer.
+  void* rows_at(int layer, int which) const { return (char*)storage + ((size_t)layer * layer_elems + (which ? page_elems * prm.num_pages : 0)) * elem_bytes(); }
+  size_t layer_scales() const { return (size_t)prm.num_pages * prm.gqa_num_kv_heads * 2 * prm.page_tokens; }
+  float* scales_at(int layer) const { return scales + (size_t)layer * layer_scales(); }
   void* meta = nullptr;         // one device block: table, lengths, status, ids, row offsets, time slots of the attention calls
   int32_t* d_table = nullptr;   // [max_seqs][max_pages_per_seq]
   int32_t* d_len = nullptr;     // [num_layers][max_seqs]
@@ -148,7 +155,8 @@ struct Pool {
   cudaEvent_t stage_ev[kStageSlots] = {};
   bool stage_busy[kStageSlots] = {};
   uint32_t stage_next = 0;
-  size_t stage_slot_ints() const { return 4 * ((size_t)prm.max_seqs + 1); }
+  // per sequence four ints, and of a GQA pool a tree's parents, 64 bytes
+  size_t stage_slot_ints() const { return (prm.kind == RELUX_POOL_GQA ? 20 : 4) * ((size_t)prm.max_seqs + 1); }
   // staging of activations that arrive in host memory, and outputs that leave to it
   GrowBuf in_a, in_b, out_buf, q_conv;
   GrowBuf expand_buf;  // expanded keys / values of an MLA prompt (+ the sequences' first rows)
@@ -233,10 +241,19 @@ struct GqaAppend {
   int dtype, layout, advance;
   const int32_t* rows;   // host: new rows per sequence
 };
+// The nodes of a drafted tree as the new rows of a call: node j of sequence i continues node parents[64 i + j], or (-1) the cached rows.
+struct GqaTree {
+  const int8_t* parents;   // host: [n_seqs, or with `one` 1][64]
+  bool one;
+};
 bool gqa_stream_eligible(const Pool* p, const relux_attn_args& a);
 bool gqa_append_fusable(const Pool* p, const relux_attn_args& a, int max_new_rows, bool advance);
 int32_t launch_gqa_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16,
-                          const GqaAppend* app);
+                          const GqaAppend* app, const GqaTree* tree = nullptr);
+// Rows of either grouped-query cache read back, the commit of a tree's path (gqa_rows.cu).
+int32_t launch_read_kv(Pool* p, const SeqBatch& sb, int layer0, int layers, const int32_t* tok0, const int32_t* n, int dtype, void* k_out, void* v_out);
+int32_t do_read_kv(Pool* p, const relux_read_kv_args* a);
+int32_t do_tree_commit(Pool* p, const relux_tree_commit_args* a);
 // True when this call is a multi-token call that the tcgen05 prefill kernel serves (it takes bf16 queries).
 bool mla_expand_eligible(const Pool* p, int num_heads, int head_dim);
 int64_t mla_expand_rows(const Pool* p, const SeqBatch& sb, int layer, int extra);

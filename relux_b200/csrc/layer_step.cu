@@ -841,6 +841,7 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) {
   const bool faithful = a->mode == RELUX_ATTN_REFERENCE_FAITHFUL;
   if (faithful && (!p->compat || !a->advance)) { set_error("RELUX_ATTN_REFERENCE_FAITHFUL needs a pool created with RELUX_POOL_FLAG_REFERENCE_COMPAT and advance != 0"); return RELUX_ERR_INVALID_ARG; }
   if (a->x_dtype != RELUX_DTYPE_F32) { set_error("x must be float32"); return RELUX_ERR_UNSUPPORTED; }
+  if (p->int8 && a->mode != RELUX_ATTN_FAST) { set_error("a pool of 8-bit rows takes RELUX_ATTN_FAST only"); return RELUX_ERR_UNSUPPORTED; }
   if (a->mode == RELUX_ATTN_FAST && (!p->has_tmap || prm.page_tokens != 64 || hd != 128 || H / Hkv > 32)) {
     // checked before anything is written to the cache
     set_error("GQA FAST kernels need page_tokens=64, head_dim=128 and num_heads/num_kv_heads <= 32 "

@@ -4,6 +4,7 @@
 #include <cstdlib>
 #include <new>
 
+#include "gqa_parts.cuh"
 #include "internal.h"
 
 namespace relux {
@@ -281,7 +282,7 @@ static void pool_free_all(Pool* p) {
     }
   for (cudaEvent_t e : p->pipe_calls.done)
     if (e) cudaEventDestroy(e);
-  fr(p->storage); fr(p->meta);
+  fr(p->storage); fr(p->scales); fr(p->meta);
   fr(p->in_a.p); fr(p->in_b.p); fr(p->out_buf.p); fr(p->q_abs.p); fr(p->part_o.p); fr(p->part_ml.p); fr(p->work.p); fr(p->stream_done.p); fr(p->seq_list.p);
   fr(p->o_lat.p); fr(p->q_conv.p); fr(p->rope_tab.p); fr(p->layer_buf.p); fr(p->shadow_f32); fr(p->chunk_tab.p); fr(p->step_rows.p); fr(p->expand_buf.p);
   if (p->h_stage) cudaFreeHost(p->h_stage);
@@ -510,7 +511,8 @@ static bool pipes_output(const Pool* p, const relux_attn_args& a) {
   return (a.flags & RELUX_CALL_PIPELINED) && p->dev->h2d_stream && p->dev->d2h_stream && a.out_mem == RELUX_MEM_HOST;
 }
 
-static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const StepAppend* step = nullptr, const GqaAppend* gstep = nullptr) {
+static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const StepAppend* step = nullptr, const GqaAppend* gstep = nullptr,
+                            const GqaTree* tree = nullptr) {
   if (!a) { set_error("nil argument struct"); return RELUX_ERR_INVALID_ARG; }
   if (p->prm.kind != kind) { set_error("pool kind does not match this attention call"); return RELUX_ERR_INVALID_ARG; }
   int32_t rc = check_layer(p, a->layer);
@@ -537,6 +539,10 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
     set_error("RELUX_ATTN_REFERENCE_FAITHFUL needs a pool created with RELUX_POOL_FLAG_REFERENCE_COMPAT and extra_tokens = 0");
     return RELUX_ERR_INVALID_ARG;
   }
+  if (p->int8 && a->mode != RELUX_ATTN_FAST) {
+    set_error("a pool of 8-bit rows takes RELUX_ATTN_FAST only");
+    return RELUX_ERR_UNSUPPORTED;
+  }
   if (!(a->scale > 0.f)) { set_error("scale=%g, must be > 0", (double)a->scale); return RELUX_ERR_INVALID_ARG; }
   if (a->flags & ~RELUX_CALL_PIPELINED) { set_error("unknown call flags 0x%x", a->flags); return RELUX_ERR_INVALID_ARG; }
   if (a->q_mem == RELUX_MEM_DEVICE) {
@@ -546,12 +552,13 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
   if (a->out_mem == RELUX_MEM_DEVICE && (rc = check_dev_align(a->out, "out"))) return rc;
   if (kind == RELUX_POOL_MLA && ((rc = check_dev_align(a->w_uk, "w_uk")) || (rc = check_dev_align(a->w_uv, "w_uv")))) return rc;
   SeqBatch sb;
-  const bool gqa_stream = kind == RELUX_POOL_GQA && a->mode == RELUX_ATTN_FAST && gqa_stream_eligible(p, *a);
+  const bool gqa_stream = tree || (kind == RELUX_POOL_GQA && a->mode == RELUX_ATTN_FAST && gqa_stream_eligible(p, *a));
   rc = stage_batch(p, a->n_seqs, a->seq_ids, nullptr, a->q_tokens, &sb, !gqa_stream);
   if (rc) return rc;
   for (int i = 0; i < sb.n_seqs; i++) {
     int s = sb.seq[i];
     int T = p->h_len[(size_t)a->layer * prm.max_seqs + s] + a->extra_tokens;
+    if (tree) continue;   // do_gqa_tree has looked at its rows
     if (T < a->q_tokens || T > p->seq_pages[s] * prm.page_tokens) {
       set_error("sequence %d: %d cached rows (with extra_tokens) cannot serve %d query tokens within capacity %d", s, T,
                 a->q_tokens, p->seq_pages[s] * prm.page_tokens);
@@ -577,7 +584,7 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
   // canonical kernel input: token-major; f32 for REFERENCE, caller's dtype for FAST
   int want_dtype = (a->mode != RELUX_ATTN_FAST) ? RELUX_DTYPE_F32 : a->q_dtype;
   // a GQA prompt goes to the tcgen05 prefill kernel, whose Q tile is a TMA load of bf16 rows
-  if (kind == RELUX_POOL_GQA && a->mode == RELUX_ATTN_FAST && gqa_prompt_wants_bf16(p, *a)) want_dtype = RELUX_DTYPE_BF16;
+  if (kind == RELUX_POOL_GQA && a->mode == RELUX_ATTN_FAST && !tree && gqa_prompt_wants_bf16(p, *a)) want_dtype = RELUX_DTYPE_BF16;
   // so does an MLA prompt (expanded keys / values + the same kernel)
   if (kind == RELUX_POOL_MLA && a->mode == RELUX_ATTN_FAST && mla_prefill_eligible(p, sb, *a)) want_dtype = RELUX_DTYPE_BF16;
   const bool relayout_q = (a->q_layout == RELUX_LAYOUT_HEAD_MAJOR && S > 1) || want_dtype != a->q_dtype;
@@ -638,7 +645,7 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
     rc = (kind == RELUX_POOL_MLA) ? launch_attn_reference_mla(p, sb, aa, (const float*)dq, (const float*)dqr, (float*)kout)
                                   : launch_attn_reference_gqa(p, sb, aa, (const float*)dq, (float*)kout);
   } else if (gqa_stream) {
-    rc = launch_gqa_stream(p, sb, aa, dq, kout, k_bf16, gstep);
+    rc = launch_gqa_stream(p, sb, aa, dq, kout, k_bf16, gstep, tree);
   } else {
     rc = (kind == RELUX_POOL_MLA) ? launch_mla_decode_fast(p, sb, aa, dq, dqr, kout, k_bf16, step) : launch_gqa_decode_fast(p, sb, aa, dq, kout);
   }
@@ -931,11 +938,22 @@ API int32_t relux_pool_create(relux_device_t h, const relux_pool_params* prm, re
   }
   for (int i = 0; i < 5; i++)
     if (prm->reserved[i]) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
-  if (prm->flags & ~RELUX_POOL_FLAG_REFERENCE_COMPAT) { set_error("unknown pool flags 0x%x", prm->flags); return RELUX_ERR_INVALID_ARG; }
+  if (prm->flags & ~(RELUX_POOL_FLAG_REFERENCE_COMPAT | RELUX_POOL_FLAG_CACHE_INT8)) { set_error("unknown pool flags 0x%x", prm->flags); return RELUX_ERR_INVALID_ARG; }
+  const bool int8 = (prm->flags & RELUX_POOL_FLAG_CACHE_INT8) != 0;
+  if (int8 && (prm->flags & RELUX_POOL_FLAG_REFERENCE_COMPAT)) {
+    set_error("RELUX_POOL_FLAG_CACHE_INT8 and RELUX_POOL_FLAG_REFERENCE_COMPAT exclude each other: the reference's arithmetic has no 8-bit rows");
+    return RELUX_ERR_INVALID_ARG;
+  }
+  if (int8 && (prm->kind != RELUX_POOL_GQA || prm->page_tokens != 64 || prm->gqa_head_dim != 128)) {
+    set_error("RELUX_POOL_FLAG_CACHE_INT8 needs a GQA pool with page_tokens=64 and head_dim=128 (got kind=%d page_tokens=%d head_dim=%d)", prm->kind,
+              prm->page_tokens, prm->gqa_head_dim);
+    return RELUX_ERR_UNSUPPORTED;
+  }
   Pool* p = new (std::nothrow) Pool();
   if (!p) return RELUX_ERR_OUT_OF_MEMORY;
   p->dev = dev;
   p->prm = *prm;
+  p->int8 = int8;
   if (prm->kind == RELUX_POOL_MLA) {
     if (prm->mla_dc <= 0 || prm->mla_dhr <= 0 || prm->mla_dhr % 2 || (prm->mla_dc % 8) || (prm->mla_dhr % 8)) {
       set_error("MLA pool: dC=%d and dHR=%d must be positive multiples of 8 (16-byte rows)", prm->mla_dc, prm->mla_dhr);
@@ -959,11 +977,13 @@ API int32_t relux_pool_create(relux_device_t h, const relux_pool_params* prm, re
     delete p;
     return RELUX_ERR_INVALID_ARG;
   }
-  const size_t storage_bytes = p->layer_elems * prm->num_layers * sizeof(uint16_t);
+  const size_t storage_bytes = p->layer_elems * prm->num_layers * p->elem_bytes();
+  const size_t scale_bytes = int8 ? p->layer_scales() * prm->num_layers * sizeof(float) : 0;
   const size_t table_n = (size_t)prm->max_seqs * prm->max_pages_per_seq, len_n = (size_t)prm->num_layers * prm->max_seqs;
   cudaError_t e = cudaSuccess;
   auto A = [&](void** q, size_t bytes) { if (e == cudaSuccess) e = cudaMalloc(q, bytes); };
   A((void**)&p->storage, storage_bytes);
+  if (int8) A((void**)&p->scales, scale_bytes);
   // the small arrays in one block: [table | lengths, status (word, block counter of the append kernels), time slots |
   // sequence ids | row offsets]; the middle part starts as zeros
   auto pad = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -989,6 +1009,7 @@ API int32_t relux_pool_create(relux_device_t h, const relux_pool_params* prm, re
   if (e == cudaSuccess) e = cudaMemsetAsync(p->d_len, 0, off_ids - off_len, dev->stream);
   // The reference zero-fills new caches (kvcache.go:73-84, mla_cache.go:46-52).
   if (e == cudaSuccess) e = cudaMemsetAsync(p->storage, 0, storage_bytes, dev->stream);
+  if (e == cudaSuccess && int8) e = cudaMemsetAsync(p->scales, 0, scale_bytes, dev->stream);
   if (e != cudaSuccess) {
     int32_t rc = cuda_fail(e, "pool allocation");
     pool_free_all(p);
@@ -1014,8 +1035,14 @@ API int32_t relux_pool_create(relux_device_t h, const relux_pool_params* prm, re
                     make_tmap_2d(&p->tmap_mla_3, p->storage, rows, 64, 64, 192);
     } else if (prm->kind == RELUX_POOL_GQA && prm->gqa_head_dim % 64 == 0) {
       uint64_t rows = (uint64_t)prm->num_layers * 2 * prm->num_pages * prm->gqa_num_kv_heads * prm->page_tokens;
-      p->has_tmap = make_tmap_2d(&p->tmap_gqa, p->storage, rows, (uint64_t)prm->gqa_head_dim, 64, 64);
+      // rows of 8-bit codes are 128 bytes, a box of 64 of them 8 KB, like half a page of bf16
+      p->has_tmap = make_tmap_2d(&p->tmap_gqa, p->storage, rows, (uint64_t)prm->gqa_head_dim / (int8 ? 2 : 1), 64, 64);
     }
+  }
+  if (int8 && !p->has_tmap) {
+    set_error("RELUX_POOL_FLAG_CACHE_INT8: the tensor map of the pool could not be encoded");
+    pool_free_all(p);
+    return RELUX_ERR_CUDA;
   }
   *out = p;
   return RELUX_OK;
@@ -1285,6 +1312,40 @@ void relux::take_rows_back(Pool* p, const SeqBatch& sb, int layer) {
   set_error("%s", why);
 }
 
+// The new rows of a GQA step that its attention launch appends, on the device: *pa and *pb; the slots of a pipelined call's (else -1).
+static int32_t stage_step_rows(Pool* p, const SeqBatch& sb, const relux_append_args* kv, const relux_attn_args* attn, const void** pa, const void** pb,
+                               int* slot_a, int* slot_b) {
+  const relux_pool_params& prm = p->prm;
+  int32_t rc;
+  if (kv->mem == RELUX_MEM_DEVICE && ((rc = check_dev_align(kv->a, "append input a")) || (rc = check_dev_align(kv->b, "append input b")))) return rc;
+  const size_t bytes = (size_t)sb.total_rows * prm.gqa_num_kv_heads * prm.gqa_head_dim * dtype_size(kv->dtype);
+  const bool piped = (kv->flags & RELUX_CALL_PIPELINED) && kv->mem == RELUX_MEM_HOST && p->dev->h2d_stream;
+  const void *&da = *pa, *&db = *pb;
+  da = kv->a;
+  db = kv->b;
+  *slot_a = *slot_b = -1;
+  if (piped) {
+    if ((rc = pipe_stage_in(p, p->pipe_app_a, kv->a, bytes, false, &da, slot_a))) return rc;
+    if ((rc = pipe_stage_in(p, p->pipe_app_b, kv->b, bytes, !pipes_queries(p, *attn), &db, slot_b))) return rc;
+  } else if (kv->mem == RELUX_MEM_HOST) {
+    // the attention call stages q in in_a: the step's rows get a block of their own
+    const size_t off_b = (bytes + 255) & ~(size_t)255;
+    const void* staged[2];
+    stage_small(p, {kv->a, kv->b}, {bytes, bytes}, kv->mem, staged);
+    if (!(da = staged[0])) {
+      if ((rc = grow(p->dev, p->step_rows, off_b + bytes))) return rc;
+      da = p->step_rows.p;
+      RELUX_CUDA_TRY(cudaMemcpyAsync((void*)da, kv->a, bytes, cudaMemcpyHostToDevice, p->dev->stream));
+    }
+    if (!(db = staged[1])) {
+      if ((rc = grow(p->dev, p->step_rows, off_b + bytes))) return rc;
+      db = (char*)p->step_rows.p + off_b;
+      RELUX_CUDA_TRY(cudaMemcpyAsync((void*)db, kv->b, bytes, cudaMemcpyHostToDevice, p->dev->stream));
+    }
+  }
+  return RELUX_OK;
+}
+
 // The rows of a GQA decode (advance) or verify step ride in the attention launch: validated and staged exactly as do_append
 // does.  An attention call that is refused leaves the rows appended, as the two calls one after the other would.
 static int32_t do_gqa_fused(Pool* p, const relux_append_args* kv, const relux_attn_args* attn) {
@@ -1305,30 +1366,9 @@ static int32_t do_gqa_fused(Pool* p, const relux_append_args* kv, const relux_at
     rc = do_append(p, kv, RELUX_POOL_GQA);
     return rc ? rc : do_attention(p, attn, RELUX_POOL_GQA);
   }
-  if (kv->mem == RELUX_MEM_DEVICE && ((rc = check_dev_align(kv->a, "append input a")) || (rc = check_dev_align(kv->b, "append input b")))) return rc;
-  const size_t bytes = (size_t)sb.total_rows * prm.gqa_num_kv_heads * prm.gqa_head_dim * dtype_size(kv->dtype);
-  const bool piped = (kv->flags & RELUX_CALL_PIPELINED) && kv->mem == RELUX_MEM_HOST && p->dev->h2d_stream;
-  const void *da = kv->a, *db = kv->b;
-  int slot_a = -1, slot_b = -1;
-  if (piped) {
-    if ((rc = pipe_stage_in(p, p->pipe_app_a, kv->a, bytes, false, &da, &slot_a))) return rc;
-    if ((rc = pipe_stage_in(p, p->pipe_app_b, kv->b, bytes, !pipes_queries(p, *attn), &db, &slot_b))) return rc;
-  } else if (kv->mem == RELUX_MEM_HOST) {
-    // the attention call stages q in in_a: the step's rows get a block of their own
-    const size_t off_b = (bytes + 255) & ~(size_t)255;
-    const void* staged[2];
-    stage_small(p, {kv->a, kv->b}, {bytes, bytes}, kv->mem, staged);
-    if (!(da = staged[0])) {
-      if ((rc = grow(p->dev, p->step_rows, off_b + bytes))) return rc;
-      da = p->step_rows.p;
-      RELUX_CUDA_TRY(cudaMemcpyAsync((void*)da, kv->a, bytes, cudaMemcpyHostToDevice, p->dev->stream));
-    }
-    if (!(db = staged[1])) {
-      if ((rc = grow(p->dev, p->step_rows, off_b + bytes))) return rc;
-      db = (char*)p->step_rows.p + off_b;
-      RELUX_CUDA_TRY(cudaMemcpyAsync((void*)db, kv->b, bytes, cudaMemcpyHostToDevice, p->dev->stream));
-    }
-  }
+  const void *da, *db;
+  int slot_a, slot_b;
+  if ((rc = stage_step_rows(p, sb, kv, attn, &da, &db, &slot_a, &slot_b))) return rc;
   const GqaAppend app{da, db, kv->dtype, kv->layout, adv, sb.rows.data()};
   if (adv)   // the host lengths count the new rows from here on
     for (int i = 0; i < sb.n_seqs; i++) hl[sb.seq[i]] += sb.rows[i];
@@ -1341,7 +1381,71 @@ static int32_t do_gqa_fused(Pool* p, const relux_append_args* kv, const relux_at
     set_error("%s", why);
     return rc;
   }
-  if (piped && !pipes_queries(p, *attn) && !pipes_output(p, *attn) && (rc = pipe_end(p))) return rc;   // else the attention call's end is this one's
+  if (slot_a >= 0 && !pipes_queries(p, *attn) && !pipes_output(p, *attn) && (rc = pipe_end(p))) return rc;   // else the attention call's end is this one's
+  pipe_release(p, p->pipe_app_a, slot_a);
+  pipe_release(p, p->pipe_app_b, slot_b);
+  return RELUX_OK;
+}
+// Attention of drafted trees: their rows are written past the cursors by the attention launch, as a verify step's are.
+static int32_t do_gqa_tree(Pool* p, const relux_attn_args* attn, const relux_append_args* kv, const relux_tree_args* t) {
+  if (!attn || !kv || !t) { set_error("nil argument struct"); return RELUX_ERR_INVALID_ARG; }
+  const relux_pool_params& prm = p->prm;
+  if (prm.kind != RELUX_POOL_GQA) { set_error("relux_gqa_tree_verify needs a GQA pool"); return RELUX_ERR_INVALID_ARG; }
+  int32_t rc = check_layer(p, attn->layer);
+  if (rc) return rc;
+  if (kv->advance != 0) { set_error("tree_verify: drafted rows must be appended with advance=0"); return RELUX_ERR_INVALID_ARG; }
+  if (kv->layer != attn->layer || kv->n_seqs != attn->n_seqs) { set_error("tree_verify: append and attention arguments disagree"); return RELUX_ERR_INVALID_ARG; }
+  if (kv->seq_ids != attn->seq_ids && (!kv->seq_ids || !attn->seq_ids || kv->n_seqs <= 0 ||
+                                       memcmp(kv->seq_ids, attn->seq_ids, sizeof(int32_t) * (size_t)kv->n_seqs) != 0)) {
+    set_error("tree_verify: append and attention arguments name different sequences");
+    return RELUX_ERR_INVALID_ARG;
+  }
+  if (attn->extra_tokens != 0) { set_error("tree_verify: extra_tokens=%d, must be 0: the tree's nodes are the rows past the cursor", attn->extra_tokens); return RELUX_ERR_INVALID_ARG; }
+  if (!kv->a || !kv->b || !t->parents) { set_error("tree_verify: nil parents, K or V"); return RELUX_ERR_INVALID_ARG; }
+  if ((kv->dtype != RELUX_DTYPE_F32 && kv->dtype != RELUX_DTYPE_BF16) || (kv->mem != RELUX_MEM_HOST && kv->mem != RELUX_MEM_DEVICE) ||
+      (kv->layout != RELUX_LAYOUT_TOKEN_MAJOR && kv->layout != RELUX_LAYOUT_HEAD_MAJOR)) {
+    set_error("bad dtype/mem/layout flag");
+    return RELUX_ERR_INVALID_ARG;
+  }
+  if (kv->flags & ~RELUX_CALL_PIPELINED) { set_error("unknown call flags 0x%x", kv->flags); return RELUX_ERR_INVALID_ARG; }
+  for (int32_t r : t->reserved)
+    if (r) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  const int S = attn->q_tokens;
+  if (S <= 0 || S > kTreeNodes) { set_error("tree_verify: q_tokens=%d outside [1, %d]", S, kTreeNodes); return S <= 0 ? RELUX_ERR_INVALID_ARG : RELUX_ERR_UNSUPPORTED; }
+  if (t->n_trees != 1 && t->n_trees != attn->n_seqs) { set_error("tree_verify: n_trees=%d, must be 1 or n_seqs=%d", t->n_trees, attn->n_seqs); return RELUX_ERR_INVALID_ARG; }
+  if (attn->mode != RELUX_ATTN_FAST || p->compat) { set_error("tree_verify: RELUX_ATTN_FAST on a pool without RELUX_POOL_FLAG_REFERENCE_COMPAT only"); return RELUX_ERR_UNSUPPORTED; }
+  const int g = attn->num_heads > 0 ? attn->num_heads / prm.gqa_num_kv_heads : 0;
+  if (!p->has_tmap || prm.page_tokens != 64 || prm.gqa_head_dim != 128 || g > 32) {
+    set_error("tree_verify needs page_tokens=64, head_dim=128 and num_heads/num_kv_heads <= 32 (got page_tokens=%d head_dim=%d group=%d)", prm.page_tokens,
+              prm.gqa_head_dim, g);
+    return RELUX_ERR_UNSUPPORTED;
+  }
+  SeqBatch sb;
+  if ((rc = stage_batch(p, kv->n_seqs, kv->seq_ids, kv->n_new, S, &sb, false))) return rc;
+  int deepest = 0;   // nodes that any sequence of a shared tree has
+  for (int i = 0; i < sb.n_seqs; i++) {
+    const int s = sb.seq[i], cap = p->seq_pages[s] * prm.page_tokens, len = p->h_len[(size_t)kv->layer * prm.max_seqs + s];
+    if (sb.rows[i] > S) { set_error("tree_verify: sequence %d has %d nodes, q_tokens=%d", s, sb.rows[i], S); return RELUX_ERR_INVALID_ARG; }
+    if (len + sb.rows[i] > cap) {
+      set_error("Append: layer %d overflow: total=%d + newLen=%d > capacity=%d (sequence %d)", kv->layer, len, sb.rows[i], cap, s);
+      return RELUX_ERR_OVERFLOW;
+    }
+    deepest = std::max(deepest, sb.rows[i]);
+  }
+  std::vector<int8_t> parents((size_t)t->n_trees * kTreeNodes, (int8_t)-1);
+  for (int i = 0; i < t->n_trees; i++)
+    for (int j = 0; j < (t->n_trees == 1 ? deepest : sb.rows[i]); j++) {
+      const int32_t up = t->parents[(size_t)i * S + j];
+      if (up < -1 || up >= j) { set_error("tree_verify: parents[%d][%d]=%d, must be -1 or an earlier node", i, j, up); return RELUX_ERR_INVALID_ARG; }
+      parents[(size_t)i * kTreeNodes + j] = (int8_t)up;
+    }
+  const void *da = nullptr, *db = nullptr;
+  int slot_a = -1, slot_b = -1;
+  if (sb.total_rows > 0 && (rc = stage_step_rows(p, sb, kv, attn, &da, &db, &slot_a, &slot_b))) return rc;
+  const GqaAppend app{da, db, kv->dtype, kv->layout, 0, sb.rows.data()};
+  const GqaTree tree{parents.data(), t->n_trees == 1};
+  if ((rc = do_attention(p, attn, RELUX_POOL_GQA, nullptr, &app, &tree))) return rc;
+  if (slot_a >= 0 && !pipes_queries(p, *attn) && !pipes_output(p, *attn) && (rc = pipe_end(p))) return rc;
   pipe_release(p, p->pipe_app_a, slot_a);
   pipe_release(p, p->pipe_app_b, slot_b);
   return RELUX_OK;
@@ -1510,6 +1614,18 @@ API int32_t relux_mla_expand_kv(relux_pool_t h, const relux_mla_expand_args* a) 
 API int32_t relux_gqa_verify(relux_pool_t h, const relux_attn_args* attn, const relux_append_args* kv) {
   GET_POOL(h);
   return do_verify(p, attn, kv, RELUX_POOL_GQA);
+}
+API int32_t relux_gqa_tree_verify(relux_pool_t h, const relux_attn_args* attn, const relux_append_args* kv, const relux_tree_args* tree) {
+  GET_POOL(h);
+  return do_gqa_tree(p, attn, kv, tree);
+}
+API int32_t relux_gqa_tree_commit(relux_pool_t h, const relux_tree_commit_args* a) {
+  GET_POOL(h);
+  return do_tree_commit(p, a);
+}
+API int32_t relux_gqa_read_kv(relux_pool_t h, const relux_read_kv_args* a) {
+  GET_POOL(h);
+  return do_read_kv(p, a);
 }
 API int32_t relux_mla_verify(relux_pool_t h, const relux_attn_args* attn, const relux_append_args* kv) {
   GET_POOL(h);

@@ -21,7 +21,7 @@ MEM_HOST, MEM_DEVICE = 0, 1
 LAYOUT_TOKEN_MAJOR, LAYOUT_HEAD_MAJOR = 0, 1
 POOL_MLA, POOL_GQA = 0, 1
 ATTN_FAST, ATTN_REFERENCE, ATTN_REFERENCE_FAITHFUL = 0, 1, 2
-POOL_FLAG_REFERENCE_COMPAT = 1
+POOL_FLAG_REFERENCE_COMPAT, POOL_FLAG_CACHE_INT8 = 1, 2
 CALL_PIPELINED = 1
 (TUNE_MLA_GENERIC, TUNE_MLA_WORKERS, TUNE_CHUNK_PAGES, TUNE_GEMM_GENERIC, TUNE_GEMM_SPLIT, TUNE_GQA_PROMPT_PARTIAL_MB, TUNE_SEL_CLUSTER,
  TUNE_SEL_LOOKAHEAD, TUNE_SEL_BATCHED, TUNE_GQA_PROMPT_SLICES, TUNE_MLA_PROMPT_MIN_TOKENS, TUNE_MLA_PROMPT_SCRATCH_MB,
@@ -39,6 +39,7 @@ EXPORTS = [
     "relux_mla_verify", "relux_pool_last_kernel_ms", "relux_pool_kernel_ms_mean", "relux_mla_forward_cached", "relux_gqa_forward_cached", "relux_stream_partition", "relux_seq_save_file", "relux_seq_load_file", "relux_pool_projection_ms_mean", "relux_gqa_decode_noalloc",
     "relux_spec_accept", "relux_sampler_sample", "relux_pool_tune", "relux_pool_kernel_ms_list", "relux_matmul_f32_bf16",
     "relux_mla_import_weights", "relux_pool_selftest_wait", "relux_pool_wait_output", "relux_mla_step", "relux_gqa_step", "relux_mla_expand_kv",
+    "relux_gqa_read_kv", "relux_gqa_tree_verify", "relux_gqa_tree_commit",
 ]
 
 
@@ -77,6 +78,20 @@ class AttnArgs(C.Structure):
                 ("q_layout", C.c_int32), ("w_uk", C.c_void_p), ("w_uv", C.c_void_p), ("out", C.c_void_p),
                 ("out_dtype", C.c_int32), ("out_mem", C.c_int32), ("out_layout", C.c_int32), ("mode", C.c_int32),
                 ("flags", C.c_int32), ("reserved", C.c_int32 * 4)]
+
+
+class ReadKvArgs(C.Structure):
+    _fields_ = [("layer", C.c_int32), ("n_seqs", C.c_int32), ("seq_ids", C.c_void_p), ("tok0", C.c_void_p), ("n_tokens", C.c_void_p),
+                ("dtype", C.c_int32), ("reserved", C.c_int32 * 3), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class TreeArgs(C.Structure):
+    _fields_ = [("parents", C.c_void_p), ("n_trees", C.c_int32), ("reserved", C.c_int32 * 3)]
+
+
+class TreeCommitArgs(C.Structure):
+    _fields_ = [("layer", C.c_int32), ("n_seqs", C.c_int32), ("seq_ids", C.c_void_p), ("path", C.c_void_p), ("path_len", C.c_void_p),
+                ("path_stride", C.c_int32), ("reserved", C.c_int32 * 3)]
 
 
 class MlaLayerWeights(C.Structure):
@@ -151,6 +166,9 @@ def _packer(cls, skip=("reserved",)):
 
 pack_append = _packer(AppendArgs)
 pack_attn = _packer(AttnArgs)
+pack_read_kv = _packer(ReadKvArgs)
+pack_tree = _packer(TreeArgs)
+pack_tree_commit = _packer(TreeCommitArgs)
 
 
 class ReluxCudaError(RuntimeError):
@@ -228,6 +246,9 @@ def load():
         L.relux_seq_load_file.argtypes = [C.c_void_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p]
         L.relux_gqa_forward_cached.argtypes = [C.c_void_p, C.POINTER(GqaLayerArgs)]
         L.relux_mla_forward_cached.argtypes = [C.c_void_p, C.POINTER(MlaLayerArgs)]
+        L.relux_gqa_read_kv.argtypes = [C.c_void_p, C.POINTER(ReadKvArgs)]
+        L.relux_gqa_tree_verify.argtypes = [C.c_void_p, C.POINTER(AttnArgs), C.POINTER(AppendArgs), C.POINTER(TreeArgs)]
+        L.relux_gqa_tree_commit.argtypes = [C.c_void_p, C.POINTER(TreeCommitArgs)]
         L.relux_spec_accept.argtypes = [C.c_void_p, C.POINTER(SpecAcceptArgs)]
         L.relux_sampler_sample.argtypes = [C.c_void_p, C.POINTER(SampleArgs)]
         L.relux_pool_last_kernel_ms.argtypes = [C.c_void_p, C.POINTER(C.c_float)]
@@ -236,7 +257,7 @@ def load():
         L.relux_cuda_stream.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
         # the per-token calls once more, taking their argument structs as packed bytes (pack_append, pack_attn)
         for name, n_structs in (("mla_append", 1), ("gqa_append", 1), ("mla_decode", 1), ("gqa_decode", 1), ("mla_verify", 2), ("gqa_verify", 2),
-                                ("mla_step", 2), ("gqa_step", 2)):
+                                ("mla_step", 2), ("gqa_step", 2), ("gqa_tree_verify", 3), ("gqa_tree_commit", 1), ("gqa_read_kv", 1)):
             f = L["relux_" + name]   # a function object of its own
             f.restype, f.argtypes = C.c_int32, [C.c_void_p] + [C.c_char_p] * n_structs
             packed[name] = f

@@ -105,6 +105,12 @@ __device__ __forceinline__ uint32_t int8x2_to_bf16(uint32_t t) {
 }
 
 // ---- queries ----
+// The power of two that brings a row's largest value, of bits `top`, to [2^14, 2^15), and its inverse.  (Not rows of zeros or of subnormal numbers.)
+__device__ __forceinline__ void query_factor(uint32_t top, float& up, float& down) {
+  const int k = min(141 - (int)(top >> 23), 126);
+  up = __uint_as_float((uint32_t)(127 + k) << 23);
+  down = __uint_as_float((uint32_t)(127 - k) << 23);
+}
 // Row of queries in shared memory: 128 binary16 values, the row's factor (what a score of theirs is multiplied by, softmax scale and log2 e included),
 // and what the row sees of the new rows.  By 16 lanes of a converged warp, eight dims each.
 __device__ __forceinline__ void int8_put_query(uint16_t* row, int ch, bool there, const void* q, size_t off, bool q_bf16, float scale_log2) {
@@ -115,8 +121,8 @@ __device__ __forceinline__ void int8_put_query(uint16_t* row, int ch, bool there
     if (q_bf16) load8(x, reinterpret_cast<const uint16_t*>(q) + off);
     else load8(x, reinterpret_cast<const float*>(q) + off);
   }
-  const int k = min(141 - (int)(row_top(x) >> 23), 126);   // the largest value comes to [2^14, 2^15); a row of zeros or of subnormal numbers does not
-  const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+  float up, down;
+  query_factor(row_top(x), up, down);
   if (!there) return;
   uint32_t w[4];
 #pragma unroll

@@ -122,6 +122,7 @@ static int32_t launch_stream(Pool* p, const SeqBatch& sb, const relux_attn_args&
 int32_t launch_gqa_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16,
                           const GqaAppend* app, const GqaTree* tree) {
   const int per = std::max(1, 32 / (a.num_heads / p->prm.gqa_num_kv_heads));   // query tokens of a launch
+  if (tree && a.q_tokens > per) return launch_gqa_tree_sm100(p, sb, a, d_q, d_out, out_bf16, *tree, app->rows);
   for (int s0 = 0; s0 < a.q_tokens; s0 += per)
     if (int32_t rc = launch_stream(p, sb, a, d_q, d_out, out_bf16, app, tree, s0 == 0, s0, std::min(per, a.q_tokens - s0))) return rc;
   return RELUX_OK;

@@ -1,0 +1,865 @@
+// Attention of drafted trees with more than 32 query rows per kv head, on the 5th-generation tensor cores (tcgen05 + TMEM), over the bf16 and the 8-bit
+// grouped-query cache.
+//
+// o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  where query token i sees every cached row and, of the drafted ones, itself
+// and its ancestors.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128 operations for the 512 (264) bytes of
+// a token and kv head, so the cache's bytes bound trees of up to some 200 rows (100 on the 8-bit cache) and the tensor cores and the softmax larger ones.
+//
+// A STREAM is a sequence's tiles of 128 keys for one kv head and up to 256 of its rows (one or two blocks of 128, M of both contractions).  All streams of the
+// call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into one equal range per SM; a PIECE is the part of a stream inside a range.
+// A piece that is a whole stream writes its output; others leave float32 partials that merge_tree_kernel joins.
+//
+// Roles of a CTA:
+//   producer   a tile's K and V by TMA, 32 KB each, into a ring; on the 8-bit cache 16 KB each and the scales into a ring of their own
+//   converters (8-bit cache, four warps) codes -> binary16 operands in the ring's swizzled layout.  K as whole numbers: a row's scale multiplies its column of
+//              scores, in float32.  V times its scale over a power of two that all of the piece's rows share so far (11 bits, as P has then; 2^29 between
+//              the largest row and one that is no longer exact to 11 bits); where a row comes that is too large for it, the power grows and O is rescaled.
+//   MMA        step k = (tile, block): S = Q K^T (S buffer k & 1), O[block] += P V with P read from tensor memory over the scores it came from
+//   softmax    eight warps of 16 rows of a block each, four lanes to a row: scores from TMEM, running max (updated lazily), P back to TMEM
+// Order of issue: QK(k + 1), PV(k): the tensor pipe executes in issue order, so QK(k + 2) finds its S buffer read.
+// A product with P = 0 does not hide an infinity or a NaN among the values: those of drafted rows and of what lies behind are set to zero in the tile, and
+// the rows that see one become NaN at the end.  (8-bit rows have them in their scale alone; a code is always a number.)
+// Every wait is bounded (RELUX_ERR_TIMEOUT, an abort flag that ends the other waits; all warps reach the end and TMEM is freed).
+#include <algorithm>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "gqa_int8_parts.cuh"
+#include "internal.h"
+#include "softmax_parts.cuh"
+#include "umma.cuh"
+
+namespace relux {
+
+namespace {
+
+constexpr int kTile = 128, kD = kGqaD, kPage = kGqaPageTok;
+constexpr int kHalf = 16384;                   // [128 rows][64 16-bit columns], 128-byte swizzle
+constexpr int kSlot = 2 * kHalf;               // K or V of a tile, or 128 query rows
+constexpr int kRawSlot = kTile * kD;           // codes of K or V of a tile
+constexpr int kFixUnits = 2;                   // tiles: what a piece costs beyond its own (queries in, results out)
+constexpr int kSoftmaxWarps = 8, kConvWarps = 4;
+constexpr int kWarpLoad = kSoftmaxWarps, kWarpMma = kSoftmaxWarps + 1, kWarpConv = kSoftmaxWarps + 2;
+constexpr uint32_t kTmemCols = 512, kTmemO = 256;
+constexpr float kRescaleThreshold = 8.0f;      // log2: P reaches 2^8 before the running max follows
+// (8-bit cache) log2: what P and its sum are larger by.  Binary16 has 11 bits down to 2^-14, and P reaches 2^(8 + 7): probabilities keep 11 bits down to 2^-21
+// of the row's largest, and below are off by at most 2^-32 of it.
+constexpr float kPUp = 7.0f;
+constexpr int kPolyPairsOf8 = 2;               // of a lane's score pairs, as many take the exponential on the FMA pipe
+constexpr int kInlineSmall = 32, kInlineLarge = 256;
+
+struct TreeSeq {
+  int32_t seq, len0, nodes;
+  int32_t unit0;               // first unit of the sequence, one stream counted
+};
+struct TreeCommon {
+  const TreeSeq* seqs;         // device copy, or nullptr: inline
+  const int8_t* parents;       // of a device copy
+  int32_t one_tree;
+  const int32_t* table;
+  int32_t table_stride, num_pages, n_seqs, range, range_more, Hkv, H, g, S, R;
+  int32_t n_rb, rows_rb;       // row groups of a kv head, rows of each (the last may have fewer)
+  int32_t krow0, vrow0;
+  const float* scales;         // 8-bit cache: of the layer
+  float scale_log2;
+  const void* q;
+  int32_t q_bf16, out_bf16;
+  void* out;
+  float* part_o;               // [2 * workers][rows_rb][128]
+  float* part_ml;              // [2 * workers][rows_rb][2]
+  int32_t* status;
+  TimeStamp time;
+};
+template <int N>
+struct TreeParams {
+  TreeCommon c;
+  TreeSeq seqs[N + 1];
+  int8_t parents[N][kTreeNodes];
+};
+
+// The streams as every role walks them: pieces of this range, in order.
+struct Piece {
+  int32_t i, st, us, tb, te, tiles;   // sequence of the call, stream of the sequence (kv head * n_rb + row group), its first unit, tiles [tb, te) of `tiles`
+};
+template <int N>
+struct Streams {
+  const TreeParams<N>& prm;
+  int32_t u_begin, u_end;
+  __device__ __forceinline__ Streams(const TreeParams<N>& p, int worker) : prm(p), u_begin(range_begin(worker)), u_end(range_begin(worker + 1)) {}
+  __device__ __forceinline__ int unit0(int i) const { return prm.c.seqs ? prm.c.seqs[i].unit0 : prm.seqs[i].unit0; }
+  __device__ __forceinline__ TreeSeq seq(int i) const { return prm.c.seqs ? prm.c.seqs[i] : prm.seqs[i]; }
+  __device__ __forceinline__ int per_seq() const { return prm.c.Hkv * prm.c.n_rb; }
+  __device__ __forceinline__ int range_begin(int w) const { return w * prm.c.range + min(w, prm.c.range_more); }
+  __device__ __forceinline__ int worker_of(int u) const {
+    const int big = prm.c.range_more * (prm.c.range + 1);
+    return u < big ? (int)((unsigned)u / (unsigned)(prm.c.range + 1)) : prm.c.range_more + (int)((unsigned)(u - big) / (unsigned)prm.c.range);
+  }
+  // The stream that unit u belongs to, from its tile at u on.
+  __device__ __forceinline__ Piece at(int u) const {
+    int lo = 0, hi = prm.c.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (unit0(mid) * per_seq() <= u) lo = mid;
+      else hi = mid;
+    }
+    Piece p;
+    p.i = lo;
+    const int n0 = unit0(lo), len = unit0(lo + 1) - n0;
+    p.st = (u - n0 * per_seq()) / len;
+    p.us = n0 * per_seq() + p.st * len;
+    p.tiles = len - kFixUnits;
+    p.tb = u - p.us;
+    p.te = min(p.tiles, u_end - p.us);
+    return p;
+  }
+  __device__ __forceinline__ bool valid(const Piece& p) const { return p.us < u_end; }
+  __device__ __forceinline__ Piece next(const Piece& q) const {
+    Piece p = q;
+    p.us += p.tiles + kFixUnits;
+    if (++p.st == per_seq()) {
+      p.st = 0;
+      p.i++;
+      if (p.us < u_end) p.tiles = unit0(p.i + 1) - unit0(p.i) - kFixUnits;
+    }
+    p.tb = 0;
+    p.te = min(p.tiles, u_end - p.us);
+    return p;
+  }
+  __device__ __forceinline__ Piece first() const {
+    const Piece p = at(u_begin);
+    return p.tb < p.tiles ? p : next(p);   // a range may begin in the fixed-cost units of a stream
+  }
+};
+
+struct Bars {
+  uint64_t full[6], empty[6], raw_full[5], raw_empty[5], info[4], s_full[2], p_full[2], q_full, pv, fin, drain;
+  uint32_t tmem_base;
+  volatile int32_t abort_flag;
+  uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
+  uint32_t bad_all[4];         // (8-bit cache) a cached row with one
+  float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
+  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys; without it there is no room for this
+};
+constexpr int kBarBytes = 3072;
+static_assert(sizeof(Bars) <= kBarBytes && kBarBytes - sizeof(Bars::k_scale) >= offsetof(Bars, k_scale), "barrier block too large");
+
+template <bool kI8, int kNB>
+struct Plan {
+  static constexpr int kSlots = kI8 ? 3 : kNB == 2 ? 5 : 6;       // of 32 KB
+  static constexpr int kRaw = kI8 ? (kNB == 2 ? 3 : 5) : 0;       // of 16 KB
+  static constexpr int kScaleSlots = kI8 ? 4 : 0;                 // scales as they come, of a tile, 1 KB
+  static constexpr int kQ = 0;
+  static constexpr int kRing = kNB * kSlot;
+  static constexpr int kRawAt = kRing + kSlots * kSlot;
+  static constexpr int kScaleAt = kRawAt + kRaw * kRawSlot;
+  static constexpr int kBars = kScaleAt + kScaleSlots * 1024;
+  static constexpr int kTotal = 1024 + kBars + (kI8 ? kBarBytes : kBarBytes - kTile * 16);
+  static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
+  static constexpr int kThreads = 32 * (kI8 ? kWarpConv + kConvWarps : kWarpConv);
+};
+__device__ __noinline__ void wait_slow(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
+  for (uint32_t i = 0; i < kSpinLimit; i++) {
+    if (mbar_try_wait(bar, parity)) return;
+    if ((i & 255) == 255 && b->abort_flag) return;
+    if (i > 512) __nanosleep(20);
+  }
+  b->abort_flag = 1;
+  set_status(status, RELUX_ERR_TIMEOUT);
+}
+__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
+  if (!mbar_try_wait(bar, parity)) wait_slow(bar, parity, b, status);
+}
+
+// Instruction descriptor of binary16 operands: make_idesc_bf16 with formats 0.
+constexpr uint32_t idesc_of(bool f16, bool b_mn_major) { return make_idesc_bf16(128, 128, false, b_mn_major) & (f16 ? ~((7u << 7) | (7u << 10)) : ~0u); }
+
+template <bool kI8>
+__device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
+  if constexpr (kI8) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return round_bf16x2(lo, hi);
+  }
+}
+// exp2(score * factor - max) of a lane's 2 x 32 scores (tmem_ld_16x256b_x16), packed in the order of tmem_st_16x128b_x16; row sums are added to ps2.
+template <bool kI8, bool kPoly>
+__device__ __forceinline__ void exp_scores(const uint32_t (&sv)[64], const uint64_t (&factor2)[2], const uint64_t (&neg_m2)[2], uint32_t (&pw)[32], uint64_t (&ps2)[2]) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) {   // pair i: row i & 1
+    const uint64_t x2 = fma2(pack2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), factor2[i & 1], neg_m2[i & 1]);
+    uint64_t p2;
+    if (kPoly && (i & 7) < kPolyPairsOf8) {
+      p2 = ex2_poly2(x2);
+    } else {
+      float x0, x1;
+      unpack2(x2, x0, x1);
+      p2 = pack2(ex2_approx(x0), ex2_approx(x1));
+    }
+    ps2[i & 1] = add2(ps2[i & 1], p2);
+    float p0, p1;
+    unpack2(p2, p0, p1);
+    pw[i] = pack_p<kI8>(p0, p1);
+  }
+}
+
+template <bool kI8, int kNB, int N>
+__global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
+    tree_sm100_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ TreeParams<N> prm) {
+  using PL = Plan<kI8, kNB>;
+  const TreeCommon& c = prm.c;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  Bars* bars = reinterpret_cast<Bars*>(smem + PL::kBars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 6; s++) {
+      mbar_init(&bars->full[s], kI8 ? kConvWarps : 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < 5; s++) {
+      mbar_init(&bars->raw_full[s], 1);
+      mbar_init(&bars->raw_empty[s], kConvWarps);
+    }
+    for (int s = 0; s < 4; s++) {
+      mbar_init(&bars->info[s], kConvWarps);
+      bars->bad_nodes[s] = 0;
+      bars->bad_all[s] = 0;
+    }
+    for (int s = 0; s < 2; s++) {
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], kSoftmaxWarps);
+    }
+    mbar_init(&bars->q_full, kSoftmaxWarps);
+    mbar_init(&bars->pv, 1);
+    mbar_init(&bars->fin, 2);
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap);
+  }
+  if (warp == 0) {
+    tmem_alloc<1>(&bars->tmem_base, kTmemCols);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  chain_release();
+  chain_wait();
+  if (threadIdx.x == 0) stamp_begin(c.time);
+  const Streams<N> streams(prm, blockIdx.x);
+  auto rows_of = [&](const Piece& p) -> int { return min(c.rows_rb, c.R - (p.st % c.n_rb) * c.rows_rb); };
+  auto blocks_of = [&](const Piece& p) -> int { return kNB == 1 ? 1 : (rows_of(p) + 127) / 128; };
+
+  if (warp == kWarpLoad) {
+    // =============================== producer ===============================
+    const bool el = elect_one();
+    int h = 0;   // half tiles so far: K of tile n is 2 n, V 2 n + 1
+    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p)) {
+      const TreeSeq sq = streams.seq(p.i);
+      const int kvh = p.st / c.n_rb;
+      const int last_slot = max(0, (sq.len0 + sq.nodes + kPage - 1) / kPage - 1);   // a tile's second page may lie past the rows: nobody sees those keys
+      const int32_t* row = c.table + (size_t)sq.seq * c.table_stride;
+      int32_t ids = 0;
+      for (int t = p.tb; t < p.te; t++) {
+        if (((t - p.tb) & 15) == 0) ids = __ldg(row + min(2 * t + lane, last_slot));
+        int32_t pg[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          pg[k] = __shfl_sync(0xffffffffu, ids, (2 * (t - p.tb) + k) & 31);
+          if (pg[k] < 0 || pg[k] >= c.num_pages) {   // reported, and replaced by page 0 so that no load leaves the pool
+            set_status(c.status, RELUX_ERR_BAD_PAGE);
+            pg[k] = 0;
+          }
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++, h++) {
+          const int32_t row0 = kv ? c.vrow0 : c.krow0;
+          if constexpr (kI8) {
+            const int st = h % PL::kRaw, use = h / PL::kRaw;
+            if (use > 0) wait_bar(&bars->raw_empty[st], (use - 1) & 1, bars, c.status);
+            if (el) {
+              uint8_t* dst = smem + PL::kRawAt + st * kRawSlot;
+              mbar_expect_tx(&bars->raw_full[st], kRawSlot + (kv ? 0 : 1024));
+              for (int k = 0; k < 2; k++) {
+                tma_load_2d(dst + k * 8192, &tmap, 0, row0 + (pg[k] * c.Hkv + kvh) * kPage, &bars->raw_full[st]);
+                if (!kv)   // the scales of both, [page][K, V][64]
+                  bulk_load(smem + PL::kScaleAt + ((h >> 1) & 3) * 1024 + k * kInt8ScaleBytes, c.scales + ((size_t)pg[k] * c.Hkv + kvh) * (2 * kPage),
+                            kInt8ScaleBytes, &bars->raw_full[st]);
+              }
+            }
+          } else {
+            const int st = h % PL::kSlots, use = h / PL::kSlots;
+            if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
+            if (el) {
+              uint8_t* dst = smem + PL::kRing + st * kSlot;
+              mbar_expect_tx(&bars->full[st], kSlot);
+              for (int k = 0; k < 2; k++) {
+                const int32_t y = row0 + (pg[k] * c.Hkv + kvh) * kPage;
+                tma_load_2d(dst + k * 8192, &tmap, 0, y, &bars->full[st]);
+                tma_load_2d(dst + kHalf + k * 8192, &tmap, 64, y, &bars->full[st]);
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else if (warp == kWarpMma) {
+    // =============================== MMA issuer ===============================
+    const bool el = elect_one();
+    constexpr uint32_t idesc_qk = idesc_of(kI8, false), idesc_pv = idesc_of(kI8, true);
+    const uint64_t dQ = make_desc_kmajor_sw128(smem_u32(smem + PL::kQ));
+    int k = 0, tt = 0, n = 0;   // steps, tiles, pieces so far
+    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+      const int nb = blocks_of(p), tiles = p.te - p.tb;
+      const TreeSeq sq = streams.seq(p.i);
+      wait_bar(&bars->q_full, n & 1, bars, c.status);   // the queries are there, and O of the piece before has been read
+      auto issue_qk = [&](int t, int b, int step) {
+        const int h = 2 * (tt + t), st = h % PL::kSlots;
+        if (b == 0) wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars, c.status);
+        tc_fence_after();
+        if (el) {
+          const uint64_t dK = make_desc_kmajor_sw128(smem_u32(smem + PL::kRing + st * kSlot));
+          const uint64_t dQb = dQ + ((uint32_t)(b * kSlot) >> 4);
+#pragma unroll
+          for (int ks = 0; ks < 8; ks++) {
+            const uint32_t off = (uint32_t)((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+            umma_ss<1>(tmem + (step & 1) * 128, dQb + off, dK + off, idesc_qk, ks != 0);
+          }
+          if (b == nb - 1) umma_commit<1>(&bars->empty[st]);
+          umma_commit<1>(&bars->s_full[step & 1]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int t, int b, int step) {
+        const int h = 2 * (tt + t) + 1, st = h % PL::kSlots;
+        if (b == 0) {
+          wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars, c.status);
+          if constexpr (!kI8) {   // infinities and NaN among drafted values, and behind them
+            const int from = sq.len0 - (p.tb + t) * kTile;   // first drafted row of the tile
+            if (from < kTile) {
+              uint8_t* v = smem + PL::kRing + st * kSlot;
+              bool any = false;
+              for (int r = max(from, 0) + (lane >> 4); r < kTile; r += 2) {   // 16 lanes a row
+                uint4* at = reinterpret_cast<uint4*>(v + ((lane >> 3) & 1) * kHalf + swz128(r, lane & 7));
+                const uint4 w = *at;
+                if (bf16x2_not_finite(w.x) | bf16x2_not_finite(w.y) | bf16x2_not_finite(w.z) | bf16x2_not_finite(w.w)) {
+                  *at = make_uint4(bf16x2_finite(w.x), bf16x2_finite(w.y), bf16x2_finite(w.z), bf16x2_finite(w.w));
+                  if (r - from < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << (r - from));
+                  any = true;
+                }
+              }
+              if (any) fence_proxy_async();
+              __syncwarp();
+            }
+          }
+        }
+        wait_bar(&bars->p_full[step & 1], (step >> 1) & 1, bars, c.status);
+        tc_fence_after();   // P, and a rescaled O
+        if (el) {
+          const uint64_t dV = make_desc_mnmajor_sw128(smem_u32(smem + PL::kRing + st * kSlot), kHalf);
+#pragma unroll
+          for (int ks = 0; ks < 8; ks++)
+            umma_ts<1>(tmem + kTmemO + b * 128, tmem + (step & 1) * 128 + ks * 8, dV + ((uint32_t)(ks * 2048) >> 4), idesc_pv, t != 0 || ks != 0);
+          if (b == nb - 1) umma_commit<1>(&bars->empty[st]);
+          umma_commit<1>(&bars->pv);
+        }
+        __syncwarp();
+      };
+      issue_qk(0, 0, k);
+      for (int t = 0; t < tiles; t++)
+        for (int b = 0; b < nb; b++, k++) {
+          if (b + 1 < nb) issue_qk(t, b + 1, k + 1);
+          else if (t + 1 < tiles) issue_qk(t + 1, 0, k + 1);
+          issue_pv(t, b, k);
+        }
+      tt += tiles;
+      if (el) umma_commit<1>(&bars->fin);         // the piece's products are complete
+      if (lane == 0) mbar_arrive(&bars->fin);     // and what this warp, or the converters before they handed over the values, wrote beside them
+      __syncwarp();
+    }
+    // nothing may be freed while an MMA is in flight: the read-out's waits say so, unless one gave up
+    if (el) umma_commit<1>(&bars->drain);
+    __syncwarp();
+    mbar_wait(&bars->drain, 0);
+  } else if (warp < kSoftmaxWarps) {
+    // =============================== softmax ===============================
+    // Warp w reads TMEM lanes 32 (w & 3) .. +31 (the hardware's rule), of which warps w and w + 4 take 16 each: rows 16 w .. 16 w + 15 of a block.
+    // Few rows then keep all four schedulers busy.
+    const int r16 = (warp & 3) * 32 + (warp >> 2) * 16;
+    const uint32_t lane_addr = (uint32_t)r16 << 16;
+    int k = 0, tt = 0, n = 0;
+    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+      const int nb = blocks_of(p), rows = rows_of(p), kvh = p.st / c.n_rb, row_base = (p.st % c.n_rb) * c.rows_rb;
+      const TreeSeq sq = streams.seq(p.i);
+      uint64_t see[kNB][2];
+      float q_scale[kNB][2];
+      // ---- queries in ----
+#pragma unroll
+      for (int b = 0; b < kNB; b++) {
+        if (b >= nb) continue;
+        {   // what this warp's rows see of the nodes: a row per lane, then to the lanes that work on it
+          const int r = 128 * b + 16 * warp + (lane & 15), s = (row_base + r) / c.g, tree = c.one_tree ? 0 : p.i;
+          uint64_t m = 0;
+          if (r < rows && s < sq.nodes)
+            for (int j = s; j >= 0; j = c.seqs ? c.parents[tree * kTreeNodes + j] : prm.parents[tree][j]) m |= 1ull << j;
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) see[b][hf] = __shfl_sync(0xffffffffu, (unsigned long long)m, (lane >> 2) + 8 * hf);
+        }
+        q_scale[b][0] = q_scale[b][1] = c.scale_log2;
+#pragma unroll 4
+        for (int i = 0; i < 8; i++) {   // 16 lanes a row, two rows at a time
+          const int j = 2 * i + (lane >> 4), r = 128 * b + 16 * warp + j, ch = (lane & 15) * 8;
+          const int s = (row_base + r) / c.g, hq = row_base + r - s * c.g;
+          const size_t off = (((size_t)p.i * c.S + s) * c.H + (size_t)kvh * c.g + hq) * kD + ch;
+          uint8_t* dst = smem + PL::kQ + b * kSlot + (ch >> 6) * kHalf + swz128(r16 + j, (ch & 63) >> 3);
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (kI8) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = 0.f;
+            if (r < rows) {
+              if (c.q_bf16) load8(x, reinterpret_cast<const uint16_t*>(c.q) + off);
+              else load8(x, reinterpret_cast<const float*>(c.q) + off);
+            }
+            float up, down;
+            query_factor(row_top(x), up, down);
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = pack_p<true>(x[2 * e] * up, x[2 * e + 1] * up);
+            w = make_uint4(y[0], y[1], y[2], y[3]);
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              const float f = __shfl_sync(0xffffffffu, down, ((lane >> 2) & 1) * 16);
+              if (((lane >> 2) + 8 * hf) >> 1 == i) q_scale[b][hf] = c.scale_log2 * f;
+            }
+          } else if (r < rows) {
+            if (c.q_bf16) {
+              w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(c.q) + off);
+            } else {
+              float x[8];
+              load8(x, reinterpret_cast<const float*>(c.q) + off);
+              w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+            }
+          }
+          *reinterpret_cast<uint4*>(dst) = w;
+        }
+      }
+      fence_proxy_async();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full);
+      // ---- tiles ----
+      float m_used[kNB][2], l_run[kNB][2], v_unit = 1.f;
+#pragma unroll
+      for (int b = 0; b < kNB; b++)
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          m_used[b][hf] = -INFINITY;
+          l_run[b][hf] = 0.f;
+        }
+      for (int t = p.tb; t < p.te; t++, tt++) {
+        const int from = sq.len0 - t * kTile;   // first drafted row of the tile
+        float shrink = 1.f;                     // what O's unit has grown by
+        const float* k_scale = bars->k_scale[tt & 3];
+        if constexpr (kI8) {
+          wait_bar(&bars->info[tt & 3], (tt >> 2) & 1, bars, c.status);
+          const float unit = bars->v_unit[tt & 3];
+          if (t > p.tb) shrink = v_unit / unit;
+          v_unit = unit;
+        }
+#pragma unroll
+        for (int b = 0; b < kNB; b++) {
+          if (b >= nb) continue;
+          const uint32_t tmem_s = tmem + lane_addr + (k & 1) * 128, tmem_o = tmem + lane_addr + kTmemO + b * 128;
+          wait_bar(&bars->s_full[k & 1], (k >> 1) & 1, bars, c.status);
+          if (128 * b + 16 * warp < rows) {   // else the whole warp's rows are none
+            tc_fence_after();
+            uint32_t sv[64];
+            tmem_ld_16x256b_x16(tmem_s, sv);
+            tmem_ld_wait();
+            if constexpr (kI8) {
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                const float2 s = *reinterpret_cast<const float2*>(k_scale + 8 * i + 2 * (lane & 3));
+                const uint64_t s2 = pack2(s.x, s.y);
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                  float x0, x1;
+                  unpack2(mul2(pack2(__uint_as_float(sv[4 * i + 2 * hf]), __uint_as_float(sv[4 * i + 2 * hf + 1])), s2), x0, x1);
+                  sv[4 * i + 2 * hf] = __float_as_uint(x0);
+                  sv[4 * i + 2 * hf + 1] = __float_as_uint(x1);
+                }
+              }
+            }
+            const bool whole = from >= kTile;
+            if (!whole) {
+#pragma unroll
+              for (int i = 0; i < 16; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  const int node = 8 * i + 2 * (lane & 3) + e - from;
+#pragma unroll
+                  for (int hf = 0; hf < 2; hf++)
+                    if (node >= 0 && (node >= kTreeNodes || !(see[b][hf] >> node & 1u))) sv[4 * i + 2 * hf + e] = 0xFF800000u;   // -inf
+                }
+            }
+            // row maxima of the raw scores: four chains of three-input maxima
+            float mx[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int i = 0; i < 16; i++) m4[i & 3] = max3(m4[i & 3], __uint_as_float(sv[4 * i + 2 * hf]), __uint_as_float(sv[4 * i + 2 * hf + 1]));
+              mx[hf] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * q_scale[b][hf];
+            }
+            float alpha[2] = {shrink, shrink};
+            bool rescale = kI8 && shrink != 1.f;
+            if (__any_sync(0xffffffffu, mx[0] > m_used[b][0] + kRescaleThreshold || mx[1] > m_used[b][1] + kRescaleThreshold)) {
+#pragma unroll
+              for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], o));
+#pragma unroll
+              for (int hf = 0; hf < 2; hf++)
+                if (mx[hf] > m_used[b][hf] + kRescaleThreshold) {
+                  if (m_used[b][hf] != -INFINITY) {
+                    const float a = ex2_approx(m_used[b][hf] - mx[hf]);
+                    alpha[hf] *= a;
+                    l_run[b][hf] *= a;
+                    rescale = true;
+                  }
+                  m_used[b][hf] = mx[hf];
+                }
+            }
+            uint64_t factor2[2], neg_m2[2], ps2[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              const float neg_m = (m_used[b][hf] == -INFINITY ? 0.f : -m_used[b][hf]) + (kI8 ? kPUp : 0.f);
+              factor2[hf] = pack2(q_scale[b][hf], q_scale[b][hf]);
+              neg_m2[hf] = pack2(neg_m, neg_m);
+              ps2[hf] = pack2(0.f, 0.f);
+            }
+            uint32_t pw[32];
+            if (whole) exp_scores<kI8, true>(sv, factor2, neg_m2, pw, ps2);
+            else exp_scores<kI8, false>(sv, factor2, neg_m2, pw, ps2);   // ex2(-inf) is 0, the polynomial's is not
+            tmem_st_16x128b_x16(tmem_s, pw);
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              float ps0, ps1;
+              unpack2(ps2[hf], ps0, ps1);
+              l_run[b][hf] += ps0 + ps1;
+            }
+            // O may be rescaled only behind the PV before this one on it.  With two blocks that is the one before QK(k) in the pipe, with one block
+            // PV(k - 1), which QK(k) was ahead of: `pv` has then completed k - 1 or k phases, so its parity is no riddle.
+            if (t > p.tb && __any_sync(0xffffffffu, rescale)) {
+              if (nb == 1) {
+                wait_bar(&bars->pv, (k - 1) & 1, bars, c.status);
+                tc_fence_after();
+              }
+#pragma unroll 1
+              for (int col = 0; col < kD; col += 64) {
+                uint32_t ov[32];
+                tmem_ld_16x256b_x8(tmem_o + col, ov);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha[(i >> 1) & 1]);
+                tmem_st_16x256b_x8(tmem_o + col, ov);
+              }
+            }
+            tmem_st_wait();
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_full[k & 1]);
+          k++;
+        }
+      }
+      // ---- results out ----
+      wait_bar(&bars->fin, n & 1, bars, c.status);
+      tc_fence_after();
+      const bool ok = bars->abort_flag == 0;
+      const uint64_t bad_nodes = bars->bad_nodes[n & 3];
+      const bool bad_all = bars->bad_all[n & 3] != 0;
+      const bool stream_whole = p.tb == 0 && p.te == p.tiles;
+      const int slot = 2 * (int)blockIdx.x + (p.us + p.tb == streams.u_begin ? 0 : 1);
+#pragma unroll
+      for (int b = 0; b < kNB; b++) {
+        if (b >= nb || 128 * b + 16 * warp >= rows) continue;
+        float f[2];
+        int r[2], s[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          float l = l_run[b][hf];
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          if (bad_all || (see[b][hf] & bad_nodes)) l = __uint_as_float(0x7FC00000u);
+          r[hf] = 128 * b + 16 * warp + 8 * hf + (lane >> 2);
+          s[hf] = (row_base + r[hf]) / c.g;
+          const bool there = ok && s[hf] < sq.nodes;
+          if (stream_whole) {
+            f[hf] = !there || l == 0.f ? 0.f : v_unit / l;
+          } else {
+            f[hf] = there ? v_unit : 0.f;
+            if ((lane & 3) == 0 && r[hf] < rows)
+              *reinterpret_cast<float2*>(c.part_ml + ((size_t)slot * c.rows_rb + r[hf]) * 2) = there ? make_float2(m_used[b][hf], l) : make_float2(-INFINITY, 0.f);
+          }
+        }
+#pragma unroll 1
+        for (int col = 0; col < kD; col += 64) {
+          uint32_t ov[32];
+          tmem_ld_16x256b_x8(tmem + lane_addr + kTmemO + b * 128 + col, ov);
+          tmem_ld_wait();
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            if (r[hf] >= rows) continue;
+            const size_t at = stream_whole ? ((((size_t)p.i * c.S + s[hf]) * c.H + (size_t)kvh * c.g + (row_base + r[hf] - s[hf] * c.g)) * kD)
+                                           : ((size_t)slot * c.rows_rb + r[hf]) * kD;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const int d = col + 8 * i + 2 * (lane & 3);
+              // a row that nobody fills is zero whatever the accumulator held
+              const float x0 = f[hf] == 0.f ? 0.f : __uint_as_float(ov[4 * i + 2 * hf]) * f[hf], x1 = f[hf] == 0.f ? 0.f : __uint_as_float(ov[4 * i + 2 * hf + 1]) * f[hf];
+              if (!stream_whole) *reinterpret_cast<float2*>(c.part_o + at + d) = make_float2(x0, x1);
+              else if (c.out_bf16) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(c.out) + at + d) = pack_bf16x2(x0, x1);
+              else *reinterpret_cast<float2*>(reinterpret_cast<float*>(c.out) + at + d) = make_float2(x0, x1);
+            }
+          }
+        }
+      }
+      if (warp == 0 && lane == 0) {   // of piece n + 4; who writes it next has come through q_full of piece n + 1
+        bars->bad_nodes[n & 3] = 0;
+        bars->bad_all[n & 3] = 0;
+      }
+      tc_fence_before();
+      __syncwarp();
+    }
+  } else if constexpr (kI8) {
+    // =============================== converters ===============================
+    const int ct = threadIdx.x - 32 * kWarpConv, ch = ct & 7, r0 = ct >> 3;
+    int tt = 0, n = 0;
+    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+      const TreeSeq sq = streams.seq(p.i);
+      const int end = sq.len0 + sq.nodes;
+      float limit = 0.f, down = 1.f;   // values' scales below `limit` fit behind `down`
+      for (int t = p.tb; t < p.te; t++, tt++) {
+        const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024);
+#pragma unroll 1
+        for (int kv = 0; kv < 2; kv++) {
+          const int h = 2 * tt + kv, raw = h % PL::kRaw, st = h % PL::kSlots, use = h / PL::kSlots;
+          wait_bar(&bars->raw_full[raw], (h / PL::kRaw) & 1, bars, c.status);
+          if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
+          if (kv == 0) {
+            // what the softmax needs of the tile: the keys' scales, and the unit of the values
+            bars->k_scale[tt & 3][ct] = scales[(ct >> 6) * 128 + (ct & 63)];
+            // the largest scale of the tile's values: NaN drop out, and rows past the drafted ones, whatever they hold
+            const float4 v = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 128 + 64 + (lane & 15) * 4);
+            const int there = end - t * kTile - 4 * lane;
+            const float top = warp_max(fmaxf(fmaxf(there > 0 ? v.x : 0.f, there > 1 ? v.y : 0.f), fmaxf(there > 2 ? v.z : 0.f, there > 3 ? v.w : 0.f)));
+            if (top >= limit) {
+              const int e = max((int)(__float_as_uint(top) >> 23), 8);             // 2^(e - 127) <= top < 2^(e - 126)
+              limit = __uint_as_float((uint32_t)min(e + 1, 254) << 23);
+              down = __uint_as_float((uint32_t)(261 - e) << 23);                   // 2^(7 - (e - 127)): scales come below 2^8, values below 2^15
+            }
+            if (ct == 0) bars->v_unit[tt & 3] = 1.f / down;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->info[tt & 3]);
+          }
+          const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot;
+          uint8_t* dst = smem + PL::kRing + st * kSlot + (ch >> 2) * kHalf;
+          const int c0 = 2 * (ch & 3) + (ch >> 2);   // threads of the two halves store opposite chunks of a row at a time: no bank conflicts
+#pragma unroll 4
+          for (int i = 0; i < 8; i++) {
+            const int r = 16 * i + r0;
+            const uint4 w = *reinterpret_cast<const uint4*>(src + swz128(r, ch));
+            uint32_t x[8];
+            int8x4_to_f16(w.x, x[0], x[1]);
+            int8x4_to_f16(w.y, x[2], x[3]);
+            int8x4_to_f16(w.z, x[4], x[5]);
+            int8x4_to_f16(w.w, x[6], x[7]);
+            if (kv) {
+              float s = t * kTile + r < end ? scales[(r >> 6) * 128 + 64 + (r & 63)] : 0.f;
+              if (!(s == s)) {   // the row held an infinity or a NaN
+                const int node = t * kTile + r - sq.len0;
+                if (ch == 0 && node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
+                else if (ch == 0 && node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
+                s = 0.f;
+              }
+              const __half2 s2 = __float2half2_rn(s * down);
+#pragma unroll
+              for (int j = 0; j < 8; j++) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), s2);
+                x[j] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            const uint4 lo = make_uint4(x[0], x[1], x[2], x[3]), hi = make_uint4(x[4], x[5], x[6], x[7]);
+            *reinterpret_cast<uint4*>(dst + swz128(r, c0)) = c0 & 1 ? hi : lo;
+            *reinterpret_cast<uint4*>(dst + swz128(r, c0 ^ 1)) = c0 & 1 ? lo : hi;
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars->full[st]);
+            mbar_arrive(&bars->raw_empty[raw]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0) stamp_end(c.time);
+  if (warp == 0) tmem_dealloc<1>(tmem, kTmemCols);
+}
+
+// Joins the partials of the streams that more than one range has a part of: block x is the range behind a stream's first part, a warp a row.
+template <int N>
+__global__ void __launch_bounds__(256) merge_tree_kernel(const __grid_constant__ TreeParams<N> prm) {
+  chain_release();
+  chain_wait();   // every block: the launch behind this one takes it that the one before is complete
+  const TreeCommon& c = prm.c;
+  const Streams<N> streams(prm, blockIdx.x + 1);
+  const int u = streams.u_begin, lane = threadIdx.x & 31;
+  const Piece p = streams.at(u);
+  const int w0 = streams.worker_of(p.us), np = streams.worker_of(p.us + p.tiles - 1) - w0 + 1;
+  if (p.tb <= 0 || p.tb >= p.tiles || w0 != (int)blockIdx.x) return;   // no stream goes on here, or its first part is further back
+  const int rows = min(c.rows_rb, c.R - (p.st % c.n_rb) * c.rows_rb), r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int first = streams.range_begin(w0) == p.us ? 0 : 1;
+  auto row_of = [&](int j) -> size_t { return (size_t)(2 * (w0 + j) + (j ? 0 : first)) * c.rows_rb + r; };
+  float M = -INFINITY;
+  for (int j = lane; j < np; j += 32) M = fmaxf(M, load_chained(reinterpret_cast<const float2*>(c.part_ml) + row_of(j)).x);
+  M = warp_max(M);
+  float L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = 0; j0 < np; j0 += 4) {
+    float2 ml[4];
+    float4 x[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+      if (j0 + q < np) {
+        ml[q] = load_chained(reinterpret_cast<const float2*>(c.part_ml) + row_of(j0 + q));
+        x[q] = load_chained(reinterpret_cast<const float4*>(c.part_o + row_of(j0 + q) * kD) + lane);
+      }
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+      if (j0 + q < np && ml[q].x != -INFINITY) {
+        const float w = ex2_approx(ml[q].x - M);
+        L = fmaf(ml[q].y, w, L);
+        o.x = fmaf(x[q].x, w, o.x);
+        o.y = fmaf(x[q].y, w, o.y);
+        o.z = fmaf(x[q].z, w, o.z);
+        o.w = fmaf(x[q].w, w, o.w);
+      }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int row = (p.st % c.n_rb) * c.rows_rb + r, s = row / c.g;
+  const size_t at = (((size_t)p.i * c.S + s) * c.H + (size_t)(p.st / c.n_rb) * c.g + (row - s * c.g)) * kD + 4 * lane;
+  if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+template <bool kI8, int kNB, int N>
+int32_t launch(Pool* p, const TreeParams<N>& prm, int workers) {
+  using PL = Plan<kI8, kNB>;
+  const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
+  if (int32_t rc = allow_smem(p->dev, tree_sm100_kernel<kI8, kNB, N>, PL::kTotal)) return rc;
+  RELUX_CUDA_TRY(launch_chained(chained, tree_sm100_kernel<kI8, kNB, N>, dim3(workers), dim3(PL::kThreads), (size_t)PL::kTotal, p->dev->stream, p->tmap_gqa, prm));
+  count_launch(p->dev);
+  if (workers > 1) {
+    RELUX_CUDA_TRY(launch_chained(chained, merge_tree_kernel<N>, dim3(workers - 1, (prm.c.rows_rb + 7) / 8), dim3(256), 0, p->dev->stream, prm));
+    count_launch(p->dev);
+  }
+  return RELUX_OK;
+}
+template <int N>
+int32_t launch_n(Pool* p, const TreeCommon& c, const TreeSeq* seqs, const int8_t* parents, int workers) {
+  TreeParams<N> prm;
+  prm.c = c;
+  if (!c.seqs) {
+    memcpy(prm.seqs, seqs, sizeof(TreeSeq) * ((size_t)c.n_seqs + 1));
+    memcpy(prm.parents, parents, (size_t)kTreeNodes * (c.one_tree ? 1 : c.n_seqs));
+  }
+  if (c.rows_rb <= 128) return p->int8 ? launch<true, 1, N>(p, prm, workers) : launch<false, 1, N>(p, prm, workers);
+  return p->int8 ? launch<true, 2, N>(p, prm, workers) : launch<false, 2, N>(p, prm, workers);
+}
+
+}  // namespace
+
+// q: device [n][S][H][128] token-major (f32 or bf16).  out: device, same shape, f32 or bf16.  The drafted rows are in the cache; nodes: host, of every sequence.
+int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16, const GqaTree& tree,
+                              const int32_t* nodes) {
+  const relux_pool_params& prm = p->prm;
+  const int n = sb.n_seqs, Hkv = prm.gqa_num_kv_heads, g = a.num_heads / Hkv, R = g * a.q_tokens;
+  TreeCommon c{};
+  c.n_rb = (R + 255) / 256;
+  c.rows_rb = ((R + c.n_rb - 1) / c.n_rb + 15) / 16 * 16;
+  TreeSeq inl[kInlineLarge + 1];
+  TreeSeq* seqs = inl;
+  int slot_index = 0;
+  if (n > kInlineLarge) {
+    int32_t* slot = nullptr;
+    if (int32_t rc = stage_acquire(p, &slot, &slot_index)) return rc;
+    seqs = (TreeSeq*)slot;
+  }
+  int64_t units64 = 0;
+  for (int i = 0; i < n; i++) {
+    const int s = sb.seq[i], len = p->h_len[(size_t)a.layer * prm.max_seqs + s];
+    seqs[i] = TreeSeq{s, len, nodes[i], (int32_t)units64};
+    units64 += std::max(1, (len + nodes[i] + kTile - 1) / kTile) + kFixUnits;
+  }
+  seqs[n] = TreeSeq{0, 0, 0, (int32_t)units64};
+  units64 *= Hkv * c.n_rb;
+  if (units64 >= ((int64_t)1 << 31)) { set_error("more cached pages than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
+  const int units = (int)units64;
+  const int workers = std::max(1, std::min(p->dev->sm_count, units / (kFixUnits + 1)));
+  const size_t part_rows = (size_t)2 * workers * c.rows_rb;
+  int32_t rc = grow(p->dev, p->part_o, part_rows * (kD + 2) * sizeof(float));
+  if (rc) return rc;
+  if (seqs != inl) {
+    size_t bytes = sizeof(TreeSeq) * ((size_t)n + 1);
+    const size_t tree_bytes = (size_t)kTreeNodes * (tree.one ? 1 : n);
+    memcpy((char*)seqs + bytes, tree.parents, tree_bytes);
+    bytes += tree_bytes;
+    if ((rc = grow(p->dev, p->seq_list, bytes))) return rc;
+    RELUX_CUDA_TRY(cudaMemcpyAsync(p->seq_list.p, seqs, bytes, cudaMemcpyHostToDevice, p->dev->stream));
+    if ((rc = stage_release(p, slot_index))) return rc;
+    c.seqs = (const TreeSeq*)p->seq_list.p;
+    c.parents = (const int8_t*)(c.seqs + n + 1);
+  }
+  c.one_tree = tree.one;
+  c.table = p->d_table;
+  c.table_stride = prm.max_pages_per_seq;
+  c.num_pages = prm.num_pages;
+  c.n_seqs = n;
+  c.range = units / workers;
+  c.range_more = units % workers;
+  c.Hkv = Hkv;
+  c.H = a.num_heads;
+  c.g = g;
+  c.S = a.q_tokens;
+  c.R = R;
+  const int64_t rows_per_block = (int64_t)prm.num_pages * Hkv * kPage;
+  c.krow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block);
+  c.vrow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block + rows_per_block);
+  if (p->int8) c.scales = p->scales_at(a.layer);
+  c.scale_log2 = a.scale * 1.4426950408889634f;
+  c.q = d_q;
+  c.q_bf16 = a.q_dtype == RELUX_DTYPE_BF16;
+  c.out_bf16 = out_bf16;
+  c.out = d_out;
+  c.part_o = (float*)p->part_o.p;
+  c.part_ml = c.part_o + part_rows * kD;
+  c.status = p->d_status;
+  c.time = time_stamp_next(p, p->attn_times);
+  rc = n <= kInlineSmall || c.seqs ? launch_n<kInlineSmall>(p, c, seqs, tree.parents, workers) : launch_n<kInlineLarge>(p, c, seqs, tree.parents, workers);
+  if (rc) return rc;
+  time_stamp_done(p->attn_times, c.time);
+  return RELUX_OK;
+}
+
+}  // namespace relux

@@ -1441,7 +1441,11 @@ static int32_t do_gqa_tree(Pool* p, const relux_attn_args* attn, const relux_app
     }
   const void *da = nullptr, *db = nullptr;
   int slot_a = -1, slot_b = -1;
-  if (sb.total_rows > 0 && (rc = stage_step_rows(p, sb, kv, attn, &da, &db, &slot_a, &slot_b))) return rc;
+  if (g * S > 32) {   // the tensor-core kernel finds the rows in the cache
+    relux_append_args rows = *kv;
+    rows.n_new = sb.rows.data();
+    if ((rc = do_append(p, &rows, RELUX_POOL_GQA))) return rc;
+  } else if (sb.total_rows > 0 && (rc = stage_step_rows(p, sb, kv, attn, &da, &db, &slot_a, &slot_b))) return rc;
   const GqaAppend app{da, db, kv->dtype, kv->layout, 0, sb.rows.data()};
   const GqaTree tree{parents.data(), t->n_trees == 1};
   if ((rc = do_attention(p, attn, RELUX_POOL_GQA, nullptr, &app, &tree))) return rc;

@@ -50,7 +50,10 @@ def attend(K, V, q, n, see, scale, q_rounding=0.0):
     """K, V [n + m, Hkv, D] as held, q [S, H, D], see [S][m]: query i sees the first n rows and, of the others, see[i].  Returns (out, bound) [S, H, D] in
     64 bits.  bound: how far the kernels may be off, per element.  They round P (or P times a row's scale) to bf16, 2^-8 of it; scores are sums of
     128 products of exact operands in float32, 2^-16 of the sum of magnitudes is eight times what their roundings add up to, and q_rounding of that sum where
-    queries are rounded; an error d of a score is exp(d) of its P, above and below the line.  The rest (sums of P, exponentials, merges) is 2^-14."""
+    queries are rounded; an error d of a score is exp(d) of its P, above and below the line.  The rest (sums of P, exponentials, merges) is 2^-14.
+    Over the 8-bit cache P, or the values, are binary16, whose steps do not shrink below 2^-24: P reaches 2^7 and more there, so each is off by up to 2^-25 of
+    2^7 of a row's largest even where that is more than 2^-8 of it (seen where the likeliest row's code is 0 in a dim), and values come to 2^7 of the largest
+    scale's, so theirs is 2^-25 / 2^7 of that scale, less than 2^-32 of the largest value."""
     S, H, _ = q.shape
     Hkv = K.shape[1]
     g = H // Hkv
@@ -67,7 +70,7 @@ def attend(K, V, q, n, see, scale, q_rounding=0.0):
             p = np.exp(s - s.max(-1, keepdims=True))
             p /= p.sum(-1, keepdims=True)
             out[i, h * g:(h + 1) * g] = p @ v
-            bound[i, h * g:(h + 1) * g] = (p @ np.abs(v)) * (2.0 ** -8 + 2 * np.expm1(err) + 2.0 ** -14)
+            bound[i, h * g:(h + 1) * g] = (p @ np.abs(v)) * (2.0 ** -8 + 2 * np.expm1(err) + 2.0 ** -14) + 2.0 ** -32 * (np.abs(v).sum(0) + np.abs(v).max())
     return out, bound
 
 

@@ -14,8 +14,11 @@
 // four consecutive K indices of one column, and the order of the indices is the reader's own as long as A has the same.
 //   K: thread (n, c) = (lane / 4, lane % 4) takes bytes 32 c .. 32 c + 31 of token n of a block of eight; K slice ks is its word ks.
 //   V: thread (n, c) takes bytes 16 n .. 16 n + 15 of tokens 2c, 2c + 1, 2c + 8, 2c + 9; output block j's column n is dim 16 n + j.
-// Codes become binary16 for the scores (two instructions for two codes; queries are brought to binary16 with a power of two per row, which keeps
-// 11 bits of a float32 query where bf16 keeps 8), and bfloat16 for the values: P carries s^v, whose range binary16 does not have.
+// A code is stored as c + 128: below the exponent of 1024 that is a binary16 number, and one subtraction (two instructions for two codes) makes it c, which
+// binary16 holds exactly.  Queries are brought to binary16 with a power of two per row, which keeps 11 bits of a float32 query where bf16 keeps 8.  P carries
+// s^v over a power of two that grows with the largest s^v seen so far (O is then rescaled as for a new maximum): 11 bits of it, 2^29 between the
+// largest row and one that loses bits.  (P s^v in bf16, whose range needs no unit, was off by 2.5e-3 of the result where this is 1.7e-3, the rounding of a
+// bf16 output alone, and takes four instructions for two codes.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -29,6 +32,7 @@ namespace relux {
 constexpr int kInt8StageBytes = 2 * kGqaPageTok * kGqaD;                      // K codes, V codes
 constexpr int kInt8ScaleBytes = 2 * kGqaPageTok * (int)sizeof(float);         // K scales, V scales
 constexpr float kInt8Tiny = 1e-36f;
+constexpr uint32_t kInt8Zeros = 0x80808080u;   // four codes of 0
 
 // Untiled bulk copy global -> shared (multiples of 16 bytes), completion on an mbarrier of this CTA.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -61,7 +65,7 @@ struct Int8Row {
   float scale;
 };
 __device__ __forceinline__ Int8Row int8_quantise(const float (&x)[8], uint32_t top) {
-  Int8Row r{{0u, 0u}, 0.f};
+  Int8Row r{{kInt8Zeros, kInt8Zeros}, 0.f};
   const float a = __uint_as_float(top);
   if (top >= 0x7F800000u) {
     r.scale = __uint_as_float(0x7FC00000u);
@@ -75,7 +79,7 @@ __device__ __forceinline__ Int8Row int8_quantise(const float (&x)[8], uint32_t t
       for (int i = 0; i < 4; i++) c[i] = __float2int_rn(__fmul_rn(x[4 * h + i], inv));
       w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
-    r.codes = make_uint2(w[0], w[1]);
+    r.codes = make_uint2(w[0] ^ kInt8Zeros, w[1] ^ kInt8Zeros);
     r.scale = __fdiv_rn(a, 127.f);
   }
   return r;
@@ -88,21 +92,30 @@ __device__ __forceinline__ Int8Row int8_row(const T* src) {
 }
 
 // ---- codes -> matrix operands ----
-// Four codes -> two pairs of binary16: 1024 + (c + 128) is the byte below the exponent of 1024; 1152 is taken off again.
-__device__ __forceinline__ void int8x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  w ^= 0x80808080u;
-  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-  const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
-  lo = *reinterpret_cast<const uint32_t*>(&x);
-  hi = *reinterpret_cast<const uint32_t*>(&y);
-}
-// Two codes in the even bytes under 0x43 -> bfloat16: 128 + the code's low seven bits, less 128, or 256 where its sign bit is set.
-__device__ __forceinline__ uint32_t int8x2_to_bf16(uint32_t t) {
-  const uint32_t a = t & 0xFF7FFF7Fu, s = t & 0xFF80FF80u;
-  const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&s));
+// Two bytes under 0x64, binary16 1024 + (c + 128) -> c.
+__device__ __forceinline__ uint32_t int8x2_to_f16(uint32_t t) {
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&t), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
+// Four codes -> two pairs of binary16.
+__device__ __forceinline__ void int8x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  lo = int8x2_to_f16(__byte_perm(w, 0x64646464u, 0x4140));
+  hi = int8x2_to_f16(__byte_perm(w, 0x64646464u, 0x4342));
+}
+__device__ __forceinline__ uint32_t round_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The unit of the values' scales: those below `limit` come below 2^kUp times `down`.  For the largest scale of new rows that reaches the limit.
+struct ValueUnit {
+  float limit = 0.f, down = 1.f;
+  template <int kUp>
+  __device__ __forceinline__ void grow(float top) {
+    const int e = max((int)(__float_as_uint(top) >> 23), kUp + 1);                // 2^(e - 127) <= top < 2^(e - 126)
+    limit = __uint_as_float((uint32_t)min(e + 1, 254) << 23);
+    down = __uint_as_float((uint32_t)(min(253 + kUp - e, 253)) << 23);            // 2^(kUp - 1 - (e - 127))
+  }
+};
 
 // ---- queries ----
 // The power of two that brings a row's largest value, of bits `top`, to [2^14, 2^15), and its inverse.  (Not rows of zeros or of subnormal numbers.)
@@ -160,7 +173,7 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
 
 // gqa_consume_page for a page of codes.
 template <bool kTree>
-__device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_t (&qa)[8][4], const float (&q_scale)[2], const uint8_t* page,
+__device__ __forceinline__ void int8_consume_page(GqaState<1>& st, ValueUnit& unit, const uint32_t (&qa)[8][4], const float (&q_scale)[2], const uint8_t* page,
                                                   const float* scales, int tb, int tok0, int T, int S, int g, int causal, int lane, int row0,
                                                   const TreeRows& tree) {
   const int n = lane >> 2, c = lane & 3;
@@ -194,6 +207,17 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_
 #pragma unroll
     for (int e = 0; e < 4; e++) sacc[nt][e] = (sacc[nt][e] + sodd[nt][e]) * (e & 1 ? sk.y : sk.x);
   }
+  // rows that nobody sees yet, or ever, have a part in the unit too if they are the sequence's; what lies behind T may hold anything
+  const int there = T - tok0 - 2 * c;
+  float top = fmaxf(fmaxf(there > 0 ? sv[0][0] : 0.f, there > 1 ? sv[0][1] : 0.f), fmaxf(there > 8 ? sv[1][0] : 0.f, there > 9 ? sv[1][1] : 0.f));   // NaN drop out
+  float shrink = 1.f;
+  if (__any_sync(0xffffffffu, top >= unit.limit)) {
+    top = warp_max(top);
+    const float before = unit.down;
+    const bool first = unit.limit == 0.f;
+    unit.grow<15>(top);
+    if (!first) shrink = unit.down / before;
+  }
   uint32_t hidden = 0;   // bit 4 hf + 2 nt + e
   const bool need_mask = tok0 + 16 > (kTree ? tree.len0 : T - (causal ? S : 0));
   if (need_mask) {
@@ -222,13 +246,14 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_
     mx[hf] = x * q_scale[hf];
     grow |= mx[hf] > st.m[0][hf];
   }
-  if (__any_sync(0xffffffffu, grow)) {
+  if (__any_sync(0xffffffffu, grow || shrink != 1.f)) {
 #pragma unroll
     for (int hf = 0; hf < 2; hf++) {
       const float m_new = fmaxf(st.m[0][hf], mx[hf]);
-      const float alpha = (m_new == -INFINITY) ? 0.f : gqa_ex2(st.m[0][hf] - m_new);
+      float alpha = (m_new == -INFINITY) ? 0.f : gqa_ex2(st.m[0][hf] - m_new);
       st.m[0][hf] = m_new;
       st.l[0][hf] *= alpha;
+      alpha *= shrink;
 #pragma unroll
       for (int j = 0; j < 16; j++) {
         st.o[0][j][hf * 2] *= alpha;
@@ -236,7 +261,7 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_
       }
     }
   }
-  // P times the values' scales, rounded to bf16 (2^-8 of each at most, as the bf16 cache's P)
+  // P times the values' scales over their unit, rounded to binary16: 2^-11 of each, or 2^-25 of 2^14 and more that the largest come to
   uint32_t pa[4];
 #pragma unroll
   for (int hf = 0; hf < 2; hf++) {
@@ -247,13 +272,13 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_
       float p0 = gqa_ex2(fmaf(sacc[nt][hf * 2], q_scale[hf], neg_m));
       float p1 = gqa_ex2(fmaf(sacc[nt][hf * 2 + 1], q_scale[hf], neg_m));
       ps += p0 + p1;
-      p0 *= sv[nt][0];
-      p1 *= sv[nt][1];
+      p0 *= sv[nt][0] * unit.down;
+      p1 *= sv[nt][1] * unit.down;
       if (need_mask) {   // the scale of a hidden row may be NaN
         if (hidden >> (4 * hf + 2 * nt) & 1u) p0 = 0.f;
         if (hidden >> (4 * hf + 2 * nt + 1) & 1u) p1 = 0.f;
       }
-      pa[nt * 2 + hf] = round_bf16x2(p0, p1);
+      pa[nt * 2 + hf] = round_f16x2(p0, p1);
     }
     st.l[0][hf] += ps;
   }
@@ -267,14 +292,15 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, const uint32_
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const uint32_t sel = j & 1 ? 0x4342 : 0x4140;
-      mma_bf16_16816(st.o[0][4 * w + j], pa, int8x2_to_bf16(__byte_perm(j < 2 ? a01 : a23, 0x43434343u, sel)),
-                     int8x2_to_bf16(__byte_perm(j < 2 ? b01 : b23, 0x43434343u, sel)));
+      mma_f16_16816(st.o[0][4 * w + j], pa, int8x2_to_f16(__byte_perm(j < 2 ? a01 : a23, 0x64646464u, sel)),
+                    int8x2_to_f16(__byte_perm(j < 2 ? b01 : b23, 0x64646464u, sel)));
     }
   }
 }
 
 // gqa_store_state: output block j's column 2c + e is dim 16 (2c + e) + j.
-__device__ __forceinline__ void int8_store_state(const GqaState<1>& st, float* dst0, int rows, int lane, bool alive) {
+__device__ __forceinline__ void int8_store_state(const GqaState<1>& st, const ValueUnit& unit, float* dst0, int rows, int lane, bool alive) {
+  const float up = 1.f / unit.down;
 #pragma unroll
   for (int hf = 0; hf < 2; hf++) {
     float l = st.l[0][hf];
@@ -288,7 +314,7 @@ __device__ __forceinline__ void int8_store_state(const GqaState<1>& st, float* d
 #pragma unroll
       for (int j = 0; j < 16; j += 4)
         *reinterpret_cast<float4*>(dst + 16 * (2 * (lane & 3) + e) + j) =
-            make_float4(st.o[0][j][hf * 2 + e], st.o[0][j + 1][hf * 2 + e], st.o[0][j + 2][hf * 2 + e], st.o[0][j + 3][hf * 2 + e]);
+            make_float4(st.o[0][j][hf * 2 + e] * up, st.o[0][j + 1][hf * 2 + e] * up, st.o[0][j + 2][hf * 2 + e] * up, st.o[0][j + 3][hf * 2 + e] * up);
     if ((lane & 3) == 0) {
       dst[kGqaD] = alive ? st.m[0][hf] : -INFINITY;
       dst[kGqaD + 1] = alive ? l : 0.f;

@@ -68,7 +68,7 @@ __device__ __forceinline__ void put8(void* to, size_t off, const Row8& r) {
     if constexpr (kI8) {
       const uint32_t w[2] = {r.w.x, r.w.y};
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * r.s;
+      for (int i = 0; i < 8; i++) x[i] = (float)((int)(w[i >> 2] >> (8 * (i & 3)) & 255u) - 128) * r.s;
     } else {
       const uint32_t w[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
 #pragma unroll

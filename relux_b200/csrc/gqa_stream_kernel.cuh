@@ -384,13 +384,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (kTr) tree = TreeRows{{row_tree(qs + (lane >> 2) * kGqaQStride), row_tree(qs + ((lane >> 2) + 8) * kGqaQStride)}, sq.len0};
       GqaState<1> state;
       state.clear();
+      ValueUnit unit;
       for (int page = p.pb; page < p.pe; page++, g++) {
         if (MT == 1 && (g & 1) != grp) continue;
         const int st = g % kStages;
         if (alive) alive = timed_wait(&full[st], (g / kStages) & 1);
         if (alive) {
           if constexpr (kI8)
-            int8_consume_page<kTr>(state, qa[0], q_scale, smem + st * kStageBytes, reinterpret_cast<const float*>(smem + SM::kScales + st * kInt8ScaleBytes),
+            int8_consume_page<kTr>(state, unit, qa[0], q_scale, smem + st * kStageBytes, reinterpret_cast<const float*>(smem + SM::kScales + st * kInt8ScaleBytes),
                                    tb, page * kGqaPageTok + tb, T, c.S, c.g, c.causal, lane, row0, tree);
           else
             gqa_consume_page<1, kTr>(state, qa, smem_u32(smem + st * kGqaStageBytes), tb, page * kGqaPageTok + tb, T, c.S, c.g, c.causal,
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int sb = n % kStateBufs;
       if (n >= kStateBufs && alive) alive = timed_wait(&state_empty[sb], (n / kStateBufs - 1) & 1);
       float* dst = mb + sb * SM::kStateFloats + (size_t)warp * RS * kGqaStateStride;
-      if constexpr (kI8) int8_store_state(state, dst, RS, lane, alive);
+      if constexpr (kI8) int8_store_state(state, unit, dst, RS, lane, alive);
       else gqa_store_state<1>(state, dst, RS, lane, alive);
       __syncwarp();
       if (lane == 0) mbar_arrive(&state_full[sb]);

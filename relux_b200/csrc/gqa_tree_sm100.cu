@@ -139,10 +139,11 @@ struct Bars {
   uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
   uint32_t bad_all[4];         // (8-bit cache) a cached row with one
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
-  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys; without it there is no room for this
+  uint32_t v_scale[2][kTile];  // (8-bit cache) of a tile's values, over their unit, binary16 twice
+  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys.  Without an 8-bit cache there is no room for these two
 };
-constexpr int kBarBytes = 3072;
-static_assert(sizeof(Bars) <= kBarBytes && kBarBytes - sizeof(Bars::k_scale) >= offsetof(Bars, k_scale), "barrier block too large");
+constexpr int kBarBytes = 4096;
+static_assert(sizeof(Bars) <= kBarBytes && kBarBytes - kTile * 24 >= offsetof(Bars, v_scale), "barrier block too large");
 
 template <bool kI8, int kNB>
 struct Plan {
@@ -154,7 +155,7 @@ struct Plan {
   static constexpr int kRawAt = kRing + kSlots * kSlot;
   static constexpr int kScaleAt = kRawAt + kRaw * kRawSlot;
   static constexpr int kBars = kScaleAt + kScaleSlots * 1024;
-  static constexpr int kTotal = 1024 + kBars + (kI8 ? kBarBytes : kBarBytes - kTile * 16);
+  static constexpr int kTotal = 1024 + kBars + (kI8 ? kBarBytes : kBarBytes - kTile * 24);
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
   static constexpr int kThreads = 32 * (kI8 ? kWarpConv + kConvWarps : kWarpConv);
 };
@@ -640,66 +641,75 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     }
   } else if constexpr (kI8) {
     // =============================== converters ===============================
-    const int ct = threadIdx.x - 32 * kWarpConv, ch = ct & 7, r0 = ct >> 3;
+    // 16 threads a row, eight codes each: eight rows at a time, the same place of the swizzle in all of them, so that every address is a constant away.
+    const int ct = threadIdx.x - 32 * kWarpConv, hc = ct & 15, r0 = ct >> 4;
+    const uint32_t src0 = swz128(r0, hc >> 1) + (hc & 1) * 8, dst0 = (hc >> 3) * kHalf + swz128(r0, hc & 7);
     int tt = 0, n = 0;
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
       const TreeSeq sq = streams.seq(p.i);
       const int end = sq.len0 + sq.nodes;
-      float limit = 0.f, down = 1.f;   // values' scales below `limit` fit behind `down`
+      ValueUnit unit;
       for (int t = p.tb; t < p.te; t++, tt++) {
-        const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024);
 #pragma unroll 1
         for (int kv = 0; kv < 2; kv++) {
           const int h = 2 * tt + kv, raw = h % PL::kRaw, st = h % PL::kSlots, use = h / PL::kSlots;
           wait_bar(&bars->raw_full[raw], (h / PL::kRaw) & 1, bars, c.status);
           if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
           if (kv == 0) {
-            // what the softmax needs of the tile: the keys' scales, and the unit of the values
+            // what the softmax needs of the tile, the keys' scales and the unit of the values; and the values' scales over it, a row a thread
+            const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024);
             bars->k_scale[tt & 3][ct] = scales[(ct >> 6) * 128 + (ct & 63)];
             // the largest scale of the tile's values: NaN drop out, and rows past the drafted ones, whatever they hold
             const float4 v = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 128 + 64 + (lane & 15) * 4);
             const int there = end - t * kTile - 4 * lane;
-            const float top = warp_max(fmaxf(fmaxf(there > 0 ? v.x : 0.f, there > 1 ? v.y : 0.f), fmaxf(there > 2 ? v.z : 0.f, there > 3 ? v.w : 0.f)));
-            if (top >= limit) {
-              const int e = max((int)(__float_as_uint(top) >> 23), 8);             // 2^(e - 127) <= top < 2^(e - 126)
-              limit = __uint_as_float((uint32_t)min(e + 1, 254) << 23);
-              down = __uint_as_float((uint32_t)(261 - e) << 23);                   // 2^(7 - (e - 127)): scales come below 2^8, values below 2^15
+            const float top = fmaxf(fmaxf(there > 0 ? v.x : 0.f, there > 1 ? v.y : 0.f), fmaxf(there > 2 ? v.z : 0.f, there > 3 ? v.w : 0.f));
+            if (__any_sync(0xffffffffu, top >= unit.limit)) unit.grow<8>(warp_max(top));   // codes come below 2^15
+            if (ct == 0) bars->v_unit[tt & 3] = 1.f / unit.down;
+            const int pos = t * kTile + ct;
+            float s = pos < end ? scales[(ct >> 6) * 128 + 64 + (ct & 63)] : 0.f;
+            if (!(s == s)) {   // the row held an infinity or a NaN
+              const int node = pos - sq.len0;
+              if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
+              else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
+              s = 0.f;
             }
-            if (ct == 0) bars->v_unit[tt & 3] = 1.f / down;
+            bars->v_scale[tt & 1][ct] = round_f16x2(s * unit.down, s * unit.down);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->info[tt & 3]);
+          } else {
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");   // every row's scale is there
           }
-          const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot;
-          uint8_t* dst = smem + PL::kRing + st * kSlot + (ch >> 2) * kHalf;
-          const int c0 = 2 * (ch & 3) + (ch >> 2);   // threads of the two halves store opposite chunks of a row at a time: no bank conflicts
-#pragma unroll 4
-          for (int i = 0; i < 8; i++) {
-            const int r = 16 * i + r0;
-            const uint4 w = *reinterpret_cast<const uint4*>(src + swz128(r, ch));
-            uint32_t x[8];
-            int8x4_to_f16(w.x, x[0], x[1]);
-            int8x4_to_f16(w.y, x[2], x[3]);
-            int8x4_to_f16(w.z, x[4], x[5]);
-            int8x4_to_f16(w.w, x[6], x[7]);
-            if (kv) {
-              float s = t * kTile + r < end ? scales[(r >> 6) * 128 + 64 + (r & 63)] : 0.f;
-              if (!(s == s)) {   // the row held an infinity or a NaN
-                const int node = t * kTile + r - sq.len0;
-                if (ch == 0 && node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
-                else if (ch == 0 && node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
-                s = 0.f;
-              }
-              const __half2 s2 = __float2half2_rn(s * down);
+          const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot + src0;
+          uint8_t* dst = smem + PL::kRing + st * kSlot + dst0;
+          const uint32_t* v_scale = &bars->v_scale[tt & 1][r0];
+          auto convert = [&](auto values) {
 #pragma unroll
-              for (int j = 0; j < 8; j++) {
-                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), s2);
-                x[j] = *reinterpret_cast<const uint32_t*>(&y);
+            for (int i0 = 0; i0 < 16; i0 += 8) {
+              uint2 w[8];
+              uint32_t s[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                w[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * 1024);
+                if constexpr (decltype(values)::value) s[i] = v_scale[8 * (i0 + i)];
+              }
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                uint32_t x[4];
+                int8x4_to_f16(w[i].x, x[0], x[1]);
+                int8x4_to_f16(w[i].y, x[2], x[3]);
+                if constexpr (decltype(values)::value) {
+#pragma unroll
+                  for (int j = 0; j < 4; j++) {
+                    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), *reinterpret_cast<const __half2*>(&s[i]));
+                    x[j] = *reinterpret_cast<const uint32_t*>(&y);
+                  }
+                }
+                *reinterpret_cast<uint4*>(dst + (i0 + i) * 1024) = make_uint4(x[0], x[1], x[2], x[3]);
               }
             }
-            const uint4 lo = make_uint4(x[0], x[1], x[2], x[3]), hi = make_uint4(x[4], x[5], x[6], x[7]);
-            *reinterpret_cast<uint4*>(dst + swz128(r, c0)) = c0 & 1 ? hi : lo;
-            *reinterpret_cast<uint4*>(dst + swz128(r, c0 ^ 1)) = c0 & 1 ? lo : hi;
-          }
+          };
+          if (kv) convert(std::true_type{});
+          else convert(std::false_type{});
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {

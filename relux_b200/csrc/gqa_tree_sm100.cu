@@ -10,12 +10,14 @@
 // A piece that is a whole stream writes its output; others leave float32 partials that merge_tree_kernel joins.
 //
 // Roles of a CTA:
-//   producer   a tile's K and V by TMA, 32 KB each, into a ring; on the 8-bit cache 16 KB each and the scales into a ring of their own
-//   converters (8-bit cache, four warps) codes -> binary16 operands in the ring's swizzled layout.  K as whole numbers: a row's scale multiplies its column of
+//   producer   a tile's K and V by TMA, 32 KB each, into a ring; on the 8-bit cache page by page, 8 KB each, and the scales, into rings of their own
+//   converters (8-bit cache, four warps for K, four for V) codes -> binary16 operands in the ring's swizzled layout.  K as whole numbers: a row's scale multiplies its column of
 //              scores, in float32.  V times its scale over a power of two that all of the piece's rows share so far (11 bits, as P has then; 2^29 between
 //              the largest row and one that is no longer exact to 11 bits); where a row comes that is too large for it, the power grows and O is rescaled.
 //   MMA        step k = (tile, block): S = Q K^T (S buffer k & 1), O[block] += P V with P read from tensor memory over the scores it came from
-//   softmax    eight warps of 16 rows of a block each, four lanes to a row: scores from TMEM, running max (updated lazily), P back to TMEM
+//   softmax    eight warps of 16 rows of a block each, four lanes to a row: scores from TMEM, running max (updated lazily), P back to TMEM.  A tile takes a
+//              warp 2300 clocks, most of them latency.  Up to 64 rows, four warps take the even steps and four the odd ones, each with an O of its own,
+//              which meet at the piece's end.
 // Order of issue: QK(k + 1), PV(k): the tensor pipe executes in issue order, so QK(k + 2) finds its S buffer read.
 // A product with P = 0 does not hide an infinity or a NaN among the values: those of drafted rows and of what lies behind are set to zero in the tile, and
 // the rows that see one become NaN at the end.  (8-bit rows have them in their scale alone; a code is always a number.)
@@ -37,10 +39,9 @@ namespace {
 constexpr int kTile = 128, kD = kGqaD, kPage = kGqaPageTok;
 constexpr int kHalf = 16384;                   // [128 rows][64 16-bit columns], 128-byte swizzle
 constexpr int kSlot = 2 * kHalf;               // K or V of a tile, or 128 query rows
-constexpr int kRawSlot = kTile * kD;           // codes of K or V of a tile
+constexpr int kRawSlot = kPage * kD;           // codes of K or V of a page
 constexpr int kFixUnits = 2;                   // tiles: what a piece costs beyond its own (queries in, results out)
-constexpr int kSoftmaxWarps = 8, kConvWarps = 4;
-constexpr int kWarpLoad = kSoftmaxWarps, kWarpMma = kSoftmaxWarps + 1, kWarpConv = kSoftmaxWarps + 2;
+constexpr int kSoftmaxWarps = 8, kConvWarps = 4;   // of K, and of V
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
 constexpr float kRescaleThreshold = 8.0f;      // log2: P reaches 2^8 before the running max follows
 // (8-bit cache) log2: what P and its sum are larger by.  Binary16 has 11 bits down to 2^-14, and P reaches 2^(8 + 7): probabilities keep 11 bits down to 2^-21
@@ -133,33 +134,37 @@ struct Streams {
 };
 
 struct Bars {
-  uint64_t full[6], empty[6], raw_full[5], raw_empty[5], info[4], s_full[2], p_full[2], q_full, pv, fin, drain;
+  uint64_t full[6], empty[6], raw_full[6], raw_empty[6], scale_full[4], scale_empty[4], k_info[4], v_info[4], s_full[2], p_full[2], q_full, pv, fin, drain;
   uint32_t tmem_base;
   volatile int32_t abort_flag;
   uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
   uint32_t bad_all[4];         // (8-bit cache) a cached row with one
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
+  float4 halves[2][64];        // (two) a row's max, sum and unit of O, of either half of the warps
   uint32_t v_scale[2][kTile];  // (8-bit cache) of a tile's values, over their unit, binary16 twice
-  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys.  Without an 8-bit cache there is no room for these two
+  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys.  Without an 8-bit cache there is no room for these two, nor with two blocks for `halves`
 };
-constexpr int kBarBytes = 4096;
-static_assert(sizeof(Bars) <= kBarBytes && kBarBytes - kTile * 24 >= offsetof(Bars, v_scale), "barrier block too large");
 
 template <bool kI8, int kNB>
 struct Plan {
-  static constexpr int kSlots = kI8 ? 3 : kNB == 2 ? 5 : 6;       // of 32 KB
-  static constexpr int kRaw = kI8 ? (kNB == 2 ? 3 : 5) : 0;       // of 16 KB
+  static constexpr int kSlots = kI8 ? 4 : kNB == 2 ? 5 : 6;       // of 32 KB; an even number keeps K and V apart, as the converters need it
+  static constexpr int kRaw = kI8 ? (kNB == 2 ? 3 : 6) : 0;       // of 8 KB
   static constexpr int kScaleSlots = kI8 ? 4 : 0;                 // scales as they come, of a tile, 1 KB
   static constexpr int kQ = 0;
   static constexpr int kRing = kNB * kSlot;
   static constexpr int kRawAt = kRing + kSlots * kSlot;
   static constexpr int kScaleAt = kRawAt + kRaw * kRawSlot;
   static constexpr int kBars = kScaleAt + kScaleSlots * 1024;
-  static constexpr int kTotal = 1024 + kBars + (kI8 ? kBarBytes : kBarBytes - kTile * 24);
+  static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, halves));
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
-  static constexpr int kThreads = 32 * (kI8 ? kWarpConv + kConvWarps : kWarpConv);
+  static constexpr int kWarpLoad = kSoftmaxWarps + (kI8 ? 2 * kConvWarps : 0), kWarpMma = kWarpLoad + 1;
+  // Four more warps where registers are dealt out anew, which warps do by fours: softmax 152, converters 64, the others 48 of the 96 of the launch.
+  static constexpr int kThreads = 32 * (kI8 ? kWarpLoad + 4 : kWarpMma + 1);
+  static constexpr int kRegsSoftmax = 152, kRegsConv = 64, kRegsOther = 48;
+  static_assert(!kI8 || 256 * kRegsSoftmax + 256 * kRegsConv + 128 * kRegsOther <= 640 * 96, "more registers than the block is launched with");
 };
-__device__ __noinline__ void wait_slow(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
+// (Not a function of its own: a call takes registers that a role may have given back.)
+__device__ __forceinline__ void wait_slow(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
   for (uint32_t i = 0; i < kSpinLimit; i++) {
     if (mbar_try_wait(bar, parity)) return;
     if ((i & 255) == 255 && b->abort_flag) return;
@@ -170,6 +175,16 @@ __device__ __noinline__ void wait_slow(uint64_t* bar, uint32_t parity, Bars* b, 
 }
 __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
   if (!mbar_try_wait(bar, parity)) wait_slow(bar, parity, b, status);
+}
+
+// Registers from or to the block's pool, by all warps of a warpgroup.
+template <int kRegs, bool kOn>
+__device__ __forceinline__ void regs_up() {
+  if constexpr (kOn) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs, bool kOn>
+__device__ __forceinline__ void regs_down() {
+  if constexpr (kOn) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 // Instruction descriptor of binary16 operands: make_idesc_bf16 with formats 0.
@@ -210,27 +225,35 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     tree_sm100_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ TreeParams<N> prm) {
   using PL = Plan<kI8, kNB>;
   const TreeCommon& c = prm.c;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   Bars* bars = reinterpret_cast<Bars*>(smem + PL::kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool two = kNB == 1 && c.rows_rb <= 64;   // two halves of the softmax warps on steps in turn
+  if ((smem_u32(smem) & 1023u) != 0) {            // the swizzled layouts need it
+    chain_wait();
+    if (threadIdx.x == 0) set_status(c.status, RELUX_ERR_UNSUPPORTED);
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < 6; s++) {
       mbar_init(&bars->full[s], kI8 ? kConvWarps : 1);
       mbar_init(&bars->empty[s], 1);
     }
-    for (int s = 0; s < 5; s++) {
+    for (int s = 0; s < 6; s++) {
       mbar_init(&bars->raw_full[s], 1);
       mbar_init(&bars->raw_empty[s], kConvWarps);
     }
     for (int s = 0; s < 4; s++) {
-      mbar_init(&bars->info[s], kConvWarps);
+      mbar_init(&bars->scale_full[s], 1);
+      mbar_init(&bars->scale_empty[s], 2 * kConvWarps);
+      mbar_init(&bars->k_info[s], kConvWarps);
+      mbar_init(&bars->v_info[s], kConvWarps);
       bars->bad_nodes[s] = 0;
       bars->bad_all[s] = 0;
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s], kSoftmaxWarps);
+      mbar_init(&bars->p_full[s], two ? kSoftmaxWarps / 2 : kSoftmaxWarps);
     }
     mbar_init(&bars->q_full, kSoftmaxWarps);
     mbar_init(&bars->pv, 1);
@@ -255,7 +278,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   auto rows_of = [&](const Piece& p) -> int { return min(c.rows_rb, c.R - (p.st % c.n_rb) * c.rows_rb); };
   auto blocks_of = [&](const Piece& p) -> int { return kNB == 1 ? 1 : (rows_of(p) + 127) / 128; };
 
-  if (warp == kWarpLoad) {
+  if (warp == PL::kWarpLoad) {
+    regs_down<PL::kRegsOther, kI8>();
     // =============================== producer ===============================
     const bool el = elect_one();
     int h = 0;   // half tiles so far: K of tile n is 2 n, V 2 n + 1
@@ -280,17 +304,26 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         for (int kv = 0; kv < 2; kv++, h++) {
           const int32_t row0 = kv ? c.vrow0 : c.krow0;
           if constexpr (kI8) {
-            const int st = h % PL::kRaw, use = h / PL::kRaw;
-            if (use > 0) wait_bar(&bars->raw_empty[st], (use - 1) & 1, bars, c.status);
-            if (el) {
-              uint8_t* dst = smem + PL::kRawAt + st * kRawSlot;
-              mbar_expect_tx(&bars->raw_full[st], kRawSlot + (kv ? 0 : 1024));
-              for (int k = 0; k < 2; k++) {
-                tma_load_2d(dst + k * 8192, &tmap, 0, row0 + (pg[k] * c.Hkv + kvh) * kPage, &bars->raw_full[st]);
-                if (!kv)   // the scales of both, [page][K, V][64]
-                  bulk_load(smem + PL::kScaleAt + ((h >> 1) & 3) * 1024 + k * kInt8ScaleBytes, c.scales + ((size_t)pg[k] * c.Hkv + kvh) * (2 * kPage),
-                            kInt8ScaleBytes, &bars->raw_full[st]);
+            if (kv == 0) {   // the scales of both, [page][K, V][64]
+              const int st = (h >> 1) & 3, use = h >> 3;
+              if (use > 0) wait_bar(&bars->scale_empty[st], (use - 1) & 1, bars, c.status);
+              if (el) {
+                mbar_expect_tx(&bars->scale_full[st], 2 * kInt8ScaleBytes);
+                for (int k = 0; k < 2; k++)
+                  bulk_load(smem + PL::kScaleAt + st * 1024 + k * kInt8ScaleBytes, c.scales + ((size_t)pg[k] * c.Hkv + kvh) * (2 * kPage), kInt8ScaleBytes,
+                            &bars->scale_full[st]);
               }
+              __syncwarp();
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int at = 2 * h + k, st = at % PL::kRaw, use = at / PL::kRaw;
+              if (use > 0) wait_bar(&bars->raw_empty[st], (use - 1) & 1, bars, c.status);
+              if (el) {
+                mbar_expect_tx(&bars->raw_full[st], kRawSlot);
+                tma_load_2d(smem + PL::kRawAt + st * kRawSlot, &tmap, 0, row0 + (pg[k] * c.Hkv + kvh) * kPage, &bars->raw_full[st]);
+              }
+              __syncwarp();
             }
           } else {
             const int st = h % PL::kSlots, use = h / PL::kSlots;
@@ -309,7 +342,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         }
       }
     }
-  } else if (warp == kWarpMma) {
+  } else if (warp == PL::kWarpMma) {
+    regs_down<PL::kRegsOther, kI8>();
     // =============================== MMA issuer ===============================
     const bool el = elect_one();
     constexpr uint32_t idesc_qk = idesc_of(kI8, false), idesc_pv = idesc_of(kI8, true);
@@ -337,6 +371,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         __syncwarp();
       };
       auto issue_pv = [&](int t, int b, int step) {
+        const int o = two ? step & 1 : b;
+        const bool more = t > (two ? 1 : 0);   // O holds something already
         const int h = 2 * (tt + t) + 1, st = h % PL::kSlots;
         if (b == 0) {
           wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars, c.status);
@@ -365,19 +401,19 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           const uint64_t dV = make_desc_mnmajor_sw128(smem_u32(smem + PL::kRing + st * kSlot), kHalf);
 #pragma unroll
           for (int ks = 0; ks < 8; ks++)
-            umma_ts<1>(tmem + kTmemO + b * 128, tmem + (step & 1) * 128 + ks * 8, dV + ((uint32_t)(ks * 2048) >> 4), idesc_pv, t != 0 || ks != 0);
+            umma_ts<1>(tmem + kTmemO + o * 128, tmem + (step & 1) * 128 + ks * 8, dV + ((uint32_t)(ks * 2048) >> 4), idesc_pv, more || ks != 0);
           if (b == nb - 1) umma_commit<1>(&bars->empty[st]);
           umma_commit<1>(&bars->pv);
         }
         __syncwarp();
       };
-      issue_qk(0, 0, k);
-      for (int t = 0; t < tiles; t++)
-        for (int b = 0; b < nb; b++, k++) {
-          if (b + 1 < nb) issue_qk(t, b + 1, k + 1);
-          else if (t + 1 < tiles) issue_qk(t + 1, 0, k + 1);
-          issue_pv(t, b, k);
-        }
+      const int steps = tiles * nb;
+#pragma unroll 1
+      for (int s = -1; s < steps; s++) {   // one place for each, for the sake of the registers
+        if (s + 1 < steps) issue_qk(nb == 2 ? (s + 1) >> 1 : s + 1, nb == 2 ? (s + 1) & 1 : 0, k + s + 1);
+        if (s >= 0) issue_pv(nb == 2 ? s >> 1 : s, nb == 2 ? s & 1 : 0, k + s);
+      }
+      k += steps;
       tt += tiles;
       if (el) umma_commit<1>(&bars->fin);         // the piece's products are complete
       if (lane == 0) mbar_arrive(&bars->fin);     // and what this warp, or the converters before they handed over the values, wrote beside them
@@ -390,8 +426,10 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   } else if (warp < kSoftmaxWarps) {
     // =============================== softmax ===============================
     // Warp w reads TMEM lanes 32 (w & 3) .. +31 (the hardware's rule), of which warps w and w + 4 take 16 each: rows 16 w .. 16 w + 15 of a block.
-    // Few rows then keep all four schedulers busy.
-    const int r16 = (warp & 3) * 32 + (warp >> 2) * 16;
+    // Few rows then keep all four schedulers busy.  (two: both take the same 16.)
+    regs_up<PL::kRegsSoftmax, kI8>();
+    const int set = two ? warp >> 2 : 0, row_warp = two ? warp & 3 : warp;
+    const int r16 = (warp & 3) * 32 + (two ? 0 : (warp >> 2) * 16);
     const uint32_t lane_addr = (uint32_t)r16 << 16;
     int k = 0, tt = 0, n = 0;
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
@@ -404,7 +442,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       for (int b = 0; b < kNB; b++) {
         if (b >= nb) continue;
         {   // what this warp's rows see of the nodes: a row per lane, then to the lanes that work on it
-          const int r = 128 * b + 16 * warp + (lane & 15), s = (row_base + r) / c.g, tree = c.one_tree ? 0 : p.i;
+          const int r = 128 * b + 16 * row_warp + (lane & 15), s = (row_base + r) / c.g, tree = c.one_tree ? 0 : p.i;
           uint64_t m = 0;
           if (r < rows && s < sq.nodes)
             for (int j = s; j >= 0; j = c.seqs ? c.parents[tree * kTreeNodes + j] : prm.parents[tree][j]) m |= 1ull << j;
@@ -414,7 +452,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         q_scale[b][0] = q_scale[b][1] = c.scale_log2;
 #pragma unroll 4
         for (int i = 0; i < 8; i++) {   // 16 lanes a row, two rows at a time
-          const int j = 2 * i + (lane >> 4), r = 128 * b + 16 * warp + j, ch = (lane & 15) * 8;
+          const int j = 2 * i + (lane >> 4), r = 128 * b + 16 * row_warp + j, ch = (lane & 15) * 8;
           const int s = (row_base + r) / c.g, hq = row_base + r - s * c.g;
           const size_t off = (((size_t)p.i * c.S + s) * c.H + (size_t)kvh * c.g + hq) * kD + ch;
           uint8_t* dst = smem + PL::kQ + b * kSlot + (ch >> 6) * kHalf + swz128(r16 + j, (ch & 63) >> 3);
@@ -447,7 +485,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
               w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
             }
           }
-          *reinterpret_cast<uint4*>(dst) = w;
+          if (set == 0) *reinterpret_cast<uint4*>(dst) = w;
         }
       }
       fence_proxy_async();
@@ -463,22 +501,29 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           m_used[b][hf] = -INFINITY;
           l_run[b][hf] = 0.f;
         }
-      for (int t = p.tb; t < p.te; t++, tt++) {
+      const int k0 = k, tt0 = tt, first = two && (k0 & 1) != set ? p.tb + 1 : p.tb;
+      k += (p.te - p.tb) * nb;
+      tt += p.te - p.tb;
+#pragma unroll 1
+      for (int t = first; t < p.te; t += two ? 2 : 1) {
+        const int tile = tt0 + t - p.tb;
         const int from = sq.len0 - t * kTile;   // first drafted row of the tile
         float shrink = 1.f;                     // what O's unit has grown by
-        const float* k_scale = bars->k_scale[tt & 3];
+        const float* k_scale = bars->k_scale[tile & 3];
         if constexpr (kI8) {
-          wait_bar(&bars->info[tt & 3], (tt >> 2) & 1, bars, c.status);
-          const float unit = bars->v_unit[tt & 3];
-          if (t > p.tb) shrink = v_unit / unit;
+          wait_bar(&bars->k_info[tile & 3], (tile >> 2) & 1, bars, c.status);
+          wait_bar(&bars->v_info[tile & 3], (tile >> 2) & 1, bars, c.status);
+          const float unit = bars->v_unit[tile & 3];
+          if (t > first) shrink = v_unit / unit;
           v_unit = unit;
         }
 #pragma unroll
         for (int b = 0; b < kNB; b++) {
           if (b >= nb) continue;
-          const uint32_t tmem_s = tmem + lane_addr + (k & 1) * 128, tmem_o = tmem + lane_addr + kTmemO + b * 128;
-          wait_bar(&bars->s_full[k & 1], (k >> 1) & 1, bars, c.status);
-          if (128 * b + 16 * warp < rows) {   // else the whole warp's rows are none
+          const int step = k0 + (t - p.tb) * nb + b;
+          const uint32_t tmem_s = tmem + lane_addr + (step & 1) * 128, tmem_o = tmem + lane_addr + kTmemO + (two ? set : b) * 128;
+          wait_bar(&bars->s_full[step & 1], (step >> 1) & 1, bars, c.status);
+          if (128 * b + 16 * row_warp < rows) {   // else the whole warp's rows are none
             tc_fence_after();
             uint32_t sv[64];
             tmem_ld_16x256b_x16(tmem_s, sv);
@@ -555,11 +600,11 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
               unpack2(ps2[hf], ps0, ps1);
               l_run[b][hf] += ps0 + ps1;
             }
-            // O may be rescaled only behind the PV before this one on it.  With two blocks that is the one before QK(k) in the pipe, with one block
+            // O may be rescaled only behind the PV before this one on it.  With two blocks, or two halves, that is the one before QK(k) in the pipe, else
             // PV(k - 1), which QK(k) was ahead of: `pv` has then completed k - 1 or k phases, so its parity is no riddle.
-            if (t > p.tb && __any_sync(0xffffffffu, rescale)) {
-              if (nb == 1) {
-                wait_bar(&bars->pv, (k - 1) & 1, bars, c.status);
+            if (t > first && __any_sync(0xffffffffu, rescale)) {
+              if (nb == 1 && !two) {
+                wait_bar(&bars->pv, (step - 1) & 1, bars, c.status);
                 tc_fence_after();
               }
 #pragma unroll 1
@@ -576,8 +621,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             tc_fence_before();
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->p_full[k & 1]);
-          k++;
+          if (lane == 0) mbar_arrive(&bars->p_full[step & 1]);
         }
       }
       // ---- results out ----
@@ -590,31 +634,51 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       const int slot = 2 * (int)blockIdx.x + (p.us + p.tb == streams.u_begin ? 0 : 1);
 #pragma unroll
       for (int b = 0; b < kNB; b++) {
-        if (b >= nb || 128 * b + 16 * warp >= rows) continue;
-        float f[2];
+        if (b >= nb || 128 * b + 16 * row_warp >= rows) continue;
+        float f[2], f2[2] = {0.f, 0.f};   // of this O, and (two) of the other half's
         int r[2], s[2];
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
-          float l = l_run[b][hf];
+          float l = l_run[b][hf], m = m_used[b][hf], w = v_unit;
           l += __shfl_xor_sync(0xffffffffu, l, 1);
           l += __shfl_xor_sync(0xffffffffu, l, 2);
+          if (two) {   // every row has been through one half or the other, or both
+            const int x = 16 * row_warp + 8 * hf + (lane >> 2);
+            if ((lane & 3) == 0) bars->halves[set][x] = make_float4(m, l, v_unit, 0.f);
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + row_warp) : "memory");   // the two warps of these rows
+            const float4 o = bars->halves[set ^ 1][x];
+            const float top = fmaxf(m, o.x), w0 = m == -INFINITY ? 0.f : ex2_approx(m - top), w1 = o.x == -INFINITY ? 0.f : ex2_approx(o.x - top);
+            l = l * w0 + o.y * w1;
+            w *= w0;
+            f2[hf] = o.z * w1;
+            m = top;
+          }
           if (bad_all || (see[b][hf] & bad_nodes)) l = __uint_as_float(0x7FC00000u);
-          r[hf] = 128 * b + 16 * warp + 8 * hf + (lane >> 2);
+          r[hf] = 128 * b + 16 * row_warp + 8 * hf + (lane >> 2);
           s[hf] = (row_base + r[hf]) / c.g;
           const bool there = ok && s[hf] < sq.nodes;
-          if (stream_whole) {
-            f[hf] = !there || l == 0.f ? 0.f : v_unit / l;
-          } else {
-            f[hf] = there ? v_unit : 0.f;
-            if ((lane & 3) == 0 && r[hf] < rows)
-              *reinterpret_cast<float2*>(c.part_ml + ((size_t)slot * c.rows_rb + r[hf]) * 2) = there ? make_float2(m_used[b][hf], l) : make_float2(-INFINITY, 0.f);
-          }
+          // no part of a sum that nobody has added to, of a row that is not there: zero whatever the accumulator holds
+          const float inv = !there ? 0.f : !stream_whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+          f[hf] = m_used[b][hf] == -INFINITY && l == l ? 0.f : w * inv;
+          f2[hf] *= inv;
+          if (!stream_whole && (lane & 3) == 0 && set == 0 && r[hf] < rows)
+            *reinterpret_cast<float2*>(c.part_ml + ((size_t)slot * c.rows_rb + r[hf]) * 2) = there ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         }
 #pragma unroll 1
-        for (int col = 0; col < kD; col += 64) {
+        for (int col = two ? 64 * set : 0; col < (two ? 64 * set + 64 : kD); col += 64) {   // two: a half of the columns each
           uint32_t ov[32];
-          tmem_ld_16x256b_x8(tmem + lane_addr + kTmemO + b * 128 + col, ov);
+          tmem_ld_16x256b_x8(tmem + lane_addr + kTmemO + (two ? set : b) * 128 + col, ov);
           tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i++) ov[i] = f[(i >> 1) & 1] == 0.f ? 0u : __float_as_uint(__uint_as_float(ov[i]) * f[(i >> 1) & 1]);
+          if (two) {
+            uint32_t o2[32];
+            tmem_ld_16x256b_x8(tmem + lane_addr + kTmemO + (set ^ 1) * 128 + col, o2);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if (f2[(i >> 1) & 1] != 0.f) ov[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), f2[(i >> 1) & 1], __uint_as_float(ov[i])));
+          }
 #pragma unroll
           for (int hf = 0; hf < 2; hf++) {
             if (r[hf] >= rows) continue;
@@ -623,8 +687,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
               const int d = col + 8 * i + 2 * (lane & 3);
-              // a row that nobody fills is zero whatever the accumulator held
-              const float x0 = f[hf] == 0.f ? 0.f : __uint_as_float(ov[4 * i + 2 * hf]) * f[hf], x1 = f[hf] == 0.f ? 0.f : __uint_as_float(ov[4 * i + 2 * hf + 1]) * f[hf];
+              const float x0 = __uint_as_float(ov[4 * i + 2 * hf]), x1 = __uint_as_float(ov[4 * i + 2 * hf + 1]);
               if (!stream_whole) *reinterpret_cast<float2*>(c.part_o + at + d) = make_float2(x0, x1);
               else if (c.out_bf16) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(c.out) + at + d) = pack_bf16x2(x0, x1);
               else *reinterpret_cast<float2*>(reinterpret_cast<float*>(c.out) + at + d) = make_float2(x0, x1);
@@ -639,83 +702,100 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
     }
+  } else if (warp > PL::kWarpMma) {
+    regs_down<PL::kRegsOther, kI8>();   // nothing to do
   } else if constexpr (kI8) {
     // =============================== converters ===============================
     // 16 threads a row, eight codes each: eight rows at a time, the same place of the swizzle in all of them, so that every address is a constant away.
-    const int ct = threadIdx.x - 32 * kWarpConv, hc = ct & 15, r0 = ct >> 4;
+    regs_down<PL::kRegsConv, kI8>();
+    const int ct = threadIdx.x & (32 * kConvWarps - 1), hc = ct & 15, r0 = ct >> 4;
     const uint32_t src0 = swz128(r0, hc >> 1) + (hc & 1) * 8, dst0 = (hc >> 3) * kHalf + swz128(r0, hc & 7);
-    int tt = 0, n = 0;
-    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
-      const TreeSeq sq = streams.seq(p.i);
-      const int end = sq.len0 + sq.nodes;
-      ValueUnit unit;
-      for (int t = p.tb; t < p.te; t++, tt++) {
+    auto convert = [&](int h, const uint32_t* v_scale, auto values) {   // half tile h, a page behind the other
+      const int st = h % PL::kSlots;
+      uint8_t* dst = smem + PL::kRing + st * kSlot + dst0;
 #pragma unroll 1
-        for (int kv = 0; kv < 2; kv++) {
-          const int h = 2 * tt + kv, raw = h % PL::kRaw, st = h % PL::kSlots, use = h / PL::kSlots;
-          wait_bar(&bars->raw_full[raw], (h / PL::kRaw) & 1, bars, c.status);
-          if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
-          if (kv == 0) {
-            // what the softmax needs of the tile, the keys' scales and the unit of the values; and the values' scales over it, a row a thread
-            const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024);
-            bars->k_scale[tt & 3][ct] = scales[(ct >> 6) * 128 + (ct & 63)];
-            // the largest scale of the tile's values: NaN drop out, and rows past the drafted ones, whatever they hold
-            const float4 v = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 128 + 64 + (lane & 15) * 4);
-            const int there = end - t * kTile - 4 * lane;
-            const float top = fmaxf(fmaxf(there > 0 ? v.x : 0.f, there > 1 ? v.y : 0.f), fmaxf(there > 2 ? v.z : 0.f, there > 3 ? v.w : 0.f));
-            if (__any_sync(0xffffffffu, top >= unit.limit)) unit.grow<8>(warp_max(top));   // codes come below 2^15
-            if (ct == 0) bars->v_unit[tt & 3] = 1.f / unit.down;
-            const int pos = t * kTile + ct;
-            float s = pos < end ? scales[(ct >> 6) * 128 + 64 + (ct & 63)] : 0.f;
-            if (!(s == s)) {   // the row held an infinity or a NaN
-              const int node = pos - sq.len0;
-              if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
-              else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
-              s = 0.f;
+      for (int k = 0; k < 2; k++, dst += kRawSlot) {
+        const int at = 2 * h + k, raw = at % PL::kRaw;
+        wait_bar(&bars->raw_full[raw], (at / PL::kRaw) & 1, bars, c.status);
+        const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot + src0;
+        uint2 w[8];
+        uint32_t s[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          w[i] = *reinterpret_cast<const uint2*>(src + i * 1024);
+          if constexpr (decltype(values)::value) s[i] = v_scale[64 * k + 8 * i + r0];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          uint32_t x[4];
+          int8x4_to_f16(w[i].x, x[0], x[1]);
+          int8x4_to_f16(w[i].y, x[2], x[3]);
+          if constexpr (decltype(values)::value) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), *reinterpret_cast<const __half2*>(&s[i]));
+              x[j] = *reinterpret_cast<const uint32_t*>(&y);
             }
-            bars->v_scale[tt & 1][ct] = round_f16x2(s * unit.down, s * unit.down);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->info[tt & 3]);
-          } else {
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");   // every row's scale is there
           }
-          const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot + src0;
-          uint8_t* dst = smem + PL::kRing + st * kSlot + dst0;
-          const uint32_t* v_scale = &bars->v_scale[tt & 1][r0];
-          auto convert = [&](auto values) {
-#pragma unroll
-            for (int i0 = 0; i0 < 16; i0 += 8) {
-              uint2 w[8];
-              uint32_t s[8];
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                w[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * 1024);
-                if constexpr (decltype(values)::value) s[i] = v_scale[8 * (i0 + i)];
-              }
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                uint32_t x[4];
-                int8x4_to_f16(w[i].x, x[0], x[1]);
-                int8x4_to_f16(w[i].y, x[2], x[3]);
-                if constexpr (decltype(values)::value) {
-#pragma unroll
-                  for (int j = 0; j < 4; j++) {
-                    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), *reinterpret_cast<const __half2*>(&s[i]));
-                    x[j] = *reinterpret_cast<const uint32_t*>(&y);
-                  }
-                }
-                *reinterpret_cast<uint4*>(dst + (i0 + i) * 1024) = make_uint4(x[0], x[1], x[2], x[3]);
-              }
-            }
-          };
-          if (kv) convert(std::true_type{});
-          else convert(std::false_type{});
-          fence_proxy_async();
+          *reinterpret_cast<uint4*>(dst + i * 1024) = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->raw_empty[raw]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->full[st]);
+    };
+    int tt = 0;
+    if (warp < kSoftmaxWarps + kConvWarps) {
+      for (Piece p = streams.first(); streams.valid(p); p = streams.next(p))
+        for (int t = p.tb; t < p.te; t++, tt++) {
+          const int h = 2 * tt, st = h % PL::kSlots, use = h / PL::kSlots;
+          if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
+          // the keys' scales to where the softmax reads them: this slot is free, so the tile four before this one has been through it
+          wait_bar(&bars->scale_full[tt & 3], (tt >> 2) & 1, bars, c.status);
+          bars->k_scale[tt & 3][ct] = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024)[(ct >> 6) * 128 + (ct & 63)];
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&bars->full[st]);
-            mbar_arrive(&bars->raw_empty[raw]);
+            mbar_arrive(&bars->k_info[tt & 3]);
+            mbar_arrive(&bars->scale_empty[tt & 3]);
           }
+          convert(h, nullptr, std::false_type{});
+        }
+    } else {
+      int n = 0;
+      for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+        const TreeSeq sq = streams.seq(p.i);
+        const int end = sq.len0 + sq.nodes;
+        ValueUnit unit;
+        for (int t = p.tb; t < p.te; t++, tt++) {
+          // the unit of the tile's values, and their scales over it, a row a thread
+          wait_bar(&bars->scale_full[tt & 3], (tt >> 2) & 1, bars, c.status);
+          const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024);
+          // the largest scale: NaN drop out, and rows past the drafted ones, whatever they hold
+          const float4 v = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 128 + 64 + (lane & 15) * 4);
+          const int there = end - t * kTile - 4 * lane;
+          const float top = fmaxf(fmaxf(there > 0 ? v.x : 0.f, there > 1 ? v.y : 0.f), fmaxf(there > 2 ? v.z : 0.f, there > 3 ? v.w : 0.f));
+          if (__any_sync(0xffffffffu, top >= unit.limit)) unit.grow<8>(warp_max(top));   // values come below 2^15
+          if (ct == 0) bars->v_unit[tt & 3] = 1.f / unit.down;
+          const int pos = t * kTile + ct;
+          float s = pos < end ? scales[(ct >> 6) * 128 + 64 + (ct & 63)] : 0.f;
+          if (!(s == s)) {   // the row held an infinity or a NaN
+            const int node = pos - sq.len0;
+            if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
+            else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
+            s = 0.f;
+          }
+          bars->v_scale[tt & 1][ct] = round_f16x2(s * unit.down, s * unit.down);
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars->v_info[tt & 3]);
+            mbar_arrive(&bars->scale_empty[tt & 3]);
+          }
+          const int h = 2 * tt + 1, use = h / PL::kSlots;
+          if (use > 0) wait_bar(&bars->empty[h % PL::kSlots], (use - 1) & 1, bars, c.status);
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");   // every row's scale is there
+          convert(h, bars->v_scale[tt & 1], std::true_type{});
         }
       }
     }

@@ -40,6 +40,7 @@ constexpr int kTile = 128, kD = kGqaD, kPage = kGqaPageTok;
 constexpr int kHalf = 16384;                   // [128 rows][64 16-bit columns], 128-byte swizzle
 constexpr int kSlot = 2 * kHalf;               // K or V of a tile, or 128 query rows
 constexpr int kRawSlot = kPage * kD;           // codes of K or V of a page
+constexpr int kTilesAhead = 4;                 // (8-bit cache) of a tile in L2 before its loads
 constexpr int kFixUnits = 2;                   // tiles: what a piece costs beyond its own (queries in, results out)
 constexpr int kSoftmaxWarps = 8, kConvWarps = 4;   // of K, and of V
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
@@ -63,6 +64,7 @@ struct TreeCommon {
   int32_t n_rb, rows_rb;       // row groups of a kv head, rows of each (the last may have fewer)
   int32_t krow0, vrow0;
   const float* scales;         // 8-bit cache: of the layer
+  const uint8_t* codes;        // and the pool's rows
   float scale_log2;
   const void* q;
   int32_t q_bf16, out_bf16;
@@ -147,8 +149,11 @@ struct Bars {
 
 template <bool kI8, int kNB>
 struct Plan {
-  static constexpr int kSlots = kI8 ? 4 : kNB == 2 ? 5 : 6;       // of 32 KB; an even number keeps K and V apart, as the converters need it
-  static constexpr int kRaw = kI8 ? (kNB == 2 ? 3 : 6) : 0;       // of 8 KB
+  // Rings.  On the 8-bit cache K and V have slots of their own in each: a warp that waits for some of a slot's phases only cannot tell them apart.
+  static constexpr int kSlots = kI8 ? 4 : kNB == 2 ? 5 : 6;                                      // of 32 KB
+  static constexpr int kRawK = kI8 ? (kNB == 2 ? 2 : 3) : 0, kRawV = kI8 ? (kNB == 2 ? 1 : 3) : 0;   // of 8 KB
+  static constexpr int kRaw = kRawK + kRawV;
+  static_assert(!kI8 || kSlots % 2 == 0, "K in the even slots, V in the odd ones");
   static constexpr int kScaleSlots = kI8 ? 4 : 0;                 // scales as they come, of a tile, 1 KB
   static constexpr int kQ = 0;
   static constexpr int kRing = kNB * kSlot;
@@ -288,17 +293,36 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       const int kvh = p.st / c.n_rb;
       const int last_slot = max(0, (sq.len0 + sq.nodes + kPage - 1) / kPage - 1);   // a tile's second page may lie past the rows: nobody sees those keys
       const int32_t* row = c.table + (size_t)sq.seq * c.table_stride;
-      int32_t ids = 0;
+      // page ids of sixteen tiles, a page a lane, and of the next sixteen
+      auto window = [&](int t) -> int32_t {
+        int32_t pg = __ldg(row + min(2 * t + lane, last_slot));
+        if (pg < 0 || pg >= c.num_pages) {   // reported, and replaced by page 0 so that no load leaves the pool
+          set_status(c.status, RELUX_ERR_BAD_PAGE);
+          pg = 0;
+        }
+        return pg;
+      };
+      int32_t ids = 0, ids2 = window(p.tb);
       for (int t = p.tb; t < p.te; t++) {
-        if (((t - p.tb) & 15) == 0) ids = __ldg(row + min(2 * t + lane, last_slot));
+        const int j = (t - p.tb) & 15;
+        if (j == 0) {
+          ids = ids2;
+          ids2 = window(t + 16);
+        }
         int32_t pg[2];
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          pg[k] = __shfl_sync(0xffffffffu, ids, (2 * (t - p.tb) + k) & 31);
-          if (pg[k] < 0 || pg[k] >= c.num_pages) {   // reported, and replaced by page 0 so that no load leaves the pool
-            set_status(c.status, RELUX_ERR_BAD_PAGE);
-            pg[k] = 0;
+        for (int k = 0; k < 2; k++) pg[k] = __shfl_sync(0xffffffffu, ids, 2 * j + k);
+        if constexpr (kI8) {
+          // The rings hold 48 KB at most, of which what is being converted is no prefetch: too little for the latency of HBM at 23 bytes a clock, enough for
+          // that of L2.  So the tile kTilesAhead on is asked for now, by six lanes: K, V and scales of its two pages.
+          const int a = 2 * (j + kTilesAhead) + (lane & 1);
+          const int32_t near = __shfl_sync(0xffffffffu, ids, a & 31), far = __shfl_sync(0xffffffffu, ids2, a & 31), pa = a < 32 ? near : far;
+          if (t + kTilesAhead < p.te && lane < 6) {
+            const size_t head = (size_t)pa * c.Hkv + kvh;
+            if (lane < 2) prefetch_l2(c.scales + head * (2 * kPage), kInt8ScaleBytes);
+            else prefetch_l2(c.codes + ((size_t)(lane < 4 ? c.krow0 : c.vrow0) + head * kPage) * kD, kRawSlot);
           }
+          __syncwarp();
         }
 #pragma unroll
         for (int kv = 0; kv < 2; kv++, h++) {
@@ -317,7 +341,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-              const int at = 2 * h + k, st = at % PL::kRaw, use = at / PL::kRaw;
+              const int at = 2 * (h >> 1) + k;   // page of its kind
+              const int st = kv ? PL::kRawK + at % PL::kRawV : at % PL::kRawK, use = kv ? at / PL::kRawV : at / PL::kRawK;
               if (use > 0) wait_bar(&bars->raw_empty[st], (use - 1) & 1, bars, c.status);
               if (el) {
                 mbar_expect_tx(&bars->raw_full[st], kRawSlot);
@@ -711,12 +736,13 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     const int ct = threadIdx.x & (32 * kConvWarps - 1), hc = ct & 15, r0 = ct >> 4;
     const uint32_t src0 = swz128(r0, hc >> 1) + (hc & 1) * 8, dst0 = (hc >> 3) * kHalf + swz128(r0, hc & 7);
     auto convert = [&](int h, const uint32_t* v_scale, auto values) {   // half tile h, a page behind the other
+      constexpr int kRing = decltype(values)::value ? PL::kRawV : PL::kRawK, kFirst = decltype(values)::value ? PL::kRawK : 0;
       const int st = h % PL::kSlots;
       uint8_t* dst = smem + PL::kRing + st * kSlot + dst0;
 #pragma unroll 1
       for (int k = 0; k < 2; k++, dst += kRawSlot) {
-        const int at = 2 * h + k, raw = at % PL::kRaw;
-        wait_bar(&bars->raw_full[raw], (at / PL::kRaw) & 1, bars, c.status);
+        const int at = 2 * (h >> 1) + k, raw = kFirst + at % kRing;
+        wait_bar(&bars->raw_full[raw], (at / kRing) & 1, bars, c.status);
         const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot + src0;
         uint2 w[8];
         uint32_t s[8];
@@ -936,7 +962,10 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   const int64_t rows_per_block = (int64_t)prm.num_pages * Hkv * kPage;
   c.krow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block);
   c.vrow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block + rows_per_block);
-  if (p->int8) c.scales = p->scales_at(a.layer);
+  if (p->int8) {
+    c.scales = p->scales_at(a.layer);
+    c.codes = (const uint8_t*)p->storage;
+  }
   c.scale_log2 = a.scale * 1.4426950408889634f;
   c.q = d_q;
   c.q_bf16 = a.q_dtype == RELUX_DTYPE_BF16;

@@ -11,6 +11,7 @@
 //
 // Roles of a CTA:
 //   producer   a tile's K and V by TMA, 32 KB each, into a ring; on the 8-bit cache page by page, 8 KB each, and the scales, into rings of their own
+//   scales     (8-bit cache) a warp: the keys' scales of a tile to where the softmax reads them, the values' over their unit to the converters
 //   converters (8-bit cache, four warps for K, four for V) codes -> binary16 operands in the ring's swizzled layout.  K as whole numbers: a row's scale multiplies its column of
 //              scores, in float32.  V times its scale over a power of two that all of the piece's rows share so far (11 bits, as P has then; 2^29 between
 //              the largest row and one that is no longer exact to 11 bits); where a row comes that is too large for it, the power grows and O is rescaled.
@@ -136,50 +137,49 @@ struct Streams {
 };
 
 struct Bars {
-  uint64_t full[6], empty[6], raw_full[6], raw_empty[6], scale_full[4], scale_empty[4], k_info[4], v_info[4], s_full[2], p_full[2], q_full, pv, fin, drain;
+  uint64_t full[6], empty[6], raw_full[9], raw_empty[9], scale_full[4], scale_empty[4], info[4], info_empty[4], s_full[2], p_full[2], q_full, pv, fin, drain;
   uint32_t tmem_base;
   volatile int32_t abort_flag;
   uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
   uint32_t bad_all[4];         // (8-bit cache) a cached row with one
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
   float4 halves[2][64];        // (two) a row's max, sum and unit of O, of either half of the warps
-  uint32_t v_scale[2][kTile];  // (8-bit cache) of a tile's values, over their unit, binary16 twice
+  alignas(16) uint32_t v_scale[4][kTile];   // (8-bit cache) of a tile's values, over their unit, binary16 twice
   alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys.  Without an 8-bit cache there is no room for these two, nor with two blocks for `halves`
 };
 
 template <bool kI8, int kNB>
 struct Plan {
-  // Rings.  On the 8-bit cache K and V have slots of their own in each: a warp that waits for some of a slot's phases only cannot tell them apart.
-  static constexpr int kSlots = kI8 ? 4 : kNB == 2 ? 5 : 6;                                      // of 32 KB
-  static constexpr int kRawK = kI8 ? (kNB == 2 ? 2 : 3) : 0, kRawV = kI8 ? (kNB == 2 ? 1 : 3) : 0;   // of 8 KB
-  static constexpr int kRaw = kRawK + kRawV;
-  static_assert(!kI8 || kSlots % 2 == 0, "K in the even slots, V in the odd ones");
+  // Rings.  bf16: of 32 KB slots, K and V of a tile in turn.  8-bit cache: of operands, two slots of 32 KB for K and three of a page, 16 KB, for V; of codes,
+  // slots of 8 KB, K and V apart: what is being converted is no prefetch, and HBM wants some 50 KB an SM on their way.  (K and V must have slots of their own: a
+  // warp that waits for some of a slot's phases only cannot tell them apart.)
+  static constexpr int kSlots = kI8 ? 2 : kNB == 2 ? 5 : 6, kSlotsV = kI8 ? 3 : 0;
+  static constexpr int kRawK = kI8 ? (kNB == 2 ? 3 : 4) : 0, kRawV = kI8 ? (kNB == 2 ? 2 : 5) : 0, kRaw = kRawK + kRawV;
   static constexpr int kScaleSlots = kI8 ? 4 : 0;                 // scales as they come, of a tile, 1 KB
   static constexpr int kQ = 0;
   static constexpr int kRing = kNB * kSlot;
-  static constexpr int kRawAt = kRing + kSlots * kSlot;
+  static constexpr int kRingV = kRing + kSlots * kSlot;
+  static constexpr int kRawAt = kRingV + kSlotsV * kHalf;
   static constexpr int kScaleAt = kRawAt + kRaw * kRawSlot;
   static constexpr int kBars = kScaleAt + kScaleSlots * 1024;
   static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, halves));
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
+  [[maybe_unused]] static constexpr int kWarpScale = kSoftmaxWarps + 2 * kConvWarps + 2;
   static constexpr int kWarpLoad = kSoftmaxWarps + (kI8 ? 2 * kConvWarps : 0), kWarpMma = kWarpLoad + 1;
   // Four more warps where registers are dealt out anew, which warps do by fours: softmax 152, converters 64, the others 48 of the 96 of the launch.
   static constexpr int kThreads = 32 * (kI8 ? kWarpLoad + 4 : kWarpMma + 1);
   static constexpr int kRegsSoftmax = 152, kRegsConv = 64, kRegsOther = 48;
   static_assert(!kI8 || 256 * kRegsSoftmax + 256 * kRegsConv + 128 * kRegsOther <= 640 * 96, "more registers than the block is launched with");
 };
-// (Not a function of its own: a call takes registers that a role may have given back.)
-__device__ __forceinline__ void wait_slow(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
-  for (uint32_t i = 0; i < kSpinLimit; i++) {
-    if (mbar_try_wait(bar, parity)) return;
-    if ((i & 255) == 255 && b->abort_flag) return;
-    if (i > 512) __nanosleep(20);
-  }
-  b->abort_flag = 1;
-  set_status(status, RELUX_ERR_TIMEOUT);
-}
-__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, Bars* b, int32_t* status) {
-  if (!mbar_try_wait(bar, parity)) wait_slow(bar, parity, b, status);
+// The wait that gives up raises the flag, which ends all others; the kernel's end reports it.  Short, and not a function of its own: a call takes registers that
+// a role may have given back, and the roles of a block share one instruction cache.  (With the report and a pause in every wait, and all loops of the
+// converters unrolled, the 8-bit kernel waited 5.3 cycles for an instruction per one issued; 16 x 8192 tokens, 64 rows, took 149 us.)
+__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, Bars* b) {
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); i++)
+    if (i >= kSpinLimit || b->abort_flag) {
+      b->abort_flag = 1;
+      break;
+    }
 }
 
 // Registers from or to the block's pool, by all warps of a warpgroup.
@@ -244,15 +244,15 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       mbar_init(&bars->full[s], kI8 ? kConvWarps : 1);
       mbar_init(&bars->empty[s], 1);
     }
-    for (int s = 0; s < 6; s++) {
+    for (int s = 0; s < 9; s++) {
       mbar_init(&bars->raw_full[s], 1);
       mbar_init(&bars->raw_empty[s], kConvWarps);
     }
     for (int s = 0; s < 4; s++) {
       mbar_init(&bars->scale_full[s], 1);
-      mbar_init(&bars->scale_empty[s], 2 * kConvWarps);
-      mbar_init(&bars->k_info[s], kConvWarps);
-      mbar_init(&bars->v_info[s], kConvWarps);
+      mbar_init(&bars->scale_empty[s], 1);
+      mbar_init(&bars->info[s], 1);
+      mbar_init(&bars->info_empty[s], (two ? kSoftmaxWarps / 2 : kSoftmaxWarps) + kConvWarps);
       bars->bad_nodes[s] = 0;
       bars->bad_all[s] = 0;
     }
@@ -313,8 +313,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 2; k++) pg[k] = __shfl_sync(0xffffffffu, ids, 2 * j + k);
         if constexpr (kI8) {
-          // The rings hold 48 KB at most, of which what is being converted is no prefetch: too little for the latency of HBM at 23 bytes a clock, enough for
-          // that of L2.  So the tile kTilesAhead on is asked for now, by six lanes: K, V and scales of its two pages.
+          // The tile kTilesAhead on is asked for now, by six lanes: K, V and scales of its two pages.
           const int a = 2 * (j + kTilesAhead) + (lane & 1);
           const int32_t near = __shfl_sync(0xffffffffu, ids, a & 31), far = __shfl_sync(0xffffffffu, ids2, a & 31), pa = a < 32 ? near : far;
           if (t + kTilesAhead < p.te && lane < 6) {
@@ -330,7 +329,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           if constexpr (kI8) {
             if (kv == 0) {   // the scales of both, [page][K, V][64]
               const int st = (h >> 1) & 3, use = h >> 3;
-              if (use > 0) wait_bar(&bars->scale_empty[st], (use - 1) & 1, bars, c.status);
+              if (use > 0) wait_bar(&bars->scale_empty[st], (use - 1) & 1, bars);
               if (el) {
                 mbar_expect_tx(&bars->scale_full[st], 2 * kInt8ScaleBytes);
                 for (int k = 0; k < 2; k++)
@@ -343,7 +342,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             for (int k = 0; k < 2; k++) {
               const int at = 2 * (h >> 1) + k;   // page of its kind
               const int st = kv ? PL::kRawK + at % PL::kRawV : at % PL::kRawK, use = kv ? at / PL::kRawV : at / PL::kRawK;
-              if (use > 0) wait_bar(&bars->raw_empty[st], (use - 1) & 1, bars, c.status);
+              if (use > 0) wait_bar(&bars->raw_empty[st], (use - 1) & 1, bars);
               if (el) {
                 mbar_expect_tx(&bars->raw_full[st], kRawSlot);
                 tma_load_2d(smem + PL::kRawAt + st * kRawSlot, &tmap, 0, row0 + (pg[k] * c.Hkv + kvh) * kPage, &bars->raw_full[st]);
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             }
           } else {
             const int st = h % PL::kSlots, use = h / PL::kSlots;
-            if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
+            if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars);
             if (el) {
               uint8_t* dst = smem + PL::kRing + st * kSlot;
               mbar_expect_tx(&bars->full[st], kSlot);
@@ -377,10 +376,10 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
       const int nb = blocks_of(p), tiles = p.te - p.tb;
       const TreeSeq sq = streams.seq(p.i);
-      wait_bar(&bars->q_full, n & 1, bars, c.status);   // the queries are there, and O of the piece before has been read
+      wait_bar(&bars->q_full, n & 1, bars);   // the queries are there, and O of the piece before has been read
       auto issue_qk = [&](int t, int b, int step) {
-        const int h = 2 * (tt + t), st = h % PL::kSlots;
-        if (b == 0) wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars, c.status);
+        const int h = kI8 ? tt + t : 2 * (tt + t), st = h % PL::kSlots;
+        if (b == 0) wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars);
         tc_fence_after();
         if (el) {
           const uint64_t dK = make_desc_kmajor_sw128(smem_u32(smem + PL::kRing + st * kSlot));
@@ -398,39 +397,58 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       auto issue_pv = [&](int t, int b, int step) {
         const int o = two ? step & 1 : b;
         const bool more = t > (two ? 1 : 0);   // O holds something already
-        const int h = 2 * (tt + t) + 1, st = h % PL::kSlots;
-        if (b == 0) {
-          wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars, c.status);
-          if constexpr (!kI8) {   // infinities and NaN among drafted values, and behind them
-            const int from = sq.len0 - (p.tb + t) * kTile;   // first drafted row of the tile
-            if (from < kTile) {
-              uint8_t* v = smem + PL::kRing + st * kSlot;
-              bool any = false;
-              for (int r = max(from, 0) + (lane >> 4); r < kTile; r += 2) {   // 16 lanes a row
-                uint4* at = reinterpret_cast<uint4*>(v + ((lane >> 3) & 1) * kHalf + swz128(r, lane & 7));
-                const uint4 w = *at;
-                if (bf16x2_not_finite(w.x) | bf16x2_not_finite(w.y) | bf16x2_not_finite(w.z) | bf16x2_not_finite(w.w)) {
-                  *at = make_uint4(bf16x2_finite(w.x), bf16x2_finite(w.y), bf16x2_finite(w.z), bf16x2_finite(w.w));
-                  if (r - from < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << (r - from));
-                  any = true;
+        if constexpr (kI8) {   // V page by page
+          wait_bar(&bars->p_full[step & 1], (step >> 1) & 1, bars);
+#pragma unroll 1
+          for (int k = 0; k < 2; k++) {
+            const int at = 2 * (tt + t) + k, st = at % PL::kSlotsV;
+            if (b == 0) wait_bar(&bars->full[PL::kSlots + st], (at / PL::kSlotsV) & 1, bars);
+            tc_fence_after();   // P, and a rescaled O
+            if (el) {
+              const uint64_t dV = make_desc_mnmajor_sw128(smem_u32(smem + PL::kRingV + st * kHalf), kHalf / 2);
+#pragma unroll
+              for (int ks = 0; ks < 4; ks++)
+                umma_ts<1>(tmem + kTmemO + o * 128, tmem + (step & 1) * 128 + k * 32 + ks * 8, dV + ((uint32_t)(ks * 2048) >> 4), idesc_pv, more || (k | ks) != 0);
+              if (b == nb - 1) umma_commit<1>(&bars->empty[PL::kSlots + st]);
+              if (k == 1) umma_commit<1>(&bars->pv);
+            }
+            __syncwarp();
+          }
+        } else {
+          const int h = 2 * (tt + t) + 1, st = h % PL::kSlots;
+          if (b == 0) {
+            wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars);
+            {   // infinities and NaN among drafted values, and behind them
+              const int from = sq.len0 - (p.tb + t) * kTile;   // first drafted row of the tile
+              if (from < kTile) {
+                uint8_t* v = smem + PL::kRing + st * kSlot;
+                bool any = false;
+                for (int r = max(from, 0) + (lane >> 4); r < kTile; r += 2) {   // 16 lanes a row
+                  uint4* at = reinterpret_cast<uint4*>(v + ((lane >> 3) & 1) * kHalf + swz128(r, lane & 7));
+                  const uint4 w = *at;
+                  if (bf16x2_not_finite(w.x) | bf16x2_not_finite(w.y) | bf16x2_not_finite(w.z) | bf16x2_not_finite(w.w)) {
+                    *at = make_uint4(bf16x2_finite(w.x), bf16x2_finite(w.y), bf16x2_finite(w.z), bf16x2_finite(w.w));
+                    if (r - from < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << (r - from));
+                    any = true;
+                  }
                 }
+                if (any) fence_proxy_async();
+                __syncwarp();
               }
-              if (any) fence_proxy_async();
-              __syncwarp();
             }
           }
-        }
-        wait_bar(&bars->p_full[step & 1], (step >> 1) & 1, bars, c.status);
-        tc_fence_after();   // P, and a rescaled O
-        if (el) {
-          const uint64_t dV = make_desc_mnmajor_sw128(smem_u32(smem + PL::kRing + st * kSlot), kHalf);
+          wait_bar(&bars->p_full[step & 1], (step >> 1) & 1, bars);
+          tc_fence_after();   // P, and a rescaled O
+          if (el) {
+            const uint64_t dV = make_desc_mnmajor_sw128(smem_u32(smem + PL::kRing + st * kSlot), kHalf);
 #pragma unroll
-          for (int ks = 0; ks < 8; ks++)
-            umma_ts<1>(tmem + kTmemO + o * 128, tmem + (step & 1) * 128 + ks * 8, dV + ((uint32_t)(ks * 2048) >> 4), idesc_pv, more || ks != 0);
-          if (b == nb - 1) umma_commit<1>(&bars->empty[st]);
-          umma_commit<1>(&bars->pv);
+            for (int ks = 0; ks < 8; ks++)
+              umma_ts<1>(tmem + kTmemO + o * 128, tmem + (step & 1) * 128 + ks * 8, dV + ((uint32_t)(ks * 2048) >> 4), idesc_pv, more || ks != 0);
+            if (b == nb - 1) umma_commit<1>(&bars->empty[st]);
+            umma_commit<1>(&bars->pv);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       };
       const int steps = tiles * nb;
 #pragma unroll 1
@@ -536,8 +554,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         float shrink = 1.f;                     // what O's unit has grown by
         const float* k_scale = bars->k_scale[tile & 3];
         if constexpr (kI8) {
-          wait_bar(&bars->k_info[tile & 3], (tile >> 2) & 1, bars, c.status);
-          wait_bar(&bars->v_info[tile & 3], (tile >> 2) & 1, bars, c.status);
+          wait_bar(&bars->info[tile & 3], (tile >> 2) & 1, bars);
           const float unit = bars->v_unit[tile & 3];
           if (t > first) shrink = v_unit / unit;
           v_unit = unit;
@@ -547,7 +564,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           if (b >= nb) continue;
           const int step = k0 + (t - p.tb) * nb + b;
           const uint32_t tmem_s = tmem + lane_addr + (step & 1) * 128, tmem_o = tmem + lane_addr + kTmemO + (two ? set : b) * 128;
-          wait_bar(&bars->s_full[step & 1], (step >> 1) & 1, bars, c.status);
+          wait_bar(&bars->s_full[step & 1], (step >> 1) & 1, bars);
           if (128 * b + 16 * row_warp < rows) {   // else the whole warp's rows are none
             tc_fence_after();
             uint32_t sv[64];
@@ -570,14 +587,17 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             const bool whole = from >= kTile;
             if (!whole) {
 #pragma unroll
-              for (int i = 0; i < 16; i++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                  const int node = 8 * i + 2 * (lane & 3) + e - from;
-#pragma unroll
-                  for (int hf = 0; hf < 2; hf++)
-                    if (node >= 0 && (node >= kTreeNodes || !(see[b][hf] >> node & 1u))) sv[4 * i + 2 * hf + e] = 0xFF800000u;   // -inf
+              for (int hf = 0; hf < 2; hf++) {
+                uint32_t hidden = 0;   // bit 2 i + e: key 8 i + 2 (lane & 3) + e
+#pragma unroll 1
+                for (int i = 31; i >= 0; i--) {
+                  const int node = 8 * (i >> 1) + 2 * (lane & 3) + (i & 1) - from;
+                  hidden = hidden << 1 | (node >= kTreeNodes || (node >= 0 && !(see[b][hf] >> node & 1u)));
                 }
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                  if (hidden & (1u << i)) sv[4 * (i >> 1) + 2 * hf + (i & 1)] = 0xFF800000u;   // -inf
+              }
             }
             // row maxima of the raw scores: four chains of three-input maxima
             float mx[2];
@@ -616,8 +636,10 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
               ps2[hf] = pack2(0.f, 0.f);
             }
             uint32_t pw[32];
-            if (whole) exp_scores<kI8, true>(sv, factor2, neg_m2, pw, ps2);
-            else exp_scores<kI8, false>(sv, factor2, neg_m2, pw, ps2);   // ex2(-inf) is 0, the polynomial's is not
+            // With two blocks the special-function unit is what exponentials wait for; else the instruction cache is (see wait_bar).  ex2(-inf) is 0, the
+            // polynomial's is not.
+            if (kNB == 2 && whole) exp_scores<kI8, true>(sv, factor2, neg_m2, pw, ps2);
+            else exp_scores<kI8, false>(sv, factor2, neg_m2, pw, ps2);
             tmem_st_16x128b_x16(tmem_s, pw);
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
@@ -629,7 +651,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             // PV(k - 1), which QK(k) was ahead of: `pv` has then completed k - 1 or k phases, so its parity is no riddle.
             if (t > first && __any_sync(0xffffffffu, rescale)) {
               if (nb == 1 && !two) {
-                wait_bar(&bars->pv, (step - 1) & 1, bars, c.status);
+                wait_bar(&bars->pv, (step - 1) & 1, bars);
                 tc_fence_after();
               }
 #pragma unroll 1
@@ -648,9 +670,10 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->p_full[step & 1]);
         }
+        if (kI8 && lane == 0) mbar_arrive(&bars->info_empty[tile & 3]);
       }
       // ---- results out ----
-      wait_bar(&bars->fin, n & 1, bars, c.status);
+      wait_bar(&bars->fin, n & 1, bars);
       tc_fence_after();
       const bool ok = bars->abort_flag == 0;
       const uint64_t bad_nodes = bars->bad_nodes[n & 3];
@@ -727,108 +750,125 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
     }
-  } else if (warp > PL::kWarpMma) {
-    regs_down<PL::kRegsOther, kI8>();   // nothing to do
   } else if constexpr (kI8) {
-    // =============================== converters ===============================
-    // 16 threads a row, eight codes each: eight rows at a time, the same place of the swizzle in all of them, so that every address is a constant away.
-    regs_down<PL::kRegsConv, kI8>();
-    const int ct = threadIdx.x & (32 * kConvWarps - 1), hc = ct & 15, r0 = ct >> 4;
-    const uint32_t src0 = swz128(r0, hc >> 1) + (hc & 1) * 8, dst0 = (hc >> 3) * kHalf + swz128(r0, hc & 7);
-    auto convert = [&](int h, const uint32_t* v_scale, auto values) {   // half tile h, a page behind the other
-      constexpr int kRing = decltype(values)::value ? PL::kRawV : PL::kRawK, kFirst = decltype(values)::value ? PL::kRawK : 0;
-      const int st = h % PL::kSlots;
-      uint8_t* dst = smem + PL::kRing + st * kSlot + dst0;
-#pragma unroll 1
-      for (int k = 0; k < 2; k++, dst += kRawSlot) {
-        const int at = 2 * (h >> 1) + k, raw = kFirst + at % kRing;
-        wait_bar(&bars->raw_full[raw], (at / kRing) & 1, bars, c.status);
-        const uint8_t* src = smem + PL::kRawAt + raw * kRawSlot + src0;
-        uint2 w[8];
-        uint32_t s[8];
+    if (warp > PL::kWarpScale) {
+      regs_down<PL::kRegsOther, kI8>();   // nothing to do
+    } else if (warp == PL::kWarpScale) {
+      // =============================== scales ===============================
+      regs_down<PL::kRegsOther, kI8>();
+      int tt = 0, n = 0;
+      for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+        const TreeSeq sq = streams.seq(p.i);
+        ValueUnit unit;
+        for (int t = p.tb; t < p.te; t++, tt++) {
+          const int at = tt & 3, r = 4 * lane;   // four rows a lane
+          if (tt >= 4) wait_bar(&bars->info_empty[at], ((tt >> 2) - 1) & 1, bars);
+          wait_bar(&bars->scale_full[at], (tt >> 2) & 1, bars);
+          const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + at * 1024) + (r >> 6) * 128 + (r & 63);
+          *reinterpret_cast<float4*>(&bars->k_scale[at][r]) = *reinterpret_cast<const float4*>(scales);
+          const float4 v4 = *reinterpret_cast<const float4*>(scales + 64);
+          float v[4] = {v4.x, v4.y, v4.z, v4.w};
+          const int pos = t * kTile + r, there = sq.len0 + sq.nodes - pos;
+          float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          w[i] = *reinterpret_cast<const uint2*>(src + i * 1024);
-          if constexpr (decltype(values)::value) s[i] = v_scale[64 * k + 8 * i + r0];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          uint32_t x[4];
-          int8x4_to_f16(w[i].x, x[0], x[1]);
-          int8x4_to_f16(w[i].y, x[2], x[3]);
-          if constexpr (decltype(values)::value) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), *reinterpret_cast<const __half2*>(&s[i]));
-              x[j] = *reinterpret_cast<const uint32_t*>(&y);
+          for (int i = 0; i < 4; i++) {
+            if (i >= there) v[i] = 0.f;   // behind the drafted rows, where anything may lie
+            if (!(v[i] == v[i])) {        // the row held an infinity or a NaN
+              const int node = pos + i - sq.len0;
+              if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
+              else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
+              v[i] = 0.f;
             }
+            top = fmaxf(top, v[i]);
           }
-          *reinterpret_cast<uint4*>(dst + i * 1024) = make_uint4(x[0], x[1], x[2], x[3]);
+          if (__any_sync(0xffffffffu, top >= unit.limit)) unit.grow<8>(warp_max(top));   // values come below 2^15
+          uint32_t s[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[i] = round_f16x2(v[i] * unit.down, v[i] * unit.down);
+          *reinterpret_cast<uint4*>(&bars->v_scale[at][r]) = make_uint4(s[0], s[1], s[2], s[3]);
+          if (lane == 0) bars->v_unit[at] = __uint_as_float((254u << 23) - __float_as_uint(unit.down));   // 1 / down, a power of two
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars->info[at]);
+            mbar_arrive(&bars->scale_empty[at]);
+          }
+        }
+      }
+    } else {
+      // =============================== converters ===============================
+      // 16 threads a row, eight codes each: eight rows at a time, the same place of the swizzle in all of them, so that every address is a constant away.
+      regs_down<PL::kRegsConv, kI8>();
+      const int ct = threadIdx.x & (32 * kConvWarps - 1), hc = ct & 15, r0 = ct >> 4;
+      const uint8_t* src0 = smem + PL::kRawAt + swz128(r0, hc >> 1) + (hc & 1) * 8;
+      const uint32_t dst0 = swz128(r0, hc & 7);
+      constexpr int kAtOnce = 4;
+      // A page of codes to dst; its slot of the ring of codes is free again.
+      auto convert = [&](uint8_t* dst, int raw, int use, const uint32_t* v_scale, auto values) {
+        wait_bar(&bars->raw_full[raw], use & 1, bars);
+        const uint8_t* src = src0 + raw * kRawSlot;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 8; i0 += kAtOnce, src += kAtOnce * 1024, dst += kAtOnce * 1024) {
+          uint2 w[kAtOnce];
+          uint32_t s[kAtOnce];
+#pragma unroll
+          for (int i = 0; i < kAtOnce; i++) {
+            w[i] = *reinterpret_cast<const uint2*>(src + i * 1024);
+            if constexpr (decltype(values)::value) s[i] = v_scale[8 * (i0 + i)];
+          }
+#pragma unroll
+          for (int i = 0; i < kAtOnce; i++) {
+            uint32_t x[4];
+            int8x4_to_f16(w[i].x, x[0], x[1]);
+            int8x4_to_f16(w[i].y, x[2], x[3]);
+            if constexpr (decltype(values)::value) {
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), *reinterpret_cast<const __half2*>(&s[i]));
+                x[j] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            *reinterpret_cast<uint4*>(dst + i * 1024) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->raw_empty[raw]);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->full[st]);
-    };
-    int tt = 0;
-    if (warp < kSoftmaxWarps + kConvWarps) {
+      };
+      const bool of_v = warp >= kSoftmaxWarps + kConvWarps;
+      int tt = 0;
       for (Piece p = streams.first(); streams.valid(p); p = streams.next(p))
         for (int t = p.tb; t < p.te; t++, tt++) {
-          const int h = 2 * tt, st = h % PL::kSlots, use = h / PL::kSlots;
-          if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars, c.status);
-          // the keys' scales to where the softmax reads them: this slot is free, so the tile four before this one has been through it
-          wait_bar(&bars->scale_full[tt & 3], (tt >> 2) & 1, bars, c.status);
-          bars->k_scale[tt & 3][ct] = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024)[(ct >> 6) * 128 + (ct & 63)];
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&bars->k_info[tt & 3]);
-            mbar_arrive(&bars->scale_empty[tt & 3]);
+          if (!of_v) {
+            const int st = tt % PL::kSlots, use = tt / PL::kSlots;
+            if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars);
+            uint8_t* dst = smem + PL::kRing + st * kSlot + (hc >> 3) * kHalf + dst0;
+#pragma unroll 1
+            for (int k = 0; k < 2; k++) convert(dst + k * kRawSlot, (2 * tt + k) % PL::kRawK, (2 * tt + k) / PL::kRawK, nullptr, std::false_type{});
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->full[st]);
+          } else {
+            wait_bar(&bars->info[tt & 3], (tt >> 2) & 1, bars);
+#pragma unroll 1
+            for (int k = 0; k < 2; k++) {
+              const int at = 2 * tt + k, st = at % PL::kSlotsV, use = at / PL::kSlotsV;
+              if (use > 0) wait_bar(&bars->empty[PL::kSlots + st], (use - 1) & 1, bars);
+              convert(smem + PL::kRingV + st * kHalf + (hc >> 3) * (kHalf / 2) + dst0, PL::kRawK + at % PL::kRawV, at / PL::kRawV,
+                      &bars->v_scale[tt & 3][64 * k + r0], std::true_type{});
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars->full[PL::kSlots + st]);
+            }
+            if (lane == 0) mbar_arrive(&bars->info_empty[tt & 3]);
           }
-          convert(h, nullptr, std::false_type{});
         }
-    } else {
-      int n = 0;
-      for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
-        const TreeSeq sq = streams.seq(p.i);
-        const int end = sq.len0 + sq.nodes;
-        ValueUnit unit;
-        for (int t = p.tb; t < p.te; t++, tt++) {
-          // the unit of the tile's values, and their scales over it, a row a thread
-          wait_bar(&bars->scale_full[tt & 3], (tt >> 2) & 1, bars, c.status);
-          const float* scales = reinterpret_cast<const float*>(smem + PL::kScaleAt + (tt & 3) * 1024);
-          // the largest scale: NaN drop out, and rows past the drafted ones, whatever they hold
-          const float4 v = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 128 + 64 + (lane & 15) * 4);
-          const int there = end - t * kTile - 4 * lane;
-          const float top = fmaxf(fmaxf(there > 0 ? v.x : 0.f, there > 1 ? v.y : 0.f), fmaxf(there > 2 ? v.z : 0.f, there > 3 ? v.w : 0.f));
-          if (__any_sync(0xffffffffu, top >= unit.limit)) unit.grow<8>(warp_max(top));   // values come below 2^15
-          if (ct == 0) bars->v_unit[tt & 3] = 1.f / unit.down;
-          const int pos = t * kTile + ct;
-          float s = pos < end ? scales[(ct >> 6) * 128 + 64 + (ct & 63)] : 0.f;
-          if (!(s == s)) {   // the row held an infinity or a NaN
-            const int node = pos - sq.len0;
-            if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
-            else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
-            s = 0.f;
-          }
-          bars->v_scale[tt & 1][ct] = round_f16x2(s * unit.down, s * unit.down);
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&bars->v_info[tt & 3]);
-            mbar_arrive(&bars->scale_empty[tt & 3]);
-          }
-          const int h = 2 * tt + 1, use = h / PL::kSlots;
-          if (use > 0) wait_bar(&bars->empty[h % PL::kSlots], (use - 1) & 1, bars, c.status);
-          asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");   // every row's scale is there
-          convert(h, bars->v_scale[tt & 1], std::true_type{});
-        }
-      }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0) stamp_end(c.time);
+  if (threadIdx.x == 0) {
+    stamp_end(c.time);
+    if (bars->abort_flag) set_status(c.status, RELUX_ERR_TIMEOUT);
+  }
   if (warp == 0) tmem_dealloc<1>(tmem, kTmemCols);
 }
 

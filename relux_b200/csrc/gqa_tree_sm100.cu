@@ -798,14 +798,18 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       // =============================== converters ===============================
       // 16 threads a row, eight codes each: eight rows at a time, the same place of the swizzle in all of them, so that every address is a constant away.
       regs_down<PL::kRegsConv, kI8>();
-      const int ct = threadIdx.x & (32 * kConvWarps - 1), hc = ct & 15, r0 = ct >> 4;
+      // K on two of the schedulers, V on the other two: warps of a scheduler in step share what it fetches of instructions.
+      const bool of_v = (warp & 2) != 0;
+      const int ct = 64 * ((warp >> 2) & 1) + (threadIdx.x & 63), hc = ct & 15, r0 = ct >> 4;
       const uint8_t* src0 = smem + PL::kRawAt + swz128(r0, hc >> 1) + (hc & 1) * 8;
       const uint32_t dst0 = swz128(r0, hc & 7);
       constexpr int kAtOnce = 4;
-      // A page of codes to dst; its slot of the ring of codes is free again.
-      auto convert = [&](uint8_t* dst, int raw, int use, const uint32_t* v_scale, auto values) {
-        wait_bar(&bars->raw_full[raw], use & 1, bars);
-        const uint8_t* src = src0 + raw * kRawSlot;
+      int raw = 0, raw_phase = 0;   // the next slot of the ring of codes
+      // A page of codes to dst; its slot is free again.
+      auto convert = [&](uint8_t* dst, const uint32_t* v_scale, auto values) {
+        constexpr int kFirst = decltype(values)::value ? PL::kRawK : 0, kNum = decltype(values)::value ? PL::kRawV : PL::kRawK;
+        wait_bar(&bars->raw_full[kFirst + raw], raw_phase, bars);
+        const uint8_t* src = src0 + (kFirst + raw) * kRawSlot;
 #pragma unroll 1
         for (int i0 = 0; i0 < 8; i0 += kAtOnce, src += kAtOnce * 1024, dst += kAtOnce * 1024) {
           uint2 w[kAtOnce];
@@ -831,32 +835,40 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->raw_empty[raw]);
+        if (lane == 0) mbar_arrive(&bars->raw_empty[kFirst + raw]);
+        if (++raw == kNum) {
+          raw = 0;
+          raw_phase ^= 1;
+        }
       };
-      const bool of_v = warp >= kSoftmaxWarps + kConvWarps;
-      int tt = 0;
+      int tt = 0, st = 0, phase = 1;   // tiles so far; the next slot of the ring of operands, whose first use waits for nothing
       for (Piece p = streams.first(); streams.valid(p); p = streams.next(p))
         for (int t = p.tb; t < p.te; t++, tt++) {
           if (!of_v) {
-            const int st = tt % PL::kSlots, use = tt / PL::kSlots;
-            if (use > 0) wait_bar(&bars->empty[st], (use - 1) & 1, bars);
+            wait_bar(&bars->empty[st], phase, bars);
             uint8_t* dst = smem + PL::kRing + st * kSlot + (hc >> 3) * kHalf + dst0;
 #pragma unroll 1
-            for (int k = 0; k < 2; k++) convert(dst + k * kRawSlot, (2 * tt + k) % PL::kRawK, (2 * tt + k) / PL::kRawK, nullptr, std::false_type{});
+            for (int k = 0; k < 2; k++) convert(dst + k * kRawSlot, nullptr, std::false_type{});
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->full[st]);
+            if (++st == PL::kSlots) {
+              st = 0;
+              phase ^= 1;
+            }
           } else {
             wait_bar(&bars->info[tt & 3], (tt >> 2) & 1, bars);
 #pragma unroll 1
             for (int k = 0; k < 2; k++) {
-              const int at = 2 * tt + k, st = at % PL::kSlotsV, use = at / PL::kSlotsV;
-              if (use > 0) wait_bar(&bars->empty[PL::kSlots + st], (use - 1) & 1, bars);
-              convert(smem + PL::kRingV + st * kHalf + (hc >> 3) * (kHalf / 2) + dst0, PL::kRawK + at % PL::kRawV, at / PL::kRawV,
-                      &bars->v_scale[tt & 3][64 * k + r0], std::true_type{});
+              wait_bar(&bars->empty[PL::kSlots + st], phase, bars);
+              convert(smem + PL::kRingV + st * kHalf + (hc >> 3) * (kHalf / 2) + dst0, &bars->v_scale[tt & 3][64 * k + r0], std::true_type{});
               fence_proxy_async();
               __syncwarp();
               if (lane == 0) mbar_arrive(&bars->full[PL::kSlots + st]);
+              if (++st == PL::kSlotsV) {
+                st = 0;
+                phase ^= 1;
+              }
             }
             if (lane == 0) mbar_arrive(&bars->info_empty[tt & 3]);
           }

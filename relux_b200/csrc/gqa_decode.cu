@@ -279,7 +279,8 @@ int32_t launch_gqa_decode_fast(Pool* p, const SeqBatch& sb, const relux_attn_arg
   // the kernel holds (num_heads / num_kv_heads) * q_tokens <= 32 query rows per kv head; longer multi-token calls
   // (a prompt) are cut into groups of tokens that run as the z slices of one grid
   const int per_group = std::max(1, 32 / g);
-  if (a.q_tokens <= per_group || p->int8) return launch_gqa_stream(p, sb, a, d_q, d_out, false, nullptr);
+  if (a.q_tokens <= per_group) return launch_gqa_stream(p, sb, a, d_q, d_out, false, nullptr);
+  if (p->int8) return launch_gqa_tree_sm100(p, sb, a, d_q, d_out, false, nullptr, nullptr);   // codes become matrix operands inside the kernel
   // a prompt: 128 query rows per CTA on the tcgen05 prefill kernel; the grid slices of the decode kernel serve the
   // group sizes that do not tile 128 rows, and stay selectable as a tuning knob
   if (a.q_dtype == RELUX_DTYPE_BF16 && gqa_prompt_wants_bf16(p, a)) return launch_gqa_prefill_sm100(p, sb, a, (const uint16_t*)d_q, (float*)d_out);

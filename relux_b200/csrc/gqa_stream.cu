@@ -18,17 +18,19 @@ bool gqa_append_fusable(const Pool* p, const relux_attn_args& a, int max_new_row
 
 // q: device [n][S][H][128] token-major (f32 or bf16).  out: device, same shape, f32 or bf16.  With `app` (advance = 1) the
 // host lengths already count the new rows.  `tree` (with `app`, advance = 0): the new rows are its nodes.
-static int32_t launch_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16,
-                             const GqaAppend* app, const GqaTree* tree, bool write_rows, int s0, int S) {
+int32_t launch_gqa_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16,
+                          const GqaAppend* app, const GqaTree* tree) {
   const relux_pool_params& prm = p->prm;
-  const int n = sb.n_seqs, Hkv = prm.gqa_num_kv_heads, g = a.num_heads / Hkv, R = g * S;
-  // A slice of a causal call sees the cache as if it ended with its own last token.
-  const int extra = tree ? 0 : a.causal ? a.extra_tokens - (a.q_tokens - s0 - S) : a.extra_tokens;
+  const int n = sb.n_seqs, Hkv = prm.gqa_num_kv_heads, g = a.num_heads / Hkv, R = g * a.q_tokens;
   GqaStreamCommon c{};
   GqaSeq inl[kInlineLarge + 1];
   GqaSeq* seqs = inl;
   int slot_index = 0;
   if (n > kInlineLarge) {
+    if (tree && stream_captured(p->dev)) {
+      set_error("tree_verify: a call of more than %d sequences cannot be captured", kInlineLarge);
+      return RELUX_ERR_UNSUPPORTED;
+    }
     int32_t* slot = nullptr;
     if (int32_t rc = stage_acquire(p, &slot, &slot_index)) return rc;
     seqs = (GqaSeq*)slot;
@@ -38,9 +40,8 @@ static int32_t launch_stream(Pool* p, const SeqBatch& sb, const relux_attn_args&
   for (int i = 0; i < n; i++) {
     const int s = sb.seq[i], len = p->h_len[(size_t)a.layer * prm.max_seqs + s], n_new = app ? app->rows[i] : 0;
     seqs[i] = GqaSeq{s, app && app->advance ? len - n_new : len, (int32_t)units64, rows};
-    // one page at least: a slice ahead of a sequence's rows, and a tree without nodes on an empty one, see nothing of it
-    const int pages = (len + (tree ? n_new : extra) + kGqaPageTok - 1) / kGqaPageTok;
-    units64 += std::max(1, pages) + kStreamUnits;
+    // one page at least: a tree without nodes on an empty sequence sees nothing of it
+    units64 += std::max(1, (len + (tree ? n_new : a.extra_tokens) + kGqaPageTok - 1) / kGqaPageTok) + kStreamUnits;
     rows += n_new;
   }
   seqs[n] = GqaSeq{0, 0, (int32_t)units64, rows};
@@ -82,12 +83,10 @@ static int32_t launch_stream(Pool* p, const SeqBatch& sb, const relux_attn_args&
   c.Hkv = Hkv;
   c.H = a.num_heads;
   c.g = g;
-  c.S = S;
+  c.S = a.q_tokens;
   c.R = R;
-  c.s0 = s0;
-  c.s_all = a.q_tokens;
   c.one_tree = tree && tree->one;
-  c.extra = extra;
+  c.extra = a.extra_tokens;
   c.causal = a.causal;
   const int64_t rows_per_block = (int64_t)prm.num_pages * Hkv * kGqaPageTok;
   c.krow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block);
@@ -101,7 +100,7 @@ static int32_t launch_stream(Pool* p, const SeqBatch& sb, const relux_attn_args&
   c.part_o = (float*)p->part_o.p;
   c.part_ml = c.part_o + part_rows * kGqaD;
   c.done = (uint32_t*)p->stream_done.p;
-  if (app && rows > 0 && write_rows) {
+  if (app && rows > 0) {
     c.k_new = app->k;
     c.v_new = app->v;
     c.new_f32 = app->dtype == RELUX_DTYPE_F32;
@@ -117,15 +116,6 @@ static int32_t launch_stream(Pool* p, const SeqBatch& sb, const relux_attn_args&
   const int8_t* parents = tree ? tree->parents : nullptr;
   if (tree) return p->int8 ? launch_gqa_stream_tree_int8(p, c, seqs, parents, workers) : launch_gqa_stream_tree(p, c, seqs, parents, workers);
   return p->int8 ? launch_gqa_stream_int8(p, c, seqs, workers) : launch_variant<0>(p, c, seqs, nullptr, workers);
-}
-
-int32_t launch_gqa_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16,
-                          const GqaAppend* app, const GqaTree* tree) {
-  const int per = std::max(1, 32 / (a.num_heads / p->prm.gqa_num_kv_heads));   // query tokens of a launch
-  if (tree && a.q_tokens > per) return launch_gqa_tree_sm100(p, sb, a, d_q, d_out, out_bf16, *tree, app->rows);
-  for (int s0 = 0; s0 < a.q_tokens; s0 += per)
-    if (int32_t rc = launch_stream(p, sb, a, d_q, d_out, out_bf16, app, tree, s0 == 0, s0, std::min(per, a.q_tokens - s0))) return rc;
-  return RELUX_OK;
 }
 
 }  // namespace relux

@@ -77,8 +77,6 @@ struct GqaStreamCommon {
   uint16_t* k_base;
   uint16_t* v_base;
   float* scales;           // kInt8: of this layer, [page][kv head][K, V][64]
-  // All variants but 0: the launch takes query tokens [s0, s0 + S) of the call's s_all.
-  int32_t s0, s_all;
   const int8_t* parents;   // kTree: [n_seqs or 1][kTreeNodes] where the sequences are a device copy
   int32_t one_tree;        // every sequence has the same tree
   int32_t* len;            // this layer's device lengths
@@ -160,7 +158,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto seq_of = [&](int i) -> GqaSeq { return c.seqs ? c.seqs[i] : prm.seqs[i]; };
   auto unit0_of = [&](int i) -> int { return c.seqs ? c.seqs[i].unit0 : prm.seqs[i].unit0; };
   auto row0_of = [&](int i) -> int { return c.seqs ? c.seqs[i].row0 : prm.seqs[i].row0; };
-  auto token_of = [&](int i, int s) -> size_t { return V ? (size_t)i * c.s_all + c.s0 + s : (size_t)i * c.S + s; };   // row of q and out
   // ranges: c.range units per worker, one more for the first c.range_more of them
   auto range_begin = [&](int w) -> int { return w * c.range + min(w, c.range_more); };
   auto worker_of = [&](int u) -> int {
@@ -311,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   auto store_out = [&](const Piece& q, int r, float4 o) {
     const int s = r / c.g, hq = r - s * c.g;
-    const size_t off = (token_of(q.i, s) * c.H + (size_t)q.kvh * c.g + hq) * kGqaD + lane * 4;
-    if (kTr && c.s0 + s >= row0_of(q.i + 1) - row0_of(q.i)) o = make_float4(0.f, 0.f, 0.f, 0.f);   // a row past the sequence's nodes
+    const size_t off = (((size_t)q.i * c.S + s) * c.H + (size_t)q.kvh * c.g + hq) * kGqaD + lane * 4;
+    if (kTr && s >= row0_of(q.i + 1) - row0_of(q.i)) o = make_float4(0.f, 0.f, 0.f, 0.f);   // a row past the sequence's nodes
     if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + off) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
     else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + off) = o;
   };
@@ -416,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint16_t* qs = reinterpret_cast<uint16_t*>(smem + SM::kQ + b * SM::kQBytes);
       if constexpr (kTr) {   // what the rows see of the new rows, beside their queries
         for (int r = ft; r < c.R; r += 32 * kFinishers) {
-          const int s = c.s0 + r / c.g, tree = c.one_tree ? 0 : q.i;
+          const int s = r / c.g, tree = c.one_tree ? 0 : q.i;
           uint64_t see = 0;
           if (s < row0_of(q.i + 1) - row0_of(q.i))
             for (int j = s; j >= 0; j = c.parents ? c.parents[tree * kTreeNodes + j] : prm.parents[tree][j]) see |= 1ull << j;
@@ -426,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (kI8) {   // 16 lanes a row: binary16, by a power of two that brings the row's largest value to its upper end
         for (int r0 = 2 * fw; r0 < c.R; r0 += 2 * kFinishers) {
           const int r = r0 + (lane >> 4), ch = (lane & 15) * 8, s = r / c.g, hq = r - s * c.g;
-          const size_t off = (token_of(q.i, s) * c.H + (size_t)q.kvh * c.g + hq) * kGqaD + ch;
+          const size_t off = (((size_t)q.i * c.S + s) * c.H + (size_t)q.kvh * c.g + hq) * kGqaD + ch;
           int8_put_query(qs + r * kGqaQStride, ch, r < c.R, c.q, off, c.q_bf16, c.scale_log2);
         }
         __syncwarp();
@@ -443,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (e >= total) break;
           const int r = e >> 4, ch = (e & 15) * 8;
           const int s = r / c.g, hq = r - s * c.g;
-          const size_t off = (token_of(q.i, s) * c.H + (size_t)q.kvh * c.g + hq) * kGqaD + ch;
+          const size_t off = (((size_t)q.i * c.S + s) * c.H + (size_t)q.kvh * c.g + hq) * kGqaD + ch;
           if (c.q_bf16) {
             w[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(c.q) + off);
           } else {

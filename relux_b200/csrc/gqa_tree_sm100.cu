@@ -1,11 +1,11 @@
-// Attention of drafted trees with more than 32 query rows per kv head, on the 5th-generation tensor cores (tcgen05 + TMEM), over the bf16 and the 8-bit
-// grouped-query cache.
+// Attention of more than 32 query rows per kv head, on the 5th-generation tensor cores (tcgen05 + TMEM): drafted trees over the bf16 and the 8-bit
+// grouped-query cache, and prompts (or long verifies) over the 8-bit one.
 //
 // o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  where query token i sees every cached row and, of the drafted ones, itself
-// and its ancestors.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128 operations for the 512 (264) bytes of
+// and its ancestors; of a prompt, every row up to its own.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128 operations for the 512 (264) bytes of
 // a token and kv head, so the cache's bytes bound trees of up to some 200 rows (100 on the 8-bit cache) and the tensor cores and the softmax larger ones.
 //
-// A STREAM is a sequence's tiles of 128 keys for one kv head and up to 256 of its rows (one or two blocks of 128, M of both contractions).  All streams of the
+// A STREAM is the tiles of 128 keys that up to 256 of a kv head's rows (one or two blocks of 128, M of both contractions) see.  All streams of the
 // call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into one equal range per SM; a PIECE is the part of a stream inside a range.
 // A piece that is a whole stream writes its output; others leave float32 partials that merge_tree_kernel joins.
 //
@@ -44,6 +44,7 @@ constexpr int kRawSlot = kPage * kD;           // codes of K or V of a page
 constexpr int kTilesAhead = 4;                 // (8-bit cache) of a tile in L2 before its loads
 constexpr int kFixUnits = 2;                   // tiles: what a piece costs beyond its own (queries in, results out)
 constexpr int kSoftmaxWarps = 8, kConvWarps = 4;   // of K, and of V
+constexpr int kWarpScale = kSoftmaxWarps + 2 * kConvWarps + 2;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
 constexpr float kRescaleThreshold = 8.0f;      // log2: P reaches 2^8 before the running max follows
 // (8-bit cache) log2: what P and its sum are larger by.  Binary16 has 11 bits down to 2^-14, and P reaches 2^(8 + 7): probabilities keep 11 bits down to 2^-21
@@ -52,17 +53,21 @@ constexpr float kPUp = 7.0f;
 constexpr int kPolyPairsOf8 = 2;               // of a lane's score pairs, as many take the exponential on the FMA pipe
 constexpr int kInlineSmall = 32, kInlineLarge = 256;
 
+// A group of rows of a sequence: rows [row0, row0 + rows_rb) of every kv head.
 struct TreeSeq {
-  int32_t seq, len0, nodes;
-  int32_t unit0;               // first unit of the sequence, one stream counted
+  int32_t seq, i;              // sequence of the pool, and of the call
+  int32_t len0, end;           // tokens that all of its rows see, and that any does; a tree's nodes are those from len0 on
+  int32_t row0;
+  int32_t unit0;               // first unit, one kv head counted
 };
 struct TreeCommon {
   const TreeSeq* seqs;         // device copy, or nullptr: inline
   const int8_t* parents;       // of a device copy
-  int32_t one_tree;
+  int32_t one_tree, tree;      // tree = 0: query token s sees tokens below row_end + s (causal), or below row_end
+  int32_t causal;
   const int32_t* table;
   int32_t table_stride, num_pages, n_seqs, range, range_more, Hkv, H, g, S, R;
-  int32_t n_rb, rows_rb;       // row groups of a kv head, rows of each (the last may have fewer)
+  int32_t n_rb, rows_rb;       // groups of a sequence, rows of each (the last may have fewer)
   int32_t krow0, vrow0;
   const float* scales;         // 8-bit cache: of the layer
   const uint8_t* codes;        // and the pool's rows
@@ -82,52 +87,65 @@ struct TreeParams {
   int8_t parents[N][kTreeNodes];
 };
 
-// The streams as every role walks them: pieces of this range, in order.
+// The streams as every role walks them: pieces of this range, in order.  Sequence by sequence, kv head by kv head, group by group: the groups of a kv head
+// read the same tiles.
 struct Piece {
-  int32_t i, st, us, tb, te, tiles;   // sequence of the call, stream of the sequence (kv head * n_rb + row group), its first unit, tiles [tb, te) of `tiles`
+  int32_t e, kvh, us, tb, te, tiles;   // group (of all), kv head, first unit of the stream, tiles [tb, te) of `tiles`
 };
 template <int N>
 struct Streams {
   const TreeParams<N>& prm;
   int32_t u_begin, u_end;
   __device__ __forceinline__ Streams(const TreeParams<N>& p, int worker) : prm(p), u_begin(range_begin(worker)), u_end(range_begin(worker + 1)) {}
-  __device__ __forceinline__ int unit0(int i) const { return prm.c.seqs ? prm.c.seqs[i].unit0 : prm.seqs[i].unit0; }
-  __device__ __forceinline__ TreeSeq seq(int i) const { return prm.c.seqs ? prm.c.seqs[i] : prm.seqs[i]; }
-  __device__ __forceinline__ int per_seq() const { return prm.c.Hkv * prm.c.n_rb; }
+  __device__ __forceinline__ int unit0(int e) const { return prm.c.seqs ? prm.c.seqs[e].unit0 : prm.seqs[e].unit0; }
+  __device__ __forceinline__ TreeSeq seq(int e) const { return prm.c.seqs ? prm.c.seqs[e] : prm.seqs[e]; }
   __device__ __forceinline__ int range_begin(int w) const { return w * prm.c.range + min(w, prm.c.range_more); }
   __device__ __forceinline__ int worker_of(int u) const {
     const int big = prm.c.range_more * (prm.c.range + 1);
     return u < big ? (int)((unsigned)u / (unsigned)(prm.c.range + 1)) : prm.c.range_more + (int)((unsigned)(u - big) / (unsigned)prm.c.range);
   }
+  __device__ __forceinline__ void cut(Piece& p) const {
+    if (p.us >= u_end) return;
+    p.tiles = unit0(p.e + 1) - unit0(p.e) - kFixUnits;
+    p.te = min(p.tiles, u_end - p.us);
+  }
   // The stream that unit u belongs to, from its tile at u on.
   __device__ __forceinline__ Piece at(int u) const {
+    const int n_rb = prm.c.n_rb, Hkv = prm.c.Hkv;
     int lo = 0, hi = prm.c.n_seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (unit0(mid) * per_seq() <= u) lo = mid;
+      if (unit0(mid * n_rb) * Hkv <= u) lo = mid;
       else hi = mid;
     }
+    const int e0 = lo * n_rb, n0 = unit0(e0), head = unit0(e0 + n_rb) - n0;
     Piece p;
-    p.i = lo;
-    const int n0 = unit0(lo), len = unit0(lo + 1) - n0;
-    p.st = (u - n0 * per_seq()) / len;
-    p.us = n0 * per_seq() + p.st * len;
-    p.tiles = len - kFixUnits;
+    p.kvh = (u - n0 * Hkv) / head;
+    const int base = n0 * Hkv + p.kvh * head;
+    lo = e0;
+    hi = e0 + n_rb;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (base + unit0(mid) - n0 <= u) lo = mid;
+      else hi = mid;
+    }
+    p.e = lo;
+    p.us = base + unit0(lo) - n0;
     p.tb = u - p.us;
-    p.te = min(p.tiles, u_end - p.us);
+    p.te = p.tiles = 0;
+    cut(p);
     return p;
   }
   __device__ __forceinline__ bool valid(const Piece& p) const { return p.us < u_end; }
   __device__ __forceinline__ Piece next(const Piece& q) const {
     Piece p = q;
     p.us += p.tiles + kFixUnits;
-    if (++p.st == per_seq()) {
-      p.st = 0;
-      p.i++;
-      if (p.us < u_end) p.tiles = unit0(p.i + 1) - unit0(p.i) - kFixUnits;
-    }
     p.tb = 0;
-    p.te = min(p.tiles, u_end - p.us);
+    if ((++p.e) % prm.c.n_rb == 0) {
+      if (++p.kvh < prm.c.Hkv) p.e -= prm.c.n_rb;
+      else p.kvh = 0;
+    }
+    cut(p);
     return p;
   }
   __device__ __forceinline__ Piece first() const {
@@ -164,7 +182,6 @@ struct Plan {
   static constexpr int kBars = kScaleAt + kScaleSlots * 1024;
   static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, halves));
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
-  [[maybe_unused]] static constexpr int kWarpScale = kSoftmaxWarps + 2 * kConvWarps + 2;
   static constexpr int kWarpLoad = kSoftmaxWarps + (kI8 ? 2 * kConvWarps : 0), kWarpMma = kWarpLoad + 1;
   // Four more warps where registers are dealt out anew, which warps do by fours: softmax 152, converters 64, the others 48 of the 96 of the launch.
   static constexpr int kThreads = 32 * (kI8 ? kWarpLoad + 4 : kWarpMma + 1);
@@ -280,8 +297,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   chain_wait();
   if (threadIdx.x == 0) stamp_begin(c.time);
   const Streams<N> streams(prm, blockIdx.x);
-  auto rows_of = [&](const Piece& p) -> int { return min(c.rows_rb, c.R - (p.st % c.n_rb) * c.rows_rb); };
-  auto blocks_of = [&](const Piece& p) -> int { return kNB == 1 ? 1 : (rows_of(p) + 127) / 128; };
+  auto rows_of = [&](const TreeSeq& sq) -> int { return min(c.rows_rb, c.R - sq.row0); };
+  auto blocks_of = [&](const TreeSeq& sq) -> int { return kNB == 1 ? 1 : (rows_of(sq) + 127) / 128; };
 
   if (warp == PL::kWarpLoad) {
     regs_down<PL::kRegsOther, kI8>();
@@ -289,9 +306,9 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     const bool el = elect_one();
     int h = 0;   // half tiles so far: K of tile n is 2 n, V 2 n + 1
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p)) {
-      const TreeSeq sq = streams.seq(p.i);
-      const int kvh = p.st / c.n_rb;
-      const int last_slot = max(0, (sq.len0 + sq.nodes + kPage - 1) / kPage - 1);   // a tile's second page may lie past the rows: nobody sees those keys
+      const TreeSeq sq = streams.seq(p.e);
+      const int kvh = p.kvh;
+      const int last_slot = max(0, (sq.end + kPage - 1) / kPage - 1);   // a tile's second page may lie past the rows: nobody sees those keys
       const int32_t* row = c.table + (size_t)sq.seq * c.table_stride;
       // page ids of sixteen tiles, a page a lane, and of the next sixteen
       auto window = [&](int t) -> int32_t {
@@ -374,8 +391,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     const uint64_t dQ = make_desc_kmajor_sw128(smem_u32(smem + PL::kQ));
     int k = 0, tt = 0, n = 0;   // steps, tiles, pieces so far
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
-      const int nb = blocks_of(p), tiles = p.te - p.tb;
-      const TreeSeq sq = streams.seq(p.i);
+      const TreeSeq sq = streams.seq(p.e);
+      const int nb = blocks_of(sq), tiles = p.te - p.tb;
       wait_bar(&bars->q_full, n & 1, bars);   // the queries are there, and O of the piece before has been read
       auto issue_qk = [&](int t, int b, int step) {
         const int h = kI8 ? tt + t : 2 * (tt + t), st = h % PL::kSlots;
@@ -476,19 +493,22 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     const uint32_t lane_addr = (uint32_t)r16 << 16;
     int k = 0, tt = 0, n = 0;
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
-      const int nb = blocks_of(p), rows = rows_of(p), kvh = p.st / c.n_rb, row_base = (p.st % c.n_rb) * c.rows_rb;
-      const TreeSeq sq = streams.seq(p.i);
+      const TreeSeq sq = streams.seq(p.e);
+      const int nb = blocks_of(sq), rows = rows_of(sq), kvh = p.kvh, row_base = sq.row0;
       uint64_t see[kNB][2];
       float q_scale[kNB][2];
       // ---- queries in ----
 #pragma unroll
       for (int b = 0; b < kNB; b++) {
         if (b >= nb) continue;
-        {   // what this warp's rows see of the nodes: a row per lane, then to the lanes that work on it
-          const int r = 128 * b + 16 * row_warp + (lane & 15), s = (row_base + r) / c.g, tree = c.one_tree ? 0 : p.i;
+        {   // what this warp's rows see of the nodes, or how many tokens from len0 on: a row per lane, then to the lanes that work on it
+          const int r = 128 * b + 16 * row_warp + (lane & 15), s = (row_base + r) / c.g, tree = c.one_tree ? 0 : sq.i;
           uint64_t m = 0;
-          if (r < rows && s < sq.nodes)
+          if (!c.tree) {
+            m = c.causal ? s - row_base / c.g : 0;
+          } else if (r < rows && s < sq.end - sq.len0) {
             for (int j = s; j >= 0; j = c.seqs ? c.parents[tree * kTreeNodes + j] : prm.parents[tree][j]) m |= 1ull << j;
+          }
 #pragma unroll
           for (int hf = 0; hf < 2; hf++) see[b][hf] = __shfl_sync(0xffffffffu, (unsigned long long)m, (lane >> 2) + 8 * hf);
         }
@@ -497,7 +517,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         for (int i = 0; i < 8; i++) {   // 16 lanes a row, two rows at a time
           const int j = 2 * i + (lane >> 4), r = 128 * b + 16 * row_warp + j, ch = (lane & 15) * 8;
           const int s = (row_base + r) / c.g, hq = row_base + r - s * c.g;
-          const size_t off = (((size_t)p.i * c.S + s) * c.H + (size_t)kvh * c.g + hq) * kD + ch;
+          const size_t off = (((size_t)sq.i * c.S + s) * c.H + (size_t)kvh * c.g + hq) * kD + ch;
           uint8_t* dst = smem + PL::kQ + b * kSlot + (ch >> 6) * kHalf + swz128(r16 + j, (ch & 63) >> 3);
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
           if constexpr (kI8) {
@@ -592,7 +612,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
 #pragma unroll 1
                 for (int i = 31; i >= 0; i--) {
                   const int node = 8 * (i >> 1) + 2 * (lane & 3) + (i & 1) - from;
-                  hidden = hidden << 1 | (node >= kTreeNodes || (node >= 0 && !(see[b][hf] >> node & 1u)));
+                  hidden = hidden << 1 | (!c.tree ? node >= (int)see[b][hf] : node >= kTreeNodes || (node >= 0 && !(see[b][hf] >> node & 1u)));
                 }
 #pragma unroll
                 for (int i = 0; i < 32; i++)
@@ -701,10 +721,10 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             f2[hf] = o.z * w1;
             m = top;
           }
-          if (bad_all || (see[b][hf] & bad_nodes)) l = __uint_as_float(0x7FC00000u);
+          if (bad_all || (c.tree ? (see[b][hf] & bad_nodes) != 0 : bad_nodes != 0 && (int)see[b][hf] > (int)~(uint32_t)bad_nodes)) l = __uint_as_float(0x7FC00000u);
           r[hf] = 128 * b + 16 * row_warp + 8 * hf + (lane >> 2);
           s[hf] = (row_base + r[hf]) / c.g;
-          const bool there = ok && s[hf] < sq.nodes;
+          const bool there = ok && (!c.tree || s[hf] < sq.end - sq.len0);
           // no part of a sum that nobody has added to, of a row that is not there: zero whatever the accumulator holds
           const float inv = !there ? 0.f : !stream_whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
           f[hf] = m_used[b][hf] == -INFINITY && l == l ? 0.f : w * inv;
@@ -730,7 +750,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
 #pragma unroll
           for (int hf = 0; hf < 2; hf++) {
             if (r[hf] >= rows) continue;
-            const size_t at = stream_whole ? ((((size_t)p.i * c.S + s[hf]) * c.H + (size_t)kvh * c.g + (row_base + r[hf] - s[hf] * c.g)) * kD)
+            const size_t at = stream_whole ? ((((size_t)sq.i * c.S + s[hf]) * c.H + (size_t)kvh * c.g + (row_base + r[hf] - s[hf] * c.g)) * kD)
                                            : ((size_t)slot * c.rows_rb + r[hf]) * kD;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -751,14 +771,14 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       __syncwarp();
     }
   } else if constexpr (kI8) {
-    if (warp > PL::kWarpScale) {
+    if (warp > kWarpScale) {
       regs_down<PL::kRegsOther, kI8>();   // nothing to do
-    } else if (warp == PL::kWarpScale) {
+    } else if (warp == kWarpScale) {
       // =============================== scales ===============================
       regs_down<PL::kRegsOther, kI8>();
       int tt = 0, n = 0;
       for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
-        const TreeSeq sq = streams.seq(p.i);
+        const TreeSeq sq = streams.seq(p.e);
         ValueUnit unit;
         for (int t = p.tb; t < p.te; t++, tt++) {
           const int at = tt & 3, r = 4 * lane;   // four rows a lane
@@ -768,7 +788,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           *reinterpret_cast<float4*>(&bars->k_scale[at][r]) = *reinterpret_cast<const float4*>(scales);
           const float4 v4 = *reinterpret_cast<const float4*>(scales + 64);
           float v[4] = {v4.x, v4.y, v4.z, v4.w};
-          const int pos = t * kTile + r, there = sq.len0 + sq.nodes - pos;
+          const int pos = t * kTile + r, there = sq.end - pos;
           float top = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; i++) {
@@ -776,6 +796,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             if (!(v[i] == v[i])) {        // the row held an infinity or a NaN
               const int node = pos + i - sq.len0;
               if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
+              else if (!c.tree) atomicMax(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), (unsigned long long)~(uint32_t)node);   // the first one counts
               else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
               v[i] = 0.f;
             }
@@ -895,7 +916,8 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(const __grid_constant__
   const Piece p = streams.at(u);
   const int w0 = streams.worker_of(p.us), np = streams.worker_of(p.us + p.tiles - 1) - w0 + 1;
   if (p.tb <= 0 || p.tb >= p.tiles || w0 != (int)blockIdx.x) return;   // no stream goes on here, or its first part is further back
-  const int rows = min(c.rows_rb, c.R - (p.st % c.n_rb) * c.rows_rb), r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const TreeSeq sq = streams.seq(p.e);
+  const int rows = min(c.rows_rb, c.R - sq.row0), r = blockIdx.y * 8 + (threadIdx.x >> 5);
   if (r >= rows) return;
   const int first = streams.range_begin(w0) == p.us ? 0 : 1;
   auto row_of = [&](int j) -> size_t { return (size_t)(2 * (w0 + j) + (j ? 0 : first)) * c.rows_rb + r; };
@@ -925,8 +947,8 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(const __grid_constant__
       }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int row = (p.st % c.n_rb) * c.rows_rb + r, s = row / c.g;
-  const size_t at = (((size_t)p.i * c.S + s) * c.H + (size_t)(p.st / c.n_rb) * c.g + (row - s * c.g)) * kD + 4 * lane;
+  const int row = sq.row0 + r, s = row / c.g;
+  const size_t at = (((size_t)sq.i * c.S + s) * c.H + (size_t)p.kvh * c.g + (row - s * c.g)) * kD + 4 * lane;
   if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
   else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
@@ -945,61 +967,67 @@ int32_t launch(Pool* p, const TreeParams<N>& prm, int workers) {
   return RELUX_OK;
 }
 template <int N>
-int32_t launch_n(Pool* p, const TreeCommon& c, const TreeSeq* seqs, const int8_t* parents, int workers) {
+int32_t launch_n(Pool* p, const TreeCommon& c, const TreeSeq* seqs, const GqaTree* tree, int workers) {
   TreeParams<N> prm;
   prm.c = c;
   if (!c.seqs) {
-    memcpy(prm.seqs, seqs, sizeof(TreeSeq) * ((size_t)c.n_seqs + 1));
-    memcpy(prm.parents, parents, (size_t)kTreeNodes * (c.one_tree ? 1 : c.n_seqs));
+    memcpy(prm.seqs, seqs, sizeof(TreeSeq) * ((size_t)c.n_seqs * c.n_rb + 1));
+    if (tree) memcpy(prm.parents, tree->parents, (size_t)kTreeNodes * (tree->one ? 1 : c.n_seqs));
   }
-  if (c.rows_rb <= 128) return p->int8 ? launch<true, 1, N>(p, prm, workers) : launch<false, 1, N>(p, prm, workers);
-  return p->int8 ? launch<true, 2, N>(p, prm, workers) : launch<false, 2, N>(p, prm, workers);
+  if (p->int8) return c.rows_rb <= 128 ? launch<true, 1, N>(p, prm, workers) : launch<true, 2, N>(p, prm, workers);
+  return c.rows_rb <= 128 ? launch<false, 1, N>(p, prm, workers) : launch<false, 2, N>(p, prm, workers);
 }
 
 }  // namespace
 
-// q: device [n][S][H][128] token-major (f32 or bf16).  out: device, same shape, f32 or bf16.  The drafted rows are in the cache; nodes: host, of every sequence.
-int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16, const GqaTree& tree,
+// q: device [n][S][H][128] token-major (f32 or bf16).  out: device, same shape, f32 or bf16.  All rows are in the cache.  tree: with `nodes`, host, those of
+// every sequence, which lie behind its length; nullptr: the call's own mask (causal or none).
+int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16, const GqaTree* tree,
                               const int32_t* nodes) {
   const relux_pool_params& prm = p->prm;
-  const int n = sb.n_seqs, Hkv = prm.gqa_num_kv_heads, g = a.num_heads / Hkv, R = g * a.q_tokens;
+  const int n = sb.n_seqs, Hkv = prm.gqa_num_kv_heads, g = a.num_heads / Hkv, S = a.q_tokens;
+  const int64_t R = (int64_t)g * S;
   TreeCommon c{};
-  c.n_rb = (R + 255) / 256;
-  c.rows_rb = ((R + c.n_rb - 1) / c.n_rb + 15) / 16 * 16;
-  TreeSeq inl[kInlineLarge + 1];
-  TreeSeq* seqs = inl;
-  int slot_index = 0;
-  if (n > kInlineLarge) {
-    int32_t* slot = nullptr;
-    if (int32_t rc = stage_acquire(p, &slot, &slot_index)) return rc;
-    seqs = (TreeSeq*)slot;
-  }
+  c.n_rb = (int)((R + 255) / 256);
+  c.rows_rb = (int)((R + c.n_rb - 1) / c.n_rb + 15) / 16 * 16;
+  c.n_rb = (int)((R + c.rows_rb - 1) / c.rows_rb);
+  const int64_t groups = (int64_t)n * c.n_rb;
+  if (R >= ((int64_t)1 << 30) || groups >= ((int64_t)1 << 24)) { set_error("more query rows than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
+  std::vector<TreeSeq> seqs((size_t)groups + 1);
   int64_t units64 = 0;
   for (int i = 0; i < n; i++) {
-    const int s = sb.seq[i], len = p->h_len[(size_t)a.layer * prm.max_seqs + s];
-    seqs[i] = TreeSeq{s, len, nodes[i], (int32_t)units64};
-    units64 += std::max(1, (len + nodes[i] + kTile - 1) / kTile) + kFixUnits;
+    const int s = sb.seq[i], len = p->h_len[(size_t)a.layer * prm.max_seqs + s], T = len + (tree ? nodes[i] : a.extra_tokens);
+    for (int rb = 0; rb < c.n_rb; rb++) {
+      const int row0 = rb * c.rows_rb, s0 = row0 / g, s1 = (int)(std::min<int64_t>(row0 + c.rows_rb, R) - 1) / g;   // first and last query token
+      // causal: token s sees the first T - S + s + 1
+      const int len0 = tree ? len : a.causal ? T - S + s0 + 1 : T, end = tree || !a.causal ? T : T - S + s1 + 1;
+      seqs[(size_t)i * c.n_rb + rb] = TreeSeq{s, i, len0, end, row0, (int32_t)units64};
+      units64 += std::max(1, (end + kTile - 1) / kTile) + kFixUnits;
+      if (units64 * Hkv >= ((int64_t)1 << 31)) { set_error("more cached pages than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
+    }
   }
-  seqs[n] = TreeSeq{0, 0, 0, (int32_t)units64};
-  units64 *= Hkv * c.n_rb;
-  if (units64 >= ((int64_t)1 << 31)) { set_error("more cached pages than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
-  const int units = (int)units64;
+  seqs[(size_t)groups] = TreeSeq{0, 0, 0, 0, 0, (int32_t)units64};
+  const int units = (int)(units64 * Hkv);
   const int workers = std::max(1, std::min(p->dev->sm_count, units / (kFixUnits + 1)));
   const size_t part_rows = (size_t)2 * workers * c.rows_rb;
   int32_t rc = grow(p->dev, p->part_o, part_rows * (kD + 2) * sizeof(float));
   if (rc) return rc;
-  if (seqs != inl) {
-    size_t bytes = sizeof(TreeSeq) * ((size_t)n + 1);
-    const size_t tree_bytes = (size_t)kTreeNodes * (tree.one ? 1 : n);
-    memcpy((char*)seqs + bytes, tree.parents, tree_bytes);
-    bytes += tree_bytes;
+  if (groups > kInlineLarge) {
+    if (stream_captured(p->dev)) {   // the list is this call's
+      set_error("a call of %lld groups of query rows cannot be captured (%d can)", (long long)groups, kInlineLarge);
+      return RELUX_ERR_UNSUPPORTED;
+    }
+    const size_t list = sizeof(TreeSeq) * seqs.size(), bytes = list + (tree ? (size_t)kTreeNodes * (tree->one ? 1 : n) : 0);
     if ((rc = grow(p->dev, p->seq_list, bytes))) return rc;
-    RELUX_CUDA_TRY(cudaMemcpyAsync(p->seq_list.p, seqs, bytes, cudaMemcpyHostToDevice, p->dev->stream));
-    if ((rc = stage_release(p, slot_index))) return rc;
+    // (pageable memory: the copies have read it when they return)
+    RELUX_CUDA_TRY(cudaMemcpyAsync(p->seq_list.p, seqs.data(), list, cudaMemcpyHostToDevice, p->dev->stream));
+    if (tree) RELUX_CUDA_TRY(cudaMemcpyAsync((char*)p->seq_list.p + list, tree->parents, bytes - list, cudaMemcpyHostToDevice, p->dev->stream));
     c.seqs = (const TreeSeq*)p->seq_list.p;
-    c.parents = (const int8_t*)(c.seqs + n + 1);
+    c.parents = (const int8_t*)(c.seqs + seqs.size());
   }
-  c.one_tree = tree.one;
+  c.one_tree = tree && tree->one;
+  c.tree = tree != nullptr;
+  c.causal = a.causal;
   c.table = p->d_table;
   c.table_stride = prm.max_pages_per_seq;
   c.num_pages = prm.num_pages;
@@ -1009,8 +1037,8 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.Hkv = Hkv;
   c.H = a.num_heads;
   c.g = g;
-  c.S = a.q_tokens;
-  c.R = R;
+  c.S = S;
+  c.R = (int)R;
   const int64_t rows_per_block = (int64_t)prm.num_pages * Hkv * kPage;
   c.krow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block);
   c.vrow0 = (int32_t)((int64_t)a.layer * 2 * rows_per_block + rows_per_block);
@@ -1027,7 +1055,7 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.part_ml = c.part_o + part_rows * kD;
   c.status = p->d_status;
   c.time = time_stamp_next(p, p->attn_times);
-  rc = n <= kInlineSmall || c.seqs ? launch_n<kInlineSmall>(p, c, seqs, tree.parents, workers) : launch_n<kInlineLarge>(p, c, seqs, tree.parents, workers);
+  rc = groups <= kInlineSmall || c.seqs ? launch_n<kInlineSmall>(p, c, seqs.data(), tree, workers) : launch_n<kInlineLarge>(p, c, seqs.data(), tree, workers);
   if (rc) return rc;
   time_stamp_done(p->attn_times, c.time);
   return RELUX_OK;

@@ -250,8 +250,8 @@ bool gqa_stream_eligible(const Pool* p, const relux_attn_args& a);
 bool gqa_append_fusable(const Pool* p, const relux_attn_args& a, int max_new_rows, bool advance);
 int32_t launch_gqa_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16,
                           const GqaAppend* app, const GqaTree* tree = nullptr);
-// More than 32 query rows a kv head (gqa_tree_sm100.cu); nodes: host, drafted rows of every sequence, which are in the cache.
-int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16, const GqaTree& tree,
+// More than 32 query rows a kv head of a tree, or over an 8-bit cache (gqa_tree_sm100.cu); nodes: host, drafted rows of every sequence, which are in the cache.
+int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16, const GqaTree* tree,
                               const int32_t* nodes);
 // Rows of either grouped-query cache read back, the commit of a tree's path (gqa_rows.cu).
 int32_t launch_read_kv(Pool* p, const SeqBatch& sb, int layer0, int layers, const int32_t* tok0, const int32_t* n, int dtype, void* k_out, void* v_out);

@@ -543,6 +543,7 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
     set_error("a pool of 8-bit rows takes RELUX_ATTN_FAST only");
     return RELUX_ERR_UNSUPPORTED;
   }
+  const bool q8 = p->int8 && kind == RELUX_POOL_GQA;
   if (!(a->scale > 0.f)) { set_error("scale=%g, must be > 0", (double)a->scale); return RELUX_ERR_INVALID_ARG; }
   if (a->flags & ~RELUX_CALL_PIPELINED) { set_error("unknown call flags 0x%x", a->flags); return RELUX_ERR_INVALID_ARG; }
   if (a->q_mem == RELUX_MEM_DEVICE) {
@@ -608,7 +609,7 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
   const size_t out_elems = (size_t)n * S * H * D;
   const bool out_tm = a->out_layout == RELUX_LAYOUT_TOKEN_MAJOR || S == 1;
   const bool k_bf16 = a->out_dtype == RELUX_DTYPE_BF16 && out_tm &&
-                      (gqa_stream || (kind == RELUX_POOL_MLA && a->mode == RELUX_ATTN_FAST && mla_writes_bf16(p, sb, *a)));
+                      (gqa_stream || q8 || (kind == RELUX_POOL_MLA && a->mode == RELUX_ATTN_FAST && mla_writes_bf16(p, sb, *a)));
   const int k_dtype = k_bf16 ? RELUX_DTYPE_BF16 : RELUX_DTYPE_F32;
   const bool need_conv = a->out_dtype != k_dtype || !out_tm;
   const bool direct = a->out_mem == RELUX_MEM_DEVICE && !need_conv;
@@ -644,6 +645,8 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
   if (a->mode != RELUX_ATTN_FAST) {
     rc = (kind == RELUX_POOL_MLA) ? launch_attn_reference_mla(p, sb, aa, (const float*)dq, (const float*)dqr, (float*)kout)
                                   : launch_attn_reference_gqa(p, sb, aa, (const float*)dq, (float*)kout);
+  } else if ((tree || q8) && !gqa_stream_eligible(p, aa)) {
+    rc = launch_gqa_tree_sm100(p, sb, aa, dq, kout, k_bf16, tree, tree ? gstep->rows : nullptr);
   } else if (gqa_stream) {
     rc = launch_gqa_stream(p, sb, aa, dq, kout, k_bf16, gstep, tree);
   } else {

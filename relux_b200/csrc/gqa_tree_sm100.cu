@@ -67,13 +67,14 @@ struct TreeCommon {
   int32_t causal;
   const int32_t* table;
   int32_t table_stride, num_pages, n_seqs, range, range_more, Hkv, H, g, S, R;
+  uint32_t over_g;             // 2^31 / g, rounded up: a row below 2^26 over g is a product (a division by g a row was half of a piece's fixed cost)
   int32_t n_rb, rows_rb;       // groups of a sequence, rows of each (the last may have fewer)
   int32_t krow0, vrow0;
   const float* scales;         // 8-bit cache: of the layer
   const uint8_t* codes;        // and the pool's rows
   float scale_log2;
-  const void* q;
-  int32_t q_bf16, out_bf16;
+  const uint16_t* q;           // bf16
+  int32_t out_bf16;
   void* out;
   float* part_o;               // [2 * workers][rows_rb][128]
   float* part_ml;              // [2 * workers][rows_rb][2]
@@ -84,8 +85,10 @@ template <int N>
 struct TreeParams {
   TreeCommon c;
   TreeSeq seqs[N + 1];
-  int8_t parents[N][kTreeNodes];
+  alignas(2) int8_t parents[N][kTreeNodes];
 };
+
+__device__ __forceinline__ int token_of(const TreeCommon& c, int row) { return (int)__umulhi(2u * (uint32_t)row, c.over_g); }
 
 // The streams as every role walks them: pieces of this range, in order.  Sequence by sequence, kv head by kv head, group by group: the groups of a kv head
 // read the same tiles.
@@ -161,7 +164,13 @@ struct Bars {
   uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
   uint32_t bad_all[4];         // (8-bit cache) a cached row with one
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
-  float4 halves[2][64];        // (two) a row's max, sum and unit of O, of either half of the warps
+  union {
+    uint64_t see[256];         // what a row sees: of the nodes (a bit each), or how many tokens from len0 on
+    struct {
+      uint64_t of_one[128];    // (one block)
+      float halves[2][3][64];  // (two) a row's max, sum and unit of O, of either half of the warps
+    };
+  };
   alignas(16) uint32_t v_scale[4][kTile];   // (8-bit cache) of a tile's values, over their unit, binary16 twice
   alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys.  Without an 8-bit cache there is no room for these two, nor with two blocks for `halves`
 };
@@ -180,12 +189,12 @@ struct Plan {
   static constexpr int kRawAt = kRingV + kSlotsV * kHalf;
   static constexpr int kScaleAt = kRawAt + kRaw * kRawSlot;
   static constexpr int kBars = kScaleAt + kScaleSlots * 1024;
-  static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, halves));
+  static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, see) + sizeof(Bars::see));
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
   static constexpr int kWarpLoad = kSoftmaxWarps + (kI8 ? 2 * kConvWarps : 0), kWarpMma = kWarpLoad + 1;
   // Four more warps where registers are dealt out anew, which warps do by fours: softmax 152, converters 64, the others 48 of the 96 of the launch.
   static constexpr int kThreads = 32 * (kI8 ? kWarpLoad + 4 : kWarpMma + 1);
-  static constexpr int kRegsSoftmax = 152, kRegsConv = 64, kRegsOther = 48;
+  static constexpr int kRegsSoftmax = 144, kRegsConv = 64, kRegsOther = 64;
   static_assert(!kI8 || 256 * kRegsSoftmax + 256 * kRegsConv + 128 * kRegsOther <= 640 * 96, "more registers than the block is launched with");
 };
 // The wait that gives up raises the flag, which ends all others; the kernel's end reports it.  Short, and not a function of its own: a call takes registers that
@@ -487,251 +496,263 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     // =============================== softmax ===============================
     // Warp w reads TMEM lanes 32 (w & 3) .. +31 (the hardware's rule), of which warps w and w + 4 take 16 each: rows 16 w .. 16 w + 15 of a block.
     // Few rows then keep all four schedulers busy.  (two: both take the same 16.)
+    // A lane works on two rows of a block, row_in and row_in + 8.  With two blocks their states change places after every step, so that the code is there once.
     regs_up<PL::kRegsSoftmax, kI8>();
     const int set = two ? warp >> 2 : 0, row_warp = two ? warp & 3 : warp;
-    const int r16 = (warp & 3) * 32 + (two ? 0 : (warp >> 2) * 16);
+    const int r16 = (warp & 3) * 32 + (two ? 0 : (warp >> 2) * 16), row_in = 16 * row_warp + (lane >> 2);
     const uint32_t lane_addr = (uint32_t)r16 << 16;
-    int k = 0, tt = 0, n = 0;
+    int k0 = 0, tt0 = 0, n = 0;   // steps, tiles and pieces before this one
     for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
       const TreeSeq sq = streams.seq(p.e);
-      const int nb = blocks_of(sq), rows = rows_of(sq), kvh = p.kvh, row_base = sq.row0;
-      uint64_t see[kNB][2];
-      float q_scale[kNB][2];
-      // ---- queries in ----
-#pragma unroll
-      for (int b = 0; b < kNB; b++) {
-        if (b >= nb) continue;
-        {   // what this warp's rows see of the nodes, or how many tokens from len0 on: a row per lane, then to the lanes that work on it
-          const int r = 128 * b + 16 * row_warp + (lane & 15), s = (row_base + r) / c.g, tree = c.one_tree ? 0 : sq.i;
-          uint64_t m = 0;
-          if (!c.tree) {
-            m = c.causal ? s - row_base / c.g : 0;
-          } else if (r < rows && s < sq.end - sq.len0) {
-            for (int j = s; j >= 0; j = c.seqs ? c.parents[tree * kTreeNodes + j] : prm.parents[tree][j]) m |= 1ull << j;
-          }
-#pragma unroll
-          for (int hf = 0; hf < 2; hf++) see[b][hf] = __shfl_sync(0xffffffffu, (unsigned long long)m, (lane >> 2) + 8 * hf);
+      const int nb = blocks_of(sq), rows = rows_of(sq), tiles = p.te - p.tb;
+      struct State {
+        float m[2], l[2], f[2];   // running max, sum, what a score is multiplied by
+      } st, other;
+      auto next_block = [&] {
+        if (kNB == 2 && nb == 2) {
+          const State t = st;
+          st = other;
+          other = t;
         }
-        q_scale[b][0] = q_scale[b][1] = c.scale_log2;
+      };
+      // ---- queries in: copies straight to the matrix operand's place ----
 #pragma unroll 4
-        for (int i = 0; i < 8; i++) {   // 16 lanes a row, two rows at a time
-          const int j = 2 * i + (lane >> 4), r = 128 * b + 16 * row_warp + j, ch = (lane & 15) * 8;
-          const int s = (row_base + r) / c.g, hq = row_base + r - s * c.g;
-          const size_t off = (((size_t)sq.i * c.S + s) * c.H + (size_t)kvh * c.g + hq) * kD + ch;
-          uint8_t* dst = smem + PL::kQ + b * kSlot + (ch >> 6) * kHalf + swz128(r16 + j, (ch & 63) >> 3);
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if constexpr (kI8) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = 0.f;
-            if (r < rows) {
-              if (c.q_bf16) load8(x, reinterpret_cast<const uint16_t*>(c.q) + off);
-              else load8(x, reinterpret_cast<const float*>(c.q) + off);
-            }
-            float up, down;
-            query_factor(row_top(x), up, down);
-            uint32_t y[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = pack_p<true>(x[2 * e] * up, x[2 * e + 1] * up);
-            w = make_uint4(y[0], y[1], y[2], y[3]);
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-              const float f = __shfl_sync(0xffffffffu, down, ((lane >> 2) & 1) * 16);
-              if (((lane >> 2) + 8 * hf) >> 1 == i) q_scale[b][hf] = c.scale_log2 * f;
-            }
-          } else if (r < rows) {
-            if (c.q_bf16) {
-              w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(c.q) + off);
-            } else {
-              float x[8];
-              load8(x, reinterpret_cast<const float*>(c.q) + off);
-              w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+      for (int i = 0; i < (set == 0 ? 8 * nb : 0); i++) {   // 16 lanes a row
+        const int b = kNB == 2 ? i >> 3 : 0, j = (2 * i + (lane >> 4)) & 15, row = 128 * b + 16 * row_warp + j, ch = lane & 15;
+        const bool there = row < rows;
+        const int s = token_of(c, sq.row0 + row), hq = sq.row0 + row - s * c.g;
+        const uint16_t* src = c.q + (there ? (((size_t)sq.i * c.S + s) * c.H + (size_t)p.kvh * c.g + hq) * kD + ch * 8 : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + PL::kQ + b * kSlot + (ch >> 3) * kHalf + swz128(r16 + j, ch & 7))),
+                     "l"(__cvta_generic_to_global(src)), "r"(there ? 16 : 0)
+                     : "memory");
+      }
+      // What the rows see, a row a lane (16).  A tree's parents two a lane, so that a node's way up is one of shuffles.
+      uint32_t up2 = 0xffffu;
+      if (c.tree && 2 * lane < c.S) up2 = reinterpret_cast<const uint16_t*>(c.seqs ? c.parents + (c.one_tree ? 0 : sq.i) * kTreeNodes : prm.parents[c.one_tree ? 0 : sq.i])[lane];
+#pragma unroll 1
+      for (int b = 0; b < nb; b++, next_block()) {
+        const int row = 128 * b + 16 * row_warp + (lane & 15), s = token_of(c, sq.row0 + row);
+        uint64_t see = 0;
+        if (c.tree) {
+          int j = row < rows && s < sq.end - sq.len0 ? s : -1;
+          while (__any_sync(0xffffffffu, j >= 0)) {
+            const uint32_t pair = __shfl_sync(0xffffffffu, up2, (j & 63) >> 1);
+            if (j >= 0) {
+              see |= 1ull << j;
+              j = (int8_t)(pair >> (8 * (j & 1)));
             }
           }
-          if (set == 0) *reinterpret_cast<uint4*>(dst) = w;
+        } else if (c.causal) {
+          see = s - token_of(c, sq.row0);
         }
+        if (lane < 16) bars->see[row] = see;
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          st.m[hf] = -INFINITY;
+          st.l[hf] = 0.f;
+          st.f[hf] = c.scale_log2;
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if constexpr (kI8) {   // in place to binary16, by a power of two a row
+        if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // the other warp of these rows has them from this one
+#pragma unroll 1
+        for (int b = 0; b < nb; b++, next_block())
+#pragma unroll 2
+          for (int i = 0; i < 8; i++) {
+            const int j = 2 * i + (lane >> 4), ch = lane & 15;
+            uint4* at = reinterpret_cast<uint4*>(smem + PL::kQ + b * kSlot + (ch >> 3) * kHalf + swz128(r16 + j, ch & 7));
+            float x[8], up, down;
+            load8(x, reinterpret_cast<const uint16_t*>(at));
+            query_factor(row_top(x), up, down);
+            if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // both have read it
+            if (set == 0) *at = make_uint4(pack_p<true>(x[0] * up, x[1] * up), pack_p<true>(x[2] * up, x[3] * up), pack_p<true>(x[4] * up, x[5] * up), pack_p<true>(x[6] * up, x[7] * up));
+            const float f = __shfl_sync(0xffffffffu, down, ((lane >> 2) & 1) * 16);
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++)
+              if (((lane >> 2) + 8 * hf) >> 1 == i) st.f[hf] = c.scale_log2 * f;
+          }
       }
       fence_proxy_async();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->q_full);
       // ---- tiles ----
-      float m_used[kNB][2], l_run[kNB][2], v_unit = 1.f;
-#pragma unroll
-      for (int b = 0; b < kNB; b++)
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-          m_used[b][hf] = -INFINITY;
-          l_run[b][hf] = 0.f;
-        }
-      const int k0 = k, tt0 = tt, first = two && (k0 & 1) != set ? p.tb + 1 : p.tb;
-      k += (p.te - p.tb) * nb;
-      tt += p.te - p.tb;
+      const int first = two && (k0 & 1) != set ? p.tb + 1 : p.tb;
+      float v_unit = 1.f, shrink = 1.f;   // O's unit, and what it has grown by
 #pragma unroll 1
-      for (int t = first; t < p.te; t += two ? 2 : 1) {
-        const int tile = tt0 + t - p.tb;
+      for (int t = first, b = 0; t < p.te;) {
+        const int tile = tt0 + t - p.tb, step = k0 + (t - p.tb) * nb + b;
         const int from = sq.len0 - t * kTile;   // first drafted row of the tile
-        float shrink = 1.f;                     // what O's unit has grown by
-        const float* k_scale = bars->k_scale[tile & 3];
-        if constexpr (kI8) {
+        if (kI8 && b == 0) {
           wait_bar(&bars->info[tile & 3], (tile >> 2) & 1, bars);
           const float unit = bars->v_unit[tile & 3];
-          if (t > first) shrink = v_unit / unit;
+          shrink = t > first ? v_unit / unit : 1.f;
           v_unit = unit;
         }
+        const uint32_t tmem_s = tmem + lane_addr + (step & 1) * 128, tmem_o = tmem + lane_addr + kTmemO + (two ? set : b) * 128;
+        wait_bar(&bars->s_full[step & 1], (step >> 1) & 1, bars);
+        if (128 * b + 16 * row_warp < rows) {   // else the whole warp's rows are none
+          tc_fence_after();
+          uint32_t sv[64];
+          tmem_ld_16x256b_x16(tmem_s, sv);
+          tmem_ld_wait();
+          if constexpr (kI8) {
+            const float* k_scale = bars->k_scale[tile & 3];
 #pragma unroll
-        for (int b = 0; b < kNB; b++) {
-          if (b >= nb) continue;
-          const int step = k0 + (t - p.tb) * nb + b;
-          const uint32_t tmem_s = tmem + lane_addr + (step & 1) * 128, tmem_o = tmem + lane_addr + kTmemO + (two ? set : b) * 128;
-          wait_bar(&bars->s_full[step & 1], (step >> 1) & 1, bars);
-          if (128 * b + 16 * row_warp < rows) {   // else the whole warp's rows are none
-            tc_fence_after();
-            uint32_t sv[64];
-            tmem_ld_16x256b_x16(tmem_s, sv);
-            tmem_ld_wait();
-            if constexpr (kI8) {
-#pragma unroll
-              for (int i = 0; i < 16; i++) {
-                const float2 s = *reinterpret_cast<const float2*>(k_scale + 8 * i + 2 * (lane & 3));
-                const uint64_t s2 = pack2(s.x, s.y);
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                  float x0, x1;
-                  unpack2(mul2(pack2(__uint_as_float(sv[4 * i + 2 * hf]), __uint_as_float(sv[4 * i + 2 * hf + 1])), s2), x0, x1);
-                  sv[4 * i + 2 * hf] = __float_as_uint(x0);
-                  sv[4 * i + 2 * hf + 1] = __float_as_uint(x1);
-                }
-              }
-            }
-            const bool whole = from >= kTile;
-            if (!whole) {
+            for (int i = 0; i < 16; i++) {
+              const float2 s = *reinterpret_cast<const float2*>(k_scale + 8 * i + 2 * (lane & 3));
+              const uint64_t s2 = pack2(s.x, s.y);
 #pragma unroll
               for (int hf = 0; hf < 2; hf++) {
-                uint32_t hidden = 0;   // bit 2 i + e: key 8 i + 2 (lane & 3) + e
-#pragma unroll 1
-                for (int i = 31; i >= 0; i--) {
-                  const int node = 8 * (i >> 1) + 2 * (lane & 3) + (i & 1) - from;
-                  hidden = hidden << 1 | (!c.tree ? node >= (int)see[b][hf] : node >= kTreeNodes || (node >= 0 && !(see[b][hf] >> node & 1u)));
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++)
-                  if (hidden & (1u << i)) sv[4 * (i >> 1) + 2 * hf + (i & 1)] = 0xFF800000u;   // -inf
+                float x0, x1;
+                unpack2(mul2(pack2(__uint_as_float(sv[4 * i + 2 * hf]), __uint_as_float(sv[4 * i + 2 * hf + 1])), s2), x0, x1);
+                sv[4 * i + 2 * hf] = __float_as_uint(x0);
+                sv[4 * i + 2 * hf + 1] = __float_as_uint(x1);
               }
             }
-            // row maxima of the raw scores: four chains of three-input maxima
-            float mx[2];
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-              float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-              for (int i = 0; i < 16; i++) m4[i & 3] = max3(m4[i & 3], __uint_as_float(sv[4 * i + 2 * hf]), __uint_as_float(sv[4 * i + 2 * hf + 1]));
-              mx[hf] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * q_scale[b][hf];
-            }
-            float alpha[2] = {shrink, shrink};
-            bool rescale = kI8 && shrink != 1.f;
-            if (__any_sync(0xffffffffu, mx[0] > m_used[b][0] + kRescaleThreshold || mx[1] > m_used[b][1] + kRescaleThreshold)) {
-#pragma unroll
-              for (int o = 1; o < 4; o <<= 1)
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++) mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], o));
-#pragma unroll
-              for (int hf = 0; hf < 2; hf++)
-                if (mx[hf] > m_used[b][hf] + kRescaleThreshold) {
-                  if (m_used[b][hf] != -INFINITY) {
-                    const float a = ex2_approx(m_used[b][hf] - mx[hf]);
-                    alpha[hf] *= a;
-                    l_run[b][hf] *= a;
-                    rescale = true;
-                  }
-                  m_used[b][hf] = mx[hf];
-                }
-            }
-            uint64_t factor2[2], neg_m2[2], ps2[2];
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-              const float neg_m = (m_used[b][hf] == -INFINITY ? 0.f : -m_used[b][hf]) + (kI8 ? kPUp : 0.f);
-              factor2[hf] = pack2(q_scale[b][hf], q_scale[b][hf]);
-              neg_m2[hf] = pack2(neg_m, neg_m);
-              ps2[hf] = pack2(0.f, 0.f);
-            }
-            uint32_t pw[32];
-            // With two blocks the special-function unit is what exponentials wait for; else the instruction cache is (see wait_bar).  ex2(-inf) is 0, the
-            // polynomial's is not.
-            if (kNB == 2 && whole) exp_scores<kI8, true>(sv, factor2, neg_m2, pw, ps2);
-            else exp_scores<kI8, false>(sv, factor2, neg_m2, pw, ps2);
-            tmem_st_16x128b_x16(tmem_s, pw);
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-              float ps0, ps1;
-              unpack2(ps2[hf], ps0, ps1);
-              l_run[b][hf] += ps0 + ps1;
-            }
-            // O may be rescaled only behind the PV before this one on it.  With two blocks, or two halves, that is the one before QK(k) in the pipe, else
-            // PV(k - 1), which QK(k) was ahead of: `pv` has then completed k - 1 or k phases, so its parity is no riddle.
-            if (t > first && __any_sync(0xffffffffu, rescale)) {
-              if (nb == 1 && !two) {
-                wait_bar(&bars->pv, (step - 1) & 1, bars);
-                tc_fence_after();
-              }
-#pragma unroll 1
-              for (int col = 0; col < kD; col += 64) {
-                uint32_t ov[32];
-                tmem_ld_16x256b_x8(tmem_o + col, ov);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha[(i >> 1) & 1]);
-                tmem_st_16x256b_x8(tmem_o + col, ov);
-              }
-            }
-            tmem_st_wait();
-            tc_fence_before();
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->p_full[step & 1]);
+          const bool whole = from >= kTile;
+          if (!whole) {
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              const uint64_t see = bars->see[128 * b + row_in + 8 * hf];
+              const int all = c.tree ? from : from + (int)see;   // keys below it are seen, and of the nodes some
+              const uint64_t some = c.tree ? see : 0;
+#pragma unroll
+              for (int w = 0; w < 4; w++) {
+                const int sh = all - 32 * w;   // bit i of `shown`: key 32 w + i
+                uint32_t shown = sh >= 32 ? 0xffffffffu : sh >= 0 ? (uint32_t)(some << sh) | ((1u << sh) - 1u) : sh > -64 ? (uint32_t)(some >> -sh) : 0u;
+                shown >>= 2 * (lane & 3);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                  if (!(shown >> (8 * (i >> 1) + (i & 1)) & 1u)) sv[16 * w + 4 * (i >> 1) + 2 * hf + (i & 1)] = 0xFF800000u;   // -inf
+              }
+            }
+          }
+          // row maxima of the raw scores: four chains of three-input maxima
+          float mx[2];
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 16; i++) m4[i & 3] = max3(m4[i & 3], __uint_as_float(sv[4 * i + 2 * hf]), __uint_as_float(sv[4 * i + 2 * hf + 1]));
+            mx[hf] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * st.f[hf];
+          }
+          float alpha[2] = {shrink, shrink};
+          bool rescale = kI8 && shrink != 1.f;
+          if (__any_sync(0xffffffffu, mx[0] > st.m[0] + kRescaleThreshold || mx[1] > st.m[1] + kRescaleThreshold)) {
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+              for (int hf = 0; hf < 2; hf++) mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], o));
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++)
+              if (mx[hf] > st.m[hf] + kRescaleThreshold) {
+                if (st.m[hf] != -INFINITY) {
+                  const float a = ex2_approx(st.m[hf] - mx[hf]);
+                  alpha[hf] *= a;
+                  st.l[hf] *= a;
+                  rescale = true;
+                }
+                st.m[hf] = mx[hf];
+              }
+          }
+          uint64_t factor2[2], neg_m2[2], ps2[2];
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            const float neg_m = (st.m[hf] == -INFINITY ? 0.f : -st.m[hf]) + (kI8 ? kPUp : 0.f);
+            factor2[hf] = pack2(st.f[hf], st.f[hf]);
+            neg_m2[hf] = pack2(neg_m, neg_m);
+            ps2[hf] = pack2(0.f, 0.f);
+          }
+          uint32_t pw[32];
+          // With two blocks the special-function unit is what exponentials wait for; else the instruction cache is (see wait_bar).  ex2(-inf) is 0, the
+          // polynomial's is not.
+          if (kNB == 2 && whole) exp_scores<kI8, true>(sv, factor2, neg_m2, pw, ps2);
+          else exp_scores<kI8, false>(sv, factor2, neg_m2, pw, ps2);
+          tmem_st_16x128b_x16(tmem_s, pw);
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            float ps0, ps1;
+            unpack2(ps2[hf], ps0, ps1);
+            st.l[hf] += ps0 + ps1;
+          }
+          // O may be rescaled only behind the PV before this one on it.  With two blocks, or two halves, that is the one before QK(k) in the pipe, else
+          // PV(k - 1), which QK(k) was ahead of: `pv` has then completed k - 1 or k phases, so its parity is no riddle.
+          if (t > first && __any_sync(0xffffffffu, rescale)) {
+            if (nb == 1 && !two) {
+              wait_bar(&bars->pv, (step - 1) & 1, bars);
+              tc_fence_after();
+            }
+#pragma unroll 1
+            for (int col = 0; col < kD; col += 64) {
+              uint32_t ov[32];
+              tmem_ld_16x256b_x8(tmem_o + col, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha[(i >> 1) & 1]);
+              tmem_st_16x256b_x8(tmem_o + col, ov);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
         }
-        if (kI8 && lane == 0) mbar_arrive(&bars->info_empty[tile & 3]);
+        __syncwarp();
+        const bool last = b + 1 == nb;
+        if (lane == 0) {
+          mbar_arrive(&bars->p_full[step & 1]);
+          if (kI8 && last) mbar_arrive(&bars->info_empty[tile & 3]);
+        }
+        next_block();
+        b = last ? 0 : b + 1;
+        if (last) t += two ? 2 : 1;
       }
-      // ---- results out ----
+      k0 += tiles * nb;
+      tt0 += tiles;
+      // ---- results out: through the queries' place, which nothing reads any more, to whole lines ----
       wait_bar(&bars->fin, n & 1, bars);
       tc_fence_after();
       const bool ok = bars->abort_flag == 0;
       const uint64_t bad_nodes = bars->bad_nodes[n & 3];
-      const bool bad_all = bars->bad_all[n & 3] != 0;
-      const bool stream_whole = p.tb == 0 && p.te == p.tiles;
+      const bool bad_all = bars->bad_all[n & 3] != 0, whole = p.tb == 0 && p.te == p.tiles;
       const int slot = 2 * (int)blockIdx.x + (p.us + p.tb == streams.u_begin ? 0 : 1);
-#pragma unroll
-      for (int b = 0; b < kNB; b++) {
-        if (b >= nb || 128 * b + 16 * row_warp >= rows) continue;
+#pragma unroll 1
+      for (int b = 0; b < nb; b++, next_block()) {
+        if (128 * b + 16 * row_warp >= rows) continue;
         float f[2], f2[2] = {0.f, 0.f};   // of this O, and (two) of the other half's
-        int r[2], s[2];
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
-          float l = l_run[b][hf], m = m_used[b][hf], w = v_unit;
+          float l = st.l[hf], m = st.m[hf], w = v_unit;
           l += __shfl_xor_sync(0xffffffffu, l, 1);
           l += __shfl_xor_sync(0xffffffffu, l, 2);
           if (two) {   // every row has been through one half or the other, or both
-            const int x = 16 * row_warp + 8 * hf + (lane >> 2);
-            if ((lane & 3) == 0) bars->halves[set][x] = make_float4(m, l, v_unit, 0.f);
-            asm volatile("bar.sync %0, 64;" ::"r"(2 + row_warp) : "memory");   // the two warps of these rows
-            const float4 o = bars->halves[set ^ 1][x];
-            const float top = fmaxf(m, o.x), w0 = m == -INFINITY ? 0.f : ex2_approx(m - top), w1 = o.x == -INFINITY ? 0.f : ex2_approx(o.x - top);
-            l = l * w0 + o.y * w1;
+            const int x = row_in + 8 * hf;
+            if ((lane & 3) == 0) {
+              bars->halves[set][0][x] = m;
+              bars->halves[set][1][x] = l;
+              bars->halves[set][2][x] = v_unit;
+            }
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // the two warps of these rows
+            const float o_m = bars->halves[set ^ 1][0][x], o_l = bars->halves[set ^ 1][1][x];
+            const float top = fmaxf(m, o_m), w0 = m == -INFINITY ? 0.f : ex2_approx(m - top), w1 = o_m == -INFINITY ? 0.f : ex2_approx(o_m - top);
+            l = l * w0 + o_l * w1;
             w *= w0;
-            f2[hf] = o.z * w1;
+            f2[hf] = bars->halves[set ^ 1][2][x] * w1;
             m = top;
           }
-          if (bad_all || (c.tree ? (see[b][hf] & bad_nodes) != 0 : bad_nodes != 0 && (int)see[b][hf] > (int)~(uint32_t)bad_nodes)) l = __uint_as_float(0x7FC00000u);
-          r[hf] = 128 * b + 16 * row_warp + 8 * hf + (lane >> 2);
-          s[hf] = (row_base + r[hf]) / c.g;
-          const bool there = ok && (!c.tree || s[hf] < sq.end - sq.len0);
+          const int row = 128 * b + row_in + 8 * hf;
+          const uint64_t see = bars->see[row];
+          if (bad_all || (c.tree ? (see & bad_nodes) != 0 : bad_nodes != 0 && (int)see > (int)~(uint32_t)bad_nodes)) l = __uint_as_float(0x7FC00000u);
+          const bool there = ok && row < rows && (!c.tree || token_of(c, sq.row0 + row) < sq.end - sq.len0);
           // no part of a sum that nobody has added to, of a row that is not there: zero whatever the accumulator holds
-          const float inv = !there ? 0.f : !stream_whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-          f[hf] = m_used[b][hf] == -INFINITY && l == l ? 0.f : w * inv;
+          const float inv = !there ? 0.f : !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+          f[hf] = st.m[hf] == -INFINITY && l == l ? 0.f : w * inv;
           f2[hf] *= inv;
-          if (!stream_whole && (lane & 3) == 0 && set == 0 && r[hf] < rows)
-            *reinterpret_cast<float2*>(c.part_ml + ((size_t)slot * c.rows_rb + r[hf]) * 2) = there ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+          if (!whole && (lane & 3) == 0 && set == 0 && row < rows)
+            *reinterpret_cast<float2*>(c.part_ml + ((size_t)slot * c.rows_rb + row) * 2) = there ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         }
+        uint8_t* place = smem + PL::kQ + b * kSlot + (r16 + 16 * set) * 128;   // 16 rows of 32 + 32 columns
 #pragma unroll 1
         for (int col = two ? 64 * set : 0; col < (two ? 64 * set + 64 : kD); col += 64) {   // two: a half of the columns each
           uint32_t ov[32];
@@ -747,19 +768,24 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             for (int i = 0; i < 32; i++)
               if (f2[(i >> 1) & 1] != 0.f) ov[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), f2[(i >> 1) & 1], __uint_as_float(ov[i])));
           }
+          __syncwarp();   // the columns before these have been read
 #pragma unroll
-          for (int hf = 0; hf < 2; hf++) {
-            if (r[hf] >= rows) continue;
-            const size_t at = stream_whole ? ((((size_t)sq.i * c.S + s[hf]) * c.H + (size_t)kvh * c.g + (row_base + r[hf] - s[hf] * c.g)) * kD)
-                                           : ((size_t)slot * c.rows_rb + r[hf]) * kD;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const int d = col + 8 * i + 2 * (lane & 3);
-              const float x0 = __uint_as_float(ov[4 * i + 2 * hf]), x1 = __uint_as_float(ov[4 * i + 2 * hf + 1]);
-              if (!stream_whole) *reinterpret_cast<float2*>(c.part_o + at + d) = make_float2(x0, x1);
-              else if (c.out_bf16) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(c.out) + at + d) = pack_bf16x2(x0, x1);
-              else *reinterpret_cast<float2*>(reinterpret_cast<float*>(c.out) + at + d) = make_float2(x0, x1);
-            }
+          for (int i = 0; i < 16; i++) {   // columns 8 (i >> 1) + 2 (lane & 3) + {0, 1} of row (lane / 4) + 8 (i & 1)
+            const int r = (lane >> 2) + 8 * (i & 1), chunk = 2 * ((i >> 1) & 3) + ((lane >> 1) & 1);
+            *reinterpret_cast<float2*>(place + (i >> 3) * kHalf + r * 128 + ((chunk ^ (r & 7)) << 4) + (lane & 1) * 8) =
+                make_float2(__uint_as_float(ov[2 * i]), __uint_as_float(ov[2 * i + 1]));
+          }
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < 8; i++) {   // 16 lanes a row, four columns each
+            const int r = 2 * i + (lane >> 4), row = 128 * b + 16 * row_warp + r, ch = lane & 15;
+            if (row >= rows) continue;
+            const float4 o = *reinterpret_cast<const float4*>(place + (ch >> 3) * kHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+            const int s = token_of(c, sq.row0 + row);
+            const size_t at = (whole ? (((size_t)sq.i * c.S + s) * c.H + (size_t)p.kvh * c.g + (sq.row0 + row - s * c.g)) * kD : ((size_t)slot * c.rows_rb + row) * kD) + col + 4 * ch;
+            if (!whole) *reinterpret_cast<float4*>(c.part_o + at) = o;
+            else if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+            else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = o;
           }
         }
       }
@@ -769,6 +795,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
+      if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // before the next piece's queries come to the place of the other warp's results
     }
   } else if constexpr (kI8) {
     if (warp > kWarpScale) {
@@ -947,7 +974,7 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(const __grid_constant__
       }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int row = sq.row0 + r, s = row / c.g;
+  const int row = sq.row0 + r, s = token_of(c, row);
   const size_t at = (((size_t)sq.i * c.S + s) * c.H + (size_t)p.kvh * c.g + (row - s * c.g)) * kD + 4 * lane;
   if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
   else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -980,7 +1007,7 @@ int32_t launch_n(Pool* p, const TreeCommon& c, const TreeSeq* seqs, const GqaTre
 
 }  // namespace
 
-// q: device [n][S][H][128] token-major (f32 or bf16).  out: device, same shape, f32 or bf16.  All rows are in the cache.  tree: with `nodes`, host, those of
+// q: device bf16 [n][S][H][128] token-major.  out: device, same shape, f32 or bf16.  All rows are in the cache.  tree: with `nodes`, host, those of
 // every sequence, which lie behind its length; nullptr: the call's own mask (causal or none).
 int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args& a, const void* d_q, void* d_out, bool out_bf16, const GqaTree* tree,
                               const int32_t* nodes) {
@@ -992,7 +1019,7 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.rows_rb = (int)((R + c.n_rb - 1) / c.n_rb + 15) / 16 * 16;
   c.n_rb = (int)((R + c.rows_rb - 1) / c.rows_rb);
   const int64_t groups = (int64_t)n * c.n_rb;
-  if (R >= ((int64_t)1 << 30) || groups >= ((int64_t)1 << 24)) { set_error("more query rows than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
+  if (R >= ((int64_t)1 << 26) || groups >= ((int64_t)1 << 24)) { set_error("more query rows than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
   std::vector<TreeSeq> seqs((size_t)groups + 1);
   int64_t units64 = 0;
   for (int i = 0; i < n; i++) {
@@ -1037,6 +1064,7 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.Hkv = Hkv;
   c.H = a.num_heads;
   c.g = g;
+  c.over_g = (uint32_t)((((uint64_t)1 << 31) + g - 1) / g);
   c.S = S;
   c.R = (int)R;
   const int64_t rows_per_block = (int64_t)prm.num_pages * Hkv * kPage;
@@ -1047,8 +1075,7 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
     c.codes = (const uint8_t*)p->storage;
   }
   c.scale_log2 = a.scale * 1.4426950408889634f;
-  c.q = d_q;
-  c.q_bf16 = a.q_dtype == RELUX_DTYPE_BF16;
+  c.q = (const uint16_t*)d_q;
   c.out_bf16 = out_bf16;
   c.out = d_out;
   c.part_o = (float*)p->part_o.p;

@@ -585,7 +585,8 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
   // canonical kernel input: token-major; f32 for REFERENCE, caller's dtype for FAST
   int want_dtype = (a->mode != RELUX_ATTN_FAST) ? RELUX_DTYPE_F32 : a->q_dtype;
   // a GQA prompt goes to the tcgen05 prefill kernel, whose Q tile is a TMA load of bf16 rows
-  if (kind == RELUX_POOL_GQA && a->mode == RELUX_ATTN_FAST && !tree && gqa_prompt_wants_bf16(p, *a)) want_dtype = RELUX_DTYPE_BF16;
+  const bool rows_sm100 = (tree || q8) && !gqa_stream_eligible(p, *a);   // to the tcgen05 kernel of trees and 8-bit prompts
+  if (rows_sm100 || (kind == RELUX_POOL_GQA && a->mode == RELUX_ATTN_FAST && !tree && gqa_prompt_wants_bf16(p, *a))) want_dtype = RELUX_DTYPE_BF16;
   // so does an MLA prompt (expanded keys / values + the same kernel)
   if (kind == RELUX_POOL_MLA && a->mode == RELUX_ATTN_FAST && mla_prefill_eligible(p, sb, *a)) want_dtype = RELUX_DTYPE_BF16;
   const bool relayout_q = (a->q_layout == RELUX_LAYOUT_HEAD_MAJOR && S > 1) || want_dtype != a->q_dtype;
@@ -645,7 +646,7 @@ static int32_t do_attention(Pool* p, const relux_attn_args* a, int kind, const S
   if (a->mode != RELUX_ATTN_FAST) {
     rc = (kind == RELUX_POOL_MLA) ? launch_attn_reference_mla(p, sb, aa, (const float*)dq, (const float*)dqr, (float*)kout)
                                   : launch_attn_reference_gqa(p, sb, aa, (const float*)dq, (float*)kout);
-  } else if ((tree || q8) && !gqa_stream_eligible(p, aa)) {
+  } else if (rows_sm100) {
     rc = launch_gqa_tree_sm100(p, sb, aa, dq, kout, k_bf16, tree, tree ? gstep->rows : nullptr);
   } else if (gqa_stream) {
     rc = launch_gqa_stream(p, sb, aa, dq, kout, k_bf16, gstep, tree);

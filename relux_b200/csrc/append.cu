@@ -40,9 +40,28 @@ struct AppendGeom {
   uint32_t* done;      // zero between launches; counts finished blocks of the running append
 };
 
+// The sequences of a grouped-query append as kernel arguments: no staging copies and their engine switches in front of the launch (for 16 sequences
+// of uneven length they took 20 us, ten times the append).  N = 0: what AppendGeom points to, or none.
+constexpr int kListMax = 256;
+template <int N>
+struct AppendList {
+  int32_t seq[N], off[N + 1];
+};
+template <>
+struct AppendList<0> {};
+struct AppendSpan {
+  int32_t seq, r0, n;   // pool sequence, first row of the call's, rows
+};
+template <int N>
+__device__ __forceinline__ AppendSpan span_of(const AppendGeom& g, const AppendList<N>& list, int i) {
+  if constexpr (N > 0) return AppendSpan{list.seq[i], list.off[i], list.off[i + 1] - list.off[i]};
+  else return AppendSpan{g.seq_ids ? g.seq_ids[i] : i, g.row_off ? g.row_off[i] : i * g.rows_each, g.row_off ? g.row_off[i + 1] - g.row_off[i] : g.rows_each};
+}
+
 // Length bookkeeping fused into the append: every block reads its sequence's length before it arrives here, so the
 // last block to arrive may advance all lengths (and re-arm the counter for the next launch).  grid.x = n_seqs.
-__device__ __forceinline__ void advance_lengths_by_last_block(const AppendGeom& g) {
+template <int N>
+__device__ __forceinline__ void advance_lengths_by_last_block(const AppendGeom& g, const AppendList<N>& list) {
   if (!g.advance) return;
   __shared__ bool s_last;
   __syncthreads();
@@ -53,8 +72,8 @@ __device__ __forceinline__ void advance_lengths_by_last_block(const AppendGeom& 
   __syncthreads();
   if (!s_last) return;
   for (int i = threadIdx.x; i < (int)gridDim.x; i += blockDim.x) {
-    const int seq = g.seq_ids ? g.seq_ids[i] : i;
-    g.len[seq] = load_chained(g.len + seq) + (g.row_off ? g.row_off[i + 1] - g.row_off[i] : g.rows_each);
+    const AppendSpan sp = span_of(g, list, i);
+    g.len[sp.seq] = load_chained(g.len + sp.seq) + sp.n;
   }
   if (threadIdx.x == 0) *g.done = 0u;
 }
@@ -128,20 +147,18 @@ __global__ void mla_append_kernel(AppendGeom g, uint16_t* __restrict__ layer_bas
     }
   }
   fence_chained_writes();
-  advance_lengths_by_last_block(g);
+  advance_lengths_by_last_block(g, AppendList<0>{});
 }
 
 // GQA: source rows K,V [tok][Hkv][D] (token-major) or [Hkv][n_new][D] per sequence (head-major);
 // destination pages [Hkv][page_tokens][D], K block then V block per layer.
-template <bool kF32>
-__global__ void gqa_append_kernel(AppendGeom g, uint16_t* __restrict__ k_base, uint16_t* __restrict__ v_base,
+template <bool kF32, int N>
+__global__ void gqa_append_kernel(AppendGeom g, const __grid_constant__ AppendList<N> list, uint16_t* __restrict__ k_base, uint16_t* __restrict__ v_base,
                                   const void* __restrict__ ksrc, const void* __restrict__ vsrc, int Hkv, int D, int head_major) {
   chain_release();
   chain_wait();
-  const int i = blockIdx.x;
-  const int seq = g.seq_ids ? g.seq_ids[i] : i;
-  const int r0 = g.row_off ? g.row_off[i] : i * g.rows_each;
-  const int nrows = g.row_off ? g.row_off[i + 1] - r0 : g.rows_each;
+  const AppendSpan sp = span_of(g, list, blockIdx.x);
+  const int seq = sp.seq, r0 = sp.r0, nrows = sp.n;
   const int base_len = load_chained(g.len + seq);
   const int vec_per_head = D / 8, vec_per_tok = Hkv * vec_per_head;
   constexpr int kN = kAhead;
@@ -167,21 +184,40 @@ __global__ void gqa_append_kernel(AppendGeom g, uint16_t* __restrict__ k_base, u
     }
   }
   fence_chained_writes();
-  advance_lengths_by_last_block(g);
+  advance_lengths_by_last_block(g, list);
 }
 
-// The same rows into an 8-bit cache (gqa_int8_parts.cuh): 16 lanes quantise a kv head's row, of K or of V.
+// Eight values of a row as they came.
 template <bool kF32>
-__global__ void gqa_append_int8_kernel(AppendGeom g, uint8_t* k_base, uint8_t* v_base, float* scales, const void* ksrc, const void* vsrc, int Hkv,
-                                       int head_major) {
+struct Raw8 {
+  uint4 w[kF32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* src, size_t elem_off) {
+    const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(src) + elem_off * (kF32 ? 4 : 2));
+    w[0] = load_chained(at);
+    if constexpr (kF32) w[1] = load_chained(at + 1);
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    if constexpr (kF32) {
+      x[0] = __uint_as_float(w[0].x); x[1] = __uint_as_float(w[0].y); x[2] = __uint_as_float(w[0].z); x[3] = __uint_as_float(w[0].w);
+      x[4] = __uint_as_float(w[1].x); x[5] = __uint_as_float(w[1].y); x[6] = __uint_as_float(w[1].z); x[7] = __uint_as_float(w[1].w);
+    } else {
+      x[0] = bf16_lo(w[0].x); x[1] = bf16_hi(w[0].x); x[2] = bf16_lo(w[0].y); x[3] = bf16_hi(w[0].y);
+      x[4] = bf16_lo(w[0].z); x[5] = bf16_hi(w[0].z); x[6] = bf16_lo(w[0].w); x[7] = bf16_hi(w[0].w);
+    }
+  }
+};
+
+// The same rows into an 8-bit cache (gqa_int8_parts.cuh): 16 lanes quantise a kv head's row, of K or of V.  64 registers a thread, so that four blocks
+// of kAhead rows are on an SM, and a block per kAhead rows: what one computes and stores, others load meanwhile (with 106 registers, values held as float32,
+// and blocks of several turns, 8 x 2048 float32 rows of 4 KB took twice as long).
+template <bool kF32, int N>
+__global__ void __launch_bounds__(256, 4) gqa_append_int8_kernel(AppendGeom g, const __grid_constant__ AppendList<N> list, uint8_t* k_base, uint8_t* v_base,
+                                                                 float* scales, const void* ksrc, const void* vsrc, int Hkv, int head_major) {
   chain_release();
   chain_wait();
-  using Src = typename std::conditional<kF32, float, uint16_t>::type;
   constexpr int D = kGqaD;
-  const int i = blockIdx.x;
-  const int seq = g.seq_ids ? g.seq_ids[i] : i;
-  const int r0 = g.row_off ? g.row_off[i] : i * g.rows_each;
-  const int nrows = g.row_off ? g.row_off[i + 1] - r0 : g.rows_each;
+  const AppendSpan sp = span_of(g, list, blockIdx.x);
+  const int seq = sp.seq, r0 = sp.r0, nrows = sp.n;
   const int base_len = load_chained(g.len + seq);
   const int c = (threadIdx.x & 15) * 8;
   constexpr int kN = kAhead;
@@ -190,16 +226,18 @@ __global__ void gqa_append_int8_kernel(AppendGeom g, uint8_t* k_base, uint8_t* v
     pages_of_rows<kN>(g, seq, base_len, r, nrows, pg, tok);
     for (int u = threadIdx.x >> 4; u < 2 * Hkv; u += blockDim.x >> 4) {   // two a warp: all of its lanes or none
       const int which = u >= Hkv, h = u - which * Hkv;
-      float x[kN][8];
+      Raw8<kF32> raw[kN];
 #pragma unroll
       for (int q = 0; q < kN; q++) {
         const size_t src_off = head_major ? ((size_t)r0 * Hkv * D + ((size_t)h * nrows + r + q) * D + c) : (((size_t)(r0 + r + q) * Hkv + h) * D + c);
-        if (pg[q] >= 0) load8(x[q], reinterpret_cast<const Src*>(which ? vsrc : ksrc) + src_off);
+        if (pg[q] >= 0) raw[q].load(which ? vsrc : ksrc, src_off);
       }
 #pragma unroll
       for (int q = 0; q < kN; q++) {
         if (pg[q] < 0) continue;   // the same for the whole block
-        const Int8Row row = int8_quantise(x[q], row_top(x[q]));
+        float x[8];
+        raw[q].values(x);
+        const Int8Row row = int8_quantise(x, row_top(x));
         const size_t head = (size_t)pg[q] * Hkv + h;
         *reinterpret_cast<uint2*>((which ? v_base : k_base) + (head * kGqaPageTok + tok[q]) * D + c) = row.codes;
         if (c == 0) scales[(head * 2 + which) * kGqaPageTok + tok[q]] = row.scale;
@@ -207,7 +245,7 @@ __global__ void gqa_append_int8_kernel(AppendGeom g, uint8_t* k_base, uint8_t* v
     }
   }
   fence_chained_writes();
-  advance_lengths_by_last_block(g);
+  advance_lengths_by_last_block(g, list);
 }
 
 // New lengths travel as kernel arguments: no staging copy and its engine switch in front of the launch.
@@ -264,18 +302,34 @@ int32_t launch_mla_append(Pool* p, const SeqBatch& sb, int layer, const void* ck
                        p->prm.mla_dc, p->prm.mla_dhr, (int)p->mla_blocked, shadow);
 }
 
+template <int N>
+static int32_t launch_gqa_append_n(Pool* p, const AppendGeom& g, const AppendList<N>& list, dim3 grid, int layer, const void* k, const void* v, bool f32, int hm) {
+  uint16_t *kb = (uint16_t*)p->rows_at(layer, 0), *vb = (uint16_t*)p->rows_at(layer, 1);
+  const int Hkv = p->prm.gqa_num_kv_heads;
+  if (p->int8)
+    return launch_append(p, f32 ? gqa_append_int8_kernel<true, N> : gqa_append_int8_kernel<false, N>, grid, 256, g, list, (uint8_t*)kb, (uint8_t*)vb,
+                         p->scales_at(layer), k, v, Hkv, hm);
+  return launch_append(p, f32 ? gqa_append_kernel<true, N> : gqa_append_kernel<false, N>, grid, 256, g, list, kb, vb, k, v, Hkv, p->prm.gqa_head_dim, hm);
+}
+
+bool append_list_inline(int n_seqs) { return n_seqs <= kListMax; }
+
 int32_t launch_gqa_append(Pool* p, const SeqBatch& sb, int layer, const void* k, const void* v, int dtype, int layout,
                           int advance) {
-  AppendGeom g = make_geom(p, sb, layer, advance);
-  uint16_t *kb = (uint16_t*)p->rows_at(layer, 0), *vb = (uint16_t*)p->rows_at(layer, 1);
-  dim3 grid(sb.n_seqs, row_slices(sb));
-  int threads = 256;
-  int hm = layout == RELUX_LAYOUT_HEAD_MAJOR;
-  if (p->int8)
-    return launch_append(p, dtype == RELUX_DTYPE_F32 ? gqa_append_int8_kernel<true> : gqa_append_int8_kernel<false>, grid, threads, g, (uint8_t*)kb,
-                         (uint8_t*)vb, p->scales_at(layer), k, v, p->prm.gqa_num_kv_heads, hm);
-  return launch_append(p, dtype == RELUX_DTYPE_F32 ? gqa_append_kernel<true> : gqa_append_kernel<false>, grid, threads, g, kb, vb, k, v,
-                       p->prm.gqa_num_kv_heads, p->prm.gqa_head_dim, hm);
+  const AppendGeom g = make_geom(p, sb, layer, advance);
+  const dim3 grid(sb.n_seqs, p->int8 ? std::min(std::max((sb.max_rows + kAhead - 1) / kAhead, 1), 65535) : row_slices(sb));
+  const int hm = layout == RELUX_LAYOUT_HEAD_MAJOR;
+  const bool f32 = dtype == RELUX_DTYPE_F32;
+  bool plain = true;   // sequences 0, 1, ... with the same rows each
+  for (int i = 0; i < sb.n_seqs; i++) plain &= sb.seq[i] == i && sb.rows[i] == sb.rows[0];
+  if (plain || sb.d_seq_ids || sb.d_row_off) return launch_gqa_append_n(p, g, AppendList<0>{}, grid, layer, k, v, f32, hm);
+  AppendList<kListMax> list;
+  list.off[0] = 0;
+  for (int i = 0; i < sb.n_seqs; i++) {
+    list.seq[i] = sb.seq[i];
+    list.off[i + 1] = list.off[i] + sb.rows[i];
+  }
+  return launch_gqa_append_n(p, g, list, grid, layer, k, v, f32, hm);
 }
 
 int32_t launch_set_len(Pool* p, const SeqBatch& sb, int layer0, int layers, const int32_t* new_len) {

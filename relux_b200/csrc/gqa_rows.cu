@@ -1,6 +1,6 @@
 // Rows of a grouped-query cache, bf16 or 8-bit, read back to dense device memory, and the commit of a drafted tree's accepted path.
 //
-// Both are byte movement.  Read back: n tokens are n * Hkv * 264 B of an 8-bit cache (512 of bf16) in and n * Hkv * 512 B of bf16 out; a block takes
+// Both are byte movement.  Read back: n tokens are n * Hkv * 264 B of an 8-bit cache (512 of bf16) in and n * Hkv * 512 B of bf16 out; of a bf16 cache a block takes
 // kRowsAhead tokens at a time, all their loads, then all their stores, as the append does.  Commit: a few rows of each sequence and layer, bound by the launch
 // and by the latency of a length, a page id and a row, one after the other.
 #include <algorithm>
@@ -8,6 +8,7 @@
 #include "common.cuh"
 #include "gqa_int8_parts.cuh"
 #include "internal.h"
+#include "softmax_parts.cuh"
 
 namespace relux {
 
@@ -31,6 +32,7 @@ struct ReadCommon {
   void* v_out;
   int64_t rows;           // of all sequences of the call
   int32_t* status;
+  bool wide;              // k_out and v_out are multiples of 32
 };
 template <int N>
 struct ReadParams {
@@ -38,55 +40,105 @@ struct ReadParams {
   RowSeq seqs[N];
 };
 
-// Eight values of a row.
-struct Row8 {
-  uint4 w;
-  float s;
-};
-template <bool kI8>
-__device__ __forceinline__ Row8 fetch8(const ReadCommon& c, int layer, int which, int32_t pg, int h, int tok, int d) {
-  const char* base = (const char*)(which ? c.v : c.k) + (size_t)layer * c.layer_bytes;
-  const size_t row = ((size_t)pg * c.Hkv + h) * c.page_tokens + tok;
-  Row8 r{{0u, 0u, 0u, 0u}, 0.f};
-  if constexpr (kI8) {
-    const uint2 w = load_chained(reinterpret_cast<const uint2*>(base + row * kGqaD + d));
-    r.w.x = w.x;
-    r.w.y = w.y;
-    r.s = load_chained(c.scales + (size_t)layer * c.layer_scales + ((size_t)pg * c.Hkv + h) * (2 * kGqaPageTok) + which * kGqaPageTok + tok);
+// Eight bf16 values of a row, as they are or as float32.
+template <bool kF32>
+__device__ __forceinline__ void put8(void* to, size_t off, uint4 w) {
+  if constexpr (kF32) {
+    float4* f = reinterpret_cast<float4*>(reinterpret_cast<float*>(to) + off);
+    f[0] = make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
+    f[1] = make_float4(bf16_lo(w.z), bf16_hi(w.z), bf16_lo(w.w), bf16_hi(w.w));
   } else {
-    r.w = load_chained(reinterpret_cast<const uint4*>(base + (row * c.D + d) * 2));
-  }
-  return r;
-}
-// As float32 (to: float*) or bf16.  A code times its scale is rounded once.
-template <bool kI8, bool kF32>
-__device__ __forceinline__ void put8(void* to, size_t off, const Row8& r) {
-  if constexpr (!kI8 && !kF32) {
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + off) = r.w;
-  } else {
-    float x[8];
-    if constexpr (kI8) {
-      const uint32_t w[2] = {r.w.x, r.w.y};
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = (float)((int)(w[i >> 2] >> (8 * (i & 3)) & 255u) - 128) * r.s;
-    } else {
-      const uint32_t w[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
-    }
-    if constexpr (kF32) {
-      float4* f = reinterpret_cast<float4*>(reinterpret_cast<float*>(to) + off);
-      f[0] = make_float4(x[0], x[1], x[2], x[3]);
-      f[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + off) =
-          make_uint4(round_bf16x2(x[0], x[1]), round_bf16x2(x[2], x[3]), round_bf16x2(x[4], x[5]), round_bf16x2(x[6], x[7]));
-    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + off) = w;
   }
 }
 
-// grid (sequences, slices of their tokens, layers).
-template <bool kI8, bool kF32, int N>
+// 32 bytes, in one store where the place is a multiple of 32.
+__device__ __forceinline__ void store32(bool wide, void* to, const uint32_t (&w)[8]) {
+  if (!wide) {
+    reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    return;
+  }
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(to)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+// 16 codes times their scale, to 16 values.  The product is rounded to float32, and that to bf16.
+template <bool kF32>
+__device__ __forceinline__ void put_codes(bool wide, void* to, size_t off, uint4 codes, float s) {
+  const uint32_t c[4] = {codes.x, codes.y, codes.z, codes.w};
+  const uint64_t s2 = pack2(s, s), zero2 = pack2(-8388736.f, -8388736.f);
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {   // a byte under 0x4B0000 is 2^23 + it, of which 2^23 + 128 is nothing
+    const uint32_t lo = __byte_perm(c[i >> 1], 0x4B000000u, i & 1 ? 0x7442 : 0x7440), hi = __byte_perm(c[i >> 1], 0x4B000000u, i & 1 ? 0x7443 : 0x7441);
+    float x0, x1;
+    unpack2(mul2(add2(pack2(__uint_as_float(lo), __uint_as_float(hi)), zero2), s2), x0, x1);
+    if constexpr (kF32) {
+      w[2 * i] = __float_as_uint(x0);
+      w[2 * i + 1] = __float_as_uint(x1);
+    } else {
+      w[i] = round_bf16x2(x0, x1);
+    }
+  }
+  if constexpr (kF32) {
+    float* f = reinterpret_cast<float*>(to) + off;
+    store32(wide, f, reinterpret_cast<const uint32_t(&)[8]>(w[0]));
+    store32(wide, f + 8, reinterpret_cast<const uint32_t(&)[8]>(w[8]));
+  } else {
+    store32(wide, reinterpret_cast<uint16_t*>(to) + off, reinterpret_cast<const uint32_t(&)[8]>(w[0]));
+  }
+}
+
+// 8-bit cache: grid (sequences, pages of one, layers), a warp a head's rows of a page, of K or of V: eight lanes a row, 16 codes each, kCodesAhead loads of
+// four rows on their way (with a row's codes eight a lane, and blocks that looked up a page for every four tokens, 4 x 8192 tokens took 48 us).
+constexpr int kCodesAhead = 8;
+template <bool kF32, int N>
+__global__ void __launch_bounds__(256, 4) read_codes_kernel(const __grid_constant__ ReadParams<N> prm) {
+  chain_release();
+  chain_wait();
+  const ReadCommon& c = prm.c;
+  const RowSeq sq = prm.seqs[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, d = (lane & 7) * 16;
+  const int end = sq.tok0 + sq.n;
+  for (int slot = sq.tok0 / kGqaPageTok + (int)blockIdx.y; slot < (end + kGqaPageTok - 1) / kGqaPageTok && sq.n > 0; slot += gridDim.y) {
+    const int32_t pg = __ldg(c.table + (size_t)sq.seq * c.table_stride + slot);   // the page table is written by host calls that wait for their copy
+    if (pg < 0 || pg >= c.num_pages) {
+      set_status(c.status, RELUX_ERR_BAD_PAGE);
+      continue;
+    }
+    const int base = slot * kGqaPageTok, lo = max(sq.tok0 - base, 0), hi = min(end - base, kGqaPageTok);
+    for (int u = warp; u < 2 * c.Hkv; u += blockDim.x >> 5) {
+      const int which = u >= c.Hkv, h = u - which * c.Hkv;
+      const size_t head = (size_t)pg * c.Hkv + h;
+      const uint8_t* codes = (const uint8_t*)(which ? c.v : c.k) + (size_t)blockIdx.z * c.layer_bytes + head * (kGqaPageTok * kGqaD) + d;
+      const float* scales = c.scales + (size_t)blockIdx.z * c.layer_scales + (head * 2 + which) * kGqaPageTok;
+      void* out = which ? c.v_out : c.k_out;
+      const int64_t row0 = (int64_t)blockIdx.z * c.rows + sq.row0 + base - sq.tok0;
+      for (int r0 = lo; r0 < hi; r0 += 4 * kCodesAhead) {
+        uint4 w[kCodesAhead];
+        float s[kCodesAhead];
+#pragma unroll
+        for (int q = 0; q < kCodesAhead; q++) {
+          const int r = r0 + 4 * q + sub;
+          if (r < hi) {
+            w[q] = load_chained(reinterpret_cast<const uint4*>(codes + r * kGqaD));
+            s[q] = load_chained(scales + r);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kCodesAhead; q++) {
+          const int r = r0 + 4 * q + sub;
+          if (r < hi) put_codes<kF32>(c.wide, out, (size_t)((row0 + r) * c.Hkv + h) * kGqaD + d, w[q], s[q]);
+        }
+      }
+    }
+  }
+  fence_chained_writes();
+}
+
+// bf16 cache: grid (sequences, slices of their tokens, layers).
+template <bool kF32, int N>
 __global__ void read_kv_kernel(const __grid_constant__ ReadParams<N> prm) {
   chain_release();
   chain_wait();
@@ -112,40 +164,43 @@ __global__ void read_kv_kernel(const __grid_constant__ ReadParams<N> prm) {
     }
     for (int u = threadIdx.x; u < 2 * per_tok; u += blockDim.x) {
       const int which = u >= per_tok, e = u - which * per_tok, h = e / per_head, d = (e - h * per_head) * 8;
-      Row8 x[kN];
+      const uint16_t* base = (const uint16_t*)((const char*)(which ? c.v : c.k) + (size_t)layer * c.layer_bytes);
+      uint4 x[kN];
 #pragma unroll
       for (int q = 0; q < kN; q++)
-        if (pg[q] >= 0) x[q] = fetch8<kI8>(c, layer, which, pg[q], h, tok[q], d);
+        if (pg[q] >= 0) x[q] = load_chained(reinterpret_cast<const uint4*>(base + (((size_t)pg[q] * c.Hkv + h) * c.page_tokens + tok[q]) * c.D + d));
 #pragma unroll
       for (int q = 0; q < kN; q++)
         if (pg[q] >= 0)
-          put8<kI8, kF32>(which ? c.v_out : c.k_out, (((size_t)layer * c.rows + sq.row0 + r + q) * c.Hkv + h) * c.D + d, x[q]);
+          put8<kF32>(which ? c.v_out : c.k_out, (((size_t)layer * c.rows + sq.row0 + r + q) * c.Hkv + h) * c.D + d, x[q]);
     }
   }
   fence_chained_writes();
 }
 
-template <bool kI8, bool kF32, int N>
-int32_t launch_read_n(Pool* p, const ReadCommon& c, const RowSeq* seqs, int n, int layers, int slices) {
+template <bool kF32, int N>
+int32_t launch_read_n(Pool* p, const ReadCommon& c, const RowSeq* seqs, int n, int layers) {
   ReadParams<N> prm;
   prm.c = c;
   memcpy(prm.seqs, seqs, sizeof(RowSeq) * n);
-  const int units = 2 * c.Hkv * (c.D / 8), threads = std::min(256, (units + 31) / 32 * 32);
-  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, read_kv_kernel<kI8, kF32, N>, dim3(n, slices, layers), dim3(threads), 0,
-                                p->dev->stream, prm));
+  int most = 1, pages = 1;
+  for (int i = 0; i < n; i++) {
+    most = std::max(most, seqs[i].n);
+    pages = std::max(pages, (seqs[i].tok0 + seqs[i].n + kGqaPageTok - 1) / kGqaPageTok - seqs[i].tok0 / kGqaPageTok);
+  }
+  // bf16: about five blocks an SM in all
+  const int slices = p->int8 ? std::min(pages, 65535) : std::min((most + kRowsAhead - 1) / kRowsAhead, std::max(1, 5 * p->dev->sm_count / (n * layers)));
+  const int threads = p->int8 ? std::min(256, 64 * c.Hkv) : std::min(256, (2 * c.Hkv * (c.D / 8) + 31) / 32 * 32);
+  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, p->int8 ? read_codes_kernel<kF32, N> : read_kv_kernel<kF32, N>,
+                                dim3(n, slices, layers), dim3(threads), 0, p->dev->stream, prm));
   count_launch(p->dev);
   return RELUX_OK;
 }
-template <bool kI8, bool kF32>
+template <bool kF32>
 int32_t launch_read(Pool* p, const ReadCommon& c, const std::vector<RowSeq>& seqs, int layers) {
   for (size_t at = 0; at < seqs.size(); at += kSeqsLarge) {
     const int n = (int)std::min<size_t>(kSeqsLarge, seqs.size() - at);
-    int most = 1;
-    for (int i = 0; i < n; i++) most = std::max(most, seqs[at + i].n);
-    // about five blocks an SM in all
-    const int slices = std::min((most + kRowsAhead - 1) / kRowsAhead, std::max(1, 5 * p->dev->sm_count / (n * layers)));
-    const int32_t rc = n <= kSeqsSmall ? launch_read_n<kI8, kF32, kSeqsSmall>(p, c, &seqs[at], n, layers, slices)
-                                       : launch_read_n<kI8, kF32, kSeqsLarge>(p, c, &seqs[at], n, layers, slices);
+    const int32_t rc = n <= kSeqsSmall ? launch_read_n<kF32, kSeqsSmall>(p, c, &seqs[at], n, layers) : launch_read_n<kF32, kSeqsLarge>(p, c, &seqs[at], n, layers);
     if (rc) return rc;
   }
   return RELUX_OK;
@@ -178,10 +233,10 @@ int32_t launch_read_kv(Pool* p, const SeqBatch& sb, int layer0, int layers, cons
   c.D = prm.gqa_head_dim;
   c.k_out = k_out;
   c.v_out = v_out;
+  c.wide = (((uintptr_t)k_out | (uintptr_t)v_out) & 31) == 0;
   c.rows = row;
   c.status = p->d_status;
-  if (dtype == RELUX_DTYPE_F32) return p->int8 ? launch_read<true, true>(p, c, seqs, layers) : launch_read<false, true>(p, c, seqs, layers);
-  return p->int8 ? launch_read<true, false>(p, c, seqs, layers) : launch_read<false, false>(p, c, seqs, layers);
+  return dtype == RELUX_DTYPE_F32 ? launch_read<true>(p, c, seqs, layers) : launch_read<false>(p, c, seqs, layers);
 }
 
 int32_t do_read_kv(Pool* p, const relux_read_kv_args* a) {

@@ -226,6 +226,7 @@ int32_t stage_batch(Pool* p, int32_t n_seqs, const int32_t* seq_ids, const int32
 
 // kernels (defined in the .cu files of this directory)
 int32_t launch_mla_append(Pool* p, const SeqBatch& sb, int layer, const void* ckv, const void* kr, int dtype, int advance);
+bool append_list_inline(int n_seqs);   // launch_gqa_append carries the sequences as kernel arguments: no staged copies needed
 int32_t launch_gqa_append(Pool* p, const SeqBatch& sb, int layer, const void* k, const void* v, int dtype, int layout,
                           int advance);
 int32_t launch_set_len(Pool* p, const SeqBatch& sb, int layer0, int layers, const int32_t* new_len);   // new_len: host

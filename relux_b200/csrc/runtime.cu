@@ -452,7 +452,7 @@ static int32_t do_append(Pool* p, const relux_append_args* a, int kind) {
   }
   if (a->flags & ~RELUX_CALL_PIPELINED) { set_error("unknown call flags 0x%x", a->flags); return RELUX_ERR_INVALID_ARG; }
   SeqBatch sb;
-  rc = stage_batch(p, a->n_seqs, a->seq_ids, a->n_new, 1, &sb);
+  rc = stage_batch(p, a->n_seqs, a->seq_ids, a->n_new, 1, &sb, kind == RELUX_POOL_MLA || !append_list_inline(a->n_seqs));
   if (rc) return rc;
   // capacity check on the host shadow: the reference panics on overflow (kvcache.go:282-285)
   const relux_pool_params& prm = p->prm;

@@ -449,13 +449,21 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
               if (from < kTile) {
                 uint8_t* v = smem + PL::kRing + st * kSlot;
                 bool any = false;
-                for (int r = max(from, 0) + (lane >> 4); r < kTile; r += 2) {   // 16 lanes a row
-                  uint4* at = reinterpret_cast<uint4*>(v + ((lane >> 3) & 1) * kHalf + swz128(r, lane & 7));
-                  const uint4 w = *at;
-                  if (bf16x2_not_finite(w.x) | bf16x2_not_finite(w.y) | bf16x2_not_finite(w.z) | bf16x2_not_finite(w.w)) {
-                    *at = make_uint4(bf16x2_finite(w.x), bf16x2_finite(w.y), bf16x2_finite(w.z), bf16x2_finite(w.w));
+                auto at = [&](int r) { return reinterpret_cast<uint4*>(v + ((lane >> 3) & 1) * kHalf + swz128(r, lane & 7)); };
+                for (int r0 = max(from, 0) + (lane >> 4); r0 < kTile; r0 += 16) {   // 16 lanes a row, eight of them on their way
+                  uint32_t bad = 0;
+#pragma unroll
+                  for (int q = 0; q < 8; q++)
+                    if (r0 + 2 * q < kTile) {
+                      const uint4 w = *at(r0 + 2 * q);
+                      if (bf16x2_not_finite(w.x) | bf16x2_not_finite(w.y) | bf16x2_not_finite(w.z) | bf16x2_not_finite(w.w)) bad |= 1u << q;
+                    }
+                  any |= bad != 0;
+                  for (; bad; bad &= bad - 1) {
+                    const int r = r0 + 2 * (__ffs(bad) - 1);
+                    const uint4 w = *at(r);
+                    *at(r) = make_uint4(bf16x2_finite(w.x), bf16x2_finite(w.y), bf16x2_finite(w.z), bf16x2_finite(w.w));
                     if (r - from < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << (r - from));
-                    any = true;
                   }
                 }
                 if (any) fence_proxy_async();
@@ -516,8 +524,9 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         }
       };
       // ---- queries in: copies straight to the matrix operand's place ----
+      const int i0 = 4 * set;
 #pragma unroll 4
-      for (int i = 0; i < (set == 0 ? 8 * nb : 0); i++) {   // 16 lanes a row
+      for (int i = i0; i < (two ? i0 + 4 : 8 * nb); i++) {   // 16 lanes a row; two: half of the rows each
         const int b = kNB == 2 ? i >> 3 : 0, j = (2 * i + (lane >> 4)) & 15, row = 128 * b + 16 * row_warp + j, ch = lane & 15;
         const bool there = row < rows;
         const int s = token_of(c, sq.row0 + row), hq = sq.row0 + row - s * c.g;
@@ -555,23 +564,30 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       if constexpr (kI8) {   // in place to binary16, by a power of two a row
-        if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // the other warp of these rows has them from this one
 #pragma unroll 1
         for (int b = 0; b < nb; b++, next_block())
 #pragma unroll 2
-          for (int i = 0; i < 8; i++) {
+          for (int i = i0; i < (two ? i0 + 4 : 8); i++) {
             const int j = 2 * i + (lane >> 4), ch = lane & 15;
             uint4* at = reinterpret_cast<uint4*>(smem + PL::kQ + b * kSlot + (ch >> 3) * kHalf + swz128(r16 + j, ch & 7));
             float x[8], up, down;
             load8(x, reinterpret_cast<const uint16_t*>(at));
             query_factor(row_top(x), up, down);
-            if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // both have read it
-            if (set == 0) *at = make_uint4(pack_p<true>(x[0] * up, x[1] * up), pack_p<true>(x[2] * up, x[3] * up), pack_p<true>(x[4] * up, x[5] * up), pack_p<true>(x[6] * up, x[7] * up));
-            const float f = __shfl_sync(0xffffffffu, down, ((lane >> 2) & 1) * 16);
+            *at = make_uint4(pack_p<true>(x[0] * up, x[1] * up), pack_p<true>(x[2] * up, x[3] * up), pack_p<true>(x[4] * up, x[5] * up), pack_p<true>(x[6] * up, x[7] * up));
+            if (two) {
+              if (ch == 0) bars->halves[0][0][16 * row_warp + j] = c.scale_log2 * down;
+            } else {
+              const float f = __shfl_sync(0xffffffffu, down, ((lane >> 2) & 1) * 16);
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++)
-              if (((lane >> 2) + 8 * hf) >> 1 == i) st.f[hf] = c.scale_log2 * f;
+              for (int hf = 0; hf < 2; hf++)
+                if (((lane >> 2) + 8 * hf) >> 1 == i) st.f[hf] = c.scale_log2 * f;
+            }
           }
+        if (two) {   // to the other warp of these rows
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) st.f[hf] = bars->halves[0][0][row_in + 8 * hf];
+        }
       }
       fence_proxy_async();
       tc_fence_before();
@@ -746,7 +762,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           if (bad_all || (c.tree ? (see & bad_nodes) != 0 : bad_nodes != 0 && (int)see > (int)~(uint32_t)bad_nodes)) l = __uint_as_float(0x7FC00000u);
           const bool there = ok && row < rows && (!c.tree || token_of(c, sq.row0 + row) < sq.end - sq.len0);
           // no part of a sum that nobody has added to, of a row that is not there: zero whatever the accumulator holds
-          const float inv = !there ? 0.f : !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+          const float inv = !there ? 0.f : !whole ? 1.f : l == 0.f ? 0.f : __fdividef(1.f, l);
           f[hf] = st.m[hf] == -INFINITY && l == l ? 0.f : w * inv;
           f2[hf] *= inv;
           if (!whole && (lane & 3) == 0 && set == 0 && row < rows)
@@ -932,9 +948,12 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   if (warp == 0) tmem_dealloc<1>(tmem, kTmemCols);
 }
 
-// Joins the partials of the streams that more than one range has a part of: block x is the range behind a stream's first part, a warp a row.
+// Joins the partials of the streams that more than one range has a part of: block x is the range behind a stream's first part, a warp every 8 gridDim.y-th
+// row.  What a block costs is the search for its stream, so that it is given several rows a warp, and a row's parts are read at once, in one pass with a
+// running maximum (a row a warp, and the maxima before the sums: 24 us for 148 ranges of 2 x 240 rows, 35 MB).
+constexpr int kMergeRows = 4;   // of a warp
 template <int N>
-__global__ void __launch_bounds__(256) merge_tree_kernel(const __grid_constant__ TreeParams<N> prm) {
+__global__ void __launch_bounds__(256, 4) merge_tree_kernel(const __grid_constant__ TreeParams<N> prm) {
   chain_release();
   chain_wait();   // every block: the launch behind this one takes it that the one before is complete
   const TreeCommon& c = prm.c;
@@ -944,40 +963,50 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(const __grid_constant__
   const int w0 = streams.worker_of(p.us), np = streams.worker_of(p.us + p.tiles - 1) - w0 + 1;
   if (p.tb <= 0 || p.tb >= p.tiles || w0 != (int)blockIdx.x) return;   // no stream goes on here, or its first part is further back
   const TreeSeq sq = streams.seq(p.e);
-  const int rows = min(c.rows_rb, c.R - sq.row0), r = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  const int first = streams.range_begin(w0) == p.us ? 0 : 1;
-  auto row_of = [&](int j) -> size_t { return (size_t)(2 * (w0 + j) + (j ? 0 : first)) * c.rows_rb + r; };
-  float M = -INFINITY;
-  for (int j = lane; j < np; j += 32) M = fmaxf(M, load_chained(reinterpret_cast<const float2*>(c.part_ml) + row_of(j)).x);
-  M = warp_max(M);
-  float L = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j0 = 0; j0 < np; j0 += 4) {
-    float2 ml[4];
-    float4 x[4];
+  const int rows = min(c.rows_rb, c.R - sq.row0), first = streams.range_begin(w0) == p.us ? 0 : 1;
+#pragma unroll 2
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    float M = -INFINITY, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 < np; j0 += 4) {
+      float2 ml[4];
+      float4 x[4];
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-      if (j0 + q < np) {
-        ml[q] = load_chained(reinterpret_cast<const float2*>(c.part_ml) + row_of(j0 + q));
-        x[q] = load_chained(reinterpret_cast<const float4*>(c.part_o + row_of(j0 + q) * kD) + lane);
+      for (int q = 0; q < 4; q++) {
+        ml[q] = make_float2(-INFINITY, 0.f);
+        if (j0 + q < np) {
+          const size_t at = (size_t)(2 * (w0 + j0 + q) + (j0 + q ? 0 : first)) * c.rows_rb + r;
+          ml[q] = load_chained(reinterpret_cast<const float2*>(c.part_ml) + at);
+          x[q] = load_chained(reinterpret_cast<const float4*>(c.part_o + at * kD) + lane);
+        }
       }
+      const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M);
+      if (M != -INFINITY && top > M) {
+        const float w = ex2_approx(M - top);
+        L *= w;
+        o.x *= w;
+        o.y *= w;
+        o.z *= w;
+        o.w *= w;
+      }
+      M = top;
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-      if (j0 + q < np && ml[q].x != -INFINITY) {
-        const float w = ex2_approx(ml[q].x - M);
-        L = fmaf(ml[q].y, w, L);
-        o.x = fmaf(x[q].x, w, o.x);
-        o.y = fmaf(x[q].y, w, o.y);
-        o.z = fmaf(x[q].z, w, o.z);
-        o.w = fmaf(x[q].w, w, o.w);
-      }
+      for (int q = 0; q < 4; q++)
+        if (ml[q].x != -INFINITY) {
+          const float w = ex2_approx(ml[q].x - M);
+          L = fmaf(ml[q].y, w, L);
+          o.x = fmaf(x[q].x, w, o.x);
+          o.y = fmaf(x[q].y, w, o.y);
+          o.z = fmaf(x[q].z, w, o.z);
+          o.w = fmaf(x[q].w, w, o.w);
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int row = sq.row0 + r, s = token_of(c, row);
+    const size_t at = (((size_t)sq.i * c.S + s) * c.H + (size_t)p.kvh * c.g + (row - s * c.g)) * kD + 4 * lane;
+    if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int row = sq.row0 + r, s = token_of(c, row);
-  const size_t at = (((size_t)sq.i * c.S + s) * c.H + (size_t)p.kvh * c.g + (row - s * c.g)) * kD + 4 * lane;
-  if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-  else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 template <bool kI8, int kNB, int N>
@@ -988,7 +1017,7 @@ int32_t launch(Pool* p, const TreeParams<N>& prm, int workers) {
   RELUX_CUDA_TRY(launch_chained(chained, tree_sm100_kernel<kI8, kNB, N>, dim3(workers), dim3(PL::kThreads), (size_t)PL::kTotal, p->dev->stream, p->tmap_gqa, prm));
   count_launch(p->dev);
   if (workers > 1) {
-    RELUX_CUDA_TRY(launch_chained(chained, merge_tree_kernel<N>, dim3(workers - 1, (prm.c.rows_rb + 7) / 8), dim3(256), 0, p->dev->stream, prm));
+    RELUX_CUDA_TRY(launch_chained(chained, merge_tree_kernel<N>, dim3(workers - 1, (prm.c.rows_rb + 8 * kMergeRows - 1) / (8 * kMergeRows)), dim3(256), 0, p->dev->stream, prm));
     count_launch(p->dev);
   }
   return RELUX_OK;

@@ -171,17 +171,19 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// gqa_consume_page for a page of codes.
-template <bool kTree>
-__device__ __forceinline__ void int8_consume_page(GqaState<1>& st, ValueUnit& unit, const uint32_t (&qa)[8][4], const float (&q_scale)[2], const uint8_t* page,
-                                                  const float* scales, int tb, int tok0, int T, int S, int g, int causal, int lane, int row0,
-                                                  const TreeRows& tree) {
+// A maximum is followed only once it has grown by more than this (base 2): with random scores three visits of a page in five found a larger one, and
+// moved 64 sums for it.
+constexpr float kInt8Lazy = 8.f;
+constexpr int kInt8Up = 7;   // P s^v is kept below 2^(kInt8Up + kInt8Lazy), the upper end of binary16
+
+// Scores of a warp's 16 tokens of a page, but for the queries' factors.
+__device__ __forceinline__ void int8_scores(float (&s)[2][4], const uint32_t (&qa)[8][4], const uint8_t* page, const float* scales, int tb, int lane) {
   const int n = lane >> 2, c = lane & 3;
-  float sacc[2][4], sodd[2][4];   // even and odd K slices: two chains of dependent MMAs a block
+  float odd[2][4];   // even and odd K slices: two chains of dependent MMAs a block
 #pragma unroll
   for (int nt = 0; nt < 2; nt++) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) sacc[nt][e] = sodd[nt][e] = 0.f;
+    for (int e = 0; e < 4; e++) s[nt][e] = odd[nt][e] = 0.f;
     const uint32_t row = tb + nt * 8 + n;
     const uint4 k0 = *reinterpret_cast<const uint4*>(page + swz128(row, 2 * c)), k1 = *reinterpret_cast<const uint4*>(page + swz128(row, 2 * c + 1));
     const uint32_t w[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
@@ -189,35 +191,31 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, ValueUnit& un
     for (int ks = 0; ks < 8; ks++) {
       uint32_t b0, b1;
       int8x4_to_f16(w[ks], b0, b1);
-      mma_f16_16816(ks & 1 ? sodd[nt] : sacc[nt], qa[ks], b0, b1);
+      mma_f16_16816(ks & 1 ? odd[nt] : s[nt], qa[ks], b0, b1);
     }
-  }
-  // the values' codes, while the scores are on their way
-  const uint8_t* vt = page + kGqaPageTok * kGqaD;
-  uint4 v[4];
+    const float2 sk = *reinterpret_cast<const float2*>(scales + tb + nt * 8 + 2 * c);
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const uint4*>(vt + swz128(tb + 2 * c + (i & 1) + (i >> 1) * 8, n));
+    for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + odd[nt][e]) * (e & 1 ? sk.y : sk.x);
+  }
+}
+
+// gqa_consume_page for a page of codes whose scores are in s.  next_scores(s) then computes those of the next page, beside this one's exponentials and values:
+// with two such warps on a scheduler, one page's chain of latencies after another left it idle half of the time.
+template <bool kTree, typename Next>
+__device__ __forceinline__ void int8_consume_page(GqaState<1>& st, ValueUnit& unit, float (&s)[2][4], const float (&q_scale)[2], const uint8_t* page,
+                                                  const float* scales, int tb, int tok0, int T, int S, int g, int causal, int lane, int row0,
+                                                  const TreeRows& tree, Next next_scores) {
+  const int n = lane >> 2, c = lane & 3;
   float sv[2][2];
 #pragma unroll
   for (int nt = 0; nt < 2; nt++) {
-    const float2 sk = *reinterpret_cast<const float2*>(scales + tb + nt * 8 + 2 * c);
     const float2 s2 = *reinterpret_cast<const float2*>(scales + kGqaPageTok + tb + nt * 8 + 2 * c);
     sv[nt][0] = s2.x;
     sv[nt][1] = s2.y;
-#pragma unroll
-    for (int e = 0; e < 4; e++) sacc[nt][e] = (sacc[nt][e] + sodd[nt][e]) * (e & 1 ? sk.y : sk.x);
   }
   // rows that nobody sees yet, or ever, have a part in the unit too if they are the sequence's; what lies behind T may hold anything
   const int there = T - tok0 - 2 * c;
   float top = fmaxf(fmaxf(there > 0 ? sv[0][0] : 0.f, there > 1 ? sv[0][1] : 0.f), fmaxf(there > 8 ? sv[1][0] : 0.f, there > 9 ? sv[1][1] : 0.f));   // NaN drop out
-  float shrink = 1.f;
-  if (__any_sync(0xffffffffu, top >= unit.limit)) {
-    top = warp_max(top);
-    const float before = unit.down;
-    const bool first = unit.limit == 0.f;
-    unit.grow<15>(top);
-    if (!first) shrink = unit.down / before;
-  }
   uint32_t hidden = 0;   // bit 4 hf + 2 nt + e
   const bool need_mask = tok0 + 16 > (kTree ? tree.len0 : T - (causal ? S : 0));
   if (need_mask) {
@@ -231,24 +229,31 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, ValueUnit& un
           const int tok = tok0 + nt * 8 + 2 * c + e;
           if (kTree ? tree.hides(hf, tok) : tok > limit || tok >= T) {
             hidden |= 1u << (4 * hf + 2 * nt + e);
-            sacc[nt][hf * 2 + e] = -INFINITY;
+            s[nt][hf * 2 + e] = -INFINITY;
           }
         }
     }
   }
-  float mx[2];
+  float mx[2];   // of this lane's tokens
   bool grow = false;
 #pragma unroll
   for (int hf = 0; hf < 2; hf++) {
-    float x = fmaxf(fmaxf(sacc[0][hf * 2], sacc[0][hf * 2 + 1]), fmaxf(sacc[1][hf * 2], sacc[1][hf * 2 + 1]));
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-    mx[hf] = x * q_scale[hf];
-    grow |= mx[hf] > st.m[0][hf];
+    mx[hf] = fmaxf(fmaxf(s[0][hf * 2], s[0][hf * 2 + 1]), fmaxf(s[1][hf * 2], s[1][hf * 2 + 1])) * q_scale[hf];
+    grow |= mx[hf] > st.m[0][hf] + kInt8Lazy;
   }
-  if (__any_sync(0xffffffffu, grow || shrink != 1.f)) {
+  if (__any_sync(0xffffffffu, grow || top >= unit.limit)) {
+    float shrink = 1.f;
+    top = warp_max(top);
+    if (top >= unit.limit) {
+      const float before = unit.down;
+      const bool first = unit.limit == 0.f;
+      unit.grow<kInt8Up>(top);
+      if (!first) shrink = unit.down / before;
+    }
 #pragma unroll
     for (int hf = 0; hf < 2; hf++) {
+      mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+      mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
       const float m_new = fmaxf(st.m[0][hf], mx[hf]);
       float alpha = (m_new == -INFINITY) ? 0.f : gqa_ex2(st.m[0][hf] - m_new);
       st.m[0][hf] = m_new;
@@ -261,27 +266,40 @@ __device__ __forceinline__ void int8_consume_page(GqaState<1>& st, ValueUnit& un
       }
     }
   }
-  // P times the values' scales over their unit, rounded to binary16: 2^-11 of each, or 2^-25 of 2^14 and more that the largest come to
+  float s_next[2][4];
+  next_scores(s_next);
+  // P times the values' scales over their unit, rounded to binary16: 2^-11 of each, or 2^-25 where the largest come to 2^7 and more
   uint32_t pa[4];
+  float p[2][4];
 #pragma unroll
   for (int hf = 0; hf < 2; hf++) {
     const float neg_m = (st.m[0][hf] == -INFINITY) ? 0.f : -st.m[0][hf];
     float ps = 0.f;
 #pragma unroll
     for (int nt = 0; nt < 2; nt++) {
-      float p0 = gqa_ex2(fmaf(sacc[nt][hf * 2], q_scale[hf], neg_m));
-      float p1 = gqa_ex2(fmaf(sacc[nt][hf * 2 + 1], q_scale[hf], neg_m));
-      ps += p0 + p1;
-      p0 *= sv[nt][0] * unit.down;
-      p1 *= sv[nt][1] * unit.down;
-      if (need_mask) {   // the scale of a hidden row may be NaN
-        if (hidden >> (4 * hf + 2 * nt) & 1u) p0 = 0.f;
-        if (hidden >> (4 * hf + 2 * nt + 1) & 1u) p1 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float x = gqa_ex2(fmaf(s[nt][hf * 2 + e], q_scale[hf], neg_m));
+        ps += x;
+        p[nt][hf * 2 + e] = x * (sv[nt][e] * unit.down);
       }
-      pa[nt * 2 + hf] = round_f16x2(p0, p1);
     }
     st.l[0][hf] += ps;
   }
+  if (need_mask)   // the scale of a hidden row may be NaN
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (hidden >> i & 1u) p[i >> 1 & 1][(i >> 2) * 2 + (i & 1)] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    pa[i] = round_f16x2(p[i >> 1][(i & 1) * 2], p[i >> 1][(i & 1) * 2 + 1]);
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) s[nt][i] = s_next[nt][i];
+  }
+  const uint8_t* vt = page + kGqaPageTok * kGqaD;
+  uint4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const uint4*>(vt + swz128(tb + 2 * c + (i & 1) + (i >> 1) * 8, n));
 #pragma unroll
   for (int w = 0; w < 4; w++) {
     uint32_t x[4];

@@ -218,6 +218,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (c.seqs) chain_wait();   // the list is a copy that was queued just before this launch
   Piece p = first_piece();
 
+  // 8-bit cache: the consumers take registers from the finishers and the producer, a warpgroup, so that a page's codes and the next one's scores fit too
+  if constexpr (kI8) {
+    constexpr int kRegsConsumer = 208, kRegsOther = 88;
+    static_assert(kConsumers == 8 && kThreads == 384 && 256 * kRegsConsumer + 128 * kRegsOther <= kThreads * 168, "more registers than the block is launched with");
+    if (warp < kConsumers) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsConsumer));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+  }
+
   if (warp == kConsumers + kFinishers) {
     // ---------------- producer: TMA loads, new lengths ----------------
     const bool el = elect_one();
@@ -382,19 +390,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       GqaState<1> state;
       state.clear();
       ValueUnit unit;
-      for (int page = p.pb; page < p.pe; page++, g++) {
-        if (MT == 1 && (g & 1) != grp) continue;
-        const int st = g % kStages;
-        if (alive) alive = timed_wait(&full[st], (g / kStages) & 1);
-        if (alive) {
-          if constexpr (kI8)
-            int8_consume_page<kTr>(state, unit, qa[0], q_scale, smem + st * kStageBytes, reinterpret_cast<const float*>(smem + SM::kScales + st * kInt8ScaleBytes),
-                                   tb, page * kGqaPageTok + tb, T, c.S, c.g, c.causal, lane, row0, tree);
-          else
-            gqa_consume_page<1, kTr>(state, qa, smem_u32(smem + st * kGqaStageBytes), tb, page * kGqaPageTok + tb, T, c.S, c.g, c.causal,
-                                     c.scale_log2, lane, row0, tree);
+      if constexpr (kI8) {
+        constexpr int kEvery = MT == 1 ? 2 : 1;   // of the pages, this warp's
+        const int g0 = g, g_end = g + p.pe - p.pb;
+        if (MT == 1 && (g & 1) != grp) g++;
+        float s[2][4];
+        auto scores_of = [&](int g, float(&s)[2][4]) {
+          int8_scores(s, qa[0], smem + g % kStages * kStageBytes, reinterpret_cast<const float*>(smem + SM::kScales + g % kStages * kInt8ScaleBytes), tb, lane);
+        };
+        auto consume = [&](int g, auto next) {
+          const int st = g % kStages, page = p.pb + g - g0;
+          int8_consume_page<kTr>(state, unit, s, q_scale, smem + st * kStageBytes, reinterpret_cast<const float*>(smem + SM::kScales + st * kInt8ScaleBytes), tb,
+                                 page * kGqaPageTok + tb, T, c.S, c.g, c.causal, lane, row0, tree, next);
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty[st]);
+        };
+        if (g < g_end) {
+          if (alive) alive = timed_wait(&full[g % kStages], (g / kStages) & 1);
+          if (alive) scores_of(g, s);
+          for (; alive && g + kEvery < g_end; g += kEvery) {
+            const int ahead = g + kEvery;
+            alive = timed_wait(&full[ahead % kStages], (ahead / kStages) & 1);
+            if (alive) consume(g, [&](float(&s)[2][4]) { scores_of(ahead, s); });
+          }
+          if (alive) consume(g, [](float(&s)[2][4]) { s[0][0] = s[0][1] = s[0][2] = s[0][3] = s[1][0] = s[1][1] = s[1][2] = s[1][3] = 0.f; });
+        }
+        g = g_end;
+      } else {
+        for (int page = p.pb; page < p.pe; page++, g++) {
+          if (MT == 1 && (g & 1) != grp) continue;
+          const int st = g % kStages;
+          if (alive) alive = timed_wait(&full[st], (g / kStages) & 1);
+          if (alive) {
+            gqa_consume_page<1, kTr>(state, qa, smem_u32(smem + st * kGqaStageBytes), tb, page * kGqaPageTok + tb, T, c.S, c.g, c.causal,
+                                     c.scale_log2, lane, row0, tree);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+          }
         }
       }
       const int sb = n % kStateBufs;

@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <new>
 
 #include "common.cuh"
 #include "gqa_int8_parts.cuh"
@@ -1049,7 +1050,13 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.n_rb = (int)((R + c.rows_rb - 1) / c.rows_rb);
   const int64_t groups = (int64_t)n * c.n_rb;
   if (R >= ((int64_t)1 << 26) || groups >= ((int64_t)1 << 24)) { set_error("more query rows than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
-  std::vector<TreeSeq> seqs((size_t)groups + 1);
+  std::vector<TreeSeq> seqs;
+  try {
+    seqs.resize((size_t)groups + 1);
+  } catch (const std::bad_alloc&) {
+    set_error("out of host memory for %lld groups of query rows", (long long)groups);
+    return RELUX_ERR_OUT_OF_MEMORY;
+  }
   int64_t units64 = 0;
   for (int i = 0; i < n; i++) {
     const int s = sb.seq[i], len = p->h_len[(size_t)a.layer * prm.max_seqs + s], T = len + (tree ? nodes[i] : a.extra_tokens);

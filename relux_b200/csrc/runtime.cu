@@ -1623,17 +1623,27 @@ API int32_t relux_gqa_verify(relux_pool_t h, const relux_attn_args* attn, const 
   GET_POOL(h);
   return do_verify(p, attn, kv, RELUX_POOL_GQA);
 }
+// No exception leaves a C entry: these build lists of the call's sequences.
+template <typename Call>
+static int32_t without_exceptions(Call call) {
+  try {
+    return call();
+  } catch (const std::bad_alloc&) {
+    set_error("out of host memory");
+    return RELUX_ERR_OUT_OF_MEMORY;
+  }
+}
 API int32_t relux_gqa_tree_verify(relux_pool_t h, const relux_attn_args* attn, const relux_append_args* kv, const relux_tree_args* tree) {
   GET_POOL(h);
-  return do_gqa_tree(p, attn, kv, tree);
+  return without_exceptions([&] { return do_gqa_tree(p, attn, kv, tree); });
 }
 API int32_t relux_gqa_tree_commit(relux_pool_t h, const relux_tree_commit_args* a) {
   GET_POOL(h);
-  return do_tree_commit(p, a);
+  return without_exceptions([&] { return do_tree_commit(p, a); });
 }
 API int32_t relux_gqa_read_kv(relux_pool_t h, const relux_read_kv_args* a) {
   GET_POOL(h);
-  return do_read_kv(p, a);
+  return without_exceptions([&] { return do_read_kv(p, a); });
 }
 API int32_t relux_mla_verify(relux_pool_t h, const relux_attn_args* attn, const relux_append_args* kv) {
   GET_POOL(h);

@@ -218,7 +218,7 @@ class Pool:
     def set_len(self, layer, new_len, seq_ids=None):
         nl = np.ascontiguousarray(new_len, dtype=np.int32)
         ids = None if seq_ids is None else np.ascontiguousarray(seq_ids, dtype=np.int32)
-        L.check(self.lib.relux_seq_set_len(self.h, layer, nl.size, _ptr(ids), nl.ctypes.data))
+        L.check(self.lib.relux_seq_set_len(self.h, layer, nl.size, _ptr(ids), _ptr(nl)))
 
     def status(self):
         s = C.c_int32()

@@ -210,6 +210,7 @@ struct Raw8 {
 // The same rows into an 8-bit cache (gqa_int8_parts.cuh): 16 lanes quantise a kv head's row, of K or of V.  64 registers a thread, so that four blocks
 // of kAhead rows are on an SM, and a block per kAhead rows: what one computes and stores, others load meanwhile (with 106 registers, values held as float32,
 // and blocks of several turns, 8 x 2048 float32 rows of 4 KB took twice as long).
+constexpr int int8_rows_ahead(bool f32) { return f32 ? kAhead : 2 * kAhead; }   // bf16 rows are half as many registers
 template <bool kF32, int N>
 __global__ void __launch_bounds__(256, 4) gqa_append_int8_kernel(AppendGeom g, const __grid_constant__ AppendList<N> list, uint8_t* k_base, uint8_t* v_base,
                                                                  float* scales, const void* ksrc, const void* vsrc, int Hkv, int head_major) {
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(256, 4) gqa_append_int8_kernel(AppendGeom g, c
   const int seq = sp.seq, r0 = sp.r0, nrows = sp.n;
   const int base_len = load_chained(g.len + seq);
   const int c = (threadIdx.x & 15) * 8;
-  constexpr int kN = kAhead;
+  constexpr int kN = int8_rows_ahead(kF32);
   for (int r = blockIdx.y * kN; r < nrows; r += gridDim.y * kN) {
     int32_t pg[kN], tok[kN];
     pages_of_rows<kN>(g, seq, base_len, r, nrows, pg, tok);
@@ -317,7 +318,8 @@ bool append_list_inline(int n_seqs) { return n_seqs <= kListMax; }
 int32_t launch_gqa_append(Pool* p, const SeqBatch& sb, int layer, const void* k, const void* v, int dtype, int layout,
                           int advance) {
   const AppendGeom g = make_geom(p, sb, layer, advance);
-  const dim3 grid(sb.n_seqs, p->int8 ? std::min(std::max((sb.max_rows + kAhead - 1) / kAhead, 1), 65535) : row_slices(sb));
+  const int ahead = int8_rows_ahead(dtype == RELUX_DTYPE_F32);
+  const dim3 grid(sb.n_seqs, p->int8 ? std::min(std::max((sb.max_rows + ahead - 1) / ahead, 1), 65535) : row_slices(sb));
   const int hm = layout == RELUX_LAYOUT_HEAD_MAJOR;
   const bool f32 = dtype == RELUX_DTYPE_F32;
   bool plain = true;   // sequences 0, 1, ... with the same rows each

@@ -33,6 +33,7 @@ struct ReadCommon {
   int64_t rows;           // of all sequences of the call
   int32_t* status;
   bool wide;              // k_out and v_out are multiples of 32
+  int32_t parts;          // 8-bit caches: blocks that share a page's heads
 };
 template <int N>
 struct ReadParams {
@@ -90,30 +91,29 @@ __device__ __forceinline__ void put_codes(bool wide, void* to, size_t off, uint4
   }
 }
 
-// 8-bit cache: grid (sequences, pages of one, layers), a warp a head's rows of a page, of K or of V: eight lanes a row, 16 codes each, kCodesAhead loads of
-// four rows on their way (with a row's codes eight a lane, and blocks that looked up a page for every four tokens, 4 x 8192 tokens took 48 us).
-constexpr int kCodesAhead = 8;
+// 8-bit cache: grid (sequences, pages of one times parts, layers), a warp a head's rows of a page, of K or of V: eight lanes a row, 16 codes each, kCodesAhead
+// loads of four rows on their way (with a row's codes eight a lane, and blocks that looked up a page for every four tokens, 4 x 8192 tokens took 48 us).
+constexpr int kCodesAhead = 8, kCodesWarps = 4;
 template <bool kF32, int N>
-__global__ void __launch_bounds__(256, 4) read_codes_kernel(const __grid_constant__ ReadParams<N> prm) {
+__global__ void __launch_bounds__(32 * kCodesWarps, 8) read_codes_kernel(const __grid_constant__ ReadParams<N> prm) {
   chain_release();
   chain_wait();
   const ReadCommon& c = prm.c;
   const RowSeq sq = prm.seqs[blockIdx.x];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, d = (lane & 7) * 16;
-  const int end = sq.tok0 + sq.n;
-  for (int slot = sq.tok0 / kGqaPageTok + (int)blockIdx.y; slot < (end + kGqaPageTok - 1) / kGqaPageTok && sq.n > 0; slot += gridDim.y) {
+  const int end = sq.tok0 + sq.n, first = (int)blockIdx.y / c.parts, part = (int)blockIdx.y - first * c.parts;
+  for (int slot = sq.tok0 / kGqaPageTok + first; slot < (end + kGqaPageTok - 1) / kGqaPageTok && sq.n > 0; slot += gridDim.y / c.parts) {
     const int32_t pg = __ldg(c.table + (size_t)sq.seq * c.table_stride + slot);   // the page table is written by host calls that wait for their copy
     if (pg < 0 || pg >= c.num_pages) {
       set_status(c.status, RELUX_ERR_BAD_PAGE);
       continue;
     }
     const int base = slot * kGqaPageTok, lo = max(sq.tok0 - base, 0), hi = min(end - base, kGqaPageTok);
-    for (int u = warp; u < 2 * c.Hkv; u += blockDim.x >> 5) {
+    for (int u = part * kCodesWarps + warp; u < 2 * c.Hkv; u += c.parts * kCodesWarps) {
       const int which = u >= c.Hkv, h = u - which * c.Hkv;
       const size_t head = (size_t)pg * c.Hkv + h;
       const uint8_t* codes = (const uint8_t*)(which ? c.v : c.k) + (size_t)blockIdx.z * c.layer_bytes + head * (kGqaPageTok * kGqaD) + d;
       const float* scales = c.scales + (size_t)blockIdx.z * c.layer_scales + (head * 2 + which) * kGqaPageTok;
-      void* out = which ? c.v_out : c.k_out;
       const int64_t row0 = (int64_t)blockIdx.z * c.rows + sq.row0 + base - sq.tok0;
       for (int r0 = lo; r0 < hi; r0 += 4 * kCodesAhead) {
         uint4 w[kCodesAhead];
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256, 4) read_codes_kernel(const __grid_constan
 #pragma unroll
         for (int q = 0; q < kCodesAhead; q++) {
           const int r = r0 + 4 * q + sub;
-          if (r < hi) put_codes<kF32>(c.wide, out, (size_t)((row0 + r) * c.Hkv + h) * kGqaD + d, w[q], s[q]);
+          if (r < hi) put_codes<kF32>(c.wide, which ? c.v_out : c.k_out, (size_t)((row0 + r) * c.Hkv + h) * kGqaD + d, w[q], s[q]);
         }
       }
     }
@@ -183,14 +183,15 @@ int32_t launch_read_n(Pool* p, const ReadCommon& c, const RowSeq* seqs, int n, i
   ReadParams<N> prm;
   prm.c = c;
   memcpy(prm.seqs, seqs, sizeof(RowSeq) * n);
-  int most = 1, pages = 1;
-  for (int i = 0; i < n; i++) {
-    most = std::max(most, seqs[i].n);
-    pages = std::max(pages, (seqs[i].tok0 + seqs[i].n + kGqaPageTok - 1) / kGqaPageTok - seqs[i].tok0 / kGqaPageTok);
-  }
-  // bf16: about five blocks an SM in all
-  const int slices = p->int8 ? std::min(pages, 65535) : std::min((most + kRowsAhead - 1) / kRowsAhead, std::max(1, 5 * p->dev->sm_count / (n * layers)));
-  const int threads = p->int8 ? std::min(256, 64 * c.Hkv) : std::min(256, (2 * c.Hkv * (c.D / 8) + 31) / 32 * 32);
+  int most = 1;
+  for (int i = 0; i < n; i++) most = std::max(most, seqs[i].n);
+  // bf16: about five blocks an SM in all.  8-bit: a page of tokens a block (rows that lie across two pages do not make two), or where those are few, several
+  // blocks a page, up to a head a warp (8 x 2048 tokens, 256 pages: 27 us with one, 21 with four; 64 x 5 tokens of 32 layers: 18 with one, 22 with four)
+  const int64_t pages = (most + kGqaPageTok - 1) / kGqaPageTok, blocks = pages * n * layers;
+  prm.c.parts = (int)std::min<int64_t>((2 * c.Hkv + kCodesWarps - 1) / kCodesWarps, std::max<int64_t>(1, 12 * p->dev->sm_count / blocks));
+  const int slices = p->int8 ? prm.c.parts * (int)std::max<int64_t>(1, std::min<int64_t>(pages, 65535 / prm.c.parts))
+                             : std::min((most + kRowsAhead - 1) / kRowsAhead, std::max(1, 5 * p->dev->sm_count / (n * layers)));
+  const int threads = p->int8 ? 32 * kCodesWarps : std::min(256, (2 * c.Hkv * (c.D / 8) + 31) / 32 * 32);
   RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, p->int8 ? read_codes_kernel<kF32, N> : read_kv_kernel<kF32, N>,
                                 dim3(n, slices, layers), dim3(threads), 0, p->dev->stream, prm));
   count_launch(p->dev);
@@ -375,6 +376,7 @@ int32_t do_tree_commit(Pool* p, const relux_tree_commit_args* a) {
   if (rc) return rc;
   const int l0 = a->layer < 0 ? 0 : a->layer, l1 = a->layer < 0 ? prm.num_layers : a->layer + 1;
   std::vector<CommitSeq> seqs;
+  seqs.reserve(sb.n_seqs);
   for (int i = 0; i < sb.n_seqs; i++) {
     const int n = sb.rows[i];
     if (n > a->path_stride || n > kTreeNodes) {
@@ -391,12 +393,15 @@ int32_t do_tree_commit(Pool* p, const relux_tree_commit_args* a) {
       }
       s.path[k] = (uint8_t)path[k];
     }
-    for (int l = l0; l < l1; l++)
-      if (p->h_len[(size_t)l * prm.max_seqs + s.seq] + path[n - 1] >= p->seq_pages[s.seq] * prm.page_tokens) {
-        set_error("tree_commit: node %d lies past the capacity of sequence %d on layer %d", path[n - 1], s.seq, l);
+    seqs.push_back(s);
+  }
+  for (int l = l0; l < l1; l++) {
+    const int32_t* len = &p->h_len[(size_t)l * prm.max_seqs];
+    for (const CommitSeq& s : seqs)
+      if (len[s.seq] + s.path[s.n - 1] >= p->seq_pages[s.seq] * prm.page_tokens) {
+        set_error("tree_commit: node %d lies past the capacity of sequence %d on layer %d", (int)s.path[s.n - 1], s.seq, l);
         return RELUX_ERR_OVERFLOW;
       }
-    seqs.push_back(s);
   }
   CommitCommon c{};
   c.layer_bytes = p->layer_elems * p->elem_bytes();
@@ -420,12 +425,13 @@ int32_t do_tree_commit(Pool* p, const relux_tree_commit_args* a) {
       rc = n <= kSeqsSmall ? launch_commit<kSeqsSmall>(p, c, &seqs[at], n, layers) : launch_commit<kSeqsLarge>(p, c, &seqs[at], n, layers);
       if (rc) return rc;
     }
-  for (const CommitSeq& s : seqs)
-    for (int l = l0; l < l1; l++) {
-      int32_t& len = p->h_len[(size_t)l * prm.max_seqs + s.seq];
-      note_set_len(p, l, s.seq, len, len + s.n);
-      len += s.n;
+  for (int l = l0; l < l1; l++) {
+    int32_t* len = &p->h_len[(size_t)l * prm.max_seqs];
+    for (const CommitSeq& s : seqs) {
+      if (p->compat) note_set_len(p, l, s.seq, len[s.seq], len[s.seq] + s.n);
+      len[s.seq] += s.n;
     }
+  }
   return RELUX_OK;
 }
 

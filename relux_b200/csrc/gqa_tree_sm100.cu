@@ -51,7 +51,6 @@ constexpr float kRescaleThreshold = 8.0f;      // log2: P reaches 2^8 before the
 // (8-bit cache) log2: what P and its sum are larger by.  Binary16 has 11 bits down to 2^-14, and P reaches 2^(8 + 7): probabilities keep 11 bits down to 2^-21
 // of the row's largest, and below are off by at most 2^-32 of it.
 constexpr float kPUp = 7.0f;
-constexpr int kPolyPairsOf8 = 2;               // of a lane's score pairs, as many take the exponential on the FMA pipe
 constexpr int kInlineSmall = 32, kInlineLarge = 256;
 
 // A group of rows of a sequence: rows [row0, row0 + rows_rb) of every kv head.
@@ -232,22 +231,18 @@ __device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
   }
 }
 // exp2(score * factor - max) of a lane's 2 x 32 scores (tmem_ld_16x256b_x16), packed in the order of tmem_st_16x128b_x16; row sums are added to ps2.
-template <bool kI8, bool kPoly>
+// (All of them on the special-function unit: a fourth on the FMA pipe, by a polynomial, changed nothing with bf16 rows, and with converters beside it
+// 8 x 32768 tokens, 64 nodes, 64 heads took 721 us for 658.)
+template <bool kI8>
 __device__ __forceinline__ void exp_scores(const uint32_t (&sv)[64], const uint64_t (&factor2)[2], const uint64_t (&neg_m2)[2], uint32_t (&pw)[32], uint64_t (&ps2)[2]) {
 #pragma unroll
   for (int i = 0; i < 32; i++) {   // pair i: row i & 1
     const uint64_t x2 = fma2(pack2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), factor2[i & 1], neg_m2[i & 1]);
-    uint64_t p2;
-    if (kPoly && (i & 7) < kPolyPairsOf8) {
-      p2 = ex2_poly2(x2);
-    } else {
-      float x0, x1;
-      unpack2(x2, x0, x1);
-      p2 = pack2(ex2_approx(x0), ex2_approx(x1));
-    }
-    ps2[i & 1] = add2(ps2[i & 1], p2);
     float p0, p1;
-    unpack2(p2, p0, p1);
+    unpack2(x2, p0, p1);
+    p0 = ex2_approx(p0);
+    p1 = ex2_approx(p1);
+    ps2[i & 1] = add2(ps2[i & 1], pack2(p0, p1));
     pw[i] = pack_p<kI8>(p0, p1);
   }
 }
@@ -684,10 +679,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             ps2[hf] = pack2(0.f, 0.f);
           }
           uint32_t pw[32];
-          // With two blocks the special-function unit is what exponentials wait for; else the instruction cache is (see wait_bar).  ex2(-inf) is 0, the
-          // polynomial's is not.
-          if (kNB == 2 && whole) exp_scores<kI8, true>(sv, factor2, neg_m2, pw, ps2);
-          else exp_scores<kI8, false>(sv, factor2, neg_m2, pw, ps2);
+          exp_scores<kI8>(sv, factor2, neg_m2, pw, ps2);
           tmem_st_16x128b_x16(tmem_s, pw);
 #pragma unroll
           for (int hf = 0; hf < 2; hf++) {

@@ -221,27 +221,38 @@ __global__ void __launch_bounds__(256, 4) gqa_append_int8_kernel(AppendGeom g, c
   const int seq = sp.seq, r0 = sp.r0, nrows = sp.n;
   const int base_len = load_chained(g.len + seq);
   const int c = (threadIdx.x & 15) * 8;
+  // tokens in groups that begin at a multiple of kN, so that a group lies in one page
   constexpr int kN = int8_rows_ahead(kF32);
-  for (int r = blockIdx.y * kN; r < nrows; r += gridDim.y * kN) {
-    int32_t pg[kN], tok[kN];
-    pages_of_rows<kN>(g, seq, base_len, r, nrows, pg, tok);
+  static_assert(kGqaPageTok % kN == 0, "a group of rows lies in one page");
+  const int end = base_len + nrows;
+  for (int pos = base_len / kN * kN + (int)blockIdx.y * kN; pos < end; pos += gridDim.y * kN) {
+    const int slot = pos / kGqaPageTok, tok = pos - slot * kGqaPageTok, lo = max(base_len - pos, 0), hi = min(end - pos, kN);
+    int32_t pg;
+    if (slot >= g.max_pages_per_seq) {
+      set_status(g.status, RELUX_ERR_OVERFLOW);
+      continue;
+    }
+    if (!page_of(g.table, g.table_stride, seq, slot, g.num_pages, g.status, &pg)) continue;
     for (int u = threadIdx.x >> 4; u < 2 * Hkv; u += blockDim.x >> 4) {   // two a warp: all of its lanes or none
       const int which = u >= Hkv, h = u - which * Hkv;
+      const size_t head = (size_t)pg * Hkv + h;
+      const void* src = which ? vsrc : ksrc;
+      const int64_t r = pos - base_len;   // the first row of the group (of one that begins before the new rows, below 0)
+      const int64_t at = head_major ? (int64_t)r0 * Hkv * D + ((int64_t)h * nrows + r) * D + c : ((r0 + r) * Hkv + h) * D + c, step = head_major ? D : Hkv * D;
       Raw8<kF32> raw[kN];
 #pragma unroll
-      for (int q = 0; q < kN; q++) {
-        const size_t src_off = head_major ? ((size_t)r0 * Hkv * D + ((size_t)h * nrows + r + q) * D + c) : (((size_t)(r0 + r + q) * Hkv + h) * D + c);
-        if (pg[q] >= 0) raw[q].load(which ? vsrc : ksrc, src_off);
-      }
+      for (int q = 0; q < kN; q++)
+        if (q >= lo && q < hi) raw[q].load(src, at + q * step);
+      uint8_t* codes = (which ? v_base : k_base) + (head * kGqaPageTok + tok) * D + c;
+      float* scale = scales + (head * 2 + which) * kGqaPageTok + tok;
 #pragma unroll
       for (int q = 0; q < kN; q++) {
-        if (pg[q] < 0) continue;   // the same for the whole block
+        if (q < lo || q >= hi) continue;   // the same for the whole block
         float x[8];
         raw[q].values(x);
         const Int8Row row = int8_quantise(x, row_top(x));
-        const size_t head = (size_t)pg[q] * Hkv + h;
-        *reinterpret_cast<uint2*>((which ? v_base : k_base) + (head * kGqaPageTok + tok[q]) * D + c) = row.codes;
-        if (c == 0) scales[(head * 2 + which) * kGqaPageTok + tok[q]] = row.scale;
+        *reinterpret_cast<uint2*>(codes + q * D) = row.codes;
+        if (c == 0) scale[q] = row.scale;
       }
     }
   }
@@ -319,7 +330,7 @@ int32_t launch_gqa_append(Pool* p, const SeqBatch& sb, int layer, const void* k,
                           int advance) {
   const AppendGeom g = make_geom(p, sb, layer, advance);
   const int ahead = int8_rows_ahead(dtype == RELUX_DTYPE_F32);
-  const dim3 grid(sb.n_seqs, p->int8 ? std::min(std::max((sb.max_rows + ahead - 1) / ahead, 1), 65535) : row_slices(sb));
+  const dim3 grid(sb.n_seqs, p->int8 ? std::min((std::max(sb.max_rows, 1) + ahead - 2) / ahead + 1, 65535) : row_slices(sb));
   const int hm = layout == RELUX_LAYOUT_HEAD_MAJOR;
   const bool f32 = dtype == RELUX_DTYPE_F32;
   bool plain = true;   // sequences 0, 1, ... with the same rows each

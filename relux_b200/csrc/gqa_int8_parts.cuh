@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "gqa_parts.cuh"
+#include "softmax_parts.cuh"
 
 namespace relux {
 
@@ -52,36 +53,40 @@ __device__ __forceinline__ void load8(float (&x)[8], const uint16_t* src) {
   x[4] = bf16_lo(a.z); x[5] = bf16_hi(a.z); x[6] = bf16_lo(a.w); x[7] = bf16_hi(a.w);
 }
 // Largest magnitude of a row, as bits (larger for an infinity or a NaN than for any number), by the 16 lanes that hold it; the warp is converged.
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t row_top(const float (&x)[8]) {
-  uint32_t top = 0;
+  float m[4];
 #pragma unroll
-  for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 4; i++) m[i] = max_nan(fabsf(x[i]), fabsf(x[i + 4]));
+  float top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  return top;
+  for (int o = 1; o < 16; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return __float_as_uint(top);
 }
 struct Int8Row {
   uint2 codes;   // this lane's eight
   float scale;
 };
+// The warp is converged.  Of the two divisions a row needs, its even lanes do one and its odd lanes the other.
 __device__ __forceinline__ Int8Row int8_quantise(const float (&x)[8], uint32_t top) {
-  Int8Row r{{kInt8Zeros, kInt8Zeros}, 0.f};
-  const float a = __uint_as_float(top);
-  if (top >= 0x7F800000u) {
-    r.scale = __uint_as_float(0x7FC00000u);
-  } else if (a >= kInt8Tiny) {
-    const float inv = __fdiv_rn(127.f, a);
-    uint32_t w[2];
+  const bool odd = threadIdx.x & 1, some = top < 0x7F800000u && __uint_as_float(top) >= kInt8Tiny;
+  const float a = some ? __uint_as_float(top) : 127.f;
+  const float mine = __fdiv_rn(odd ? a : 127.f, odd ? 127.f : a), other = __shfl_xor_sync(0xffffffffu, mine, 1);
+  const float inv = odd ? other : mine;
+  Int8Row r;
+  r.scale = some ? (odd ? mine : other) : top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.f;
+  // 1.5 * 2^23 more is rounded to a whole number, as a conversion would (at a fourth of the rate), and has it in its low bits.  (One value at a time: a packed
+  // product and a packed sum came out as one rounding, which takes 63.5 of half of the largest value to 63, not 64.)
+  uint32_t c[8], w[2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      int c[4];
+  for (int i = 0; i < 8; i++) c[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
 #pragma unroll
-      for (int i = 0; i < 4; i++) c[i] = __float2int_rn(__fmul_rn(x[4 * h + i], inv));
-      w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-    }
-    r.codes = make_uint2(w[0] ^ kInt8Zeros, w[1] ^ kInt8Zeros);
-    r.scale = __fdiv_rn(a, 127.f);
-  }
+  for (int h = 0; h < 2; h++) w[h] = __byte_perm(__byte_perm(c[4 * h], c[4 * h + 1], 0x0040), __byte_perm(c[4 * h + 2], c[4 * h + 3], 0x0040), 0x5410) ^ kInt8Zeros;
+  r.codes = some ? make_uint2(w[0], w[1]) : make_uint2(kInt8Zeros, kInt8Zeros);
   return r;
 }
 template <typename T>

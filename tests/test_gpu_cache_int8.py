@@ -40,6 +40,16 @@ def read(pool, dev, layer, tok0, n, f32=True, seq_ids=None):
     return got if f32 else [orc.f32_from_bf16(x) for x in got]
 
 
+def bufs_dtype(f32):
+    from relux_b200 import lib as L
+    return L.DTYPE_F32 if f32 else L.DTYPE_BF16
+
+
+def orc_f32(bits):
+    from oracle import binding as orc
+    return orc.f32_from_bf16(bits)
+
+
 def same(a, b):
     return np.array_equal(np.asarray(a, np.float32).view(np.uint32), np.asarray(b, np.float32).view(np.uint32))
 
@@ -97,6 +107,26 @@ def test_rows_of_special_values(dev):
     assert np.isnan(k[4, 0]).all() and not np.isnan(k[4, 1]).any() and np.isnan(k[5, 1]).all()
     assert k[8, 1, 1] == 2 and (k[2] == 0).all()          # 2.5 lies between 2 and 3
     assert same(np.nan_to_num(v), np.nan_to_num(G.held(x[::-1], True)))
+    pool.destroy()
+
+
+@pytest.mark.parametrize("f32", [True, False])
+def test_read_kv_to_any_multiple_of_16(dev, f32):
+    """Places that are multiples of 16 bytes only; what lies before and behind them stays."""
+    rng = np.random.default_rng(5)
+    lens, Hkv, es = [130, 61], 3, 4 if f32 else 2
+    pool, _ = filled(dev, rng, lens, Hkv, Hkv, 0, int8=True)
+    want = read(pool, dev, 0, [1, 0], [129, 61], f32=True)
+    n = int(np.prod(want[0].shape))
+    for at_k, at_v in ((16, 16), (0, 48), (16, 32)):
+        bufs = [dev.upload(np.full(n * es // 4 + 32, 0x7B7B7B7B, np.uint32)) for _ in range(2)]
+        pool.read_kv(0, 2, bufs[0].ptr + at_k, bufs[1].ptr + at_v, [1, 0], [129, 61], dtype=bufs_dtype(f32))
+        for b, at, w in zip(bufs, (at_k, at_v), want):
+            raw = b.download((n * es + 128,), np.uint8)
+            assert (raw[:at] == 0x7B).all() and (raw[at + n * es:] == 0x7B).all()
+            got = raw[at:at + n * es].view(np.float32 if f32 else np.uint16).reshape(w.shape)
+            assert same(got, w) if f32 else same(orc_f32(got), G.bf16(w))
+            b.free()
     pool.destroy()
 
 

@@ -289,6 +289,76 @@ def test_pipelined_and_device_calls_agree(dev):
         pool.destroy()
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("H,S", [(8, 6), (32, 20), (64, 40)])
+def test_a_captured_call_runs_again(dev, int8, H, S):
+    """Append of uneven sequences and a tree's verify in a graph, launched twice, with other calls of the pool between; two such graphs share its workspaces."""
+    from oracle import binding as orc
+    from relux_b200 import lib as L
+    from tests.test_gpu_latent_graphs import Graph
+    rng = np.random.default_rng(S + int8)
+    Hkv, lens, n_new = 4, [100, 20, 301], [3, 1, 2]
+    pool, cache = filled(dev, rng, lens, H, Hkv, S + 8, int8=int8)
+    parents = np.stack([G.random_tree(rng, S) for _ in lens])
+    up = lambda x: dev.upload(orc.bf16_from_f32(x))  # noqa: E731
+    calls = []
+    for ids in ([0, 1, 2], [2, 0]):
+        n = [n_new[b] for b in ids]
+        k, v, q = G.rows(rng, S * len(ids), Hkv), G.rows(rng, S * len(ids), Hkv, "v"), G.bf16(rng.standard_normal((len(ids), S, H, D)))
+        bufs = [up(x) for x in (q, k, v, k[:sum(n)], v[:sum(n)])] + [dev.upload(np.full(q.shape, np.nan, np.float32))]
+
+        def call(ids=ids, n=n, bufs=bufs):
+            m = len(ids)
+            pool.append(0, bufs[3], bufs[4], m, seq_ids=ids, n_new=n, advance=False)
+            pool.tree_verify(0, m, bufs[0], bufs[5], bufs[1], bufs[2], H, D, D ** -0.5, parents[ids], seq_ids=ids)
+        calls.append((call, bufs, ids, q, k, v))
+    want = []
+    for call, bufs, ids, q, k, v in calls:
+        call()
+        want.append(bufs[5].download(q.shape, np.float32))
+        see = [G.ancestors(parents[b], S, S) for b in ids]
+        for i, b in enumerate(ids):
+            K, V = (np.concatenate([c, G.held(G.bf16(x[i * S:(i + 1) * S]), int8)]) for c, x in ((cache.k[b], k), (cache.v[b], v)))
+            exact, bound = G.attend(K, V, q[i], lens[b], see[i], D ** -0.5)
+            G.check(want[-1][i], exact, bound)
+    graphs = [Graph(dev, c[0]) for c in calls]
+    for _ in range(2):
+        for (call, bufs, ids, q, k, v), g, w in zip(calls, graphs, want):
+            bufs[5].zero()
+            g.launch()
+            assert same(bufs[5].download(q.shape, np.float32), w)
+    assert pool.status() == 0
+    for g in graphs:
+        g.free()
+    for c in calls:
+        for b in c[1]:
+            b.free()
+    pool.destroy()
+
+
+def test_two_handles_and_pools_in_turn(dev):
+    """The same calls on two pools of each of two handles, none waited for in between, are each other's equals."""
+    import relux_b200 as rb
+    rng = np.random.default_rng(3)
+    H, Hkv, S, lens = 32, 8, 24, [500, 70]
+    other = rb.Device(0)
+    parents = np.stack([G.random_tree(rng, S) for _ in lens])
+    k, v, q = G.rows(rng, 2 * S, Hkv), G.rows(rng, 2 * S, Hkv, "v"), G.bf16(rng.standard_normal((2, S, H, D)))
+    for int8 in (False, True):
+        pools = [filled(d, np.random.default_rng(4), lens, H, Hkv, S, int8=int8)[0] for d in (dev, other, dev, other)]
+        outs = [np.empty((2, S, H, D), np.float32) for _ in pools]
+        for _ in range(3):
+            for p, o in zip(pools, outs):
+                p.tree_verify(0, 2, q, o, k, v, H, D, D ** -0.5, parents)
+        dev.sync()
+        other.sync()
+        assert np.isfinite(outs[0]).all() and all(same(o, outs[0]) for o in outs[1:])
+        for p in pools:
+            assert p.status() == 0
+            p.destroy()
+    other.close()
+
+
 def test_refusals(dev):
     import relux_b200 as rb
     from relux_b200 import lib as L

@@ -92,9 +92,10 @@ __device__ __forceinline__ void put_codes(bool wide, void* to, size_t off, uint4
 }
 
 // 8-bit cache: grid (sequences, pages of one times parts, layers), a warp a head's rows of a page, of K or of V: eight lanes a row, 16 codes each, kCodesAhead
-// loads of four rows on their way (with a row's codes eight a lane, and blocks that looked up a page for every four tokens, 4 x 8192 tokens took 48 us).
+// loads of four rows on their way.  kFew: fewer rows of any page than those, and the warp takes them one head behind another (64 x 5 tokens of 32 layers: 20 us
+// one head at a time, 15 so; 8 x 2048 tokens 18 and 23).  (With a row's codes eight a lane, and blocks that looked up a page for every four tokens, 4 x 8192 tokens took 48 us.)
 constexpr int kCodesAhead = 8, kCodesWarps = 4;
-template <bool kF32, int N>
+template <bool kF32, bool kFew, int N>
 __global__ void __launch_bounds__(32 * kCodesWarps, 8) read_codes_kernel(const __grid_constant__ ReadParams<N> prm) {
   chain_release();
   chain_wait();
@@ -109,29 +110,47 @@ __global__ void __launch_bounds__(32 * kCodesWarps, 8) read_codes_kernel(const _
       continue;
     }
     const int base = slot * kGqaPageTok, lo = max(sq.tok0 - base, 0), hi = min(end - base, kGqaPageTok);
-    for (int u = part * kCodesWarps + warp; u < 2 * c.Hkv; u += c.parts * kCodesWarps) {
-      const int which = u >= c.Hkv, h = u - which * c.Hkv;
-      const size_t head = (size_t)pg * c.Hkv + h;
-      const uint8_t* codes = (const uint8_t*)(which ? c.v : c.k) + (size_t)blockIdx.z * c.layer_bytes + head * (kGqaPageTok * kGqaD) + d;
-      const float* scales = c.scales + (size_t)blockIdx.z * c.layer_scales + (head * 2 + which) * kGqaPageTok;
-      const int64_t row0 = (int64_t)blockIdx.z * c.rows + sq.row0 + base - sq.tok0;
-      for (int r0 = lo; r0 < hi; r0 += 4 * kCodesAhead) {
-        uint4 w[kCodesAhead];
-        float s[kCodesAhead];
-#pragma unroll
-        for (int q = 0; q < kCodesAhead; q++) {
-          const int r = r0 + 4 * q + sub;
-          if (r < hi) {
-            w[q] = load_chained(reinterpret_cast<const uint4*>(codes + r * kGqaD));
-            s[q] = load_chained(scales + r);
-          }
+    const int64_t row0 = (int64_t)blockIdx.z * c.rows + sq.row0 + base - sq.tok0;
+    // kCodesAhead groups of four rows at a time
+    const int step = c.parts * kCodesWarps;
+    auto load = [&](int u, int r, uint4& w, float& s) {   // K or V of a head, u, row r
+      if (u >= 2 * c.Hkv || r >= hi) return;
+      const int which = u >= c.Hkv;
+      const size_t head = (size_t)pg * c.Hkv + (u - which * c.Hkv);
+      const uint8_t* codes = (const uint8_t*)(which ? c.v : c.k) + (size_t)blockIdx.z * c.layer_bytes;
+      w = load_chained(reinterpret_cast<const uint4*>(codes + (head * kGqaPageTok + r) * kGqaD + d));
+      s = load_chained(c.scales + (size_t)blockIdx.z * c.layer_scales + (head * 2 + which) * kGqaPageTok + r);
+    };
+    auto put = [&](int u, int r, const uint4& w, float s) {
+      if (u >= 2 * c.Hkv || r >= hi) return;
+      const int which = u >= c.Hkv;
+      put_codes<kF32>(c.wide, which ? c.v_out : c.k_out, (size_t)((row0 + r) * c.Hkv + (u - which * c.Hkv)) * kGqaD + d, w, s);
+    };
+    uint4 w[kCodesAhead];
+    float s[kCodesAhead];
+    int u = part * kCodesWarps + warp;
+    if constexpr (kFew) {
+      auto next = [&](int& u, int& r) {
+        if ((r += 4) >= hi) {
+          r = lo;
+          u += step;
         }
+      };
+      for (int r = lo; u < 2 * c.Hkv;) {
+        int u1 = u, r1 = r;
 #pragma unroll
-        for (int q = 0; q < kCodesAhead; q++) {
-          const int r = r0 + 4 * q + sub;
-          if (r < hi) put_codes<kF32>(c.wide, which ? c.v_out : c.k_out, (size_t)((row0 + r) * c.Hkv + h) * kGqaD + d, w[q], s[q]);
-        }
+        for (int q = 0; q < kCodesAhead; q++, next(u1, r1)) load(u1, r1 + sub, w[q], s[q]);
+#pragma unroll
+        for (int q = 0; q < kCodesAhead; q++, next(u, r)) put(u, r + sub, w[q], s[q]);
       }
+    } else {
+      for (; u < 2 * c.Hkv; u += step)
+        for (int r0 = lo + sub; r0 < hi; r0 += 4 * kCodesAhead) {
+#pragma unroll
+          for (int q = 0; q < kCodesAhead; q++) load(u, r0 + 4 * q, w[q], s[q]);
+#pragma unroll
+          for (int q = 0; q < kCodesAhead; q++) put(u, r0 + 4 * q, w[q], s[q]);
+        }
     }
   }
   fence_chained_writes();
@@ -192,7 +211,7 @@ int32_t launch_read_n(Pool* p, const ReadCommon& c, const RowSeq* seqs, int n, i
   const int slices = p->int8 ? prm.c.parts * (int)std::max<int64_t>(1, std::min<int64_t>(pages, 65535 / prm.c.parts))
                              : std::min((most + kRowsAhead - 1) / kRowsAhead, std::max(1, 5 * p->dev->sm_count / (n * layers)));
   const int threads = p->int8 ? 32 * kCodesWarps : std::min(256, (2 * c.Hkv * (c.D / 8) + 31) / 32 * 32);
-  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, p->int8 ? read_codes_kernel<kF32, N> : read_kv_kernel<kF32, N>,
+  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, !p->int8 ? read_kv_kernel<kF32, N> : most < 4 * kCodesAhead ? read_codes_kernel<kF32, true, N> : read_codes_kernel<kF32, false, N>,
                                 dim3(n, slices, layers), dim3(threads), 0, p->dev->stream, prm));
   count_launch(p->dev);
   return RELUX_OK;

@@ -81,6 +81,7 @@ extern "C" {
  * 128 values, scale = a / 127 and number = value * (127 / a) to the nearest, even on a tie, each operation rounded to float32; a row with
  * a < 1e-36 is stored as zeros, one that holds an infinity or a NaN reads back as NaN in every place.  Rows are quantised as they are
  * appended, attention takes number * scale for the value, relux_pool_read_rows, relux_seq_save_file and relux_gqa_read_kv give it.
+ * Queries: up to 32 rows a kv head (heads of its group times query tokens) keep 11 bits of every value, of more rows 8 (bf16).
  * All calls of a GQA pool take such a pool in RELUX_ATTN_FAST; the two reference modes and relux_gqa_decode_noalloc refuse it. */
 #define RELUX_POOL_FLAG_CACHE_INT8 2
 
@@ -212,7 +213,7 @@ int32_t relux_pool_read_rows(relux_pool_t pool, const relux_read_rows_args* args
 
 /* Cached K and V rows of a batch of sequences, copied to dense device memory as float32 or bf16: tokens tok0[i] .. tok0[i] +
  * n_tokens[i] - 1 of every named sequence, one sequence behind the other, on one layer or on all.  An 8-bit cache's rows are number *
- * scale, rounded once; a bf16 cache's are its bits.  Asynchronous on the handle's stream.  KVCache.View (kvcache.go:363-380) for
+ * scale in float32, which for bf16 is rounded once more; a bf16 cache's are its bits.  Asynchronous on the handle's stream.  KVCache.View (kvcache.go:363-380) for
  * a batch, without the way through host memory. */
 typedef struct relux_read_kv_args {
   int32_t layer;             /* < 0: every layer, results [num_layers][sum of n_tokens][...] */

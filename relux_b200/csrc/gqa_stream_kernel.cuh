@@ -28,7 +28,10 @@
 // All mbarrier waits are bounded; a wait that runs out records RELUX_ERR_TIMEOUT and the CTA finishes with neutral data.
 //
 // Variants (template parameter V, a sum of kInt8 and kTree; 0 is the bf16 cache with a causal mask or none):
-//   kInt8   the pages hold int8 codes and a scale per row (gqa_int8_parts.cuh): a page is 16.5 KB instead of 32, in eight stages
+//   kInt8   the pages hold int8 codes and a scale per row (gqa_int8_parts.cuh): a page is 16.5 KB instead of 32, in eight stages.  A page takes the consumers as
+//           many MMAs as on bf16 and 200 instructions a warp more, for half the bytes, so they are the bound: 128 x 8192 tokens, four drafted, 459-474 us (4.7
+//           TB/s) where bf16 is 617 (6.9 TB/s).  What brought it there from 545: the next page's scores beside this page's exponentials and values, a
+//           maximum that is followed lazily, registers taken from the finishers.  (More of the pages asked for in L2 ahead of the ring: 468 -> 517 us.)
 //   kTree   the new rows are the nodes of a drafted tree: a query sees the cached rows and, of the new ones, itself and its ancestors
 #pragma once
 

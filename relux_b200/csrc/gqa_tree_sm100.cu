@@ -2,8 +2,10 @@
 // grouped-query cache, and prompts (or long verifies) over the 8-bit one.
 //
 // o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  where query token i sees every cached row and, of the drafted ones, itself
-// and its ancestors; of a prompt, every row up to its own.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128 operations for the 512 (264) bytes of
-// a token and kv head, so the cache's bytes bound trees of up to some 200 rows (100 on the 8-bit cache) and the tensor cores and the softmax larger ones.
+// and its ancestors; of a prompt, every row up to its own.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128
+// operations for the 512 (264) bytes of a token and kv head, so the cache's bytes bound trees of up to some 200 rows (100 on the 8-bit cache) and the tensor
+// cores and the softmax larger ones.  Measured: 64 x 8192 tokens, 64 rows 332 us on bf16 (6.5 TB/s), 410 on 8 bits (2.7 TB/s); 8 x 32768 tokens, 512 rows
+// 546 us (1.0 PFLOP/s), 660 on 8 bits.
 //
 // A STREAM is the tiles of 128 keys that up to 256 of a kv head's rows (one or two blocks of 128, M of both contractions) see.  All streams of the
 // call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into one equal range per SM; a PIECE is the part of a stream inside a range.
@@ -16,9 +18,13 @@
 //              scores, in float32.  V times its scale over a power of two that all of the piece's rows share so far (11 bits, as P has then; 2^29 between
 //              the largest row and one that is no longer exact to 11 bits); where a row comes that is too large for it, the power grows and O is rescaled.
 //   MMA        step k = (tile, block): S = Q K^T (S buffer k & 1), O[block] += P V with P read from tensor memory over the scores it came from
-//   softmax    eight warps of 16 rows of a block each, four lanes to a row: scores from TMEM, running max (updated lazily), P back to TMEM.  A tile takes a
-//              warp 2300 clocks, most of them latency.  Up to 64 rows, four warps take the even steps and four the odd ones, each with an O of its own,
+//   softmax    eight warps of 16 rows of a block each, four lanes to a row: scores from TMEM, running max (updated lazily), P back to TMEM.  Up to
+//              64 rows, four warps take the even steps and four the odd ones, each with an O of its own,
 //              which meet at the piece's end.
+// What bounds it.  bf16, up to 64 rows: HBM.  More rows: the softmax warps, for whom a step of 128 rows takes 1550 clocks (2570 beside converters), most of it
+// the latency of their instructions (512 of exponentials a warp), against 1020 of MMAs.  8 bits, up to 64 rows: converters and softmax share issue slots and
+// shared memory, through which a tile's operands, codes and queries come to 1760 clocks, and each alone adds a fourth to what the rest takes: 410 us of 64 x 8192
+// tokens were 300 without the converters' work, 332 without the softmax's, 234 without either.
 // Order of issue: QK(k + 1), PV(k): the tensor pipe executes in issue order, so QK(k + 2) finds its S buffer read.
 // A product with P = 0 does not hide an infinity or a NaN among the values: those of drafted rows and of what lies behind are set to zero in the tile, and
 // the rows that see one become NaN at the end.  (8-bit rows have them in their scale alone; a code is always a number.)
@@ -192,14 +198,15 @@ struct Plan {
   static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, see) + sizeof(Bars::see));
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
   static constexpr int kWarpLoad = kSoftmaxWarps + (kI8 ? 2 * kConvWarps : 0), kWarpMma = kWarpLoad + 1;
-  // Four more warps where registers are dealt out anew, which warps do by fours: softmax 152, converters 64, the others 48 of the 96 of the launch.
+  // Four more warps where registers are dealt out anew, of the 96 of the launch, which warps do by fours.  (With 152, 64 and 48 the warp that issues the MMAs
+  // kept a pointer in local memory, and 8 x 32768 tokens, 64 nodes, 64 heads took 934 us where it is 770 with these.)
   static constexpr int kThreads = 32 * (kI8 ? kWarpLoad + 4 : kWarpMma + 1);
   static constexpr int kRegsSoftmax = 144, kRegsConv = 64, kRegsOther = 64;
   static_assert(!kI8 || 256 * kRegsSoftmax + 256 * kRegsConv + 128 * kRegsOther <= 640 * 96, "more registers than the block is launched with");
 };
 // The wait that gives up raises the flag, which ends all others; the kernel's end reports it.  Short, and not a function of its own: a call takes registers that
 // a role may have given back, and the roles of a block share one instruction cache.  (With the report and a pause in every wait, and all loops of the
-// converters unrolled, the 8-bit kernel waited 5.3 cycles for an instruction per one issued; 16 x 8192 tokens, 64 rows, took 149 us.)
+// converters unrolled, the 8-bit kernel waited 5.3 cycles for an instruction per one issued, now 0.6 to 1.4; 16 x 8192 tokens, 64 rows, took 149 us, now 113.)
 __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, Bars* b) {
   for (uint32_t i = 0; !mbar_try_wait(bar, parity); i++)
     if (i >= kSpinLimit || b->abort_flag) {

@@ -49,7 +49,9 @@ constexpr int kHalf = 16384;                   // [128 rows][64 16-bit columns],
 constexpr int kSlot = 2 * kHalf;               // K or V of a tile, or 128 query rows
 constexpr int kRawSlot = kPage * kD;           // codes of K or V of a page
 constexpr int kTilesAhead = 4;                 // (8-bit cache) of a tile in L2 before its loads
-constexpr int kFixUnits = 2;                   // tiles: what a piece costs beyond its own (queries in, results out)
+// Tiles: what a piece costs beyond its own (queries in, results out).  With 1, 2 and 4: 100 x 700 tokens, 64 rows, 8 bits 101, 99.5, 96 us; 4 x 500 tokens behind
+// 1500 122, 123, 119; 40 x 1500, 64 rows, bf16 53.5, 51.6, 51.2; long ones the same.
+constexpr int kFixUnits = 4;
 constexpr int kSoftmaxWarps = 8, kConvWarps = 4;   // of K, and of V
 constexpr int kWarpScale = kSoftmaxWarps + 2 * kConvWarps + 2;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
@@ -538,33 +540,13 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
                      "l"(__cvta_generic_to_global(src)), "r"(there ? 16 : 0)
                      : "memory");
       }
-      // What the rows see, a row a lane (16).  A tree's parents two a lane, so that a node's way up is one of shuffles.
-      uint32_t up2 = 0xffffu;
-      if (c.tree && 2 * lane < c.S) up2 = reinterpret_cast<const uint16_t*>(c.seqs ? c.parents + (c.one_tree ? 0 : sq.i) * kTreeNodes : prm.parents[c.one_tree ? 0 : sq.i])[lane];
-#pragma unroll 1
-      for (int b = 0; b < nb; b++, next_block()) {
-        const int row = 128 * b + 16 * row_warp + (lane & 15), s = token_of(c, sq.row0 + row);
-        uint64_t see = 0;
-        if (c.tree) {
-          int j = row < rows && s < sq.end - sq.len0 ? s : -1;
-          while (__any_sync(0xffffffffu, j >= 0)) {
-            const uint32_t pair = __shfl_sync(0xffffffffu, up2, (j & 63) >> 1);
-            if (j >= 0) {
-              see |= 1ull << j;
-              j = (int8_t)(pair >> (8 * (j & 1)));
-            }
-          }
-        } else if (c.causal) {
-          see = s - token_of(c, sq.row0);
-        }
-        if (lane < 16) bars->see[row] = see;
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-          st.m[hf] = -INFINITY;
-          st.l[hf] = 0.f;
-          st.f[hf] = c.scale_log2;
-        }
+      for (int hf = 0; hf < 2; hf++) {
+        st.m[hf] = -INFINITY;
+        st.l[hf] = 0.f;
+        st.f[hf] = c.scale_log2;
       }
+      other = st;
       asm volatile("cp.async.wait_all;" ::: "memory");
       if constexpr (kI8) {   // in place to binary16, by a power of two a row
 #pragma unroll 1
@@ -596,6 +578,31 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->q_full);
+      // What the rows see, a row a lane (16), while the first scores are on their way, and only of a piece that has tiles in which rows differ.  A tree's
+      // parents two a lane, so that a node's way up is one of shuffles.
+      if (p.te * kTile > sq.len0) {
+        uint32_t up2 = 0xffffu;
+        if (c.tree && 2 * lane < c.S) up2 = reinterpret_cast<const uint16_t*>(c.seqs ? c.parents + (c.one_tree ? 0 : sq.i) * kTreeNodes : prm.parents[c.one_tree ? 0 : sq.i])[lane];
+#pragma unroll 1
+        for (int b = 0; b < nb; b++) {
+          const int row = 128 * b + 16 * row_warp + (lane & 15), s = token_of(c, sq.row0 + row);
+          uint64_t see = 0;
+          if (c.tree) {
+            int j = row < rows && s < sq.end - sq.len0 ? s : -1;
+            while (__any_sync(0xffffffffu, j >= 0)) {
+              const uint32_t pair = __shfl_sync(0xffffffffu, up2, (j & 63) >> 1);
+              if (j >= 0) {
+                see |= 1ull << j;
+                j = (int8_t)(pair >> (8 * (j & 1)));
+              }
+            }
+          } else if (c.causal) {
+            see = s - token_of(c, sq.row0);
+          }
+          if (lane < 16) bars->see[row] = see;
+        }
+        __syncwarp();
+      }
       // ---- tiles ----
       const int first = two && (k0 & 1) != set ? p.tb + 1 : p.tb;
       float v_unit = 1.f, shrink = 1.f;   // O's unit, and what it has grown by
@@ -758,7 +765,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             m = top;
           }
           const int row = 128 * b + row_in + 8 * hf;
-          const uint64_t see = bars->see[row];
+          const uint64_t see = bars->see[row];   // nobody's where the piece has none, and then no node of it is bad
           if (bad_all || (c.tree ? (see & bad_nodes) != 0 : bad_nodes != 0 && (int)see > (int)~(uint32_t)bad_nodes)) l = __uint_as_float(0x7FC00000u);
           const bool there = ok && row < rows && (!c.tree || token_of(c, sq.row0 + row) < sq.end - sq.len0);
           // no part of a sum that nobody has added to, of a row that is not there: zero whatever the accumulator holds

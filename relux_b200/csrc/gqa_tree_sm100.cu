@@ -1050,6 +1050,7 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   const relux_pool_params& prm = p->prm;
   const int n = sb.n_seqs, Hkv = prm.gqa_num_kv_heads, g = a.num_heads / Hkv, S = a.q_tokens;
   const int64_t R = (int64_t)g * S;
+  if (a.q_dtype != RELUX_DTYPE_BF16) { set_error("queries of this kernel are bf16"); return RELUX_ERR_UNSUPPORTED; }
   TreeCommon c{};
   c.n_rb = (int)((R + 255) / 256);
   c.rows_rb = (int)((R + c.n_rb - 1) / c.n_rb + 15) / 16 * 16;

@@ -294,16 +294,17 @@ def test_many_sequences(dev):
     pool.destroy()
 
 
-def test_a_layer_step(dev):
-    """relux_gqa_forward_cached on an 8-bit pool: its attention over the rows that the pool holds afterwards."""
+@pytest.mark.parametrize("calls", [(1, 2), (20, 1)])
+def test_a_layer_step(dev, calls):
+    """relux_gqa_forward_cached on an 8-bit pool: its attention over the rows that the pool holds afterwards; of a step and of a prompt."""
     from oracle import binding as orc
     rng = np.random.default_rng(9)
     H, Hkv, lens, dm = 2, 1, [90, 0], 256
-    pool, cache = filled(dev, rng, lens, H, Hkv, 4)
+    pool, cache = filled(dev, rng, lens, H, Hkv, 24)
     w = {n: orc.bf16_from_f32(rng.standard_normal((dm, c)).astype(np.float32) * dm ** -0.5) for n, c in (("w_q", dm), ("w_k", D), ("w_v", D), ("w_o", dm))}
     dw = {n: dev.upload(x) for n, x in w.items()}
     f = {n: orc.f32_from_bf16(x).astype(np.float64) for n, x in w.items()}
-    for S in (1, 2):
+    for S in calls:
         before = [pool.seq_len(0, b) for b in range(2)]
         x, out = rng.standard_normal((2, S, dm)).astype(np.float32), np.empty((2, S, dm), np.float32)
         pool.forward_cached(0, 2, x, out, dw, dm, H, q_tokens=S, rope=False)

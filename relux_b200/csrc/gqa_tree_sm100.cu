@@ -8,7 +8,8 @@
 // 546 us (1.0 PFLOP/s), 660 on 8 bits.
 //
 // A STREAM is the tiles of 128 keys that up to 256 of a kv head's rows (one or two blocks of 128, M of both contractions) see.  All streams of the
-// call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into one equal range per SM; a PIECE is the part of a stream inside a range.
+// call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into a range per SM (make_ranges); a PIECE is the part of a stream inside a
+// range.
 // A piece that is a whole stream writes its output; others leave float32 partials that merge_tree_kernel joins.
 //
 // Roles of a CTA:
@@ -60,6 +61,7 @@ constexpr float kRescaleThreshold = 8.0f;      // log2: P reaches 2^8 before the
 // of the row's largest, and below are off by at most 2^-32 of it.
 constexpr float kPUp = 7.0f;
 constexpr int kInlineSmall = 32, kInlineLarge = 256;
+constexpr int kMaxWorkers = 160;
 
 // A group of rows of a sequence: rows [row0, row0 + rows_rb) of every kv head.
 struct TreeSeq {
@@ -74,7 +76,7 @@ struct TreeCommon {
   int32_t one_tree, tree;      // tree = 0: query token s sees tokens below row_end + s (causal), or below row_end
   int32_t causal;
   const int32_t* table;
-  int32_t table_stride, num_pages, n_seqs, range, range_more, Hkv, H, g, S, R;
+  int32_t table_stride, num_pages, n_seqs, Hkv, H, g, S, R;
   uint32_t over_g;             // 2^31 / g, rounded up: a row below 2^26 over g is a product (a division by g a row was half of a piece's fixed cost)
   int32_t n_rb, rows_rb;       // groups of a sequence, rows of each (the last may have fewer)
   int32_t krow0, vrow0;
@@ -94,6 +96,7 @@ struct TreeParams {
   TreeCommon c;
   TreeSeq seqs[N + 1];
   alignas(2) int8_t parents[N][kTreeNodes];
+  int32_t cuts[kMaxWorkers + 1];   // ranges: units cuts[w] to cuts[w + 1]
 };
 
 __device__ __forceinline__ int token_of(const TreeCommon& c, int row) { return (int)__umulhi(2u * (uint32_t)row, c.over_g); }
@@ -107,14 +110,9 @@ template <int N>
 struct Streams {
   const TreeParams<N>& prm;
   int32_t u_begin, u_end;
-  __device__ __forceinline__ Streams(const TreeParams<N>& p, int worker) : prm(p), u_begin(range_begin(worker)), u_end(range_begin(worker + 1)) {}
+  __device__ __forceinline__ Streams(const TreeParams<N>& p, int worker) : prm(p), u_begin(p.cuts[worker]), u_end(p.cuts[worker + 1]) {}
   __device__ __forceinline__ int unit0(int e) const { return prm.c.seqs ? prm.c.seqs[e].unit0 : prm.seqs[e].unit0; }
   __device__ __forceinline__ TreeSeq seq(int e) const { return prm.c.seqs ? prm.c.seqs[e] : prm.seqs[e]; }
-  __device__ __forceinline__ int range_begin(int w) const { return w * prm.c.range + min(w, prm.c.range_more); }
-  __device__ __forceinline__ int worker_of(int u) const {
-    const int big = prm.c.range_more * (prm.c.range + 1);
-    return u < big ? (int)((unsigned)u / (unsigned)(prm.c.range + 1)) : prm.c.range_more + (int)((unsigned)(u - big) / (unsigned)prm.c.range);
-  }
   __device__ __forceinline__ void cut(Piece& p) const {
     if (p.us >= u_end) return;
     p.tiles = unit0(p.e + 1) - unit0(p.e) - kFixUnits;
@@ -308,9 +306,14 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   chain_release();
+  if (c.seqs) chain_wait();   // the list is a copy that was queued just before this launch
+  const Streams<N> streams(prm, blockIdx.x);
+  // With one block the search for it is there once, before the wait, which shortens the code (64 x 8192 tokens, 64 rows, 8 bits: 424 -> 390 us; with two
+  // blocks a piece held from there on costs registers: 8 x 32768 tokens of 512 rows 651 -> 771).
+  const Piece shared_first = kNB == 1 ? streams.first() : Piece{};
+  auto first_piece = [&]() -> Piece { return kNB == 1 ? shared_first : streams.first(); };
   chain_wait();
   if (threadIdx.x == 0) stamp_begin(c.time);
-  const Streams<N> streams(prm, blockIdx.x);
   auto rows_of = [&](const TreeSeq& sq) -> int { return min(c.rows_rb, c.R - sq.row0); };
   auto blocks_of = [&](const TreeSeq& sq) -> int { return kNB == 1 ? 1 : (rows_of(sq) + 127) / 128; };
 
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     // =============================== producer ===============================
     const bool el = elect_one();
     int h = 0;   // half tiles so far: K of tile n is 2 n, V 2 n + 1
-    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p)) {
+    for (Piece p = first_piece(); streams.valid(p); p = streams.next(p)) {
       const TreeSeq sq = streams.seq(p.e);
       const int kvh = p.kvh;
       const int last_slot = max(0, (sq.end + kPage - 1) / kPage - 1);   // a tile's second page may lie past the rows: nobody sees those keys
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     constexpr uint32_t idesc_qk = idesc_of(kI8, false), idesc_pv = idesc_of(kI8, true);
     const uint64_t dQ = make_desc_kmajor_sw128(smem_u32(smem + PL::kQ));
     int k = 0, tt = 0, n = 0;   // steps, tiles, pieces so far
-    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+    for (Piece p = first_piece(); streams.valid(p); p = streams.next(p), n++) {
       const TreeSeq sq = streams.seq(p.e);
       const int nb = blocks_of(sq), tiles = p.te - p.tb;
       wait_bar(&bars->q_full, n & 1, bars);   // the queries are there, and O of the piece before has been read
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     const int r16 = (warp & 3) * 32 + (two ? 0 : (warp >> 2) * 16), row_in = 16 * row_warp + (lane >> 2);
     const uint32_t lane_addr = (uint32_t)r16 << 16;
     int k0 = 0, tt0 = 0, n = 0;   // steps, tiles and pieces before this one
-    for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+    for (Piece p = first_piece(); streams.valid(p); p = streams.next(p), n++) {
       const TreeSeq sq = streams.seq(p.e);
       const int nb = blocks_of(sq), rows = rows_of(sq), tiles = p.te - p.tb;
       struct State {
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       // =============================== scales ===============================
       regs_down<PL::kRegsOther, kI8>();
       int tt = 0, n = 0;
-      for (Piece p = streams.first(); streams.valid(p); p = streams.next(p), n++) {
+      for (Piece p = first_piece(); streams.valid(p); p = streams.next(p), n++) {
         const TreeSeq sq = streams.seq(p.e);
         ValueUnit unit;
         for (int t = p.tb; t < p.te; t++, tt++) {
@@ -913,7 +916,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         }
       };
       int tt = 0, st = 0, phase = 1;   // tiles so far; the next slot of the ring of operands, whose first use waits for nothing
-      for (Piece p = streams.first(); streams.valid(p); p = streams.next(p))
+      for (Piece p = first_piece(); streams.valid(p); p = streams.next(p))
         for (int t = p.tb; t < p.te; t++, tt++) {
           if (!of_v) {
             wait_bar(&bars->empty[st], phase, bars);
@@ -967,10 +970,12 @@ __global__ void __launch_bounds__(256, 4) merge_tree_kernel(const __grid_constan
   const Streams<N> streams(prm, blockIdx.x + 1);
   const int u = streams.u_begin, lane = threadIdx.x & 31;
   const Piece p = streams.at(u);
-  const int w0 = streams.worker_of(p.us), np = streams.worker_of(p.us + p.tiles - 1) - w0 + 1;
-  if (p.tb <= 0 || p.tb >= p.tiles || w0 != (int)blockIdx.x) return;   // no stream goes on here, or its first part is further back
+  const int w0 = blockIdx.x;
+  if (p.tb <= 0 || p.tb >= p.tiles || prm.cuts[w0] > p.us) return;   // no stream goes on here, or its first part is further back
+  int np = 2;
+  while (w0 + np <= (int)gridDim.x && prm.cuts[w0 + np] < p.us + p.tiles) np++;
   const TreeSeq sq = streams.seq(p.e);
-  const int rows = min(c.rows_rb, c.R - sq.row0), first = streams.range_begin(w0) == p.us ? 0 : 1;
+  const int rows = min(c.rows_rb, c.R - sq.row0), first = prm.cuts[w0] == p.us ? 0 : 1;
 #pragma unroll 2
   for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
     float M = -INFINITY, L = 0.f;
@@ -1017,28 +1022,101 @@ __global__ void __launch_bounds__(256, 4) merge_tree_kernel(const __grid_constan
 }
 
 template <bool kI8, int kNB, int N>
-int32_t launch(Pool* p, const TreeParams<N>& prm, int workers) {
+int32_t launch(Pool* p, const TreeParams<N>& prm, int workers, bool parts) {
   using PL = Plan<kI8, kNB>;
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
   if (int32_t rc = allow_smem(p->dev, tree_sm100_kernel<kI8, kNB, N>, PL::kTotal)) return rc;
   RELUX_CUDA_TRY(launch_chained(chained, tree_sm100_kernel<kI8, kNB, N>, dim3(workers), dim3(PL::kThreads), (size_t)PL::kTotal, p->dev->stream, p->tmap_gqa, prm));
   count_launch(p->dev);
-  if (workers > 1) {
+  if (parts) {
     RELUX_CUDA_TRY(launch_chained(chained, merge_tree_kernel<N>, dim3(workers - 1, (prm.c.rows_rb + 8 * kMergeRows - 1) / (8 * kMergeRows)), dim3(256), 0, p->dev->stream, prm));
     count_launch(p->dev);
   }
   return RELUX_OK;
 }
+// The ranges.  Equal ones cut nearly every stream where there are about as many streams as SMs: two parts an SM, each with its queries, its float32 sums out and
+// in again, and a launch that joins them.  So where there are few streams a range (kPackStreams), whole ones are dealt out as well, in their order and none cut that
+// is no longer than the longest range, and taken where that longest range is no more than what the parts would cost.  (16 x 3000 tokens of 240 rows, 128
+// streams: 86 us with equal ranges, PACKED_A with whole streams; 4 x 500 tokens behind 1500, 256 streams, 143 and PACKED_B.)
+struct Ranges {
+  int32_t cuts[kMaxWorkers + 1];
+  int workers;
+  bool parts;   // some stream is in several ranges
+};
+constexpr int kPackStreams = 3;             // of a range, at most
+
+// Whole streams in their order, ranges of up to `most` units; false: that takes more than `workers`.
+bool pack_streams(const TreeSeq* seqs, int n, int n_rb, int Hkv, int workers, int64_t most, int part, Ranges& out) {
+  int w = 0;
+  int64_t room = most, pos = 0;
+  out.cuts[0] = 0;
+  out.parts = false;
+  for (int i = 0; i < n; i++)
+    for (int h = 0; h < Hkv; h++)
+      for (int e = i * n_rb; e < (i + 1) * n_rb; e++) {
+        const int units = seqs[e + 1].unit0 - seqs[e].unit0, tiles = units - kFixUnits;
+        for (int done = 0; done < tiles;) {
+          const int rest = tiles - done, need = rest + kFixUnits + (done ? part : 0);
+          if (need <= room) {
+            room -= need;
+            done = tiles;
+          } else {
+            const int64_t fit = room - kFixUnits - part;   // tiles of a part
+            if (units > most && fit >= 4) {
+              done += (int)std::min<int64_t>(fit, rest - 1);
+              out.parts = true;
+            } else if (room == most) {
+              return false;
+            }
+            if (++w == workers) return false;
+            out.cuts[w] = (int32_t)(pos + done);
+            room = most;
+          }
+        }
+        pos += units;
+      }
+  out.workers = w + 1;
+  out.cuts[w + 1] = (int32_t)pos;
+  return true;
+}
+Ranges make_ranges(const TreeSeq* seqs, int n, int n_rb, int Hkv, int units, int sm_count, int blocks) {
+  const int part = blocks, join = blocks == 2 ? 5 : 2;   // tiles: what a part costs beyond a whole stream, and the join of all (parts of one block: half the bytes)
+  Ranges r;
+  r.workers = std::max(1, std::min({sm_count, kMaxWorkers, units / (kFixUnits + 1)}));
+  for (int w = 0; w <= r.workers; w++) r.cuts[w] = w * (units / r.workers) + std::min(w, units % r.workers);
+  r.parts = r.workers > 1;
+  const int64_t streams = (int64_t)n * n_rb * Hkv;
+  if (2 * streams >= r.workers && streams <= (int64_t)kPackStreams * r.workers) {
+    const int64_t equal = (units + r.workers - 1) / r.workers, cost = equal + kFixUnits + 2 * part + join;
+    Ranges best;
+    int64_t lo = equal - 1, hi = cost + 1;   // lo: too few; hi: not looked at, or found
+    while (hi - lo > 1) {
+      const int64_t most = (lo + hi) / 2;
+      Ranges some;
+      if (pack_streams(seqs, n, n_rb, Hkv, r.workers, most, part, some)) {
+        best = some;
+        hi = most;
+      } else {
+        lo = most;
+      }
+    }
+    if (hi + (hi <= cost && best.parts ? join : 0) <= cost) return best;
+  }
+  return r;
+}
+
 template <int N>
-int32_t launch_n(Pool* p, const TreeCommon& c, const TreeSeq* seqs, const GqaTree* tree, int workers) {
+int32_t launch_n(Pool* p, const TreeCommon& c, const TreeSeq* seqs, const GqaTree* tree, const Ranges& ranges) {
+  const int workers = ranges.workers;
   TreeParams<N> prm;
   prm.c = c;
+  memcpy(prm.cuts, ranges.cuts, sizeof(int32_t) * ((size_t)workers + 1));
   if (!c.seqs) {
     memcpy(prm.seqs, seqs, sizeof(TreeSeq) * ((size_t)c.n_seqs * c.n_rb + 1));
     if (tree) memcpy(prm.parents, tree->parents, (size_t)kTreeNodes * (tree->one ? 1 : c.n_seqs));
   }
-  if (p->int8) return c.rows_rb <= 128 ? launch<true, 1, N>(p, prm, workers) : launch<true, 2, N>(p, prm, workers);
-  return c.rows_rb <= 128 ? launch<false, 1, N>(p, prm, workers) : launch<false, 2, N>(p, prm, workers);
+  if (p->int8) return c.rows_rb <= 128 ? launch<true, 1, N>(p, prm, workers, ranges.parts) : launch<true, 2, N>(p, prm, workers, ranges.parts);
+  return c.rows_rb <= 128 ? launch<false, 1, N>(p, prm, workers, ranges.parts) : launch<false, 2, N>(p, prm, workers, ranges.parts);
 }
 
 }  // namespace
@@ -1078,8 +1156,8 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   }
   seqs[(size_t)groups] = TreeSeq{0, 0, 0, 0, 0, (int32_t)units64};
   const int units = (int)(units64 * Hkv);
-  const int workers = std::max(1, std::min(p->dev->sm_count, units / (kFixUnits + 1)));
-  const size_t part_rows = (size_t)2 * workers * c.rows_rb;
+  const Ranges ranges = make_ranges(seqs.data(), n, c.n_rb, Hkv, units, p->dev->sm_count, c.rows_rb <= 128 ? 1 : 2);
+  const size_t part_rows = (size_t)2 * ranges.workers * c.rows_rb;
   int32_t rc = grow(p->dev, p->part_o, part_rows * (kD + 2) * sizeof(float));
   if (rc) return rc;
   if (groups > kInlineLarge) {
@@ -1102,8 +1180,6 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.table_stride = prm.max_pages_per_seq;
   c.num_pages = prm.num_pages;
   c.n_seqs = n;
-  c.range = units / workers;
-  c.range_more = units % workers;
   c.Hkv = Hkv;
   c.H = a.num_heads;
   c.g = g;
@@ -1125,7 +1201,7 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.part_ml = c.part_o + part_rows * kD;
   c.status = p->d_status;
   c.time = time_stamp_next(p, p->attn_times);
-  rc = groups <= kInlineSmall || c.seqs ? launch_n<kInlineSmall>(p, c, seqs.data(), tree, workers) : launch_n<kInlineLarge>(p, c, seqs.data(), tree, workers);
+  rc = groups <= kInlineSmall || c.seqs ? launch_n<kInlineSmall>(p, c, seqs.data(), tree, ranges) : launch_n<kInlineLarge>(p, c, seqs.data(), tree, ranges);
   if (rc) return rc;
   time_stamp_done(p->attn_times, c.time);
   return RELUX_OK;

@@ -164,11 +164,12 @@ struct Streams {
 };
 
 struct Bars {
-  uint64_t full[6], empty[6], raw_full[9], raw_empty[9], scale_full[4], scale_empty[4], info[4], info_empty[4], s_full[2], p_full[2], q_full, pv, fin, drain;
+  uint64_t full[6], empty[6], s_full[2], p_full[2], q_full, pv, fin, drain;
   uint32_t tmem_base;
   volatile int32_t abort_flag;
+  int32_t first[4];            // piece of this range: its e, kvh, us, tb
   uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
-  uint32_t bad_all[4];         // (8-bit cache) a cached row with one
+  uint32_t bad_all;            // (8-bit cache) a cached row with one, a bit a piece
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
   union {
     uint64_t see[256];         // what a row sees: of the nodes (a bit each), or how many tokens from len0 on
@@ -178,7 +179,9 @@ struct Bars {
     };
   };
   alignas(16) uint32_t v_scale[4][kTile];   // (8-bit cache) of a tile's values, over their unit, binary16 twice
-  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys.  Without an 8-bit cache there is no room for these two, nor with two blocks for `halves`
+  alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys
+  uint64_t raw_full[9], raw_empty[9], scale_full[4], scale_empty[4], info[4], info_empty[4];
+  // Without an 8-bit cache there is no room for these from v_scale on, nor with two blocks for `halves`.
 };
 
 template <bool kI8, int kNB>
@@ -273,18 +276,20 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       mbar_init(&bars->full[s], kI8 ? kConvWarps : 1);
       mbar_init(&bars->empty[s], 1);
     }
-    for (int s = 0; s < 9; s++) {
-      mbar_init(&bars->raw_full[s], 1);
-      mbar_init(&bars->raw_empty[s], kConvWarps);
+    if constexpr (kI8) {
+      for (int s = 0; s < 9; s++) {
+        mbar_init(&bars->raw_full[s], 1);
+        mbar_init(&bars->raw_empty[s], kConvWarps);
+      }
+      for (int s = 0; s < 4; s++) {
+        mbar_init(&bars->scale_full[s], 1);
+        mbar_init(&bars->scale_empty[s], 1);
+        mbar_init(&bars->info[s], 1);
+        mbar_init(&bars->info_empty[s], (two ? kSoftmaxWarps / 2 : kSoftmaxWarps) + kConvWarps);
+      }
     }
-    for (int s = 0; s < 4; s++) {
-      mbar_init(&bars->scale_full[s], 1);
-      mbar_init(&bars->scale_empty[s], 1);
-      mbar_init(&bars->info[s], 1);
-      mbar_init(&bars->info_empty[s], (two ? kSoftmaxWarps / 2 : kSoftmaxWarps) + kConvWarps);
-      bars->bad_nodes[s] = 0;
-      bars->bad_all[s] = 0;
-    }
+    for (int s = 0; s < 4; s++) bars->bad_nodes[s] = 0;
+    bars->bad_all = 0;
     for (int s = 0; s < 2; s++) {
       mbar_init(&bars->s_full[s], 1);
       mbar_init(&bars->p_full[s], two ? kSoftmaxWarps / 2 : kSoftmaxWarps);
@@ -297,6 +302,18 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     fence_mbar_init();
     tma_prefetch_desc(&tmap);
   }
+  const Streams<N> streams(prm, blockIdx.x);
+  // (One block) the first piece, of every role, is searched for by one thread, before the wait for the launch ahead: the search in every role was a good
+  // part of the roles' code, which share one instruction cache (64 x 8192 tokens, 64 rows, 8 bits: 424 us, 389 so; 100 x 700 97 and 94).  With two blocks the steps
+  // come out of the compiler slower for it, whatever its reason: 8 x 32768 tokens of 512 rows 648 us and 807.
+  if (kNB == 1 && threadIdx.x == 32) {
+    if (c.seqs) chain_wait();   // the list is a copy that was queued just before this launch
+    const Piece p = streams.first();
+    bars->first[0] = p.e;
+    bars->first[1] = p.kvh;
+    bars->first[2] = p.us;
+    bars->first[3] = p.tb;
+  }
   if (warp == 0) {
     tmem_alloc<1>(&bars->tmem_base, kTmemCols);
     tmem_relinquish<1>();
@@ -306,14 +323,14 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   chain_release();
-  if (c.seqs) chain_wait();   // the list is a copy that was queued just before this launch
-  const Streams<N> streams(prm, blockIdx.x);
-  // With one block the search for it is there once, before the wait, which shortens the code (64 x 8192 tokens, 64 rows, 8 bits: 424 -> 390 us; with two
-  // blocks a piece held from there on costs registers: 8 x 32768 tokens of 512 rows 651 -> 771).
-  const Piece shared_first = kNB == 1 ? streams.first() : Piece{};
-  auto first_piece = [&]() -> Piece { return kNB == 1 ? shared_first : streams.first(); };
   chain_wait();
   if (threadIdx.x == 0) stamp_begin(c.time);
+  auto first_piece = [&]() -> Piece {
+    if constexpr (kNB == 2) return streams.first();
+    Piece p{bars->first[0], bars->first[1], bars->first[2], bars->first[3], 0, 0};
+    streams.cut(p);
+    return p;
+  };
   auto rows_of = [&](const TreeSeq& sq) -> int { return min(c.rows_rb, c.R - sq.row0); };
   auto blocks_of = [&](const TreeSeq& sq) -> int { return kNB == 1 ? 1 : (rows_of(sq) + 127) / 128; };
 
@@ -741,7 +758,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       tc_fence_after();
       const bool ok = bars->abort_flag == 0;
       const uint64_t bad_nodes = bars->bad_nodes[n & 3];
-      const bool bad_all = bars->bad_all[n & 3] != 0, whole = p.tb == 0 && p.te == p.tiles;
+      const bool bad_all = bars->bad_all >> (n & 3) & 1u, whole = p.tb == 0 && p.te == p.tiles;
       const int slot = 2 * (int)blockIdx.x + (p.us + p.tb == streams.u_begin ? 0 : 1);
 #pragma unroll 1
       for (int b = 0; b < nb; b++, next_block()) {
@@ -817,7 +834,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       }
       if (warp == 0 && lane == 0) {   // of piece n + 4; who writes it next has come through q_full of piece n + 1
         bars->bad_nodes[n & 3] = 0;
-        bars->bad_all[n & 3] = 0;
+        atomicAnd(&bars->bad_all, ~(1u << (n & 3)));
       }
       tc_fence_before();
       __syncwarp();
@@ -848,7 +865,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             if (i >= there) v[i] = 0.f;   // behind the drafted rows, where anything may lie
             if (!(v[i] == v[i])) {        // the row held an infinity or a NaN
               const int node = pos + i - sq.len0;
-              if (node < 0) atomicOr(&bars->bad_all[n & 3], 1u);
+              if (node < 0) atomicOr(&bars->bad_all, 1u << (n & 3));
               else if (!c.tree) atomicMax(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), (unsigned long long)~(uint32_t)node);   // the first one counts
               else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
               v[i] = 0.f;
@@ -1036,8 +1053,9 @@ int32_t launch(Pool* p, const TreeParams<N>& prm, int workers, bool parts) {
 }
 // The ranges.  Equal ones cut nearly every stream where there are about as many streams as SMs: two parts an SM, each with its queries, its float32 sums out and
 // in again, and a launch that joins them.  So where there are few streams a range (kPackStreams), whole ones are dealt out as well, in their order and none cut that
-// is no longer than the longest range, and taken where that longest range is no more than what the parts would cost.  (16 x 3000 tokens of 240 rows, 128
-// streams: 86 us with equal ranges, PACKED_A with whole streams; 4 x 500 tokens behind 1500, 256 streams, 143 and PACKED_B.)
+// is no longer than the longest range, and taken where that longest range is no more than what the parts would cost.  (Calls of 240 rows: 128 streams of 3000
+// tokens 86 us with equal ranges, 74 with whole streams, on 8 bits 112 and 100; 144 of 1000 57 and 45; 296 of 2000 118 and 115; a prompt's 256 of 1564 to 2000
+// 143 and 138.)
 struct Ranges {
   int32_t cuts[kMaxWorkers + 1];
   int workers;

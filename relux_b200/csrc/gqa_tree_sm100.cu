@@ -4,8 +4,8 @@
 // o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  where query token i sees every cached row and, of the drafted ones, itself
 // and its ancestors; of a prompt, every row up to its own.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128
 // operations for the 512 (264) bytes of a token and kv head, so the cache's bytes bound trees of up to some 200 rows (100 on the 8-bit cache) and the tensor
-// cores and the softmax larger ones.  Measured: 64 x 8192 tokens, 64 rows 332 us on bf16 (6.5 TB/s), 410 on 8 bits (2.7 TB/s); 8 x 32768 tokens, 512 rows
-// 546 us (1.0 PFLOP/s), 660 on 8 bits.
+// cores and the softmax larger ones.  Measured: 64 x 8192 tokens, 64 rows 332 us on bf16 (6.5 TB/s), 378 on 8 bits (2.9 TB/s); 8 x 32768 tokens, 512 rows
+// 546 us (1.0 PFLOP/s), 648 on 8 bits.
 //
 // A STREAM is the tiles of 128 keys that up to 256 of a kv head's rows (one or two blocks of 128, M of both contractions) see.  All streams of the
 // call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into a range per SM (make_ranges); a PIECE is the part of a stream inside a
@@ -24,8 +24,8 @@
 //              which meet at the piece's end.
 // What bounds it.  bf16, up to 64 rows: HBM.  More rows: the softmax warps, for whom a step of 128 rows takes 1550 clocks (2570 beside converters), most of it
 // the latency of their instructions (512 of exponentials a warp), against 1020 of MMAs.  8 bits, up to 64 rows: converters and softmax share issue slots and
-// shared memory, through which a tile's operands, codes and queries come to 1760 clocks, and each alone adds a fourth to what the rest takes: 410 us of 64 x 8192
-// tokens were 300 without the converters' work, 332 without the softmax's, 234 without either.
+// shared memory, through which a tile's operands, codes and queries come to 1760 clocks, and each alone adds a fourth to what the rest takes: 408 us of 64 x 8192
+// tokens, a build before the last, were 300 without the converters' work, 332 without the softmax's, 234 without either.
 // Order of issue: QK(k + 1), PV(k): the tensor pipe executes in issue order, so QK(k + 2) finds its S buffer read.
 // A product with P = 0 does not hide an infinity or a NaN among the values: those of drafted rows and of what lies behind are set to zero in the tile, and
 // the rows that see one become NaN at the end.  (8-bit rows have them in their scale alone; a code is always a number.)
@@ -201,10 +201,11 @@ struct Plan {
   static constexpr int kTotal = kBars + (int)(kI8 ? sizeof(Bars) : kNB == 1 ? offsetof(Bars, v_scale) : offsetof(Bars, see) + sizeof(Bars::see));
   static_assert(kTotal <= 232448, "more shared memory than a CTA may use");
   static constexpr int kWarpLoad = kSoftmaxWarps + (kI8 ? 2 * kConvWarps : 0), kWarpMma = kWarpLoad + 1;
-  // Four more warps where registers are dealt out anew, of the 96 of the launch, which warps do by fours.  (With 152, 64 and 48 the warp that issues the MMAs
-  // kept a pointer in local memory, and 8 x 32768 tokens, 64 nodes, 64 heads took 934 us where it is 770 with these.)
+  // Four more warps where registers are dealt out anew, of the 96 of the launch, which warps do by fours.  Two blocks: with 152, 64 and 48 the warp that issues the
+  // MMAs kept a pointer in local memory, and 8 x 32768 tokens, 64 nodes, 64 heads took 934 us where it was 770 with these.  One block: 64 x 8192 tokens of 64 rows 392
+  // us with 144, 64 and 64, 397 with 144, 72 and 48, 384 with 128, 80 and 64, 378 with these.
   static constexpr int kThreads = 32 * (kI8 ? kWarpLoad + 4 : kWarpMma + 1);
-  static constexpr int kRegsSoftmax = 144, kRegsConv = 64, kRegsOther = 64;
+  static constexpr int kRegsSoftmax = kNB == 1 ? 136 : 144, kRegsConv = kNB == 1 ? 72 : 64, kRegsOther = 64;
   static_assert(!kI8 || 256 * kRegsSoftmax + 256 * kRegsConv + 128 * kRegsOther <= 640 * 96, "more registers than the block is launched with");
 };
 // The wait that gives up raises the flag, which ends all others; the kernel's end reports it.  Short, and not a function of its own: a call takes registers that
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
   }
   const Streams<N> streams(prm, blockIdx.x);
   // (One block) the first piece, of every role, is searched for by one thread, before the wait for the launch ahead: the search in every role was a good
-  // part of the roles' code, which share one instruction cache (64 x 8192 tokens, 64 rows, 8 bits: 424 us, 389 so; 100 x 700 97 and 94).  With two blocks the steps
+  // part of the roles' code, which share one instruction cache (64 x 8192 tokens, 64 rows, 8 bits: 424 us, 390 so; 100 x 700 97 and 94).  With two blocks the steps
   // come out of the compiler slower for it, whatever its reason: 8 x 32768 tokens of 512 rows 648 us and 807.
   if (kNB == 1 && threadIdx.x == 32) {
     if (c.seqs) chain_wait();   // the list is a copy that was queued just before this launch

@@ -967,6 +967,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         }
     }
   }
+  if (c.out_bf16) fence_chained_writes();   // activations, which a later launch may read by TMA
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -1037,6 +1038,7 @@ __global__ void __launch_bounds__(256, 4) merge_tree_kernel(const __grid_constan
     if (c.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c.out) + at) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
     else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   }
+  if (c.out_bf16) fence_chained_writes();
 }
 
 template <bool kI8, int kNB, int N>

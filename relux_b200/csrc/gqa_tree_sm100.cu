@@ -168,20 +168,27 @@ struct Bars {
   uint32_t tmem_base;
   volatile int32_t abort_flag;
   int32_t first[4];            // piece of this range: its e, kvh, us, tb
-  uint64_t bad_nodes[4];       // of a piece, in turn: nodes with an infinity or a NaN among their values
-  uint32_t bad_all;            // (8-bit cache) a cached row with one, a bit a piece
+  uint64_t bad_nodes[4];       // (bf16) of a piece, in turn: nodes with an infinity or a NaN among their values
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
   union {
     uint64_t see[256];         // what a row sees: of the nodes (a bit each), or how many tokens from len0 on
     struct {
-      uint64_t of_one[128];    // (one block)
-      float halves[2][3][64];  // (two) a row's max, sum and unit of O, of either half of the warps
+      uint64_t of_two[64];     // (two: up to 64 rows)
+      float halves[2][3][64];  // a row's max, sum and unit of O, of either half of the warps
     };
   };
   alignas(16) uint32_t v_scale[4][kTile];   // (8-bit cache) of a tile's values, over their unit, binary16 twice
   alignas(16) float k_scale[4][kTile];   // (8-bit cache) of a tile's keys
+  // (8-bit cache) Of piece n, in place n & 7: nodes with an infinity or a NaN among their values, and whether a cached row has one.  The warp of the scales
+  // writes a piece's once, before it hands over the piece's last tile, and nobody clears them.  It may be four tiles ahead of the softmax warps, of pieces of
+  // one tile four pieces, one of which has not been read out.  Place n & 7 is written again for piece n + 8: the last tile of that is handed over only when
+  // the softmax warps have left a tile of piece n + 4 or a later one, behind their reading of piece n's flags.
+  struct {
+    uint64_t nodes;
+    uint32_t all;
+  } bad[8];
   uint64_t raw_full[9], raw_empty[9], scale_full[4], scale_empty[4], info[4], info_empty[4];
-  // Without an 8-bit cache there is no room for these from v_scale on, nor with two blocks for `halves`.
+  // Without an 8-bit cache there is no room for these from v_scale on.
 };
 
 template <bool kI8, int kNB>
@@ -290,7 +297,6 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       }
     }
     for (int s = 0; s < 4; s++) bars->bad_nodes[s] = 0;
-    bars->bad_all = 0;
     for (int s = 0; s < 2; s++) {
       mbar_init(&bars->s_full[s], 1);
       mbar_init(&bars->p_full[s], two ? kSoftmaxWarps / 2 : kSoftmaxWarps);
@@ -758,8 +764,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       wait_bar(&bars->fin, n & 1, bars);
       tc_fence_after();
       const bool ok = bars->abort_flag == 0;
-      const uint64_t bad_nodes = bars->bad_nodes[n & 3];
-      const bool bad_all = bars->bad_all >> (n & 3) & 1u, whole = p.tb == 0 && p.te == p.tiles;
+      const uint64_t bad_nodes = kI8 ? bars->bad[n & 7].nodes : bars->bad_nodes[n & 3];
+      const bool bad_all = kI8 && bars->bad[n & 7].all, whole = p.tb == 0 && p.te == p.tiles;
       const int slot = 2 * (int)blockIdx.x + (p.us + p.tb == streams.u_begin ? 0 : 1);
 #pragma unroll 1
       for (int b = 0; b < nb; b++, next_block()) {
@@ -833,10 +839,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           }
         }
       }
-      if (warp == 0 && lane == 0) {   // of piece n + 4; who writes it next has come through q_full of piece n + 1
-        bars->bad_nodes[n & 3] = 0;
-        atomicAnd(&bars->bad_all, ~(1u << (n & 3)));
-      }
+      if (!kI8 && warp == 0 && lane == 0) bars->bad_nodes[n & 3] = 0;   // of piece n + 4; who writes it next has come through q_full of piece n + 1
       tc_fence_before();
       __syncwarp();
       if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // before the next piece's queries come to the place of the other warp's results
@@ -851,6 +854,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       for (Piece p = first_piece(); streams.valid(p); p = streams.next(p), n++) {
         const TreeSeq sq = streams.seq(p.e);
         ValueUnit unit;
+        uint64_t bad_nodes = 0;   // this lane's of the piece
+        bool bad_all = false;
         for (int t = p.tb; t < p.te; t++, tt++) {
           const int at = tt & 3, r = 4 * lane;   // four rows a lane
           if (tt >= 4) wait_bar(&bars->info_empty[at], ((tt >> 2) - 1) & 1, bars);
@@ -866,9 +871,9 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             if (i >= there) v[i] = 0.f;   // behind the drafted rows, where anything may lie
             if (!(v[i] == v[i])) {        // the row held an infinity or a NaN
               const int node = pos + i - sq.len0;
-              if (node < 0) atomicOr(&bars->bad_all, 1u << (n & 3));
-              else if (!c.tree) atomicMax(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), (unsigned long long)~(uint32_t)node);   // the first one counts
-              else if (node < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << node);
+              if (node < 0) bad_all = true;
+              else if (!c.tree) bad_nodes = max(bad_nodes, (uint64_t)~(uint32_t)node);   // the first one counts
+              else if (node < kTreeNodes) bad_nodes |= 1ull << node;
               v[i] = 0.f;
             }
             top = fmaxf(top, v[i]);
@@ -879,6 +884,15 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           for (int i = 0; i < 4; i++) s[i] = round_f16x2(v[i] * unit.down, v[i] * unit.down);
           *reinterpret_cast<uint4*>(&bars->v_scale[at][r]) = make_uint4(s[0], s[1], s[2], s[3]);
           if (lane == 0) bars->v_unit[at] = __uint_as_float((254u << 23) - __float_as_uint(unit.down));   // 1 / down, a power of two
+          if (t + 1 == p.te) {
+            const uint32_t lo = (uint32_t)bad_nodes, hi = (uint32_t)(bad_nodes >> 32);
+            const uint32_t all_lo = c.tree ? __reduce_or_sync(0xffffffffu, lo) : __reduce_max_sync(0xffffffffu, lo), all_hi = __reduce_or_sync(0xffffffffu, hi);
+            const bool any = __any_sync(0xffffffffu, bad_all);
+            if (lane == 0) {
+              bars->bad[n & 7].nodes = (uint64_t)all_hi << 32 | all_lo;
+              bars->bad[n & 7].all = any;
+            }
+          }
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(&bars->info[at]);

@@ -1,0 +1,71 @@
+"""Infinities and NaN in calls of more than 32 query rows a kv head (drafted trees, verifies over the 8-bit cache): they reach the outputs of who sees them, and no
+others, however the streams of a call fall into ranges."""
+import numpy as np
+import pytest
+
+from tests import gqa_plain as G
+from tests.test_gpu_cache_int8 import filled
+
+pytestmark = pytest.mark.gpu
+D, PAGE = 128, 64
+
+
+@pytest.fixture(scope="module")
+def dev():
+    import relux_b200 as rb
+    d = rb.Device(0)
+    yield d
+    d.close()
+
+
+def short_streams(dev, int8, H, S, tree):
+    """Streams of one tile, several to a range: the flags of a piece are of that piece alone.  Every ninth sequence has a NaN or an infinity among the values of one
+    of its new rows, every eleventh one among those of a cached row, of one kv head each."""
+    rng = np.random.default_rng(S + H)
+    B, Hkv, g = 160, 8, H // 8
+    lens = [int(x) for x in rng.integers(1, 128 - S, B)]
+    pool, cache = filled(dev, rng, [0] * B, H, Hkv, 128, int8=int8)
+    k0, v0 = [G.rows(rng, n, Hkv) for n in lens], [G.rows(rng, n, Hkv, "v") for n in lens]
+    k, v = G.rows(rng, B * S, Hkv).reshape(B, S, Hkv, D), G.rows(rng, B * S, Hkv, "v").reshape(B, S, Hkv, D)
+    cached, new = {}, {}
+    for b in range(B):
+        if b % 11 == 5:
+            cached[b] = int(rng.integers(Hkv))
+            v0[b][int(rng.integers(lens[b])), cached[b], int(rng.integers(D))] = np.inf
+        if b % 9 == 4:
+            new[b] = int(rng.integers(S)), int(rng.integers(Hkv))
+            v[b, new[b][0], new[b][1], int(rng.integers(D))] = np.nan if b % 2 else -np.inf
+    pool.append(0, np.concatenate(k0), np.concatenate(v0), B, n_new=lens)
+    parents = np.stack([G.random_tree(rng, S) for _ in range(B)])
+    q, out = G.bf16(rng.standard_normal((B, S, H, D))), np.empty((B, S, H, D), np.float32)
+    outs = []
+    for _ in range(3):
+        out[...] = 7
+        args = (0, B, q, out, k.reshape(-1, Hkv, D), v.reshape(-1, Hkv, D), H, D, D ** -0.5)
+        if tree:
+            pool.tree_verify(*args, parents)
+        else:
+            pool.verify(*args, S)
+        outs.append(out.copy())
+    for b in range(B):
+        see = G.ancestors(parents[b], S, S) if tree else G.causal(S)
+        bad = np.zeros((S, H), bool)
+        if b in cached:
+            bad[:, cached[b] * g:(cached[b] + 1) * g] = True
+        if b in new:
+            bad[see[:, new[b][0]], new[b][1] * g:(new[b][1] + 1) * g] = True
+        with np.errstate(invalid="ignore"):
+            K, V = (np.concatenate([G.held(x, int8), G.held(y, int8)]) for x, y in ((k0[b], k[b]), (v0[b], v[b])))
+        want, bound = G.attend(K, np.nan_to_num(V, posinf=0, neginf=0), q[b], lens[b], see, D ** -0.5)
+        for o in outs:
+            # an infinity that is seen may stay one in its dim; over the 8-bit cache, and of a drafted row, the whole head is NaN
+            assert not np.isfinite(o[b]).all(-1)[bad].any(), "sequence %d" % b
+            G.check(o[b][~bad], want[~bad], bound[~bad], "sequence %d" % b)
+    assert pool.status() == 0
+    pool.destroy()
+
+
+@pytest.mark.parametrize("H,S", [(32, 12), (32, 25), (64, 40)])
+@pytest.mark.parametrize("tree", [True, False])
+def test_short_streams_of_the_8_bit_cache(dev, H, S, tree):
+    short_streams(dev, True, H, S, tree)

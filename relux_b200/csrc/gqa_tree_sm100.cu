@@ -168,7 +168,9 @@ struct Bars {
   uint32_t tmem_base;
   volatile int32_t abort_flag;
   int32_t first[4];            // piece of this range: its e, kvh, us, tb
-  uint64_t bad_nodes[4];       // (bf16) of a piece, in turn: nodes with an infinity or a NaN among their values
+  // (bf16) Of a piece: nodes with an infinity or a NaN among their values.  The MMA warp writes it once a piece, before `fin`; of the next piece it does so
+  // behind that one's q_full, at which every softmax warp arrives when it has read this.
+  uint64_t bad_nodes;
   float v_unit[4];             // (8-bit cache) of a tile: what O is to be multiplied by
   union {
     uint64_t see[256];         // what a row sees: of the nodes (a bit each), or how many tokens from len0 on
@@ -296,7 +298,6 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
         mbar_init(&bars->info_empty[s], (two ? kSoftmaxWarps / 2 : kSoftmaxWarps) + kConvWarps);
       }
     }
-    for (int s = 0; s < 4; s++) bars->bad_nodes[s] = 0;
     for (int s = 0; s < 2; s++) {
       mbar_init(&bars->s_full[s], 1);
       mbar_init(&bars->p_full[s], two ? kSoftmaxWarps / 2 : kSoftmaxWarps);
@@ -434,7 +435,8 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
     for (Piece p = first_piece(); streams.valid(p); p = streams.next(p), n++) {
       const TreeSeq sq = streams.seq(p.e);
       const int nb = blocks_of(sq), tiles = p.te - p.tb;
-      wait_bar(&bars->q_full, n & 1, bars);   // the queries are there, and O of the piece before has been read
+      uint64_t bad_nodes = 0;                 // (bf16) this lane's of the piece
+      wait_bar(&bars->q_full, n & 1, bars);   // the queries are there, and O and the flags of the piece before have been read
       auto issue_qk = [&](int t, int b, int step) {
         const int h = kI8 ? tt + t : 2 * (tt + t), st = h % PL::kSlots;
         if (b == 0) wait_bar(&bars->full[st], (h / PL::kSlots) & 1, bars);
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
                     const int r = r0 + 2 * (__ffs(bad) - 1);
                     const uint4 w = *at(r);
                     *at(r) = make_uint4(bf16x2_finite(w.x), bf16x2_finite(w.y), bf16x2_finite(w.z), bf16x2_finite(w.w));
-                    if (r - from < kTreeNodes) atomicOr(reinterpret_cast<unsigned long long*>(&bars->bad_nodes[n & 3]), 1ull << (r - from));
+                    if (r - from < kTreeNodes) bad_nodes |= 1ull << (r - from);
                   }
                 }
                 if (any) fence_proxy_async();
@@ -524,6 +526,10 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       }
       k += steps;
       tt += tiles;
+      if constexpr (!kI8) {
+        const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)bad_nodes), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad_nodes >> 32));
+        if (lane == 0) bars->bad_nodes = (uint64_t)hi << 32 | lo;
+      }
       if (el) umma_commit<1>(&bars->fin);         // the piece's products are complete
       if (lane == 0) mbar_arrive(&bars->fin);     // and what this warp, or the converters before they handed over the values, wrote beside them
       __syncwarp();
@@ -764,7 +770,7 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
       wait_bar(&bars->fin, n & 1, bars);
       tc_fence_after();
       const bool ok = bars->abort_flag == 0;
-      const uint64_t bad_nodes = kI8 ? bars->bad[n & 7].nodes : bars->bad_nodes[n & 3];
+      const uint64_t bad_nodes = kI8 ? bars->bad[n & 7].nodes : bars->bad_nodes;
       const bool bad_all = kI8 && bars->bad[n & 7].all, whole = p.tb == 0 && p.te == p.tiles;
       const int slot = 2 * (int)blockIdx.x + (p.us + p.tb == streams.u_begin ? 0 : 1);
 #pragma unroll 1
@@ -839,7 +845,6 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           }
         }
       }
-      if (!kI8 && warp == 0 && lane == 0) bars->bad_nodes[n & 3] = 0;   // of piece n + 4; who writes it next has come through q_full of piece n + 1
       tc_fence_before();
       __syncwarp();
       if (two) asm volatile("bar.sync %0, 64;" ::"r"(1 + row_warp) : "memory");   // before the next piece's queries come to the place of the other warp's results

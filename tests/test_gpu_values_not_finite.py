@@ -69,3 +69,8 @@ def short_streams(dev, int8, H, S, tree):
 @pytest.mark.parametrize("tree", [True, False])
 def test_short_streams_of_the_8_bit_cache(dev, H, S, tree):
     short_streams(dev, True, H, S, tree)
+
+
+@pytest.mark.parametrize("H,S", [(32, 12), (32, 25), (64, 40)])
+def test_short_streams_of_the_bf16_cache(dev, H, S):
+    short_streams(dev, False, H, S, True)

@@ -1042,7 +1042,8 @@ __global__ void __launch_bounds__(256, 4) merge_tree_kernel(const __grid_constan
       M = top;
 #pragma unroll
       for (int q = 0; q < 4; q++)
-        if (ml[q].x != -INFINITY) {
+        // A part whose scores of this row are all NaN has a maximum of nothing and a sum of NaN: exp2(-inf - M) of that is NaN or nothing, and so is L then NaN.
+        if (ml[q].x != -INFINITY || ml[q].y != ml[q].y) {
           const float w = ex2_approx(ml[q].x - M);
           L = fmaf(ml[q].y, w, L);
           o.x = fmaf(x[q].x, w, o.x);

@@ -74,3 +74,51 @@ def test_short_streams_of_the_8_bit_cache(dev, H, S, tree):
 @pytest.mark.parametrize("H,S", [(32, 12), (32, 25), (64, 40)])
 def test_short_streams_of_the_bf16_cache(dev, H, S):
     short_streams(dev, False, H, S, True)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("S", [4, 12, 25, 64])
+@pytest.mark.parametrize("lens", [[2048], [100] * 40, [1500] * 40])
+def test_a_nan_among_queries_reaches_their_output(dev, int8, S, lens):
+    """Streams that one range has, and streams that are cut: the row of the NaN is NaN, and no other."""
+    rng = np.random.default_rng(S + len(lens))
+    B, H, Hkv = len(lens), 32, 8
+    pool, cache = filled(dev, rng, lens, H, Hkv, S, int8=int8)
+    parents = G.random_tree(rng, S)
+    k, v, q = G.rows(rng, B * S, Hkv), G.rows(rng, B * S, Hkv, "v"), G.bf16(rng.standard_normal((B, S, H, D)))
+    bad = np.zeros((B, S, H), bool)
+    for b in range(B):
+        s, h = int(rng.integers(S)), int(rng.integers(H))
+        bad[b, s, h] = True
+        q[b, s, h, int(rng.integers(D))] = np.nan
+    see, out = G.ancestors(parents, S, S), np.full((B, S, H, D), 7, np.float32)
+    for tree in (True, False) if int8 or S <= 8 else (True,):
+        if tree:
+            pool.tree_verify(0, B, q, out, k, v, H, D, D ** -0.5, parents)
+        else:
+            pool.verify(0, B, q, out, k, v, H, D, D ** -0.5, S)
+        assert np.isnan(out[bad]).all() and np.isfinite(out[~bad]).all()
+        for b in range(0, B, 13):
+            K, V = (np.concatenate([c[b], G.held(x[b * S:(b + 1) * S], int8)]) for c, x in ((cache.k, k), (cache.v, v)))
+            want, bound = G.attend(K, V, np.nan_to_num(q[b]), lens[b], see if tree else G.causal(S), D ** -0.5)
+            G.check(out[b][~bad[b]], want[~bad[b]], bound[~bad[b]], "sequence %d" % b)
+    pool.destroy()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("S", [3, 12, 25, 64])
+def test_a_nan_key_that_is_all_of_a_part(dev, int8, S):
+    """The tile of the new rows by itself is a part of its stream in some of these calls, and a query sees one row there, whose key is NaN."""
+    rng = np.random.default_rng(S)
+    H, Hkv = 32, 8
+    for n in range(8, 25):
+        pool, _ = filled(dev, rng, [128 * n], H, Hkv, S, int8=int8)
+        k, v, q = G.rows(rng, S, Hkv), G.rows(rng, S, Hkv, "v"), G.bf16(rng.standard_normal((1, S, H, D)))
+        k[0, :, 5] = np.nan
+        out = np.full((1, S, H, D), 7, np.float32)
+        pool.tree_verify(0, 1, q, out, k, v, H, D, D ** -0.5, np.full(S, -1))      # only roots
+        assert np.isnan(out[0, 0]).all() and np.isfinite(out[0, 1:]).all(), n
+        if int8 or S <= 8:
+            pool.verify(0, 1, q, out, k, v, H, D, D ** -0.5, S)                     # the first draft, which all see
+            assert np.isnan(out).all(), n
+        pool.destroy()

@@ -111,7 +111,7 @@ def test_a_nan_key_that_is_all_of_a_part(dev, int8, S):
     """The tile of the new rows by itself is a part of its stream in some of these calls, and a query sees one row there, whose key is NaN."""
     rng = np.random.default_rng(S)
     H, Hkv = 32, 8
-    for n in range(8, 25):
+    for n in range(8, 23):
         pool, _ = filled(dev, rng, [128 * n], H, Hkv, S, int8=int8)
         k, v, q = G.rows(rng, S, Hkv), G.rows(rng, S, Hkv, "v"), G.bf16(rng.standard_normal((1, S, H, D)))
         k[0, :, 5] = np.nan

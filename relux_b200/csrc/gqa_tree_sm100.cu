@@ -802,9 +802,9 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
           if (bad_all || (c.tree ? (see & bad_nodes) != 0 : bad_nodes != 0 && (int)see > (int)~(uint32_t)bad_nodes)) l = __uint_as_float(0x7FC00000u);
           const bool there = ok && row < rows && (!c.tree || token_of(c, sq.row0 + row) < sq.end - sq.len0);
           // no part of a sum that nobody has added to, of a row that is not there: zero whatever the accumulator holds
-          const float inv = !there ? 0.f : !whole ? 1.f : l == 0.f ? 0.f : __fdividef(1.f, l);
-          f[hf] = st.m[hf] == -INFINITY && l == l ? 0.f : w * inv;
-          f2[hf] *= inv;
+          const float inv = !whole ? 1.f : l == 0.f ? 0.f : __fdividef(1.f, l);
+          f[hf] = !there || (st.m[hf] == -INFINITY && l == l) ? 0.f : w * inv;   // (the weights of a row that is not there may be NaN: its query is anything)
+          f2[hf] = there ? f2[hf] * inv : 0.f;
           if (!whole && (lane & 3) == 0 && set == 0 && row < rows)
             *reinterpret_cast<float2*>(c.part_ml + ((size_t)slot * c.rows_rb + row) * 2) = there ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         }

@@ -122,3 +122,33 @@ def test_a_nan_key_that_is_all_of_a_part(dev, int8, S):
             pool.verify(0, 1, q, out, k, v, H, D, D ** -0.5, S)                     # the first draft, which all see
             assert np.isnan(out).all(), n
         pool.destroy()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("S", [6, 12, 16, 25, 64])
+@pytest.mark.parametrize("lens", [[700], [90, 128, 0], [300] * 40])
+def test_whatever_stands_in_rows_past_the_nodes(dev, int8, S, lens):
+    """Queries of a padded batch may be anything: their outputs are zeros, and nobody else's change."""
+    rng = np.random.default_rng(S + len(lens))
+    B, H, Hkv = len(lens), 32, 8
+    pool, cache = filled(dev, rng, lens, H, Hkv, S, int8=int8)
+    nodes = [int(x) for x in rng.integers(0, S, B)]
+    n, parents = sum(nodes), G.random_tree(rng, S)
+    k, v, q = G.rows(rng, n, Hkv), G.rows(rng, n, Hkv, "v"), G.bf16(rng.standard_normal((B, S, H, D)))
+    want, at = [], 0
+    for b, m in enumerate(nodes):
+        K, V = (np.concatenate([c[b], G.held(y[at:at + m], int8)]) for c, y in ((cache.k, k), (cache.v, v)))
+        want.append(G.attend(K, V, q[b, :m], lens[b], G.ancestors(parents, m, S)[:m, :m], D ** -0.5) if b < 4 else None)
+        at += m
+    for fill in (0.0, np.inf, -np.inf, np.nan, 3e38):
+        x = q.copy()
+        for b in range(B):
+            x[b, nodes[b]:] = G.bf16(np.float32(fill)) * (np.sign(q[b, nodes[b]:]) if fill == 3e38 else 1)
+        out = np.full((B, S, H, D), 7, np.float32)
+        pool.tree_verify(0, B, x, out, k, v, H, D, D ** -0.5, parents, n_nodes=nodes)
+        for b, m in enumerate(nodes):
+            assert (out[b, m:] == 0).all(), fill
+            if want[b] and m:
+                G.check(out[b, :m], *want[b], "sequence %d, %g" % (b, fill))
+    assert pool.status() == 0
+    pool.destroy()

@@ -129,6 +129,9 @@ __device__ __forceinline__ void query_factor(uint32_t top, float& up, float& dow
   up = __uint_as_float((uint32_t)(127 + k) << 23);
   down = __uint_as_float((uint32_t)(127 - k) << 23);
 }
+// What a score is multiplied by: the softmax scale (times log2 e) over the row's power of two.  Not nothing, even of a row of zeros, whose power is the largest, under a
+// scale below 2^-23: minus infinity, a hidden key's score, times nothing is NaN.
+__device__ __forceinline__ float score_factor(float scale_log2, float down) { return fmaxf(scale_log2 * down, __uint_as_float(1u)); }
 // Row of queries in shared memory: 128 binary16 values, the row's factor (what a score of theirs is multiplied by, softmax scale and log2 e included),
 // and what the row sees of the new rows.  By 16 lanes of a converged warp, eight dims each.
 __device__ __forceinline__ void int8_put_query(uint16_t* row, int ch, bool there, const void* q, size_t off, bool q_bf16, float scale_log2) {
@@ -149,7 +152,7 @@ __device__ __forceinline__ void int8_put_query(uint16_t* row, int ch, bool there
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
   *reinterpret_cast<uint4*>(row + ch) = make_uint4(w[0], w[1], w[2], w[3]);
-  if (ch == 0) *reinterpret_cast<float*>(row + kGqaD) = scale_log2 * down;
+  if (ch == 0) *reinterpret_cast<float*>(row + kGqaD) = score_factor(scale_log2, down);
 }
 // 16 such rows -> A fragments in the order of K's bytes, and the factors of this lane's two rows.
 __device__ __forceinline__ void int8_load_q(uint32_t (&qa)[8][4], float (&q_scale)[2], const uint16_t* qs, int lane) {

@@ -593,12 +593,12 @@ __global__ void __launch_bounds__(Plan<kI8, kNB>::kThreads, 1)
             query_factor(row_top(x), up, down);
             *at = make_uint4(pack_p<true>(x[0] * up, x[1] * up), pack_p<true>(x[2] * up, x[3] * up), pack_p<true>(x[4] * up, x[5] * up), pack_p<true>(x[6] * up, x[7] * up));
             if (two) {
-              if (ch == 0) bars->halves[0][0][16 * row_warp + j] = c.scale_log2 * down;
+              if (ch == 0) bars->halves[0][0][16 * row_warp + j] = score_factor(c.scale_log2, down);
             } else {
               const float f = __shfl_sync(0xffffffffu, down, ((lane >> 2) & 1) * 16);
 #pragma unroll
               for (int hf = 0; hf < 2; hf++)
-                if (((lane >> 2) + 8 * hf) >> 1 == i) st.f[hf] = c.scale_log2 * f;
+                if (((lane >> 2) + 8 * hf) >> 1 == i) st.f[hf] = score_factor(c.scale_log2, f);
             }
           }
         if (two) {   // to the other warp of these rows

@@ -152,3 +152,27 @@ def test_whatever_stands_in_rows_past_the_nodes(dev, int8, S, lens):
                 G.check(out[b, :m], *want[b], "sequence %d, %g" % (b, fill))
     assert pool.status() == 0
     pool.destroy()
+
+
+@pytest.mark.parametrize("S", [1, 4, 12, 25, 64])
+@pytest.mark.parametrize("scale", [1e-8, 1e-30])
+def test_queries_of_zeros_under_a_small_scale(dev, S, scale):
+    """Over the 8-bit cache a query comes with a factor that holds the softmax scale: it must not vanish, or a hidden score, minus infinity, becomes NaN."""
+    rng = np.random.default_rng(S)
+    H, Hkv, lens = 32, 8, [100, 7]
+    pool, cache = filled(dev, rng, lens, H, Hkv, S)
+    k, v = G.rows(rng, 2 * S, Hkv), G.rows(rng, 2 * S, Hkv, "v")
+    q = G.bf16(rng.standard_normal((2, S, H, D)))
+    q[:, :, ::2] = 0
+    q[:, :, 1] = 1e-38
+    out = np.empty((2, S, H, D), np.float32)
+    for tree in (False, True):
+        if tree:
+            pool.tree_verify(0, 2, q, out, k, v, H, D, scale, np.arange(-1, S - 1))
+        else:
+            pool.verify(0, 2, q, out, k, v, H, D, scale, S)
+        for b in range(2):
+            K, V = (np.concatenate([c[b], G.held(x[b * S:(b + 1) * S], True)]) for c, x in ((cache.k, k), (cache.v, v)))
+            want, bound = G.attend(K, V, q[b], lens[b], G.causal(S), scale, q_rounding=2.0 ** -8)
+            G.check(out[b], want, bound, "sequence %d" % b)
+    pool.destroy()

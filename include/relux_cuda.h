@@ -588,7 +588,8 @@ int32_t relux_stream_partition(const relux_stream_partition_args* args);
  * token selection, of the selection kernel).  The tensor-core kernels stamp %globaltimer themselves: from the first block
  * that has its inputs (the kernel before it in the stream complete) to the end of the last block; launch overhead is not in
  * it, nor is the way to L2 of results that the latent decode kernel (up to 0.7 us) and the projections have just stored, and
- * for a GQA step the append and the merge are.  The reference-mode and generic kernels, and GQA prompts as grid
+ * for a GQA step the append and the merge are.  Of trees, and of calls over the 8-bit cache, with more than 32 query rows per kv head
+ * the join of split streams' parts is in it, the append of the new rows, a launch of its own, is not.  The reference-mode and generic kernels, and GQA prompts as grid
  * slices, are timed by CUDA events around their launches.  Synchronises the stream.  Measurement aid: no counterpart in
  * the reference. */
 int32_t relux_pool_last_kernel_ms(relux_pool_t pool, float* ms);

@@ -1059,6 +1059,8 @@ __global__ void __launch_bounds__(256, 4) merge_tree_kernel(const __grid_constan
     else *reinterpret_cast<float4*>(reinterpret_cast<float*>(c.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   }
   if (c.out_bf16) fence_chained_writes();
+  __syncthreads();
+  if (threadIdx.x == 0) stamp_end(c.time);   // of every block that joined rows: the attention's time ends with the last of them
 }
 
 template <bool kI8, int kNB, int N>

@@ -154,6 +154,7 @@ struct Pool {
   int32_t* h_stage = nullptr;    // pinned [kStageSlots][4 * (max_seqs + 1)]
   cudaEvent_t stage_ev[kStageSlots] = {};
   bool stage_busy[kStageSlots] = {};
+  std::vector<void*> stage_held;   // of captured calls, a block each: every launch of their graph copies from it
   uint32_t stage_next = 0;
   // per sequence four ints, and of a GQA pool a tree's parents, 64 bytes
   size_t stage_slot_ints() const { return (prm.kind == RELUX_POOL_GQA ? 20 : 4) * ((size_t)prm.max_seqs + 1); }
@@ -206,7 +207,7 @@ int32_t pipe_end(Pool* p);
 inline void pipe_release(Pool* p, PipeSlots& ps, int slot) {
   if (slot >= 0) ps.reader[slot] = p->pipe_calls.last;
 }
-// Next staging slot (waits for the copy that last used it); call stage_release after the copies are enqueued.
+// Next staging slot (waits for the copy that last used it; of a captured call a block of its own); call stage_release after the copies are enqueued.
 int32_t stage_acquire(Pool* p, int32_t** slot, int* slot_index);
 int32_t stage_release(Pool* p, int slot_index);
 

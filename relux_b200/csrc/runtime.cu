@@ -101,6 +101,18 @@ int32_t time_events_end(Pool* p, TimeRing& r) {
 }
 
 int32_t stage_acquire(Pool* p, int32_t** slot, int* slot_index) {
+  if (stream_captured(p->dev)) {   // a slot would be filled anew by later calls, and an event recorded here cannot be waited for
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    void* block = nullptr;
+    RELUX_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = cudaMallocHost(&block, p->stage_slot_ints() * sizeof(int32_t));
+    RELUX_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    if (e != cudaSuccess) return cuda_fail(e, "staging block of a captured call");
+    p->stage_held.push_back(block);
+    *slot = (int32_t*)block;
+    *slot_index = -1;
+    return RELUX_OK;
+  }
   const int i = (int)(p->stage_next++ % Pool::kStageSlots);
   if (p->stage_busy[i]) {
     RELUX_CUDA_TRY(cudaEventSynchronize(p->stage_ev[i]));
@@ -111,6 +123,7 @@ int32_t stage_acquire(Pool* p, int32_t** slot, int* slot_index) {
   return RELUX_OK;
 }
 int32_t stage_release(Pool* p, int slot_index) {
+  if (slot_index < 0) return RELUX_OK;
   RELUX_CUDA_TRY(cudaEventRecord(p->stage_ev[slot_index], p->dev->stream));
   p->stage_busy[slot_index] = true;
   return RELUX_OK;
@@ -286,6 +299,7 @@ static void pool_free_all(Pool* p) {
   fr(p->in_a.p); fr(p->in_b.p); fr(p->out_buf.p); fr(p->q_abs.p); fr(p->part_o.p); fr(p->part_ml.p); fr(p->work.p); fr(p->stream_done.p); fr(p->seq_list.p);
   fr(p->o_lat.p); fr(p->q_conv.p); fr(p->rope_tab.p); fr(p->layer_buf.p); fr(p->shadow_f32); fr(p->chunk_tab.p); fr(p->step_rows.p); fr(p->expand_buf.p);
   if (p->h_stage) cudaFreeHost(p->h_stage);
+  for (void* block : p->stage_held) cudaFreeHost(block);
   if (p->sel_host) cudaFreeHost(p->sel_host);
   for (cudaEvent_t ev : p->stage_ev)
     if (ev) cudaEventDestroy(ev);

@@ -57,10 +57,9 @@ int32_t launch_gqa_stream(Pool* p, const SeqBatch& sb, const relux_attn_args& a,
   int32_t rc = grow(p->dev, p->part_o, part_rows * (kGqaD + 2) * sizeof(float));
   if (rc) return rc;
   const size_t ctr_bytes = (size_t)n * Hkv * kFinishers * sizeof(uint32_t);
-  if (ctr_bytes > p->stream_done.cap) {
-    if ((rc = grow(p->dev, p->stream_done, ctr_bytes))) return rc;
-    RELUX_CUDA_TRY(cudaMemsetAsync(p->stream_done.p, 0, p->stream_done.cap, p->dev->stream));
-  }
+  const size_t ctr_cap = p->stream_done.cap;
+  if ((rc = grow(p->dev, p->stream_done, ctr_bytes))) return rc;
+  if (p->stream_done.cap != ctr_cap) RELUX_CUDA_TRY(cudaMemsetAsync(p->stream_done.p, 0, p->stream_done.cap, p->dev->stream));
   if (seqs != inl) {
     size_t bytes = sizeof(GqaSeq) * ((size_t)n + 1);
     if (tree) {   // behind the sequences

@@ -64,10 +64,13 @@ struct Device {
 };
 
 // A device buffer that grows on demand (never shrinks) for inputs that arrive in host memory
-// and for kernel scratch.  Growth synchronises the stream before the old block is freed.
+// and for kernel scratch.  Growth synchronises the stream before the old block is freed; one that a captured call has taken is
+// kept until the pool goes, since the launches of its graph read and write it.
 struct GrowBuf {
   void* p = nullptr;
   size_t cap = 0;
+  bool captured = false;
+  std::vector<void*> kept;
 };
 
 // Tuning knobs of a pool.  Defaults come from the environment ONCE, when the pool is created (RELUX_MLA_GENERIC,

@@ -26,17 +26,22 @@ int32_t cuda_fail(cudaError_t e, const char* what) {
 }
 
 int32_t grow(Device* dev, GrowBuf& b, size_t bytes) {
-  if (bytes <= b.cap) return RELUX_OK;
+  if (bytes <= b.cap) {
+    if (!b.captured && stream_captured(dev)) b.captured = true;
+    return RELUX_OK;
+  }
   size_t want = std::max(bytes, b.cap + b.cap / 2);
   want = (want + 255) & ~(size_t)255;
   if (b.p) {
     RELUX_CUDA_TRY(cudaStreamSynchronize(dev->stream));
-    RELUX_CUDA_TRY(cudaFree(b.p));
+    if (b.captured) b.kept.push_back(b.p);
+    else RELUX_CUDA_TRY(cudaFree(b.p));
     b.p = nullptr;
     b.cap = 0;
   }
   RELUX_CUDA_TRY(cudaMalloc(&b.p, want));
   b.cap = want;
+  b.captured = stream_captured(dev);
   return RELUX_OK;
 }
 
@@ -286,18 +291,22 @@ void tuning_defaults(Tuning* t);
 
 static void pool_free_all(Pool* p) {
   auto fr = [](void* q) { if (q) cudaFree(q); };
+  auto fr_buf = [&](const GrowBuf& b) {
+    fr(b.p);
+    for (void* q : b.kept) fr(q);
+  };
   for (cudaStream_t st : {p->dev->h2d_stream, p->dev->d2h_stream})
     if (st) cudaStreamSynchronize(st);
   for (PipeSlots* ps : {&p->pipe_in_a, &p->pipe_in_b, &p->pipe_app_a, &p->pipe_app_b, &p->pipe_out})
     for (int i = 0; i < PipeSlots::kSlots; i++) {
-      fr(ps->buf[i].p);
+      fr_buf(ps->buf[i]);
       if (ps->copied[i]) cudaEventDestroy(ps->copied[i]);
     }
   for (cudaEvent_t e : p->pipe_calls.done)
     if (e) cudaEventDestroy(e);
   fr(p->storage); fr(p->scales); fr(p->meta);
-  fr(p->in_a.p); fr(p->in_b.p); fr(p->out_buf.p); fr(p->q_abs.p); fr(p->part_o.p); fr(p->part_ml.p); fr(p->work.p); fr(p->stream_done.p); fr(p->seq_list.p);
-  fr(p->o_lat.p); fr(p->q_conv.p); fr(p->rope_tab.p); fr(p->layer_buf.p); fr(p->shadow_f32); fr(p->chunk_tab.p); fr(p->step_rows.p); fr(p->expand_buf.p);
+  fr_buf(p->in_a); fr_buf(p->in_b); fr_buf(p->out_buf); fr_buf(p->q_abs); fr_buf(p->part_o); fr_buf(p->part_ml); fr_buf(p->work); fr_buf(p->stream_done); fr_buf(p->seq_list);
+  fr_buf(p->o_lat); fr_buf(p->q_conv); fr_buf(p->rope_tab); fr_buf(p->layer_buf); fr(p->shadow_f32); fr_buf(p->chunk_tab); fr_buf(p->step_rows); fr_buf(p->expand_buf);
   if (p->h_stage) cudaFreeHost(p->h_stage);
   for (void* block : p->stage_held) cudaFreeHost(block);
   if (p->sel_host) cudaFreeHost(p->sel_host);
@@ -381,10 +390,11 @@ static int32_t pipe_event(cudaEvent_t* e) {
 }
 // A slot's buffer may be replaced only when nothing queued on any stream still uses it.
 static int32_t pipe_grow(Pool* p, GrowBuf& b, size_t bytes) {
-  if (bytes <= b.cap) return RELUX_OK;
   Device* dev = p->dev;
-  if (dev->h2d_stream) RELUX_CUDA_TRY(cudaStreamSynchronize(dev->h2d_stream));
-  if (dev->d2h_stream) RELUX_CUDA_TRY(cudaStreamSynchronize(dev->d2h_stream));
+  if (bytes > b.cap) {
+    if (dev->h2d_stream) RELUX_CUDA_TRY(cudaStreamSynchronize(dev->h2d_stream));
+    if (dev->d2h_stream) RELUX_CUDA_TRY(cudaStreamSynchronize(dev->d2h_stream));
+  }
   return grow(dev, b, bytes);
 }
 // Small calls are bound by what they queue: with events for each of four inputs and the output a latent step had 20 waits and records, and has 7:

@@ -44,3 +44,46 @@ def test_plain_calls_behind_a_captured_prompt(dev, int8):
     dq.free()
     out.free()
     pool.destroy()
+
+
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("S", [6, 12, 64])
+def test_workspaces_that_grow_behind_a_capture(dev, int8, S):
+    """A tree's call in a graph, float32 queries and head-major outputs, so that they are converted in workspaces too; then plain calls of forty times its size,
+    which need larger ones; then the graph's launches."""
+    from relux_b200 import lib as L
+    rng = np.random.default_rng(S)
+    B, H, Hkv, few = 40, 32, 8, 2
+    lens = [int(x) for x in rng.integers(150, 300, B)]
+    pool, cache = filled(dev, rng, lens, H, Hkv, S, int8=int8)
+    parents = G.random_tree(rng, S)
+    k, v, q = G.rows(rng, B * S, Hkv), G.rows(rng, B * S, Hkv, "v"), G.bf16(rng.standard_normal((B, S, H, D)))
+
+    def case(m):
+        return [dev.upload(x) for x in (q[:m], k[:m * S], v[:m * S], np.zeros((m, H, S, D), np.float32))]
+
+    def call(m, b):
+        pool.tree_verify(0, m, b[0], b[3], b[1], b[2], H, D, D ** -0.5, parents, out_layout=L.LAYOUT_HEAD_MAJOR)
+
+    small, large = case(few), case(B)
+    call(few, small)
+    want = small[3].download((few, H, S, D), np.float32)
+    for b in range(few):
+        K, V = (np.concatenate([c[b], G.held(x[b * S:(b + 1) * S], int8)]) for c, x in ((cache.k, k), (cache.v, v)))
+        exact, bound = G.attend(K, V, q[b], lens[b], G.ancestors(parents, S, S), D ** -0.5)
+        G.check(want[b].transpose(1, 0, 2), exact, bound)
+    graph = Graph(dev, lambda: call(few, small))
+    call(B, large)
+    dev.sync()
+    spoil = [dev.upload(np.full(1 << m, np.nan, np.float32)) for m in range(12, 24)]      # in whatever is free now
+    for _ in range(2):
+        small[3].zero()
+        graph.launch()
+        assert same(small[3].download(want.shape, np.float32), want)
+        call(B, large)
+    assert all(np.isnan(s.download((1 << m,), np.float32)).all() for m, s in zip(range(12, 24), spoil))
+    assert pool.status() == 0
+    graph.free()
+    for x in small + large + spoil:
+        x.free()
+    pool.destroy()

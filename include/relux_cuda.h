@@ -82,7 +82,8 @@ extern "C" {
  * a < 1e-36 is stored as zeros, one that holds an infinity or a NaN reads back as NaN in every place.  Rows are quantised as they are
  * appended, attention takes number * scale for the value, relux_pool_read_rows, relux_seq_save_file and relux_gqa_read_kv give it.
  * Queries: up to 32 rows a kv head (heads of its group times query tokens) keep 11 bits of every value, of more rows 8 (bf16).
- * All calls of a GQA pool take such a pool in RELUX_ATTN_FAST; the two reference modes and relux_gqa_decode_noalloc refuse it. */
+ * All calls of a GQA pool take such a pool in RELUX_ATTN_FAST; the two reference modes and relux_gqa_decode_noalloc refuse it.
+ * relux_gqa_decode, _verify and _step take groups of more than 32 heads on such a pool (a bf16 pool's FAST calls, trees and relux_gqa_forward_cached do not). */
 #define RELUX_POOL_FLAG_CACHE_INT8 2
 
 typedef void* relux_device_t;

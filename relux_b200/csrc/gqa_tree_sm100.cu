@@ -77,7 +77,7 @@ struct TreeCommon {
   int32_t causal;
   const int32_t* table;
   int32_t table_stride, num_pages, n_seqs, Hkv, H, g, S, R;
-  uint32_t over_g;             // 2^31 / g, rounded up: a row below 2^26 over g is a product (a division by g a row was half of a piece's fixed cost)
+  uint32_t over_g;             // 2^31 / g, rounded up: a row below 2^31 / g over g is a product (a division by g a row was half of a piece's fixed cost)
   int32_t n_rb, rows_rb;       // groups of a sequence, rows of each (the last may have fewer)
   int32_t krow0, vrow0;
   const float* scales;         // 8-bit cache: of the layer
@@ -1177,7 +1177,8 @@ int32_t launch_gqa_tree_sm100(Pool* p, const SeqBatch& sb, const relux_attn_args
   c.rows_rb = (int)((R + c.n_rb - 1) / c.n_rb + 15) / 16 * 16;
   c.n_rb = (int)((R + c.rows_rb - 1) / c.rows_rb);
   const int64_t groups = (int64_t)n * c.n_rb;
-  if (R >= ((int64_t)1 << 26) || groups >= ((int64_t)1 << 24)) { set_error("more query rows than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
+  // R g: over_g g is less than 2^31 + g, so that a row times it stays below the next whole number while row g is below 2^31
+  if (R >= ((int64_t)1 << 26) || R * g > ((int64_t)1 << 31) || groups >= ((int64_t)1 << 24)) { set_error("more query rows than one attention launch addresses"); return RELUX_ERR_UNSUPPORTED; }
   std::vector<TreeSeq> seqs;
   try {
     seqs.resize((size_t)groups + 1);

@@ -80,8 +80,12 @@ extern "C" {
  * [-127, 127] and one float32 scale, 264 bytes of K and V a token and kv head instead of 512.  With a the largest magnitude of the row's
  * 128 values, scale = a / 127 and number = value * (127 / a) to the nearest, even on a tie, each operation rounded to float32; a row with
  * a < 1e-36 is stored as zeros, one that holds an infinity or a NaN reads back as NaN in every place.  Rows are quantised as they are
- * appended, attention takes number * scale for the value, relux_pool_read_rows, relux_seq_save_file and relux_gqa_read_kv give it.
+ * appended, attention takes number * scale for the value and relux_gqa_read_kv gives it (as float32, or rounded to bf16).
+ * relux_pool_read_rows and relux_seq_save_file give it rounded to bf16: loading such a file into an 8-bit pool quantises rounded values, so the
+ * rows that come back are not bit for bit those that were saved (a scale moves by up to 2^-8 of itself, a number by one).
  * Queries: up to 32 rows a kv head (heads of its group times query tokens) keep 11 bits of every value, of more rows 8 (bf16).
+ * Values: a row's scale is taken in 11 bits, over the largest scale of the kv head's rows that the call has read so far, those of its new rows included that a
+ * query does not see; of scales more than 2^21 below that one fewer bits are left, and of some 2^32 below none.
  * All calls of a GQA pool take such a pool in RELUX_ATTN_FAST; the two reference modes and relux_gqa_decode_noalloc refuse it.
  * relux_gqa_decode, _verify and _step take groups of more than 32 heads on such a pool (a bf16 pool's FAST calls, trees and relux_gqa_forward_cached do not). */
 #define RELUX_POOL_FLAG_CACHE_INT8 2
@@ -360,7 +364,7 @@ int32_t relux_mla_verify(relux_pool_t pool, const relux_attn_args* attn, const r
  * An infinity or a NaN in a row past the cursor (a node's, or what an older draft has left) reaches the outputs of the queries that see it
  * and no others; where it is among a node's values, all of the output of that head becomes NaN.
  * Shapes: GQA pools (bf16 or 8-bit) with page_tokens = 64 and head_dim = 128, num_heads / num_kv_heads <= 32, up to 64 nodes,
- * RELUX_ATTN_FAST; others are refused.  Commit what was accepted with relux_gqa_tree_commit.  No counterpart in the reference, whose
+ * RELUX_ATTN_FAST; others are refused.  Above 32 rows a kv head (heads of its group times nodes) queries are rounded to bf16.  Commit what was accepted with relux_gqa_tree_commit.  No counterpart in the reference, whose
  * speculative decoder drafts one chain (speculative.go:189-207). */
 typedef struct relux_tree_args {
   const int32_t* parents;    /* host [n_trees][q_tokens]; entries past a sequence's nodes are not read */

@@ -85,7 +85,7 @@ extern "C" {
  * rows that come back are not bit for bit those that were saved (a scale moves by up to 2^-8 of itself, a number by one).
  * Queries: up to 32 rows a kv head (heads of its group times query tokens) keep 11 bits of every value, of more rows 8 (bf16).
  * Values: a row's scale is taken in 11 bits, over the largest scale of the kv head's rows that the call has read so far, those of its new rows included that a
- * query does not see; of scales more than 2^21 below that one fewer bits are left, and of some 2^32 below none.
+ * query does not see; of scales more than 2^20 below that one fewer bits may be left, and of some 2^31 below none.
  * All calls of a GQA pool take such a pool in RELUX_ATTN_FAST; the two reference modes and relux_gqa_decode_noalloc refuse it.
  * relux_gqa_decode, _verify and _step take groups of more than 32 heads on such a pool (a bf16 pool's FAST calls, trees and relux_gqa_forward_cached do not). */
 #define RELUX_POOL_FLAG_CACHE_INT8 2
@@ -114,7 +114,8 @@ int32_t relux_cuda_device_info(relux_device_t dev, char* name, int32_t name_len,
 int32_t relux_cuda_launch_count(relux_device_t dev, int64_t* count);
 /* The CUDA stream (cudaStream_t) all work of this handle is issued on, for callers that order their own device work
  * with it.  Where a caller captures calls on it, a launch of the graph runs with, and changes, the lengths that the device has
- * then; the host's (relux_seq_len, capacity checks) know of the calls alone.  A latent decode, verify or step call on a pool on which a
+ * then (attention and trees of a GQA pool keep those of the capture); the host's (relux_seq_len, capacity checks) know of the calls alone.  What a captured call
+ * uses of the pool's memory stays until the pool is destroyed.  A latent decode, verify or step call on a pool on which a
  * call that changes lengths has been captured runs with the device's lengths as well.  No counterpart in the reference. */
 int32_t relux_cuda_stream(relux_device_t dev, void** stream);
 

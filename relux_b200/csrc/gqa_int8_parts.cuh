@@ -16,8 +16,8 @@
 //   V: thread (n, c) takes bytes 16 n .. 16 n + 15 of tokens 2c, 2c + 1, 2c + 8, 2c + 9; output block j's column n is dim 16 n + j.
 // A code is stored as c + 128: below the exponent of 1024 that is a binary16 number, and one subtraction (two instructions for two codes) makes it c, which
 // binary16 holds exactly.  Queries are brought to binary16 with a power of two per row, which keeps 11 bits of a float32 query where bf16 keeps 8.  P carries
-// s^v over a power of two that grows with the largest s^v seen so far (O is then rescaled as for a new maximum): 11 bits of it, 2^21 between the
-// largest row and one that loses bits.  (P s^v in bf16, whose range needs no unit, was off by 2.5e-3 of the result where this is 1.7e-3, the rounding of a
+// s^v over a power of two that grows with the largest s^v seen so far (O is then rescaled as for a new maximum): 11 bits of it, 2^20 between the
+// largest row and one that may lose bits.  (P s^v in bf16, whose range needs no unit, was off by 2.5e-3 of the result where this is 1.7e-3, the rounding of a
 // bf16 output alone, and takes four instructions for two codes.)
 #pragma once
 

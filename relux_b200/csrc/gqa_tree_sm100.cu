@@ -4,8 +4,9 @@
 // o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  where query token i sees every cached row and, of the drafted ones, itself
 // and its ancestors; of a prompt, every row up to its own.  The g query heads of a kv head times the S nodes are R rows that read the same keys: R * 4 * 128
 // operations for the 512 (264) bytes of a token and kv head, so the cache's bytes bound trees of up to some 200 rows (100 on the 8-bit cache) and the tensor
-// cores and the softmax larger ones.  Measured: 64 x 8192 tokens, 64 rows 332 us on bf16 (6.5 TB/s), 378 on 8 bits (2.9 TB/s); 8 x 32768 tokens, 512 rows
-// 546 us (1.0 PFLOP/s), 648 on 8 bits.
+// cores and the softmax larger ones.  Measured, join of the parts included, on a card that was idle before (1965 MHz): 64 x 8192 tokens, 64 rows 337 us on bf16 (6.4
+// TB/s), 396 on 8 bits (2.8 TB/s); 8 x 32768 tokens, 512 rows 546 us (1.0 PFLOP/s), 667 on 8 bits.  After a second of such calls, under the power cap (990 W, 1360
+// to 1480 MHz on bf16, 1770 on 8 bits): 385, 440, 645 and 750.  Times further down are of this kernel alone, from idle.
 //
 // A STREAM is the tiles of 128 keys that up to 256 of a kv head's rows (one or two blocks of 128, M of both contractions) see.  All streams of the
 // call, each its tiles and kFixUnits units of fixed cost, laid end to end, are cut into a range per SM (make_ranges); a PIECE is the part of a stream inside a
@@ -16,8 +17,8 @@
 //   producer   a tile's K and V by TMA, 32 KB each, into a ring; on the 8-bit cache page by page, 8 KB each, and the scales, into rings of their own
 //   scales     (8-bit cache) a warp: the keys' scales of a tile to where the softmax reads them, the values' over their unit to the converters
 //   converters (8-bit cache, four warps for K, four for V) codes -> binary16 operands in the ring's swizzled layout.  K as whole numbers: a row's scale multiplies its column of
-//              scores, in float32.  V times its scale over a power of two that all of the piece's rows share so far (11 bits, as P has then; 2^29 between
-//              the largest row and one that is no longer exact to 11 bits); where a row comes that is too large for it, the power grows and O is rescaled.
+//              scores, in float32.  V times its scale over a power of two that all of the piece's rows share so far (11 bits, as P has then; 2^21 between
+//              the largest row and one that may not be exact to 11 bits); where a row comes that is too large for it, the power grows and O is rescaled.
 //   MMA        step k = (tile, block): S = Q K^T (S buffer k & 1), O[block] += P V with P read from tensor memory over the scores it came from
 //   softmax    eight warps of 16 rows of a block each, four lanes to a row: scores from TMEM, running max (updated lazily), P back to TMEM.  Up to
 //              64 rows, four warps take the even steps and four the odd ones, each with an O of its own,

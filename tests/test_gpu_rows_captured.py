@@ -87,3 +87,29 @@ def test_workspaces_that_grow_behind_a_capture(dev, int8, S):
     for x in small + large + spoil:
         x.free()
     pool.destroy()
+
+
+@pytest.mark.parametrize("mode", [0, 1])     # cudaStreamCaptureModeGlobal, ThreadLocal: no call that allocates may be seen by the capture
+def test_a_prompt_captured_in_a_strict_mode(dev, mode):
+    import ctypes as C
+    from relux_b200 import lib as L
+    rng = np.random.default_rng(2)
+    H, Hkv, S, lens, ids = 16, 4, 24, [50, 90, 30], [2, 1]
+    pool, _ = filled(dev, rng, lens, H, Hkv, 0)
+    q = G.bf16(rng.standard_normal((2, S, H, D)))
+    dq, out = dev.upload(q), dev.upload(np.zeros(q.shape, np.float32))
+    call = lambda: pool.decode(0, 2, dq, out, H, D, D ** -0.5, q_tokens=S, seq_ids=ids)  # noqa: E731
+    call()
+    want = out.download(q.shape, np.float32)
+    rt, stream, graph, ready = C.CDLL("libcudart.so.12"), C.c_void_p(), C.c_void_p(), C.c_void_p()
+    L.check(dev.lib.relux_cuda_stream(dev.h, C.byref(stream)))
+    assert rt.cudaStreamBeginCapture(stream, mode) == 0
+    call()
+    assert rt.cudaStreamEndCapture(stream, C.byref(graph)) == 0 and rt.cudaGraphInstantiate(C.byref(ready), graph, C.c_ulonglong(0)) == 0
+    out.zero()
+    assert rt.cudaGraphLaunch(ready, stream) == 0
+    assert same(out.download(q.shape, np.float32), want)
+    assert rt.cudaGraphExecDestroy(ready) == 0 and rt.cudaGraphDestroy(graph) == 0
+    dq.free()
+    out.free()
+    pool.destroy()

@@ -113,3 +113,46 @@ def test_a_prompt_captured_in_a_strict_mode(dev, mode):
     dq.free()
     out.free()
     pool.destroy()
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_a_captured_commit_and_read_back(dev, int8):
+    """Commits in a graph go by the lengths that the device has: a second launch commits the next nodes behind the first one's."""
+    from tests.test_gpu_cache_int8 import read
+    rng = np.random.default_rng(4)
+    Hkv, S, lens = 3, 64, [50, 127, 3]
+    pool, cache = filled(dev, rng, lens, Hkv, Hkv, S, int8=int8)
+    k, v = G.rows(rng, 3 * S, Hkv), G.rows(rng, 3 * S, Hkv, "v")
+    pool.append(0, k, v, 3, n_new=[S] * 3, advance=False)
+    ids, path, n = np.array([2, 0], np.int32), np.array([[1, 4, 5, 20], [0, 3, 0, 0]], np.int32), np.array([4, 2], np.int32)
+    bufs = [dev.upload(np.zeros((8, Hkv, D), np.float32)) for _ in range(2)]
+
+    def call():
+        pool.tree_commit(0, path, n, seq_ids=ids)
+        pool.read_kv(0, 2, bufs[0], bufs[1], [3, 50], [6, 2], seq_ids=ids)
+
+    graph = Graph(dev, call)
+    pool.set_len(0, [50, 3], seq_ids=[0, 2])          # the host's lengths know of the captured call; the device's have not moved
+    want = [[np.concatenate([G.held(x[b * S:(b + 1) * S], int8)]) for x in (k, v)] for b in range(3)]
+    at = {0: 0, 2: 0}
+    for _ in range(2):
+        graph.launch()
+        for b, p, m in ((2, path[0], 4), (0, path[1], 2)):
+            for w in want[b]:
+                w[at[b]:at[b] + m] = w[at[b] + p[:m]]
+            at[b] += m
+        for i, buf in enumerate(bufs):
+            assert same(buf.download((8, Hkv, D), np.float32), np.concatenate([want[2][i][:6], want[0][i][:2]]))
+    for b in range(3):
+        gk, gv = read(pool, dev, 0, [lens[b]], [S], seq_ids=[b])
+        assert same(gk, want[b][0]) and same(gv, want[b][1])
+    x = G.rows(rng, 2, Hkv)
+    pool.append(0, x, x, 2, seq_ids=[0, 2])           # by the device's lengths
+    for i, b in enumerate((0, 2)):
+        gk, _ = read(pool, dev, 0, [lens[b] + at[b]], [1], seq_ids=[b])
+        assert same(gk, G.held(x[i:i + 1], int8))
+    assert pool.status() == 0
+    graph.free()
+    for b in bufs:
+        b.free()
+    pool.destroy()

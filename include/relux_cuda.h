@@ -636,6 +636,68 @@ typedef struct relux_matmul_args {
 } relux_matmul_args;
 int32_t relux_matmul_f32_bf16(relux_pool_t pool, const relux_matmul_args* args);
 
+/* ---- rows between the projections -----------------------------------------------------------------
+ * RMSNorm.Forward (internal/transformer/rmsnorm.go:69-97) with the residual's addition of Block.Forward
+ * (internal/transformer/transformer_block.go:119-142) in one pass over the rows:
+ *   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
+ * h goes to residual_out (rounded to the residual's type), y to out as float32 or bf16, and / or to codes and scales as an 8-bit row for
+ * relux_matmul_int8: d whole numbers of [-127, 127] and one float32 scale, by the rule of the 8-bit cache (RELUX_POOL_FLAG_CACHE_INT8).
+ * Everything is float32 up to the one rounding of each result; the norm is that of h before it is rounded.  Sums of squares past
+ * float32's range give what float32 gives (rows of zeros).  A row that holds an infinity or a NaN comes out as NaN wherever the formula does,
+ * and its 8-bit form is NaN in every place (the scale); other rows are not touched by it.
+ * x, residual, residual_out and out may be the same memory where their types are: each value is read before it is written.
+ * Shapes: d a multiple of 8 (16 with codes), up to 32768.  All memory is the device's.  Asynchronous on the handle's stream. */
+typedef struct relux_rmsnorm_args {
+  int32_t n_rows, d;
+  float eps;                 /* 1e-5 in the reference's blocks (transformer_block.go:62-63) */
+  int32_t x_dtype, residual_dtype, weight_dtype, out_dtype;   /* RELUX_DTYPE_* */
+  int32_t reserved[5];
+  const void* x;             /* [n_rows][d] */
+  const void* residual;      /* [n_rows][d], or NULL: h = x */
+  const void* weight;        /* [d], or NULL: ones */
+  void* residual_out;        /* [n_rows][d] of residual_dtype, or NULL */
+  void* out;                 /* [n_rows][d] of out_dtype, or NULL */
+  int8_t* codes;             /* [n_rows][d], or NULL; with scales */
+  float* scales;             /* [n_rows] */
+} relux_rmsnorm_args;
+int32_t relux_rmsnorm(relux_pool_t pool, const relux_rmsnorm_args* args);
+
+/* The 8-bit form of rows as they are (attention's output ahead of the output projection; weights in checkpoint order [out][in], a
+ * row an output), by the same rule.  d a multiple of 16, up to 32768.  Asynchronous on the handle's stream.  No counterpart in the
+ * reference, whose weights and activations are bf16 and float32. */
+typedef struct relux_int8_rows_args {
+  int32_t n_rows, d, x_dtype, reserved;
+  const void* x;             /* device [n_rows][d] */
+  int8_t* codes;             /* device [n_rows][d] */
+  float* scales;             /* device [n_rows] */
+} relux_int8_rows_args;
+int32_t relux_int8_rows(relux_pool_t pool, const relux_int8_rows_args* args);
+
+/* Weights [k][n] (the layout of optim.Param.Data) as 8-bit weights for relux_matmul_int8: codes [n][k], a scale per output column, by the same
+ * rule.  k a multiple of 16, n of 8.  Once per model.  Asynchronous on the handle's stream.  No counterpart in the reference. */
+typedef struct relux_int8_weights_args {
+  int32_t k, n, w_dtype, reserved;
+  const void* w;             /* device [k][n] */
+  int8_t* codes;             /* device [n][k] */
+  float* scales;             /* device [n] */
+} relux_int8_weights_args;
+int32_t relux_int8_weights(relux_pool_t pool, const relux_int8_weights_args* args);
+
+/* C [m][n] = a_scales[m] * w_scales[n] * sum over k of a[m][k] * w[n][k]: relux_matmul_f32_bf16 on 8-bit rows and weights.  The sum is
+ * exact (32-bit whole numbers), so a row's result does not depend on the rows around it nor on the GPU's schedule; it is rounded to float32, multiplied by
+ * the row's scale, then by the column's, and rounded once more for a bf16 result.  k a multiple of 16, up to 131056, n of 8.
+ * Asynchronous on the handle's stream.  No counterpart in the reference. */
+typedef struct relux_matmul_int8_args {
+  int32_t m, k, n, out_dtype;
+  const int8_t* a;           /* device [m][k] */
+  const float* a_scales;     /* device [m] */
+  const int8_t* w;           /* device [n][k] */
+  const float* w_scales;     /* device [n] */
+  void* out;                 /* device [m][n] */
+  int32_t reserved[4];
+} relux_matmul_int8_args;
+int32_t relux_matmul_int8(relux_pool_t pool, const relux_matmul_int8_args* args);
+
 /* ---- expansion of the cached MLA latents --------------------------------------------------------
  * What MLA.forwardCached does before it scores a multi-token call: every cached latent row times W_UK and W_UV
  * (internal/transformer/mla.go:323-326), here as one tensor-core GEMM with bf16 results.  The library's own prompt path

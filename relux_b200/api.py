@@ -48,6 +48,10 @@ def _dtype_flag(a, explicit=None):
     raise TypeError("arrays must be float32 or uint16 (bf16 bits), got %s" % a.dtype)
 
 
+def _size(flag):
+    return 2 if flag == L.DTYPE_BF16 else 4
+
+
 class Device:
     """One GPU.  Mirrors compute.NewComputeBackend's role for this path (internal/compute/factory.go:32-85):
     it either opens a usable sm_100 device or raises -- there is no silent native fallback."""
@@ -273,6 +277,54 @@ class Pool:
         args = L.MatmulArgs(m=m, k=k, n=n, mode=mode, a=_ptr(a), a_mem=_mem(a), c_mem=_mem(res), b=_ptr(w), c=_ptr(res))
         L.check(self.lib.relux_matmul_f32_bf16(self.h, C.byref(args)))
         return res
+
+    @staticmethod
+    def _device_only(call, needs, **arrays):
+        """Addresses of device arrays: buffers (checked against `needs` bytes), or plain addresses."""
+        out = {}
+        for name, a in arrays.items():
+            if a is not None and not isinstance(a, (DeviceBuffer, int)):
+                raise TypeError("%s: %s must be device memory" % (call, name))
+            if isinstance(a, DeviceBuffer) and a.nbytes < needs[name]:
+                raise ValueError("%s: %s has %d bytes, %d needed" % (call, name, a.nbytes, needs[name]))
+            out[name] = _ptr(a) or 0
+        return out
+
+    def rmsnorm(self, n_rows, d, x, weight=None, eps=1e-5, residual=None, residual_out=None, out=None, codes=None, scales=None, dtype=None,
+                residual_dtype=None, weight_dtype=None, out_dtype=None):
+        """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, row by row (relux_rmsnorm): h to residual_out, y to out and / or, in 8 bits, to
+        codes and scales.  Device buffers, or addresses with their dtypes; residual and out are of x's type and an addressed weight is bf16 where
+        nothing else is said."""
+        xt = _dtype_flag(x, dtype)
+
+        def flag(a, explicit, otherwise):
+            return explicit if explicit is not None else a.dtype_flag if isinstance(a, DeviceBuffer) else otherwise
+        rt, wt, ot = flag(residual, residual_dtype, xt), flag(weight, weight_dtype, L.DTYPE_BF16), flag(out, out_dtype, xt)
+        size = n_rows * d
+        a = self._device_only("rmsnorm", dict(x=size * _size(xt), residual=size * _size(rt), weight=d * _size(wt), residual_out=size * _size(rt),
+                                              out=size * _size(ot), codes=size, scales=4 * n_rows),
+                              x=x, residual=residual, weight=weight, residual_out=residual_out, out=out, codes=codes, scales=scales)
+        L.check(L.packed["rmsnorm"](self.h, L.pack_rmsnorm(n_rows, d, float(eps), xt, rt, wt, ot, a["x"], a["residual"], a["weight"], a["residual_out"],
+                                                           a["out"], a["codes"], a["scales"])))
+
+    def int8_rows(self, n_rows, d, x, codes, scales, dtype=None):
+        """The 8-bit form of rows x [n_rows, d] (relux_int8_rows): codes int8 [n_rows, d], scales float32 [n_rows]."""
+        t = _dtype_flag(x, dtype)
+        a = self._device_only("int8_rows", dict(x=n_rows * d * _size(t), codes=n_rows * d, scales=4 * n_rows), x=x, codes=codes, scales=scales)
+        L.check(L.packed["int8_rows"](self.h, L.pack_int8_rows(n_rows, d, t, a["x"], a["codes"], a["scales"])))
+
+    def int8_weights(self, k, n, w, codes, scales, dtype=None):
+        """Weights w [k, n] as 8-bit weights (relux_int8_weights): codes int8 [n, k], scales float32 [n]."""
+        t = _dtype_flag(w, dtype)
+        a = self._device_only("int8_weights", dict(w=k * n * _size(t), codes=k * n, scales=4 * n), w=w, codes=codes, scales=scales)
+        L.check(L.packed["int8_weights"](self.h, L.pack_int8_weights(k, n, t, a["w"], a["codes"], a["scales"])))
+
+    def matmul_int8(self, m, k, n, a, a_scales, w, w_scales, out, out_dtype=None):
+        """out [m, n] = a_scales[m] * w_scales[n] * sum a[m] w[n] (relux_matmul_int8): a int8 [m, k], w int8 [n, k], on the device."""
+        t = _dtype_flag(out, out_dtype)
+        b = self._device_only("matmul_int8", dict(a=m * k, a_scales=4 * m, w=n * k, w_scales=4 * n, out=m * n * _size(t)), a=a, a_scales=a_scales, w=w,
+                              w_scales=w_scales, out=out)
+        L.check(L.packed["matmul_int8"](self.h, L.pack_matmul_int8(m, k, n, t, b["a"], b["a_scales"], b["w"], b["w_scales"], b["out"])))
 
     def import_mla_weights(self, d_model, num_heads, nope_dim, rope_dim, v_dim, dc, dst, q_proj=None, kv_a_proj_with_mqa=None,
                            kv_b_proj=None, o_proj=None, q_pe_proj=None, k_pe_proj=None, fused_rope=False):

@@ -183,6 +183,9 @@ struct Pool {
   CUtensorMap tmap_gqa{};   // 2-D [rows][D],      box 64 x 64, 128-byte swizzle
   bool has_tmap = false;
   bool mla_blocked = false;   // MLA pages stored as 64-column blocks (see mla_page_off)
+  GrowBuf int8_part;                  // 8-bit products: pieces of tiles
+  static constexpr int kArrived = 1024;
+  int32_t* int8_arrived = nullptr;    // and how many of a tile's have arrived, zero between launches
   // layer-level step (layer_step.cu): RoPE tables [cos | sin][positions][dHR / 2] and the step's scratch block
   GrowBuf rope_tab, layer_buf;
   int rope_dim = 0, rope_positions = 0;
@@ -291,6 +294,10 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a);
 int32_t do_spec_accept(Pool* p, const relux_spec_accept_args* a);
 int32_t do_sample(Pool* p, const relux_sample_args* a);
 int32_t do_matmul(Pool* p, const relux_matmul_args* a);
+int32_t do_rmsnorm(Pool* p, const relux_rmsnorm_args* a);
+int32_t do_int8_rows(Pool* p, const relux_int8_rows_args* a);
+int32_t do_int8_weights(Pool* p, const relux_int8_weights_args* a);
+int32_t do_matmul_int8(Pool* p, const relux_matmul_int8_args* a);
 int32_t do_import_mla(Pool* p, const relux_mla_import_args* a);
 int32_t do_selftest_wait(Pool* p, int32_t polls);
 // After a fused call that counted sb's rows and failed: the lengths before it, on the host and, whatever the call had queued

@@ -18,6 +18,7 @@
 #include <cstdlib>
 #include "common.cuh"
 #include "internal.h"
+#include "projection.cuh"
 #include "umma.cuh"
 
 namespace relux {
@@ -26,78 +27,9 @@ int32_t stage_in(Pool* p, GrowBuf& buf, const void* src, size_t bytes, int mem, 
 
 namespace {
 
-constexpr int kMaxWeights = 4;   // weight matrices that share one activation matrix in a launch
-constexpr int kTileN = 128, kTileK = 64;
+constexpr int kTileN = kGemmTileCols, kTileK = 64;
 constexpr int kStageW = kTileK * kTileN * 2;   // 16 KB of weights: two [64 k][64 n] blocks, 128-byte swizzle, MN-major
 constexpr int kMaxTok = 256;                   // activation rows of one block
-
-// How a launch's tiles (128 weight columns x one block of rows) are dealt out.  `full` rounds of whole tiles, neighbouring tiles
-// side by side: the workers then walk K in step and together read whole weight rows, which DRAM serves faster than 256-byte
-// pieces of rows that lie far apart (0.54 GB: 86.8 us so, 90.1 us with every worker somewhere else in K; 0.82 GB: 128.5 against
-// 130.8 us).  The tiles that are left are cut along K, `split` equal parts each (also in step), or (split = 0) their K steps,
-// laid end to end, are cut into ranges that differ by at most one step.  A PIECE is the part of a tile that one worker does;
-// piece j of a tile (in K order) is split j of the result.
-// With more rows than a block holds, `beside` blocks have workers of their own that walk the same columns of weights in step, so
-// that a column is read once for all of them; the blocks after those are further tiles of the same workers.
-struct GemmRanges {
-  int32_t workers, steps, full, split;   // of one of the blocks beside each other.  steps: K steps per tile (0: one piece per tile)
-  int32_t range, more;                   // split = 0: steps per worker, one more for the first `more` of them
-  int32_t rest;                          // tiles that are left after the full rounds
-  int32_t beside, row_blocks, block_rows, col_tiles;
-  bool in_turns() const { return row_blocks != beside; }
-  __host__ __device__ int tile_of(int col, int row) const { return row / block_rows / beside * col_tiles + col; }
-  __host__ __device__ int begin(int w) const {   // in steps of the tiles that are left
-    if (!split) return w * range + (w < more ? w : more);
-    return w < rest * split ? w / split * steps + w % split * steps / split : rest * steps;
-  }
-  __host__ __device__ int worker_of(int u) const {   // split = 0
-    const int big = more * (range + 1);
-    return u < big ? (int)((unsigned)u / (unsigned)(range + 1)) : more + (int)((unsigned)(u - big) / (unsigned)range);
-  }
-  __host__ __device__ int pieces(int tile) const {
-    const int t = tile - full * workers;
-    if (!steps || t < 0) return 1;
-    return split ? split : worker_of((t + 1) * steps - 1) - worker_of(t * steps) + 1;
-  }
-};
-// The pieces of one worker: GemmWalk walk(rg, w); while (walk.next()) ... walk.col, walk.block, steps [k0, k1), split.
-// kBlocks: there may be more than one row block.
-template <bool kBlocks>
-struct GemmWalk {
-  const GemmRanges& g;
-  int w, n, u, u1, col, block, block0, k0, k1, split;
-  __device__ GemmWalk(const GemmRanges& rg, int id)
-      : g(rg), w(kBlocks ? id / rg.beside : id), n(0), u(rg.begin(w)), u1(rg.begin(w + 1)), col(0), block(0), block0(kBlocks ? id - w * rg.beside : 0),
-        k0(0), k1(0), split(0) {}
-  __device__ int total() const { return g.full * g.steps + g.begin(w + 1) - g.begin(w); }
-  __device__ bool next() {
-    int tile;
-    split = 0;
-    if (n < g.full) {
-      tile = n++ * g.workers + w;
-      k0 = 0;
-      k1 = g.steps;
-    } else {
-      if (u >= u1) return false;
-      const int t = u / g.steps;
-      tile = g.full * g.workers + t;
-      k0 = u - t * g.steps;
-      u = min(u1, (t + 1) * g.steps);
-      k1 = u - t * g.steps;
-      split = g.split ? w - t * g.split : w - g.worker_of(t * g.steps);
-    }
-    col = tile;
-    if constexpr (kBlocks) {
-      block = block0;
-      if (g.row_blocks != g.beside) {
-        const int turn = tile / g.col_tiles;
-        col = tile - turn * g.col_tiles;
-        block += turn * g.beside;
-      }
-    }
-    return true;
-  }
-};
 
 struct GemmMaps {
   CUtensorMap a;                 // activations [M][K] bf16, box: 64 k x NT rows
@@ -420,11 +352,6 @@ __global__ void sum_splits_kernel(const float* __restrict__ part, GemmRanges rg,
   reinterpret_cast<float4*>(out)[i] = acc;
 }
 
-struct WeightRef {
-  const void* w;
-  int n;
-};
-
 template <int NT>
 int32_t launch_skinny_gemm_rows(Pool* p, const GemmMaps& maps, const GemmParams& g, int workers) {
   if (int32_t rc = allow_smem(p->dev, skinny_gemm_sm100_kernel<NT>, GemmShape<NT>::kSmem)) return rc;
@@ -434,53 +361,10 @@ int32_t launch_skinny_gemm_rows(Pool* p, const GemmMaps& maps, const GemmParams&
   return RELUX_OK;
 }
 
-// Deals the tiles to one worker per SM, `beside` blocks of `block_rows` rows beside each other.  max_pieces: pieces of a tile that
-// the scratch holds.  *cost_us: what this takes beyond what every dealing takes, from measured parts (4 to 25600 rows against
-// weights of 1024 x 1024 to 16384 x 16384): a step takes an SM 0.28 us whatever the rows of its block, and a tenth more where the
-// workers don't walk in step; the weights come at 7 TB/s, again for every turn of blocks when they exceed L2; the last piece of
-// a worker is written at 16 ns per row with nothing to hide it; pieces are written and read at 3 TB/s.
-GemmRanges deal_tiles(int sms, int col_tiles, int M, int block_rows, int beside, int K, int cols, int max_pieces, int split_knob, double* cost_us) {
-  GemmRanges r{};
-  r.steps = (K + kTileK - 1) / kTileK;
-  r.col_tiles = col_tiles;
-  r.row_blocks = (M + block_rows - 1) / block_rows;
-  r.block_rows = block_rows;
-  r.beside = beside;
-  const int turns = (r.row_blocks + beside - 1) / beside, tiles = col_tiles * turns, units = tiles * r.steps;
-  r.workers = std::max(1, std::min(std::max(1, sms / beside), units / 4));   // pieces of fewer than four steps do not pay for their share of the result
-  if (split_knob) r.workers = std::max(1, (int)std::min<int64_t>(units, (int64_t)tiles * split_knob));
-  r.full = tiles / r.workers;
-  r.rest = tiles % r.workers;
-  r.range = r.rest * r.steps / r.workers;
-  r.more = r.rest * r.steps % r.workers;
-  const double step = 0.28, write = 0.016 * std::min(block_rows, M), per_piece = (double)M * cols * 4 / tiles / 3e6, bytes = (double)K * cols * 2;
-  const double weights = bytes * (bytes > 60e6 ? turns : 1) / 7e6;
-  auto cost = [&](double steps, double pieces) { return std::max((r.full * r.steps + steps) * step, weights) + write + pieces * per_piece; };
-  if (!r.rest) {
-    *cost_us = cost(0, tiles);
-    return r;
-  }
-  const int fits = std::max(1, std::min(r.workers / r.rest, max_pieces)), most_split = std::max(1, r.steps / 4);
-  const bool even = r.range > 0 && (r.steps - 2) / r.range + 2 <= max_pieces;   // may the ranges be even?
-  const double even_cost = cost(1.1 * r.rest * r.steps / r.workers, tiles + r.workers) + std::max(0.0, write - r.range * step / 2);
-  auto split_cost = [&](int s) { return cost((r.steps + s - 1) / s, tiles + (double)r.rest * (s - 1)); };
-  if (block_rows <= 64) {
-    // few rows: results are small, and what counts is that no SM idles
-    if (fits >= most_split) r.split = most_split;
-    else if (!even || 6 * fits * r.rest >= 5 * r.workers) r.split = fits;
-  } else {
-    r.split = 1;
-    for (int s = 2; s <= std::min(fits, most_split); s++)
-      if (split_cost(s) < split_cost(r.split)) r.split = s;
-    if (even && even_cost < split_cost(r.split)) r.split = 0;
-  }
-  *cost_us = r.split ? split_cost(r.split) : even_cost;
-  return r;
-}
+}  // namespace
 
-// part[piece][M][n_total] = A[M][K] x [W_0 | W_1 | ...]; returns the ranges, which say how many pieces every tile has.
 int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const WeightRef* ws, int nw, float* part, size_t part_cap_bytes,
-                           GemmRanges* ranges, TimeStamp time = TimeStamp{nullptr, nullptr}) {
+                           GemmRanges* ranges, TimeStamp time) {
   GemmMaps maps;
   GemmParams g;
   memset(&g, 0, sizeof(g));
@@ -514,7 +398,7 @@ int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const 
   for (int rows = nt; rows >= std::min(nt, 128); rows /= 2)
     for (int beside = std::min(16, (M + rows - 1) / rows); beside >= 1; beside--) {
       double cost = 0;
-      const GemmRanges r = deal_tiles(p->dev->sm_count, tiles, M, rows, beside, K, cols, max_pieces, p->tune.get(RELUX_TUNE_GEMM_SPLIT), &cost);
+      const GemmRanges r = deal_tiles(p->dev->sm_count, tiles, M, rows, beside, steps, cols, (double)K * cols * 2, max_pieces, p->tune.get(RELUX_TUNE_GEMM_SPLIT), &cost);
       if (!g.rg.workers || cost < best) {
         g.rg = r;
         best = cost;
@@ -549,6 +433,8 @@ bool gemm_sm100_eligible(int K, const WeightRef* ws, int nw) {
     if (ws[j].n % 8 != 0 || ((uintptr_t)ws[j].w & 15) != 0) return false;
   return true;
 }
+
+namespace {
 
 int32_t launch_gemm_reference(Pool* p, const float* x, int M, int K, const WeightRef* ws, int nw, float* out, int out_stride) {
   int col = 0;
@@ -698,13 +584,10 @@ int32_t layer_batch(Pool* p, int layer, int n_seqs, const int32_t* seq_ids, int 
   return RELUX_OK;
 }
 
-struct LayerScratch {
-  uint16_t* a_bf16;
-  float* part;
-  size_t part_cap;
-  char* rest;
-};
-// [activations as bf16 (M x max_k) | split partials | caller's buffers (rest_bytes)]
+inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+}  // namespace
+
 int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, LayerScratch* out) {
   const size_t part_cap = std::max<size_t>((size_t)64 << 20, (size_t)M * max_n * 4 * 4);
   const size_t off_part = ((size_t)M * max_k * 2 + 255) & ~(size_t)255;
@@ -718,9 +601,6 @@ int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, L
   out->rest = base + off_rest;
   return RELUX_OK;
 }
-inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
-
-}  // namespace
 
 int32_t do_mla_layer(Pool* p, const relux_mla_layer_args* a) {
   if (!a || !a->w) { set_error("nil argument struct"); return RELUX_ERR_INVALID_ARG; }

@@ -1,0 +1,343 @@
+// Rows between two projections: the root-mean-square norm with the residual's addition (RMSNorm.Forward, rmsnorm.go:69-97, and the
+// additions of Block.Forward, transformer_block.go:119-142), and rows in 8 bits for relux_matmul_int8.
+//
+//   h = x + residual,  y = h * (1 / sqrt(mean(h^2) + eps)) * weight
+//   8 bits: a = max |y|,  scale = a / 127,  code = y * (127 / a) to the nearest whole number, even on a tie: the rule of the 8-bit cache
+//
+// Everything is float32 from the inputs to the one rounding of each result (h is normalised before it is rounded for residual_out); sums of
+// squares are taken by thread, then by tree.  Bound: HBM, x and the residual read once, the results written once; up to some hundred KB the
+// latency of one load, two reductions and a store.
+#include "common.cuh"
+#include "internal.h"
+
+namespace relux {
+
+namespace {
+
+constexpr int kMaxRowThreads = 1024, kMaxNV = 4;
+constexpr int kMaxNormDim = 8 * kMaxRowThreads * kMaxNV;
+constexpr float kTiny = 1e-36f;   // rows without a value this large have no finite 127 / a: zeros
+
+struct NormParams {
+  const void* x;
+  const void* residual;      // nullptr: h = x
+  const void* weight;        // nullptr: ones
+  void* residual_out;        // type of the residual
+  void* out;
+  int8_t* codes;
+  float* scales;
+  int32_t n_rows, d;
+  int32_t weight_bf16, out_bf16, by_tma;   // by_tma: the next launch reads codes or out by TMA
+  float eps, inv_d;
+};
+
+__device__ __forceinline__ float top_of(float a, float b) {   // a NaN stays one
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+struct alignas(16) Raw8 {   // eight values as they lie in memory
+  uint4 lo, hi;             // hi: float32 only
+};
+template <bool kBf16>
+__device__ __forceinline__ Raw8 load_raw(const void* p, size_t at) {
+  Raw8 r;
+  if constexpr (kBf16) {
+    r.lo = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at));
+  } else {
+    r.lo = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at));
+    r.hi = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at) + 1);
+  }
+  return r;
+}
+template <bool kBf16>
+__device__ __forceinline__ void widen(const Raw8& r, float (&v)[8]) {
+  if constexpr (kBf16) {
+    v[0] = bf16_lo(r.lo.x); v[1] = bf16_hi(r.lo.x); v[2] = bf16_lo(r.lo.y); v[3] = bf16_hi(r.lo.y);
+    v[4] = bf16_lo(r.lo.z); v[5] = bf16_hi(r.lo.z); v[6] = bf16_lo(r.lo.w); v[7] = bf16_hi(r.lo.w);
+  } else {
+    v[0] = __uint_as_float(r.lo.x); v[1] = __uint_as_float(r.lo.y); v[2] = __uint_as_float(r.lo.z); v[3] = __uint_as_float(r.lo.w);
+    v[4] = __uint_as_float(r.hi.x); v[5] = __uint_as_float(r.hi.y); v[6] = __uint_as_float(r.hi.z); v[7] = __uint_as_float(r.hi.w);
+  }
+}
+__device__ __forceinline__ void store8(void* p, size_t at, const float (&v)[8], bool bf16) {
+  if (bf16) {
+    reinterpret_cast<uint4*>(p)[at >> 3] = make_uint4(round_bf16x2(v[0], v[1]), round_bf16x2(v[2], v[3]), round_bf16x2(v[4], v[5]), round_bf16x2(v[6], v[7]));
+  } else {
+    float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at);
+    q[0] = make_float4(v[0], v[1], v[2], v[3]);
+    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// One row a team: `lanes` lanes of a warp (kWarp: a power of two, blockDim.x), or a whole block.  A thread holds kNV times eight values of the row, chunk
+// threadIdx.x + i * blockDim.x.  kNorm = false: only the 8-bit form of x.
+template <bool kXBf16, bool kRBf16, int kNV, bool kWarp, bool kNorm>
+__global__ void __launch_bounds__(kWarp ? 256 : kMaxRowThreads) norm_rows_kernel(const NormParams p) {
+  __shared__ float sums[32], tops[32];
+  // waits before it releases: a launch behind this one may rely on everything older (launch_chained, head of a chain)
+  chain_wait();
+  chain_release();
+  const int row = kWarp ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
+  const bool there = !kWarp || row < p.n_rows;
+  const int chunks = p.d >> 3, lanes = blockDim.x;
+  const size_t base = (size_t)(there ? row : 0) * p.d;
+  const bool adds = kNorm && p.residual;
+
+  Raw8 rx[kNV], rr[kNV];
+#pragma unroll
+  for (int i = 0; i < kNV; i++) {
+    const int c = threadIdx.x + i * lanes;
+    if (there && c < chunks) rx[i] = load_raw<kXBf16>(p.x, base + 8 * c);
+  }
+  if (adds)
+#pragma unroll
+    for (int i = 0; i < kNV; i++) {
+      const int c = threadIdx.x + i * lanes;
+      if (there && c < chunks) rr[i] = load_raw<kRBf16>(p.residual, base + 8 * c);
+    }
+
+  float v[kNV][8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kNV; i++) {
+    const int c = threadIdx.x + i * lanes;
+    const bool mine = there && c < chunks;
+    widen<kXBf16>(rx[i], v[i]);
+    if (adds) {
+      float r[8];
+      widen<kRBf16>(rr[i], r);
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[i][k] += r[k];
+      if (mine && p.residual_out) store8(p.residual_out, base + 8 * c, v[i], kRBf16);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      if (!mine) v[i][k] = 0.f;
+      if constexpr (kNorm) sum = fmaf(v[i][k], v[i][k], sum);
+    }
+  }
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (kNorm) {
+    for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if constexpr (!kWarp) {
+      if (lane == 0) sums[warp] = sum;
+      __syncthreads();
+      sum = warp_sum(lane < warps ? sums[lane] : 0.f);
+    }
+    const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+#pragma unroll
+    for (int i = 0; i < kNV; i++) {
+      const int c = threadIdx.x + i * lanes;
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[i][k] *= r;
+      if (p.weight && c < chunks) {
+        float w[8];
+        if (p.weight_bf16) widen<true>(load_raw<true>(p.weight, 8 * c), w);
+        else widen<false>(load_raw<false>(p.weight, 8 * c), w);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[i][k] *= w[k];
+      }
+      if (there && c < chunks && p.out) store8(p.out, base + 8 * c, v[i], p.out_bf16);
+    }
+  }
+  if (p.codes) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kNV; i++) {
+      const bool mine = there && threadIdx.x + i * lanes < chunks;
+#pragma unroll
+      for (int k = 0; k < 8; k++) top = top_of(top, mine ? fabsf(v[i][k]) : 0.f);
+    }
+    for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if constexpr (!kWarp) {
+      if (lane == 0) tops[warp] = top;
+      __syncthreads();
+      top = lane < warps ? tops[lane] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    // an infinity or a NaN: the scale is NaN and the codes are zeros, so that the row, and nothing else, comes out as NaN
+    const bool finite = __float_as_uint(top) < 0x7F800000u, some = finite && top >= kTiny;
+    const float up = some ? __fdiv_rn(127.f, top) : 0.f;
+    if (there && threadIdx.x == 0) p.scales[row] = some ? __fdiv_rn(top, 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
+#pragma unroll
+    for (int i = 0; i < kNV; i++) {
+      const int c = threadIdx.x + i * lanes;
+      uint32_t q[8], w[2];
+#pragma unroll
+      for (int k = 0; k < 8; k++) q[k] = some ? (uint32_t)__float2int_rn(__fmul_rn(v[i][k], up)) : 0u;
+#pragma unroll
+      for (int k = 0; k < 2; k++) w[k] = __byte_perm(__byte_perm(q[4 * k], q[4 * k + 1], 0x0040), __byte_perm(q[4 * k + 2], q[4 * k + 3], 0x0040), 0x5410);
+      if (there && c < chunks) *reinterpret_cast<uint2*>(p.codes + base + 8 * c) = make_uint2(w[0], w[1]);
+    }
+  }
+  if (p.by_tma) fence_chained_writes();
+}
+
+template <bool kXBf16, bool kRBf16, int kNV, bool kWarp, bool kNorm>
+int32_t launch_one(Pool* p, const NormParams& prm, dim3 grid, dim3 block) {
+  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, norm_rows_kernel<kXBf16, kRBf16, kNV, kWarp, kNorm>, grid, block, 0,
+                                p->dev->stream, prm));
+  count_launch(p->dev);
+  return RELUX_OK;
+}
+template <bool kXBf16, bool kRBf16, bool kNorm>
+int32_t launch_typed(Pool* p, const NormParams& prm) {
+  const int chunks = prm.d / 8;
+  if (chunks <= 32) {
+    int lanes = 1;
+    while (lanes < chunks) lanes *= 2;
+    const dim3 block(lanes, 256 / lanes);
+    return launch_one<kXBf16, kRBf16, 1, true, kNorm>(p, prm, dim3((unsigned)((prm.n_rows + (int)block.y - 1) / (int)block.y)), block);
+  }
+  // a row a block: as few chunks a thread as the block's limit lets
+  const int nv = chunks <= kMaxRowThreads ? 1 : chunks <= 2 * kMaxRowThreads ? 2 : 4;
+  const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+  const dim3 grid((unsigned)prm.n_rows), block((unsigned)threads);
+  return nv == 1 ? launch_one<kXBf16, kRBf16, 1, false, kNorm>(p, prm, grid, block)
+       : nv == 2 ? launch_one<kXBf16, kRBf16, 2, false, kNorm>(p, prm, grid, block)
+                 : launch_one<kXBf16, kRBf16, 4, false, kNorm>(p, prm, grid, block);
+}
+
+// w [k][n] -> codes [n][k] and a scale per column.  One block per 64 columns: their largest magnitudes, then the codes through shared memory, so
+// that reads and writes are coalesced.  Once per model.
+constexpr int kImpCols = 64, kImpRows = 64;
+template <bool kBf16>
+__global__ void __launch_bounds__(256) int8_weights_kernel(const void* w, int k, int n, int8_t* codes, float* scales) {
+  __shared__ float top[4][kImpCols], ups[kImpCols];
+  __shared__ int8_t tile[kImpRows][kImpCols + 4];
+  const int col = threadIdx.x & (kImpCols - 1), part = threadIdx.x / kImpCols, n0 = blockIdx.x * kImpCols;
+  const bool mine = n0 + col < n;
+  auto value = [&](int r) -> float {
+    const size_t at = (size_t)r * n + n0 + col;
+    return kBf16 ? f32_from_bf16_bits(reinterpret_cast<const uint16_t*>(w)[at]) : reinterpret_cast<const float*>(w)[at];
+  };
+  float t = 0.f;
+  if (mine)
+#pragma unroll 8
+    for (int r = part; r < k; r += 4) t = top_of(t, fabsf(value(r)));
+  top[part][col] = t;
+  __syncthreads();
+  if (part == 0) {
+    t = top_of(top_of(top[0][col], top[1][col]), top_of(top[2][col], top[3][col]));
+    const bool finite = __float_as_uint(t) < 0x7F800000u, some = finite && t >= kTiny;
+    ups[col] = some ? __fdiv_rn(127.f, t) : 0.f;
+    if (mine) scales[n0 + col] = some ? __fdiv_rn(t, 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
+  }
+  __syncthreads();
+  const float up = ups[col];
+  for (int r0 = 0; r0 < k; r0 += kImpRows) {
+#pragma unroll 4
+    for (int r = part; r < kImpRows; r += 4) tile[r][col] = mine && up != 0.f && r0 + r < k ? (int8_t)__float2int_rn(__fmul_rn(value(r0 + r), up)) : (int8_t)0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kImpCols * (kImpRows / 4); i += 256) {
+      const int c = i / (kImpRows / 4), r = i % (kImpRows / 4) * 4;   // four codes of one column; k is a multiple of 16
+      if (n0 + c < n && r0 + r < k) {
+        const uint32_t v = (uint8_t)tile[r][c] | (uint32_t)(uint8_t)tile[r + 1][c] << 8 | (uint32_t)(uint8_t)tile[r + 2][c] << 16 | (uint32_t)(uint8_t)tile[r + 3][c] << 24;
+        *reinterpret_cast<uint32_t*>(codes + (size_t)(n0 + c) * k + r0 + r) = v;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+bool dtype_ok(int32_t t) { return t == RELUX_DTYPE_F32 || t == RELUX_DTYPE_BF16; }
+
+template <bool kNorm>
+int32_t launch_rows(Pool* p, const NormParams& prm, bool x_bf16, bool r_bf16) {
+  if constexpr (kNorm)
+    return x_bf16 ? (r_bf16 ? launch_typed<true, true, true>(p, prm) : launch_typed<true, false, true>(p, prm))
+                  : (r_bf16 ? launch_typed<false, true, true>(p, prm) : launch_typed<false, false, true>(p, prm));
+  else
+    return x_bf16 ? launch_typed<true, true, false>(p, prm) : launch_typed<false, false, false>(p, prm);
+}
+
+int32_t check_codes(const int8_t* codes, const float* scales, int d) {
+  if (!codes || !scales) { set_error("8-bit rows need codes and scales"); return RELUX_ERR_INVALID_ARG; }
+  if (d % 16 != 0) { set_error("8-bit rows of %d numbers: must be a multiple of 16", d); return RELUX_ERR_UNSUPPORTED; }
+  int32_t rc = check_dev_align(codes, "codes");
+  return rc ? rc : check_dev_align(scales, "scales");
+}
+
+}  // namespace
+
+// Checks of a norm's arguments, before anything is launched.
+int32_t check_rmsnorm(const relux_rmsnorm_args* a) {
+  if (!a || !a->x) { set_error("nil argument"); return RELUX_ERR_INVALID_ARG; }
+  if (a->n_rows <= 0 || a->d <= 0) { set_error("RMSNorm: rows=%d d=%d must be positive", a->n_rows, a->d); return RELUX_ERR_INVALID_ARG; }
+  if (a->d % 8 != 0 || a->d > kMaxNormDim) {
+    set_error("RMSNorm: d=%d must be a multiple of 8, up to %d", a->d, kMaxNormDim);
+    return RELUX_ERR_UNSUPPORTED;
+  }
+  if (!dtype_ok(a->x_dtype) || !dtype_ok(a->residual_dtype) || !dtype_ok(a->weight_dtype) || !dtype_ok(a->out_dtype)) { set_error("bad dtype flag"); return RELUX_ERR_INVALID_ARG; }
+  if (!(a->eps >= 0.f)) { set_error("RMSNorm: eps=%g must not be negative", (double)a->eps); return RELUX_ERR_INVALID_ARG; }
+  for (int i = 0; i < 5; i++)
+    if (a->reserved[i]) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  if (a->residual_out && !a->residual) { set_error("RMSNorm: residual_out without a residual"); return RELUX_ERR_INVALID_ARG; }
+  if (!a->out && !a->codes) { set_error("RMSNorm: no output given"); return RELUX_ERR_INVALID_ARG; }
+  int32_t rc;
+  if (a->codes || a->scales)
+    if ((rc = check_codes(a->codes, a->scales, a->d))) return rc;
+  if ((rc = check_dev_align(a->x, "x")) || (rc = check_dev_align(a->residual, "residual")) || (rc = check_dev_align(a->residual_out, "residual_out")) ||
+      (rc = check_dev_align(a->weight, "weight")) || (rc = check_dev_align(a->out, "out")))
+    return rc;
+  return RELUX_OK;
+}
+
+int32_t do_rmsnorm(Pool* p, const relux_rmsnorm_args* a) {
+  if (int32_t rc = check_rmsnorm(a)) return rc;
+  NormParams prm{};
+  prm.x = a->x;
+  prm.residual = a->residual;
+  prm.weight = a->weight;
+  prm.residual_out = a->residual_out;
+  prm.out = a->out;
+  prm.codes = a->codes;
+  prm.scales = a->scales;
+  prm.n_rows = a->n_rows;
+  prm.d = a->d;
+  prm.weight_bf16 = a->weight_dtype == RELUX_DTYPE_BF16;
+  prm.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
+  prm.by_tma = 1;   // codes, and bf16 rows, are a projection's operands
+  prm.eps = a->eps;
+  prm.inv_d = 1.f / (float)a->d;
+  return launch_rows<true>(p, prm, a->x_dtype == RELUX_DTYPE_BF16, a->residual_dtype == RELUX_DTYPE_BF16);
+}
+
+int32_t do_int8_rows(Pool* p, const relux_int8_rows_args* a) {
+  if (!a || !a->x) { set_error("nil argument"); return RELUX_ERR_INVALID_ARG; }
+  if (a->n_rows <= 0 || a->d <= 0) { set_error("int8_rows: rows=%d d=%d must be positive", a->n_rows, a->d); return RELUX_ERR_INVALID_ARG; }
+  if (!dtype_ok(a->x_dtype)) { set_error("bad dtype flag"); return RELUX_ERR_INVALID_ARG; }
+  if (a->reserved) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  int32_t rc = check_codes(a->codes, a->scales, a->d);
+  if (rc || (rc = check_dev_align(a->x, "x"))) return rc;
+  if (a->d > kMaxNormDim) { set_error("int8_rows: d=%d above %d", a->d, kMaxNormDim); return RELUX_ERR_UNSUPPORTED; }
+  NormParams prm{};
+  prm.x = a->x;
+  prm.codes = a->codes;
+  prm.scales = a->scales;
+  prm.n_rows = a->n_rows;
+  prm.d = a->d;
+  prm.by_tma = 1;
+  const bool bf16 = a->x_dtype == RELUX_DTYPE_BF16;
+  return launch_rows<false>(p, prm, bf16, bf16);
+}
+
+int32_t do_int8_weights(Pool* p, const relux_int8_weights_args* a) {
+  if (!a || !a->w) { set_error("nil argument"); return RELUX_ERR_INVALID_ARG; }
+  if (a->k <= 0 || a->n <= 0) { set_error("int8_weights: K=%d N=%d must be positive", a->k, a->n); return RELUX_ERR_INVALID_ARG; }
+  if (!dtype_ok(a->w_dtype)) { set_error("bad dtype flag"); return RELUX_ERR_INVALID_ARG; }
+  if (a->reserved) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  int32_t rc = check_codes(a->codes, a->scales, a->k);
+  if (rc || (rc = check_dev_align(a->w, "w"))) return rc;
+  if (a->n % 8 != 0) { set_error("int8_weights: N=%d must be a multiple of 8", a->n); return RELUX_ERR_UNSUPPORTED; }
+  const dim3 grid((unsigned)((a->n + kImpCols - 1) / kImpCols));
+  if (a->w_dtype == RELUX_DTYPE_BF16) int8_weights_kernel<true><<<grid, 256, 0, p->dev->stream>>>(a->w, a->k, a->n, a->codes, a->scales);
+  else int8_weights_kernel<false><<<grid, 256, 0, p->dev->stream>>>(a->w, a->k, a->n, a->codes, a->scales);
+  RELUX_CUDA_TRY(cudaGetLastError());
+  count_launch(p->dev);
+  return RELUX_OK;
+}
+
+}  // namespace relux

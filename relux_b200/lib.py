@@ -39,7 +39,8 @@ EXPORTS = [
     "relux_mla_verify", "relux_pool_last_kernel_ms", "relux_pool_kernel_ms_mean", "relux_mla_forward_cached", "relux_gqa_forward_cached", "relux_stream_partition", "relux_seq_save_file", "relux_seq_load_file", "relux_pool_projection_ms_mean", "relux_gqa_decode_noalloc",
     "relux_spec_accept", "relux_sampler_sample", "relux_pool_tune", "relux_pool_kernel_ms_list", "relux_matmul_f32_bf16",
     "relux_mla_import_weights", "relux_pool_selftest_wait", "relux_pool_wait_output", "relux_mla_step", "relux_gqa_step", "relux_mla_expand_kv",
-    "relux_gqa_read_kv", "relux_gqa_tree_verify", "relux_gqa_tree_commit",
+    "relux_gqa_read_kv", "relux_gqa_tree_verify", "relux_gqa_tree_commit", "relux_rmsnorm", "relux_int8_rows", "relux_int8_weights",
+    "relux_matmul_int8",
 ]
 
 
@@ -92,6 +93,28 @@ class TreeArgs(C.Structure):
 class TreeCommitArgs(C.Structure):
     _fields_ = [("layer", C.c_int32), ("n_seqs", C.c_int32), ("seq_ids", C.c_void_p), ("path", C.c_void_p), ("path_len", C.c_void_p),
                 ("path_stride", C.c_int32), ("reserved", C.c_int32 * 3)]
+
+
+class RmsnormArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int32), ("d", C.c_int32), ("eps", C.c_float), ("x_dtype", C.c_int32), ("residual_dtype", C.c_int32),
+                ("weight_dtype", C.c_int32), ("out_dtype", C.c_int32), ("reserved", C.c_int32 * 5), ("x", C.c_void_p),
+                ("residual", C.c_void_p), ("weight", C.c_void_p), ("residual_out", C.c_void_p), ("out", C.c_void_p), ("codes", C.c_void_p),
+                ("scales", C.c_void_p)]
+
+
+class Int8RowsArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int32), ("d", C.c_int32), ("x_dtype", C.c_int32), ("reserved", C.c_int32), ("x", C.c_void_p), ("codes", C.c_void_p),
+                ("scales", C.c_void_p)]
+
+
+class Int8WeightsArgs(C.Structure):
+    _fields_ = [("k", C.c_int32), ("n", C.c_int32), ("w_dtype", C.c_int32), ("reserved", C.c_int32), ("w", C.c_void_p), ("codes", C.c_void_p),
+                ("scales", C.c_void_p)]
+
+
+class MatmulInt8Args(C.Structure):
+    _fields_ = [("m", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("out_dtype", C.c_int32), ("a", C.c_void_p), ("a_scales", C.c_void_p),
+                ("w", C.c_void_p), ("w_scales", C.c_void_p), ("out", C.c_void_p), ("reserved", C.c_int32 * 4)]
 
 
 class MlaLayerWeights(C.Structure):
@@ -169,6 +192,10 @@ pack_attn = _packer(AttnArgs)
 pack_read_kv = _packer(ReadKvArgs)
 pack_tree = _packer(TreeArgs)
 pack_tree_commit = _packer(TreeCommitArgs)
+pack_rmsnorm = _packer(RmsnormArgs)
+pack_int8_rows = _packer(Int8RowsArgs)
+pack_int8_weights = _packer(Int8WeightsArgs)
+pack_matmul_int8 = _packer(MatmulInt8Args)
 
 
 class ReluxCudaError(RuntimeError):
@@ -249,6 +276,10 @@ def load():
         L.relux_gqa_read_kv.argtypes = [C.c_void_p, C.POINTER(ReadKvArgs)]
         L.relux_gqa_tree_verify.argtypes = [C.c_void_p, C.POINTER(AttnArgs), C.POINTER(AppendArgs), C.POINTER(TreeArgs)]
         L.relux_gqa_tree_commit.argtypes = [C.c_void_p, C.POINTER(TreeCommitArgs)]
+        L.relux_rmsnorm.argtypes = [C.c_void_p, C.POINTER(RmsnormArgs)]
+        L.relux_int8_rows.argtypes = [C.c_void_p, C.POINTER(Int8RowsArgs)]
+        L.relux_int8_weights.argtypes = [C.c_void_p, C.POINTER(Int8WeightsArgs)]
+        L.relux_matmul_int8.argtypes = [C.c_void_p, C.POINTER(MatmulInt8Args)]
         L.relux_spec_accept.argtypes = [C.c_void_p, C.POINTER(SpecAcceptArgs)]
         L.relux_sampler_sample.argtypes = [C.c_void_p, C.POINTER(SampleArgs)]
         L.relux_pool_last_kernel_ms.argtypes = [C.c_void_p, C.POINTER(C.c_float)]
@@ -257,7 +288,8 @@ def load():
         L.relux_cuda_stream.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
         # the per-token calls once more, taking their argument structs as packed bytes (pack_append, pack_attn)
         for name, n_structs in (("mla_append", 1), ("gqa_append", 1), ("mla_decode", 1), ("gqa_decode", 1), ("mla_verify", 2), ("gqa_verify", 2),
-                                ("mla_step", 2), ("gqa_step", 2), ("gqa_tree_verify", 3), ("gqa_tree_commit", 1), ("gqa_read_kv", 1)):
+                                ("mla_step", 2), ("gqa_step", 2), ("gqa_tree_verify", 3), ("gqa_tree_commit", 1), ("gqa_read_kv", 1),
+                                ("rmsnorm", 1), ("int8_rows", 1), ("int8_weights", 1), ("matmul_int8", 1)):
             f = L["relux_" + name]   # a function object of its own
             f.restype, f.argtypes = C.c_int32, [C.c_void_p] + [C.c_char_p] * n_structs
             packed[name] = f

@@ -46,6 +46,7 @@ struct Device {
   std::mutex mu;
   int64_t launches = 0;
   std::vector<std::pair<const void*, size_t>> smem_allowed;   // what allow_smem knows of the kernels' limits, under mu
+  int int8_clusters[9] = {};   // clusters of so many CTAs of an 8-bit product (one CTA an SM) that are resident at once, 0: not asked yet
   void* flush_buf = nullptr;
   size_t flush_bytes = 0;
   // Page-locked memory for results of host calls, written by the kernel that makes them: the call waits for the stream and
@@ -183,9 +184,6 @@ struct Pool {
   CUtensorMap tmap_gqa{};   // 2-D [rows][D],      box 64 x 64, 128-byte swizzle
   bool has_tmap = false;
   bool mla_blocked = false;   // MLA pages stored as 64-column blocks (see mla_page_off)
-  GrowBuf int8_part;                  // 8-bit products: pieces of tiles
-  static constexpr int kArrived = 1024;
-  int32_t* int8_arrived = nullptr;    // and how many of a tile's have arrived, zero between launches
   // layer-level step (layer_step.cu): RoPE tables [cos | sin][positions][dHR / 2] and the step's scratch block
   GrowBuf rope_tab, layer_buf;
   int rope_dim = 0, rope_positions = 0;

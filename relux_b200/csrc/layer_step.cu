@@ -361,6 +361,50 @@ int32_t launch_skinny_gemm_rows(Pool* p, const GemmMaps& maps, const GemmParams&
   return RELUX_OK;
 }
 
+// Deals the tiles to one worker per SM, `beside` blocks of `block_rows` rows beside each other.  max_pieces: pieces of a tile that
+// the scratch holds.  *cost_us: what this takes beyond what every dealing takes, from measured parts (4 to 25600 rows against
+// weights of 1024 x 1024 to 16384 x 16384): a step takes an SM 0.28 us whatever the rows of its block, and a tenth more where the
+// workers don't walk in step; the weights come at 7 TB/s, again for every turn of blocks when they exceed L2; the last piece of
+// a worker is written at 16 ns per row with nothing to hide it; pieces are written and read at 3 TB/s.
+GemmRanges deal_tiles(int sms, int col_tiles, int M, int block_rows, int beside, int K, int cols, int max_pieces, int split_knob, double* cost_us) {
+  GemmRanges r{};
+  r.steps = (K + kTileK - 1) / kTileK;
+  r.col_tiles = col_tiles;
+  r.row_blocks = (M + block_rows - 1) / block_rows;
+  r.block_rows = block_rows;
+  r.beside = beside;
+  const int turns = (r.row_blocks + beside - 1) / beside, tiles = col_tiles * turns, units = tiles * r.steps;
+  r.workers = std::max(1, std::min(std::max(1, sms / beside), units / 4));   // pieces of fewer than four steps do not pay for their share of the result
+  if (split_knob) r.workers = std::max(1, (int)std::min<int64_t>(units, (int64_t)tiles * split_knob));
+  r.full = tiles / r.workers;
+  r.rest = tiles % r.workers;
+  r.range = r.rest * r.steps / r.workers;
+  r.more = r.rest * r.steps % r.workers;
+  const double step = 0.28, write = 0.016 * std::min(block_rows, M), per_piece = (double)M * cols * 4 / tiles / 3e6, bytes = (double)K * cols * 2;
+  const double weights = bytes * (bytes > 60e6 ? turns : 1) / 7e6;
+  auto cost = [&](double steps, double pieces) { return std::max((r.full * r.steps + steps) * step, weights) + write + pieces * per_piece; };
+  if (!r.rest) {
+    *cost_us = cost(0, tiles);
+    return r;
+  }
+  const int fits = std::max(1, std::min(r.workers / r.rest, max_pieces)), most_split = std::max(1, r.steps / 4);
+  const bool even = r.range > 0 && (r.steps - 2) / r.range + 2 <= max_pieces;   // may the ranges be even?
+  const double even_cost = cost(1.1 * r.rest * r.steps / r.workers, tiles + r.workers) + std::max(0.0, write - r.range * step / 2);
+  auto split_cost = [&](int s) { return cost((r.steps + s - 1) / s, tiles + (double)r.rest * (s - 1)); };
+  if (block_rows <= 64) {
+    // few rows: results are small, and what counts is that no SM idles
+    if (fits >= most_split) r.split = most_split;
+    else if (!even || 6 * fits * r.rest >= 5 * r.workers) r.split = fits;
+  } else {
+    r.split = 1;
+    for (int s = 2; s <= std::min(fits, most_split); s++)
+      if (split_cost(s) < split_cost(r.split)) r.split = s;
+    if (even && even_cost < split_cost(r.split)) r.split = 0;
+  }
+  *cost_us = r.split ? split_cost(r.split) : even_cost;
+  return r;
+}
+
 }  // namespace
 
 int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const WeightRef* ws, int nw, float* part, size_t part_cap_bytes,
@@ -398,7 +442,7 @@ int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const 
   for (int rows = nt; rows >= std::min(nt, 128); rows /= 2)
     for (int beside = std::min(16, (M + rows - 1) / rows); beside >= 1; beside--) {
       double cost = 0;
-      const GemmRanges r = deal_tiles(p->dev->sm_count, tiles, M, rows, beside, steps, cols, (double)K * cols * 2, max_pieces, p->tune.get(RELUX_TUNE_GEMM_SPLIT), &cost);
+      const GemmRanges r = deal_tiles(p->dev->sm_count, tiles, M, rows, beside, K, cols, max_pieces, p->tune.get(RELUX_TUNE_GEMM_SPLIT), &cost);
       if (!g.rg.workers || cost < best) {
         g.rg = r;
         best = cost;

@@ -305,7 +305,7 @@ static void pool_free_all(Pool* p) {
   for (cudaEvent_t e : p->pipe_calls.done)
     if (e) cudaEventDestroy(e);
   fr(p->storage); fr(p->scales); fr(p->meta);
-  fr_buf(p->in_a); fr_buf(p->in_b); fr_buf(p->out_buf); fr_buf(p->q_abs); fr_buf(p->part_o); fr_buf(p->part_ml); fr_buf(p->work); fr_buf(p->stream_done); fr_buf(p->seq_list); fr_buf(p->int8_part);
+  fr_buf(p->in_a); fr_buf(p->in_b); fr_buf(p->out_buf); fr_buf(p->q_abs); fr_buf(p->part_o); fr_buf(p->part_ml); fr_buf(p->work); fr_buf(p->stream_done); fr_buf(p->seq_list);
   fr_buf(p->o_lat); fr_buf(p->q_conv); fr_buf(p->rope_tab); fr_buf(p->layer_buf); fr(p->shadow_f32); fr_buf(p->chunk_tab); fr_buf(p->step_rows); fr_buf(p->expand_buf);
   if (p->h_stage) cudaFreeHost(p->h_stage);
   for (void* block : p->stage_held) cudaFreeHost(block);
@@ -1012,17 +1012,16 @@ API int32_t relux_pool_create(relux_device_t h, const relux_pool_params* prm, re
   auto A = [&](void** q, size_t bytes) { if (e == cudaSuccess) e = cudaMalloc(q, bytes); };
   A((void**)&p->storage, storage_bytes);
   if (int8) A((void**)&p->scales, scale_bytes);
-  // the small arrays in one block: [table | lengths, status (word, block counter of the append kernels), time slots, arrivals of 8-bit products |
+  // the small arrays in one block: [table | lengths, status (word, block counter of the append kernels), time slots |
   // sequence ids | row offsets]; the middle part starts as zeros
   auto pad = [](size_t b) { return (b + 255) & ~(size_t)255; };
   const size_t off_len = pad(table_n * 4), off_status = off_len + pad(len_n * 4), off_slots = off_status + 256,
-               off_arrived = off_slots + pad(sizeof(TimeSlot) * TimeRing::kSlots), off_ids = off_arrived + Pool::kArrived * 4, off_row = off_ids + pad((size_t)prm->max_seqs * 4);
+               off_ids = off_slots + pad(sizeof(TimeSlot) * TimeRing::kSlots), off_row = off_ids + pad((size_t)prm->max_seqs * 4);
   A(&p->meta, off_row + pad(((size_t)prm->max_seqs + 1) * 4));
   p->d_table = (int32_t*)p->meta;
   p->d_len = (int32_t*)((char*)p->meta + off_len);
   p->d_status = (int32_t*)((char*)p->meta + off_status);
   p->attn_times.slots = (TimeSlot*)((char*)p->meta + off_slots);
-  p->int8_arrived = (int32_t*)((char*)p->meta + off_arrived);
   p->d_seq_ids = (int32_t*)((char*)p->meta + off_ids);
   p->d_row_off = (int32_t*)((char*)p->meta + off_row);
   p->compat = (prm->flags & RELUX_POOL_FLAG_REFERENCE_COMPAT) != 0;

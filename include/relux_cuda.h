@@ -698,6 +698,32 @@ typedef struct relux_matmul_int8_args {
 } relux_matmul_int8_args;
 int32_t relux_matmul_int8(relux_pool_t pool, const relux_matmul_int8_args* args);
 
+/* C [m][n] = x [m][k] w + the low-rank adapter of each row's request: f_s (x A_s^T) B_s^T, s the request's slot.  relux_matmul_f32_bf16 for a batch
+ * whose requests have adapters of their own, in as many launches; rows of requests without one (-1) are the shared projection alone.
+ * x is rounded to bf16 as in relux_matmul_f32_bf16's FAST mode (bf16 x is taken as it is); x A_s^T is summed in float32 and keeps 16 bits; sums are float32
+ * up to the one rounding of the result.  A request's rows depend on its own adapter alone, whatever other slots hold.
+ * w NULL: no shared projection (it came from relux_matmul_int8, say: with accumulate the adapters are added to what out holds).
+ * Requests own neighbouring rows, n_rows[i] of them in order; several may name the same slot.  The host arrays are read before the call returns; a captured
+ * call keeps its adapters' places in the batch, the slots' contents are read at every launch.
+ * Shapes: k and n multiples of 8, rank 8, 16, 32, 64 or 128 (a smaller adapter is filled up with zeros).  Adapters as checkpoints hold them (lora_A [rank][in],
+ * lora_B [out][rank]).  out must not overlap x.  Asynchronous on the handle's stream.  No counterpart in the reference, which serves one model. */
+typedef struct relux_matmul_lora_args {
+  int32_t m, k, n;
+  int32_t rank, n_slots, n_seqs;
+  int32_t x_dtype, out_dtype;
+  int32_t accumulate;
+  int32_t reserved[3];
+  const void* x;             /* device [m][k] */
+  const void* w;             /* device bf16 [k][n], or NULL */
+  const void* lora_a;        /* device bf16 [n_slots][rank][k] */
+  const void* lora_b;        /* device bf16 [n_slots][n][rank] */
+  const float* factors;      /* device [n_slots], or NULL: ones */
+  const int32_t* adapter;    /* host [n_seqs]: slot, or -1 */
+  const int32_t* n_rows;     /* host [n_seqs]; NULL = 1 each */
+  void* out;                 /* device [m][n] */
+} relux_matmul_lora_args;
+int32_t relux_matmul_lora(relux_pool_t pool, const relux_matmul_lora_args* args);
+
 /* ---- expansion of the cached MLA latents --------------------------------------------------------
  * What MLA.forwardCached does before it scores a multi-token call: every cached latent row times W_UK and W_UV
  * (internal/transformer/mla.go:323-326), here as one tensor-core GEMM with bf16 results.  The library's own prompt path

@@ -326,6 +326,22 @@ class Pool:
                               w_scales=w_scales, out=out)
         L.check(L.packed["matmul_int8"](self.h, L.pack_matmul_int8(m, k, n, t, b["a"], b["a_scales"], b["w"], b["w_scales"], b["out"])))
 
+    def matmul_lora(self, m, k, n, x, w, out, lora_a, lora_b, rank, n_slots, adapter, rows=None, factors=None, accumulate=False, x_dtype=None,
+                    out_dtype=None):
+        """out [m, n] = x [m, k] w + each request's low-rank adapter (relux_matmul_lora): adapter [requests], slots or -1; rows [requests], None: one
+        each; lora_a [n_slots, rank, k], lora_b [n_slots, n, rank], factors float32 [n_slots] or None.  w None: no shared projection; accumulate: added to
+        what out holds."""
+        ids = np.ascontiguousarray(adapter, dtype=np.int32)
+        nr = None if rows is None else np.ascontiguousarray(rows, dtype=np.int32)
+        if ids.ndim != 1 or (nr is not None and nr.shape != ids.shape):
+            raise ValueError("matmul_lora: adapters of shape %s, rows of shape %s" % (ids.shape, None if nr is None else nr.shape))
+        xt, ot = _dtype_flag(x, x_dtype), _dtype_flag(out, out_dtype)
+        a = self._device_only("matmul_lora", dict(x=m * k * _size(xt), w=2 * k * n, out=m * n * _size(ot), lora_a=2 * n_slots * rank * k,
+                                                  lora_b=2 * n_slots * rank * n, factors=4 * n_slots),
+                              x=x, w=w, out=out, lora_a=lora_a, lora_b=lora_b, factors=factors)
+        L.check(L.packed["matmul_lora"](self.h, L.pack_matmul_lora(m, k, n, rank, n_slots, ids.size, xt, ot, int(bool(accumulate)), a["x"], a["w"], a["lora_a"],
+                                                                   a["lora_b"], a["factors"], _ptr(ids) or 0, _ptr(nr) or 0, a["out"])))
+
     def import_mla_weights(self, d_model, num_heads, nope_dim, rope_dim, v_dim, dc, dst, q_proj=None, kv_a_proj_with_mqa=None,
                            kv_b_proj=None, o_proj=None, q_pe_proj=None, k_pe_proj=None, fused_rope=False):
         """Splits and transposes one layer's DeepSeek-style checkpoint tensors (numpy float32 or uint16 bf16 bits, all of

@@ -1,0 +1,481 @@
+// A shared projection with low-rank adapters of many requests beside it: C[m] = x[m] W + f_s (x[m] A_s^T) B_s^T, s the adapter of the
+// request that row m belongs to, or none.  A_s [rank][K], B_s [N][rank] in slots of two arrays, as checkpoints hold them (lora_A, lora_B).
+//
+// Three launches, as many as the projection alone: lora_down_kernel rounds x to bf16 for the projection and takes t = x A_s^T while it holds the
+// rows; the projection's GEMM (skinny_gemm_sm100_kernel); lora_up_kernel adds up the GEMM's pieces and, on the way out, t B_s^T.
+// The adapters stay out of the GEMM's tiles on purpose: a tile holds rows of many requests, and a product with another request's B, even by
+// zeros, would carry its infinities and NaN into this one's rows.
+// Rows are taken in groups of one adapter, wherever in the batch they lie: the host sorts the requests by adapter, so that an adapter is read
+// once for 16 (long calls 32 or 64) rows of it.  Bound: HBM, W and the adapters in use once, for few rows; for prompts the GEMM.
+#include <algorithm>
+#include <vector>
+
+#include "common.cuh"
+#include "internal.h"
+#include "projection.cuh"
+
+namespace relux {
+
+namespace {
+
+constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
+constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
+constexpr int kMaxKSplit = 8;
+constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
+
+// The rows of a call (or of a part of it), in the order of their adapters.  A piece is a range of neighbouring rows of one adapter; a run is
+// all the pieces of one.  Groups are cut within runs.
+template <int kCap>
+struct LoraList {
+  int32_t n_pieces, n_runs;
+  int32_t at[kCap + 1];      // first place, in this order, of a piece
+  int32_t row[kCap];         // its first row
+  int32_t slot[kCap];        // of a run: adapter, or -1
+  int32_t run_at[kCap + 1];  // first place of a run
+  int32_t group[kCap + 1];   // first group of a run
+};
+// The last of n ascending entries that is no more than v.
+__device__ __forceinline__ int last_up_to(const int32_t* a, int n, int v) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a[mid] <= v) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+// Rows of a group to shared memory (-1: none), and its adapter.  By all threads; a barrier follows.
+template <int kGroupRows, class List>
+__device__ __forceinline__ int group_rows(const List& list, int group, int32_t* rows) {
+  const int run = last_up_to(list.group, list.n_runs, group);
+  const int first = list.run_at[run] + (group - list.group[run]) * kGroupRows, end = list.run_at[run + 1];
+  if (threadIdx.x < kGroupRows) {
+    const int v = first + threadIdx.x;
+    int r = -1;
+    if (v < end) {
+      const int piece = last_up_to(list.at, list.n_pieces, v);
+      r = list.row[piece] + v - list.at[piece];
+    }
+    rows[threadIdx.x] = r;
+  }
+  return list.slot[run];
+}
+
+struct DownParams {
+  const void* x;
+  uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr
+  const uint16_t* a;      // [slots][rank][K]
+  float* t;               // [split][M][rank]
+  int32_t M, K;
+};
+
+// t[row][r] = sum over this block's part of K of x[row][k] A_s[r][k].  grid (groups, parts of K), 8 warps that take 32 k each in turn.  mma.sync: a group is a handful of
+// rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
+template <int kRank, int kMT, bool kXBf16, class List>
+__global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
+  constexpr int kTiles = kRank / 8;
+  extern __shared__ __align__(16) float slabs[];   // [warp][16 kMT][kRank]
+  __shared__ int32_t rows[16 * kMT];
+  // waits before it releases: the projection behind it may read its weights early (launch_chained, head of a chain)
+  chain_wait();
+  chain_release();
+  const int slot = group_rows<16 * kMT>(list, blockIdx.x, rows);
+  if (slot < 0 && !p.x_bf16) return;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
+  int32_t r[kMT][2];
+#pragma unroll
+  for (int m = 0; m < kMT; m++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) r[m][h] = rows[16 * m + 8 * h + g];
+  float acc[kMT][kTiles][4];
+#pragma unroll
+  for (int m = 0; m < kMT; m++)
+#pragma unroll
+    for (int j = 0; j < kTiles; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[m][j][i] = 0.f;
+  const uint16_t* const a = p.a + (size_t)max(slot, 0) * kRank * p.K;
+  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+
+#pragma unroll(kMT == 1 && kRank <= 32 ? 4 : kMT == 1 || kRank <= 16 ? 2 : 1)
+  for (int s = s0 + warp; s < s1; s += kLoraWarps) {
+    const int k = s * 32 + 8 * t;
+    const bool in = k < p.K;   // K is a multiple of 8
+    uint4 x[kMT][2], w[kTiles];
+    if (slot >= 0)
+#pragma unroll
+      for (int j = 0; j < kTiles; j++) w[j] = in ? load_chained(reinterpret_cast<const uint4*>(a + (size_t)(8 * j + g) * p.K + k)) : none;
+#pragma unroll
+    for (int m = 0; m < kMT; m++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const size_t at = (size_t)max(r[m][h], 0) * p.K + k;
+        const bool there = in && r[m][h] >= 0;
+        if constexpr (kXBf16) {
+          x[m][h] = there ? load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at)) : none;
+        } else {
+          const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
+          const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), u = there ? load_chained(src) : zero, v = there ? load_chained(src + 1) : zero;
+          x[m][h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+          if (there && p.x_bf16) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[m][h];
+        }
+      }
+    if (slot >= 0)
+#pragma unroll
+      for (int m = 0; m < kMT; m++) {
+        const uint32_t lo[4] = {x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y}, hi[4] = {x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w};
+#pragma unroll
+        for (int j = 0; j < kTiles; j++) {
+          mma_bf16_16816(acc[m][j], lo, w[j].x, w[j].y);
+          mma_bf16_16816(acc[m][j], hi, w[j].z, w[j].w);
+        }
+      }
+  }
+  if constexpr (!kXBf16) fence_chained_writes();
+  if (slot < 0) return;
+  // the warps' sums, in their order
+  constexpr int kSlab = 16 * kMT * kRank;
+  float* const mine = slabs + warp * kSlab;
+#pragma unroll
+  for (int m = 0; m < kMT; m++)
+#pragma unroll
+    for (int j = 0; j < kTiles; j++) {
+      *reinterpret_cast<float2*>(mine + (16 * m + g) * kRank + 8 * j + 2 * t) = make_float2(acc[m][j][0], acc[m][j][1]);
+      *reinterpret_cast<float2*>(mine + (16 * m + 8 + g) * kRank + 8 * j + 2 * t) = make_float2(acc[m][j][2], acc[m][j][3]);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kSlab / 4; i += kLoraThreads) {
+    const int row = rows[4 * i / kRank];
+    float4 sum = reinterpret_cast<const float4*>(slabs)[i];
+#pragma unroll
+    for (int w = 1; w < kLoraWarps; w++) {
+      const float4 v = reinterpret_cast<const float4*>(slabs + w * kSlab)[i];
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    if (row >= 0) *reinterpret_cast<float4*>(p.t + ((size_t)blockIdx.y * p.M + row) * kRank + 4 * i % kRank) = sum;
+  }
+}
+
+struct UpParams {
+  const float* part;      // the GEMM's pieces [piece][M][N]; nullptr: no shared projection
+  GemmRanges rg;
+  const float* t;         // [split][M][rank]
+  const uint16_t* b;      // [slots][N][rank]
+  const float* factors;   // [slots], or nullptr: ones
+  void* out;
+  int32_t M, N, t_splits, out_bf16, adds;   // adds: to what out holds
+};
+
+// out[row][n] = sum of the GEMM's pieces (+ what out holds) + f_s sum over r of t[row][r] B_s[n][r].  grid (groups, blocks of 256 columns), 32 columns a warp: its four
+// tiles of the MMA take columns 8 (n / 2) + 2 tile + n % 2, so that a thread's results of a row are eight neighbours.  t is split into two bf16 halves, hi and lo:
+// 16 bits of it, where the projection's x has eight.
+template <int kRank, int kMT, bool kTurns, class List>
+__global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p, const __grid_constant__ List list) {
+  constexpr int kRows = 16 * kMT, kStride = kRank + 8, kSlices = (kRank + 31) / 32;   // k slices of 32 (one, of 8 or 16, for small ranks)
+  __shared__ __align__(16) uint16_t t_hi[kRows * kStride], t_lo[kRows * kStride];
+  __shared__ int32_t rows[kRows];
+  chain_release();
+  const int slot = group_rows<kRows>(list, blockIdx.x, rows);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.y * kUpCols + warp * 32, n = n0 + 8 * t;
+  // adapters were complete before the chain's head began: read ahead of the launches before this one
+  uint4 w[kSlices][4];
+  float factor = 1.f;
+  if (slot >= 0) {
+    const uint16_t* const b = p.b + (size_t)slot * p.N * kRank;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int col = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+      const uint16_t* src = b + (size_t)min(col, p.N - 1) * kRank;
+#pragma unroll
+      for (int s = 0; s < kSlices; s++) {
+        w[s][j] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (kRank >= 32) {
+          w[s][j] = load_chained(reinterpret_cast<const uint4*>(src + 32 * s + 8 * t));
+        } else if constexpr (kRank == 16) {
+          const uint2 v = load_chained(reinterpret_cast<const uint2*>(src + 4 * t));
+          w[s][j].x = v.x;
+          w[s][j].y = v.y;
+        } else {
+          w[s][j].x = load_chained(reinterpret_cast<const uint32_t*>(src + 2 * t));
+        }
+      }
+    }
+    if (p.factors) factor = load_chained(p.factors + slot);
+  }
+  __syncthreads();
+  chain_wait();
+  float acc[kMT][4][4];
+#pragma unroll
+  for (int m = 0; m < kMT; m++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[m][j][i] = 0.f;
+  if (slot >= 0) {
+    for (int i = threadIdx.x; i < kRows * kRank / 4; i += kLoraThreads) {
+      const int at = 4 * i / kRank, r = 4 * i % kRank, row = rows[at];
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row >= 0)
+        for (int s = 0; s < p.t_splits; s++) {
+          const float4 u = load_chained(reinterpret_cast<const float4*>(p.t + ((size_t)s * p.M + row) * kRank + r));
+          v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        }
+      v.x *= factor; v.y *= factor; v.z *= factor; v.w *= factor;
+      const uint2 hi = make_uint2(round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+      auto rest = [](float x, float h) { return fabsf(h) < __uint_as_float(0x7F800000u) ? x - h : 0.f; };   // an infinity has no second half
+      const uint2 lo = make_uint2(round_bf16x2(rest(v.x, bf16_lo(hi.x)), rest(v.y, bf16_hi(hi.x))), round_bf16x2(rest(v.z, bf16_lo(hi.y)), rest(v.w, bf16_hi(hi.y))));
+      *reinterpret_cast<uint2*>(t_hi + at * kStride + r) = hi;
+      *reinterpret_cast<uint2*>(t_lo + at * kStride + r) = lo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const uint16_t* const src = half ? t_lo : t_hi;
+#pragma unroll
+      for (int s = 0; s < kSlices; s++)
+#pragma unroll
+        for (int m = 0; m < kMT; m++) {
+          const uint16_t* const row0 = src + (16 * m + g) * kStride;
+          const uint16_t* const row1 = row0 + 8 * kStride;
+          if constexpr (kRank >= 32) {
+            const uint4 u = *reinterpret_cast<const uint4*>(row0 + 32 * s + 8 * t), v = *reinterpret_cast<const uint4*>(row1 + 32 * s + 8 * t);
+            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              mma_bf16_16816(acc[m][j], a0, w[s][j].x, w[s][j].y);
+              mma_bf16_16816(acc[m][j], a1, w[s][j].z, w[s][j].w);
+            }
+          } else {
+            uint32_t a0[4];
+            if constexpr (kRank == 16) {
+              const uint2 u = *reinterpret_cast<const uint2*>(row0 + 4 * t), v = *reinterpret_cast<const uint2*>(row1 + 4 * t);
+              a0[0] = u.x; a0[1] = v.x; a0[2] = u.y; a0[3] = v.y;
+            } else {
+              a0[0] = *reinterpret_cast<const uint32_t*>(row0 + 2 * t);
+              a0[1] = *reinterpret_cast<const uint32_t*>(row1 + 2 * t);
+              a0[2] = a0[3] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) mma_bf16_16816(acc[m][j], a0, w[s][j].x, w[s][j].y);
+          }
+        }
+    }
+  }
+  if (n >= p.N) return;   // N is a multiple of 8
+  const int col_tile = n / kGemmTileCols;
+  const int same = kTurns || !p.part ? 1 : p.rg.pieces(col_tile);
+#pragma unroll
+  for (int m = 0; m < kMT; m++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int row = rows[16 * m + 8 * h + g];
+      if (row < 0) continue;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[2 * j] = 0.f;
+        v[2 * j + 1] = 0.f;
+      }
+      const size_t at = (size_t)row * p.N + n;
+      if (p.part) {
+        const int pieces = kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row)) : same;
+#pragma unroll 2
+        for (int s = 0; s < pieces; s++) {
+          const float4* src = reinterpret_cast<const float4*>(p.part + (size_t)s * p.M * p.N + at);
+          const float4 a = load_chained(src), b = load_chained(src + 1);
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        }
+      }
+      if (p.adds) {
+        if (p.out_bf16) {
+          const uint4 a = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.out) + at));
+          v[0] += bf16_lo(a.x); v[1] += bf16_hi(a.x); v[2] += bf16_lo(a.y); v[3] += bf16_hi(a.y);
+          v[4] += bf16_lo(a.z); v[5] += bf16_hi(a.z); v[6] += bf16_lo(a.w); v[7] += bf16_hi(a.w);
+        } else {
+          const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.out) + at);
+          const float4 a = load_chained(src), b = load_chained(src + 1);
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[2 * j] += acc[m][j][2 * h];
+        v[2 * j + 1] += acc[m][j][2 * h + 1];
+      }
+      if (p.out_bf16) {
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + at) =
+            make_uint4(round_bf16x2(v[0], v[1]), round_bf16x2(v[2], v[3]), round_bf16x2(v[4], v[5]), round_bf16x2(v[6], v[7]));
+      } else {
+        float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+  fence_chained_writes();
+}
+
+// ---- the host's half ----
+struct Request {
+  int32_t row, n, slot;
+};
+// Neighbouring requests of one adapter as one, in row order.
+std::vector<Request> merged_requests(int n_seqs, const int32_t* n_rows, const int32_t* adapter) {
+  std::vector<Request> v;
+  int row = 0;
+  for (int i = 0; i < n_seqs; i++) {
+    const int n = n_rows ? n_rows[i] : 1;
+    if (!n) continue;
+    if (!v.empty() && v.back().slot == adapter[i]) v.back().n += n;
+    else v.push_back(Request{row, n, adapter[i]});
+    row += n;
+  }
+  return v;
+}
+// The list of some of them; returns the groups.
+template <class List>
+int make_list(std::vector<Request> r, int group_rows, List* list) {
+  std::stable_sort(r.begin(), r.end(), [](const Request& a, const Request& b) { return a.slot < b.slot; });
+  list->n_pieces = (int)r.size();
+  list->n_runs = 0;
+  int at = 0, groups = 0;
+  for (size_t i = 0; i < r.size(); i++) {
+    if (i == 0 || r[i].slot != r[i - 1].slot) {
+      if (i) groups += (at - list->run_at[list->n_runs - 1] + group_rows - 1) / group_rows;
+      list->slot[list->n_runs] = r[i].slot;
+      list->run_at[list->n_runs] = at;
+      list->group[list->n_runs++] = groups;
+    }
+    list->at[i] = at;
+    list->row[i] = r[i].row;
+    at += r[i].n;
+  }
+  groups += (at - list->run_at[list->n_runs - 1] + group_rows - 1) / group_rows;
+  list->at[r.size()] = list->run_at[list->n_runs] = at;
+  list->group[list->n_runs] = groups;
+  return groups;
+}
+
+template <int kRank, int kMT, class List>
+int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int splits, bool x_bf16) {
+  constexpr size_t smem = (size_t)kLoraWarps * 16 * kMT * kRank * sizeof(float);
+  const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
+  const dim3 grid((unsigned)groups, (unsigned)splits);
+  auto go = [&](auto kernel) -> int32_t {
+    if (smem > 48 << 10)
+      if (int32_t rc = allow_smem(p->dev, kernel, smem)) return rc;
+    RELUX_CUDA_TRY(launch_chained(chained, kernel, grid, dim3(kLoraThreads), smem, p->dev->stream, prm, list));
+    count_launch(p->dev);
+    return RELUX_OK;
+  };
+  return x_bf16 ? go(lora_down_kernel<kRank, kMT, true, List>) : go(lora_down_kernel<kRank, kMT, false, List>);
+}
+template <int kRank, int kMT, class List>
+int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {
+  const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
+  const dim3 grid((unsigned)groups, (unsigned)((prm.N + kUpCols - 1) / kUpCols));
+  if (prm.part && prm.rg.in_turns())
+    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, kMT, true, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+  else
+    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, kMT, false, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+  count_launch(p->dev);
+  return RELUX_OK;
+}
+
+// All launches of a call for one rank.  Groups of 16 rows; of calls of more than 512 rows, whose runs are long, of 64 (ranks 64 and 128: 32, what the sums of a
+// warp leave registers for).
+template <int kRank>
+int32_t run_lora(Pool* p, const relux_matmul_lora_args* a, const std::vector<Request>& requests, DownParams down, UpParams up, const WeightRef* w, const LayerScratch& sc,
+                 int t_splits) {
+  constexpr int kLong = kRank >= 64 ? 2 : 4;
+  const bool x_bf16 = a->x_dtype == RELUX_DTYPE_BF16, many = a->m > 512;
+  auto each = [&](auto&& launch) -> int32_t {   // by parts of up to kLargeList requests
+    for (size_t i = 0; i < requests.size(); i += kLargeList) {
+      std::vector<Request> part(requests.begin() + i, requests.begin() + std::min(requests.size(), i + kLargeList));
+      int32_t rc;
+      if (part.size() <= kSmallList) {
+        LoraList<kSmallList> list;
+        rc = launch(list, make_list(part, 16 * (many ? kLong : 1), &list));
+      } else {
+        LoraList<kLargeList> list;
+        rc = launch(list, make_list(part, 16 * (many ? kLong : 1), &list));
+      }
+      if (rc) return rc;
+    }
+    return RELUX_OK;
+  };
+  int32_t rc = each([&](const auto& list, int groups) {
+    return many ? launch_down<kRank, kLong>(p, down, list, groups, t_splits, x_bf16) : launch_down<kRank, 1>(p, down, list, groups, t_splits, x_bf16);
+  });
+  if (rc) return rc;
+  if (w)
+    if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
+  return each([&](const auto& list, int groups) { return many ? launch_up<kRank, kLong>(p, up, list, groups) : launch_up<kRank, 1>(p, up, list, groups); });
+}
+
+}  // namespace
+
+int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
+  if (!a || !a->x || !a->lora_a || !a->lora_b || !a->adapter || !a->out) { set_error("nil argument"); return RELUX_ERR_INVALID_ARG; }
+  if (a->m <= 0 || a->k <= 0 || a->n <= 0 || a->n_seqs <= 0 || a->n_slots <= 0) {
+    set_error("matmul_lora: M=%d K=%d N=%d, %d requests and %d slots must be positive", a->m, a->k, a->n, a->n_seqs, a->n_slots);
+    return RELUX_ERR_INVALID_ARG;
+  }
+  auto dtype_ok = [](int32_t t) { return t == RELUX_DTYPE_F32 || t == RELUX_DTYPE_BF16; };
+  if (!dtype_ok(a->x_dtype) || !dtype_ok(a->out_dtype)) { set_error("bad dtype flag"); return RELUX_ERR_INVALID_ARG; }
+  for (int i = 0; i < 3; i++)
+    if (a->reserved[i]) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  int64_t rows = 0;
+  for (int i = 0; i < a->n_seqs; i++) {
+    const int n = a->n_rows ? a->n_rows[i] : 1;
+    if (n < 0) { set_error("matmul_lora: negative row count of request %d", i); return RELUX_ERR_INVALID_ARG; }
+    if (a->adapter[i] < -1 || a->adapter[i] >= a->n_slots) {
+      set_error("matmul_lora: adapter %d of request %d outside [-1, %d)", a->adapter[i], i, a->n_slots);
+      return RELUX_ERR_INVALID_ARG;
+    }
+    rows += n;
+  }
+  if (rows != a->m) { set_error("matmul_lora: the requests have %lld rows, M=%d", (long long)rows, a->m); return RELUX_ERR_INVALID_ARG; }
+  int32_t rc;
+  if ((rc = check_dev_align(a->x, "x")) || (rc = check_dev_align(a->w, "w")) || (rc = check_dev_align(a->lora_a, "lora_a")) || (rc = check_dev_align(a->lora_b, "lora_b")) ||
+      (rc = check_dev_align(a->factors, "factors")) || (rc = check_dev_align(a->out, "out")))
+    return rc;
+  if (a->k % 8 != 0 || a->n % 8 != 0 || (a->rank != 8 && a->rank != 16 && a->rank != 32 && a->rank != 64 && a->rank != 128)) {
+    set_error("matmul_lora: K=%d and N=%d must be multiples of 8, rank=%d one of 8, 16, 32, 64, 128", a->k, a->n, a->rank);
+    return RELUX_ERR_UNSUPPORTED;
+  }
+  const std::vector<Request> requests = merged_requests(a->n_seqs, a->n_rows, a->adapter);
+  // parts of K of t: enough blocks for the SMs, of 256 k at least (a step of every warp)
+  const int groups_least = (a->m + 15) / 16 + (int)requests.size() / 2;
+  const int t_splits = std::max(1, std::min({kMaxKSplit, p->dev->sm_count / groups_least, a->k / 256}));
+  LayerScratch sc;
+  const size_t t_bytes = (size_t)t_splits * a->m * a->rank * sizeof(float);
+  if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes, &sc))) return rc;
+  DownParams down{a->x, a->w && a->x_dtype == RELUX_DTYPE_F32 ? sc.a_bf16 : nullptr, (const uint16_t*)a->lora_a, (float*)sc.rest, a->m, a->k};
+  UpParams up{};
+  up.part = a->w ? sc.part : nullptr;
+  up.t = (const float*)sc.rest;
+  up.b = (const uint16_t*)a->lora_b;
+  up.factors = a->factors;
+  up.out = a->out;
+  up.M = a->m;
+  up.N = a->n;
+  up.t_splits = t_splits;
+  up.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
+  up.adds = a->accumulate != 0;
+  const WeightRef w{a->w, a->n};
+  const WeightRef* shared = a->w ? &w : nullptr;
+  switch (a->rank) {
+    case 8: return run_lora<8>(p, a, requests, down, up, shared, sc, t_splits);
+    case 16: return run_lora<16>(p, a, requests, down, up, shared, sc, t_splits);
+    case 32: return run_lora<32>(p, a, requests, down, up, shared, sc, t_splits);
+    case 64: return run_lora<64>(p, a, requests, down, up, shared, sc, t_splits);
+    default: return run_lora<128>(p, a, requests, down, up, shared, sc, t_splits);
+  }
+}
+
+}  // namespace relux

@@ -1715,6 +1715,10 @@ API int32_t relux_matmul_int8(relux_pool_t h, const relux_matmul_int8_args* a) {
   GET_POOL(h);
   return without_exceptions([&] { return do_matmul_int8(p, a); });
 }
+API int32_t relux_matmul_lora(relux_pool_t h, const relux_matmul_lora_args* a) {
+  GET_POOL(h);
+  return without_exceptions([&] { return do_matmul_lora(p, a); });
+}
 
 API int32_t relux_mla_import_weights(relux_pool_t h, const relux_mla_import_args* a) {
   GET_POOL(h);

@@ -40,7 +40,7 @@ EXPORTS = [
     "relux_spec_accept", "relux_sampler_sample", "relux_pool_tune", "relux_pool_kernel_ms_list", "relux_matmul_f32_bf16",
     "relux_mla_import_weights", "relux_pool_selftest_wait", "relux_pool_wait_output", "relux_mla_step", "relux_gqa_step", "relux_mla_expand_kv",
     "relux_gqa_read_kv", "relux_gqa_tree_verify", "relux_gqa_tree_commit", "relux_rmsnorm", "relux_int8_rows", "relux_int8_weights",
-    "relux_matmul_int8",
+    "relux_matmul_int8", "relux_matmul_lora",
 ]
 
 
@@ -115,6 +115,13 @@ class Int8WeightsArgs(C.Structure):
 class MatmulInt8Args(C.Structure):
     _fields_ = [("m", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("out_dtype", C.c_int32), ("a", C.c_void_p), ("a_scales", C.c_void_p),
                 ("w", C.c_void_p), ("w_scales", C.c_void_p), ("out", C.c_void_p), ("reserved", C.c_int32 * 4)]
+
+
+class MatmulLoraArgs(C.Structure):
+    _fields_ = [("m", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("rank", C.c_int32), ("n_slots", C.c_int32), ("n_seqs", C.c_int32),
+                ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("accumulate", C.c_int32), ("reserved", C.c_int32 * 3), ("x", C.c_void_p),
+                ("w", C.c_void_p), ("lora_a", C.c_void_p), ("lora_b", C.c_void_p), ("factors", C.c_void_p), ("adapter", C.c_void_p),
+                ("n_rows", C.c_void_p), ("out", C.c_void_p)]
 
 
 class MlaLayerWeights(C.Structure):
@@ -196,6 +203,7 @@ pack_rmsnorm = _packer(RmsnormArgs)
 pack_int8_rows = _packer(Int8RowsArgs)
 pack_int8_weights = _packer(Int8WeightsArgs)
 pack_matmul_int8 = _packer(MatmulInt8Args)
+pack_matmul_lora = _packer(MatmulLoraArgs)
 
 
 class ReluxCudaError(RuntimeError):
@@ -280,6 +288,7 @@ def load():
         L.relux_int8_rows.argtypes = [C.c_void_p, C.POINTER(Int8RowsArgs)]
         L.relux_int8_weights.argtypes = [C.c_void_p, C.POINTER(Int8WeightsArgs)]
         L.relux_matmul_int8.argtypes = [C.c_void_p, C.POINTER(MatmulInt8Args)]
+        L.relux_matmul_lora.argtypes = [C.c_void_p, C.POINTER(MatmulLoraArgs)]
         L.relux_spec_accept.argtypes = [C.c_void_p, C.POINTER(SpecAcceptArgs)]
         L.relux_sampler_sample.argtypes = [C.c_void_p, C.POINTER(SampleArgs)]
         L.relux_pool_last_kernel_ms.argtypes = [C.c_void_p, C.POINTER(C.c_float)]
@@ -289,7 +298,7 @@ def load():
         # the per-token calls once more, taking their argument structs as packed bytes (pack_append, pack_attn)
         for name, n_structs in (("mla_append", 1), ("gqa_append", 1), ("mla_decode", 1), ("gqa_decode", 1), ("mla_verify", 2), ("gqa_verify", 2),
                                 ("mla_step", 2), ("gqa_step", 2), ("gqa_tree_verify", 3), ("gqa_tree_commit", 1), ("gqa_read_kv", 1),
-                                ("rmsnorm", 1), ("int8_rows", 1), ("int8_weights", 1), ("matmul_int8", 1)):
+                                ("rmsnorm", 1), ("int8_rows", 1), ("int8_weights", 1), ("matmul_int8", 1), ("matmul_lora", 1)):
             f = L["relux_" + name]   # a function object of its own
             f.restype, f.argtypes = C.c_int32, [C.c_void_p] + [C.c_char_p] * n_structs
             packed[name] = f

@@ -46,7 +46,7 @@ struct Device {
   std::mutex mu;
   int64_t launches = 0;
   std::vector<std::pair<const void*, size_t>> smem_allowed;   // what allow_smem knows of the kernels' limits, under mu
-  int int8_clusters[9] = {};   // clusters of so many CTAs of an 8-bit product (one CTA an SM) that are resident at once, 0: not asked yet
+  int tile_clusters[9] = {};   // clusters of so many CTAs, one an SM, that are resident at once (launch_tiles), 0: not asked yet
   void* flush_buf = nullptr;
   size_t flush_bytes = 0;
   // Page-locked memory for results of host calls, written by the kernel that makes them: the call waits for the stream and

@@ -1,17 +1,20 @@
 // A shared projection with low-rank adapters of many requests beside it: C[m] = x[m] W + f_s (x[m] A_s^T) B_s^T, s the adapter of the
 // request that row m belongs to, or none.  A_s [rank][K], B_s [N][rank] in slots of two arrays, as checkpoints hold them (lora_A, lora_B).
 //
-// Three launches, as many as the projection alone: lora_down_kernel rounds x to bf16 for the projection and takes t = x A_s^T while it holds the
-// rows; the projection's GEMM (skinny_gemm_sm100_kernel); lora_up_kernel adds up the GEMM's pieces and, on the way out, t B_s^T.
-// The adapters stay out of the GEMM's tiles on purpose: a tile holds rows of many requests, and a product with another request's B, even by
-// zeros, would carry its infinities and NaN into this one's rows.
-// Rows are taken in groups of one adapter, wherever in the batch they lie: the host sorts the requests by adapter, so that an adapter is read
-// once for 16 (long calls 32 or 64) rows of it.  Bound: HBM, W and the adapters in use once, for few rows; for prompts the GEMM.
+// Two launches: lora_down_kernel takes t = x A_s^T, and rounds a float32 x to bf16 while it holds the rows; lora_gemm_kernel (lora_gemm.cu) is the projection,
+// whose epilogue or last steps add t B_s^T.  Three where the rows are many and of so many requests that tiles of one request's rows would be mostly
+// empty, or where the projection is not this call's: lora_down_kernel, the projection's GEMM (skinny_gemm_sm100_kernel), and lora_up_kernel, which adds up
+// the GEMM's pieces and, on the way out, t B_s^T.
+// No tile of a product holds rows of one request and another's adapter: a product with that by zeros would carry its infinities and NaN over.
+// In lora_down_kernel and lora_up_kernel rows are taken in groups of 16 of one adapter, wherever in the batch they lie: the host sorts the requests by adapter,
+// so that an adapter is read once for 16 of its rows.  Bound: HBM, W and the adapters in use once, for few rows; for prompts the GEMM.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "common.cuh"
 #include "internal.h"
+#include "lora.cuh"
 #include "projection.cuh"
 
 namespace relux {
@@ -20,13 +23,24 @@ namespace {
 
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
-constexpr int kMaxKSplit = 8;
+constexpr int kMaxKSplit = 8, kGroupRows = 16;
+constexpr int kSomeRows = 512;                       // of up to so many rows a list names each
 constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
 
-// The rows of a call (or of a part of it), in the order of their adapters.  A piece is a range of neighbouring rows of one adapter; a run is
-// all the pieces of one.  Groups are cut within runs.
+// The rows of a call (or of a part of it), in the order of their adapters, cut into groups of one adapter.
+// Of few rows: every group and its rows.
 template <int kCap>
-struct LoraList {
+struct RowList {
+  struct Group {
+    int32_t slot;        // adapter, or -1
+    int16_t first, n;    // its rows' places
+  };
+  Group group[kCap];
+  int16_t row[kCap];
+};
+// Of many: a piece is a range of neighbouring rows of one adapter, a run all the pieces of one; groups are cut within runs, all but a run's last of full size.
+template <int kCap>
+struct RunList {
   int32_t n_pieces, n_runs;
   int32_t at[kCap + 1];      // first place, in this order, of a piece
   int32_t row[kCap];         // its first row
@@ -35,7 +49,7 @@ struct LoraList {
   int32_t group[kCap + 1];   // first group of a run
 };
 // The last of n ascending entries that is no more than v.
-__device__ __forceinline__ int last_up_to(const int32_t* a, int n, int v) {
+__host__ __device__ __forceinline__ int last_up_to(const int32_t* a, int n, int v) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -45,8 +59,14 @@ __device__ __forceinline__ int last_up_to(const int32_t* a, int n, int v) {
   return lo;
 }
 // Rows of a group to shared memory (-1: none), and its adapter.  By all threads; a barrier follows.
-template <int kGroupRows, class List>
-__device__ __forceinline__ int group_rows(const List& list, int group, int32_t* rows) {
+template <int kCap>
+__device__ __forceinline__ int group_rows(const RowList<kCap>& list, int group, int32_t* rows) {
+  const auto g = list.group[group];
+  if (threadIdx.x < kGroupRows) rows[threadIdx.x] = (int)threadIdx.x < g.n ? list.row[g.first + threadIdx.x] : -1;
+  return g.slot;
+}
+template <int kCap>
+__device__ __forceinline__ int group_rows(const RunList<kCap>& list, int group, int32_t* rows) {
   const int run = last_up_to(list.group, list.n_runs, group);
   const int first = list.run_at[run] + (group - list.group[run]) * kGroupRows, end = list.run_at[run + 1];
   if (threadIdx.x < kGroupRows) {
@@ -61,7 +81,18 @@ __device__ __forceinline__ int group_rows(const List& list, int group, int32_t* 
   return list.slot[run];
 }
 
+// f v as two bf16 halves, 16 bits of it.
+__device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2& lo) {
+  auto rest = [](float x, float h) { return fabsf(h) < __uint_as_float(0x7F800000u) ? x - h : 0.f; };   // an infinity has no second half
+  v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+  hi = make_uint2(round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+  lo = make_uint2(round_bf16x2(rest(v.x, bf16_lo(hi.x)), rest(v.y, bf16_hi(hi.x))), round_bf16x2(rest(v.z, bf16_lo(hi.y)), rest(v.w, bf16_hi(hi.y))));
+}
+
 struct DownParams {
+  uint16_t* t_hi;         // [M][rank], factors included, the first bf16 half, or nullptr
+  uint16_t* t_lo;         // and the second
+  const float* factors;
   const void* x;
   uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr
   const uint16_t* a;      // [slots][rank][K]
@@ -71,80 +102,68 @@ struct DownParams {
 
 // t[row][r] = sum over this block's part of K of x[row][k] A_s[r][k].  grid (groups, parts of K), 8 warps that take 32 k each in turn.  mma.sync: a group is a handful of
 // rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
-template <int kRank, int kMT, bool kXBf16, class List>
+template <int kRank, bool kXBf16, class List>
 __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
   constexpr int kTiles = kRank / 8;
-  extern __shared__ __align__(16) float slabs[];   // [warp][16 kMT][kRank]
-  __shared__ int32_t rows[16 * kMT];
+  extern __shared__ __align__(16) float slabs[];   // [warp][16][kRank]
+  __shared__ int32_t rows[kGroupRows];
   // waits before it releases: the projection behind it may read its weights early (launch_chained, head of a chain)
   chain_wait();
   chain_release();
-  const int slot = group_rows<16 * kMT>(list, blockIdx.x, rows);
+  const int slot = group_rows(list, blockIdx.x, rows);
   if (slot < 0 && !p.x_bf16) return;
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
-  int32_t r[kMT][2];
+  const int32_t r[2] = {rows[g], rows[8 + g]};
+  float acc[kTiles][4];
 #pragma unroll
-  for (int m = 0; m < kMT; m++)
+  for (int j = 0; j < kTiles; j++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) r[m][h] = rows[16 * m + 8 * h + g];
-  float acc[kMT][kTiles][4];
-#pragma unroll
-  for (int m = 0; m < kMT; m++)
-#pragma unroll
-    for (int j = 0; j < kTiles; j++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) acc[m][j][i] = 0.f;
+    for (int i = 0; i < 4; i++) acc[j][i] = 0.f;
   const uint16_t* const a = p.a + (size_t)max(slot, 0) * kRank * p.K;
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
 
-#pragma unroll(kMT == 1 && kRank <= 32 ? 4 : kMT == 1 || kRank <= 16 ? 2 : 1)
+#pragma unroll(kRank <= 32 ? 4 : 2)
   for (int s = s0 + warp; s < s1; s += kLoraWarps) {
     const int k = s * 32 + 8 * t;
     const bool in = k < p.K;   // K is a multiple of 8
-    uint4 x[kMT][2], w[kTiles];
+    uint4 x[2], w[kTiles];
     if (slot >= 0)
 #pragma unroll
       for (int j = 0; j < kTiles; j++) w[j] = in ? load_chained(reinterpret_cast<const uint4*>(a + (size_t)(8 * j + g) * p.K + k)) : none;
 #pragma unroll
-    for (int m = 0; m < kMT; m++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const size_t at = (size_t)max(r[m][h], 0) * p.K + k;
-        const bool there = in && r[m][h] >= 0;
-        if constexpr (kXBf16) {
-          x[m][h] = there ? load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at)) : none;
-        } else {
-          const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
-          const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), u = there ? load_chained(src) : zero, v = there ? load_chained(src + 1) : zero;
-          x[m][h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
-          if (there && p.x_bf16) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[m][h];
-        }
+    for (int h = 0; h < 2; h++) {
+      const size_t at = (size_t)max(r[h], 0) * p.K + k;
+      const bool there = in && r[h] >= 0;
+      if constexpr (kXBf16) {
+        x[h] = there ? load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at)) : none;
+      } else {
+        const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), u = there ? load_chained(src) : zero, v = there ? load_chained(src + 1) : zero;
+        x[h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+        if (there && p.x_bf16) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[h];
       }
-    if (slot >= 0)
+    }
+    if (slot >= 0) {
+      const uint32_t lo[4] = {x[0].x, x[1].x, x[0].y, x[1].y}, hi[4] = {x[0].z, x[1].z, x[0].w, x[1].w};
 #pragma unroll
-      for (int m = 0; m < kMT; m++) {
-        const uint32_t lo[4] = {x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y}, hi[4] = {x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w};
-#pragma unroll
-        for (int j = 0; j < kTiles; j++) {
-          mma_bf16_16816(acc[m][j], lo, w[j].x, w[j].y);
-          mma_bf16_16816(acc[m][j], hi, w[j].z, w[j].w);
-        }
+      for (int j = 0; j < kTiles; j++) {
+        mma_bf16_16816(acc[j], lo, w[j].x, w[j].y);
+        mma_bf16_16816(acc[j], hi, w[j].z, w[j].w);
       }
+    }
   }
   if constexpr (!kXBf16) fence_chained_writes();
   if (slot < 0) return;
   // the warps' sums, in their order
-  constexpr int kSlab = 16 * kMT * kRank;
+  constexpr int kSlab = kGroupRows * kRank;
   float* const mine = slabs + warp * kSlab;
 #pragma unroll
-  for (int m = 0; m < kMT; m++)
-#pragma unroll
-    for (int j = 0; j < kTiles; j++) {
-      *reinterpret_cast<float2*>(mine + (16 * m + g) * kRank + 8 * j + 2 * t) = make_float2(acc[m][j][0], acc[m][j][1]);
-      *reinterpret_cast<float2*>(mine + (16 * m + 8 + g) * kRank + 8 * j + 2 * t) = make_float2(acc[m][j][2], acc[m][j][3]);
-    }
+  for (int j = 0; j < kTiles; j++) {
+    *reinterpret_cast<float2*>(mine + g * kRank + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(mine + (8 + g) * kRank + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < kSlab / 4; i += kLoraThreads) {
     const int row = rows[4 * i / kRank];
@@ -154,8 +173,17 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParam
       const float4 v = reinterpret_cast<const float4*>(slabs + w * kSlab)[i];
       sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
     }
-    if (row >= 0) *reinterpret_cast<float4*>(p.t + ((size_t)blockIdx.y * p.M + row) * kRank + 4 * i % kRank) = sum;
+    if (row < 0) continue;
+    if (p.t_hi) {
+      uint2 hi, lo;
+      split_halves(sum, p.factors ? load_chained(p.factors + slot) : 1.f, hi, lo);
+      *reinterpret_cast<uint2*>(p.t_hi + (size_t)row * kRank + 4 * i % kRank) = hi;
+      *reinterpret_cast<uint2*>(p.t_lo + (size_t)row * kRank + 4 * i % kRank) = lo;
+    } else {
+      *reinterpret_cast<float4*>(p.t + ((size_t)blockIdx.y * p.M + row) * kRank + 4 * i % kRank) = sum;
+    }
   }
+  if (p.t_hi) fence_chained_writes();
 }
 
 struct UpParams {
@@ -171,13 +199,13 @@ struct UpParams {
 // out[row][n] = sum of the GEMM's pieces (+ what out holds) + f_s sum over r of t[row][r] B_s[n][r].  grid (groups, blocks of 256 columns), 32 columns a warp: its four
 // tiles of the MMA take columns 8 (n / 2) + 2 tile + n % 2, so that a thread's results of a row are eight neighbours.  t is split into two bf16 halves, hi and lo:
 // 16 bits of it, where the projection's x has eight.
-template <int kRank, int kMT, bool kTurns, class List>
+template <int kRank, bool kTurns, class List>
 __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p, const __grid_constant__ List list) {
-  constexpr int kRows = 16 * kMT, kStride = kRank + 8, kSlices = (kRank + 31) / 32;   // k slices of 32 (one, of 8 or 16, for small ranks)
-  __shared__ __align__(16) uint16_t t_hi[kRows * kStride], t_lo[kRows * kStride];
-  __shared__ int32_t rows[kRows];
+  constexpr int kStride = kRank + 8, kSlices = (kRank + 31) / 32;   // k slices of 32 (one, of 8 or 16, for small ranks)
+  __shared__ __align__(16) uint16_t t_hi[kGroupRows * kStride], t_lo[kGroupRows * kStride];
+  __shared__ int32_t rows[kGroupRows];
   chain_release();
-  const int slot = group_rows<kRows>(list, blockIdx.x, rows);
+  const int slot = group_rows(list, blockIdx.x, rows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.y * kUpCols + warp * 32, n = n0 + 8 * t;
   // adapters were complete before the chain's head began: read ahead of the launches before this one
@@ -207,15 +235,51 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
   }
   __syncthreads();
   chain_wait();
-  float acc[kMT][4][4];
+  // the shared projection's sums, and what out holds, are where the adapter's begin
+  const int col_tile = n / kGemmTileCols;
+  const int same = kTurns || !p.part ? 1 : p.rg.pieces(col_tile);
+  float acc[4][4];
+  auto add = [&](int h, const float (&v)[8]) {
 #pragma unroll
-  for (int m = 0; m < kMT; m++)
+    for (int j = 0; j < 4; j++) {
+      acc[j][2 * h] += v[2 * j];
+      acc[j][2 * h + 1] += v[2 * j + 1];
+    }
+  };
+  auto add_f32 = [&](int h, const float* src) {
+    const float4 a = load_chained(reinterpret_cast<const float4*>(src)), b = load_chained(reinterpret_cast<const float4*>(src) + 1);
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    add(h, v);
+  };
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+  for (int j = 0; j < 4; j++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[m][j][i] = 0.f;
+    for (int i = 0; i < 4; i++) acc[j][i] = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {   // (the first pieces of both rows are on their way together)
+    const int row = rows[8 * h + g];
+    if (p.part && row >= 0 && n < p.N) add_f32(h, p.part + (size_t)row * p.N + n);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int row = rows[8 * h + g];
+    if (row < 0 || n >= p.N) continue;
+    const size_t at = (size_t)row * p.N + n;
+    const int pieces = !p.part ? 1 : kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row)) : same;
+#pragma unroll 2
+    for (int s = 1; s < pieces; s++) add_f32(h, p.part + (size_t)s * p.M * p.N + at);
+    if (p.adds) {
+      if (p.out_bf16) {
+        const uint4 a = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.out) + at));
+        const float v[8] = {bf16_lo(a.x), bf16_hi(a.x), bf16_lo(a.y), bf16_hi(a.y), bf16_lo(a.z), bf16_hi(a.z), bf16_lo(a.w), bf16_hi(a.w)};
+        add(h, v);
+      } else {
+        add_f32(h, reinterpret_cast<const float*>(p.out) + at);
+      }
+    }
+  }
   if (slot >= 0) {
-    for (int i = threadIdx.x; i < kRows * kRank / 4; i += kLoraThreads) {
+    for (int i = threadIdx.x; i < kGroupRows * kRank / 4; i += kLoraThreads) {
       const int at = 4 * i / kRank, r = 4 * i % kRank, row = rows[at];
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row >= 0)
@@ -223,10 +287,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
           const float4 u = load_chained(reinterpret_cast<const float4*>(p.t + ((size_t)s * p.M + row) * kRank + r));
           v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
         }
-      v.x *= factor; v.y *= factor; v.z *= factor; v.w *= factor;
-      const uint2 hi = make_uint2(round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
-      auto rest = [](float x, float h) { return fabsf(h) < __uint_as_float(0x7F800000u) ? x - h : 0.f; };   // an infinity has no second half
-      const uint2 lo = make_uint2(round_bf16x2(rest(v.x, bf16_lo(hi.x)), rest(v.y, bf16_hi(hi.x))), round_bf16x2(rest(v.z, bf16_lo(hi.y)), rest(v.w, bf16_hi(hi.y))));
+      uint2 hi, lo;
+      split_halves(v, factor, hi, lo);
       *reinterpret_cast<uint2*>(t_hi + at * kStride + r) = hi;
       *reinterpret_cast<uint2*>(t_lo + at * kStride + r) = lo;
     }
@@ -235,87 +297,49 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
     for (int half = 0; half < 2; half++) {
       const uint16_t* const src = half ? t_lo : t_hi;
 #pragma unroll
-      for (int s = 0; s < kSlices; s++)
+      for (int s = 0; s < kSlices; s++) {
+        const uint16_t* const row0 = src + g * kStride;
+        const uint16_t* const row1 = row0 + 8 * kStride;
+        if constexpr (kRank >= 32) {
+          const uint4 u = *reinterpret_cast<const uint4*>(row0 + 32 * s + 8 * t), v = *reinterpret_cast<const uint4*>(row1 + 32 * s + 8 * t);
+          const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
-        for (int m = 0; m < kMT; m++) {
-          const uint16_t* const row0 = src + (16 * m + g) * kStride;
-          const uint16_t* const row1 = row0 + 8 * kStride;
-          if constexpr (kRank >= 32) {
-            const uint4 u = *reinterpret_cast<const uint4*>(row0 + 32 * s + 8 * t), v = *reinterpret_cast<const uint4*>(row1 + 32 * s + 8 * t);
-            const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              mma_bf16_16816(acc[m][j], a0, w[s][j].x, w[s][j].y);
-              mma_bf16_16816(acc[m][j], a1, w[s][j].z, w[s][j].w);
-            }
-          } else {
-            uint32_t a0[4];
-            if constexpr (kRank == 16) {
-              const uint2 u = *reinterpret_cast<const uint2*>(row0 + 4 * t), v = *reinterpret_cast<const uint2*>(row1 + 4 * t);
-              a0[0] = u.x; a0[1] = v.x; a0[2] = u.y; a0[3] = v.y;
-            } else {
-              a0[0] = *reinterpret_cast<const uint32_t*>(row0 + 2 * t);
-              a0[1] = *reinterpret_cast<const uint32_t*>(row1 + 2 * t);
-              a0[2] = a0[3] = 0u;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) mma_bf16_16816(acc[m][j], a0, w[s][j].x, w[s][j].y);
+          for (int j = 0; j < 4; j++) {
+            mma_bf16_16816(acc[j], a0, w[s][j].x, w[s][j].y);
+            mma_bf16_16816(acc[j], a1, w[s][j].z, w[s][j].w);
           }
+        } else {
+          uint32_t a0[4];
+          if constexpr (kRank == 16) {
+            const uint2 u = *reinterpret_cast<const uint2*>(row0 + 4 * t), v = *reinterpret_cast<const uint2*>(row1 + 4 * t);
+            a0[0] = u.x; a0[1] = v.x; a0[2] = u.y; a0[3] = v.y;
+          } else {
+            a0[0] = *reinterpret_cast<const uint32_t*>(row0 + 2 * t);
+            a0[1] = *reinterpret_cast<const uint32_t*>(row1 + 2 * t);
+            a0[2] = a0[3] = 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) mma_bf16_16816(acc[j], a0, w[s][j].x, w[s][j].y);
         }
+      }
     }
   }
   if (n >= p.N) return;   // N is a multiple of 8
-  const int col_tile = n / kGemmTileCols;
-  const int same = kTurns || !p.part ? 1 : p.rg.pieces(col_tile);
 #pragma unroll
-  for (int m = 0; m < kMT; m++)
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int row = rows[16 * m + 8 * h + g];
-      if (row < 0) continue;
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        v[2 * j] = 0.f;
-        v[2 * j + 1] = 0.f;
-      }
-      const size_t at = (size_t)row * p.N + n;
-      if (p.part) {
-        const int pieces = kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row)) : same;
-#pragma unroll 2
-        for (int s = 0; s < pieces; s++) {
-          const float4* src = reinterpret_cast<const float4*>(p.part + (size_t)s * p.M * p.N + at);
-          const float4 a = load_chained(src), b = load_chained(src + 1);
-          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-        }
-      }
-      if (p.adds) {
-        if (p.out_bf16) {
-          const uint4 a = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.out) + at));
-          v[0] += bf16_lo(a.x); v[1] += bf16_hi(a.x); v[2] += bf16_lo(a.y); v[3] += bf16_hi(a.y);
-          v[4] += bf16_lo(a.z); v[5] += bf16_hi(a.z); v[6] += bf16_lo(a.w); v[7] += bf16_hi(a.w);
-        } else {
-          const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.out) + at);
-          const float4 a = load_chained(src), b = load_chained(src + 1);
-          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        v[2 * j] += acc[m][j][2 * h];
-        v[2 * j + 1] += acc[m][j][2 * h + 1];
-      }
-      if (p.out_bf16) {
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + at) =
-            make_uint4(round_bf16x2(v[0], v[1]), round_bf16x2(v[2], v[3]), round_bf16x2(v[4], v[5]), round_bf16x2(v[6], v[7]));
-      } else {
-        float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
-        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-      }
+  for (int h = 0; h < 2; h++) {
+    const int row = rows[8 * h + g];
+    if (row < 0) continue;
+    const size_t at = (size_t)row * p.N + n;
+    if (p.out_bf16) {
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + at) =
+          make_uint4(round_bf16x2(acc[0][2 * h], acc[0][2 * h + 1]), round_bf16x2(acc[1][2 * h], acc[1][2 * h + 1]), round_bf16x2(acc[2][2 * h], acc[2][2 * h + 1]),
+                     round_bf16x2(acc[3][2 * h], acc[3][2 * h + 1]));
+    } else {
+      float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
+      dst[0] = make_float4(acc[0][2 * h], acc[0][2 * h + 1], acc[1][2 * h], acc[1][2 * h + 1]);
+      dst[1] = make_float4(acc[2][2 * h], acc[2][2 * h + 1], acc[3][2 * h], acc[3][2 * h + 1]);
     }
+  }
   fence_chained_writes();
 }
 
@@ -336,16 +360,29 @@ std::vector<Request> merged_requests(int n_seqs, const int32_t* n_rows, const in
   }
   return v;
 }
-// The list of some of them; returns the groups.
-template <class List>
-int make_list(std::vector<Request> r, int group_rows, List* list) {
-  std::stable_sort(r.begin(), r.end(), [](const Request& a, const Request& b) { return a.slot < b.slot; });
+bool by_slot(const Request& a, const Request& b) { return a.slot < b.slot; }
+// The list of all of them, or of some; returns the groups.
+template <int kCap>
+int make_list(std::vector<Request> r, RowList<kCap>* list) {
+  std::stable_sort(r.begin(), r.end(), by_slot);
+  int groups = 0, at = 0;
+  for (const Request& q : r)
+    for (int i = 0; i < q.n; i++, at++) {
+      if (!groups || list->group[groups - 1].slot != q.slot || list->group[groups - 1].n == kGroupRows) list->group[groups++] = {q.slot, (int16_t)at, 0};
+      list->group[groups - 1].n++;
+      list->row[at] = (int16_t)(q.row + i);
+    }
+  return groups;
+}
+template <int kCap>
+int make_list(std::vector<Request> r, RunList<kCap>* list) {
+  std::stable_sort(r.begin(), r.end(), by_slot);
   list->n_pieces = (int)r.size();
   list->n_runs = 0;
   int at = 0, groups = 0;
   for (size_t i = 0; i < r.size(); i++) {
     if (i == 0 || r[i].slot != r[i - 1].slot) {
-      if (i) groups += (at - list->run_at[list->n_runs - 1] + group_rows - 1) / group_rows;
+      if (i) groups += (at - list->run_at[list->n_runs - 1] + kGroupRows - 1) / kGroupRows;
       list->slot[list->n_runs] = r[i].slot;
       list->run_at[list->n_runs] = at;
       list->group[list->n_runs++] = groups;
@@ -354,15 +391,15 @@ int make_list(std::vector<Request> r, int group_rows, List* list) {
     list->row[i] = r[i].row;
     at += r[i].n;
   }
-  groups += (at - list->run_at[list->n_runs - 1] + group_rows - 1) / group_rows;
+  groups += (at - list->run_at[list->n_runs - 1] + kGroupRows - 1) / kGroupRows;
   list->at[r.size()] = list->run_at[list->n_runs] = at;
   list->group[list->n_runs] = groups;
   return groups;
 }
 
-template <int kRank, int kMT, class List>
+template <int kRank, class List>
 int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int splits, bool x_bf16) {
-  constexpr size_t smem = (size_t)kLoraWarps * 16 * kMT * kRank * sizeof(float);
+  constexpr size_t smem = (size_t)kLoraWarps * kGroupRows * kRank * sizeof(float);
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
   const dim3 grid((unsigned)groups, (unsigned)splits);
   auto go = [&](auto kernel) -> int32_t {
@@ -372,49 +409,75 @@ int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups
     count_launch(p->dev);
     return RELUX_OK;
   };
-  return x_bf16 ? go(lora_down_kernel<kRank, kMT, true, List>) : go(lora_down_kernel<kRank, kMT, false, List>);
+  return x_bf16 ? go(lora_down_kernel<kRank, true, List>) : go(lora_down_kernel<kRank, false, List>);
 }
-template <int kRank, int kMT, class List>
+template <int kRank, class List>
 int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
   const dim3 grid((unsigned)groups, (unsigned)((prm.N + kUpCols - 1) / kUpCols));
   if (prm.part && prm.rg.in_turns())
-    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, kMT, true, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, true, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
   else
-    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, kMT, false, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, false, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
   count_launch(p->dev);
   return RELUX_OK;
 }
 
-// All launches of a call for one rank.  Groups of 16 rows; of calls of more than 512 rows, whose runs are long, of 64 (ranks 64 and 128: 32, what the sums of a
-// warp leave registers for).
-template <int kRank>
-int32_t run_lora(Pool* p, const relux_matmul_lora_args* a, const std::vector<Request>& requests, DownParams down, UpParams up, const WeightRef* w, const LayerScratch& sc,
-                 int t_splits) {
-  constexpr int kLong = kRank >= 64 ? 2 : 4;
-  const bool x_bf16 = a->x_dtype == RELUX_DTYPE_BF16, many = a->m > 512;
-  auto each = [&](auto&& launch) -> int32_t {   // by parts of up to kLargeList requests
-    for (size_t i = 0; i < requests.size(); i += kLargeList) {
-      std::vector<Request> part(requests.begin() + i, requests.begin() + std::min(requests.size(), i + kLargeList));
-      int32_t rc;
-      if (part.size() <= kSmallList) {
-        LoraList<kSmallList> list;
-        rc = launch(list, make_list(part, 16 * (many ? kLong : 1), &list));
-      } else {
-        LoraList<kLargeList> list;
-        rc = launch(list, make_list(part, 16 * (many ? kLong : 1), &list));
-      }
-      if (rc) return rc;
+// A call's lists, one launch each: of every row, or by parts of up to kLargeList requests.
+template <class Launch>
+int32_t for_lists(int M, const std::vector<Request>& requests, Launch launch) {
+  if (M <= kNarrowRows) {
+    RowList<kNarrowRows> list;
+    return launch(list, make_list(requests, &list));
+  }
+  if (M <= kSomeRows) {
+    RowList<kSomeRows> list;
+    return launch(list, make_list(requests, &list));
+  }
+  for (size_t i = 0; i < requests.size(); i += kLargeList) {
+    std::vector<Request> part(requests.begin() + i, requests.begin() + std::min(requests.size(), i + kLargeList));
+    int32_t rc;
+    if (part.size() <= kSmallList) {
+      RunList<kSmallList> list;
+      rc = launch(list, make_list(part, &list));
+    } else {
+      RunList<kLargeList> list;
+      rc = launch(list, make_list(part, &list));
     }
-    return RELUX_OK;
-  };
-  int32_t rc = each([&](const auto& list, int groups) {
-    return many ? launch_down<kRank, kLong>(p, down, list, groups, t_splits, x_bf16) : launch_down<kRank, 1>(p, down, list, groups, t_splits, x_bf16);
+    if (rc) return rc;
+  }
+  return RELUX_OK;
+}
+// Calls f with the rank as a constant.
+template <class F>
+int32_t with_rank(int rank, F f) {
+  switch (rank) {
+    case 8: return f(std::integral_constant<int, 8>());
+    case 16: return f(std::integral_constant<int, 16>());
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    default: return f(std::integral_constant<int, 128>());
+  }
+}
+int32_t run_down(Pool* p, int rank, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests, int splits) {
+  return with_rank(rank, [&](auto r) {
+    return for_lists(prm.M, requests, [&](const auto& list, int groups) { return launch_down<decltype(r)::value>(p, prm, list, groups, splits, x_bf16); });
   });
-  if (rc) return rc;
-  if (w)
-    if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
-  return each([&](const auto& list, int groups) { return many ? launch_up<kRank, kLong>(p, up, list, groups) : launch_up<kRank, 1>(p, up, list, groups); });
+}
+
+// Tiles of rows of one adapter for lora_gemm_kernel; false where they are too many, or would hold less than two thirds of rows (3000 rows of ... each: to be measured).
+bool make_tiles(int M, const std::vector<Request>& requests, LoraTiles* tiles) {
+  int64_t n = 0;
+  for (const Request& r : requests) n += (r.n + 127) / 128;
+  if (n > kMaxLoraTiles || 2 * 128 * n > 3 * (int64_t)std::max(M, 256)) return false;
+  tiles->n = 0;
+  for (const Request& r : requests)
+    for (int i = 0; i < r.n; i += 128) {
+      tiles->row[tiles->n] = r.row + i;
+      tiles->rows[tiles->n] = (int16_t)std::min(128, r.n - i);
+      tiles->slot[tiles->n++] = r.slot;
+    }
+  return true;
 }
 
 }  // namespace
@@ -449,16 +512,52 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     return RELUX_ERR_UNSUPPORTED;
   }
   const std::vector<Request> requests = merged_requests(a->n_seqs, a->n_rows, a->adapter);
-  // parts of K of t: enough blocks for the SMs, of 256 k at least (a step of every warp)
-  const int groups_least = (a->m + 15) / 16 + (int)requests.size() / 2;
-  const int t_splits = std::max(1, std::min({kMaxKSplit, p->dev->sm_count / groups_least, a->k / 256}));
+  const bool x_bf16 = a->x_dtype == RELUX_DTYPE_BF16;
+  DownParams down{};
+  down.factors = a->factors;
+  down.x = a->x;
+  down.a = (const uint16_t*)a->lora_a;
+  down.M = a->m;
+  down.K = a->k;
+  // parts of K of t: one block an SM, of 256 k at least, a step of every warp
+  const int groups = std::max<int>((int)std::min<size_t>(requests.size(), 1 << 20), a->m / kGroupRows);
+  const int t_splits = std::max(1, std::min({kMaxKSplit, p->dev->sm_count / groups, a->k / 256}));
+  const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // of a part, or of the two halves
+
+  const bool narrow = a->w && a->m <= kNarrowRows && a->n_slots <= 32767;
+  LoraTiles tiles;
+  const bool wide = a->w && !narrow && (int64_t)a->n_slots * a->n < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
+  if (narrow || wide) {
+    const size_t x_bytes = x_bf16 ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
+    if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes * (narrow ? t_splits : 1)))) return rc;
+    char* const base = (char*)p->layer_buf.p;
+    if (!x_bf16) down.x_bf16 = (uint16_t*)base;
+    if (narrow) {
+      down.t = (float*)(base + x_bytes);
+    } else {
+      down.t_hi = (uint16_t*)(base + x_bytes);
+      down.t_lo = down.t_hi + (size_t)a->m * a->rank;
+    }
+    if ((rc = run_down(p, a->rank, x_bf16, down, requests, narrow ? t_splits : 1))) return rc;
+    const uint16_t* x = x_bf16 ? (const uint16_t*)a->x : down.x_bf16;
+    if (wide) return launch_lora_gemm(p, a, x, nullptr, &tiles, nullptr, 1, down.t_hi, down.t_lo);
+    int16_t row_slots[kNarrowRows];
+    for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
+    return launch_lora_gemm(p, a, x, row_slots, nullptr, down.t, t_splits, nullptr, nullptr);
+  }
+
   LayerScratch sc;
-  const size_t t_bytes = (size_t)t_splits * a->m * a->rank * sizeof(float);
-  if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes, &sc))) return rc;
-  DownParams down{a->x, a->w && a->x_dtype == RELUX_DTYPE_F32 ? sc.a_bf16 : nullptr, (const uint16_t*)a->lora_a, (float*)sc.rest, a->m, a->k};
+  if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes * t_splits, &sc))) return rc;
+  if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
+  down.t = (float*)sc.rest;
+  if ((rc = run_down(p, a->rank, x_bf16, down, requests, t_splits))) return rc;
   UpParams up{};
-  up.part = a->w ? sc.part : nullptr;
-  up.t = (const float*)sc.rest;
+  if (a->w) {
+    const WeightRef w{a->w, a->n};
+    if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
+    up.part = sc.part;
+  }
+  up.t = down.t;
   up.b = (const uint16_t*)a->lora_b;
   up.factors = a->factors;
   up.out = a->out;
@@ -467,15 +566,9 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   up.t_splits = t_splits;
   up.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
   up.adds = a->accumulate != 0;
-  const WeightRef w{a->w, a->n};
-  const WeightRef* shared = a->w ? &w : nullptr;
-  switch (a->rank) {
-    case 8: return run_lora<8>(p, a, requests, down, up, shared, sc, t_splits);
-    case 16: return run_lora<16>(p, a, requests, down, up, shared, sc, t_splits);
-    case 32: return run_lora<32>(p, a, requests, down, up, shared, sc, t_splits);
-    case 64: return run_lora<64>(p, a, requests, down, up, shared, sc, t_splits);
-    default: return run_lora<128>(p, a, requests, down, up, shared, sc, t_splits);
-  }
+  return with_rank(a->rank, [&](auto r) {
+    return for_lists(a->m, requests, [&](const auto& list, int groups) { return launch_up<decltype(r)::value>(p, up, list, groups); });
+  });
 }
 
 }  // namespace relux

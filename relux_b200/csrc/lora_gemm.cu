@@ -1,0 +1,424 @@
+// The shared projection of a call with low-rank adapters, C[m] = x[m] W + t[m] B_s^T, s the adapter of row m, in one launch behind lora_down_kernel
+// (lora.cu), which takes t = f_s x A_s^T.  x and W are bf16, W as the layers hold it ([K][N]: MN-major in the MMA), B_s [N][rank].  Tiles as in tile_gemm.cuh.
+//
+//   * Up to 128 rows (bound: HBM, W and the adapters in use): the epilogue's warps, idle while W streams, take t B_s^T on the CUDA cores in
+//     float32, a thread a column, and add it to the sums when they come: a row meets its own adapter only.
+//   * Wide tiles (bound: the tensor cores): every tile holds rows of one request, so that t B_s^T is further K steps of the same accumulator, t as two
+//     bf16 halves, hi and lo.  Rows of the tile past the request's end are computed with the wrong adapter and not stored.
+//     A row never meets another request's adapter by way of a zero: zero times an infinity in that adapter would be NaN in this row.
+// W may be read ahead of the launch before this one, and bf16 x too: lora_down_kernel is a chain's head (launch_chained).
+#include "lora.cuh"
+#include "tile_gemm.cuh"
+
+namespace relux {
+
+namespace {
+
+constexpr int kRowsT = 16 << 10;   // bytes of t of the rows that the epilogue has at hand at a time
+template <int NC>
+using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT, NC + 8>;   // the adapter's part of a slice lies with the others'
+static_assert(slices_fit(16, 1, 8, 1, LoraShape<16>::kSlices) && slices_fit(32, 1, 8, 1, LoraShape<32>::kSlices) && slices_fit(64, 1, 8, 1, LoraShape<64>::kSlices) &&
+              slices_fit(128, 1, 8, 1, LoraShape<128>::kSlices) && slices_fit(256, 32, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage) &&
+              slices_fit(256, 64, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage), "no room for the slices");
+
+struct LoraMaps {
+  CUtensorMap x;      // [M][K], box 64 k x the rows of an operand
+  CUtensorMap w;      // [K][N], box 64 n x 64 k
+  CUtensorMap t[2];   // wide: hi and lo [M][rank], box 64 x 128 rows, zeros past the rank
+  CUtensorMap b;      // wide: [slots * N][rank], box 64 x 256 rows
+  CUtensorMap out;    // wide: rows of two-byte elements, two for a float32
+};
+struct LoraGemmParams {
+  int32_t M, N, rank, steps, tiles, col_tiles, out_bf16, adds;
+  int32_t x_early;           // x is the caller's: complete before the chain's head began
+  const float* t;            // narrow: [split][M][rank]
+  int32_t t_splits;
+  const uint16_t* b;         // narrow: [slots][N][rank]
+  const float* factors;      // narrow: [slots], or nullptr
+  void* out;
+  int32_t* status;
+};
+struct NarrowRows {
+  int16_t slot[kNarrowRows];   // of every row, or -1
+};
+
+template <int NC, class Rows>
+__global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant__ LoraMaps maps, const __grid_constant__ LoraGemmParams prm, const __grid_constant__ Rows list) {
+  using SH = LoraShape<NC>;
+  constexpr int kStages = SH::kStages;
+  constexpr bool kWide = SH::kWide;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* const out_tiles = smem + kStages * SH::kStage;
+  uint8_t* const slices = kWide ? smem : out_tiles + SH::kOut;
+  float* const t_rows = reinterpret_cast<float*>(out_tiles + SH::kOut + SH::kSlices);
+  TileBars* bars = reinterpret_cast<TileBars*>(out_tiles + SH::kOut + SH::kSlices + SH::kMore);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int size = (int)cluster_size(), rank = (int)cluster_ctarank();
+  const int first = blockIdx.x / size, stride = gridDim.x / size;
+  const int t_steps = (prm.rank + 63) / 64;   // of one half of t
+  // place of a tile, its rows and its steps of K
+  struct Place {
+    int c, row0, rows, slot, k0, k1;
+  };
+  auto place = [&](int tile) {
+    Place at;
+    if constexpr (kWide) {
+      int r;
+      wide_place(tile, list.n, prm.col_tiles, r, at.c);
+      at.row0 = list.row[r];
+      at.rows = list.rows[r];
+      at.slot = list.slot[r];
+    } else {
+      at.c = tile;
+      at.row0 = 0;
+      at.rows = prm.M;
+      at.slot = -1;
+    }
+    const int steps = prm.steps + (at.slot >= 0 ? 2 * t_steps : 0);
+    at.k0 = rank * steps / size;
+    at.k1 = (rank + 1) * steps / size;
+    return at;
+  };
+  chain_release();
+  if ((smem_u32(smem) & 1023u) != 0) {   // (the same in every CTA)
+    chain_wait();
+    if (threadIdx.x == 0) set_status(prm.status, RELUX_ERR_UNSUPPORTED);
+    return;
+  }
+  const uint32_t tmem = tile_setup<SH>(bars, size);
+
+  if (warp == 4) {
+    const bool el = elect_one();
+    if (el) {
+      tma_prefetch_desc(&maps.x);
+      tma_prefetch_desc(&maps.w);
+    }
+    const int w_at = kWide ? kStageRows : 0, x_at = kWide ? 0 : kStageRows;   // the M operand comes first
+    auto load_w = [&](const Place& at, int k, int s) {   // W of one step; arms the stage for both operands (out-of-range parts of a box are zero-filled and still counted)
+      uint8_t* st = smem + s * SH::kStage + w_at;
+      mbar_expect_tx(&bars->full[s], SH::kStage);
+#pragma unroll
+      for (int i = 0; i < (kWide ? 4 : 2); i++) tma_load_2d(st + i * 8192, &maps.w, at.c * (kWide ? 256 : kRowsOp) + 64 * i, k * 64, &bars->full[s]);
+    };
+    auto load_x = [&](const Place& at, int k, int s) { tma_load_2d(smem + s * SH::kStage + x_at, &maps.x, k * 64, at.row0, &bars->full[s]); };
+    // W of the first steps ahead of the launch before this one, and x where it may be
+    bool waited = false;
+    auto wait_once = [&] {
+      if (!waited) chain_wait();
+      waited = true;
+    };
+    int g = 0, early = 0;
+    if (!prm.x_early && first < prm.tiles) {
+      const Place at = place(first);
+      for (int k = at.k0; k < min(at.k1, prm.steps) && early < kStages; k++, early++)
+        if (el) load_w(at, k, early);
+      __syncwarp();
+      wait_once();
+    }
+    for (int tile = first; tile < prm.tiles; tile += stride) {
+      const Place at = place(tile);
+      for (int k = at.k0; k < at.k1; k++, g++) {
+        const int s = g % kStages;
+        if (g >= kStages) tile_wait(&bars->empty[s], (g / kStages - 1) & 1, bars, prm.status);
+        if (k < prm.steps) {
+          if (el) {
+            if (g >= early) load_w(at, k, s);
+            load_x(at, k, s);
+          }
+        } else if constexpr (kWide) {
+          wait_once();   // t is the launch's before this one
+          if (el) {
+            const int e = k - prm.steps, half = e / t_steps, r = (e - half * t_steps) * 64;
+            uint8_t* st = smem + s * SH::kStage;
+            mbar_expect_tx(&bars->full[s], SH::kStage);
+            tma_load_2d(st, &maps.t[half], r, at.row0, &bars->full[s]);
+            tma_load_2d(st + kStageRows, &maps.b, r, at.slot * prm.N + at.c * 256, &bars->full[s]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 5) {
+    const bool el = elect_one();
+    const uint32_t idesc = make_idesc_bf16(kRowsOp, NC, !kWide, kWide), idesc_t = make_idesc_bf16(kRowsOp, NC, false, false);
+    int g = 0, piece = 0;
+    for (int tile = first; tile < prm.tiles; tile += stride, piece++) {
+      const Place at = place(tile);
+      const uint32_t d = tmem + (piece & 1) * SH::kAcc;
+      if (piece >= 2) tile_wait(&bars->acc_empty[piece & 1], ((piece >> 1) - 1) & 1, bars, prm.status);
+      tc_fence_after();
+      for (int k = at.k0; k < at.k1; k++, g++) {
+        const int s = g % kStages;
+        tile_wait(&bars->full[s], (g / kStages) & 1, bars, prm.status);
+        tc_fence_after();
+        if (el) {
+          const uint32_t st = smem_u32(smem + s * SH::kStage);
+          if (k < prm.steps) {
+            const uint64_t dW = make_desc_mnmajor_sw128(st + (kWide ? kStageRows : 0), 8192), dX = make_desc_kmajor_sw128(st + (kWide ? 0 : kStageRows));
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) {
+              const uint64_t w = dW + ((uint32_t)(kk * 2048) >> 4), x = dX + ((uint32_t)(kk * 32) >> 4);
+              umma_ss<1>(d, kWide ? x : w, kWide ? w : x, idesc, k != at.k0 || kk != 0);
+            }
+          } else if constexpr (kWide) {
+            const uint64_t dT = make_desc_kmajor_sw128(st), dB = make_desc_kmajor_sw128(st + kStageRows);
+            const int e = k - prm.steps, left = prm.rank - e % t_steps * 64;   // (of rank 8 the second half of the slice is zeros)
+            for (int kk = 0; kk < 4 && 16 * kk < left; kk++)
+              umma_ss<1>(d, dT + ((uint32_t)(kk * 32) >> 4), dB + ((uint32_t)(kk * 32) >> 4), idesc_t, k != at.k0 || kk != 0);
+          }
+          umma_commit<1>(&bars->empty[s]);
+        }
+        __syncwarp();
+      }
+      if (el) umma_commit<1>(&bars->acc_full[piece & 1]);
+      __syncwarp();
+    }
+  } else {
+    chain_wait();
+    int piece = 0, staged = 0;
+    for (int tile = first; tile < prm.tiles; tile += stride, piece++) {
+      const Place at = place(tile);
+      const int buf = piece & 1;
+      const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + buf * SH::kAcc;
+      const int cols = kWide ? min(256, prm.N - at.c * 256) : prm.M;   // of the N operand that exist
+      const int grain = !kWide ? 1 : prm.out_bf16 ? 64 : 32;
+      const int q0 = size > 1 ? slice_begin(rank, cols, grain, size) : 0, q1 = size > 1 ? slice_begin(rank + 1, cols, grain, size) : cols;
+      const float* const got = reinterpret_cast<const float*>(slices) + threadIdx.x;
+      if constexpr (!kWide) {
+        // t B_s^T of this CTA's rows, behind the slices of the others
+        const int n = at.c * kRowsOp + warp * 32 + lane;
+        const bool mine = n < prm.N;
+        float* const low = reinterpret_cast<float*>(slices) + (size - 1) * (q1 - q0) * kRowsOp + threadIdx.x;
+        const int batch = kRowsT / 4 / prm.rank;
+        for (int b0 = q0; b0 < q1; b0 += batch) {
+          const int b1 = min(q1, b0 + batch);
+          epilogue_sync();   // the batch before is done with
+          for (int i = threadIdx.x; i < (b1 - b0) * prm.rank / 4; i += 128) {
+            const int row = b0 + 4 * i / prm.rank, slot = list.slot[row];
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (slot >= 0) {
+              for (int s = 0; s < prm.t_splits; s++) {
+                const float4 u = load_chained(reinterpret_cast<const float4*>(prm.t + ((size_t)s * prm.M + b0) * prm.rank) + i);
+                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+              }
+              const float f = prm.factors ? load_chained(prm.factors + slot) : 1.f;
+              v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+            }
+            reinterpret_cast<float4*>(t_rows)[i] = v;
+          }
+          epilogue_sync();
+#pragma unroll 1
+          for (int q = b0; q < b1; q += 4) {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint16_t* b[4];
+            bool some[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int slot = q + i < b1 ? list.slot[q + i] : -1;
+              some[i] = slot >= 0 && mine;
+              b[i] = prm.b + ((size_t)max(slot, 0) * prm.N + (mine ? n : 0)) * prm.rank;
+            }
+#pragma unroll 2
+            for (int r = 0; r < prm.rank; r += 8) {
+              uint4 v[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) v[i] = some[i] ? load_chained(reinterpret_cast<const uint4*>(b[i] + r)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                if (some[i]) {
+                  const float4* t = reinterpret_cast<const float4*>(t_rows + (q + i - b0) * prm.rank + r);
+                  const float4 t0 = t[0], t1 = t[1];
+                  sum[i] = fmaf(t0.x, bf16_lo(v[i].x), sum[i]); sum[i] = fmaf(t0.y, bf16_hi(v[i].x), sum[i]);
+                  sum[i] = fmaf(t0.z, bf16_lo(v[i].y), sum[i]); sum[i] = fmaf(t0.w, bf16_hi(v[i].y), sum[i]);
+                  sum[i] = fmaf(t1.x, bf16_lo(v[i].z), sum[i]); sum[i] = fmaf(t1.y, bf16_hi(v[i].z), sum[i]);
+                  sum[i] = fmaf(t1.z, bf16_lo(v[i].w), sum[i]); sum[i] = fmaf(t1.w, bf16_hi(v[i].w), sum[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (q + i < b1) low[(q + i - q0) * kRowsOp] = sum[i];
+          }
+        }
+      }
+      tile_wait(&bars->acc_full[buf], (piece >> 1) & 1, bars, prm.status);
+      tc_fence_after();
+      const bool ok = !bars->abort_flag;
+      if (size > 1) swap_slices<SH>(acc, cols, grain, size, rank, slices);
+      if constexpr (!kWide) {
+        // thread = column; a warp writes 64 or 128 bytes of a row at once
+        const int n = at.c * kRowsOp + warp * 32 + lane;
+        const bool mine = n < prm.N;
+#pragma unroll 1
+        for (int q = q0; q < q1; q += 8) {
+          uint32_t v[8];
+          tmem_ld_32x32b_x8(acc + q, v);
+          const size_t to = (size_t)q * prm.N + n;
+          float before[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) before[i] = 0.f;
+          if (prm.adds)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (mine && q + i < q1)
+                before[i] = prm.out_bf16 ? f32_from_bf16_bits(load_chained(reinterpret_cast<const uint16_t*>(prm.out) + to + (size_t)i * prm.N))
+                                         : load_chained(reinterpret_cast<const float*>(prm.out) + to + (size_t)i * prm.N);
+          tmem_ld_wait();
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = ok ? __uint_as_float(v[i]) : 0.f;
+#pragma unroll 1
+          for (int s = 0; s < size; s++)   // the others' parts, then the adapter's
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (q + i < q1) x[i] += got[(s * (q1 - q0) + q - q0 + i) * kRowsOp];
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] += before[i];
+          if (prm.out_bf16) {
+            uint16_t* const dst = reinterpret_cast<uint16_t*>(prm.out) + to;
+#pragma unroll
+            for (int i = 0; i < 8; i++) store_if(dst + (size_t)i * prm.N, __bfloat16_as_ushort(__float2bfloat16_rn(x[i])), mine && q + i < q1);
+          } else {
+            float* const dst = reinterpret_cast<float*>(prm.out) + to;
+#pragma unroll
+            for (int i = 0; i < 8; i++) store_if(dst + (size_t)i * prm.N, x[i], mine && q + i < q1);
+          }
+        }
+      } else {
+        // thread = row: 32 (bf16: 64) columns at a time to a staging tile of the warp, 128-byte swizzle, and out by TMA, which leaves out what lies past the last
+        // column; of warps with rows past the request's end straight to the rows
+        uint8_t* const tiles = out_tiles + warp * 2 * 32 * kOutRow;
+        const int wide = prm.out_bf16 ? 64 : 32, m = warp * 32 + lane;
+        const bool whole = warp * 32 + 32 <= at.rows, mine = m < at.rows;
+#pragma unroll 1
+        for (int q = q0; q < q1; q += wide, staged += whole) {
+          uint8_t* const tile_smem = tiles + (staged & 1) * 32 * kOutRow;
+          if (whole) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store before the last has read its tile
+            __syncwarp();
+          }
+#pragma unroll 1
+          for (int h = 0; h < wide && q + h < q1; h += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(acc + q + h, v);
+            tmem_ld_wait();
+            float x[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[i] = ok ? __uint_as_float(v[i]) : 0.f;
+#pragma unroll 1
+            for (int s = 0; s < size - 1; s++)
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if (q + h + i < q1) x[i] += got[(s * (q1 - q0) + q + h - q0 + i) * kRowsOp];
+            const int col = at.c * 256 + q + h;
+            const size_t to = (size_t)(at.row0 + m) * prm.N + col;
+            if (prm.adds && mine)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                if (col + 8 * i < prm.N) {   // N is a multiple of 8
+                  if (prm.out_bf16) {
+                    const uint4 a = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(prm.out) + to) + i);
+                    x[8 * i] += bf16_lo(a.x); x[8 * i + 1] += bf16_hi(a.x); x[8 * i + 2] += bf16_lo(a.y); x[8 * i + 3] += bf16_hi(a.y);
+                    x[8 * i + 4] += bf16_lo(a.z); x[8 * i + 5] += bf16_hi(a.z); x[8 * i + 6] += bf16_lo(a.w); x[8 * i + 7] += bf16_hi(a.w);
+                  } else {
+                    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(prm.out) + to) + 2 * i;
+                    const float4 a = load_chained(src), b = load_chained(src + 1);
+                    x[8 * i] += a.x; x[8 * i + 1] += a.y; x[8 * i + 2] += a.z; x[8 * i + 3] += a.w;
+                    x[8 * i + 4] += b.x; x[8 * i + 5] += b.y; x[8 * i + 6] += b.z; x[8 * i + 7] += b.w;
+                  }
+                }
+            if (prm.out_bf16) {
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const uint4 y = make_uint4(round_bf16x2(x[8 * i], x[8 * i + 1]), round_bf16x2(x[8 * i + 2], x[8 * i + 3]), round_bf16x2(x[8 * i + 4], x[8 * i + 5]),
+                                           round_bf16x2(x[8 * i + 6], x[8 * i + 7]));
+                if (whole) *reinterpret_cast<uint4*>(tile_smem + swz128(lane, h / 8 + i)) = y;
+                else if (mine && col + 8 * i < prm.N) reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(prm.out) + to)[i] = y;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const float4 y = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                if (whole) *reinterpret_cast<float4*>(tile_smem + swz128(lane, i)) = y;
+                else if (mine && col + 4 * i < prm.N) reinterpret_cast<float4*>(reinterpret_cast<float*>(prm.out) + to)[i] = y;
+              }
+            }
+          }
+          if (whole) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&maps.out, (at.c * 256 + q) * (prm.out_bf16 ? 1 : 2), at.row0 + warp * 32, tile_smem);
+              tma_store_commit();
+            }
+            __syncwarp();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->acc_empty[buf]);
+    }
+    if constexpr (kWide) {
+      if (lane == 0) tma_store_wait_all();
+      __syncwarp();
+    }
+    fence_chained_writes();
+  }
+  tile_end<SH>(tmem, size);
+}
+
+template <int NC, class Rows>
+int32_t launch_rows(Pool* p, const LoraMaps& maps, const LoraGemmParams& prm, const Rows& rows) {
+  return launch_tiles<LoraShape<NC>>(p, lora_gemm_kernel<NC, Rows>, prm.tiles, prm.steps, maps, prm, rows);
+}
+
+}  // namespace
+
+int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t, int t_splits,
+                         const uint16_t* t_hi, const uint16_t* t_lo) {
+  LoraGemmParams prm{};
+  LoraMaps maps{};
+  const int M = a->m, K = a->k, N = a->n;
+  int nc = 16;
+  while (nc < M && nc < kNarrowRows) nc *= 2;
+  if (tiles) nc = 256;
+  prm.M = M;
+  prm.N = N;
+  prm.rank = a->rank;
+  prm.steps = (K + 63) / 64;
+  prm.col_tiles = (N + (tiles ? nc : kRowsOp) - 1) / (tiles ? nc : kRowsOp);
+  const int64_t count = (int64_t)prm.col_tiles * (tiles ? tiles->n : 1);
+  if (count * (prm.steps + 4) >= (int64_t)1 << 31) { set_error("a product of more than 2^31 steps"); return RELUX_ERR_UNSUPPORTED; }
+  prm.tiles = (int)count;
+  prm.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
+  prm.adds = a->accumulate != 0;
+  prm.x_early = a->x_dtype == RELUX_DTYPE_BF16;
+  prm.t = t;
+  prm.t_splits = t_splits;
+  prm.b = (const uint16_t*)a->lora_b;
+  prm.factors = a->factors;
+  prm.out = a->out;
+  prm.status = p->d_status;
+  bool made = make_tmap_2d(&maps.x, (void*)x, (uint64_t)M, (uint64_t)K, 64, tiles ? kRowsOp : nc) && make_tmap_2d(&maps.w, (void*)a->w, (uint64_t)K, (uint64_t)N, 64, 64);
+  if (tiles)
+    made = made && make_tmap_2d(&maps.t[0], (void*)t_hi, (uint64_t)M, (uint64_t)a->rank, 64, kRowsOp) &&
+           make_tmap_2d(&maps.t[1], (void*)t_lo, (uint64_t)M, (uint64_t)a->rank, 64, kRowsOp) &&
+           make_tmap_2d(&maps.b, (void*)a->lora_b, (uint64_t)a->n_slots * N, (uint64_t)a->rank, 64, 256) &&
+           make_tmap_2d(&maps.out, a->out, (uint64_t)M, (uint64_t)N * (prm.out_bf16 ? 1 : 2), kOutRow / 2, 32);
+  if (!made) {
+    set_error("tensor map for a projection with adapters could not be encoded");
+    return RELUX_ERR_CUDA;
+  }
+  if (tiles) return launch_rows<256>(p, maps, prm, *tiles);
+  NarrowRows rows;
+  std::copy(row_slots, row_slots + M, rows.slot);
+  std::fill(rows.slot + M, rows.slot + kNarrowRows, (int16_t)-1);
+  switch (nc) {
+    case 16: return launch_rows<16>(p, maps, prm, rows);
+    case 32: return launch_rows<32>(p, maps, prm, rows);
+    case 64: return launch_rows<64>(p, maps, prm, rows);
+    default: return launch_rows<128>(p, maps, prm, rows);
+  }
+}
+
+}  // namespace relux

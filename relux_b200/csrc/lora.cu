@@ -16,6 +16,7 @@
 #include "internal.h"
 #include "lora.cuh"
 #include "projection.cuh"
+#include "tile_gemm.cuh"
 
 namespace relux {
 
@@ -23,7 +24,7 @@ namespace {
 
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
-constexpr int kMaxKSplit = 8, kGroupRows = 16;
+constexpr int kMaxParts = 8, kGroupRows = 16;
 constexpr int kSomeRows = 512;                       // of up to so many rows a list names each
 constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
 
@@ -96,22 +97,24 @@ struct DownParams {
   const void* x;
   uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr
   const uint16_t* a;      // [slots][rank][K]
-  float* t;               // [split][M][rank]
+  float* t;               // [M][rank], without factors
   int32_t M, K;
 };
 
-// t[row][r] = sum over this block's part of K of x[row][k] A_s[r][k].  grid (groups, parts of K), 8 warps that take 32 k each in turn.  mma.sync: a group is a handful of
-// rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
+// t[row][r] = sum over k of x[row][k] A_s[r][k].  grid (groups, parts of K), the parts of a group a cluster, 8 warps that take 32 k each in turn.  mma.sync: a group is a
+// handful of rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
 template <int kRank, bool kXBf16, class List>
-__global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
+__global__ void __launch_bounds__(kLoraThreads, kRank <= 64 ? 2 : 1) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
   constexpr int kTiles = kRank / 8;
-  extern __shared__ __align__(16) float slabs[];   // [warp][16][kRank]
+  constexpr int kSlab = kGroupRows * kRank;
+  extern __shared__ __align__(16) float slabs[];   // [warp][16][kRank], then what the other parts send to the first one
   __shared__ int32_t rows[kGroupRows];
   // waits before it releases: the projection behind it may read its weights early (launch_chained, head of a chain)
   chain_wait();
   chain_release();
   const int slot = group_rows(list, blockIdx.x, rows);
-  if (slot < 0 && !p.x_bf16) return;
+  if (slot < 0 && !p.x_bf16) return;   // (the same in all parts)
+  if (slot >= 0 && gridDim.y > 1) cluster_arrive();
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
@@ -124,7 +127,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParam
   const uint16_t* const a = p.a + (size_t)max(slot, 0) * kRank * p.K;
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
 
-#pragma unroll(kRank <= 32 ? 4 : 2)
+#pragma unroll(kRank <= 32 ? 4 : 1)
   for (int s = s0 + warp; s < s1; s += kLoraWarps) {
     const int k = s * 32 + 8 * t;
     const bool in = k < p.K;   // K is a multiple of 8
@@ -156,8 +159,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParam
   }
   if constexpr (!kXBf16) fence_chained_writes();
   if (slot < 0) return;
-  // the warps' sums, in their order
-  constexpr int kSlab = kGroupRows * kRank;
+  // the warps' sums, then the parts', in their order
+  const int parts = gridDim.y, part = blockIdx.y;
   float* const mine = slabs + warp * kSlab;
 #pragma unroll
   for (int j = 0; j < kTiles; j++) {
@@ -165,22 +168,59 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParam
     *reinterpret_cast<float2*>(mine + (8 + g) * kRank + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kSlab / 4; i += kLoraThreads) {
-    const int row = rows[4 * i / kRank];
-    float4 sum = reinterpret_cast<const float4*>(slabs)[i];
+  constexpr int kEach = (kSlab / 4 + kLoraThreads - 1) / kLoraThreads;
+  float4 sum[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    const int i = threadIdx.x + e * kLoraThreads;
+    if (i >= kSlab / 4) continue;
+    sum[e] = reinterpret_cast<const float4*>(slabs)[i];
 #pragma unroll
     for (int w = 1; w < kLoraWarps; w++) {
       const float4 v = reinterpret_cast<const float4*>(slabs + w * kSlab)[i];
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+      sum[e].x += v.x; sum[e].y += v.y; sum[e].z += v.z; sum[e].w += v.w;
     }
+  }
+  if (parts > 1) {
+    float4* const inbox = reinterpret_cast<float4*>(slabs + kLoraWarps * kSlab);
+    cluster_wait();   // the first part has begun
+    if (part > 0)
+#pragma unroll
+      for (int e = 0; e < kEach; e++) {
+        const int i = threadIdx.x + e * kLoraThreads;
+        if (i >= kSlab / 4) continue;
+        const uint32_t to = mapa_u32(smem_u32(inbox + (part - 1) * (kSlab / 4) + i), 0u);
+        store_cluster(to, __float_as_uint(sum[e].x));
+        store_cluster(to + 4, __float_as_uint(sum[e].y));
+        store_cluster(to + 8, __float_as_uint(sum[e].z));
+        store_cluster(to + 12, __float_as_uint(sum[e].w));
+      }
+    cluster_arrive();
+    cluster_wait();
+    if (part > 0) return;
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+      const int i = threadIdx.x + e * kLoraThreads;
+      if (i >= kSlab / 4) continue;
+      for (int k = 0; k < parts - 1; k++) {
+        const float4 v = inbox[k * (kSlab / 4) + i];
+        sum[e].x += v.x; sum[e].y += v.y; sum[e].z += v.z; sum[e].w += v.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    const int i = threadIdx.x + e * kLoraThreads;
+    if (i >= kSlab / 4) continue;
+    const int row = rows[4 * i / kRank];
     if (row < 0) continue;
     if (p.t_hi) {
       uint2 hi, lo;
-      split_halves(sum, p.factors ? load_chained(p.factors + slot) : 1.f, hi, lo);
+      split_halves(sum[e], p.factors ? load_chained(p.factors + slot) : 1.f, hi, lo);
       *reinterpret_cast<uint2*>(p.t_hi + (size_t)row * kRank + 4 * i % kRank) = hi;
       *reinterpret_cast<uint2*>(p.t_lo + (size_t)row * kRank + 4 * i % kRank) = lo;
     } else {
-      *reinterpret_cast<float4*>(p.t + ((size_t)blockIdx.y * p.M + row) * kRank + 4 * i % kRank) = sum;
+      *reinterpret_cast<float4*>(p.t + (size_t)row * kRank + 4 * i % kRank) = sum[e];
     }
   }
   if (p.t_hi) fence_chained_writes();
@@ -189,11 +229,11 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const DownParam
 struct UpParams {
   const float* part;      // the GEMM's pieces [piece][M][N]; nullptr: no shared projection
   GemmRanges rg;
-  const float* t;         // [split][M][rank]
+  const float* t;         // [M][rank]
   const uint16_t* b;      // [slots][N][rank]
   const float* factors;   // [slots], or nullptr: ones
   void* out;
-  int32_t M, N, t_splits, out_bf16, adds;   // adds: to what out holds
+  int32_t M, N, out_bf16, adds;   // adds: to what out holds
 };
 
 // out[row][n] = sum of the GEMM's pieces (+ what out holds) + f_s sum over r of t[row][r] B_s[n][r].  grid (groups, blocks of 256 columns), 32 columns a warp: its four
@@ -281,12 +321,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
   if (slot >= 0) {
     for (int i = threadIdx.x; i < kGroupRows * kRank / 4; i += kLoraThreads) {
       const int at = 4 * i / kRank, r = 4 * i % kRank, row = rows[at];
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row >= 0)
-        for (int s = 0; s < p.t_splits; s++) {
-          const float4 u = load_chained(reinterpret_cast<const float4*>(p.t + ((size_t)s * p.M + row) * kRank + r));
-          v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-        }
+      const float4 v = row >= 0 ? load_chained(reinterpret_cast<const float4*>(p.t + (size_t)row * kRank + r)) : make_float4(0.f, 0.f, 0.f, 0.f);
       uint2 hi, lo;
       split_halves(v, factor, hi, lo);
       *reinterpret_cast<uint2*>(t_hi + at * kStride + r) = hi;
@@ -398,14 +433,25 @@ int make_list(std::vector<Request> r, RunList<kCap>* list) {
 }
 
 template <int kRank, class List>
-int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int splits, bool x_bf16) {
-  constexpr size_t smem = (size_t)kLoraWarps * kGroupRows * kRank * sizeof(float);
-  const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
-  const dim3 grid((unsigned)groups, (unsigned)splits);
+int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int parts, bool x_bf16) {
+  const size_t smem = (size_t)(kLoraWarps + parts - 1) * kGroupRows * kRank * sizeof(float);
   auto go = [&](auto kernel) -> int32_t {
     if (smem > 48 << 10)
       if (int32_t rc = allow_smem(p->dev, kernel, smem)) return rc;
-    RELUX_CUDA_TRY(launch_chained(chained, kernel, grid, dim3(kLoraThreads), smem, p->dev->stream, prm, list));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)groups, (unsigned)parts);
+    cfg.blockDim = dim3(kLoraThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = p->dev->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.y = (unsigned)parts;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0 ? 2 : 1;
+    RELUX_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, prm, list));
     count_launch(p->dev);
     return RELUX_OK;
   };
@@ -459,9 +505,13 @@ int32_t with_rank(int rank, F f) {
     default: return f(std::integral_constant<int, 128>());
   }
 }
-int32_t run_down(Pool* p, int rank, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests, int splits) {
+int32_t run_down(Pool* p, int rank, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests) {
   return with_rank(rank, [&](auto r) {
-    return for_lists(prm.M, requests, [&](const auto& list, int groups) { return launch_down<decltype(r)::value>(p, prm, list, groups, splits, x_bf16); });
+    return for_lists(prm.M, requests, [&](const auto& list, int groups) {
+      // parts of K: two blocks an SM, of 256 k at least, a step of every warp
+      const int parts = std::max(1, std::min({kMaxParts, 2 * p->dev->sm_count / groups, prm.K / 256}));
+      return launch_down<decltype(r)::value>(p, prm, list, groups, parts, x_bf16);
+    });
   });
 }
 
@@ -519,38 +569,36 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   down.a = (const uint16_t*)a->lora_a;
   down.M = a->m;
   down.K = a->k;
-  // parts of K of t: one block an SM, of 256 k at least, a step of every warp
-  const int groups = std::max<int>((int)std::min<size_t>(requests.size(), 1 << 20), a->m / kGroupRows);
-  const int t_splits = std::max(1, std::min({kMaxKSplit, p->dev->sm_count / groups, a->k / 256}));
-  const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // of a part, or of the two halves
+  const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
 
   const bool narrow = a->w && a->m <= kNarrowRows && a->n_slots <= 32767;
   LoraTiles tiles;
   const bool wide = a->w && !narrow && (int64_t)a->n_slots * a->n < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
   if (narrow || wide) {
-    const size_t x_bytes = x_bf16 ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
-    if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes * (narrow ? t_splits : 1)))) return rc;
+    const bool rounds = narrow && !x_bf16 && a->m <= kRoundedRows;
+    const size_t x_bytes = x_bf16 || rounds ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
+    if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes))) return rc;
     char* const base = (char*)p->layer_buf.p;
-    if (!x_bf16) down.x_bf16 = (uint16_t*)base;
+    if (!x_bf16 && !rounds) down.x_bf16 = (uint16_t*)base;
     if (narrow) {
       down.t = (float*)(base + x_bytes);
     } else {
       down.t_hi = (uint16_t*)(base + x_bytes);
       down.t_lo = down.t_hi + (size_t)a->m * a->rank;
     }
-    if ((rc = run_down(p, a->rank, x_bf16, down, requests, narrow ? t_splits : 1))) return rc;
+    if ((rc = run_down(p, a->rank, x_bf16, down, requests))) return rc;
     const uint16_t* x = x_bf16 ? (const uint16_t*)a->x : down.x_bf16;
-    if (wide) return launch_lora_gemm(p, a, x, nullptr, &tiles, nullptr, 1, down.t_hi, down.t_lo);
+    if (wide) return launch_lora_gemm(p, a, x, nullptr, &tiles, nullptr, down.t_hi, down.t_lo);
     int16_t row_slots[kNarrowRows];
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
-    return launch_lora_gemm(p, a, x, row_slots, nullptr, down.t, t_splits, nullptr, nullptr);
+    return launch_lora_gemm(p, a, x, row_slots, nullptr, down.t, nullptr, nullptr);
   }
 
   LayerScratch sc;
-  if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes * t_splits, &sc))) return rc;
+  if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes, &sc))) return rc;
   if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
   down.t = (float*)sc.rest;
-  if ((rc = run_down(p, a->rank, x_bf16, down, requests, t_splits))) return rc;
+  if ((rc = run_down(p, a->rank, x_bf16, down, requests))) return rc;
   UpParams up{};
   if (a->w) {
     const WeightRef w{a->w, a->n};
@@ -563,7 +611,6 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   up.out = a->out;
   up.M = a->m;
   up.N = a->n;
-  up.t_splits = t_splits;
   up.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
   up.adds = a->accumulate != 0;
   return with_rank(a->rank, [&](auto r) {

@@ -14,12 +14,16 @@ namespace relux {
 
 namespace {
 
+constexpr int kPrefetchSteps = 32;
 constexpr int kRowsT = 16 << 10;   // bytes of t of the rows that the epilogue has at hand at a time
 template <int NC>
 using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT, NC + 8>;   // the adapter's part of a slice lies with the others'
 static_assert(slices_fit(16, 1, 8, 1, LoraShape<16>::kSlices) && slices_fit(32, 1, 8, 1, LoraShape<32>::kSlices) && slices_fit(64, 1, 8, 1, LoraShape<64>::kSlices) &&
               slices_fit(128, 1, 8, 1, LoraShape<128>::kSlices) && slices_fit(256, 32, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage) &&
               slices_fit(256, 64, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage), "no room for the slices");
+
+template <int NC>
+constexpr int kLoraGemmThreads = NC == 256 ? 192 : 320;
 
 struct LoraMaps {
   CUtensorMap x;      // [M][K], box 64 k x the rows of an operand
@@ -31,8 +35,9 @@ struct LoraMaps {
 struct LoraGemmParams {
   int32_t M, N, rank, steps, tiles, col_tiles, out_bf16, adds;
   int32_t x_early;           // x is the caller's: complete before the chain's head began
-  const float* t;            // narrow: [split][M][rank]
-  int32_t t_splits;
+  const float* x_f32;        // up to 16 rows of float32: rounded here, into the stages [M][K]
+  int32_t K;
+  const float* t;            // narrow: [M][rank], without factors
   const uint16_t* b;         // narrow: [slots][N][rank]
   const float* factors;      // narrow: [slots], or nullptr
   void* out;
@@ -43,7 +48,7 @@ struct NarrowRows {
 };
 
 template <int NC, class Rows>
-__global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant__ LoraMaps maps, const __grid_constant__ LoraGemmParams prm, const __grid_constant__ Rows list) {
+__global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(const __grid_constant__ LoraMaps maps, const __grid_constant__ LoraGemmParams prm, const __grid_constant__ Rows list) {
   using SH = LoraShape<NC>;
   constexpr int kStages = SH::kStages;
   constexpr bool kWide = SH::kWide;
@@ -85,18 +90,92 @@ __global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant
     if (threadIdx.x == 0) set_status(prm.status, RELUX_ERR_UNSUPPORTED);
     return;
   }
-  const uint32_t tmem = tile_setup<SH>(bars, size);
+  const bool rounds_x = NC == 16 && prm.x_f32;
+  const uint32_t tmem = tile_setup<SH>(bars, size, rounds_x ? 5 : 1);
+
+  bool has_t = false;
+  auto low_sync = [] { asm volatile("bar.sync 2, 256;" ::: "memory"); };
+  auto low_wait = [&] {
+    if (!has_t) chain_wait();
+    has_t = true;
+    low_sync();   // the tile before is done with t
+  };
+  // Up to 128 rows: t B_s^T of a tile and this CTA's rows, behind the slices of the others.  By the epilogue's warps (half 0) and the helpers (half 1), a thread a
+  // column, blocks of eight rows in turn: eight of every row's rank
+  // are loaded while the two pieces before them are multiplied, the first two ahead of t.
+  auto low_half = [&](const Place& at, int half) {
+    const int id = half ? threadIdx.x - 192 : threadIdx.x, n = at.c * kRowsOp + id;
+    const int q0 = size > 1 ? slice_begin(rank, prm.M, 1, size) : 0, q1 = size > 1 ? slice_begin(rank + 1, prm.M, 1, size) : prm.M;
+    const bool mine = n < prm.N;
+    float* const low = reinterpret_cast<float*>(slices) + (size - 1) * (q1 - q0) * kRowsOp + id;
+    const int batch = kRowsT / 4 / prm.rank;   // rows whose t is at hand, a multiple of 16
+    for (int b0 = q0; b0 < q1; b0 += batch) {
+      const int b1 = min(q1, b0 + batch), blocks = (b1 - b0 + 7) / 8, chunks = prm.rank / 8, count = (blocks + 1 - half) / 2 * chunks;
+      uint4 v[3][8];
+      auto row_of = [&](int i) { return b0 + (i / chunks * 2 + half) * 8; };
+      auto load = [&](int i, uint4 (&w)[8]) {
+        const int q = row_of(i), r = i % chunks * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int slot = q + j < b1 ? list.slot[q + j] : -1;
+          const uint4* src = reinterpret_cast<const uint4*>(prm.b + ((size_t)max(slot, 0) * prm.N + (mine ? n : 0)) * prm.rank + r);
+          w[j] = slot >= 0 && mine ? load_chained(src) : make_uint4(0u, 0u, 0u, 0u);
+        }
+      };
+      auto multiply = [&](int i, const uint4 (&w)[8]) {
+        const int q = row_of(i), r = i % chunks * 8;
+        float sum[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          sum[j] = r && q + j < b1 ? low[(q + j - q0) * kRowsOp] : 0.f;
+          const float4* t = reinterpret_cast<const float4*>(t_rows + (min(q + j, b1 - 1) - b0) * prm.rank + r);   // of a row without an adapter zeros, as its w
+          const float4 t0 = t[0], t1 = t[1];
+          sum[j] = fmaf(t0.x, bf16_lo(w[j].x), sum[j]); sum[j] = fmaf(t0.y, bf16_hi(w[j].x), sum[j]);
+          sum[j] = fmaf(t0.z, bf16_lo(w[j].y), sum[j]); sum[j] = fmaf(t0.w, bf16_hi(w[j].y), sum[j]);
+          sum[j] = fmaf(t1.x, bf16_lo(w[j].z), sum[j]); sum[j] = fmaf(t1.y, bf16_hi(w[j].z), sum[j]);
+          sum[j] = fmaf(t1.z, bf16_lo(w[j].w), sum[j]); sum[j] = fmaf(t1.w, bf16_hi(w[j].w), sum[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (q + j < b1) low[(q + j - q0) * kRowsOp] = sum[j];
+      };
+      if (count > 0) load(0, v[0]);   // adapters were complete before the chain's head began
+      if (count > 1) load(1, v[1]);
+      if (b0 == q0) low_wait();
+      else low_sync();                // the batch before is done with
+      for (int i = threadIdx.x - (half ? 64 : 0); i < (b1 - b0) * prm.rank / 4; i += 256) {
+        const int slot = list.slot[b0 + 4 * i / prm.rank];
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (slot >= 0) {
+          u = load_chained(reinterpret_cast<const float4*>(prm.t + (size_t)b0 * prm.rank) + i);
+          const float f = prm.factors ? load_chained(prm.factors + slot) : 1.f;
+          u.x *= f; u.y *= f; u.z *= f; u.w *= f;
+        }
+        reinterpret_cast<float4*>(t_rows)[i] = u;
+      }
+      low_sync();
+#pragma unroll 1
+      for (int i = 0; i < count; i += 3)
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          if (i + k < count) {
+            if (i + k + 2 < count) load(i + k + 2, v[(k + 2) % 3]);
+            multiply(i + k, v[k]);
+          }
+    }
+    low_sync();
+  };
 
   if (warp == 4) {
     const bool el = elect_one();
     if (el) {
-      tma_prefetch_desc(&maps.x);
+      if (!rounds_x) tma_prefetch_desc(&maps.x);
       tma_prefetch_desc(&maps.w);
     }
     const int w_at = kWide ? kStageRows : 0, x_at = kWide ? 0 : kStageRows;   // the M operand comes first
     auto load_w = [&](const Place& at, int k, int s) {   // W of one step; arms the stage for both operands (out-of-range parts of a box are zero-filled and still counted)
       uint8_t* st = smem + s * SH::kStage + w_at;
-      mbar_expect_tx(&bars->full[s], SH::kStage);
+      mbar_expect_tx(&bars->full[s], rounds_x ? kStageRows : SH::kStage);
 #pragma unroll
       for (int i = 0; i < (kWide ? 4 : 2); i++) tma_load_2d(st + i * 8192, &maps.w, at.c * (kWide ? 256 : kRowsOp) + 64 * i, k * 64, &bars->full[s]);
     };
@@ -110,8 +189,14 @@ __global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant
     int g = 0, early = 0;
     if (!prm.x_early && first < prm.tiles) {
       const Place at = place(first);
-      for (int k = at.k0; k < min(at.k1, prm.steps) && early < kStages; k++, early++)
+      int k = at.k0;
+      for (; k < min(at.k1, prm.steps) && early < kStages; k++, early++)
         if (el) load_w(at, k, early);
+      // and to L2 what there are no stages for (a prefetch returns no data, so it could be early anyway)
+      for (int ahead = 0; k < min(at.k1, prm.steps) && ahead < kPrefetchSteps; k++, ahead++)
+        if (el)
+#pragma unroll
+          for (int i = 0; i < (kWide ? 4 : 2); i++) tma_prefetch_2d(&maps.w, at.c * (kWide ? 256 : kRowsOp) + 64 * i, k * 64);
       __syncwarp();
       wait_once();
     }
@@ -123,7 +208,7 @@ __global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant
         if (k < prm.steps) {
           if (el) {
             if (g >= early) load_w(at, k, s);
-            load_x(at, k, s);
+            if (!rounds_x) load_x(at, k, s);
           }
         } else if constexpr (kWide) {
           wait_once();   // t is the launch's before this one
@@ -173,8 +258,43 @@ __global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant
       if (el) umma_commit<1>(&bars->acc_full[piece & 1]);
       __syncwarp();
     }
+  } else if (!kWide && warp >= 6) {
+    // helpers: the rounding of few float32 rows, and half of t B_s^T
+    const int id = threadIdx.x - 192;
+    int g = 0;
+    for (int tile = first; tile < prm.tiles; tile += stride) {
+      const Place at = place(tile);
+      if (rounds_x) {   // thread: eight k of a row, four steps' loads on their way together
+        const int row = id >> 3, chunk = id & 7;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = at.k0; k < at.k1; k += 4) {
+          float4 u[4], v[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int col = (k + i) * 64 + 8 * chunk;
+            const bool in = k + i < at.k1 && row < prm.M && col < prm.K;   // K is a multiple of 8
+            const float4* src = reinterpret_cast<const float4*>(prm.x_f32 + (size_t)(in ? row : 0) * prm.K + (in ? col : 0));
+            u[i] = in ? load_chained(src) : zero;
+            v[i] = in ? load_chained(src + 1) : zero;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (k + i < at.k1) {
+              const int s = g % kStages;
+              if (g >= kStages) tile_wait(&bars->empty[s], (g / kStages - 1) & 1, bars, prm.status);
+              *reinterpret_cast<uint4*>(smem + s * SH::kStage + kStageRows + swz128(row, chunk)) =
+                  make_uint4(round_bf16x2(u[i].x, u[i].y), round_bf16x2(u[i].z, u[i].w), round_bf16x2(v[i].x, v[i].y), round_bf16x2(v[i].z, v[i].w));
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars->full[s]);
+              g++;
+            }
+        }
+      }
+      low_half(at, 1);
+    }
   } else {
-    chain_wait();
+    if constexpr (kWide) chain_wait();
     int piece = 0, staged = 0;
     for (int tile = first; tile < prm.tiles; tile += stride, piece++) {
       const Place at = place(tile);
@@ -184,62 +304,7 @@ __global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant
       const int grain = !kWide ? 1 : prm.out_bf16 ? 64 : 32;
       const int q0 = size > 1 ? slice_begin(rank, cols, grain, size) : 0, q1 = size > 1 ? slice_begin(rank + 1, cols, grain, size) : cols;
       const float* const got = reinterpret_cast<const float*>(slices) + threadIdx.x;
-      if constexpr (!kWide) {
-        // t B_s^T of this CTA's rows, behind the slices of the others
-        const int n = at.c * kRowsOp + warp * 32 + lane;
-        const bool mine = n < prm.N;
-        float* const low = reinterpret_cast<float*>(slices) + (size - 1) * (q1 - q0) * kRowsOp + threadIdx.x;
-        const int batch = kRowsT / 4 / prm.rank;
-        for (int b0 = q0; b0 < q1; b0 += batch) {
-          const int b1 = min(q1, b0 + batch);
-          epilogue_sync();   // the batch before is done with
-          for (int i = threadIdx.x; i < (b1 - b0) * prm.rank / 4; i += 128) {
-            const int row = b0 + 4 * i / prm.rank, slot = list.slot[row];
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (slot >= 0) {
-              for (int s = 0; s < prm.t_splits; s++) {
-                const float4 u = load_chained(reinterpret_cast<const float4*>(prm.t + ((size_t)s * prm.M + b0) * prm.rank) + i);
-                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-              }
-              const float f = prm.factors ? load_chained(prm.factors + slot) : 1.f;
-              v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-            }
-            reinterpret_cast<float4*>(t_rows)[i] = v;
-          }
-          epilogue_sync();
-#pragma unroll 1
-          for (int q = b0; q < b1; q += 4) {
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint16_t* b[4];
-            bool some[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const int slot = q + i < b1 ? list.slot[q + i] : -1;
-              some[i] = slot >= 0 && mine;
-              b[i] = prm.b + ((size_t)max(slot, 0) * prm.N + (mine ? n : 0)) * prm.rank;
-            }
-#pragma unroll 2
-            for (int r = 0; r < prm.rank; r += 8) {
-              uint4 v[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) v[i] = some[i] ? load_chained(reinterpret_cast<const uint4*>(b[i] + r)) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-              for (int i = 0; i < 4; i++)
-                if (some[i]) {
-                  const float4* t = reinterpret_cast<const float4*>(t_rows + (q + i - b0) * prm.rank + r);
-                  const float4 t0 = t[0], t1 = t[1];
-                  sum[i] = fmaf(t0.x, bf16_lo(v[i].x), sum[i]); sum[i] = fmaf(t0.y, bf16_hi(v[i].x), sum[i]);
-                  sum[i] = fmaf(t0.z, bf16_lo(v[i].y), sum[i]); sum[i] = fmaf(t0.w, bf16_hi(v[i].y), sum[i]);
-                  sum[i] = fmaf(t1.x, bf16_lo(v[i].z), sum[i]); sum[i] = fmaf(t1.y, bf16_hi(v[i].z), sum[i]);
-                  sum[i] = fmaf(t1.z, bf16_lo(v[i].w), sum[i]); sum[i] = fmaf(t1.w, bf16_hi(v[i].w), sum[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (q + i < b1) low[(q + i - q0) * kRowsOp] = sum[i];
-          }
-        }
-      }
+      if constexpr (!kWide) low_half(at, 0);
       tile_wait(&bars->acc_full[buf], (piece >> 1) & 1, bars, prm.status);
       tc_fence_after();
       const bool ok = !bars->abort_flag;
@@ -369,12 +434,12 @@ __global__ void __launch_bounds__(192, 1) lora_gemm_kernel(const __grid_constant
 
 template <int NC, class Rows>
 int32_t launch_rows(Pool* p, const LoraMaps& maps, const LoraGemmParams& prm, const Rows& rows) {
-  return launch_tiles<LoraShape<NC>>(p, lora_gemm_kernel<NC, Rows>, prm.tiles, prm.steps, maps, prm, rows);
+  return launch_tiles<LoraShape<NC>, kLoraGemmThreads<NC>>(p, lora_gemm_kernel<NC, Rows>, prm.tiles, prm.steps, maps, prm, rows);
 }
 
 }  // namespace
 
-int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t, int t_splits,
+int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t,
                          const uint16_t* t_hi, const uint16_t* t_lo) {
   LoraGemmParams prm{};
   LoraMaps maps{};
@@ -392,14 +457,15 @@ int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_
   prm.tiles = (int)count;
   prm.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
   prm.adds = a->accumulate != 0;
-  prm.x_early = a->x_dtype == RELUX_DTYPE_BF16;
+  prm.x_early = a->x_dtype == RELUX_DTYPE_BF16 || !x;
+  prm.x_f32 = x ? nullptr : (const float*)a->x;
+  prm.K = K;
   prm.t = t;
-  prm.t_splits = t_splits;
   prm.b = (const uint16_t*)a->lora_b;
   prm.factors = a->factors;
   prm.out = a->out;
   prm.status = p->d_status;
-  bool made = make_tmap_2d(&maps.x, (void*)x, (uint64_t)M, (uint64_t)K, 64, tiles ? kRowsOp : nc) && make_tmap_2d(&maps.w, (void*)a->w, (uint64_t)K, (uint64_t)N, 64, 64);
+  bool made = (!x || make_tmap_2d(&maps.x, (void*)x, (uint64_t)M, (uint64_t)K, 64, tiles ? kRowsOp : nc)) && make_tmap_2d(&maps.w, (void*)a->w, (uint64_t)K, (uint64_t)N, 64, 64);
   if (tiles)
     made = made && make_tmap_2d(&maps.t[0], (void*)t_hi, (uint64_t)M, (uint64_t)a->rank, 64, kRowsOp) &&
            make_tmap_2d(&maps.t[1], (void*)t_lo, (uint64_t)M, (uint64_t)a->rank, 64, kRowsOp) &&

@@ -89,11 +89,11 @@ __device__ __forceinline__ void cluster_wait() {
 __device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// Barriers and tensor memory of a CTA of 192 threads (warp 0 allocates); returns the base of tensor memory.
+// Barriers and tensor memory of a CTA (warp 0 allocates); returns the base of tensor memory.  fills: arrivals that fill a stage, TMA's among them.
 template <class SH>
-__device__ __forceinline__ uint32_t tile_setup(TileBars* bars, int size) {
+__device__ __forceinline__ uint32_t tile_setup(TileBars* bars, int size, int fills = 1) {
   if (threadIdx.x == 0) {
-    for (int s = 0; s < SH::kStages; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+    for (int s = 0; s < SH::kStages; s++) { mbar_init(&bars->full[s], fills); mbar_init(&bars->empty[s], 1); }
     for (int b = 0; b < 2; b++) { mbar_init(&bars->acc_full[b], 1); mbar_init(&bars->acc_empty[b], 4); }
     bars->abort_flag = 0;
     fence_mbar_init();
@@ -161,11 +161,11 @@ __device__ __forceinline__ void wide_place(int tile, int row_blocks, int col_til
 
 // Launches `kernel` over `tiles` tiles.  As many CTAs to a tile as leave every tile a cluster that is resident at once: a cluster lies within one of the
 // GPU's groups of SMs, so there are fewer of them than SMs / size (74 of two, 45 of three, 33 of four).
-template <class SH, typename... KArgs, typename... Args>
+template <class SH, int kThreads = 192, typename... KArgs, typename... Args>
 int32_t launch_tiles(Pool* p, void (*kernel)(KArgs...), int tiles, int steps, const Args&... args) {
   if (int32_t rc = allow_smem(p->dev, kernel, SH::kSmem)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = SH::kSmem;
   cfg.stream = p->dev->stream;
   cudaLaunchAttribute at[2];

@@ -515,12 +515,16 @@ int32_t ensure_rope_table(Pool* p, int dHR, float base, int positions) {
   return RELUX_OK;
 }
 
+}  // namespace
+
 int32_t launch_cast(Pool* p, const float* src, uint16_t* dst, size_t n) {
   RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, cast_bf16_kernel, dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0,
                                 p->dev->stream, src, dst, n / 8));
   count_launch(p->dev);
   return RELUX_OK;
 }
+
+namespace {
 
 // x [M][K] f32 -> every segment's buffer: cast + split-K tensor-core GEMM (or the reference-order GEMM), then the
 // finish kernel.  The GEMM's device time goes to the pool's projection ring.

@@ -25,13 +25,14 @@ namespace {
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
 constexpr int kMaxParts = 8, kGroupRows = 16;
-constexpr int kSomeRows = 512;                       // of up to so many rows a list names each
+constexpr int kFewRows = 128, kSomeRows = 512;       // of up to so many rows a list names each
 constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
 
 // The rows of a call (or of a part of it), in the order of their adapters, cut into groups of one adapter.
 // Of few rows: every group and its rows.
 template <int kCap>
 struct RowList {
+  static constexpr bool kNamesRows = true;
   struct Group {
     int32_t slot;        // adapter, or -1
     int16_t first, n;    // its rows' places
@@ -42,6 +43,7 @@ struct RowList {
 // Of many: a piece is a range of neighbouring rows of one adapter, a run all the pieces of one; groups are cut within runs, all but a run's last of full size.
 template <int kCap>
 struct RunList {
+  static constexpr bool kNamesRows = false;
   int32_t n_pieces, n_runs;
   int32_t at[kCap + 1];      // first place, in this order, of a piece
   int32_t row[kCap];         // its first row
@@ -98,36 +100,45 @@ struct DownParams {
   uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr
   const uint16_t* a;      // [slots][rank][K]
   float* t;               // [M][rank], without factors
-  int32_t M, K;
+  int32_t M, K, rank;
 };
 
-// t[row][r] = sum over k of x[row][k] A_s[r][k].  grid (groups, parts of K), the parts of a group a cluster, 8 warps that take 32 k each in turn.  mma.sync: a group is a
+// t[row][r] = sum over k of x[row][k] A_s[r][k].  grid (groups, parts of K, kSlice-th parts of the rank), the parts of K a cluster, 8 warps that take 32 k each in turn.  mma.sync: a group is a
 // handful of rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
-template <int kRank, bool kXBf16, class List>
-__global__ void __launch_bounds__(kLoraThreads, kRank <= 64 ? 2 : 1) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
-  constexpr int kTiles = kRank / 8;
-  constexpr int kSlab = kGroupRows * kRank;
-  extern __shared__ __align__(16) float slabs[];   // [warp][16][kRank], then what the other parts send to the first one
+template <int kSlice, bool kXBf16, class List>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
+  constexpr int kTiles = kSlice / 8;
+  constexpr int kSlab = kGroupRows * kSlice;
+  extern __shared__ __align__(16) float slabs[];   // [warp][16][kSlice], then what the other parts send to the first one
   __shared__ int32_t rows[kGroupRows];
+  const int slot = group_rows(list, blockIdx.x, rows);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
+  const int r0 = blockIdx.z * kSlice;
+  const uint16_t* const a = p.a + ((size_t)max(slot, 0) * p.rank + r0) * p.K;
+  const bool rounds = p.x_bf16 && r0 == 0;
+  if (slot >= 0)   // the adapter's first pieces to L2, while the launch before this one ends (a prefetch returns no data, so it may be early)
+    for (int s = s0 + warp; s < min(s1, s0 + 4 * kLoraWarps); s += kLoraWarps) {
+      const int k = s * 32 + 8 * t;
+      if (t == 0 && k < p.K)
+#pragma unroll
+        for (int j = 0; j < kTiles; j++) asm volatile("prefetch.global.L2 [%0];" ::"l"(a + (size_t)(8 * j + g) * p.K + k));
+    }
   // waits before it releases: the projection behind it may read its weights early (launch_chained, head of a chain)
   chain_wait();
   chain_release();
-  const int slot = group_rows(list, blockIdx.x, rows);
-  if (slot < 0 && !p.x_bf16) return;   // (the same in all parts)
+  if (slot < 0 && !rounds) return;   // (the same in all parts)
   if (slot >= 0 && gridDim.y > 1) cluster_arrive();
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
   const int32_t r[2] = {rows[g], rows[8 + g]};
   float acc[kTiles][4];
 #pragma unroll
   for (int j = 0; j < kTiles; j++)
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[j][i] = 0.f;
-  const uint16_t* const a = p.a + (size_t)max(slot, 0) * kRank * p.K;
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
 
-#pragma unroll(kRank <= 32 ? 4 : 1)
+#pragma unroll(kSlice <= 32 ? 4 : 1)
   for (int s = s0 + warp; s < s1; s += kLoraWarps) {
     const int k = s * 32 + 8 * t;
     const bool in = k < p.K;   // K is a multiple of 8
@@ -145,7 +156,7 @@ __global__ void __launch_bounds__(kLoraThreads, kRank <= 64 ? 2 : 1) lora_down_k
         const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), u = there ? load_chained(src) : zero, v = there ? load_chained(src + 1) : zero;
         x[h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
-        if (there && p.x_bf16) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[h];
+        if (there && rounds) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[h];
       }
     }
     if (slot >= 0) {
@@ -164,8 +175,8 @@ __global__ void __launch_bounds__(kLoraThreads, kRank <= 64 ? 2 : 1) lora_down_k
   float* const mine = slabs + warp * kSlab;
 #pragma unroll
   for (int j = 0; j < kTiles; j++) {
-    *reinterpret_cast<float2*>(mine + g * kRank + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(mine + (8 + g) * kRank + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    *reinterpret_cast<float2*>(mine + g * kSlice + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(mine + (8 + g) * kSlice + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
   }
   __syncthreads();
   constexpr int kEach = (kSlab / 4 + kLoraThreads - 1) / kLoraThreads;
@@ -212,15 +223,16 @@ __global__ void __launch_bounds__(kLoraThreads, kRank <= 64 ? 2 : 1) lora_down_k
   for (int e = 0; e < kEach; e++) {
     const int i = threadIdx.x + e * kLoraThreads;
     if (i >= kSlab / 4) continue;
-    const int row = rows[4 * i / kRank];
+    const int row = rows[4 * i / kSlice];
     if (row < 0) continue;
+    const size_t to = (size_t)row * p.rank + r0 + 4 * i % kSlice;
     if (p.t_hi) {
       uint2 hi, lo;
       split_halves(sum[e], p.factors ? load_chained(p.factors + slot) : 1.f, hi, lo);
-      *reinterpret_cast<uint2*>(p.t_hi + (size_t)row * kRank + 4 * i % kRank) = hi;
-      *reinterpret_cast<uint2*>(p.t_lo + (size_t)row * kRank + 4 * i % kRank) = lo;
+      *reinterpret_cast<uint2*>(p.t_hi + to) = hi;
+      *reinterpret_cast<uint2*>(p.t_lo + to) = lo;
     } else {
-      *reinterpret_cast<float4*>(p.t + (size_t)row * kRank + 4 * i % kRank) = sum[e];
+      *reinterpret_cast<float4*>(p.t + to) = sum[e];
     }
   }
   if (p.t_hi) fence_chained_writes();
@@ -432,14 +444,14 @@ int make_list(std::vector<Request> r, RunList<kCap>* list) {
   return groups;
 }
 
-template <int kRank, class List>
+template <int kSlice, class List>
 int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int parts, bool x_bf16) {
-  const size_t smem = (size_t)(kLoraWarps + parts - 1) * kGroupRows * kRank * sizeof(float);
+  const size_t smem = (size_t)(kLoraWarps + parts - 1) * kGroupRows * kSlice * sizeof(float);
   auto go = [&](auto kernel) -> int32_t {
     if (smem > 48 << 10)
       if (int32_t rc = allow_smem(p->dev, kernel, smem)) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)groups, (unsigned)parts);
+    cfg.gridDim = dim3((unsigned)groups, (unsigned)parts, (unsigned)(prm.rank / kSlice));
     cfg.blockDim = dim3(kLoraThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = p->dev->stream;
@@ -455,7 +467,7 @@ int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups
     count_launch(p->dev);
     return RELUX_OK;
   };
-  return x_bf16 ? go(lora_down_kernel<kRank, true, List>) : go(lora_down_kernel<kRank, false, List>);
+  return x_bf16 ? go(lora_down_kernel<kSlice, true, List>) : go(lora_down_kernel<kSlice, false, List>);
 }
 template <int kRank, class List>
 int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {
@@ -472,8 +484,8 @@ int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {
 // A call's lists, one launch each: of every row, or by parts of up to kLargeList requests.
 template <class Launch>
 int32_t for_lists(int M, const std::vector<Request>& requests, Launch launch) {
-  if (M <= kNarrowRows) {
-    RowList<kNarrowRows> list;
+  if (M <= kFewRows) {
+    RowList<kFewRows> list;
     return launch(list, make_list(requests, &list));
   }
   if (M <= kSomeRows) {
@@ -505,21 +517,31 @@ int32_t with_rank(int rank, F f) {
     default: return f(std::integral_constant<int, 128>());
   }
 }
-int32_t run_down(Pool* p, int rank, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests) {
-  return with_rank(rank, [&](auto r) {
-    return for_lists(prm.M, requests, [&](const auto& list, int groups) {
-      // parts of K: two blocks an SM, of 256 k at least, a step of every warp
-      const int parts = std::max(1, std::min({kMaxParts, 2 * p->dev->sm_count / groups, prm.K / 256}));
-      return launch_down<decltype(r)::value>(p, prm, list, groups, parts, x_bf16);
-    });
+int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests) {
+  return for_lists(prm.M, requests, [&](const auto& list, int groups) {
+    using List = std::decay_t<decltype(list)>;
+    // parts of K: two blocks an SM where groups are full, of 256 k at least, a step of every warp.  By the call's sizes alone: a row's sums do not depend on the
+    // adapters of the others.
+    const int parts = std::max(1, std::min({kMaxParts, 2 * p->dev->sm_count / ((prm.M + kGroupRows - 1) / kGroupRows), prm.K / 256}));
+    // slices of the rank: of few rows 16, so that more SMs read an adapter (one row of rank 128 x 4096 x 4096: 23 us with the whole rank a block); of many 64, since
+    // every slice reads x again
+    if (prm.rank == 8) return launch_down<8>(p, prm, list, groups, parts, x_bf16);
+    if constexpr (List::kNamesRows) {
+      return launch_down<16>(p, prm, list, groups, parts, x_bf16);
+    } else {
+      if (prm.rank == 16) return launch_down<16>(p, prm, list, groups, parts, x_bf16);
+      if (prm.rank == 32) return launch_down<32>(p, prm, list, groups, parts, x_bf16);
+      return launch_down<64>(p, prm, list, groups, parts, x_bf16);
+    }
   });
 }
 
-// Tiles of rows of one adapter for lora_gemm_kernel; false where they are too many, or would hold less than two thirds of rows (3000 rows of ... each: to be measured).
+// Tiles of rows of one adapter for lora_gemm_kernel; false where they are too many, or less than seven tenths full (16 requests of 80 rows, rank 16, 4096 x 4096, 62 %
+// full: 75.8 us in tiles, 61.8 without; of 100 rows, 78 %: 63.2 and 69.3).
 bool make_tiles(int M, const std::vector<Request>& requests, LoraTiles* tiles) {
   int64_t n = 0;
   for (const Request& r : requests) n += (r.n + 127) / 128;
-  if (n > kMaxLoraTiles || 2 * 128 * n > 3 * (int64_t)std::max(M, 256)) return false;
+  if (M <= 128 || n > kMaxLoraTiles || 7 * 128 * n > 10 * (int64_t)M) return false;
   tiles->n = 0;
   for (const Request& r : requests)
     for (int i = 0; i < r.n; i += 128) {
@@ -569,25 +591,28 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   down.a = (const uint16_t*)a->lora_a;
   down.M = a->m;
   down.K = a->k;
+  down.rank = a->rank;
   const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
 
-  const bool narrow = a->w && a->m <= kNarrowRows && a->n_slots <= 32767;
+  // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16: one row 11.6 us so and 13.3 with lora_up_kernel, 16
+  // rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are rounded there too, by every CTA for itself: 16 rows x 4096 x 14336 31.4 and 26.0, one 11.9 and 13.3.
+  const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 4) && a->m * a->rank <= 512 && a->n_slots <= 32767;
   LoraTiles tiles;
   const bool wide = a->w && !narrow && (int64_t)a->n_slots * a->n < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
   if (narrow || wide) {
-    const bool rounds = narrow && !x_bf16 && a->m <= kRoundedRows;
-    const size_t x_bytes = x_bf16 || rounds ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
+    const bool rounds = wide && !x_bf16;
+    const size_t x_bytes = rounds ? ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255 : 0;
     if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes))) return rc;
     char* const base = (char*)p->layer_buf.p;
-    if (!x_bf16 && !rounds) down.x_bf16 = (uint16_t*)base;
+    if (rounds) down.x_bf16 = (uint16_t*)base;
+    const uint16_t* x = x_bf16 ? (const uint16_t*)a->x : down.x_bf16;
     if (narrow) {
       down.t = (float*)(base + x_bytes);
     } else {
       down.t_hi = (uint16_t*)(base + x_bytes);
       down.t_lo = down.t_hi + (size_t)a->m * a->rank;
     }
-    if ((rc = run_down(p, a->rank, x_bf16, down, requests))) return rc;
-    const uint16_t* x = x_bf16 ? (const uint16_t*)a->x : down.x_bf16;
+    if ((rc = run_down(p, x_bf16, down, requests))) return rc;
     if (wide) return launch_lora_gemm(p, a, x, nullptr, &tiles, nullptr, down.t_hi, down.t_lo);
     int16_t row_slots[kNarrowRows];
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
@@ -598,7 +623,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes, &sc))) return rc;
   if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
   down.t = (float*)sc.rest;
-  if ((rc = run_down(p, a->rank, x_bf16, down, requests))) return rc;
+  if ((rc = run_down(p, x_bf16, down, requests))) return rc;
   UpParams up{};
   if (a->w) {
     const WeightRef w{a->w, a->n};

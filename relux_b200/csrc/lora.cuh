@@ -5,8 +5,7 @@
 
 namespace relux {
 
-constexpr int kNarrowRows = 128;    // calls of up to so many rows: one block of rows, adapters on the CUDA cores
-constexpr int kRoundedRows = 16;    // of up to so many lora_gemm_kernel rounds float32 rows itself
+constexpr int kNarrowRows = 16;     // calls of up to so many rows: one block of rows, rounded by lora_gemm_kernel, adapters on the CUDA cores
 constexpr int kMaxLoraTiles = 1024; // row tiles of a longer call
 
 // Tiles of up to 128 neighbouring rows of one adapter.
@@ -16,7 +15,8 @@ struct LoraTiles {
   int16_t rows[kMaxLoraTiles];
 };
 
-// out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kRoundedRows float32 rows of the caller's.  Without tiles (up to kNarrowRows rows): row_slots
+// out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kNarrowRows float32 rows of the
+// caller's.  Without tiles (up to kNarrowRows rows): row_slots
 // [M], t [M][rank] without factors; with tiles: t as two bf16 halves [M][rank], factors included.
 int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t,
                          const uint16_t* t_hi, const uint16_t* t_lo);

@@ -1,8 +1,9 @@
 // The shared projection of a call with low-rank adapters, C[m] = x[m] W + t[m] B_s^T, s the adapter of row m, in one launch behind lora_down_kernel
 // (lora.cu), which takes t = f_s x A_s^T.  x and W are bf16, W as the layers hold it ([K][N]: MN-major in the MMA), B_s [N][rank].  Tiles as in tile_gemm.cuh.
 //
-//   * Up to 128 rows (bound: HBM, W and the adapters in use): the epilogue's warps, idle while W streams, take t B_s^T on the CUDA cores in
-//     float32, a thread a column, and add it to the sums when they come: a row meets its own adapter only.
+//   * Up to 16 rows (bound: HBM, W and the adapters in use): the epilogue's warps and as many helpers, idle while W streams, take t B_s^T on the CUDA cores
+//     in float32, a thread a column, and add it to the sums when they come: a row meets its own adapter only.  (Of 17 to 128 rows that takes longer than W: 64 rows of
+//     rank 16 x 4096 x 6144 24 us so, 21 by lora_up_kernel behind a GEMM of its own.)
 //   * Wide tiles (bound: the tensor cores): every tile holds rows of one request, so that t B_s^T is further K steps of the same accumulator, t as two
 //     bf16 halves, hi and lo.  Rows of the tile past the request's end are computed with the wrong adapter and not stored.
 //     A row never meets another request's adapter by way of a zero: zero times an infinity in that adapter would be NaN in this row.
@@ -16,10 +17,10 @@ namespace {
 
 constexpr int kPrefetchSteps = 32;
 constexpr int kRowsT = 16 << 10;   // bytes of t of the rows that the epilogue has at hand at a time
+constexpr int kRing = 8;           // pieces of adapters, eight of a row's rank for a column, that are on their way for each of 256 threads
 template <int NC>
-using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT, NC + 8>;   // the adapter's part of a slice lies with the others'
-static_assert(slices_fit(16, 1, 8, 1, LoraShape<16>::kSlices) && slices_fit(32, 1, 8, 1, LoraShape<32>::kSlices) && slices_fit(64, 1, 8, 1, LoraShape<64>::kSlices) &&
-              slices_fit(128, 1, 8, 1, LoraShape<128>::kSlices) && slices_fit(256, 32, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage) &&
+using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT + kRing * 256 * 16, NC + 8>;   // the adapter's part of a slice lies with the others'
+static_assert(slices_fit(16, 1, 8, 1, LoraShape<16>::kSlices) && slices_fit(256, 32, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage) &&
               slices_fit(256, 64, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage), "no room for the slices");
 
 template <int NC>
@@ -34,8 +35,8 @@ struct LoraMaps {
 };
 struct LoraGemmParams {
   int32_t M, N, rank, steps, tiles, col_tiles, out_bf16, adds;
-  int32_t x_early;           // x is the caller's: complete before the chain's head began
-  const float* x_f32;        // up to 16 rows of float32: rounded here, into the stages [M][K]
+  int32_t x_early;           // x was complete before the chain's head began
+  const float* x_f32;        // up to kNarrowRows rows of float32: rounded here, into the stages [M][K]
   int32_t K;
   const float* t;            // narrow: [M][rank], without factors
   const uint16_t* b;         // narrow: [slots][N][rank]
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
     if (threadIdx.x == 0) set_status(prm.status, RELUX_ERR_UNSUPPORTED);
     return;
   }
-  const bool rounds_x = NC == 16 && prm.x_f32;
+  const bool rounds_x = NC == kNarrowRows && prm.x_f32;
   const uint32_t tmem = tile_setup<SH>(bars, size, rounds_x ? 5 : 1);
 
   bool has_t = false;
@@ -100,52 +101,37 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
     has_t = true;
     low_sync();   // the tile before is done with t
   };
-  // Up to 128 rows: t B_s^T of a tile and this CTA's rows, behind the slices of the others.  By the epilogue's warps (half 0) and the helpers (half 1), a thread a
-  // column, blocks of eight rows in turn: eight of every row's rank
-  // are loaded while the two pieces before them are multiplied, the first two ahead of t.
+  // Up to 16 rows: t B_s^T of a tile and this CTA's rows, behind the slices of the others.  By the epilogue's warps (half 0) and the helpers (half 1), a thread a
+  // column, rows in turn.  What a thread reads of B_s goes through a ring of its own in shared memory, the first pieces ahead of t.  (Through registers, by
+  // unrolled loops, 32 rows of rank 16 took 11000 clocks: code that runs once is fetched as it goes.)
   auto low_half = [&](const Place& at, int half) {
     const int id = half ? threadIdx.x - 192 : threadIdx.x, n = at.c * kRowsOp + id;
     const int q0 = size > 1 ? slice_begin(rank, prm.M, 1, size) : 0, q1 = size > 1 ? slice_begin(rank + 1, prm.M, 1, size) : prm.M;
     const bool mine = n < prm.N;
     float* const low = reinterpret_cast<float*>(slices) + (size - 1) * (q1 - q0) * kRowsOp + id;
-    const int batch = kRowsT / 4 / prm.rank;   // rows whose t is at hand, a multiple of 16
+    const int batch = kRowsT / 4 / prm.rank;   // rows whose t is at hand
+    const int shift = 31 - __clz(prm.rank >> 3), chunks = 1 << shift;   // ranks are powers of two
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(t_rows) + kRowsT + (half * 128 + id) * 16;
     for (int b0 = q0; b0 < q1; b0 += batch) {
-      const int b1 = min(q1, b0 + batch), blocks = (b1 - b0 + 7) / 8, chunks = prm.rank / 8, count = (blocks + 1 - half) / 2 * chunks;
-      uint4 v[3][8];
-      auto row_of = [&](int i) { return b0 + (i / chunks * 2 + half) * 8; };
-      auto load = [&](int i, uint4 (&w)[8]) {
-        const int q = row_of(i), r = i % chunks * 8;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int slot = q + j < b1 ? list.slot[q + j] : -1;
-          const uint4* src = reinterpret_cast<const uint4*>(prm.b + ((size_t)max(slot, 0) * prm.N + (mine ? n : 0)) * prm.rank + r);
-          w[j] = slot >= 0 && mine ? load_chained(src) : make_uint4(0u, 0u, 0u, 0u);
+      const int b1 = min(q1, b0 + batch), count = ((b1 - b0 + 1 - half) >> 1) << shift;
+      constexpr int kFetch = kRing / 2;
+      auto fetch = [&](int first_piece) {   // half a ring: piece i is chunk i % chunks of row i / chunks of this half
+#pragma unroll 1
+        for (int i = first_piece; i < min(first_piece + kFetch, count); i++) {
+          const int slot = list.slot[b0 + 2 * (i >> shift) + half];
+          const bool some = slot >= 0 && mine;
+          const uint16_t* src = prm.b + ((size_t)(some ? slot : 0) * prm.N + (some ? n : 0)) * prm.rank + (i & (chunks - 1)) * 8;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(ring + (i & (kRing - 1)) * (256 * 16))), "l"(src), "r"(some ? 16 : 0) : "memory");
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      auto multiply = [&](int i, const uint4 (&w)[8]) {
-        const int q = row_of(i), r = i % chunks * 8;
-        float sum[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          sum[j] = r && q + j < b1 ? low[(q + j - q0) * kRowsOp] : 0.f;
-          const float4* t = reinterpret_cast<const float4*>(t_rows + (min(q + j, b1 - 1) - b0) * prm.rank + r);   // of a row without an adapter zeros, as its w
-          const float4 t0 = t[0], t1 = t[1];
-          sum[j] = fmaf(t0.x, bf16_lo(w[j].x), sum[j]); sum[j] = fmaf(t0.y, bf16_hi(w[j].x), sum[j]);
-          sum[j] = fmaf(t0.z, bf16_lo(w[j].y), sum[j]); sum[j] = fmaf(t0.w, bf16_hi(w[j].y), sum[j]);
-          sum[j] = fmaf(t1.x, bf16_lo(w[j].z), sum[j]); sum[j] = fmaf(t1.y, bf16_hi(w[j].z), sum[j]);
-          sum[j] = fmaf(t1.z, bf16_lo(w[j].w), sum[j]); sum[j] = fmaf(t1.w, bf16_hi(w[j].w), sum[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (q + j < b1) low[(q + j - q0) * kRowsOp] = sum[j];
-      };
-      if (count > 0) load(0, v[0]);   // adapters were complete before the chain's head began
-      if (count > 1) load(1, v[1]);
+      fetch(0);   // adapters were complete before the chain's head began
+      fetch(kFetch);
       if (b0 == q0) low_wait();
       else low_sync();                // the batch before is done with
       for (int i = threadIdx.x - (half ? 64 : 0); i < (b1 - b0) * prm.rank / 4; i += 256) {
         const int slot = list.slot[b0 + 4 * i / prm.rank];
-        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);   // (what t holds of a row without an adapter is nobody's)
         if (slot >= 0) {
           u = load_chained(reinterpret_cast<const float4*>(prm.t + (size_t)b0 * prm.rank) + i);
           const float f = prm.factors ? load_chained(prm.factors + slot) : 1.f;
@@ -154,14 +140,23 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
         reinterpret_cast<float4*>(t_rows)[i] = u;
       }
       low_sync();
+      float sum = 0.f;
 #pragma unroll 1
-      for (int i = 0; i < count; i += 3)
-#pragma unroll
-        for (int k = 0; k < 3; k++)
-          if (i + k < count) {
-            if (i + k + 2 < count) load(i + k + 2, v[(k + 2) % 3]);
-            multiply(i + k, v[k]);
-          }
+      for (int g = 0; g < count; g += kFetch) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+#pragma unroll 1
+        for (int i = g; i < min(g + kFetch, count); i++) {
+          const int c = i & (chunks - 1), q = 2 * (i >> shift) + half;
+          const uint4 w = *reinterpret_cast<const uint4*>(ring + (i & (kRing - 1)) * (256 * 16));
+          const float4* t = reinterpret_cast<const float4*>(t_rows + q * prm.rank + c * 8);
+          const float4 t0 = t[0], t1 = t[1];
+          if (c == 0) sum = 0.f;
+          sum = fmaf(t0.x, bf16_lo(w.x), sum); sum = fmaf(t0.y, bf16_hi(w.x), sum); sum = fmaf(t0.z, bf16_lo(w.y), sum); sum = fmaf(t0.w, bf16_hi(w.y), sum);
+          sum = fmaf(t1.x, bf16_lo(w.z), sum); sum = fmaf(t1.y, bf16_hi(w.z), sum); sum = fmaf(t1.z, bf16_lo(w.w), sum); sum = fmaf(t1.w, bf16_hi(w.w), sum);
+          if (c == chunks - 1) low[(b0 - q0 + q) * kRowsOp] = sum;
+        }
+        fetch(g + 2 * kFetch);
+      }
     }
     low_sync();
   };
@@ -444,9 +439,7 @@ int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_
   LoraGemmParams prm{};
   LoraMaps maps{};
   const int M = a->m, K = a->k, N = a->n;
-  int nc = 16;
-  while (nc < M && nc < kNarrowRows) nc *= 2;
-  if (tiles) nc = 256;
+  const int nc = tiles ? 256 : kNarrowRows;
   prm.M = M;
   prm.N = N;
   prm.rank = a->rank;
@@ -479,12 +472,7 @@ int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_
   NarrowRows rows;
   std::copy(row_slots, row_slots + M, rows.slot);
   std::fill(rows.slot + M, rows.slot + kNarrowRows, (int16_t)-1);
-  switch (nc) {
-    case 16: return launch_rows<16>(p, maps, prm, rows);
-    case 32: return launch_rows<32>(p, maps, prm, rows);
-    case 64: return launch_rows<64>(p, maps, prm, rows);
-    default: return launch_rows<128>(p, maps, prm, rows);
-  }
+  return launch_rows<kNarrowRows>(p, maps, prm, rows);
 }
 
 }  // namespace relux

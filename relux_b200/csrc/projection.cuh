@@ -88,6 +88,8 @@ struct LayerScratch {
 };
 // [activations as bf16 (M x max_k) | split partials | caller's buffers (rest_bytes)]
 int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, LayerScratch* out);
+// n float32 values, a multiple of 8, rounded to bf16 by the reference's rule.
+int32_t launch_cast(Pool* p, const float* src, uint16_t* dst, size_t n);
 bool gemm_sm100_eligible(int K, const WeightRef* ws, int nw);
 // part[piece][M][n_total] = A[M][K] x [W_0 | W_1 | ...]; returns the ranges, which say how many pieces every tile has.
 int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const WeightRef* ws, int nw, float* part, size_t part_cap_bytes,

@@ -724,6 +724,34 @@ typedef struct relux_matmul_lora_args {
 } relux_matmul_lora_args;
 int32_t relux_matmul_lora(relux_pool_t pool, const relux_matmul_lora_args* args);
 
+/* The attention half of a block in one call: Block.Forward's residual, norm and attention (internal/transformer/transformer_block.go:119-142) around
+ * MHA.forwardCached.  layer: as for relux_gqa_forward_cached in RELUX_ATTN_FAST (x may be bf16 too); with it
+ *   h = x + residual (relux_rmsnorm: h goes to residual_out),  y = norm(h),  out = attention layer of y
+ * The first block has the embedding as x and residual NULL; a later one has what the feed-forward half before it
+ * gave as x and the sum so far as residual.  The feed-forward half begins with relux_rmsnorm of out and that sum.
+ * Each of the four projections has the layer's bf16 weight or, where codes are given, 8-bit weights (relux_int8_weights, relux_matmul_int8: the rows are
+ * quantised one by one), and adapters of the requests beside it where lora_a is given (relux_matmul_lora; rank and slots are common to the four).  A projection with
+ * codes needs no weight in layer->w.  Everything is checked before anything is written to the cache. */
+typedef struct relux_block_projection {
+  const int8_t* codes;       /* device [n][k], or NULL: the layer's weight */
+  const float* scales;       /* device [n], with codes */
+  const void* lora_a;        /* device bf16 [n_slots][rank][k], or NULL: no adapters */
+  const void* lora_b;        /* device bf16 [n_slots][n][rank], with lora_a */
+  const float* factors;      /* device [n_slots], or NULL: ones */
+} relux_block_projection;
+typedef struct relux_gqa_block_args {
+  const void* residual;      /* device [n_seqs][q_tokens][d_model], or NULL */
+  void* residual_out;        /* device, or NULL; may be residual */
+  const void* norm_weight;   /* device [d_model], or NULL: ones */
+  int32_t residual_dtype, norm_dtype;
+  float eps;
+  int32_t rank, n_slots;
+  int32_t reserved[3];
+  const int32_t* adapter;    /* host [n_seqs]: slot, or -1; with adapters */
+  relux_block_projection q, k, v, o;
+} relux_gqa_block_args;
+int32_t relux_gqa_block_cached(relux_pool_t pool, const relux_gqa_layer_args* layer, const relux_gqa_block_args* block);
+
 /* ---- expansion of the cached MLA latents --------------------------------------------------------
  * What MLA.forwardCached does before it scores a multi-token call: every cached latent row times W_UK and W_UV
  * (internal/transformer/mla.go:323-326), here as one tensor-core GEMM with bf16 results.  The library's own prompt path

@@ -573,6 +573,42 @@ class Pool:
                               x=_ptr(x), x_dtype=_dtype_flag(x), x_mem=_mem(x), out=_ptr(out), out_mem=_mem(out), w=C.pointer(w))
         L.check(self.lib.relux_gqa_forward_cached(self.h, C.byref(args)))
 
+    def block_cached(self, layer, n_seqs, x, out, weights, d_model, num_heads, norm_weight=None, eps=1e-5, residual=None, residual_out=None, int8=None, lora=None,
+                     rank=0, n_slots=0, adapter=None, q_tokens=1, causal=True, rope_base=0.0, seq_ids=None, rope=True, advance=True, x_dtype=None,
+                     residual_dtype=None, norm_dtype=None):
+        """The attention half of a block (relux_gqa_block_cached): h = x + residual, its norm, and the layer step of it.  weights: w_q, w_k, w_v, w_o in bf16;
+        int8: some of the same names -> (codes, scales) device buffers of 8-bit weights; lora: some of them -> (lora_a, lora_b, factors or None), with rank,
+        n_slots and adapter [n_seqs].  x and out as for forward_cached (x may be bf16), residual and residual_out on the device."""
+        ids = None if seq_ids is None else np.ascontiguousarray(seq_ids, dtype=np.int32)
+        slots = None if adapter is None else np.ascontiguousarray(adapter, dtype=np.int32)
+        if slots is not None and slots.shape != (n_seqs,):
+            raise ValueError("block_cached: adapters of shape %s for %d sequences" % (slots.shape, n_seqs))
+        for name, a in (("residual", residual), ("residual_out", residual_out), ("norm_weight", norm_weight)):
+            if a is not None and not isinstance(a, (DeviceBuffer, int)):
+                raise TypeError("block_cached: %s must be device memory" % name)
+        names = ("w_q", "w_k", "w_v", "w_o")
+        for given in (weights, int8 or {}, lora or {}):
+            for n in given:
+                if n not in names:
+                    raise ValueError("block_cached: no projection %s" % n)
+        w = L.GqaLayerWeights(**{n: _ptr(weights.get(n)) for n in names})
+        xt = _dtype_flag(x, x_dtype)
+        args = L.GqaLayerArgs(layer=layer, n_seqs=n_seqs, seq_ids=_ptr(ids), q_tokens=q_tokens, causal=int(causal), d_model=d_model, num_heads=num_heads,
+                              rope=int(rope), rope_base=float(rope_base), advance=int(advance), mode=L.ATTN_FAST, x=_ptr(x), x_dtype=xt, x_mem=_mem(x),
+                              out=_ptr(out), out_mem=_mem(out), w=C.pointer(w))
+
+        def flag(a, explicit, otherwise):
+            return explicit if explicit is not None else a.dtype_flag if isinstance(a, DeviceBuffer) else otherwise
+
+        def projection(n):
+            codes, scales = (int8 or {}).get(n, (None, None))
+            a, b, f = (lora or {}).get(n, (None, None, None))
+            return L.BlockProjection(codes=_ptr(codes), scales=_ptr(scales), lora_a=_ptr(a), lora_b=_ptr(b), factors=_ptr(f))
+        block = L.GqaBlockArgs(residual=_ptr(residual), residual_out=_ptr(residual_out), norm_weight=_ptr(norm_weight),
+                               residual_dtype=flag(residual, residual_dtype, xt), norm_dtype=flag(norm_weight, norm_dtype, L.DTYPE_BF16), eps=float(eps), rank=rank,
+                               n_slots=n_slots, adapter=_ptr(slots), **{n[2]: projection(n) for n in names})
+        L.check(self.lib.relux_gqa_block_cached(self.h, C.byref(args), C.byref(block)))
+
     def _mla_forward_cached(self, layer, n_seqs, x, out, weights, d_model, num_heads, q_tokens=1, causal=True, rope_base=0.0,
                             mode=L.ATTN_FAST, seq_ids=None):
         """One MLA layer step (MLA.forwardCached, mla.go:272-397): x [n_seqs, q_tokens, d_model] float32 ->

@@ -185,7 +185,7 @@ struct Pool {
   bool has_tmap = false;
   bool mla_blocked = false;   // MLA pages stored as 64-column blocks (see mla_page_off)
   // layer-level step (layer_step.cu): RoPE tables [cos | sin][positions][dHR / 2] and the step's scratch block
-  GrowBuf rope_tab, layer_buf;
+  GrowBuf rope_tab, layer_buf, block_buf;
   int rope_dim = 0, rope_positions = 0;
   float rope_base = 0.f;
   // device times of the dominant kernel of the last kTimeRing attention calls, and of the input-projection GEMM of the
@@ -292,6 +292,9 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a);
 int32_t do_spec_accept(Pool* p, const relux_spec_accept_args* a);
 int32_t do_sample(Pool* p, const relux_sample_args* a);
 int32_t do_matmul(Pool* p, const relux_matmul_args* a);
+int32_t do_gqa_block(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b);
+int32_t check_rmsnorm(const relux_rmsnorm_args* a);   // before anything is launched
+int32_t launch_matmul_int8(Pool* p, int M, int K, int N, const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale, void* out, bool out_bf16);
 int32_t do_rmsnorm(Pool* p, const relux_rmsnorm_args* a);
 int32_t do_int8_rows(Pool* p, const relux_int8_rows_args* a);
 int32_t do_int8_weights(Pool* p, const relux_int8_weights_args* a);

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <vector>
 #include "common.cuh"
 #include "internal.h"
 #include "projection.cuh"
@@ -273,6 +274,7 @@ struct ProjSeg {
   void* dst;          // [M][n], f32 or bf16
   int32_t bf16;
   int32_t by_tma;     // the next launch reads it by TMA
+  const float* src;   // [M][n] where its projection is whole, a call of its own; nullptr: the pieces of the joint one
 };
 struct FinishParams {
   const float* part;
@@ -300,16 +302,22 @@ __global__ void proj_finish_kernel(const FinishParams p) {
     c -= p.seg[j].n;
     j++;
   }
-  const int col_tile = p.tile_first[j] + c / kTileN;
-  const int pieces = p.rg.pieces(kTurns ? p.rg.tile_of(col_tile, m) : col_tile);
-  float v0 = 0.f, v1 = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < pieces; s++) {
-    const float2 t = load_chained(reinterpret_cast<const float2*>(p.part + ((size_t)s * p.M + m) * p.n_total + col));
-    v0 += t.x;
-    v1 += t.y;
-  }
   const ProjSeg sg = p.seg[j];
+  float v0 = 0.f, v1 = 0.f;
+  if (sg.src) {
+    const float2 t = load_chained(reinterpret_cast<const float2*>(sg.src + (size_t)m * sg.n + c));
+    v0 = t.x;
+    v1 = t.y;
+  } else {
+    const int col_tile = p.tile_first[j] + c / kTileN;
+    const int pieces = p.rg.pieces(kTurns ? p.rg.tile_of(col_tile, m) : col_tile);
+#pragma unroll 4
+    for (int s = 0; s < pieces; s++) {
+      const float2 t = load_chained(reinterpret_cast<const float2*>(p.part + ((size_t)s * p.M + m) * p.n_total + col));
+      v0 += t.x;
+      v1 += t.y;
+    }
+  }
   if (sg.rope_dim > 0) {
     const int i = m / p.S, s = m % p.S;
     const int seq = p.seq_ids ? p.seq_ids[i] : i;
@@ -526,40 +534,20 @@ int32_t launch_cast(Pool* p, const float* src, uint16_t* dst, size_t n) {
 
 namespace {
 
-// x [M][K] f32 -> every segment's buffer: cast + split-K tensor-core GEMM (or the reference-order GEMM), then the
-// finish kernel.  The GEMM's device time goes to the pool's projection ring.
-int32_t project_and_finish(Pool* p, const SeqBatch& sb, int layer, const float* dx, int M, int K, int S, const WeightRef* ws,
-                           const ProjSeg* segs, int nw, bool mma, uint16_t* a_bf16, float* part, size_t part_cap, bool same_pos = false) {
-  cudaStream_t st = p->dev->stream;
-  const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
-  int n_total = 0;
-  for (int j = 0; j < nw; j++) n_total += ws[j].n;
-  GemmRanges ranges{};
-  if (mma) {
-    int32_t rc = launch_cast(p, dx, a_bf16, (size_t)M * K);
-    const TimeStamp time = time_stamp_next(p, p->proj_times);
-    if (!rc) rc = launch_skinny_gemm(p, a_bf16, M, K, ws, nw, part, part_cap, &ranges, time);
-    if (rc) return rc;
-    time_stamp_done(p->proj_times, time);
-  } else {
-    int32_t rc = time_events_begin(p, p->proj_times);
-    if (rc) return rc;
-    rc = launch_gemm_reference(p, dx, M, K, ws, nw, part, n_total);
-    if (rc) return rc;
-    if ((rc = time_events_end(p, p->proj_times))) return rc;
-  }
+// The finish kernel behind the projections of a layer.
+int32_t finish_projections(Pool* p, const SeqBatch& sb, int layer, int M, int S, const ProjSeg* segs, int nw, const float* part, const GemmRanges& ranges, bool same_pos) {
   FinishParams f;
   memset(&f, 0, sizeof(f));
   f.part = part;
   f.rg = ranges;
-  for (int j = 1; j < nw; j++) f.tile_first[j] = f.tile_first[j - 1] + (ws[j - 1].n + kTileN - 1) / kTileN;
+  for (int j = 1; j < nw; j++) f.tile_first[j] = f.tile_first[j - 1] + (segs[j - 1].n + kTileN - 1) / kTileN;
   f.M = M;
-  f.n_total = n_total;
   f.S = S;
   f.n_segs = nw;
   int rope_dim = 0;
   for (int j = 0; j < nw; j++) {
     f.seg[j] = segs[j];
+    f.n_total += segs[j].n;
     if (segs[j].rope_dim) rope_dim = segs[j].rope_dim;
   }
   f.len = p->d_len + (size_t)layer * p->prm.max_seqs;
@@ -569,10 +557,36 @@ int32_t project_and_finish(Pool* p, const SeqBatch& sb, int layer, const float* 
   f.rope_positions = p->rope_positions;
   f.same_pos = same_pos ? 1 : 0;
   f.status = p->d_status;
-  dim3 grid((n_total / 2 + 255) / 256, M);
-  RELUX_CUDA_TRY(launch_chained(chained, ranges.in_turns() ? proj_finish_kernel<true> : proj_finish_kernel<false>, grid, dim3(256), 0, st, f));
+  dim3 grid((f.n_total / 2 + 255) / 256, M);
+  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, ranges.in_turns() ? proj_finish_kernel<true> : proj_finish_kernel<false>, grid, dim3(256),
+                                0, p->dev->stream, f));
   count_launch(p->dev);
   return RELUX_OK;
+}
+
+// x [M][K] f32 -> every segment's buffer: cast (or the norm that a block begins with) + split-K tensor-core GEMM (or the reference-order GEMM), then the
+// finish kernel.  The GEMM's device time goes to the pool's projection ring.
+int32_t project_and_finish(Pool* p, const SeqBatch& sb, int layer, const float* dx, int M, int K, int S, const WeightRef* ws,
+                           const ProjSeg* segs, int nw, bool mma, uint16_t* a_bf16, float* part, size_t part_cap, bool same_pos = false,
+                           const relux_rmsnorm_args* norm = nullptr) {
+  int n_total = 0;
+  for (int j = 0; j < nw; j++) n_total += ws[j].n;
+  GemmRanges ranges{};
+  if (mma) {
+    int32_t rc = norm ? do_rmsnorm(p, norm) : launch_cast(p, dx, a_bf16, (size_t)M * K);
+    if (rc) return rc;
+    const TimeStamp time = time_stamp_next(p, p->proj_times);
+    rc = launch_skinny_gemm(p, a_bf16, M, K, ws, nw, part, part_cap, &ranges, time);
+    if (rc) return rc;
+    time_stamp_done(p->proj_times, time);
+  } else {
+    int32_t rc = time_events_begin(p, p->proj_times);
+    if (rc) return rc;
+    rc = launch_gemm_reference(p, dx, M, K, ws, nw, part, n_total);
+    if (rc) return rc;
+    if ((rc = time_events_end(p, p->proj_times))) return rc;
+  }
+  return finish_projections(p, sb, layer, M, S, segs, nw, part, ranges, same_pos);
 }
 
 // out [M][N] f32 = attn [M][K] x W_O [K][N]; `out` is the caller's buffer (host or device).  d_attn: float32, or nullptr when
@@ -748,14 +762,173 @@ int32_t do_mla_layer(Pool* p, const relux_mla_layer_args* a) {
   return output_projection(p, o_bf16 ? nullptr : d_attn, M, H * Dh, w.w_o, D, mma, sc.a_bf16, sc.part, sc.part_cap, a->out, a->out_mem);
 }
 
+// ---- the attention half of a block: what relux_gqa_block_cached adds to a layer step ----
+namespace {
+
+struct BlockScratch {
+  uint16_t* y;        // the norm's rows, then attention's, as bf16 [M][D]
+  int8_t* codes;      // and in 8 bits
+  float* scales;
+  float* projected;   // [M][n_q + n_k + n_v], a projection behind the other
+  char* rest;
+};
+int32_t block_scratch(Pool* p, int M, int D, int n_total, size_t rest_bytes, BlockScratch* out) {
+  const size_t off_codes = pad256((size_t)M * D * 2), off_scales = off_codes + pad256((size_t)M * D), off_proj = off_scales + pad256((size_t)M * 4),
+               off_rest = off_proj + pad256((size_t)M * n_total * 4);
+  if (int32_t rc = grow(p->dev, p->block_buf, off_rest + rest_bytes)) return rc;
+  char* base = (char*)p->block_buf.p;
+  *out = BlockScratch{(uint16_t*)base, (int8_t*)(base + off_codes), (float*)(base + off_scales), (float*)(base + off_proj), base + off_rest};
+  return RELUX_OK;
+}
+
+relux_rmsnorm_args block_norm(const relux_gqa_layer_args* a, const relux_gqa_block_args* b, const void* x, int M) {
+  relux_rmsnorm_args n;
+  memset(&n, 0, sizeof(n));
+  n.n_rows = M;
+  n.d = a->d_model;
+  n.eps = b->eps;
+  n.x_dtype = a->x_dtype;
+  n.residual_dtype = b->residual_dtype;
+  n.weight_dtype = b->norm_dtype;
+  n.x = x;
+  n.residual = b->residual;
+  n.weight = b->norm_weight;
+  n.residual_out = b->residual_out;
+  return n;
+}
+
+// Before anything is launched or written to the cache.
+int32_t check_block(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b) {
+  if (a->mode != RELUX_ATTN_FAST) { set_error("a block runs in RELUX_ATTN_FAST only"); return RELUX_ERR_UNSUPPORTED; }
+  for (int i = 0; i < 3; i++)
+    if (b->reserved[i]) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  int32_t rc;
+  bool lora = false;
+  for (const relux_block_projection* q : {&b->q, &b->k, &b->v, &b->o}) {
+    if ((q->codes == nullptr) != (q->scales == nullptr) || (q->lora_a == nullptr) != (q->lora_b == nullptr)) {
+      set_error("a block's projection: codes need scales, and lora_a lora_b");
+      return RELUX_ERR_INVALID_ARG;
+    }
+    if ((rc = check_dev_align(q->codes, "codes")) || (rc = check_dev_align(q->scales, "scales")) || (rc = check_dev_align(q->lora_a, "lora_a")) ||
+        (rc = check_dev_align(q->lora_b, "lora_b")) || (rc = check_dev_align(q->factors, "factors")))
+      return rc;
+    lora = lora || q->lora_a;
+  }
+  relux_rmsnorm_args n = block_norm(a, b, a->x, 1);
+  n.out = (void*)16;   // an output is given later
+  if (a->x_mem == RELUX_MEM_HOST) n.x = n.out;
+  if ((rc = check_rmsnorm(&n))) return rc;
+  if (!lora) return RELUX_OK;
+  if (!b->adapter || b->n_slots <= 0) { set_error("a block's adapters need the requests' slots"); return RELUX_ERR_INVALID_ARG; }
+  if (b->rank != 8 && b->rank != 16 && b->rank != 32 && b->rank != 64 && b->rank != 128) { set_error("rank=%d must be one of 8, 16, 32, 64, 128", b->rank); return RELUX_ERR_UNSUPPORTED; }
+  for (int i = 0; i < a->n_seqs && a->n_seqs <= p->prm.max_seqs; i++)
+    if (b->adapter[i] < -1 || b->adapter[i] >= b->n_slots) {
+      set_error("adapter %d of request %d outside [-1, %d)", b->adapter[i], i, b->n_slots);
+      return RELUX_ERR_INVALID_ARG;
+    }
+  return RELUX_OK;
+}
+
+// dst [M][N] f32 = rows x one projection of a block: its 8-bit or bf16 weights, and its adapters.  y: the rows as bf16 or (y_f32) float32, codes: in 8 bits, each
+// where it is needed.
+int32_t project_one(Pool* p, int M, int K, int N, const relux_gqa_block_args* b, const relux_block_projection& q, const void* w, const void* y, bool y_f32,
+                    const BlockScratch& bs, int n_seqs, const int32_t* rows_each, float* dst) {
+  int32_t rc;
+  if (q.codes)
+    if ((rc = launch_matmul_int8(p, M, K, N, bs.codes, bs.scales, q.codes, q.scales, dst, false))) return rc;
+  if (q.lora_a) {
+    relux_matmul_lora_args l;
+    memset(&l, 0, sizeof(l));
+    l.m = M;
+    l.k = K;
+    l.n = N;
+    l.rank = b->rank;
+    l.n_slots = b->n_slots;
+    l.n_seqs = n_seqs;
+    l.x_dtype = y_f32 ? RELUX_DTYPE_F32 : RELUX_DTYPE_BF16;
+    l.out_dtype = RELUX_DTYPE_F32;
+    l.accumulate = q.codes != nullptr;
+    l.x = y;
+    l.w = q.codes ? nullptr : w;
+    l.lora_a = q.lora_a;
+    l.lora_b = q.lora_b;
+    l.factors = q.factors;
+    l.adapter = b->adapter;
+    l.n_rows = rows_each;
+    l.out = dst;
+    return do_matmul_lora(p, &l);
+  }
+  if (q.codes) return RELUX_OK;
+  LayerScratch sc;
+  if ((rc = layer_scratch(p, M, K, N, 0, &sc))) return rc;
+  return output_projection(p, y_f32 ? (const float*)y : nullptr, M, K, w, N, true, y_f32 ? sc.a_bf16 : (uint16_t*)y, sc.part, sc.part_cap, dst, RELUX_MEM_DEVICE);
+}
+
+// h = x + residual, its norm, and q, k, v in their buffers.
+int32_t block_projections(Pool* p, const SeqBatch& sb, const relux_gqa_layer_args* a, const relux_gqa_block_args* b, const void* dx, int M, const WeightRef* proj,
+                          ProjSeg* segs, const BlockScratch& bs, const int32_t* rows_each) {
+  const relux_block_projection* q[3] = {&b->q, &b->k, &b->v};
+  bool wants_bf16 = false, wants_codes = false, joint = true;
+  for (const relux_block_projection* r : q) {
+    wants_bf16 = wants_bf16 || !r->codes || r->lora_a;
+    wants_codes = wants_codes || r->codes;
+    joint = joint && !r->codes && !r->lora_a;
+  }
+  relux_rmsnorm_args n = block_norm(a, b, dx, M);
+  n.out_dtype = RELUX_DTYPE_BF16;
+  n.out = wants_bf16 ? bs.y : nullptr;
+  n.codes = wants_codes ? bs.codes : nullptr;
+  n.scales = wants_codes ? bs.scales : nullptr;
+  int32_t rc;
+  if (joint) {
+    int n_total = 0;
+    for (int j = 0; j < 3; j++) n_total += proj[j].n;
+    LayerScratch sc;
+    if ((rc = layer_scratch(p, M, a->d_model, n_total, 0, &sc))) return rc;
+    return project_and_finish(p, sb, a->layer, nullptr, M, a->d_model, a->q_tokens, proj, segs, 3, true, bs.y, sc.part, sc.part_cap, false, &n);
+  }
+  if ((rc = do_rmsnorm(p, &n))) return rc;
+  float* dst = bs.projected;
+  for (int j = 0; j < 3; j++) {
+    if ((rc = project_one(p, M, a->d_model, proj[j].n, b, *q[j], proj[j].w, bs.y, false, bs, sb.n_seqs, rows_each, dst))) return rc;
+    segs[j].src = dst;
+    dst += (size_t)M * proj[j].n;
+  }
+  return finish_projections(p, sb, a->layer, M, a->q_tokens, segs, 3, nullptr, GemmRanges{}, false);
+}
+
+// out [M][d_model] = attention's rows x W_O.
+int32_t block_output(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b, const void* attn, bool attn_bf16, int M, int K, const BlockScratch& bs,
+                     const int32_t* rows_each) {
+  const int N = a->d_model;
+  const bool direct = a->out_mem == RELUX_MEM_DEVICE;
+  int32_t rc;
+  if (!direct && (rc = grow(p->dev, p->out_buf, (size_t)M * N * 4))) return rc;
+  float* dst = direct ? (float*)a->out : (float*)p->out_buf.p;
+  if (b->o.codes) {
+    const relux_int8_rows_args r{M, K, attn_bf16 ? RELUX_DTYPE_BF16 : RELUX_DTYPE_F32, 0, attn, bs.codes, bs.scales};
+    if ((rc = do_int8_rows(p, &r))) return rc;
+  }
+  if ((rc = project_one(p, M, K, N, b, b->o, a->w->w_o, attn, !attn_bf16, bs, M / a->q_tokens, rows_each, dst))) return rc;
+  if (!direct) {
+    RELUX_CUDA_TRY(cudaMemcpyAsync(a->out, dst, (size_t)M * N * 4, cudaMemcpyDeviceToHost, p->dev->stream));
+    RELUX_CUDA_TRY(cudaStreamSynchronize(p->dev->stream));
+  }
+  return RELUX_OK;
+}
+
+}  // namespace
+
 // MHA.forwardCached (mha.go:245-369) for a batch of independent sequences: projections with Wq / Wk / Wv, RoPE on q
-// and k at position cacheLen + s (when the layer has a rotary embedding), append of k / v, GQA attention, Wo.
-int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) {
+// and k at position cacheLen + s (when the layer has a rotary embedding), append of k / v, GQA attention, Wo.  With b the attention half of a
+// block around it: the residual's addition and the norm first, and projections with adapters or 8-bit weights.
+static int32_t gqa_layer(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b) {
   if (!a || !a->w) { set_error("nil argument struct"); return RELUX_ERR_INVALID_ARG; }
   const relux_pool_params& prm = p->prm;
   if (prm.kind != RELUX_POOL_GQA) { set_error("pool kind does not match this call (GQA pool needed)"); return RELUX_ERR_INVALID_ARG; }
   const relux_gqa_layer_weights& w = *a->w;
-  if (!a->x || !a->out || !w.w_q || !w.w_k || !w.w_v || !w.w_o) {
+  const relux_block_projection none{}, bq = b ? b->q : none, bk = b ? b->k : none, bv = b ? b->v : none, bo = b ? b->o : none;
+  if (!a->x || !a->out || (!w.w_q && !bq.codes) || (!w.w_k && !bk.codes) || (!w.w_v && !bv.codes) || (!w.w_o && !bo.codes)) {
     set_error("nil input, output or weight pointer");
     return RELUX_ERR_INVALID_ARG;
   }
@@ -768,7 +941,8 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) {
   if (a->mode != RELUX_ATTN_FAST && a->mode != RELUX_ATTN_REFERENCE && a->mode != RELUX_ATTN_REFERENCE_FAITHFUL) { set_error("bad mode"); return RELUX_ERR_INVALID_ARG; }
   const bool faithful = a->mode == RELUX_ATTN_REFERENCE_FAITHFUL;
   if (faithful && (!p->compat || !a->advance)) { set_error("RELUX_ATTN_REFERENCE_FAITHFUL needs a pool created with RELUX_POOL_FLAG_REFERENCE_COMPAT and advance != 0"); return RELUX_ERR_INVALID_ARG; }
-  if (a->x_dtype != RELUX_DTYPE_F32) { set_error("x must be float32"); return RELUX_ERR_UNSUPPORTED; }
+  const bool x_bf16 = b && a->x_dtype == RELUX_DTYPE_BF16;
+  if (a->x_dtype != RELUX_DTYPE_F32 && !x_bf16) { set_error("x must be float32"); return RELUX_ERR_UNSUPPORTED; }
   if (p->int8 && a->mode != RELUX_ATTN_FAST) { set_error("a pool of 8-bit rows takes RELUX_ATTN_FAST only"); return RELUX_ERR_UNSUPPORTED; }
   if (a->mode == RELUX_ATTN_FAST && (!p->has_tmap || prm.page_tokens != 64 || hd != 128 || H / Hkv > 32)) {
     // checked before anything is written to the cache
@@ -776,6 +950,8 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) {
               "(got page_tokens=%d head_dim=%d group=%d); use RELUX_ATTN_REFERENCE for other shapes", prm.page_tokens, hd, H / Hkv);
     return RELUX_ERR_UNSUPPORTED;
   }
+  if (b)
+    if (int32_t rc = check_block(p, a, b)) return rc;
   const float rope_base = a->rope_base == 0.f ? 10000.f : a->rope_base;
   SeqBatch sb;
   int32_t rc = layer_batch(p, a->layer, a->n_seqs, a->seq_ids, S, "Append", &sb);
@@ -786,25 +962,39 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) {
     if (rc) return rc;
   }
   const void* dx = nullptr;
-  rc = stage_in(p, p->in_a, a->x, (size_t)M * D * 4, a->x_mem, &dx);
+  rc = stage_in(p, p->in_a, a->x, (size_t)M * D * (x_bf16 ? 2 : 4), a->x_mem, &dx);
   if (rc) return rc;
   const WeightRef proj[3] = {{w.w_q, H * hd}, {w.w_k, Hkv * hd}, {w.w_v, Hkv * hd}};
   const WeightRef outp[1] = {{w.w_o, D}};
   const int n_total = (H + 2 * Hkv) * hd;
   const bool fast = a->mode == RELUX_ATTN_FAST;
   const bool mma = fast && !p->tune.get(RELUX_TUNE_GEMM_GENERIC) && gemm_sm100_eligible(D, proj, 3) && gemm_sm100_eligible(H * hd, outp, 1);
+  if (b && !mma) { set_error("a block needs the tensor-core projections: knob RELUX_TUNE_GEMM_GENERIC is set, or a weight is not 16-byte aligned"); return RELUX_ERR_UNSUPPORTED; }
   const size_t q_es = fast ? 2 : 4;
   const size_t b_q = pad256((size_t)M * H * hd * q_es), b_kv = pad256((size_t)M * Hkv * hd * 4);
-  LayerScratch sc;
-  rc = layer_scratch(p, M, std::max(D, H * hd), std::max(n_total, D), b_q + 2 * b_kv + (size_t)M * H * hd * 4, &sc);
+  LayerScratch sc{};
+  BlockScratch bs{};
+  if (b) {   // in a block of its own: projections with adapters use the layers' scratch themselves
+    rc = block_scratch(p, M, D, n_total, b_q + 2 * b_kv + (size_t)M * H * hd * 4, &bs);
+    sc.rest = bs.rest;
+    sc.a_bf16 = bs.y;
+  } else {
+    rc = layer_scratch(p, M, std::max(D, H * hd), std::max(n_total, D), b_q + 2 * b_kv + (size_t)M * H * hd * 4, &sc);
+  }
   if (rc) return rc;
   void* d_q = sc.rest;
   float* d_k = (float*)(sc.rest + b_q);
   float* d_v = (float*)(sc.rest + b_q + b_kv);
   float* d_attn = (float*)(sc.rest + b_q + 2 * b_kv);
   const int rd = a->rope ? hd : 0;
-  const ProjSeg segs[3] = {{H * hd, rd, d_q, fast ? 1 : 0, S > 1}, {Hkv * hd, rd, d_k, 0, 0}, {Hkv * hd, 0, d_v, 0, 0}};
-  rc = project_and_finish(p, sb, a->layer, (const float*)dx, M, D, S, proj, segs, 3, mma, sc.a_bf16, sc.part, sc.part_cap, faithful);
+  ProjSeg segs[3] = {{H * hd, rd, d_q, fast ? 1 : 0, S > 1}, {Hkv * hd, rd, d_k, 0, 0}, {Hkv * hd, 0, d_v, 0, 0}};
+  std::vector<int32_t> rows_each;
+  if (b) {
+    rows_each.assign((size_t)sb.n_seqs, S);
+    rc = block_projections(p, sb, a, b, dx, M, proj, segs, bs, rows_each.data());
+  } else {
+    rc = project_and_finish(p, sb, a->layer, (const float*)dx, M, D, S, proj, segs, 3, mma, sc.a_bf16, sc.part, sc.part_cap, faithful);
+  }
   if (rc) return rc;
   // append: the GEMM rows are token-major [row][Hkv][hd]; advance = 0 leaves the rows past the cursor (verify).  A short
   // step leaves the append to the attention launch.
@@ -842,8 +1032,15 @@ int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) {
     if (fused_append && a->advance) take_rows_back(p, sb, a->layer);   // nobody appended them
     return rc;
   }
+  if (b) return block_output(p, a, b, o_bf16 ? (const void*)sc.a_bf16 : d_attn, o_bf16, M, H * hd, bs, rows_each.data());
   return output_projection(p, o_bf16 ? nullptr : d_attn, M, H * hd, w.w_o, D, mma, sc.a_bf16, sc.part, sc.part_cap, a->out, a->out_mem);
 }
+int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) { return gqa_layer(p, a, nullptr); }
+int32_t do_gqa_block(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b) {
+  if (!b) { set_error("nil argument struct"); return RELUX_ERR_INVALID_ARG; }
+  return gqa_layer(p, a, b);
+}
+
 
 // ComputeBackend.MatMulFloat32 as matmulBatched3D uses it (interface.go:25-29, mha.go:759-785): C = A x B with A, C float32
 // and B a bf16 weight matrix [K][N] on the device.

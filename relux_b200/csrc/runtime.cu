@@ -306,7 +306,7 @@ static void pool_free_all(Pool* p) {
     if (e) cudaEventDestroy(e);
   fr(p->storage); fr(p->scales); fr(p->meta);
   fr_buf(p->in_a); fr_buf(p->in_b); fr_buf(p->out_buf); fr_buf(p->q_abs); fr_buf(p->part_o); fr_buf(p->part_ml); fr_buf(p->work); fr_buf(p->stream_done); fr_buf(p->seq_list);
-  fr_buf(p->o_lat); fr_buf(p->q_conv); fr_buf(p->rope_tab); fr_buf(p->layer_buf); fr(p->shadow_f32); fr_buf(p->chunk_tab); fr_buf(p->step_rows); fr_buf(p->expand_buf);
+  fr_buf(p->o_lat); fr_buf(p->q_conv); fr_buf(p->rope_tab); fr_buf(p->layer_buf); fr_buf(p->block_buf); fr(p->shadow_f32); fr_buf(p->chunk_tab); fr_buf(p->step_rows); fr_buf(p->expand_buf);
   if (p->h_stage) cudaFreeHost(p->h_stage);
   for (void* block : p->stage_held) cudaFreeHost(block);
   if (p->sel_host) cudaFreeHost(p->sel_host);
@@ -1699,6 +1699,10 @@ API int32_t relux_matmul_f32_bf16(relux_pool_t h, const relux_matmul_args* a) {
   return do_matmul(p, a);
 }
 
+API int32_t relux_gqa_block_cached(relux_pool_t h, const relux_gqa_layer_args* a, const relux_gqa_block_args* b) {
+  GET_POOL(h);
+  return without_exceptions([&] { return do_gqa_block(p, a, b); });
+}
 API int32_t relux_rmsnorm(relux_pool_t h, const relux_rmsnorm_args* a) {
   GET_POOL(h);
   return do_rmsnorm(p, a);

@@ -40,7 +40,7 @@ EXPORTS = [
     "relux_spec_accept", "relux_sampler_sample", "relux_pool_tune", "relux_pool_kernel_ms_list", "relux_matmul_f32_bf16",
     "relux_mla_import_weights", "relux_pool_selftest_wait", "relux_pool_wait_output", "relux_mla_step", "relux_gqa_step", "relux_mla_expand_kv",
     "relux_gqa_read_kv", "relux_gqa_tree_verify", "relux_gqa_tree_commit", "relux_rmsnorm", "relux_int8_rows", "relux_int8_weights",
-    "relux_matmul_int8", "relux_matmul_lora",
+    "relux_matmul_int8", "relux_matmul_lora", "relux_gqa_block_cached",
 ]
 
 
@@ -159,6 +159,16 @@ class GqaLayerArgs(C.Structure):
                 ("rope_base", C.c_float), ("advance", C.c_int32), ("mode", C.c_int32), ("x", C.c_void_p), ("x_dtype", C.c_int32),
                 ("x_mem", C.c_int32), ("out", C.c_void_p), ("out_mem", C.c_int32), ("reserved", C.c_int32 * 3),
                 ("w", C.POINTER(GqaLayerWeights))]
+
+
+class BlockProjection(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("lora_a", C.c_void_p), ("lora_b", C.c_void_p), ("factors", C.c_void_p)]
+
+
+class GqaBlockArgs(C.Structure):
+    _fields_ = [("residual", C.c_void_p), ("residual_out", C.c_void_p), ("norm_weight", C.c_void_p), ("residual_dtype", C.c_int32),
+                ("norm_dtype", C.c_int32), ("eps", C.c_float), ("rank", C.c_int32), ("n_slots", C.c_int32), ("reserved", C.c_int32 * 3),
+                ("adapter", C.c_void_p), ("q", BlockProjection), ("k", BlockProjection), ("v", BlockProjection), ("o", BlockProjection)]
 
 
 class SamplerParams(C.Structure):
@@ -281,6 +291,7 @@ def load():
         L.relux_seq_load_file.argtypes = [C.c_void_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p]
         L.relux_gqa_forward_cached.argtypes = [C.c_void_p, C.POINTER(GqaLayerArgs)]
         L.relux_mla_forward_cached.argtypes = [C.c_void_p, C.POINTER(MlaLayerArgs)]
+        L.relux_gqa_block_cached.argtypes = [C.c_void_p, C.POINTER(GqaLayerArgs), C.POINTER(GqaBlockArgs)]
         L.relux_gqa_read_kv.argtypes = [C.c_void_p, C.POINTER(ReadKvArgs)]
         L.relux_gqa_tree_verify.argtypes = [C.c_void_p, C.POINTER(AttnArgs), C.POINTER(AppendArgs), C.POINTER(TreeArgs)]
         L.relux_gqa_tree_commit.argtypes = [C.c_void_p, C.POINTER(TreeCommitArgs)]

@@ -30,7 +30,8 @@ def buffer(nbytes, flag):
 def structs():
     from relux_b200 import lib as L
     return [("relux_rmsnorm_args", L.RmsnormArgs), ("relux_int8_rows_args", L.Int8RowsArgs), ("relux_int8_weights_args", L.Int8WeightsArgs),
-            ("relux_matmul_int8_args", L.MatmulInt8Args), ("relux_matmul_lora_args", L.MatmulLoraArgs)]
+            ("relux_matmul_int8_args", L.MatmulInt8Args), ("relux_matmul_lora_args", L.MatmulLoraArgs),
+            ("relux_block_projection", L.BlockProjection), ("relux_gqa_block_args", L.GqaBlockArgs)]
 
 
 def test_struct_layouts(tmp_path):

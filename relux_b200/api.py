@@ -48,6 +48,10 @@ def _dtype_flag(a, explicit=None):
     raise TypeError("arrays must be float32 or uint16 (bf16 bits), got %s" % a.dtype)
 
 
+def _flag_or(a, explicit, otherwise):
+    return explicit if explicit is not None else a.dtype_flag if isinstance(a, DeviceBuffer) else otherwise
+
+
 def _size(flag):
     return 2 if flag == L.DTYPE_BF16 else 4
 
@@ -279,16 +283,17 @@ class Pool:
         return res
 
     @staticmethod
-    def _device_only(call, needs, **arrays):
-        """Addresses of device arrays: buffers (checked against `needs` bytes), or plain addresses."""
-        out = {}
-        for name, a in arrays.items():
-            if a is not None and not isinstance(a, (DeviceBuffer, int)):
-                raise TypeError("%s: %s must be device memory" % (call, name))
-            if isinstance(a, DeviceBuffer) and a.nbytes < needs[name]:
-                raise ValueError("%s: %s has %d bytes, %d needed" % (call, name, a.nbytes, needs[name]))
-            out[name] = _ptr(a) or 0
-        return out
+    def _at(call, name, a, need):
+        """Address of a device array: a plain address, None (0), or a buffer of at least `need` bytes."""
+        if a.__class__ is int:
+            return a
+        if a is None:
+            return 0
+        if not isinstance(a, DeviceBuffer):
+            raise TypeError("%s: %s must be device memory" % (call, name))
+        if a.nbytes < need:
+            raise ValueError("%s: %s has %d bytes, %d needed" % (call, name, a.nbytes, need))
+        return a.ptr
 
     def rmsnorm(self, n_rows, d, x, weight=None, eps=1e-5, residual=None, residual_out=None, out=None, codes=None, scales=None, dtype=None,
                 residual_dtype=None, weight_dtype=None, out_dtype=None):
@@ -297,34 +302,34 @@ class Pool:
         nothing else is said."""
         xt = _dtype_flag(x, dtype)
 
-        def flag(a, explicit, otherwise):
-            return explicit if explicit is not None else a.dtype_flag if isinstance(a, DeviceBuffer) else otherwise
-        rt, wt, ot = flag(residual, residual_dtype, xt), flag(weight, weight_dtype, L.DTYPE_BF16), flag(out, out_dtype, xt)
-        size = n_rows * d
-        a = self._device_only("rmsnorm", dict(x=size * _size(xt), residual=size * _size(rt), weight=d * _size(wt), residual_out=size * _size(rt),
-                                              out=size * _size(ot), codes=size, scales=4 * n_rows),
-                              x=x, residual=residual, weight=weight, residual_out=residual_out, out=out, codes=codes, scales=scales)
-        L.check(L.packed["rmsnorm"](self.h, L.pack_rmsnorm(n_rows, d, float(eps), xt, rt, wt, ot, a["x"], a["residual"], a["weight"], a["residual_out"],
-                                                           a["out"], a["codes"], a["scales"])))
+        rt, wt, ot = _flag_or(residual, residual_dtype, xt), _flag_or(weight, weight_dtype, L.DTYPE_BF16), _flag_or(out, out_dtype, xt)
+        at, size = self._at, n_rows * d
+        L.check(L.packed["rmsnorm"](self.h, L.pack_rmsnorm(
+            n_rows, d, eps, xt, rt, wt, ot, at("rmsnorm", "x", x, size * _size(xt)), at("rmsnorm", "residual", residual, size * _size(rt)),
+            at("rmsnorm", "weight", weight, d * _size(wt)), at("rmsnorm", "residual_out", residual_out, size * _size(rt)), at("rmsnorm", "out", out, size * _size(ot)),
+            at("rmsnorm", "codes", codes, size), at("rmsnorm", "scales", scales, 4 * n_rows))))
 
     def int8_rows(self, n_rows, d, x, codes, scales, dtype=None):
         """The 8-bit form of rows x [n_rows, d] (relux_int8_rows): codes int8 [n_rows, d], scales float32 [n_rows]."""
         t = _dtype_flag(x, dtype)
-        a = self._device_only("int8_rows", dict(x=n_rows * d * _size(t), codes=n_rows * d, scales=4 * n_rows), x=x, codes=codes, scales=scales)
-        L.check(L.packed["int8_rows"](self.h, L.pack_int8_rows(n_rows, d, t, a["x"], a["codes"], a["scales"])))
+        at = self._at
+        L.check(L.packed["int8_rows"](self.h, L.pack_int8_rows(n_rows, d, t, at("int8_rows", "x", x, n_rows * d * _size(t)), at("int8_rows", "codes", codes, n_rows * d),
+                                                               at("int8_rows", "scales", scales, 4 * n_rows))))
 
     def int8_weights(self, k, n, w, codes, scales, dtype=None):
         """Weights w [k, n] as 8-bit weights (relux_int8_weights): codes int8 [n, k], scales float32 [n]."""
         t = _dtype_flag(w, dtype)
-        a = self._device_only("int8_weights", dict(w=k * n * _size(t), codes=k * n, scales=4 * n), w=w, codes=codes, scales=scales)
-        L.check(L.packed["int8_weights"](self.h, L.pack_int8_weights(k, n, t, a["w"], a["codes"], a["scales"])))
+        at = self._at
+        L.check(L.packed["int8_weights"](self.h, L.pack_int8_weights(k, n, t, at("int8_weights", "w", w, k * n * _size(t)), at("int8_weights", "codes", codes, k * n),
+                                                                     at("int8_weights", "scales", scales, 4 * n))))
 
     def matmul_int8(self, m, k, n, a, a_scales, w, w_scales, out, out_dtype=None):
         """out [m, n] = a_scales[m] * w_scales[n] * sum a[m] w[n] (relux_matmul_int8): a int8 [m, k], w int8 [n, k], on the device."""
         t = _dtype_flag(out, out_dtype)
-        b = self._device_only("matmul_int8", dict(a=m * k, a_scales=4 * m, w=n * k, w_scales=4 * n, out=m * n * _size(t)), a=a, a_scales=a_scales, w=w,
-                              w_scales=w_scales, out=out)
-        L.check(L.packed["matmul_int8"](self.h, L.pack_matmul_int8(m, k, n, t, b["a"], b["a_scales"], b["w"], b["w_scales"], b["out"])))
+        at = self._at
+        L.check(L.packed["matmul_int8"](self.h, L.pack_matmul_int8(
+            m, k, n, t, at("matmul_int8", "a", a, m * k), at("matmul_int8", "a_scales", a_scales, 4 * m), at("matmul_int8", "w", w, n * k),
+            at("matmul_int8", "w_scales", w_scales, 4 * n), at("matmul_int8", "out", out, m * n * _size(t)))))
 
     def matmul_lora(self, m, k, n, x, w, out, lora_a, lora_b, rank, n_slots, adapter, rows=None, factors=None, accumulate=False, x_dtype=None,
                     out_dtype=None):
@@ -336,11 +341,11 @@ class Pool:
         if ids.ndim != 1 or (nr is not None and nr.shape != ids.shape):
             raise ValueError("matmul_lora: adapters of shape %s, rows of shape %s" % (ids.shape, None if nr is None else nr.shape))
         xt, ot = _dtype_flag(x, x_dtype), _dtype_flag(out, out_dtype)
-        a = self._device_only("matmul_lora", dict(x=m * k * _size(xt), w=2 * k * n, out=m * n * _size(ot), lora_a=2 * n_slots * rank * k,
-                                                  lora_b=2 * n_slots * rank * n, factors=4 * n_slots),
-                              x=x, w=w, out=out, lora_a=lora_a, lora_b=lora_b, factors=factors)
-        L.check(L.packed["matmul_lora"](self.h, L.pack_matmul_lora(m, k, n, rank, n_slots, ids.size, xt, ot, int(bool(accumulate)), a["x"], a["w"], a["lora_a"],
-                                                                   a["lora_b"], a["factors"], _ptr(ids) or 0, _ptr(nr) or 0, a["out"])))
+        at = self._at
+        L.check(L.packed["matmul_lora"](self.h, L.pack_matmul_lora(
+            m, k, n, rank, n_slots, ids.size, xt, ot, 1 if accumulate else 0, at("matmul_lora", "x", x, m * k * _size(xt)), at("matmul_lora", "w", w, 2 * k * n),
+            at("matmul_lora", "lora_a", lora_a, 2 * n_slots * rank * k), at("matmul_lora", "lora_b", lora_b, 2 * n_slots * rank * n),
+            at("matmul_lora", "factors", factors, 4 * n_slots), _ptr(ids) or 0, _ptr(nr) or 0, at("matmul_lora", "out", out, m * n * _size(ot)))))
 
     def import_mla_weights(self, d_model, num_heads, nope_dim, rope_dim, v_dim, dc, dst, q_proj=None, kv_a_proj_with_mqa=None,
                            kv_b_proj=None, o_proj=None, q_pe_proj=None, k_pe_proj=None, fused_rope=False):
@@ -597,15 +602,12 @@ class Pool:
                               rope=int(rope), rope_base=float(rope_base), advance=int(advance), mode=L.ATTN_FAST, x=_ptr(x), x_dtype=xt, x_mem=_mem(x),
                               out=_ptr(out), out_mem=_mem(out), w=C.pointer(w))
 
-        def flag(a, explicit, otherwise):
-            return explicit if explicit is not None else a.dtype_flag if isinstance(a, DeviceBuffer) else otherwise
-
         def projection(n):
             codes, scales = (int8 or {}).get(n, (None, None))
             a, b, f = (lora or {}).get(n, (None, None, None))
             return L.BlockProjection(codes=_ptr(codes), scales=_ptr(scales), lora_a=_ptr(a), lora_b=_ptr(b), factors=_ptr(f))
         block = L.GqaBlockArgs(residual=_ptr(residual), residual_out=_ptr(residual_out), norm_weight=_ptr(norm_weight),
-                               residual_dtype=flag(residual, residual_dtype, xt), norm_dtype=flag(norm_weight, norm_dtype, L.DTYPE_BF16), eps=float(eps), rank=rank,
+                               residual_dtype=_flag_or(residual, residual_dtype, xt), norm_dtype=_flag_or(norm_weight, norm_dtype, L.DTYPE_BF16), eps=float(eps), rank=rank,
                                n_slots=n_slots, adapter=_ptr(slots), **{n[2]: projection(n) for n in names})
         L.check(self.lib.relux_gqa_block_cached(self.h, C.byref(args), C.byref(block)))
 

@@ -357,23 +357,20 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
             __syncwarp();
           }
 #pragma unroll 1
-          for (int h = 0; h < wide && q + h < q1; h += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(acc + q + h, v);
+          for (int h = 0; h < wide && q + h < q1; h += 16) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x8(acc + q + h, *reinterpret_cast<uint32_t(*)[8]>(v));
+            tmem_ld_32x32b_x8(acc + q + h + 8, *reinterpret_cast<uint32_t(*)[8]>(v + 8));
             tmem_ld_wait();
-            float x[32];
+            float x[16];
 #pragma unroll
-            for (int i = 0; i < 32; i++) x[i] = ok ? __uint_as_float(v[i]) : 0.f;
-#pragma unroll 1
-            for (int s = 0; s < size - 1; s++)
-#pragma unroll
-              for (int i = 0; i < 32; i++)
-                if (q + h + i < q1) x[i] += got[(s * (q1 - q0) + q + h - q0 + i) * kRowsOp];
+            for (int i = 0; i < 16; i++) x[i] = ok ? __uint_as_float(v[i]) : 0.f;
+            add_slices(slices, size, q1 - q0, q + h - q0, [&](int i, uint32_t u) { x[i] += __uint_as_float(u); });
             const int col = at.c * 256 + q + h;
             const size_t to = (size_t)(at.row0 + m) * prm.N + col;
             if (prm.adds && mine)
 #pragma unroll
-              for (int i = 0; i < 4; i++)
+              for (int i = 0; i < 2; i++)
                 if (col + 8 * i < prm.N) {   // N is a multiple of 8
                   if (prm.out_bf16) {
                     const uint4 a = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(prm.out) + to) + i);
@@ -388,7 +385,7 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
                 }
             if (prm.out_bf16) {
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
+              for (int i = 0; i < 2; i++) {
                 const uint4 y = make_uint4(round_bf16x2(x[8 * i], x[8 * i + 1]), round_bf16x2(x[8 * i + 2], x[8 * i + 3]), round_bf16x2(x[8 * i + 4], x[8 * i + 5]),
                                            round_bf16x2(x[8 * i + 6], x[8 * i + 7]));
                 if (whole) *reinterpret_cast<uint4*>(tile_smem + swz128(lane, h / 8 + i)) = y;
@@ -396,9 +393,9 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
+              for (int i = 0; i < 4; i++) {
                 const float4 y = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-                if (whole) *reinterpret_cast<float4*>(tile_smem + swz128(lane, i)) = y;
+                if (whole) *reinterpret_cast<float4*>(tile_smem + swz128(lane, h / 4 + i)) = y;
                 else if (mine && col + 4 * i < prm.N) reinterpret_cast<float4*>(reinterpret_cast<float*>(prm.out) + to)[i] = y;
               }
             }

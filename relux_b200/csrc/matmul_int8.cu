@@ -159,23 +159,25 @@ __global__ void __launch_bounds__(192, 1) matmul_int8_kernel(const __grid_consta
         q1 = slice_begin(rank + 1, cols, grain, size);
         swap_slices<SH>(acc, cols, grain, size, rank, slices);
       }
-      const int32_t* const got = reinterpret_cast<const int32_t*>(slices) + warp * 32 + lane;
       if constexpr (!kWide) {
+        const int32_t* const got = reinterpret_cast<const int32_t*>(slices) + warp * 32 + lane;
         // thread = column; a warp writes 64 or 128 bytes of a row at once
+        constexpr int kAtOnce = NC <= 32 ? 8 : 16;
 #pragma unroll 1
-        for (int q = q0; q < q1; q += 8) {
-          uint32_t v[8];
-          tmem_ld_32x32b_x8(acc + q, v);
+        for (int q = q0; q < q1; q += kAtOnce) {
+          uint32_t v[kAtOnce];
+#pragma unroll
+          for (int i = 0; i < kAtOnce; i += 8) tmem_ld_32x32b_x8(acc + q + i, *reinterpret_cast<uint32_t(*)[8]>(v + i));
           tmem_ld_wait();
 #pragma unroll 1
           for (int s = 0; s < size - 1; s++)
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < kAtOnce; i++)
               if (q + i < q1) v[i] += (uint32_t)got[(s * (q1 - q0) + q - q0 + i) * kRowsOp];
-          // (all eight before the first store: one by one each waited for the one before, 180 clocks a row)
-          float x[8];
+          // (all before the first store: one by one each waited for the one before, 180 clocks a row)
+          float x[kAtOnce];
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
+          for (int i = 0; i < kAtOnce; i++) {
             float sa = sa_of[0];
 #pragma unroll
             for (int j = 1; j < (NC + 31) / 32; j++)
@@ -186,11 +188,11 @@ __global__ void __launch_bounds__(192, 1) matmul_int8_kernel(const __grid_consta
           if (prm.out_bf16) {
             uint16_t* const to = reinterpret_cast<uint16_t*>(prm.out) + at;
 #pragma unroll
-            for (int i = 0; i < 8; i++) store_if(to + (size_t)i * prm.N, __bfloat16_as_ushort(__float2bfloat16_rn(x[i])), mine && q + i < q1);
+            for (int i = 0; i < kAtOnce; i++) store_if(to + (size_t)i * prm.N, __bfloat16_as_ushort(__float2bfloat16_rn(x[i])), mine && q + i < q1);
           } else {
             float* const to = reinterpret_cast<float*>(prm.out) + at;
 #pragma unroll
-            for (int i = 0; i < 8; i++) store_if(to + (size_t)i * prm.N, x[i], mine && q + i < q1);
+            for (int i = 0; i < kAtOnce; i++) store_if(to + (size_t)i * prm.N, x[i], mine && q + i < q1);
           }
         }
       } else {
@@ -204,19 +206,16 @@ __global__ void __launch_bounds__(192, 1) matmul_int8_kernel(const __grid_consta
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store before the last has read its tile
           __syncwarp();
 #pragma unroll 1
-          for (int h = 0; h < wide && q + h < q1; h += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(acc + q + h, v);
+          for (int h = 0; h < wide && q + h < q1; h += 16) {   // (sixteen: code that runs once is fetched as it goes)
+            uint32_t v[16];
+            tmem_ld_32x32b_x8(acc + q + h, *reinterpret_cast<uint32_t(*)[8]>(v));
+            tmem_ld_32x32b_x8(acc + q + h + 8, *reinterpret_cast<uint32_t(*)[8]>(v + 8));
             tmem_ld_wait();
-#pragma unroll 1
-            for (int s = 0; s < size - 1; s++)
-#pragma unroll
-              for (int i = 0; i < 32; i++)
-                if (q + h + i < q1) v[i] += (uint32_t)got[(s * (q1 - q0) + q + h - q0 + i) * kRowsOp];
+            add_slices(slices, size, q1 - q0, q + h - q0, [&](int i, uint32_t u) { v[i] += u; });
             const float4* sw = reinterpret_cast<const float4*>(scales + buf * NC + q + h);
-            float x[32];
+            float x[16];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 4; i++) {
               const float4 s4 = sw[i];
               x[4 * i] = int8_scaled(ok ? v[4 * i] : 0u, own, s4.x);
               x[4 * i + 1] = int8_scaled(ok ? v[4 * i + 1] : 0u, own, s4.y);
@@ -225,13 +224,13 @@ __global__ void __launch_bounds__(192, 1) matmul_int8_kernel(const __grid_consta
             }
             if (prm.out_bf16) {
 #pragma unroll
-              for (int i = 0; i < 4; i++)
+              for (int i = 0; i < 2; i++)
                 *reinterpret_cast<uint4*>(tile_smem + swz128(lane, h / 8 + i)) =
                     make_uint4(round_bf16x2(x[8 * i], x[8 * i + 1]), round_bf16x2(x[8 * i + 2], x[8 * i + 3]), round_bf16x2(x[8 * i + 4], x[8 * i + 5]),
                                round_bf16x2(x[8 * i + 6], x[8 * i + 7]));
             } else {
 #pragma unroll
-              for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(tile_smem + swz128(lane, i)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+              for (int i = 0; i < 4; i++) *reinterpret_cast<float4*>(tile_smem + swz128(lane, h / 4 + i)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
           }
           fence_proxy_async();

@@ -9,12 +9,15 @@
 // latency of one load, two reductions and a store.
 #include "common.cuh"
 #include "internal.h"
+#include "tile_gemm.cuh"
 
 namespace relux {
 
 namespace {
 
-constexpr int kMaxRowThreads = 1024, kMaxNV = 4;
+constexpr int kMaxRowThreads = 1024, kMaxNV = 4, kMaxParts = 4;
+// Of a row's traffic, from which on a part of it has a block of its own while there are idle SMs (60 rows of 16384, float32: 6.7 us in one block each, 5.5 in two).
+constexpr int64_t kPartBytes = 128 << 10;
 constexpr int kMaxNormDim = 8 * kMaxRowThreads * kMaxNV;
 constexpr float kTiny = 1e-36f;   // rows without a value this large have no finite 127 / a: zeros
 
@@ -71,114 +74,155 @@ __device__ __forceinline__ void store8(void* p, size_t at, const float (&v)[8], 
   }
 }
 
-// One row a team: `lanes` lanes of a warp (kWarp: a power of two, blockDim.x), or a whole block.  A thread holds kNV times eight values of the row, chunk
-// threadIdx.x + i * blockDim.x.  kNorm = false: only the 8-bit form of x.
-template <bool kXBf16, bool kRBf16, int kNV, bool kWarp, bool kNorm>
-__global__ void __launch_bounds__(kWarp ? 256 : kMaxRowThreads) norm_rows_kernel(const NormParams p) {
-  __shared__ float sums[32], tops[32];
+// One team a row: kLanes: `blockDim.x` lanes of a warp, a power of two, with kNV rows to a team; kBlock; kCluster: a cluster of blocks, a part of the row each.
+// A thread holds kNV times eight values: chunk threadIdx.x + i * blockDim.x of its part of the row, or chunk threadIdx.x of row i.  kNorm = false: only the
+// 8-bit form of x.
+enum Team { kLanes, kBlock, kCluster };
+template <bool kXBf16, bool kRBf16, int kNV, Team kTeam, bool kNorm>
+__global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_rows_kernel(const NormParams p) {
+  constexpr bool kWarp = kTeam == kLanes, kParts = kTeam == kCluster;
+  __shared__ float sums[32], tops[32], part_sums[kMaxParts], part_tops[kMaxParts];
+  constexpr int kRows = kWarp ? kNV : 1, kEach = kWarp ? 1 : kNV;   // rows, and chunks of each
+  const int parts = kParts ? (int)cluster_size() : 1, part = kParts ? (int)cluster_ctarank() : 0;
+  if constexpr (kParts) cluster_arrive();   // this block has begun: its shared memory may be written from the others
   // waits before it releases: a launch behind this one may rely on everything older (launch_chained, head of a chain)
   chain_wait();
   chain_release();
-  const int row = kWarp ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
-  const bool there = !kWarp || row < p.n_rows;
-  const int chunks = p.d >> 3, lanes = blockDim.x;
-  const size_t base = (size_t)(there ? row : 0) * p.d;
+  const int row0 = kWarp ? (blockIdx.x * blockDim.y + threadIdx.y) * kNV : blockIdx.x / parts;
+  const int chunks = p.d >> 3, lanes = blockDim.x, per = (chunks + parts - 1) / parts, first = part * per, end = min(chunks, first + per);
   const bool adds = kNorm && p.residual;
+  auto row_of = [&](int i) { return kWarp ? row0 + i : row0; };
+  auto chunk_of = [&](int i) { return kWarp ? (int)threadIdx.x : first + (int)threadIdx.x + i * lanes; };
+  auto mine = [&](int i) { return row_of(i) < p.n_rows && chunk_of(i) < end; };
+  auto at = [&](int i) { return (size_t)row_of(i) * p.d + 8 * chunk_of(i); };
 
   Raw8 rx[kNV], rr[kNV];
 #pragma unroll
-  for (int i = 0; i < kNV; i++) {
-    const int c = threadIdx.x + i * lanes;
-    if (there && c < chunks) rx[i] = load_raw<kXBf16>(p.x, base + 8 * c);
-  }
+  for (int i = 0; i < kNV; i++)
+    if (mine(i)) rx[i] = load_raw<kXBf16>(p.x, at(i));
   if (adds)
 #pragma unroll
-    for (int i = 0; i < kNV; i++) {
-      const int c = threadIdx.x + i * lanes;
-      if (there && c < chunks) rr[i] = load_raw<kRBf16>(p.residual, base + 8 * c);
-    }
+    for (int i = 0; i < kNV; i++)
+      if (mine(i)) rr[i] = load_raw<kRBf16>(p.residual, at(i));
 
-  float v[kNV][8], sum = 0.f;
+  float v[kNV][8], sum[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; i++) sum[i] = 0.f;
 #pragma unroll
   for (int i = 0; i < kNV; i++) {
-    const int c = threadIdx.x + i * lanes;
-    const bool mine = there && c < chunks;
     widen<kXBf16>(rx[i], v[i]);
     if (adds) {
       float r[8];
       widen<kRBf16>(rr[i], r);
 #pragma unroll
       for (int k = 0; k < 8; k++) v[i][k] += r[k];
-      if (mine && p.residual_out) store8(p.residual_out, base + 8 * c, v[i], kRBf16);
+      if (mine(i) && p.residual_out) store8(p.residual_out, at(i), v[i], kRBf16);
     }
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      if (!mine) v[i][k] = 0.f;
-      if constexpr (kNorm) sum = fmaf(v[i][k], v[i][k], sum);
+      if (!mine(i)) v[i][k] = 0.f;
+      if constexpr (kNorm) sum[i / kEach] = fmaf(v[i][k], v[i][k], sum[i / kEach]);
     }
   }
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   if constexpr (kNorm) {
-    for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int i = 0; i < kRows; i++)
+      for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
     if constexpr (!kWarp) {
-      if (lane == 0) sums[warp] = sum;
+      if (lane == 0) sums[warp] = sum[0];
       __syncthreads();
-      sum = warp_sum(lane < warps ? sums[lane] : 0.f);
+      sum[0] = warp_sum(lane < warps ? sums[lane] : 0.f);
+      if constexpr (kParts) {   // to all parts, which add them up in their order
+        cluster_wait();
+        if (threadIdx.x < parts) store_cluster(mapa_u32(smem_u32(part_sums + part), threadIdx.x), __float_as_uint(sum[0]));
+        cluster_arrive();
+        cluster_wait();
+        sum[0] = 0.f;
+        for (int k = 0; k < parts; k++) sum[0] += part_sums[k];
+      }
     }
-    const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+#pragma unroll
+    for (int i = 0; i < kRows; i++) sum[i] = rsqrtf(fmaf(sum[i], p.inv_d, p.eps));
+    float w[8];
 #pragma unroll
     for (int i = 0; i < kNV; i++) {
-      const int c = threadIdx.x + i * lanes;
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[i][k] *= r;
-      if (p.weight && c < chunks) {
-        float w[8];
-        if (p.weight_bf16) widen<true>(load_raw<true>(p.weight, 8 * c), w);
-        else widen<false>(load_raw<false>(p.weight, 8 * c), w);
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[i][k] *= w[k];
+      const float r = sum[i / kEach];
+      const bool there = chunk_of(i) < end;
+      if (p.weight && there && (!kWarp || i == 0)) {
+        if (p.weight_bf16) widen<true>(load_raw<true>(p.weight, 8 * chunk_of(i)), w);
+        else widen<false>(load_raw<false>(p.weight, 8 * chunk_of(i)), w);
       }
-      if (there && c < chunks && p.out) store8(p.out, base + 8 * c, v[i], p.out_bf16);
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        v[i][k] *= r;
+        if (p.weight && there) v[i][k] *= w[k];
+      }
+      if (mine(i) && p.out) store8(p.out, at(i), v[i], p.out_bf16);
     }
   }
   if (p.codes) {
-    float top = 0.f;
+    float top[kRows];
 #pragma unroll
-    for (int i = 0; i < kNV; i++) {
-      const bool mine = there && threadIdx.x + i * lanes < chunks;
+    for (int i = 0; i < kRows; i++) top[i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; k++) top = top_of(top, mine ? fabsf(v[i][k]) : 0.f);
-    }
-    for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < kNV; i++)
+#pragma unroll
+      for (int k = 0; k < 8; k++) top[i / kEach] = top_of(top[i / kEach], mine(i) ? fabsf(v[i][k]) : 0.f);
+#pragma unroll
+    for (int i = 0; i < kRows; i++)
+      for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) top[i] = top_of(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
     if constexpr (!kWarp) {
-      if (lane == 0) tops[warp] = top;
+      if (lane == 0) tops[warp] = top[0];
       __syncthreads();
-      top = lane < warps ? tops[lane] : 0.f;
+      top[0] = lane < warps ? tops[lane] : 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 16; o > 0; o >>= 1) top[0] = top_of(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+      if constexpr (kParts) {
+        if constexpr (!kNorm) cluster_wait();
+        if (threadIdx.x < parts) store_cluster(mapa_u32(smem_u32(part_tops + part), threadIdx.x), __float_as_uint(top[0]));
+        cluster_arrive();
+        cluster_wait();
+        for (int k = 0; k < parts; k++) top[0] = top_of(top[0], part_tops[k]);
+      }
     }
-    // an infinity or a NaN: the scale is NaN and the codes are zeros, so that the row, and nothing else, comes out as NaN
-    const bool finite = __float_as_uint(top) < 0x7F800000u, some = finite && top >= kTiny;
-    const float up = some ? __fdiv_rn(127.f, top) : 0.f;
-    if (there && threadIdx.x == 0) p.scales[row] = some ? __fdiv_rn(top, 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
 #pragma unroll
     for (int i = 0; i < kNV; i++) {
-      const int c = threadIdx.x + i * lanes;
+      // an infinity or a NaN: the scale is NaN and the codes are zeros, so that the row, and nothing else, comes out as NaN
+      const float t = top[i / kEach];
+      const bool finite = __float_as_uint(t) < 0x7F800000u, some = finite && t >= kTiny;
+      const float up = some ? __fdiv_rn(127.f, t) : 0.f;
+      if (mine(i) && chunk_of(i) == 0) p.scales[row_of(i)] = some ? __fdiv_rn(t, 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
       uint32_t q[8], w[2];
 #pragma unroll
       for (int k = 0; k < 8; k++) q[k] = some ? (uint32_t)__float2int_rn(__fmul_rn(v[i][k], up)) : 0u;
 #pragma unroll
       for (int k = 0; k < 2; k++) w[k] = __byte_perm(__byte_perm(q[4 * k], q[4 * k + 1], 0x0040), __byte_perm(q[4 * k + 2], q[4 * k + 3], 0x0040), 0x5410);
-      if (there && c < chunks) *reinterpret_cast<uint2*>(p.codes + base + 8 * c) = make_uint2(w[0], w[1]);
+      if (mine(i)) *reinterpret_cast<uint2*>(p.codes + at(i)) = make_uint2(w[0], w[1]);
     }
   }
   if (p.by_tma) fence_chained_writes();
 }
 
-template <bool kXBf16, bool kRBf16, int kNV, bool kWarp, bool kNorm>
-int32_t launch_one(Pool* p, const NormParams& prm, dim3 grid, dim3 block) {
-  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, norm_rows_kernel<kXBf16, kRBf16, kNV, kWarp, kNorm>, grid, block, 0,
-                                p->dev->stream, prm));
+template <bool kXBf16, bool kRBf16, int kNV, Team kTeam, bool kNorm>
+int32_t launch_one(Pool* p, const NormParams& prm, dim3 grid, dim3 block, int parts = 1) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = p->dev->stream;
+  cudaLaunchAttribute at[2];
+  cfg.attrs = at;
+  if (p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (kTeam == kCluster) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)parts;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    cfg.numAttrs++;
+  }
+  RELUX_CUDA_TRY(cudaLaunchKernelEx(&cfg, norm_rows_kernel<kXBf16, kRBf16, kNV, kTeam, kNorm>, prm));
   count_launch(p->dev);
   return RELUX_OK;
 }
@@ -189,15 +233,31 @@ int32_t launch_typed(Pool* p, const NormParams& prm) {
     int lanes = 1;
     while (lanes < chunks) lanes *= 2;
     const dim3 block(lanes, 256 / lanes);
-    return launch_one<kXBf16, kRBf16, 1, true, kNorm>(p, prm, dim3((unsigned)((prm.n_rows + (int)block.y - 1) / (int)block.y)), block);
+    auto grid = [&](int rows) { return dim3((unsigned)((prm.n_rows + (int64_t)block.y * rows - 1) / ((int64_t)block.y * rows))); };
+    // four rows a team once the SMs are full of teams of one (20440 rows of 128, bf16: 6.1 us with one, 4.0 with four)
+    if ((int64_t)prm.n_rows * lanes > (int64_t)p->dev->sm_count * 2048) return launch_one<kXBf16, kRBf16, 4, kLanes, kNorm>(p, prm, grid(4), block);
+    return launch_one<kXBf16, kRBf16, 1, kLanes, kNorm>(p, prm, grid(1), block);
   }
-  // a row a block: as few chunks a thread as the block's limit lets
-  const int nv = chunks <= kMaxRowThreads ? 1 : chunks <= 2 * kMaxRowThreads ? 2 : 4;
-  const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
-  const dim3 grid((unsigned)prm.n_rows), block((unsigned)threads);
-  return nv == 1 ? launch_one<kXBf16, kRBf16, 1, false, kNorm>(p, prm, grid, block)
-       : nv == 2 ? launch_one<kXBf16, kRBf16, 2, false, kNorm>(p, prm, grid, block)
-                 : launch_one<kXBf16, kRBf16, 4, false, kNorm>(p, prm, grid, block);
+  int parts = 1;
+  const int64_t bytes = (int64_t)prm.d * ((kXBf16 ? 2 : 4) + (prm.residual ? (kRBf16 ? 4 : 8) : 0) + (prm.out ? (prm.out_bf16 ? 2 : 4) : 0));
+  while (parts < kMaxParts && bytes / parts >= kPartBytes && 2 * parts * prm.n_rows <= p->dev->sm_count) parts *= 2;
+  // As few chunks a thread as the block's limit lets.  Of more rows than are resident at once as many as keep blocks at 256 threads, so that more rows are on their way
+  // (8192 rows of 8192, bf16: 91 us in blocks of 1024 threads, 84 in blocks of 256); of float32 two at most, four cost more registers than they are worth (400 rows of
+  // 16384: 27.8 us and 22.7).
+  const int each = (chunks + parts - 1) / parts;
+  int nv = each <= kMaxRowThreads ? 1 : each <= 2 * kMaxRowThreads ? 2 : 4;
+  if (prm.n_rows > 2 * p->dev->sm_count)
+    while (nv < (kXBf16 && kRBf16 ? 4 : 2) && each > 256 * nv) nv *= 2;
+  const int threads = ((each + nv - 1) / nv + 31) / 32 * 32;
+  const dim3 grid((unsigned)prm.n_rows * (unsigned)parts), block((unsigned)threads);
+  if (parts > 1) {
+    return nv == 1 ? launch_one<kXBf16, kRBf16, 1, kCluster, kNorm>(p, prm, grid, block, parts)
+         : nv == 2 ? launch_one<kXBf16, kRBf16, 2, kCluster, kNorm>(p, prm, grid, block, parts)
+                   : launch_one<kXBf16, kRBf16, 4, kCluster, kNorm>(p, prm, grid, block, parts);
+  }
+  return nv == 1 ? launch_one<kXBf16, kRBf16, 1, kBlock, kNorm>(p, prm, grid, block)
+       : nv == 2 ? launch_one<kXBf16, kRBf16, 2, kBlock, kNorm>(p, prm, grid, block)
+                 : launch_one<kXBf16, kRBf16, 4, kBlock, kNorm>(p, prm, grid, block);
 }
 
 // w [k][n] -> codes [n][k] and a scale per column.  One block per 64 columns: their largest magnitudes, then the codes through shared memory, so

@@ -109,21 +109,23 @@ __device__ __forceinline__ uint32_t tile_setup(TileBars* bars, int size, int fil
   if (size > 1) cluster_arrive();   // this CTA has begun: its shared memory may be written from the others
   return bars->tmem_base;
 }
-// The epilogue's warps, a tile of a cluster of more than one CTA: slices to the others, [from][column of the slice][128 rows], and back when all have arrived.
+// The epilogue's warps, a tile that is cut along K: slices to the others, [from][column of the slice][128 rows], and back when all have arrived.
 // (A warp's store is 128 neighbouring bytes; 16 bytes a thread to rows that lie apart took 3 us longer for 200 x 4096 x 4096.)
-template <class SH>
+// part i of K is CTA i of the cluster, or (kPer 2) the CTA of this one's side in pair i.
+template <class SH, int kPer = 1>
 __device__ __forceinline__ void swap_slices(uint32_t acc, int cols, int grain, int size, int rank, const uint8_t* slices) {
   cluster_wait();
   if constexpr (SH::kWide) {   // the others' stages: they are free once their MMAs are done
     cluster_arrive();
     cluster_wait();
   }
+  const uint32_t side = kPer == 2 ? cluster_ctarank() & 1u : 0u;
   constexpr int kAtOnce = SH::kWide ? 16 : 8;
 #pragma unroll 1
   for (int to = 0; to < size; to++) {
     if (to == rank) continue;
     const int b = slice_begin(to, cols, grain, size), e = slice_begin(to + 1, cols, grain, size);
-    const uint32_t there = mapa_u32(smem_u32(slices) + threadIdx.x * 4, (uint32_t)to) + (uint32_t)((rank < to ? rank : rank - 1) * (e - b)) * (kRowsOp * 4);
+    const uint32_t there = mapa_u32(smem_u32(slices) + threadIdx.x * 4, (uint32_t)to * kPer + side) + (uint32_t)((rank < to ? rank : rank - 1) * (e - b)) * (kRowsOp * 4);
 #pragma unroll 1
     for (int q = b; q < e; q += kAtOnce) {
       uint32_t v[kAtOnce];
@@ -174,9 +176,9 @@ __device__ __forceinline__ void wide_place(int tile, int row_blocks, int col_til
   r = group * kGroup + rest - c * rows;
 }
 
-// Launches `kernel` over `tiles` tiles.  As many CTAs to a tile as leave every tile a cluster that is resident at once: a cluster lies within one of the
-// GPU's groups of SMs, so there are fewer of them than SMs / size (74 of two, 45 of three, 33 of four).
-template <class SH, int kThreads = 192, typename... KArgs, typename... Args>
+// Launches `kernel` over `tiles` tiles of kPer CTAs each, in as many parts of K as leave every tile a cluster that is resident at once: a cluster lies within
+// one of the GPU's groups of SMs, so there are fewer of them than SMs / size (74 of two, 45 of three, 33 of four CTAs).
+template <class SH, int kThreads = 192, int kPer = 1, typename... KArgs, typename... Args>
 int32_t launch_tiles(Pool* p, void (*kernel)(KArgs...), int tiles, int steps, const Args&... args) {
   if (int32_t rc = allow_smem(p->dev, kernel, SH::kSmem)) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -188,18 +190,25 @@ int32_t launch_tiles(Pool* p, void (*kernel)(KArgs...), int tiles, int steps, co
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  int size = 1;
-  for (int s = 2; s <= SH::kMaxCluster && 2 * s <= steps && tiles * s <= p->dev->sm_count; s++) {
-    int& most = p->dev->tile_clusters[s];
-    if (!most) {
-      at[0].val.clusterDim.x = (unsigned)s;
-      cfg.gridDim = dim3((unsigned)(s * p->dev->sm_count));
-      RELUX_CUDA_TRY(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
+  auto resident = [&](int size, int* most) -> int32_t {
+    int& known = p->dev->tile_clusters[size];
+    if (!known) {
+      at[0].val.clusterDim.x = (unsigned)size;
+      cfg.gridDim = dim3((unsigned)(size * p->dev->sm_count));
+      RELUX_CUDA_TRY(cudaOccupancyMaxActiveClusters(&known, kernel, &cfg));
     }
-    if (tiles <= most) size = s;
+    *most = known;
+    return RELUX_OK;
+  };
+  int parts = 1, most = p->dev->sm_count;
+  for (int s = 2; s <= SH::kMaxCluster && 2 * s <= steps && tiles * s * kPer <= p->dev->sm_count; s++) {
+    if (int32_t rc = resident(s * kPer, &most)) return rc;
+    if (tiles <= most) parts = s;
   }
-  cfg.gridDim = dim3((unsigned)(size > 1 ? tiles * size : std::min(tiles, p->dev->sm_count)));
-  at[0].val.clusterDim.x = (unsigned)size;
+  if (parts == 1 && kPer > 1)
+    if (int32_t rc = resident(kPer, &most)) return rc;
+  cfg.gridDim = dim3((unsigned)((parts > 1 ? tiles * parts : std::min(tiles, kPer > 1 ? most : p->dev->sm_count)) * kPer));
+  at[0].val.clusterDim.x = (unsigned)(parts * kPer);
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0 ? 2 : 1;

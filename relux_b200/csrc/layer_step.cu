@@ -650,8 +650,9 @@ inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 }  // namespace
 
-int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, LayerScratch* out) {
-  const size_t part_cap = std::max<size_t>((size_t)64 << 20, (size_t)M * max_n * 4 * 4);
+int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, LayerScratch* out, bool few_pieces) {
+  const size_t piece = (size_t)M * max_n * 4, most = (size_t)64 << 20;
+  const size_t part_cap = pad256(std::max<size_t>(few_pieces ? std::min(most, 8 * piece) : most, piece * 4));
   const size_t off_part = ((size_t)M * max_k * 2 + 255) & ~(size_t)255;
   const size_t off_rest = off_part + part_cap;
   int32_t rc = grow(p->dev, p->layer_buf, off_rest + rest_bytes);

@@ -84,14 +84,6 @@ __device__ __forceinline__ int group_rows(const RunList<kCap>& list, int group, 
   return list.slot[run];
 }
 
-// f v as two bf16 halves, 16 bits of it.
-__device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2& lo) {
-  auto rest = [](float x, float h) { return fabsf(h) < __uint_as_float(0x7F800000u) ? x - h : 0.f; };   // an infinity has no second half
-  v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-  hi = make_uint2(round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
-  lo = make_uint2(round_bf16x2(rest(v.x, bf16_lo(hi.x)), rest(v.y, bf16_hi(hi.x))), round_bf16x2(rest(v.z, bf16_lo(hi.y)), rest(v.w, bf16_hi(hi.y))));
-}
-
 struct DownParams {
   uint16_t* t_hi;         // [M][rank], factors included, the first bf16 half, or nullptr
   uint16_t* t_lo;         // and the second
@@ -142,7 +134,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   for (int s = s0 + warp; s < s1; s += kLoraWarps) {
     const int k = s * 32 + 8 * t;
     const bool in = k < p.K;   // K is a multiple of 8
-    uint4 x[2], w[kTiles];
+    uint4 x[2], low[2], w[kTiles];   // low: of float32 rows that are not rounded for a projection what bf16 leaves
     if (slot >= 0)
 #pragma unroll
       for (int j = 0; j < kTiles; j++) w[j] = in ? load_chained(reinterpret_cast<const uint4*>(a + (size_t)(8 * j + g) * p.K + k)) : none;
@@ -155,17 +147,30 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
       } else {
         const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), u = there ? load_chained(src) : zero, v = there ? load_chained(src + 1) : zero;
-        x[h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+        if (p.x_bf16) {
+          x[h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+        } else {
+          uint2 hi[2], lo[2];
+          split_halves(u, 1.f, hi[0], lo[0]);
+          split_halves(v, 1.f, hi[1], lo[1]);
+          x[h] = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+          low[h] = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
+        }
         if (there && rounds) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[h];
       }
     }
     if (slot >= 0) {
-      const uint32_t lo[4] = {x[0].x, x[1].x, x[0].y, x[1].y}, hi[4] = {x[0].z, x[1].z, x[0].w, x[1].w};
+      auto multiply = [&](const uint4 (&y)[2]) {
+        const uint32_t a0[4] = {y[0].x, y[1].x, y[0].y, y[1].y}, a1[4] = {y[0].z, y[1].z, y[0].w, y[1].w};
 #pragma unroll
-      for (int j = 0; j < kTiles; j++) {
-        mma_bf16_16816(acc[j], lo, w[j].x, w[j].y);
-        mma_bf16_16816(acc[j], hi, w[j].z, w[j].w);
-      }
+        for (int j = 0; j < kTiles; j++) {
+          mma_bf16_16816(acc[j], a0, w[j].x, w[j].y);
+          mma_bf16_16816(acc[j], a1, w[j].z, w[j].w);
+        }
+      };
+      multiply(x);
+      if constexpr (!kXBf16)
+        if (!p.x_bf16) multiply(low);
     }
   }
   if constexpr (!kXBf16) fence_chained_writes();
@@ -595,8 +600,9 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
 
   // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16: one row 11.6 us so and 13.3 with lora_up_kernel, 16
-  // rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are rounded there too, by every CTA for itself: 16 rows x 4096 x 14336 31.4 and 26.0, one 11.9 and 13.3.
-  const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 4) && a->m * a->rank <= 512 && a->n_slots <= 32767;
+  // rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with one launch and most of their
+  // rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
+  const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256) && a->n_slots <= 32767;
   LoraTiles tiles;
   const bool wide = a->w && !narrow && (int64_t)a->n_slots * a->n < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
   if (narrow || wide) {
@@ -620,7 +626,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   }
 
   LayerScratch sc;
-  if ((rc = layer_scratch(p, a->m, a->k, a->n, t_bytes, &sc))) return rc;
+  if ((rc = layer_scratch(p, a->m, a->k, a->w ? a->n : 0, t_bytes, &sc, true))) return rc;
   if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
   down.t = (float*)sc.rest;
   if ((rc = run_down(p, x_bf16, down, requests))) return rc;

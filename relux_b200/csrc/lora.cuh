@@ -1,11 +1,12 @@
 // What lora.cu asks of lora_gemm.cu.
 #pragma once
 
+#include "common.cuh"
 #include "internal.h"
 
 namespace relux {
 
-constexpr int kNarrowRows = 16;     // calls of up to so many rows: one block of rows, rounded by lora_gemm_kernel, adapters on the CUDA cores
+constexpr int kNarrowRows = 16;     // calls of up to so many rows: one block of rows, float32 ones split by lora_gemm_kernel, adapters on the CUDA cores
 constexpr int kMaxLoraTiles = 1024; // row tiles of a longer call
 
 // Tiles of up to 128 neighbouring rows of one adapter.
@@ -14,6 +15,14 @@ struct LoraTiles {
   int32_t row[kMaxLoraTiles], slot[kMaxLoraTiles];
   int16_t rows[kMaxLoraTiles];
 };
+
+// f v as two bf16 halves, 16 bits of it.
+__device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2& lo) {
+  auto rest = [](float x, float h) { return fabsf(h) < __uint_as_float(0x7F800000u) ? x - h : 0.f; };   // an infinity has no second half
+  v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+  hi = make_uint2(round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
+  lo = make_uint2(round_bf16x2(rest(v.x, bf16_lo(hi.x)), rest(v.y, bf16_hi(hi.x))), round_bf16x2(rest(v.z, bf16_lo(hi.y)), rest(v.w, bf16_hi(hi.y))));
+}
 
 // out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kNarrowRows float32 rows of the
 // caller's.  Without tiles (up to kNarrowRows rows): row_slots

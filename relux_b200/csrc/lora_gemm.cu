@@ -2,7 +2,8 @@
 // (lora.cu), which takes t = f_s x A_s^T.  x and W are bf16, W as the layers hold it ([K][N]: MN-major in the MMA), B_s [N][rank].  Tiles as in tile_gemm.cuh.
 //
 //   * Up to 16 rows (bound: HBM, W and the adapters in use): the epilogue's warps and as many helpers, idle while W streams, take t B_s^T on the CUDA cores
-//     in float32, a thread a column, and add it to the sums when they come: a row meets its own adapter only.  (Of 17 to 128 rows that takes longer than W: 64 rows of
+//     in float32, a thread a column, and add it to the sums when they come: a row meets its own adapter only.  float32 rows are split in two bf16 halves on
+//     their way into the stages: W is multiplied with both, which costs MMAs and no bytes.  (Of 17 to 128 rows that takes longer than W: 64 rows of
 //     rank 16 x 4096 x 6144 24 us so, 21 by lora_up_kernel behind a GEMM of its own.)
 //   * Wide tiles (bound: the tensor cores): every tile holds rows of one request, so that t B_s^T is further K steps of the same accumulator, t as two
 //     bf16 halves, hi and lo.  Rows of the tile past the request's end are computed with the wrong adapter and not stored.
@@ -19,7 +20,7 @@ constexpr int kPrefetchSteps = 32;
 constexpr int kRowsT = 16 << 10;   // bytes of t of the rows that the epilogue has at hand at a time
 constexpr int kRing = 8;           // pieces of adapters, eight of a row's rank for a column, that are on their way for each of 256 threads
 template <int NC>
-using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT + kRing * 256 * 16, NC + 8>;   // the adapter's part of a slice lies with the others'
+using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT + kRing * 256 * 16, NC + 8, NC == 256 ? 1 : 2>;   // the adapter's part of a slice lies with the others'
 static_assert(slices_fit(16, 1, 8, 1, LoraShape<16>::kSlices) && slices_fit(256, 32, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage) &&
               slices_fit(256, 64, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage), "no room for the slices");
 
@@ -36,7 +37,7 @@ struct LoraMaps {
 struct LoraGemmParams {
   int32_t M, N, rank, steps, tiles, col_tiles, out_bf16, adds;
   int32_t x_early;           // x was complete before the chain's head began
-  const float* x_f32;        // up to kNarrowRows rows of float32: rounded here, into the stages [M][K]
+  const float* x_f32;        // up to kNarrowRows rows of float32 [M][K]: split here, into the stages
   int32_t K;
   const float* t;            // narrow: [M][rank], without factors
   const uint16_t* b;         // narrow: [slots][N][rank]
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
     const int w_at = kWide ? kStageRows : 0, x_at = kWide ? 0 : kStageRows;   // the M operand comes first
     auto load_w = [&](const Place& at, int k, int s) {   // W of one step; arms the stage for both operands (out-of-range parts of a box are zero-filled and still counted)
       uint8_t* st = smem + s * SH::kStage + w_at;
-      mbar_expect_tx(&bars->full[s], rounds_x ? kStageRows : SH::kStage);
+      mbar_expect_tx(&bars->full[s], rounds_x ? kStageRows : kStageRows + NC * kStepBytes);
 #pragma unroll
       for (int i = 0; i < (kWide ? 4 : 2); i++) tma_load_2d(st + i * 8192, &maps.w, at.c * (kWide ? 256 : kRowsOp) + 64 * i, k * 64, &bars->full[s]);
     };
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
             for (int kk = 0; kk < 4; kk++) {
               const uint64_t w = dW + ((uint32_t)(kk * 2048) >> 4), x = dX + ((uint32_t)(kk * 32) >> 4);
               umma_ss<1>(d, kWide ? x : w, kWide ? w : x, idesc, k != at.k0 || kk != 0);
+              if (rounds_x) umma_ss<1>(d, w, x + ((uint32_t)(NC * kStepBytes) >> 4), idesc, true);   // the rows' second half
             }
           } else if constexpr (kWide) {
             const uint64_t dT = make_desc_kmajor_sw128(st), dB = make_desc_kmajor_sw128(st + kStageRows);
@@ -254,32 +256,39 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
       __syncwarp();
     }
   } else if (!kWide && warp >= 6) {
-    // helpers: the rounding of few float32 rows, and half of t B_s^T
+    // helpers: few float32 rows as two bf16 halves, and half of t B_s^T
     const int id = threadIdx.x - 192;
     int g = 0;
     for (int tile = first; tile < prm.tiles; tile += stride) {
       const Place at = place(tile);
-      if (rounds_x) {   // thread: eight k of a row, four steps' loads on their way together
+      if (rounds_x) {   // thread: eight k of a row, four steps' loads on their way together (of rows that do not exist the stages hold anything: no one reads their sums)
         const int row = id >> 3, chunk = id & 7;
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool there = row < prm.M;
         for (int k = at.k0; k < at.k1; k += 4) {
           float4 u[4], v[4];
+          if (there)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int col = (k + i) * 64 + 8 * chunk;
-            const bool in = k + i < at.k1 && row < prm.M && col < prm.K;   // K is a multiple of 8
-            const float4* src = reinterpret_cast<const float4*>(prm.x_f32 + (size_t)(in ? row : 0) * prm.K + (in ? col : 0));
-            u[i] = in ? load_chained(src) : zero;
-            v[i] = in ? load_chained(src + 1) : zero;
-          }
+            for (int i = 0; i < 4; i++) {
+              const int col = (k + i) * 64 + 8 * chunk;
+              const bool in = k + i < at.k1 && col < prm.K;   // K is a multiple of 8
+              const float4* src = reinterpret_cast<const float4*>(prm.x_f32 + (size_t)row * prm.K + (in ? col : 0));
+              u[i] = in ? load_chained(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[i] = in ? load_chained(src + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (k + i < at.k1) {
               const int s = g % kStages;
               if (g >= kStages) tile_wait(&bars->empty[s], (g / kStages - 1) & 1, bars, prm.status);
-              *reinterpret_cast<uint4*>(smem + s * SH::kStage + kStageRows + swz128(row, chunk)) =
-                  make_uint4(round_bf16x2(u[i].x, u[i].y), round_bf16x2(u[i].z, u[i].w), round_bf16x2(v[i].x, v[i].y), round_bf16x2(v[i].z, v[i].w));
-              fence_proxy_async();
+              if (there) {
+                uint2 hi[2], lo[2];
+                split_halves(u[i], 1.f, hi[0], lo[0]);
+                split_halves(v[i], 1.f, hi[1], lo[1]);
+                uint8_t* const to = smem + s * SH::kStage + kStageRows + swz128(row, chunk);
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+                *reinterpret_cast<uint4*>(to + NC * kStepBytes) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
+                fence_proxy_async();
+              }
               __syncwarp();
               if (lane == 0) mbar_arrive(&bars->full[s]);
               g++;

@@ -89,7 +89,7 @@ struct DownParams {
   uint16_t* t_lo;         // and the second
   const float* factors;
   const void* x;
-  uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr
+  uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr: x in two halves
   const uint16_t* a;      // [slots][rank][K]
   float* t;               // [M][rank], without factors
   int32_t M, K, rank;
@@ -97,7 +97,8 @@ struct DownParams {
 
 // t[row][r] = sum over k of x[row][k] A_s[r][k].  grid (groups, parts of K, kSlice-th parts of the rank), the parts of K a cluster, 8 warps that take 32 k each in turn.  mma.sync: a group is a
 // handful of rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
-template <int kSlice, bool kXBf16, class List>
+enum Rows { kBf16, kRounded, kSplit };   // x: bf16; float32, rounded, for the projection too where it asks; float32, in two halves
+template <int kSlice, Rows kX, class List>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
   constexpr int kTiles = kSlice / 8;
   constexpr int kSlab = kGroupRows * kSlice;
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
   const int r0 = blockIdx.z * kSlice;
   const uint16_t* const a = p.a + ((size_t)max(slot, 0) * p.rank + r0) * p.K;
-  const bool rounds = p.x_bf16 && r0 == 0;
+  const bool rounds = kX == kRounded && p.x_bf16 && r0 == 0;
   if (slot >= 0)   // the adapter's first pieces to L2, while the launch before this one ends (a prefetch returns no data, so it may be early)
     for (int s = s0 + warp; s < min(s1, s0 + 4 * kLoraWarps); s += kLoraWarps) {
       const int k = s * 32 + 8 * t;
@@ -142,12 +143,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
     for (int h = 0; h < 2; h++) {
       const size_t at = (size_t)max(r[h], 0) * p.K + k;
       const bool there = in && r[h] >= 0;
-      if constexpr (kXBf16) {
+      if constexpr (kX == kBf16) {
         x[h] = there ? load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at)) : none;
       } else {
         const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), u = there ? load_chained(src) : zero, v = there ? load_chained(src + 1) : zero;
-        if (p.x_bf16) {
+        if constexpr (kX == kRounded) {
           x[h] = make_uint4(round_bf16x2(u.x, u.y), round_bf16x2(u.z, u.w), round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
         } else {
           uint2 hi[2], lo[2];
@@ -169,11 +170,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
         }
       };
       multiply(x);
-      if constexpr (!kXBf16)
-        if (!p.x_bf16) multiply(low);
+      if constexpr (kX == kSplit) multiply(low);
     }
   }
-  if constexpr (!kXBf16) fence_chained_writes();
+  if constexpr (kX == kRounded) fence_chained_writes();
   if (slot < 0) return;
   // the warps' sums, then the parts', in their order
   const int parts = gridDim.y, part = blockIdx.y;
@@ -472,7 +472,7 @@ int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups
     count_launch(p->dev);
     return RELUX_OK;
   };
-  return x_bf16 ? go(lora_down_kernel<kSlice, true, List>) : go(lora_down_kernel<kSlice, false, List>);
+  return x_bf16 ? go(lora_down_kernel<kSlice, kBf16, List>) : prm.x_bf16 ? go(lora_down_kernel<kSlice, kRounded, List>) : go(lora_down_kernel<kSlice, kSplit, List>);
 }
 template <int kRank, class List>
 int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {

@@ -815,6 +815,7 @@ int32_t check_block(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_bloc
       return rc;
     lora = lora || q->lora_a;
   }
+  if (a->out_mem == RELUX_MEM_DEVICE && (rc = check_dev_align(a->out, "out"))) return rc;
   relux_rmsnorm_args n = block_norm(a, b, a->x, 1);
   n.out = (void*)16;   // an output is given later
   if (a->x_mem == RELUX_MEM_HOST) n.x = n.out;

@@ -88,12 +88,12 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
   // waits before it releases: a launch behind this one may rely on everything older (launch_chained, head of a chain)
   chain_wait();
   chain_release();
-  const int row0 = kWarp ? (blockIdx.x * blockDim.y + threadIdx.y) * kNV : blockIdx.x / parts;
+  const uint32_t row0 = kWarp ? (blockIdx.x * blockDim.y + threadIdx.y) * kNV : blockIdx.x / parts;   // past 2^31 in the last block of that many rows
   const int chunks = p.d >> 3, lanes = blockDim.x, per = (chunks + parts - 1) / parts, first = part * per, end = min(chunks, first + per);
   const bool adds = kNorm && p.residual;
   auto row_of = [&](int i) { return kWarp ? row0 + i : row0; };
   auto chunk_of = [&](int i) { return kWarp ? (int)threadIdx.x : first + (int)threadIdx.x + i * lanes; };
-  auto mine = [&](int i) { return row_of(i) < p.n_rows && chunk_of(i) < end; };
+  auto mine = [&](int i) { return row_of(i) < (uint32_t)p.n_rows && chunk_of(i) < end; };
   auto at = [&](int i) { return (size_t)row_of(i) * p.d + 8 * chunk_of(i); };
 
   Raw8 rx[kNV], rr[kNV];
@@ -240,7 +240,7 @@ int32_t launch_typed(Pool* p, const NormParams& prm) {
   }
   int parts = 1;
   const int64_t bytes = (int64_t)prm.d * ((kXBf16 ? 2 : 4) + (prm.residual ? (kRBf16 ? 4 : 8) : 0) + (prm.out ? (prm.out_bf16 ? 2 : 4) : 0));
-  while (parts < kMaxParts && bytes / parts >= kPartBytes && 2 * parts * prm.n_rows <= p->dev->sm_count) parts *= 2;
+  while (parts < kMaxParts && bytes / parts >= kPartBytes && prm.n_rows <= p->dev->sm_count / (2 * parts)) parts *= 2;
   // As few chunks a thread as the block's limit lets.  Of more rows than are resident at once as many as keep blocks at 256 threads, so that more rows are on their way
   // (8192 rows of 8192, bf16: 91 us in blocks of 1024 threads, 84 in blocks of 256); of float32 two at most, four cost more registers than they are worth (400 rows of
   // 16384: 27.8 us and 22.7).

@@ -204,6 +204,8 @@ def test_refusals_leave_the_cache_as_it_was(dev):
     refused(L.ERR_INVALID_ARG, int8={"w_q": (layer.int8["w_q"][0], None)})
     refused(L.ERR_INVALID_ARG, lora={"w_q": (layer.lora["w_q"][0], None, None)}, rank=16, n_slots=3, adapter=[0, 1])
     refused(L.ERR_INVALID_ARG, norm_weight=layer.dg.ptr + 4)
+    refused(L.ERR_INVALID_ARG, out=out.ptr + 4)
+    refused(L.ERR_INVALID_ARG, x=dx.ptr + 4, x_dtype=0)
     with pytest.raises(L.ReluxCudaError):
         pool.tune(L.TUNE_GEMM_GENERIC, 1)
         try:

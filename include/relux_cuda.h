@@ -685,7 +685,7 @@ int32_t relux_int8_weights(relux_pool_t pool, const relux_int8_weights_args* arg
 
 /* C [m][n] = a_scales[m] * w_scales[n] * sum over k of a[m][k] * w[n][k]: relux_matmul_f32_bf16 on 8-bit rows and weights.  The sum is
  * exact (32-bit whole numbers), so a row's result does not depend on the rows around it nor on the GPU's schedule; it is rounded to float32, multiplied by
- * the row's scale, then by the column's, and rounded once more for a bf16 result.  k a multiple of 16, up to 131056, n of 8.
+ * the row's scale, then by the column's, and rounded once more for a bf16 result.  k a multiple of 16, up to 131056, n of 8.  out must not overlap an input.
  * Asynchronous on the handle's stream.  No counterpart in the reference. */
 typedef struct relux_matmul_int8_args {
   int32_t m, k, n, out_dtype;
@@ -706,7 +706,7 @@ int32_t relux_matmul_int8(relux_pool_t pool, const relux_matmul_int8_args* args)
  * w NULL: no shared projection (it came from relux_matmul_int8, say: with accumulate the adapters are added to what out holds).
  * Requests own neighbouring rows, n_rows[i] of them in order; several may name the same slot.  The host arrays are read before the call returns; a captured
  * call keeps its adapters' places in the batch, the slots' contents are read at every launch.
- * Shapes: k and n multiples of 8, rank 8, 16, 32, 64 or 128 (a smaller adapter is filled up with zeros).  Adapters as checkpoints hold them (lora_A [rank][in],
+ * Shapes: m up to 2^30, k and n multiples of 8, rank 8, 16, 32, 64 or 128 (a smaller adapter is filled up with zeros).  Adapters as checkpoints hold them (lora_A [rank][in],
  * lora_B [out][rank]).  out must not overlap x.  Asynchronous on the handle's stream.  No counterpart in the reference, which serves one model. */
 typedef struct relux_matmul_lora_args {
   int32_t m, k, n;

@@ -25,6 +25,7 @@ namespace {
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
 constexpr int kMaxParts = 8, kGroupRows = 16;
+constexpr int kMostRows = 1 << 30;                   // places are counted in 32 bits, a group past the last
 constexpr int kFewRows = 128, kSomeRows = 512;       // of up to so many rows a list names each
 constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
 
@@ -579,6 +580,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     }
     rows += n;
   }
+  if (a->m > kMostRows) { set_error("matmul_lora: M=%d above %d", a->m, kMostRows); return RELUX_ERR_UNSUPPORTED; }
   if (rows != a->m) { set_error("matmul_lora: the requests have %lld rows, M=%d", (long long)rows, a->m); return RELUX_ERR_INVALID_ARG; }
   int32_t rc;
   if ((rc = check_dev_align(a->x, "x")) || (rc = check_dev_align(a->w, "w")) || (rc = check_dev_align(a->lora_a, "lora_a")) || (rc = check_dev_align(a->lora_b, "lora_b")) ||

@@ -396,8 +396,8 @@ int32_t launch_matmul_int8(Pool* p, int M, int K, int N, const int8_t* a, const 
   prm.M = M;
   prm.N = N;
   prm.steps = (K + kStepBytes - 1) / kStepBytes;
-  prm.row_blocks = (M + PairShape::kTile - 1) / PairShape::kTile;
-  prm.col_tiles = (N + (wide ? PairShape::kTile : kRowsOp) - 1) / (wide ? PairShape::kTile : kRowsOp);
+  prm.row_blocks = (M - 1) / PairShape::kTile + 1;
+  prm.col_tiles = (N - 1) / (wide ? PairShape::kTile : kRowsOp) + 1;
   const int64_t tiles = wide ? (int64_t)prm.row_blocks * prm.col_tiles : prm.col_tiles;
   if (tiles * prm.steps >= (int64_t)1 << 31) { set_error("a product of more than 2^31 steps"); return RELUX_ERR_UNSUPPORTED; }
   prm.tiles = (int)tiles;

@@ -201,7 +201,7 @@ int32_t launch_tiles(Pool* p, void (*kernel)(KArgs...), int tiles, int steps, co
     return RELUX_OK;
   };
   int parts = 1, most = p->dev->sm_count;
-  for (int s = 2; s <= SH::kMaxCluster && 2 * s <= steps && tiles * s * kPer <= p->dev->sm_count; s++) {
+  for (int s = 2; s <= SH::kMaxCluster && 2 * s <= steps && tiles <= p->dev->sm_count / (s * kPer); s++) {
     if (int32_t rc = resident(s * kPer, &most)) return rc;
     if (tiles <= most) parts = s;
   }

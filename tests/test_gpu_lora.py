@@ -185,6 +185,45 @@ def test_infinities_and_nan_stay_with_their_request(dev, pool):
     c.free()
 
 
+# requests of a row each, few and so few that float32 rows are split; requests whose tiles are nearly full, with rows past their ends
+FORMS = [([1] * 12, [0, 1, 2, -1] * 3, True), ([1] * 8, [0, 1, 2, -1] * 2, False), ([250, 128, 380, 90], [0, 1, 2, -1], True), ([90, 380, 128, 250], [2, -1, 1, 0], False)]
+
+
+@pytest.mark.parametrize("rows,adapter,x_bf16", FORMS)
+@pytest.mark.parametrize("out_bf16", [False, True])
+@pytest.mark.parametrize("K,N,rank", [(264, 392, 16), (2048, 520, 8), (520, 1288, 32)])
+def test_added_in_every_form(dev, pool, rows, adapter, x_bf16, out_bf16, K, N, rank):
+    from oracle import binding as orc
+    rng = np.random.default_rng(16)
+    c = Case(dev, rng, rows, adapter, K, N, rank, 3, x_bf16, out_bf16)
+    before = G.bf16(rng.standard_normal((c.M, c.N)).astype(np.float32))
+    c.out.upload(orc.bf16_from_f32(before) if out_bf16 else before)
+    c.call(pool, accumulate=True)
+    out, bound = c.plain(before)
+    assert (np.abs(c.get() - out) <= bound + np.abs(before) * 2.0 ** -23).all()
+    c.free()
+
+
+@pytest.mark.parametrize("rows,adapter,x_bf16", FORMS)
+def test_infinities_and_nan_in_every_form(dev, pool, rows, adapter, x_bf16):
+    """The second adapter and a row of the third's hold NaN, a column of the third an infinity: what the formula leaves finite is."""
+    from oracle import binding as orc
+    rng = np.random.default_rng(17)
+    c = Case(dev, rng, rows, adapter, 264, 392, 16, 3, x_bf16)
+    c.a[1, 3, 7], c.b[2, 5, :] = np.nan, np.inf
+    c.da.upload(orc.bf16_from_f32(c.a)), c.db.upload(orc.bf16_from_f32(c.b))
+    ids = np.repeat(np.asarray(adapter), rows)
+    bad = np.flatnonzero(ids == 2)[-1]
+    c.x[bad, 9], c.x[np.flatnonzero(ids == -1)[0], 8] = np.inf, np.nan
+    c.dx.upload(orc.bf16_from_f32(c.x) if x_bf16 else c.x)
+    c.call(pool)
+    got, (out, bound) = c.get(), c.plain()
+    fine = np.isfinite(out)
+    assert fine[ids == 0].all() and not fine[ids == 1].any() and not fine[bad].any()
+    assert (np.isfinite(got) == fine).all() and (np.abs(got - out)[fine] <= bound[fine]).all()
+    c.free()
+
+
 def test_rows_alone_and_among_others(dev, pool):
     """A request's rows are the same bits whatever other requests' adapters are."""
     rng = np.random.default_rng(13)
@@ -280,4 +319,5 @@ def test_refusals(dev, pool):
     refused(L.ERR_UNSUPPORTED, k=60)
     refused(L.ERR_UNSUPPORTED, n=60)
     refused(L.ERR_UNSUPPORTED, rank=24)
+    refused(L.ERR_UNSUPPORTED, m=(1 << 30) + 8, rows=[1 << 30, 8], x=b.ptr, out=b.ptr, x_dtype=L.DTYPE_BF16, out_dtype=L.DTYPE_BF16)
     b.free()

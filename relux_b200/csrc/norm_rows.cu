@@ -7,6 +7,8 @@
 // Everything is float32 from the inputs to the one rounding of each result (h is normalised before it is rounded for residual_out); sums of
 // squares are taken by thread, then by tree.  Bound: HBM, x and the residual read once, the results written once; up to some hundred KB the
 // latency of one load, two reductions and a store.
+#include <type_traits>
+
 #include "common.cuh"
 #include "internal.h"
 #include "tile_gemm.cuh"
@@ -40,17 +42,23 @@ __device__ __forceinline__ float top_of(float a, float b) {   // a NaN stays one
   return d;
 }
 
-struct alignas(16) Raw8 {   // eight values as they lie in memory
+// Eight values of a thread: a chunk of eight neighbours, or (kApart, where a type is float32) two quads that lie a team's width apart, so that a warp's load is of whole
+// 32-byte sectors: halves of them, 16 bytes a thread of 32, ask L2 for everything twice.
+struct alignas(16) Raw8 {   // as they lie in memory
   uint4 lo, hi;             // hi: float32 only
 };
-template <bool kBf16>
-__device__ __forceinline__ Raw8 load_raw(const void* p, size_t at) {
+template <bool kBf16, bool kApart>
+__device__ __forceinline__ Raw8 load_raw(const void* p, size_t lo, size_t hi) {
   Raw8 r;
-  if constexpr (kBf16) {
-    r.lo = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at));
+  if constexpr (kBf16 && kApart) {
+    const uint2 a = load_chained(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + lo)),
+                b = load_chained(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + hi));
+    r.lo = make_uint4(a.x, a.y, b.x, b.y);
+  } else if constexpr (kBf16) {
+    r.lo = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + lo));
   } else {
-    r.lo = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at));
-    r.hi = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at) + 1);
+    r.lo = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + lo));
+    r.hi = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + hi));
   }
   return r;
 }
@@ -64,23 +72,36 @@ __device__ __forceinline__ void widen(const Raw8& r, float (&v)[8]) {
     v[4] = __uint_as_float(r.hi.x); v[5] = __uint_as_float(r.hi.y); v[6] = __uint_as_float(r.hi.z); v[7] = __uint_as_float(r.hi.w);
   }
 }
-__device__ __forceinline__ void store8(void* p, size_t at, const float (&v)[8], bool bf16) {
+template <bool kApart>
+__device__ __forceinline__ void store8(void* p, size_t lo, size_t hi, const float (&v)[8], bool bf16) {
   if (bf16) {
-    reinterpret_cast<uint4*>(p)[at >> 3] = make_uint4(round_bf16x2(v[0], v[1]), round_bf16x2(v[2], v[3]), round_bf16x2(v[4], v[5]), round_bf16x2(v[6], v[7]));
+    const uint4 u = make_uint4(round_bf16x2(v[0], v[1]), round_bf16x2(v[2], v[3]), round_bf16x2(v[4], v[5]), round_bf16x2(v[6], v[7]));
+    uint16_t* const q = reinterpret_cast<uint16_t*>(p);
+    if constexpr (kApart) {
+      *reinterpret_cast<uint2*>(q + lo) = make_uint2(u.x, u.y);
+      *reinterpret_cast<uint2*>(q + hi) = make_uint2(u.z, u.w);
+    } else {
+      *reinterpret_cast<uint4*>(q + lo) = u;
+    }
   } else {
-    float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at);
-    q[0] = make_float4(v[0], v[1], v[2], v[3]);
-    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    float* const q = reinterpret_cast<float*>(p);
+    *reinterpret_cast<float4*>(q + lo) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(q + hi) = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
 
+__device__ __forceinline__ void store4(void* p, size_t at, const float (&v)[8], bool bf16) {   // the first four of them
+  if (bf16) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + at) = make_uint2(round_bf16x2(v[0], v[1]), round_bf16x2(v[2], v[3]));
+  else *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
 // One team a row: kLanes: `blockDim.x` lanes of a warp, a power of two, with kNV rows to a team; kBlock; kCluster: a cluster of blocks, a part of the row each.
-// A thread holds kNV times eight values: chunk threadIdx.x + i * blockDim.x of its part of the row, or chunk threadIdx.x of row i.  kNorm = false: only the
+// A thread holds kNV times eight values: of its part of the row the chunks threadIdx.x + i * blockDim.x, or chunk threadIdx.x of row i.  kNorm = false: only the
 // 8-bit form of x.
 enum Team { kLanes, kBlock, kCluster };
 template <bool kXBf16, bool kRBf16, int kNV, Team kTeam, bool kNorm>
 __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_rows_kernel(const NormParams p) {
-  constexpr bool kWarp = kTeam == kLanes, kParts = kTeam == kCluster;
+  constexpr bool kWarp = kTeam == kLanes, kParts = kTeam == kCluster, kApart = !kXBf16 || !kRBf16;
   __shared__ float sums[32], tops[32], part_sums[kMaxParts], part_tops[kMaxParts];
   constexpr int kRows = kWarp ? kNV : 1, kEach = kWarp ? 1 : kNV;   // rows, and chunks of each
   const int parts = kParts ? (int)cluster_size() : 1, part = kParts ? (int)cluster_ctarank() : 0;
@@ -91,21 +112,30 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
   const uint32_t row0 = kWarp ? (blockIdx.x * blockDim.y + threadIdx.y) * kNV : blockIdx.x / parts;   // past 2^31 in the last block of that many rows
   const int chunks = p.d >> 3, lanes = blockDim.x, per = (chunks + parts - 1) / parts, first = part * per, end = min(chunks, first + per);
   const bool adds = kNorm && p.residual;
-  auto row_of = [&](int i) { return kWarp ? row0 + i : row0; };
-  auto chunk_of = [&](int i) { return kWarp ? (int)threadIdx.x : first + (int)threadIdx.x + i * lanes; };
-  auto mine = [&](int i) { return row_of(i) < (uint32_t)p.n_rows && chunk_of(i) < end; };
-  auto at = [&](int i) { return (size_t)row_of(i) * p.d + 8 * chunk_of(i); };
-
   Raw8 rx[kNV], rr[kNV];
+  float v[kNV][8], sum[kRows];
+  auto row_of = [&](int i) { return kWarp ? row0 + i : row0; };
+  auto quad_of = [&](int i, int h) {   // half h of the eight values
+    const int j = kWarp ? 0 : i;
+    return 2 * first + (kApart ? (int)threadIdx.x + (2 * j + h) * lanes : 2 * ((int)threadIdx.x + j * lanes) + h);
+  };
+  auto there = [&](int i, int h) { return quad_of(i, h) < 2 * end; };   // (not apart: both halves or none)
+  auto mine = [&](int i, int h) { return row_of(i) < (uint32_t)p.n_rows && there(i, h); };
+  auto at = [&](int i, int h) { return (size_t)row_of(i) * p.d + 4 * quad_of(i, h); };
+  auto load = [&](auto bf16, const void* from, int i) { return load_raw<decltype(bf16)::value, kApart>(from, at(i, 0), mine(i, 1) ? at(i, 1) : at(i, 0)); };
+  auto store = [&](void* to, int i, bool bf16) {
+    if (mine(i, 1)) store8<kApart>(to, at(i, 0), at(i, 1), v[i], bf16);
+    else if (mine(i, 0)) store4(to, at(i, 0), v[i], bf16);
+  };
+
 #pragma unroll
   for (int i = 0; i < kNV; i++)
-    if (mine(i)) rx[i] = load_raw<kXBf16>(p.x, at(i));
+    if (mine(i, 0)) rx[i] = load(std::bool_constant<kXBf16>(), p.x, i);
   if (adds)
 #pragma unroll
     for (int i = 0; i < kNV; i++)
-      if (mine(i)) rr[i] = load_raw<kRBf16>(p.residual, at(i));
+      if (mine(i, 0)) rr[i] = load(std::bool_constant<kRBf16>(), p.residual, i);
 
-  float v[kNV][8], sum[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; i++) sum[i] = 0.f;
 #pragma unroll
@@ -116,11 +146,11 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
       widen<kRBf16>(rr[i], r);
 #pragma unroll
       for (int k = 0; k < 8; k++) v[i][k] += r[k];
-      if (mine(i) && p.residual_out) store8(p.residual_out, at(i), v[i], kRBf16);
+      if (p.residual_out) store(p.residual_out, i, kRBf16);
     }
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      if (!mine(i)) v[i][k] = 0.f;
+      if (!mine(i, k / 4)) v[i][k] = 0.f;
       if constexpr (kNorm) sum[i / kEach] = fmaf(v[i][k], v[i][k], sum[i / kEach]);
     }
   }
@@ -148,17 +178,17 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
 #pragma unroll
     for (int i = 0; i < kNV; i++) {
       const float r = sum[i / kEach];
-      const bool there = chunk_of(i) < end;
-      if (p.weight && there && (!kWarp || i == 0)) {
-        if (p.weight_bf16) widen<true>(load_raw<true>(p.weight, 8 * chunk_of(i)), w);
-        else widen<false>(load_raw<false>(p.weight, 8 * chunk_of(i)), w);
+      if (p.weight && there(i, 0) && (!kWarp || i == 0)) {
+        const size_t lo = 4 * quad_of(i, 0), hi = there(i, 1) ? 4 * quad_of(i, 1) : lo;
+        if (p.weight_bf16) widen<true>(load_raw<true, kApart>(p.weight, lo, hi), w);
+        else widen<false>(load_raw<false, kApart>(p.weight, lo, hi), w);
       }
 #pragma unroll
       for (int k = 0; k < 8; k++) {
         v[i][k] *= r;
-        if (p.weight && there) v[i][k] *= w[k];
+        if (p.weight && there(i, 0)) v[i][k] *= w[k];
       }
-      if (mine(i) && p.out) store8(p.out, at(i), v[i], p.out_bf16);
+      if (p.out) store(p.out, i, p.out_bf16);
     }
   }
   if (p.codes) {
@@ -168,7 +198,7 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
 #pragma unroll
     for (int i = 0; i < kNV; i++)
 #pragma unroll
-      for (int k = 0; k < 8; k++) top[i / kEach] = top_of(top[i / kEach], mine(i) ? fabsf(v[i][k]) : 0.f);
+      for (int k = 0; k < 8; k++) top[i / kEach] = top_of(top[i / kEach], mine(i, k / 4) ? fabsf(v[i][k]) : 0.f);
 #pragma unroll
     for (int i = 0; i < kRows; i++)
       for (int o = kWarp ? lanes >> 1 : 16; o > 0; o >>= 1) top[i] = top_of(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
@@ -192,13 +222,19 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
       const float t = top[i / kEach];
       const bool finite = __float_as_uint(t) < 0x7F800000u, some = finite && t >= kTiny;
       const float up = some ? __fdiv_rn(127.f, t) : 0.f;
-      if (mine(i) && chunk_of(i) == 0) p.scales[row_of(i)] = some ? __fdiv_rn(t, 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
+      if (mine(i, 0) && quad_of(i, 0) == 0) p.scales[row_of(i)] = some ? __fdiv_rn(t, 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
       uint32_t q[8], w[2];
 #pragma unroll
       for (int k = 0; k < 8; k++) q[k] = some ? (uint32_t)__float2int_rn(__fmul_rn(v[i][k], up)) : 0u;
 #pragma unroll
       for (int k = 0; k < 2; k++) w[k] = __byte_perm(__byte_perm(q[4 * k], q[4 * k + 1], 0x0040), __byte_perm(q[4 * k + 2], q[4 * k + 3], 0x0040), 0x5410);
-      if (mine(i)) *reinterpret_cast<uint2*>(p.codes + at(i)) = make_uint2(w[0], w[1]);
+      if constexpr (kApart) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (mine(i, h)) *reinterpret_cast<uint32_t*>(p.codes + at(i, h)) = w[h];
+      } else {
+        if (mine(i, 0)) *reinterpret_cast<uint2*>(p.codes + at(i, 0)) = make_uint2(w[0], w[1]);
+      }
     }
   }
   if (p.by_tma) fence_chained_writes();

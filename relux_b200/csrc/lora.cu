@@ -1,8 +1,8 @@
 // A shared projection with low-rank adapters of many requests beside it: C[m] = x[m] W + f_s (x[m] A_s^T) B_s^T, s the adapter of the
 // request that row m belongs to, or none.  A_s [rank][K], B_s [N][rank] in slots of two arrays, as checkpoints hold them (lora_A, lora_B).
 //
-// Two launches: lora_down_kernel takes t = x A_s^T, and rounds a float32 x to bf16 while it holds the rows; lora_gemm_kernel (lora_gemm.cu) is the projection,
-// whose epilogue or last steps add t B_s^T.  Three where the rows are many and of so many requests that tiles of one request's rows would be mostly
+// Two launches: lora_down_kernel, or lora_rows_kernel (lora_rows.cu) for tiles of one request's rows, takes t = x A_s^T, and rounds a float32 x to bf16 while it holds the
+// rows; lora_gemm_kernel (lora_gemm.cu) is the projection, whose epilogue or last steps add t B_s^T.  Three where the rows are many and of so many requests that tiles of one request's rows would be mostly
 // empty, or where the projection is not this call's: lora_down_kernel, the projection's GEMM (skinny_gemm_sm100_kernel), and lora_up_kernel, which adds up
 // the GEMM's pieces and, on the way out, t B_s^T.
 // No tile of a product holds rows of one request and another's adapter: a product with that by zeros would carry its infinities and NaN over.
@@ -86,9 +86,6 @@ __device__ __forceinline__ int group_rows(const RunList<kCap>& list, int group, 
 }
 
 struct DownParams {
-  uint16_t* t_hi;         // [M][rank], factors included, the first bf16 half, or nullptr
-  uint16_t* t_lo;         // and the second
-  const float* factors;
   const void* x;
   uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr: x in two halves
   const uint16_t* a;      // [slots][rank][K]
@@ -232,16 +229,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
     const int row = rows[4 * i / kSlice];
     if (row < 0) continue;
     const size_t to = (size_t)row * p.rank + r0 + 4 * i % kSlice;
-    if (p.t_hi) {
-      uint2 hi, lo;
-      split_halves(sum[e], p.factors ? load_chained(p.factors + slot) : 1.f, hi, lo);
-      *reinterpret_cast<uint2*>(p.t_hi + to) = hi;
-      *reinterpret_cast<uint2*>(p.t_lo + to) = lo;
-    } else {
-      *reinterpret_cast<float4*>(p.t + to) = sum[e];
-    }
+    *reinterpret_cast<float4*>(p.t + to) = sum[e];
   }
-  if (p.t_hi) fence_chained_writes();
 }
 
 struct UpParams {
@@ -593,7 +582,6 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   const std::vector<Request> requests = merged_requests(a->n_seqs, a->n_rows, a->adapter);
   const bool x_bf16 = a->x_dtype == RELUX_DTYPE_BF16;
   DownParams down{};
-  down.factors = a->factors;
   down.x = a->x;
   down.a = (const uint16_t*)a->lora_a;
   down.M = a->m;
@@ -607,24 +595,22 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256) && a->n_slots <= 32767;
   LoraTiles tiles;
   const bool wide = a->w && !narrow && (int64_t)a->n_slots * a->n < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
-  if (narrow || wide) {
-    const bool rounds = wide && !x_bf16;
-    const size_t x_bytes = rounds ? ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255 : 0;
+  if (wide) {
+    const size_t x_bytes = x_bf16 ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
     if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes))) return rc;
-    char* const base = (char*)p->layer_buf.p;
-    if (rounds) down.x_bf16 = (uint16_t*)base;
-    const uint16_t* x = x_bf16 ? (const uint16_t*)a->x : down.x_bf16;
-    if (narrow) {
-      down.t = (float*)(base + x_bytes);
-    } else {
-      down.t_hi = (uint16_t*)(base + x_bytes);
-      down.t_lo = down.t_hi + (size_t)a->m * a->rank;
-    }
+    uint16_t* const rounded = x_bf16 ? nullptr : (uint16_t*)p->layer_buf.p;
+    uint16_t* const t_hi = (uint16_t*)((char*)p->layer_buf.p + x_bytes);
+    uint16_t* const t_lo = t_hi + (size_t)a->m * a->rank;
+    if ((rc = launch_lora_rows(p, a, tiles, rounded, t_hi, t_lo))) return rc;
+    return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : rounded, nullptr, &tiles, nullptr, t_hi, t_lo);
+  }
+  if (narrow) {
+    if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;
+    down.t = (float*)p->layer_buf.p;
     if ((rc = run_down(p, x_bf16, down, requests))) return rc;
-    if (wide) return launch_lora_gemm(p, a, x, nullptr, &tiles, nullptr, down.t_hi, down.t_lo);
     int16_t row_slots[kNarrowRows];
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
-    return launch_lora_gemm(p, a, x, row_slots, nullptr, down.t, nullptr, nullptr);
+    return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : nullptr, row_slots, nullptr, down.t, nullptr, nullptr);
   }
 
   LayerScratch sc;

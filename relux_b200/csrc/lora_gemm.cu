@@ -1,5 +1,5 @@
 // The shared projection of a call with low-rank adapters, C[m] = x[m] W + t[m] B_s^T, s the adapter of row m, in one launch behind lora_down_kernel
-// (lora.cu), which takes t = f_s x A_s^T.  x and W are bf16, W as the layers hold it ([K][N]: MN-major in the MMA), B_s [N][rank].  Tiles as in tile_gemm.cuh.
+// (lora.cu) or lora_rows_kernel (lora_rows.cu), which take t = x A_s^T.  x and W are bf16, W as the layers hold it ([K][N]: MN-major in the MMA), B_s [N][rank].  Tiles as in tile_gemm.cuh.
 //
 //   * Up to 16 rows (bound: HBM, W and the adapters in use): the epilogue's warps and as many helpers, idle while W streams, take t B_s^T on the CUDA cores
 //     in float32, a thread a column, and add it to the sums when they come: a row meets its own adapter only.  float32 rows are split in two bf16 halves on
@@ -8,7 +8,7 @@
 //   * Wide tiles (bound: the tensor cores): every tile holds rows of one request, so that t B_s^T is further K steps of the same accumulator, t as two
 //     bf16 halves, hi and lo.  Rows of the tile past the request's end are computed with the wrong adapter and not stored.
 //     A row never meets another request's adapter by way of a zero: zero times an infinity in that adapter would be NaN in this row.
-// W may be read ahead of the launch before this one, and bf16 x too: lora_down_kernel is a chain's head (launch_chained).
+// W may be read ahead of the launch before this one, and bf16 x too: the launch before is a chain's head (launch_chained).
 #include "lora.cuh"
 #include "tile_gemm.cuh"
 

@@ -300,21 +300,32 @@ class Pool:
         """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, row by row (relux_rmsnorm): h to residual_out, y to out and / or, in 8 bits, to
         codes and scales.  Device buffers, or addresses with their dtypes; residual and out are of x's type and an addressed weight is bf16 where
         nothing else is said."""
-        xt = _dtype_flag(x, dtype)
-
-        rt, wt, ot = _flag_or(residual, residual_dtype, xt), _flag_or(weight, weight_dtype, L.DTYPE_BF16), _flag_or(out, out_dtype, xt)
+        # (addresses take the short way: two thirds of a call's time in Python were calls that found them to be such)
+        xt = dtype if dtype is not None else _dtype_flag(x)
+        rt = residual_dtype if residual_dtype is not None else _flag_or(residual, None, xt)
+        wt = weight_dtype if weight_dtype is not None else _flag_or(weight, None, L.DTYPE_BF16)
+        ot = out_dtype if out_dtype is not None else _flag_or(out, None, xt)
         at, size = self._at, n_rows * d
-        L.check(L.packed["rmsnorm"](self.h, L.pack_rmsnorm(
-            n_rows, d, eps, xt, rt, wt, ot, at("rmsnorm", "x", x, size * _size(xt)), at("rmsnorm", "residual", residual, size * _size(rt)),
-            at("rmsnorm", "weight", weight, d * _size(wt)), at("rmsnorm", "residual_out", residual_out, size * _size(rt)), at("rmsnorm", "out", out, size * _size(ot)),
-            at("rmsnorm", "codes", codes, size), at("rmsnorm", "scales", scales, 4 * n_rows))))
+        rc = L.packed["rmsnorm"](self.h, L.pack_rmsnorm(
+            n_rows, d, eps, xt, rt, wt, ot, x if x.__class__ is int else at("rmsnorm", "x", x, size * _size(xt)),
+            0 if residual is None else residual if residual.__class__ is int else at("rmsnorm", "residual", residual, size * _size(rt)),
+            0 if weight is None else weight if weight.__class__ is int else at("rmsnorm", "weight", weight, d * _size(wt)),
+            0 if residual_out is None else residual_out if residual_out.__class__ is int else at("rmsnorm", "residual_out", residual_out, size * _size(rt)),
+            0 if out is None else out if out.__class__ is int else at("rmsnorm", "out", out, size * _size(ot)),
+            0 if codes is None else codes if codes.__class__ is int else at("rmsnorm", "codes", codes, size),
+            0 if scales is None else scales if scales.__class__ is int else at("rmsnorm", "scales", scales, 4 * n_rows)))
+        if rc:
+            L.check(rc)
 
     def int8_rows(self, n_rows, d, x, codes, scales, dtype=None):
         """The 8-bit form of rows x [n_rows, d] (relux_int8_rows): codes int8 [n_rows, d], scales float32 [n_rows]."""
-        t = _dtype_flag(x, dtype)
+        t = dtype if dtype is not None else _dtype_flag(x)
         at = self._at
-        L.check(L.packed["int8_rows"](self.h, L.pack_int8_rows(n_rows, d, t, at("int8_rows", "x", x, n_rows * d * _size(t)), at("int8_rows", "codes", codes, n_rows * d),
-                                                               at("int8_rows", "scales", scales, 4 * n_rows))))
+        rc = L.packed["int8_rows"](self.h, L.pack_int8_rows(n_rows, d, t, x if x.__class__ is int else at("int8_rows", "x", x, n_rows * d * _size(t)),
+                                                            codes if codes.__class__ is int else at("int8_rows", "codes", codes, n_rows * d),
+                                                            scales if scales.__class__ is int else at("int8_rows", "scales", scales, 4 * n_rows)))
+        if rc:
+            L.check(rc)
 
     def int8_weights(self, k, n, w, codes, scales, dtype=None):
         """Weights w [k, n] as 8-bit weights (relux_int8_weights): codes int8 [n, k], scales float32 [n]."""
@@ -325,11 +336,15 @@ class Pool:
 
     def matmul_int8(self, m, k, n, a, a_scales, w, w_scales, out, out_dtype=None):
         """out [m, n] = a_scales[m] * w_scales[n] * sum a[m] w[n] (relux_matmul_int8): a int8 [m, k], w int8 [n, k], on the device."""
-        t = _dtype_flag(out, out_dtype)
+        t = out_dtype if out_dtype is not None else _dtype_flag(out)
         at = self._at
-        L.check(L.packed["matmul_int8"](self.h, L.pack_matmul_int8(
-            m, k, n, t, at("matmul_int8", "a", a, m * k), at("matmul_int8", "a_scales", a_scales, 4 * m), at("matmul_int8", "w", w, n * k),
-            at("matmul_int8", "w_scales", w_scales, 4 * n), at("matmul_int8", "out", out, m * n * _size(t)))))
+        rc = L.packed["matmul_int8"](self.h, L.pack_matmul_int8(
+            m, k, n, t, a if a.__class__ is int else at("matmul_int8", "a", a, m * k),
+            a_scales if a_scales.__class__ is int else at("matmul_int8", "a_scales", a_scales, 4 * m), w if w.__class__ is int else at("matmul_int8", "w", w, n * k),
+            w_scales if w_scales.__class__ is int else at("matmul_int8", "w_scales", w_scales, 4 * n),
+            out if out.__class__ is int else at("matmul_int8", "out", out, m * n * _size(t))))
+        if rc:
+            L.check(rc)
 
     def matmul_lora(self, m, k, n, x, w, out, lora_a, lora_b, rank, n_slots, adapter, rows=None, factors=None, accumulate=False, x_dtype=None,
                     out_dtype=None):
@@ -340,12 +355,18 @@ class Pool:
         nr = None if rows is None else np.ascontiguousarray(rows, dtype=np.int32)
         if ids.ndim != 1 or (nr is not None and nr.shape != ids.shape):
             raise ValueError("matmul_lora: adapters of shape %s, rows of shape %s" % (ids.shape, None if nr is None else nr.shape))
-        xt, ot = _dtype_flag(x, x_dtype), _dtype_flag(out, out_dtype)
+        xt = x_dtype if x_dtype is not None else _dtype_flag(x)
+        ot = out_dtype if out_dtype is not None else _dtype_flag(out)
         at = self._at
-        L.check(L.packed["matmul_lora"](self.h, L.pack_matmul_lora(
-            m, k, n, rank, n_slots, ids.size, xt, ot, 1 if accumulate else 0, at("matmul_lora", "x", x, m * k * _size(xt)), at("matmul_lora", "w", w, 2 * k * n),
-            at("matmul_lora", "lora_a", lora_a, 2 * n_slots * rank * k), at("matmul_lora", "lora_b", lora_b, 2 * n_slots * rank * n),
-            at("matmul_lora", "factors", factors, 4 * n_slots), _ptr(ids) or 0, _ptr(nr) or 0, at("matmul_lora", "out", out, m * n * _size(ot)))))
+        rc = L.packed["matmul_lora"](self.h, L.pack_matmul_lora(
+            m, k, n, rank, n_slots, ids.size, xt, ot, 1 if accumulate else 0, x if x.__class__ is int else at("matmul_lora", "x", x, m * k * _size(xt)),
+            0 if w is None else w if w.__class__ is int else at("matmul_lora", "w", w, 2 * k * n),
+            lora_a if lora_a.__class__ is int else at("matmul_lora", "lora_a", lora_a, 2 * n_slots * rank * k),
+            lora_b if lora_b.__class__ is int else at("matmul_lora", "lora_b", lora_b, 2 * n_slots * rank * n),
+            0 if factors is None else factors if factors.__class__ is int else at("matmul_lora", "factors", factors, 4 * n_slots), _ptr(ids) or 0, _ptr(nr) or 0,
+            out if out.__class__ is int else at("matmul_lora", "out", out, m * n * _size(ot))))
+        if rc:
+            L.check(rc)
 
     def import_mla_weights(self, d_model, num_heads, nope_dim, rope_dim, v_dim, dc, dst, q_proj=None, kv_a_proj_with_mqa=None,
                            kv_b_proj=None, o_proj=None, q_pe_proj=None, k_pe_proj=None, fused_rope=False):

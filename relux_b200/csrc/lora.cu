@@ -531,8 +531,8 @@ int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<
   });
 }
 
-// Tiles of rows of one adapter for lora_gemm_kernel; false where they are too many, or less than seven tenths full (16 requests of 80 rows, rank 16, 4096 x 4096, 62 %
-// full: 75.8 us in tiles, 61.8 without; of 100 rows, 78 %: 63.2 and 69.3).
+// Tiles of rows of one adapter for lora_rows_kernel and lora_gemm_kernel; false where they are too many, or less than seven tenths full (16 requests of 80 rows, rank 16,
+// 4096 x 4096, 62 % full: 58.1 us in tiles, 54.2 without; of 100 rows, 78 %: 61.1 and 67.8; one request of 1024 rows, rank 64: 38.0 and 53.3).
 bool make_tiles(int M, const std::vector<Request>& requests, LoraTiles* tiles) {
   int64_t n = 0;
   for (const Request& r : requests) n += (r.n + 127) / 128;
@@ -601,8 +601,15 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     uint16_t* const rounded = x_bf16 ? nullptr : (uint16_t*)p->layer_buf.p;
     uint16_t* const t_hi = (uint16_t*)((char*)p->layer_buf.p + x_bytes);
     uint16_t* const t_lo = t_hi + (size_t)a->m * a->rank;
-    if ((rc = launch_lora_rows(p, a, tiles, rounded, t_hi, t_lo))) return rc;
-    return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : rounded, nullptr, &tiles, nullptr, t_hi, t_lo);
+    const uint16_t* x = (const uint16_t*)(x_bf16 ? a->x : nullptr);   // nullptr: lora_rows_kernel rounds
+    // so few tiles that even in eight parts of K they leave half of the SMs idle: float32 rows are rounded by a launch of their own, but for short K (rank 16, 4096 x 4096: 256
+    // rows 28.1 us so and 32.9 without, 1024 rows 45.5 and 46.8, 1536 66.3 and 64.4; 1024 rows of K 8192 48 to 62 and 62, of K 1024 22.6 and 21.3)
+    if (!x_bf16 && tiles.n * 16 <= p->dev->sm_count && a->k >= 2048) {
+      if ((rc = launch_cast(p, (const float*)a->x, rounded, (size_t)a->m * a->k))) return rc;
+      x = rounded;
+    }
+    if ((rc = launch_lora_rows(p, a, tiles, x, rounded, t_hi, t_lo))) return rc;
+    return launch_lora_gemm(p, a, x_bf16 ? x : rounded, nullptr, &tiles, nullptr, t_hi, t_lo);
   }
   if (narrow) {
     if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;

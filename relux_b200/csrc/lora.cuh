@@ -30,7 +30,7 @@ __device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2
 int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t,
                          const uint16_t* t_hi, const uint16_t* t_lo);
 
-// t = f_s x A_s^T of the rows of `tiles` as two bf16 halves [M][rank]; float32 rows are rounded to x_bf16 [M][K] as well.
-int32_t launch_lora_rows(Pool* p, const relux_matmul_lora_args* a, const LoraTiles& tiles, uint16_t* x_bf16, uint16_t* t_hi, uint16_t* t_lo);
+// t = f_s x A_s^T of the rows of `tiles` as two bf16 halves [M][rank].  x: bf16 rows [M][K]; nullptr: the caller's float32 ones, which are rounded to `rounded` as well.
+int32_t launch_lora_rows(Pool* p, const relux_matmul_lora_args* a, const LoraTiles& tiles, const uint16_t* x, uint16_t* rounded, uint16_t* t_hi, uint16_t* t_lo);
 
 }  // namespace relux

@@ -101,7 +101,8 @@ lora_rows_kernel(const __grid_constant__ DownMaps maps, const __grid_constant__ 
     }
   } else if (kRounds && warp >= 6) {
     // thread: four pieces of four k of a step, the next step's on their way while they are rounded.  (A warp loads 256 neighbouring bytes of two rows at once;
-    // pieces of eight k, half of each 32 bytes a load, asked L2 for everything twice.)
+    // pieces of eight k, half of each 32 bytes a load, asked L2 for everything twice: 3300 rows of
+    // 8192, rank 16, N 1024, 125 us so and 99.  Two or three steps on their way are no faster for long K, and slower for short.)
     const int id = threadIdx.x - 192, quad = id & 15;
     constexpr int kRowsAtOnce = 2 * kRoundWarps, kPieces = 128 / kRowsAtOnce;
     int g = 0;
@@ -207,21 +208,21 @@ int32_t launch_nc(Pool* p, const DownMaps& maps, const DownTileParams& prm, cons
 
 }  // namespace
 
-int32_t launch_lora_rows(Pool* p, const relux_matmul_lora_args* a, const LoraTiles& tiles, uint16_t* x_bf16, uint16_t* t_hi, uint16_t* t_lo) {
+int32_t launch_lora_rows(Pool* p, const relux_matmul_lora_args* a, const LoraTiles& tiles, const uint16_t* x, uint16_t* rounded, uint16_t* t_hi, uint16_t* t_lo) {
   DownTileParams prm{};
   DownMaps maps{};
   prm.rank = a->rank;
   prm.steps = (a->k + 63) / 64;
   prm.tiles = tiles.n;
   prm.K = a->k;
-  if (a->x_dtype == RELUX_DTYPE_F32) prm.x_f32 = (const float*)a->x;
-  prm.x_bf16 = x_bf16;
+  if (!x) prm.x_f32 = (const float*)a->x;
+  prm.x_bf16 = rounded;
   prm.factors = a->factors;
   prm.t_hi = t_hi;
   prm.t_lo = t_lo;
   prm.status = p->d_status;
   const int nc = std::max(16, a->rank);
-  if ((!prm.x_f32 && !make_tmap_2d(&maps.x, (void*)a->x, (uint64_t)a->m, (uint64_t)a->k, 64, kRowsOp)) ||
+  if ((x && !make_tmap_2d(&maps.x, (void*)x, (uint64_t)a->m, (uint64_t)a->k, 64, kRowsOp)) ||
       !make_tmap_2d(&maps.a, (void*)a->lora_a, (uint64_t)a->n_slots * a->rank, (uint64_t)a->k, 64, nc)) {
     set_error("tensor map for rows with adapters could not be encoded");
     return RELUX_ERR_CUDA;

@@ -18,7 +18,7 @@ namespace relux {
 namespace {
 
 constexpr int kMaxRowThreads = 1024, kMaxNV = 4, kMaxParts = 4;
-// Of a row's traffic, from which on a part of it has a block of its own while there are idle SMs (60 rows of 16384, float32: 6.7 us in one block each, 5.5 in two).
+// Of a row's traffic, from which on a part of it has a block of its own while there are idle SMs (float32 rows of 16384: 60 of them 5.0 us in one block each, 4.65 in two; 30 of them 5.1 and, in four, 4.0).
 constexpr int64_t kPartBytes = 128 << 10;
 constexpr int kMaxNormDim = 8 * kMaxRowThreads * kMaxNV;
 constexpr float kTiny = 1e-36f;   // rows without a value this large have no finite 127 / a: zeros
@@ -270,20 +270,20 @@ int32_t launch_typed(Pool* p, const NormParams& prm) {
     while (lanes < chunks) lanes *= 2;
     const dim3 block(lanes, 256 / lanes);
     auto grid = [&](int rows) { return dim3((unsigned)((prm.n_rows + (int64_t)block.y * rows - 1) / ((int64_t)block.y * rows))); };
-    // four rows a team once the SMs are full of teams of one (20440 rows of 128, bf16: 6.1 us with one, 4.0 with four)
+    // four rows a team once the SMs are full of teams of one (20440 rows of 128, bf16: 6.1 us with one, 4.1 with four)
     if ((int64_t)prm.n_rows * lanes > (int64_t)p->dev->sm_count * 2048) return launch_one<kXBf16, kRBf16, 4, kLanes, kNorm>(p, prm, grid(4), block);
     return launch_one<kXBf16, kRBf16, 1, kLanes, kNorm>(p, prm, grid(1), block);
   }
   int parts = 1;
   const int64_t bytes = (int64_t)prm.d * ((kXBf16 ? 2 : 4) + (prm.residual ? (kRBf16 ? 4 : 8) : 0) + (prm.out ? (prm.out_bf16 ? 2 : 4) : 0));
   while (parts < kMaxParts && bytes / parts >= kPartBytes && prm.n_rows <= p->dev->sm_count / (2 * parts)) parts *= 2;
-  // As few chunks a thread as the block's limit lets.  Of more rows than are resident at once as many as keep blocks at 256 threads, so that more rows are on their way
-  // (8192 rows of 8192, bf16: 91 us in blocks of 1024 threads, 84 in blocks of 256); of float32 two at most, four cost more registers than they are worth (400 rows of
-  // 16384: 27.8 us and 22.7).
+  // As few chunks a thread as the block's limit lets.  Of more bf16 rows than are resident at once as many as keep blocks at 256 threads, so that more rows are on their
+  // way (8192 rows of 8192: 91 us in blocks of 1024 threads, 84 in blocks of 256); of float32 that gives nothing (5000 rows of 4096: 30.7 us with two chunks a thread,
+  // 29.4 with one; 400 of 16384 23.7 with four and 22.1 with two).
   const int each = (chunks + parts - 1) / parts;
   int nv = each <= kMaxRowThreads ? 1 : each <= 2 * kMaxRowThreads ? 2 : 4;
-  if (prm.n_rows > 2 * p->dev->sm_count)
-    while (nv < (kXBf16 && kRBf16 ? 4 : 2) && each > 256 * nv) nv *= 2;
+  if (kXBf16 && kRBf16 && prm.n_rows > 2 * p->dev->sm_count)
+    while (nv < 4 && each > 256 * nv) nv *= 2;
   const int threads = ((each + nv - 1) / nv + 31) / 32 * 32;
   const dim3 grid((unsigned)prm.n_rows * (unsigned)parts), block((unsigned)threads);
   if (parts > 1) {

@@ -612,9 +612,14 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     return launch_lora_gemm(p, a, x_bf16 ? x : rounded, nullptr, &tiles, nullptr, t_hi, t_lo);
   }
   if (narrow) {
-    if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;
-    down.t = (float*)p->layer_buf.p;
-    if ((rc = run_down(p, x_bf16, down, requests))) return rc;
+    // In one launch, every CTA of which takes t over its part of K: of so few sums, and so few tiles that read the same pieces of an adapter at once (one row x 4096 x 4096, rank 16:
+    // 10.8 us so, 12.3 in two; rank 32 11.3 and 13.2; rank 64 15.9 and 13.2; rank 16 x 4096 x 14336 27.9 and 21.9).
+    const bool one = a->m * a->rank <= kOneT && (a->n - 1) / kRowsOp + 1 <= p->dev->sm_count / 4;
+    if (!one) {
+      if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;
+      down.t = (float*)p->layer_buf.p;
+      if ((rc = run_down(p, x_bf16, down, requests))) return rc;
+    }
     int16_t row_slots[kNarrowRows];
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
     return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : nullptr, row_slots, nullptr, down.t, nullptr, nullptr);

@@ -7,6 +7,7 @@
 namespace relux {
 
 constexpr int kNarrowRows = 16;     // calls of up to so many rows: one block of rows, float32 ones split by lora_gemm_kernel, adapters on the CUDA cores
+constexpr int kOneT = 32;           // rows x rank of calls in one launch
 constexpr int kMaxLoraTiles = 1024; // row tiles of a longer call
 
 // Tiles of up to 128 neighbouring rows of one adapter.
@@ -25,7 +26,7 @@ __device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2
 }
 
 // out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kNarrowRows float32 rows of the
-// caller's.  Without tiles (up to kNarrowRows rows): row_slots
+// caller's.  Without tiles or t: lora_gemm_kernel takes t itself.  Without tiles (up to kNarrowRows rows): row_slots
 // [M], t [M][rank] without factors; with tiles: t as two bf16 halves [M][rank], factors included.
 int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t,
                          const uint16_t* t_hi, const uint16_t* t_lo);

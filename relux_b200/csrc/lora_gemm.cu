@@ -8,7 +8,8 @@
 //   * Wide tiles (bound: the tensor cores): every tile holds rows of one request, so that t B_s^T is further K steps of the same accumulator, t as two
 //     bf16 halves, hi and lo.  Rows of the tile past the request's end are computed with the wrong adapter and not stored.
 //     A row never meets another request's adapter by way of a zero: zero times an infinity in that adapter would be NaN in this row.
-// W may be read ahead of the launch before this one, and bf16 x too: the launch before is a chain's head (launch_chained).
+//   * Of a row or two every CTA takes t over its part of K itself, and adds t B_s^T to its own part of the sums: no launch before this one.
+// Behind another launch of the call W is read ahead of it, and bf16 x too: that one is a chain's head (launch_chained).
 #include "lora.cuh"
 #include "tile_gemm.cuh"
 
@@ -24,8 +25,8 @@ using LoraShape = TileShape<NC, NC == 256 ? 0 : kRowsT + kRing * 256 * 16, NC + 
 static_assert(slices_fit(16, 1, 8, 1, LoraShape<16>::kSlices) && slices_fit(256, 32, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage) &&
               slices_fit(256, 64, 4, 0, LoraShape<256>::kStages * LoraShape<256>::kStage), "no room for the slices");
 
-template <int NC>
-constexpr int kLoraGemmThreads = NC == 256 ? 192 : 320;
+template <int NC, bool kOne>
+constexpr int kLoraGemmThreads = NC == 256 ? 192 : kOne ? 448 : 320;
 
 struct LoraMaps {
   CUtensorMap x;      // [M][K], box 64 k x the rows of an operand
@@ -42,15 +43,18 @@ struct LoraGemmParams {
   const float* t;            // narrow: [M][rank], without factors
   const uint16_t* b;         // narrow: [slots][N][rank]
   const float* factors;      // narrow: [slots], or nullptr
+  const uint16_t* a;         // in one launch: [slots][rank][K]
+  const void* x_rows;        // in one launch: the caller's rows, bf16 or (x_f32) float32
   void* out;
   int32_t* status;
 };
+static_assert(kOneT * 4 <= kRowsT && kOneT / 8 * kRowsOp * 4 <= kRing * 256 * 16, "no room for a part's t");
 struct NarrowRows {
   int16_t slot[kNarrowRows];   // of every row, or -1
 };
 
-template <int NC, class Rows>
-__global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(const __grid_constant__ LoraMaps maps, const __grid_constant__ LoraGemmParams prm, const __grid_constant__ Rows list) {
+template <int NC, class Rows, bool kOne>
+__global__ void __launch_bounds__(kLoraGemmThreads<NC, kOne>, 1) lora_gemm_kernel(const __grid_constant__ LoraMaps maps, const __grid_constant__ LoraGemmParams prm, const __grid_constant__ Rows list) {
   using SH = LoraShape<NC>;
   constexpr int kStages = SH::kStages;
   constexpr bool kWide = SH::kWide;
@@ -162,11 +166,90 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
     low_sync();
   };
 
+  // In one launch: a row's slice of t over this CTA's part of K, [row][rank] with factors, by the epilogue's warps and the last four, four sums of a row a warp at a time.
+  auto down_part = [&] {
+    const int c0 = rank * prm.steps / size * 64, c1 = min((rank + 1) * prm.steps / size * 64, prm.K);
+    for (int d = 4 * (warp < 4 ? warp : warp - 6); d < prm.M * prm.rank; d += 32) {   // (a rank is a multiple of eight)
+      const int row = d / prm.rank, slot = list.slot[row];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      if (slot >= 0) {
+        const uint16_t* const a = prm.a + ((size_t)slot * prm.rank + d % prm.rank) * prm.K;
+#pragma unroll 4
+        for (int k = c0 + 8 * lane; k < c1; k += 256) {
+          uint4 w[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) w[i] = load_chained(reinterpret_cast<const uint4*>(a + (size_t)i * prm.K + k));
+          float x[8];
+          if (prm.x_f32) {
+            const float4* src = reinterpret_cast<const float4*>(prm.x_f32 + (size_t)row * prm.K + k);
+            const float4 u = load_chained(src), v = load_chained(src + 1);
+            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+          } else {
+            const uint4 u = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(prm.x_rows) + (size_t)row * prm.K + k));
+            x[0] = bf16_lo(u.x); x[1] = bf16_hi(u.x); x[2] = bf16_lo(u.y); x[3] = bf16_hi(u.y); x[4] = bf16_lo(u.z); x[5] = bf16_hi(u.z); x[6] = bf16_lo(u.w); x[7] = bf16_hi(u.w);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            sum[i] = fmaf(x[0], bf16_lo(w[i].x), sum[i]); sum[i] = fmaf(x[1], bf16_hi(w[i].x), sum[i]);
+            sum[i] = fmaf(x[2], bf16_lo(w[i].y), sum[i]); sum[i] = fmaf(x[3], bf16_hi(w[i].y), sum[i]);
+            sum[i] = fmaf(x[4], bf16_lo(w[i].z), sum[i]); sum[i] = fmaf(x[5], bf16_hi(w[i].z), sum[i]);
+            sum[i] = fmaf(x[6], bf16_lo(w[i].w), sum[i]); sum[i] = fmaf(x[7], bf16_hi(w[i].w), sum[i]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) sum[i] = warp_sum(sum[i]);
+      const float f = slot >= 0 && prm.factors ? load_chained(prm.factors + slot) : 1.f;
+      if (lane < 4) t_rows[d + lane] = f * (lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3]);
+    }
+  };
+  // and that part's t B_s^T of a tile, a thread a column: to the CTA's own sums of the tile, [row][128]
+  float* const part_low = t_rows + kRowsT / 4 + threadIdx.x;
+  auto low_part = [&](const Place& at, bool first_tile) {
+    const int n = at.c * kRowsOp + threadIdx.x, shift = 31 - __clz(prm.rank >> 3), last = (prm.rank >> 3) - 1;   // ranks are powers of two
+    uint4 w[kOneT / 8];
+#pragma unroll
+    for (int i = 0; i < kOneT / 8; i++) {
+      const int row = i >> shift, slot = row < prm.M ? list.slot[row] : -1;
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (slot >= 0 && n < prm.N) w[i] = load_chained(reinterpret_cast<const uint4*>(prm.b + ((size_t)slot * prm.N + n) * prm.rank) + (i & last));
+    }
+    if (first_tile) {
+      down_part();
+      low_sync();
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kOneT / 8; i++) {
+      const float4* t = reinterpret_cast<const float4*>(t_rows + 8 * i);
+      if (8 * i < prm.M * prm.rank) {
+        const float4 t0 = t[0], t1 = t[1];
+        if ((i & last) == 0) sum = 0.f;
+        sum = fmaf(t0.x, bf16_lo(w[i].x), sum); sum = fmaf(t0.y, bf16_hi(w[i].x), sum); sum = fmaf(t0.z, bf16_lo(w[i].y), sum); sum = fmaf(t0.w, bf16_hi(w[i].y), sum);
+        sum = fmaf(t1.x, bf16_lo(w[i].z), sum); sum = fmaf(t1.y, bf16_hi(w[i].z), sum); sum = fmaf(t1.z, bf16_lo(w[i].w), sum); sum = fmaf(t1.w, bf16_hi(w[i].w), sum);
+        if ((i & last) == last) part_low[(i >> shift) * kRowsOp] = sum;
+      }
+    }
+  };
+
   if (warp == 4) {
     const bool el = elect_one();
     if (el) {
       if (!rounds_x) tma_prefetch_desc(&maps.x);
       tma_prefetch_desc(&maps.w);
+    }
+    if constexpr (kOne) {   // no launch of this call before this one: nothing is read early, but brought into L2
+      if (el) {
+        int left = kPrefetchSteps;
+        for (int tile = first; tile < prm.tiles && left > 0; tile += stride) {
+          const Place at = place(tile);
+          for (int k = at.k0; k < at.k1 && left > 0; k++, left--)
+#pragma unroll
+            for (int i = 0; i < 2; i++) tma_prefetch_2d(&maps.w, at.c * kRowsOp + 64 * i, k * 64);
+        }
+      }
+      __syncwarp();
+      chain_wait();
     }
     const int w_at = kWide ? kStageRows : 0, x_at = kWide ? 0 : kStageRows;   // the M operand comes first
     auto load_w = [&](const Place& at, int k, int s) {   // W of one step; arms the stage for both operands (out-of-range parts of a box are zero-filled and still counted)
@@ -255,9 +338,16 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
       if (el) umma_commit<1>(&bars->acc_full[piece & 1]);
       __syncwarp();
     }
+  } else if (kOne && warp >= 10) {
+    chain_wait();
+    if (first < prm.tiles) {
+      down_part();
+      low_sync();
+    }
   } else if (!kWide && warp >= 6) {
     // helpers: few float32 rows as two bf16 halves, and half of t B_s^T
     const int id = threadIdx.x - 192;
+    if constexpr (kOne) chain_wait();
     int g = 0;
     for (int tile = first; tile < prm.tiles; tile += stride) {
       const Place at = place(tile);
@@ -295,10 +385,10 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
             }
         }
       }
-      low_half(at, 1);
+      if constexpr (!kOne) low_half(at, 1);
     }
   } else {
-    if constexpr (kWide) chain_wait();
+    if constexpr (kWide || kOne) chain_wait();
     int piece = 0, staged = 0;
     for (int tile = first; tile < prm.tiles; tile += stride, piece++) {
       const Place at = place(tile);
@@ -308,11 +398,15 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
       const int grain = !kWide ? 1 : prm.out_bf16 ? 64 : 32;
       const int q0 = size > 1 ? slice_begin(rank, cols, grain, size) : 0, q1 = size > 1 ? slice_begin(rank + 1, cols, grain, size) : cols;
       const float* const got = reinterpret_cast<const float*>(slices) + threadIdx.x;
-      if constexpr (!kWide) low_half(at, 0);
+      if constexpr (kOne) low_part(at, tile == first);
+      else if constexpr (!kWide) low_half(at, 0);
       tile_wait(&bars->acc_full[buf], (piece >> 1) & 1, bars, prm.status);
       tc_fence_after();
       const bool ok = !bars->abort_flag;
-      if (size > 1) swap_slices<SH>(acc, cols, grain, size, rank, slices);
+      if (size > 1) {
+        if constexpr (kOne) swap_slices<SH>(acc, cols, grain, size, rank, slices, [&](int q, uint32_t v) { return __float_as_uint(__uint_as_float(v) + part_low[q * kRowsOp]); });
+        else swap_slices<SH>(acc, cols, grain, size, rank, slices);
+      }
       if constexpr (!kWide) {
         // thread = column; a warp writes 64 or 128 bytes of a row at once
         const int n = at.c * kRowsOp + warp * 32 + lane;
@@ -335,8 +429,12 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
           float x[8];
 #pragma unroll
           for (int i = 0; i < 8; i++) x[i] = ok ? __uint_as_float(v[i]) : 0.f;
+          if constexpr (kOne)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (q + i < q1) x[i] += part_low[(q + i) * kRowsOp];
 #pragma unroll 1
-          for (int s = 0; s < size; s++)   // the others' parts, then the adapter's
+          for (int s = 0; s < (kOne ? size - 1 : size); s++)   // the others' parts, then the adapter's
 #pragma unroll
             for (int i = 0; i < 8; i++)
               if (q + i < q1) x[i] += got[(s * (q1 - q0) + q - q0 + i) * kRowsOp];
@@ -433,9 +531,9 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC>, 1) lora_gemm_kernel(cons
   tile_end<SH>(tmem, size);
 }
 
-template <int NC, class Rows>
+template <int NC, bool kOne, class Rows>
 int32_t launch_rows(Pool* p, const LoraMaps& maps, const LoraGemmParams& prm, const Rows& rows) {
-  return launch_tiles<LoraShape<NC>, kLoraGemmThreads<NC>>(p, lora_gemm_kernel<NC, Rows>, prm.tiles, prm.steps, maps, prm, rows);
+  return launch_tiles<LoraShape<NC>, kLoraGemmThreads<NC, kOne>>(p, lora_gemm_kernel<NC, Rows, kOne>, prm.tiles, prm.steps, maps, prm, rows);
 }
 
 }  // namespace
@@ -460,6 +558,8 @@ int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_
   prm.x_f32 = x ? nullptr : (const float*)a->x;
   prm.K = K;
   prm.t = t;
+  prm.a = (const uint16_t*)a->lora_a;
+  prm.x_rows = a->x;
   prm.b = (const uint16_t*)a->lora_b;
   prm.factors = a->factors;
   prm.out = a->out;
@@ -474,11 +574,11 @@ int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_
     set_error("tensor map for a projection with adapters could not be encoded");
     return RELUX_ERR_CUDA;
   }
-  if (tiles) return launch_rows<256>(p, maps, prm, *tiles);
+  if (tiles) return launch_rows<256, false>(p, maps, prm, *tiles);
   NarrowRows rows;
   std::copy(row_slots, row_slots + M, rows.slot);
   std::fill(rows.slot + M, rows.slot + kNarrowRows, (int16_t)-1);
-  return launch_rows<kNarrowRows>(p, maps, prm, rows);
+  return t ? launch_rows<kNarrowRows, false>(p, maps, prm, rows) : launch_rows<kNarrowRows, true>(p, maps, prm, rows);
 }
 
 }  // namespace relux

@@ -186,7 +186,7 @@ def test_infinities_and_nan_stay_with_their_request(dev, pool):
 
 
 # requests of a row each, few and so few that float32 rows are split; requests whose tiles are nearly full, with rows past their ends
-FORMS = [([1] * 12, [0, 1, 2, -1] * 3, True), ([1] * 8, [0, 1, 2, -1] * 2, False), ([250, 128, 380, 90], [0, 1, 2, -1], True), ([90, 380, 128, 250], [2, -1, 1, 0], False)]
+FORMS = [([1] * 4, [0, 1, 2, -1], True), ([1] * 4, [-1, 2, 1, 0], False), ([1] * 12, [0, 1, 2, -1] * 3, True), ([1] * 8, [0, 1, 2, -1] * 2, False), ([250, 128, 380, 90], [0, 1, 2, -1], True), ([90, 380, 128, 250], [2, -1, 1, 0], False)]
 
 
 @pytest.mark.parametrize("rows,adapter,x_bf16", FORMS)
@@ -205,11 +205,12 @@ def test_added_in_every_form(dev, pool, rows, adapter, x_bf16, out_bf16, K, N, r
 
 
 @pytest.mark.parametrize("rows,adapter,x_bf16", FORMS)
-def test_infinities_and_nan_in_every_form(dev, pool, rows, adapter, x_bf16):
+@pytest.mark.parametrize("rank", [16, 8])
+def test_infinities_and_nan_in_every_form(dev, pool, rows, adapter, x_bf16, rank):
     """The second adapter and a row of the third's hold NaN, a column of the third an infinity: what the formula leaves finite is."""
     from oracle import binding as orc
     rng = np.random.default_rng(17)
-    c = Case(dev, rng, rows, adapter, 264, 392, 16, 3, x_bf16)
+    c = Case(dev, rng, rows, adapter, 264, 392, rank, 3, x_bf16)
     c.a[1, 3, 7], c.b[2, 5, :] = np.nan, np.inf
     c.da.upload(orc.bf16_from_f32(c.a)), c.db.upload(orc.bf16_from_f32(c.b))
     ids = np.repeat(np.asarray(adapter), rows)
@@ -221,6 +222,18 @@ def test_infinities_and_nan_in_every_form(dev, pool, rows, adapter, x_bf16):
     fine = np.isfinite(out)
     assert fine[ids == 0].all() and not fine[ids == 1].any() and not fine[bad].any()
     assert (np.isfinite(got) == fine).all() and (np.abs(got - out)[fine] <= bound[fine]).all()
+    c.free()
+
+
+@pytest.mark.parametrize("M,rank", [(1, 8), (1, 16), (2, 16), (1, 32), (4, 8), (3, 8)])
+@pytest.mark.parametrize("K,N", [(8, 8), (72, 136), (1032, 520), (4096, 4736), (4096, 4744), (16384, 1024)])
+@pytest.mark.parametrize("x_bf16", [False, True])
+def test_a_few_rows(dev, pool, M, rank, K, N, x_bf16):
+    rng = np.random.default_rng(M * rank + K)
+    c = Case(dev, rng, [1] * M, [i % 4 for i in range(M)], K, N, rank, 4, x_bf16, x_bf16)
+    for _ in range(3):
+        c.call(pool)
+    c.check()
     c.free()
 
 

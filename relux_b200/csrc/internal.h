@@ -356,8 +356,9 @@ inline void count_launch(Device* d, int n = 1) { d->launches += n; }
 //      without weights_ready.  Those who read early, and why they may:
 //        - page tables, everywhere: the host calls that change them wait for the stream and for their copy;
 //        - skinny_gemm_sm100_kernel, the weights: the first launch of a layer step or matmul is cast_bf16_kernel, of a block's norm_rows_kernel, of a projection
-//          with adapters lora_down_kernel or lora_rows_kernel; the second GEMM of a layer follows it, a plain absorb launch, or a cast of its own;
-//        - lora_gemm_kernel, W, the adapters and rows that are the caller's, and lora_up_kernel, the adapters: behind the lora_down_kernel or lora_rows_kernel of the same call (alone, lora_gemm_kernel waits first);
+//          with adapters one of the three heads, or a plain launch of the GEMM itself; the second GEMM of a layer follows it, a plain absorb launch, or a cast of its own;
+//        - lora_gemm_kernel, W, the adapters and rows that are the caller's, and lora_up_kernel, the adapters: behind the lora_down_kernel, lora_rows_kernel, cast or plain GEMM of the same call (alone,
+//          lora_gemm_kernel waits first);
 //        - mla_prep_kernel with weights_ready, W_UK: only behind the projections of the same call (do_mla_layer);
 //        - build_stream_kernel, the lengths (and it writes the plan, which the launches of older calls read): behind an mla_prep_kernel that is
 //          a head, or a plain absorb launch;

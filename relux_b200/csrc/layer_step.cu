@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 #include <vector>
 #include "common.cuh"
 #include "internal.h"
@@ -67,6 +68,43 @@ struct GemmShape {
   static constexpr int kAcc = NT < 32 ? 32 : NT;    // columns of one of the two accumulators
 };
 
+// A launch's part in AdapterColumns, or nothing.
+struct NoItems {};
+struct AdapterItems {
+  CUtensorMap a;                         // [n_slots * rank][K], box: 64 k x an adapter
+  int32_t items, parts, steps, rank, n_used, shift;   // shift: log2 of the adapters of a tile
+  float* t;
+  int32_t slot[kMaxUsed];
+};
+// GemmWalk, then the worker's items; first to those who have the fewest steps.
+template <bool kBlocks>
+struct ItemWalk : GemmWalk<kBlocks> {
+  const AdapterItems& it;
+  int item, mine;   // item: the current one, or -1
+  __device__ ItemWalk(const GemmRanges& rg, int id, const AdapterItems& items) : GemmWalk<kBlocks>(rg, id), it(items), item(-1), mine(gridDim.x - 1 - id) {}
+  __device__ int total() const {
+    int n = GemmWalk<kBlocks>::total();
+    for (int i = mine; i < it.items; i += gridDim.x) n += (i % it.parts + 1) * it.steps / it.parts - i % it.parts * it.steps / it.parts;
+    return n;
+  }
+  __device__ bool next() {
+    if (item < 0) {
+      if (GemmWalk<kBlocks>::next()) return true;
+      item = mine;
+    } else {
+      item += gridDim.x;
+    }
+    if (item >= it.items) return false;
+    const int p = item % it.parts;
+    this->col = 0;
+    this->k0 = p * it.steps / it.parts;
+    this->k1 = (p + 1) * it.steps / it.parts;
+    return true;
+  }
+  __device__ int tile() const { return item / it.parts; }
+  __device__ int adapters() const { return min(1 << it.shift, it.n_used - (tile() << it.shift)); }   // of the item's tile
+};
+
 struct GemmBars {
   uint64_t full[12], empty[12], acc_full[2], acc_empty[2];
   uint32_t tmem_base;
@@ -100,15 +138,23 @@ __device__ __forceinline__ void gemm_wait(uint64_t* bar, uint32_t parity, GemmBa
 //     successors only when everything before the step is complete, so that weights written earlier in the stream are there.
 // Measured with the chained launches around it (a layer step, before -> now): 16 rows of d_model 16384, 1.36 GB of weights,
 // 308 -> 272 us; 24 rows of d_model 4096, 84 MB, 82.8 -> 67.0 us.
-template <int NT>
-__global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams prm) {
+template <int NT, class Items>
+__global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams prm, const __grid_constant__ Items items) {
+  constexpr bool kItems = std::is_same_v<Items, AdapterItems>;
   using SH = GemmShape<NT>;
   constexpr int kStages = SH::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   GemmBars* bars = reinterpret_cast<GemmBars*>(smem + kStages * SH::kStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr bool kBlocks = NT >= 128;   // smaller blocks hold all rows
-  GemmWalk<kBlocks> walk(prm.rg, blockIdx.x);
+  auto walk = [&] {
+    if constexpr (kItems) return ItemWalk<kBlocks>(prm.rg, blockIdx.x, items);
+    else return GemmWalk<kBlocks>(prm.rg, blockIdx.x);
+  }();
+  auto in_items = [&](const auto& w) {
+    if constexpr (kItems) return w.item >= 0;
+    else return false;
+  };
   auto weight_of = [&](int tile) -> int {
     int j = 0;
     while (j + 1 < prm.n_weights && tile >= prm.tile_first[j + 1]) j++;
@@ -149,10 +195,19 @@ __global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_
       const int s = g % kStages;
       if (el) {
         uint8_t* sw = smem + s * SH::kStage;
+        if constexpr (kItems)
+          if (in_items(walk)) {
+            const int some = walk.adapters();
+            mbar_expect_tx(&bars->full[s], some * items.rank * 128 + SH::kStageX);
+            for (int q = 0; q < some; q++)
+              tma_load_2d(sw + q * items.rank * 128, &items.a, k * kTileK, items.slot[(walk.tile() << items.shift) + q] * items.rank, &bars->full[s]);
+          }
         const int n0 = (walk.col - prm.tile_first[j]) * kTileN;
+        if (!in_items(walk)) {
         mbar_expect_tx(&bars->full[s], SH::kStage);   // out-of-range parts of a box are zero-filled and still counted
         tma_load_2d_hint(sw, &maps.w[j], n0, k * kTileK, &bars->full[s], policy);
         tma_load_2d_hint(sw + kStageW / 2, &maps.w[j], n0 + 64, k * kTileK, &bars->full[s], policy);
+        }
       }
       __syncwarp();
       if (++k == walk.k1 && walk.next()) {
@@ -178,7 +233,7 @@ __global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_
   } else if (warp == 5) {
     chain_wait();
     const bool el = elect_one();
-    const uint32_t idesc = make_idesc_bf16(kTileN, NT, true, false);
+    const uint32_t idesc = make_idesc_bf16(kTileN, NT, true, false), idesc_items = make_idesc_bf16(kTileN, NT, false, false);
     int g = 0;
     for (int piece = 0; walk.next(); piece++) {
       const uint32_t d = tmem + (piece & 1) * SH::kAcc;
@@ -192,9 +247,16 @@ __global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_
           const uint32_t sw = smem_u32(smem + s * SH::kStage);
           const uint64_t dW = make_desc_mnmajor_sw128(sw, kStageW / 2);
           const uint64_t dX = make_desc_kmajor_sw128(sw + kStageW);
+          if (!in_items(walk)) {
 #pragma unroll
-          for (int kk = 0; kk < kTileK / 16; kk++)
-            umma_ss<1>(d, dW + ((uint32_t)(kk * 2048) >> 4), dX + ((uint32_t)(kk * 32) >> 4), idesc, k != walk.k0 || kk != 0);
+            for (int kk = 0; kk < kTileK / 16; kk++)
+              umma_ss<1>(d, dW + ((uint32_t)(kk * 2048) >> 4), dX + ((uint32_t)(kk * 32) >> 4), idesc, k != walk.k0 || kk != 0);
+          } else {
+            const uint64_t dA = make_desc_kmajor_sw128(sw);   // adapters lie K-major; rows of the tile behind the last one hold anything
+#pragma unroll
+            for (int kk = 0; kk < kTileK / 16; kk++)
+              umma_ss<1>(d, dA + ((uint32_t)(kk * 32) >> 4), dX + ((uint32_t)(kk * 32) >> 4), idesc_items, k != walk.k0 || kk != 0);
+          }
           umma_commit<1>(&bars->empty[s]);
         }
         __syncwarp();
@@ -209,12 +271,18 @@ __global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_
     chain_wait();
     for (int piece = 0; walk.next(); piece++) {
       const int j = weight_of(walk.col), m0 = kBlocks ? walk.block * NT : 0;
-      const int n = (walk.col - prm.tile_first[j]) * kTileN + warp * 32 + lane;
+      int n = (walk.col - prm.tile_first[j]) * kTileN + warp * 32 + lane, n_cols = prm.n_cols[j], row_stride = prm.n_total;
       const int m_end = min(NT, prm.M - m0);
       float* dst = prm.part + ((size_t)walk.split * prm.M + m0) * prm.n_total + prm.col_first[j] + n;
+      if constexpr (kItems)
+        if (in_items(walk)) {
+          n = walk.tile() * kTileN + warp * 32 + lane;
+          n_cols = row_stride = items.n_used * items.rank;
+          dst = items.t + (size_t)(walk.item % items.parts) * prm.M * row_stride + n;
+        }
       gemm_wait(&bars->acc_full[piece & 1], (piece >> 1) & 1, bars, prm.status);
       tc_fence_after();
-      const bool ok = !bars->abort_flag, mine = n < prm.n_cols[j];
+      const bool ok = !bars->abort_flag, mine = n < n_cols;
 #pragma unroll 1
       for (int c = 0; c < m_end; c += 32) {
         uint32_t v[32];
@@ -223,7 +291,7 @@ __global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_
 #pragma unroll
         for (int q = 0; q < 32; q++)
           if (mine && c + q < m_end) {
-            float* to = dst + (size_t)(c + q) * prm.n_total;
+            float* to = dst + (size_t)(c + q) * row_stride;
             const float x = ok ? __uint_as_float(v[q]) : 0.f;
             if constexpr (kKeep) store_hint(to, x, stay);
             else *to = x;
@@ -360,11 +428,11 @@ __global__ void sum_splits_kernel(const float* __restrict__ part, GemmRanges rg,
   reinterpret_cast<float4*>(out)[i] = acc;
 }
 
-template <int NT>
-int32_t launch_skinny_gemm_rows(Pool* p, const GemmMaps& maps, const GemmParams& g, int workers) {
-  if (int32_t rc = allow_smem(p->dev, skinny_gemm_sm100_kernel<NT>, GemmShape<NT>::kSmem)) return rc;
-  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, skinny_gemm_sm100_kernel<NT>, dim3(workers), dim3(192),
-                                (size_t)GemmShape<NT>::kSmem, p->dev->stream, maps, g));
+template <int NT, class Items>
+int32_t launch_skinny_gemm_rows(Pool* p, const GemmMaps& maps, const GemmParams& g, int workers, const Items& items, bool chained) {
+  if (int32_t rc = allow_smem(p->dev, skinny_gemm_sm100_kernel<NT, Items>, GemmShape<NT>::kSmem)) return rc;
+  RELUX_CUDA_TRY(launch_chained(chained && p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, skinny_gemm_sm100_kernel<NT, Items>, dim3(workers), dim3(192),
+                                (size_t)GemmShape<NT>::kSmem, p->dev->stream, maps, g, items));
   count_launch(p->dev);
   return RELUX_OK;
 }
@@ -416,7 +484,7 @@ GemmRanges deal_tiles(int sms, int col_tiles, int M, int block_rows, int beside,
 }  // namespace
 
 int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const WeightRef* ws, int nw, float* part, size_t part_cap_bytes,
-                           GemmRanges* ranges, TimeStamp time) {
+                           GemmRanges* ranges, TimeStamp time, const AdapterColumns* adapters, bool head) {
   GemmMaps maps;
   GemmParams g;
   memset(&g, 0, sizeof(g));
@@ -470,12 +538,34 @@ int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const 
   g.status = p->d_status;
   g.time = time;
   *ranges = g.rg;
+  if (adapters) {   // of up to 128 rows, in one block
+    AdapterItems items;
+    if (!make_tmap_2d(&items.a, (void*)adapters->lora_a, (uint64_t)adapters->n_slots * adapters->rank, (uint64_t)K, kTileK, adapters->rank)) {
+      set_error("tensor map for adapters could not be encoded");
+      return RELUX_ERR_CUDA;
+    }
+    items.shift = 0;
+    while (adapters->rank << (items.shift + 1) <= kTileN) items.shift++;
+    items.parts = adapters->parts;
+    items.items = ((adapters->n_used - 1 >> items.shift) + 1) * items.parts;
+    items.steps = steps;
+    items.rank = adapters->rank;
+    items.n_used = adapters->n_used;
+    items.t = adapters->t;
+    std::copy(adapters->slot, adapters->slot + adapters->n_used, items.slot);
+    switch (nt) {
+      case 16: return launch_skinny_gemm_rows<16>(p, maps, g, workers, items, !head);
+      case 32: return launch_skinny_gemm_rows<32>(p, maps, g, workers, items, !head);
+      case 64: return launch_skinny_gemm_rows<64>(p, maps, g, workers, items, !head);
+      default: return launch_skinny_gemm_rows<128>(p, maps, g, workers, items, !head);
+    }
+  }
   switch (nt) {
-    case 16: return launch_skinny_gemm_rows<16>(p, maps, g, workers);
-    case 32: return launch_skinny_gemm_rows<32>(p, maps, g, workers);
-    case 64: return launch_skinny_gemm_rows<64>(p, maps, g, workers);
-    case 128: return launch_skinny_gemm_rows<128>(p, maps, g, workers);
-    default: return launch_skinny_gemm_rows<kMaxTok>(p, maps, g, workers);
+    case 16: return launch_skinny_gemm_rows<16>(p, maps, g, workers, NoItems{}, !head);
+    case 32: return launch_skinny_gemm_rows<32>(p, maps, g, workers, NoItems{}, !head);
+    case 64: return launch_skinny_gemm_rows<64>(p, maps, g, workers, NoItems{}, !head);
+    case 128: return launch_skinny_gemm_rows<128>(p, maps, g, workers, NoItems{}, !head);
+    default: return launch_skinny_gemm_rows<kMaxTok>(p, maps, g, workers, NoItems{}, !head);
   }
 }
 

@@ -2,8 +2,8 @@
 // request that row m belongs to, or none.  A_s [rank][K], B_s [N][rank] in slots of two arrays, as checkpoints hold them (lora_A, lora_B).
 //
 // Two launches: lora_down_kernel, or lora_rows_kernel (lora_rows.cu) for tiles of one request's rows, takes t = x A_s^T, and rounds a float32 x to bf16 while it holds the
-// rows; lora_gemm_kernel (lora_gemm.cu) is the projection, whose epilogue or last steps add t B_s^T.  Three where the rows are many and of so many requests that tiles of one request's rows would be mostly
-// empty, or where the projection is not this call's: lora_down_kernel, the projection's GEMM (skinny_gemm_sm100_kernel), and lora_up_kernel, which adds up
+// rows; lora_gemm_kernel (lora_gemm.cu) is the projection, whose epilogue or last steps add t B_s^T.  (Of a row or two in one.)  Three where the rows are many and of so many requests that tiles of one request's rows would be mostly
+// empty, or where the projection is not this call's: lora_down_kernel, the projection's GEMM (skinny_gemm_sm100_kernel, which may take t itself), and lora_up_kernel, which adds up
 // the GEMM's pieces and, on the way out, t B_s^T.
 // No tile of a product holds rows of one request and another's adapter: a product with that by zeros would carry its infinities and NaN over.
 // In lora_down_kernel and lora_up_kernel rows are taken in groups of 16 of one adapter, wherever in the batch they lie: the host sorts the requests by adapter,
@@ -37,6 +37,7 @@ struct RowList {
   struct Group {
     int32_t slot;        // adapter, or -1
     int16_t first, n;    // its rows' places
+    int32_t used;        // which of the call's adapters, in order
   };
   Group group[kCap];
   int16_t row[kCap];
@@ -63,6 +64,8 @@ __host__ __device__ __forceinline__ int last_up_to(const int32_t* a, int n, int 
   return lo;
 }
 // Rows of a group to shared memory (-1: none), and its adapter.  By all threads; a barrier follows.
+template <int kCap>
+__device__ __forceinline__ int used_of(const RowList<kCap>& list, int group) { return list.group[group].used; }
 template <int kCap>
 __device__ __forceinline__ int group_rows(const RowList<kCap>& list, int group, int32_t* rows) {
   const auto g = list.group[group];
@@ -233,10 +236,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   }
 }
 
+enum Up { kPlain, kInTurns, kTInPieces };   // the GEMM's blocks of rows come in turns; t comes in pieces, from the GEMM
 struct UpParams {
   const float* part;      // the GEMM's pieces [piece][M][N]; nullptr: no shared projection
   GemmRanges rg;
-  const float* t;         // [M][rank]
+  const float* t;         // [M][rank], or (t_parts) in as many pieces [M][t_cols], of every adapter in use for every row
+  int32_t t_parts, t_cols;
   const uint16_t* b;      // [slots][N][rank]
   const float* factors;   // [slots], or nullptr: ones
   void* out;
@@ -246,11 +251,12 @@ struct UpParams {
 // out[row][n] = sum of the GEMM's pieces (+ what out holds) + f_s sum over r of t[row][r] B_s[n][r].  grid (groups, blocks of 256 columns), 32 columns a warp: its four
 // tiles of the MMA take columns 8 (n / 2) + 2 tile + n % 2, so that a thread's results of a row are eight neighbours.  t is split into two bf16 halves, hi and lo:
 // 16 bits of it, where the projection's x has eight.
-template <int kRank, bool kTurns, class List>
+template <int kRank, Up kUp, class List>
 __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p, const __grid_constant__ List list) {
   constexpr int kStride = kRank + 8, kSlices = (kRank + 31) / 32;   // k slices of 32 (one, of 8 or 16, for small ranks)
   __shared__ __align__(16) uint16_t t_hi[kGroupRows * kStride], t_lo[kGroupRows * kStride];
   __shared__ int32_t rows[kGroupRows];
+  constexpr bool kTurns = kUp == kInTurns, kFew = kUp == kTInPieces;
   chain_release();
   const int slot = group_rows(list, blockIdx.x, rows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -328,7 +334,19 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
   if (slot >= 0) {
     for (int i = threadIdx.x; i < kGroupRows * kRank / 4; i += kLoraThreads) {
       const int at = 4 * i / kRank, r = 4 * i % kRank, row = rows[at];
-      const float4 v = row >= 0 ? load_chained(reinterpret_cast<const float4*>(p.t + (size_t)row * kRank + r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (List::kNamesRows && kFew) {
+        if (row >= 0) {
+          const float* src = p.t + (size_t)row * p.t_cols + used_of(list, blockIdx.x) * kRank + r;
+#pragma unroll 8
+          for (int s = 0; s < p.t_parts; s++) {
+            const float4 u = load_chained(reinterpret_cast<const float4*>(src + (size_t)s * p.M * p.t_cols));
+            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+          }
+        }
+      } else {
+        if (row >= 0) v = load_chained(reinterpret_cast<const float4*>(p.t + (size_t)row * kRank + r));
+      }
       uint2 hi, lo;
       split_halves(v, factor, hi, lo);
       *reinterpret_cast<uint2*>(t_hi + at * kStride + r) = hi;
@@ -407,10 +425,13 @@ bool by_slot(const Request& a, const Request& b) { return a.slot < b.slot; }
 template <int kCap>
 int make_list(std::vector<Request> r, RowList<kCap>* list) {
   std::stable_sort(r.begin(), r.end(), by_slot);
-  int groups = 0, at = 0;
+  int groups = 0, at = 0, used = -1;
   for (const Request& q : r)
     for (int i = 0; i < q.n; i++, at++) {
-      if (!groups || list->group[groups - 1].slot != q.slot || list->group[groups - 1].n == kGroupRows) list->group[groups++] = {q.slot, (int16_t)at, 0};
+      if (!groups || list->group[groups - 1].slot != q.slot || list->group[groups - 1].n == kGroupRows) {
+        used += q.slot >= 0 && (!groups || list->group[groups - 1].slot != q.slot);
+        list->group[groups++] = {q.slot, (int16_t)at, 0, used};
+      }
       list->group[groups - 1].n++;
       list->row[at] = (int16_t)(q.row + i);
     }
@@ -468,10 +489,19 @@ template <int kRank, class List>
 int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
   const dim3 grid((unsigned)groups, (unsigned)((prm.N + kUpCols - 1) / kUpCols));
-  if (prm.part && prm.rg.in_turns())
-    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, true, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
-  else
-    RELUX_CUDA_TRY(launch_chained(chained, lora_up_kernel<kRank, false, List>, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+  auto go = [&](auto kernel) -> int32_t {
+    RELUX_CUDA_TRY(launch_chained(chained, kernel, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+    return RELUX_OK;
+  };
+  int32_t rc;
+  if (prm.part && prm.rg.in_turns()) {
+    rc = go(lora_up_kernel<kRank, kInTurns, List>);
+  } else if constexpr (std::is_same_v<List, RowList<kFewRows>>) {
+    rc = prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
+  } else {
+    rc = go(lora_up_kernel<kRank, kPlain, List>);
+  }
+  if (rc) return rc;
   count_launch(p->dev);
   return RELUX_OK;
 }
@@ -625,18 +655,43 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : nullptr, row_slots, nullptr, down.t, nullptr, nullptr);
   }
 
+  // Of up to 128 rows t may be further columns of the projection, all rows with every adapter in use (AdapterColumns): their bytes are the adapters', read once, and a launch less.  It
+  // pays where they are few or many: between, a step of adapters of small rank is more boxes than a step of W, and the other form reads little (bf16 rows x 4096 x 4096: 64 rows, rank 16, 16
+  // slots 15.5 us so, 19.0 by lora_down_kernel; 64 rows x 6144, rank 16, 48 slots 24.6 and 20.6, rank 32 25.3 and 27.4; 32 rows, rank 128 29.7 and 46.4; 16 float32 rows, rank 64
+  // 20.3 and 18.3; 40 rows x 1024 x 1024, rank 8, 8 slots 13.4 and 9.7).  Parts of K by the call's sizes alone, so that a row's sums do not depend on the adapters of the others.
+  const int most = std::min(a->m, a->n_slots);
+  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 256 || most * a->rank >= 1536);
+  const int tiles_of_t = (std::min(most, kFewRows) * a->rank + 127) / 128;
+  const int t_parts = std::min({8, 2 * p->dev->sm_count / tiles_of_t, (a->k + 63) / 64 / 4});
   LayerScratch sc;
-  if ((rc = layer_scratch(p, a->m, a->k, a->w ? a->n : 0, t_bytes, &sc, true))) return rc;
-  if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
-  down.t = (float*)sc.rest;
-  if ((rc = run_down(p, x_bf16, down, requests))) return rc;
+  if ((rc = layer_scratch(p, a->m, a->k, a->w ? a->n : 0, columns ? t_bytes * most * t_parts : t_bytes, &sc, true))) return rc;
   UpParams up{};
-  if (a->w) {
+  if (columns) {
+    AdapterColumns cols{a->lora_a, a->n_slots, a->rank, 0, t_parts, (float*)sc.rest, {}};
+    std::vector<int32_t> ids;
+    for (const Request& r : requests)
+      if (r.slot >= 0) ids.push_back(r.slot);
+    std::sort(ids.begin(), ids.end());
+    cols.n_used = (int)(std::unique_copy(ids.begin(), ids.end(), cols.slot) - cols.slot);
+    if (!x_bf16 && (rc = launch_cast(p, (const float*)a->x, sc.a_bf16, (size_t)a->m * a->k))) return rc;
     const WeightRef w{a->w, a->n};
-    if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
+    if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg, TimeStamp{nullptr, nullptr}, &cols, x_bf16)))
+      return rc;
     up.part = sc.part;
+    up.t_parts = t_parts;
+    up.t_cols = cols.n_used * a->rank;
+    up.t = cols.t;
+  } else {
+    if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
+    down.t = (float*)sc.rest;
+    if ((rc = run_down(p, x_bf16, down, requests))) return rc;
+    if (a->w) {
+      const WeightRef w{a->w, a->n};
+      if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
+      up.part = sc.part;
+    }
+    up.t = down.t;
   }
-  up.t = down.t;
   up.b = (const uint16_t*)a->lora_b;
   up.factors = a->factors;
   up.out = a->out;

@@ -76,6 +76,15 @@ struct GemmWalk {
   }
 };
 
+// Further columns of a projection of up to 128 rows: x A_s^T of every adapter in use, for every row (a row's own are what is read of them).  A tile is 128 / rank adapters, cut into
+// `parts` equal parts of K, which are dealt to the workers behind their pieces: cuts that do not depend on which adapters they are.
+constexpr int kMaxUsed = 128;
+struct AdapterColumns {
+  const void* lora_a;        // [n_slots][rank][K]
+  int32_t n_slots, rank, n_used, parts;
+  float* t;                  // [part][M][n_used * rank]
+  int32_t slot[kMaxUsed];
+};
 struct WeightRef {
   const void* w;
   int n;
@@ -92,8 +101,8 @@ int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, L
 // n float32 values, a multiple of 8, rounded to bf16 by the reference's rule.
 int32_t launch_cast(Pool* p, const float* src, uint16_t* dst, size_t n);
 bool gemm_sm100_eligible(int K, const WeightRef* ws, int nw);
-// part[piece][M][n_total] = A[M][K] x [W_0 | W_1 | ...]; returns the ranges, which say how many pieces every tile has.
+// part[piece][M][n_total] = A[M][K] x [W_0 | W_1 | ...]; returns the ranges, which say how many pieces every tile has.  head: nothing of the call is before it.
 int32_t launch_skinny_gemm(Pool* p, const uint16_t* a_bf16, int M, int K, const WeightRef* ws, int nw, float* part, size_t part_cap_bytes,
-                           GemmRanges* ranges, TimeStamp time = TimeStamp{nullptr, nullptr});
+                           GemmRanges* ranges, TimeStamp time = TimeStamp{nullptr, nullptr}, const AdapterColumns* adapters = nullptr, bool head = false);
 
 }  // namespace relux

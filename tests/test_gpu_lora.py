@@ -186,7 +186,8 @@ def test_infinities_and_nan_stay_with_their_request(dev, pool):
 
 
 # requests of a row each, few and so few that float32 rows are split; requests whose tiles are nearly full, with rows past their ends
-FORMS = [([1] * 4, [0, 1, 2, -1], True), ([1] * 4, [-1, 2, 1, 0], False), ([1] * 12, [0, 1, 2, -1] * 3, True), ([1] * 8, [0, 1, 2, -1] * 2, False), ([250, 128, 380, 90], [0, 1, 2, -1], True), ([90, 380, 128, 250], [2, -1, 1, 0], False)]
+FORMS = [([1] * 4, [0, 1, 2, -1], True), ([1] * 4, [-1, 2, 1, 0], False), ([1] * 12, [0, 1, 2, -1] * 3, True), ([1] * 8, [0, 1, 2, -1] * 2, False), ([250, 128, 380, 90], [0, 1, 2, -1], True), ([90, 380, 128, 250], [2, -1, 1, 0], False),
+         ([1, 2, 0, 7, 5, 3, 1, 11], [0, 1, 2, -1] * 2, True), ([9, 1, 60, 20, 3], [2, -1, 1, 0, 2], False)]
 
 
 @pytest.mark.parametrize("rows,adapter,x_bf16", FORMS)
@@ -205,12 +206,12 @@ def test_added_in_every_form(dev, pool, rows, adapter, x_bf16, out_bf16, K, N, r
 
 
 @pytest.mark.parametrize("rows,adapter,x_bf16", FORMS)
-@pytest.mark.parametrize("rank", [16, 8])
-def test_infinities_and_nan_in_every_form(dev, pool, rows, adapter, x_bf16, rank):
+@pytest.mark.parametrize("K,rank", [(264, 16), (264, 8), (2056, 16), (2056, 64)])
+def test_infinities_and_nan_in_every_form(dev, pool, rows, adapter, x_bf16, K, rank):
     """The second adapter and a row of the third's hold NaN, a column of the third an infinity: what the formula leaves finite is."""
     from oracle import binding as orc
     rng = np.random.default_rng(17)
-    c = Case(dev, rng, rows, adapter, 264, 392, rank, 3, x_bf16)
+    c = Case(dev, rng, rows, adapter, K, 392, rank, 3, x_bf16)
     c.a[1, 3, 7], c.b[2, 5, :] = np.nan, np.inf
     c.da.upload(orc.bf16_from_f32(c.a)), c.db.upload(orc.bf16_from_f32(c.b))
     ids = np.repeat(np.asarray(adapter), rows)
@@ -237,13 +238,27 @@ def test_a_few_rows(dev, pool, M, rank, K, N, x_bf16):
     c.free()
 
 
-def test_rows_alone_and_among_others(dev, pool):
+@pytest.mark.parametrize("M,slots,rank", [(17, 1, 8), (17, 40, 128), (33, 3, 64), (40, 15, 16), (64, 64, 32), (100, 2, 128), (128, 128, 128), (128, 30, 8), (65, 48, 64)])
+@pytest.mark.parametrize("K,N", [(2048, 8), (2056, 1288), (4096, 136)])
+@pytest.mark.parametrize("x_bf16", [False, True])
+def test_few_rows_of_long_k(dev, pool, M, slots, rank, K, N, x_bf16):
+    rng = np.random.default_rng(M + slots + K)
+    for adapter in (rng.integers(-1, slots, M), rng.permutation(M) % (slots + 1) - 1, np.full(M, -1)):
+        c = Case(dev, rng, [1] * M, adapter, K, N, rank, slots, x_bf16, not x_bf16)
+        for _ in range(2):
+            c.call(pool)
+        c.check()
+        c.free()
+
+
+@pytest.mark.parametrize("K,rank,slots", [(520, 32, 5), (2056, 32, 5), (4096, 128, 24)])
+def test_rows_alone_and_among_others(dev, pool, K, rank, slots):
     """A request's rows are the same bits whatever other requests' adapters are."""
     rng = np.random.default_rng(13)
-    c = Case(dev, rng, [1] * 24, [0] * 24, 520, 392, 32, 5)
+    c = Case(dev, rng, [1] * 24, [0] * 24, K, 392, rank, slots)
     c.call(pool)
     alone = c.get()
-    c.adapter = rng.integers(-1, 5, 24).astype(np.int32)
+    c.adapter = rng.integers(-1, slots, 24).astype(np.int32)
     c.adapter[[3, 17]] = 0
     c.call(pool)
     assert np.array_equal(c.get()[[3, 17]], alone[[3, 17]])
@@ -256,7 +271,8 @@ def test_calls_without_waiting_and_in_graphs(dev, pool):
     from relux_b200 import lib as L
     rng = np.random.default_rng(14)
     cases = [Case(dev, rng, rows, ad, K, N, r, 6, xb) for rows, ad, K, N, r, xb in
-             [([1], [2], 1024, 520, 16, False), ([1] * 40, list(rng.integers(-1, 6, 40)), 264, 1032, 8, True), ([300, 5, 77], [3, -1, 5], 520, 264, 64, False)]]
+             [([1], [2], 1024, 520, 16, False), ([1] * 40, list(rng.integers(-1, 6, 40)), 264, 1032, 8, True), ([300, 5, 77], [3, -1, 5], 520, 264, 64, False),
+              ([1] * 40, list(rng.integers(-1, 6, 40)), 2056, 1032, 32, True), ([1] * 20, list(rng.integers(-1, 6, 20)), 4096, 264, 128, False)]]
     for c in cases:
         c.call(pool)
     graph = Graph(dev, lambda: [c.call(pool) for c in cases])

@@ -624,7 +624,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   // rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
   const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256) && a->n_slots <= 32767;
   LoraTiles tiles;
-  const bool wide = a->w && !narrow && (int64_t)a->n_slots * a->n < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
+  const bool wide = a->w && !narrow && (int64_t)a->n_slots * std::max(a->n, a->rank) < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
   if (wide) {
     const size_t x_bytes = x_bf16 ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
     if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes))) return rc;

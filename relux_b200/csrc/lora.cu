@@ -657,10 +657,10 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
 
   // Of up to 128 rows t may be further columns of the projection, all rows with every adapter in use (AdapterColumns): their bytes are the adapters', read once, and a launch less.  It
   // pays where they are few or many: between, a step of adapters of small rank is more boxes than a step of W, and the other form reads little (bf16 rows x 4096 x 4096: 64 rows, rank 16, 16
-  // slots 15.5 us so, 19.0 by lora_down_kernel; 64 rows x 6144, rank 16, 48 slots 24.6 and 20.6, rank 32 25.3 and 27.4; 32 rows, rank 128 29.7 and 46.4; 16 float32 rows, rank 64
+  // slots 15.5 us so, 19.0 by lora_down_kernel; 20 float32 rows, rank 16, 20 slots 14.9 and 16.3; 64 rows x 6144, rank 16, 48 slots 24.6 and 20.6, rank 32 25.3 and 27.4; 32 rows, rank 128 29.7 and 46.4; 16 float32 rows, rank 64
   // 20.3 and 18.3; 40 rows x 1024 x 1024, rank 8, 8 slots 13.4 and 9.7).  Parts of K by the call's sizes alone, so that a row's sums do not depend on the adapters of the others.
   const int most = std::min(a->m, a->n_slots);
-  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 256 || most * a->rank >= 1536);
+  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 320 || most * a->rank >= 1536);
   const int tiles_of_t = (std::min(most, kFewRows) * a->rank + 127) / 128;
   const int t_parts = std::min({8, 2 * p->dev->sm_count / tiles_of_t, (a->k + 63) / 64 / 4});
   LayerScratch sc;

@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
-constexpr int kMaxParts = 8, kGroupRows = 16;
+constexpr int kGroupRows = 16;
 constexpr int kMostRows = 1 << 30;                   // places are counted in 32 bits, a group past the last
 constexpr int kFewRows = 128, kSomeRows = 512;       // of up to so many rows a list names each
 constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
@@ -542,12 +542,14 @@ int32_t with_rank(int rank, F f) {
     default: return f(std::integral_constant<int, 128>());
   }
 }
-int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests) {
+// beside: the launch behind it streams W meanwhile.
+int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests, bool beside) {
   return for_lists(prm.M, requests, [&](const auto& list, int groups) {
     using List = std::decay_t<decltype(list)>;
-    // parts of K: two blocks an SM where groups are full, of 256 k at least, a step of every warp.  By the call's sizes alone: a row's sums do not depend on the
-    // adapters of the others.
-    const int parts = std::max(1, std::min({kMaxParts, 2 * p->dev->sm_count / ((prm.M + kGroupRows - 1) / kGroupRows), prm.K / 256}));
+    // parts of K: two blocks an SM where groups are full, of 1024 k at least, four at most and beside another launch two: larger clusters start late (64 bf16 rows x 4096 x 6144, rank
+    // 16: 23.3 us in one part, 19.5 in four, 20.7 in eight; 300 rows x 4096: 29.5 in four, 35.0 in eight; beside lora_gemm_kernel, 12 rows x 4096: 12.0 in two, 13.2 in four, 13.8 in eight).
+    // By the call's sizes alone: a row's sums do not depend on the adapters of the others.
+    const int parts = std::max(1, std::min({beside ? 2 : 4, 2 * p->dev->sm_count / ((prm.M + kGroupRows - 1) / kGroupRows), prm.K / 1024}));
     // slices of the rank: of few rows 16, so that more SMs read an adapter (one row of rank 128 x 4096 x 4096: 23 us with the whole rank a block); of many 64, since
     // every slice reads x again
     if (prm.rank == 8) return launch_down<8>(p, prm, list, groups, parts, x_bf16);
@@ -648,7 +650,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     if (!one) {
       if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;
       down.t = (float*)p->layer_buf.p;
-      if ((rc = run_down(p, x_bf16, down, requests))) return rc;
+      if ((rc = run_down(p, x_bf16, down, requests, true))) return rc;
     }
     int16_t row_slots[kNarrowRows];
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
@@ -684,7 +686,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   } else {
     if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
     down.t = (float*)sc.rest;
-    if ((rc = run_down(p, x_bf16, down, requests))) return rc;
+    if ((rc = run_down(p, x_bf16, down, requests, false))) return rc;
     if (a->w) {
       const WeightRef w{a->w, a->n};
       if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg))) return rc;

@@ -621,9 +621,9 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   down.rank = a->rank;
   const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
 
-  // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16: one row 11.6 us so and 13.3 with lora_up_kernel, 16
-  // rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with one launch and most of their
-  // rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
+  // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16, with lora_down_kernel in eight parts of K both: one row 11.6 us so and
+  // 13.3 with lora_up_kernel, 16 rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with most of
+  // their rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
   const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256) && a->n_slots <= 32767;
   LoraTiles tiles;
   const bool wide = a->w && !narrow && (int64_t)a->n_slots * std::max(a->n, a->rank) < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
@@ -644,8 +644,8 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     return launch_lora_gemm(p, a, x_bf16 ? x : rounded, nullptr, &tiles, nullptr, t_hi, t_lo);
   }
   if (narrow) {
-    // In one launch, every CTA of which takes t over its part of K: of so few sums, and so few tiles that read the same pieces of an adapter at once (one row x 4096 x 4096, rank 16:
-    // 10.8 us so, 12.3 in two; rank 32 11.3 and 13.2; rank 64 15.9 and 13.2; rank 16 x 4096 x 14336 27.9 and 21.9).
+    // In one launch, every CTA of which takes t over its part of K: of so few sums, and so few tiles that read the same pieces of an adapter at once (one row, rank 16, x 4096 x 1024
+    // 6.6 us so, 7.9 in two; x 256 x 4096 4.4 and 5.6; x 4096 x 4096 10.3 and 10.5; rank 32 10.9 and 10.75; rank 16 x 4096 x 14336 27.9 and 21.9).
     const bool one = a->m * a->rank <= kOneT && (a->n - 1) / kRowsOp + 1 <= p->dev->sm_count / 4;
     if (!one) {
       if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;
@@ -658,11 +658,12 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   }
 
   // Of up to 128 rows t may be further columns of the projection, all rows with every adapter in use (AdapterColumns): their bytes are the adapters', read once, and a launch less.  It
-  // pays where they are few or many: between, a step of adapters of small rank is more boxes than a step of W, and the other form reads little (bf16 rows x 4096 x 4096: 64 rows, rank 16, 16
-  // slots 15.5 us so, 19.0 by lora_down_kernel; 20 float32 rows, rank 16, 20 slots 14.9 and 16.3; 64 rows x 6144, rank 16, 48 slots 24.6 and 20.6, rank 32 25.3 and 27.4; 32 rows, rank 128 29.7 and 46.4; 16 float32 rows, rank 64
-  // 20.3 and 18.3; 40 rows x 1024 x 1024, rank 8, 8 slots 13.4 and 9.7).  Parts of K by the call's sizes alone, so that a row's sums do not depend on the adapters of the others.
+  // pays where they are few, or large: of small rank a step of adapters is more boxes than a step of W (bf16 rows x 4096 x 4096: 64 rows, 16 slots of rank 16 15.6 us so, 18.1 by
+  // lora_down_kernel; 32 rows, rank 128 29.9 and 36.3; 64 float32 rows, 48 slots of rank 64 29.2 and 31.2; 20, rank 16, 20 slots 15.2 and 15.7; 64 rows x 6144, 48 slots, rank 16 24.6
+  // and 19.5, rank 32 25.3 and 22.7; 40 rows x 1024 x 1024, 8 slots of rank 8 13.4 and 9.7).  Parts of K by the call's sizes alone, so that a row's sums do not depend on the
+  // adapters of the others.
   const int most = std::min(a->m, a->n_slots);
-  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 320 || most * a->rank >= 1536);
+  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 320 || (a->rank >= 64 && most * a->rank >= 2048));
   const int tiles_of_t = (std::min(most, kFewRows) * a->rank + 127) / 128;
   const int t_parts = std::min({8, 2 * p->dev->sm_count / tiles_of_t, (a->k + 63) / 64 / 4});
   LayerScratch sc;

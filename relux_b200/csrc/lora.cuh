@@ -7,7 +7,7 @@
 namespace relux {
 
 constexpr int kNarrowRows = 16;     // calls of up to so many rows: one block of rows, float32 ones split by lora_gemm_kernel, adapters on the CUDA cores
-constexpr int kOneT = 32;           // rows x rank of calls in one launch
+constexpr int kOneT = 16;           // rows x rank of calls in one launch
 constexpr int kMaxLoraTiles = 1024; // row tiles of a longer call
 
 // Tiles of up to 128 neighbouring rows of one adapter.

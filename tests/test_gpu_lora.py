@@ -238,6 +238,24 @@ def test_a_few_rows(dev, pool, M, rank, K, N, x_bf16):
     c.free()
 
 
+@pytest.mark.parametrize("adapter", [[0, 1], [1, 0], [-1, 1], [0, -1], [0, 0]])
+@pytest.mark.parametrize("x_bf16", [False, True])
+def test_two_rows_added_beside_nan(dev, pool, adapter, x_bf16):
+    """The second adapter is NaN throughout: rows of the other, or of none, are as if it were not there."""
+    from oracle import binding as orc
+    rng = np.random.default_rng(18)
+    c = Case(dev, rng, [1, 1], adapter, 1032, 520, 8, 2, x_bf16)
+    c.a[1], c.b[1] = np.nan, np.nan
+    c.da.upload(orc.bf16_from_f32(c.a)), c.db.upload(orc.bf16_from_f32(c.b))
+    before = G.bf16(rng.standard_normal((2, 520)).astype(np.float32))
+    c.out.upload(before)
+    c.call(pool, accumulate=True)
+    out, bound = c.plain(before)
+    got, fine = c.get(), np.asarray(adapter) != 1
+    assert np.isnan(got[~fine]).all() and (np.abs(got - out)[fine] <= (bound + np.abs(before) * 2.0 ** -23)[fine]).all()
+    c.free()
+
+
 @pytest.mark.parametrize("M,slots,rank", [(17, 1, 8), (17, 40, 128), (33, 3, 64), (40, 15, 16), (64, 64, 32), (100, 2, 128), (128, 128, 128), (128, 30, 8), (65, 48, 64)])
 @pytest.mark.parametrize("K,N", [(2048, 8), (2056, 1288), (4096, 136)])
 @pytest.mark.parametrize("x_bf16", [False, True])

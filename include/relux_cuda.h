@@ -702,7 +702,8 @@ int32_t relux_matmul_int8(relux_pool_t pool, const relux_matmul_int8_args* args)
  * whose requests have adapters of their own, in as many launches; rows of requests without one (-1) are the shared projection alone.
  * bf16 x is taken as it is.  float32 x is rounded to bf16, as in relux_matmul_f32_bf16's FAST mode; it keeps 16 bits where w is NULL, or m is up to 8 and m * rank up
  * to 256.  x A_s^T is summed in float32 and keeps 16 bits.  Sums are float32 up to the one rounding of the result.  A request's rows depend on its own adapter alone, whatever
- * other slots hold (the order of the sums may go by how the batch's rows are spread over requests).
+ * other slots hold (the order of the sums may go by how the batch's rows are spread over requests).  Infinities and NaN, in x, w, or an adapter, come out where the formula has them and
+ * with its sign.
  * w NULL: no shared projection (it came from relux_matmul_int8, say: with accumulate the adapters are added to what out holds).
  * Requests own neighbouring rows, n_rows[i] of them in order; several may name the same slot.  The host arrays are read before the call returns; a captured
  * call keeps its adapters' places in the batch, the slots' contents are read at every launch.

@@ -17,12 +17,19 @@ struct LoraTiles {
   int16_t rows[kMaxLoraTiles];
 };
 
-// f v as two bf16 halves, 16 bits of it.
+// f v as two bf16 halves, 16 bits of it.  Both have its sign and neither is zero where it is not: the first is the largest of smaller magnitude, the second the rest.  So an infinity that
+// they are multiplied with comes out as the formula has it (with the nearest value first the rest is zero or of the other sign, and the sum of both products NaN).  An infinity, a NaN, a
+// zero are both halves themselves.  The rest is up to 2^-7 of the value, rounded by 2^-9 of itself.
 __device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2& lo) {
-  auto rest = [](float x, float h) { return fabsf(h) < __uint_as_float(0x7F800000u) ? x - h : 0.f; };   // an infinity has no second half
+  auto first = [](float x) {
+    const uint32_t u = __float_as_uint(x), m = u & 0x7FFFFFFFu;
+    return m - 1u < 0x7F7FFFFFu ? __uint_as_float((u & 0x80000000u) | ((m - 1u) & 0xFFFF0000u)) : x;
+  };
+  auto rest = [](float x, float h) { return h == x || x != x ? x : x - h; };
   v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-  hi = make_uint2(round_bf16x2(v.x, v.y), round_bf16x2(v.z, v.w));
-  lo = make_uint2(round_bf16x2(rest(v.x, bf16_lo(hi.x)), rest(v.y, bf16_hi(hi.x))), round_bf16x2(rest(v.z, bf16_lo(hi.y)), rest(v.w, bf16_hi(hi.y))));
+  const float4 h = make_float4(first(v.x), first(v.y), first(v.z), first(v.w));
+  hi = make_uint2(round_bf16x2(h.x, h.y), round_bf16x2(h.z, h.w));
+  lo = make_uint2(round_bf16x2(rest(v.x, h.x), rest(v.y, h.y)), round_bf16x2(rest(v.z, h.z), rest(v.w, h.w)));
 }
 
 // out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kNarrowRows float32 rows of the

@@ -8,7 +8,7 @@
 //   * Wide tiles (bound: the tensor cores): every tile holds rows of one request, so that t B_s^T is further K steps of the same accumulator, t as two
 //     bf16 halves, hi and lo.  Rows of the tile past the request's end are computed with the wrong adapter and not stored.
 //     A row never meets another request's adapter by way of a zero: zero times an infinity in that adapter would be NaN in this row.
-//   * Of a row or two every CTA takes t over its part of K itself, and adds t B_s^T to its own part of the sums: no launch before this one.
+//   * Of a row or two every CTA takes t over its part of K itself, and the parts of t go to the others with the slices of the sums: no launch before this one.
 // Behind another launch of the call W is read ahead of it, and bf16 x too: that one is a chain's head (launch_chained).
 #include "lora.cuh"
 #include "tile_gemm.cuh"
@@ -48,7 +48,7 @@ struct LoraGemmParams {
   void* out;
   int32_t* status;
 };
-static_assert(kOneT * 4 <= kRowsT && kOneT / 8 * kRowsOp * 4 <= kRing * 256 * 16, "no room for a part's t");
+static_assert(LoraShape<kNarrowRows>::kMaxCluster * kOneT * 4 <= kRowsT && LoraShape<kNarrowRows>::kMaxCluster * kOneT <= 128, "no room for the parts of t, or no thread");
 struct NarrowRows {
   int16_t slot[kNarrowRows];   // of every row, or -1
 };
@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC, kOne>, 1) lora_gemm_kerne
     low_sync();
   };
 
-  // In one launch: a row's slice of t over this CTA's part of K, [row][rank] with factors, by the epilogue's warps and the last four, four sums of a row a warp at a time.
+  // In one launch: the part of t that comes from this CTA's part of K, [row][rank] with factors, by the epilogue's warps and the last four, four sums of a row a warp at a time.  The
+  // cluster's parts lie side by side, kOneT values each.
   auto down_part = [&] {
     const int c0 = rank * prm.steps / size * 64, c1 = min((rank + 1) * prm.steps / size * 64, prm.K);
     for (int d = 4 * (warp < 4 ? warp : warp - 6); d < prm.M * prm.rank; d += 32) {   // (a rank is a multiple of eight)
@@ -200,35 +201,47 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC, kOne>, 1) lora_gemm_kerne
 #pragma unroll
       for (int i = 0; i < 4; i++) sum[i] = warp_sum(sum[i]);
       const float f = slot >= 0 && prm.factors ? load_chained(prm.factors + slot) : 1.f;
-      if (lane < 4) t_rows[d + lane] = f * (lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3]);
+      if (lane < 4) t_rows[rank * kOneT + d + lane] = f * (lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3]);
     }
   };
-  // and that part's t B_s^T of a tile, a thread a column: to the CTA's own sums of the tile, [row][128]
-  float* const part_low = t_rows + kRowsT / 4 + threadIdx.x;
-  auto low_part = [&](const Place& at, bool first_tile) {
-    const int n = at.c * kRowsOp + threadIdx.x, shift = 31 - __clz(prm.rank >> 3), last = (prm.rank >> 3) - 1;   // ranks are powers of two
-    uint4 w[kOneT / 8];
+  // The parts to the others, with the slices: a thread a value and a CTA.
+  auto send_parts = [&] {
+    const int i = threadIdx.x % kOneT, to = threadIdx.x / kOneT;
+    if (to < size && to != rank && i < prm.M * prm.rank)
+      store_cluster(mapa_u32(smem_u32(t_rows + rank * kOneT + i), (uint32_t)to), __float_as_uint(t_rows[rank * kOneT + i]));
+  };
+  // t B_s^T of a tile, a thread a column, for each of up to kOneT / 8 rows: of all of t, since parts of it that an infinity in B_s is multiplied with may differ in sign.
+  uint4 b_own[kOneT / 8];
+  const int one_shift = 31 - __clz(prm.rank >> 3), one_last = (prm.rank >> 3) - 1;   // ranks are powers of two
+  auto load_b = [&](const Place& at) {
+    const int n = at.c * kRowsOp + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kOneT / 8; i++) {
-      const int row = i >> shift, slot = row < prm.M ? list.slot[row] : -1;
-      w[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (slot >= 0 && n < prm.N) w[i] = load_chained(reinterpret_cast<const uint4*>(prm.b + ((size_t)slot * prm.N + n) * prm.rank) + (i & last));
+      const int row = i >> one_shift, slot = row < prm.M ? list.slot[row] : -1;
+      b_own[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (slot >= 0 && n < prm.N) b_own[i] = load_chained(reinterpret_cast<const uint4*>(prm.b + ((size_t)slot * prm.N + n) * prm.rank) + (i & one_last));
     }
-    if (first_tile) {
-      down_part();
-      low_sync();
-    }
+  };
+  auto low_of = [&](float (&low)[kOneT / 8]) {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kOneT / 8; i++) {
-      const float4* t = reinterpret_cast<const float4*>(t_rows + 8 * i);
-      if (8 * i < prm.M * prm.rank) {
-        const float4 t0 = t[0], t1 = t[1];
-        if ((i & last) == 0) sum = 0.f;
-        sum = fmaf(t0.x, bf16_lo(w[i].x), sum); sum = fmaf(t0.y, bf16_hi(w[i].x), sum); sum = fmaf(t0.z, bf16_lo(w[i].y), sum); sum = fmaf(t0.w, bf16_hi(w[i].y), sum);
-        sum = fmaf(t1.x, bf16_lo(w[i].z), sum); sum = fmaf(t1.y, bf16_hi(w[i].z), sum); sum = fmaf(t1.z, bf16_lo(w[i].w), sum); sum = fmaf(t1.w, bf16_hi(w[i].w), sum);
-        if ((i & last) == last) part_low[(i >> shift) * kRowsOp] = sum;
+      if (8 * i >= prm.M * prm.rank) continue;
+      float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
+#pragma unroll 1
+      for (int s = 0; s < size; s++) {
+        const float4* t = reinterpret_cast<const float4*>(t_rows + s * kOneT + 8 * i);
+        const float4 u = t[0], v = t[1];
+        t0.x += u.x; t0.y += u.y; t0.z += u.z; t0.w += u.w;
+        t1.x += v.x; t1.y += v.y; t1.z += v.z; t1.w += v.w;
       }
+      const uint4 w = b_own[i];
+      if ((i & one_last) == 0) sum = 0.f;
+      sum = fmaf(t0.x, bf16_lo(w.x), sum); sum = fmaf(t0.y, bf16_hi(w.x), sum); sum = fmaf(t0.z, bf16_lo(w.y), sum); sum = fmaf(t0.w, bf16_hi(w.y), sum);
+      sum = fmaf(t1.x, bf16_lo(w.z), sum); sum = fmaf(t1.y, bf16_hi(w.z), sum); sum = fmaf(t1.z, bf16_lo(w.w), sum); sum = fmaf(t1.w, bf16_hi(w.w), sum);
+#pragma unroll
+      for (int r = 0; r < kOneT / 8; r++)
+        if (r == i >> one_shift) low[r] = sum;   // the last of a row's chunks stays
     }
   };
 
@@ -398,19 +411,28 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC, kOne>, 1) lora_gemm_kerne
       const int grain = !kWide ? 1 : prm.out_bf16 ? 64 : 32;
       const int q0 = size > 1 ? slice_begin(rank, cols, grain, size) : 0, q1 = size > 1 ? slice_begin(rank + 1, cols, grain, size) : cols;
       const float* const got = reinterpret_cast<const float*>(slices) + threadIdx.x;
-      if constexpr (kOne) low_part(at, tile == first);
-      else if constexpr (!kWide) low_half(at, 0);
+      if constexpr (kOne) {
+        load_b(at);
+        if (tile == first) {
+          down_part();
+          low_sync();
+        }
+      } else if constexpr (!kWide) {
+        low_half(at, 0);
+      }
       tile_wait(&bars->acc_full[buf], (piece >> 1) & 1, bars, prm.status);
       tc_fence_after();
       const bool ok = !bars->abort_flag;
       if (size > 1) {
-        if constexpr (kOne) swap_slices<SH>(acc, cols, grain, size, rank, slices, [&](int q, uint32_t v) { return __float_as_uint(__uint_as_float(v) + part_low[q * kRowsOp]); });
+        if constexpr (kOne) swap_slices<SH>(acc, cols, grain, size, rank, slices, send_parts);
         else swap_slices<SH>(acc, cols, grain, size, rank, slices);
       }
       if constexpr (!kWide) {
         // thread = column; a warp writes 64 or 128 bytes of a row at once
         const int n = at.c * kRowsOp + warp * 32 + lane;
         const bool mine = n < prm.N;
+        float low[kOneT / 8] = {};
+        if constexpr (kOne) low_of(low);
 #pragma unroll 1
         for (int q = q0; q < q1; q += 8) {
           uint32_t v[8];
@@ -429,15 +451,17 @@ __global__ void __launch_bounds__(kLoraGemmThreads<NC, kOne>, 1) lora_gemm_kerne
           float x[8];
 #pragma unroll
           for (int i = 0; i < 8; i++) x[i] = ok ? __uint_as_float(v[i]) : 0.f;
-          if constexpr (kOne)
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-              if (q + i < q1) x[i] += part_low[(q + i) * kRowsOp];
 #pragma unroll 1
           for (int s = 0; s < (kOne ? size - 1 : size); s++)   // the others' parts, then the adapter's
 #pragma unroll
             for (int i = 0; i < 8; i++)
               if (q + i < q1) x[i] += got[(s * (q1 - q0) + q - q0 + i) * kRowsOp];
+          if constexpr (kOne)
+#pragma unroll
+            for (int r = 0; r < kOneT / 8; r++)
+#pragma unroll
+              for (int i = 0; i < 8; i++)
+                if (q + i == r) x[i] += low[r];
 #pragma unroll
           for (int i = 0; i < 8; i++) x[i] += before[i];
           if (prm.out_bf16) {

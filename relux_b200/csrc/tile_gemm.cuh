@@ -112,13 +112,14 @@ __device__ __forceinline__ uint32_t tile_setup(TileBars* bars, int size, int fil
 // The epilogue's warps, a tile that is cut along K: slices to the others, [from][column of the slice][128 rows], and back when all have arrived.
 // (A warp's store is 128 neighbouring bytes; 16 bytes a thread to rows that lie apart took 3 us longer for 200 x 4096 x 4096.)
 // part i of K is CTA i of the cluster, or (kPer 2) the CTA of this one's side in pair i.
-// sent(column, v): what goes out for v.
-struct AsItIs {
-  __device__ __forceinline__ uint32_t operator()(int, uint32_t v) const { return v; }
+// also(): sends more with them, by all of these warps.
+struct NothingMore {
+  __device__ __forceinline__ void operator()() const {}
 };
-template <class SH, int kPer = 1, class Sent = AsItIs>
-__device__ __forceinline__ void swap_slices(uint32_t acc, int cols, int grain, int size, int rank, const uint8_t* slices, Sent sent = Sent()) {
+template <class SH, int kPer = 1, class Also = NothingMore>
+__device__ __forceinline__ void swap_slices(uint32_t acc, int cols, int grain, int size, int rank, const uint8_t* slices, Also also = Also()) {
   cluster_wait();
+  also();
   if constexpr (SH::kWide) {   // the others' stages: they are free once their MMAs are done
     cluster_arrive();
     cluster_wait();
@@ -138,7 +139,7 @@ __device__ __forceinline__ void swap_slices(uint32_t acc, int cols, int grain, i
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < kAtOnce; i++)
-        if (q + i < e) store_cluster(there + (uint32_t)(q - b + i) * (kRowsOp * 4), sent(q + i, v[i]));
+        if (q + i < e) store_cluster(there + (uint32_t)(q - b + i) * (kRowsOp * 4), v[i]);
     }
   }
   cluster_arrive();

@@ -11,7 +11,7 @@ from tests.test_gpu_lora import Case, dev, pool  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 # every form of the call: one launch, few rows, columns of the projection, groups of 16 rows with and without explicit lists, tiles of one request; each with bf16 and float32 rows
-FORMS = [([1], [1], 264, 16), ([1] * 6, [1, 2, 0, -1, 2, 1], 264, 32), ([1] * 16, [1, 2, 0, -1] * 4, 264, 16), ([1] * 20, [1, 2, 0, -1] * 5, 264, 16),
+FORMS = [([1], [1], 264, 16), ([1, 1], [1, 2], 520, 8), ([1] * 6, [1, 2, 0, -1, 2, 1], 264, 32), ([1] * 16, [1, 2, 0, -1] * 4, 264, 16), ([1] * 20, [1, 2, 0, -1] * 5, 264, 16),
          ([1] * 24, [1, 2, 0, -1] * 6, 2056, 64), ([80, 90, 70, 75], [1, 2, -1, 0], 264, 16), ([1] * 700, [i % 4 - 1 for i in range(700)], 264, 32),
          ([250, 128, 380, 90], [1, 2, 0, -1], 264, 16), ([250, 128, 380, 90], [1, 2, 0, -1], 520, 64), ([250, 128, 380, 90], [1, 2, 0, -1], 2056, 8)]
 N, K_W, COL_W, K_A, COL_B = 392, 11, 17, 7, 5

@@ -624,7 +624,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16, with lora_down_kernel in eight parts of K both: one row 11.6 us so and
   // 13.3 with lora_up_kernel, 16 rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with most of
   // their rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
-  const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256) && a->n_slots <= 32767;
+  const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256);
   LoraTiles tiles;
   const bool wide = a->w && !narrow && (int64_t)a->n_slots * std::max(a->n, a->rank) < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
   if (wide) {
@@ -652,8 +652,8 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
       down.t = (float*)p->layer_buf.p;
       if ((rc = run_down(p, x_bf16, down, requests, true))) return rc;
     }
-    int16_t row_slots[kNarrowRows];
-    for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, (int16_t)r.slot);
+    int32_t row_slots[kNarrowRows];
+    for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, r.slot);
     return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : nullptr, row_slots, nullptr, down.t, nullptr, nullptr);
   }
 

@@ -35,7 +35,7 @@ __device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2
 // out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kNarrowRows float32 rows of the
 // caller's.  Without tiles or t: lora_gemm_kernel takes t itself.  Without tiles (up to kNarrowRows rows): row_slots
 // [M], t [M][rank] without factors; with tiles: t as two bf16 halves [M][rank], factors included.
-int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t,
+int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int32_t* row_slots, const LoraTiles* tiles, const float* t,
                          const uint16_t* t_hi, const uint16_t* t_lo);
 
 // t = f_s x A_s^T of the rows of `tiles` as two bf16 halves [M][rank].  x: bf16 rows [M][K]; nullptr: the caller's float32 ones, which are rounded to `rounded` as well.

@@ -50,7 +50,7 @@ struct LoraGemmParams {
 };
 static_assert(LoraShape<kNarrowRows>::kMaxCluster * kOneT * 4 <= kRowsT && LoraShape<kNarrowRows>::kMaxCluster * kOneT <= 128, "no room for the parts of t, or no thread");
 struct NarrowRows {
-  int16_t slot[kNarrowRows];   // of every row, or -1
+  int32_t slot[kNarrowRows];   // of every row, or -1
 };
 
 template <int NC, class Rows, bool kOne>
@@ -562,7 +562,7 @@ int32_t launch_rows(Pool* p, const LoraMaps& maps, const LoraGemmParams& prm, co
 
 }  // namespace
 
-int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int16_t* row_slots, const LoraTiles* tiles, const float* t,
+int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_t* x, const int32_t* row_slots, const LoraTiles* tiles, const float* t,
                          const uint16_t* t_hi, const uint16_t* t_lo) {
   LoraGemmParams prm{};
   LoraMaps maps{};
@@ -601,7 +601,7 @@ int32_t launch_lora_gemm(Pool* p, const relux_matmul_lora_args* a, const uint16_
   if (tiles) return launch_rows<256, false>(p, maps, prm, *tiles);
   NarrowRows rows;
   std::copy(row_slots, row_slots + M, rows.slot);
-  std::fill(rows.slot + M, rows.slot + kNarrowRows, (int16_t)-1);
+  std::fill(rows.slot + M, rows.slot + kNarrowRows, -1);
   return t ? launch_rows<kNarrowRows, false>(p, maps, prm, rows) : launch_rows<kNarrowRows, true>(p, maps, prm, rows);
 }
 

@@ -707,7 +707,7 @@ int32_t relux_matmul_int8(relux_pool_t pool, const relux_matmul_int8_args* args)
  * w NULL: no shared projection (it came from relux_matmul_int8, say: with accumulate the adapters are added to what out holds).
  * Requests own neighbouring rows, n_rows[i] of them in order; several may name the same slot.  The host arrays are read before the call returns; a captured
  * call keeps its adapters' places in the batch, the slots' contents are read at every launch.
- * Shapes: m up to 2^30, k and n multiples of 8, rank 8, 16, 32, 64 or 128 (a smaller adapter is filled up with zeros).  Adapters as checkpoints hold them (lora_A [rank][in],
+ * Shapes: m, k and n up to 2^30, k and n multiples of 8, rank 8, 16, 32, 64 or 128 (a smaller adapter is filled up with zeros).  Adapters as checkpoints hold them (lora_A [rank][in],
  * lora_B [out][rank]).  out must not overlap x.  Asynchronous on the handle's stream.  No counterpart in the reference, which serves one model. */
 typedef struct relux_matmul_lora_args {
   int32_t m, k, n;

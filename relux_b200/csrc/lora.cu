@@ -25,7 +25,8 @@ namespace {
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
 constexpr int kGroupRows = 16;
-constexpr int kMostRows = 1 << 30;                   // places are counted in 32 bits, a group past the last
+constexpr int kMost = 1 << 30;                       // rows, k, n: counted in 32 bits, a tile past the last
+constexpr int kMostGridY = 65535;
 constexpr int kFewRows = 128, kSomeRows = 512;       // of up to so many rows a list names each
 constexpr int kSmallList = 128, kLargeList = 1024;   // pieces of a list that travels as an argument of the launch
 
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
 enum Up { kPlain, kInTurns, kTInPieces };   // the GEMM's blocks of rows come in turns; t comes in pieces, from the GEMM
 struct UpParams {
   const float* part;      // the GEMM's pieces [piece][M][N]; nullptr: no shared projection
+  int32_t first_block;    // of 256 columns, of this launch
   GemmRanges rg;
   const float* t;         // [M][rank], or (t_parts) in as many pieces [M][t_cols], of every adapter in use for every row
   int32_t t_parts, t_cols;
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
   chain_release();
   const int slot = group_rows(list, blockIdx.x, rows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.y * kUpCols + warp * 32, n = n0 + 8 * t;
+  const int n0 = (p.first_block + (int)blockIdx.y) * kUpCols + warp * 32, n = n0 + 8 * t;
   // adapters were complete before the chain's head began: read ahead of the launches before this one
   uint4 w[kSlices][4];
   float factor = 1.f;
@@ -486,23 +488,26 @@ int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups
   return x_bf16 ? go(lora_down_kernel<kSlice, kBf16, List>) : prm.x_bf16 ? go(lora_down_kernel<kSlice, kRounded, List>) : go(lora_down_kernel<kSlice, kSplit, List>);
 }
 template <int kRank, class List>
-int32_t launch_up(Pool* p, const UpParams& prm, const List& list, int groups) {
+int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups) {
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
-  const dim3 grid((unsigned)groups, (unsigned)((prm.N + kUpCols - 1) / kUpCols));
-  auto go = [&](auto kernel) -> int32_t {
-    RELUX_CUDA_TRY(launch_chained(chained, kernel, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
-    return RELUX_OK;
-  };
-  int32_t rc;
-  if (prm.part && prm.rg.in_turns()) {
-    rc = go(lora_up_kernel<kRank, kInTurns, List>);
-  } else if constexpr (std::is_same_v<List, RowList<kFewRows>>) {
-    rc = prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
-  } else {
-    rc = go(lora_up_kernel<kRank, kPlain, List>);
+  const int blocks = (prm.N + kUpCols - 1) / kUpCols;
+  for (prm.first_block = 0; prm.first_block < blocks; prm.first_block += kMostGridY) {
+    const dim3 grid((unsigned)groups, (unsigned)std::min(blocks - prm.first_block, kMostGridY));
+    auto go = [&](auto kernel) -> int32_t {
+      RELUX_CUDA_TRY(launch_chained(chained, kernel, grid, dim3(kLoraThreads), 0, p->dev->stream, prm, list));
+      return RELUX_OK;
+    };
+    int32_t rc;
+    if (prm.part && prm.rg.in_turns()) {
+      rc = go(lora_up_kernel<kRank, kInTurns, List>);
+    } else if constexpr (std::is_same_v<List, RowList<kFewRows>>) {
+      rc = prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
+    } else {
+      rc = go(lora_up_kernel<kRank, kPlain, List>);
+    }
+    if (rc) return rc;
+    count_launch(p->dev);
   }
-  if (rc) return rc;
-  count_launch(p->dev);
   return RELUX_OK;
 }
 
@@ -601,7 +606,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     }
     rows += n;
   }
-  if (a->m > kMostRows) { set_error("matmul_lora: M=%d above %d", a->m, kMostRows); return RELUX_ERR_UNSUPPORTED; }
+  if (a->m > kMost || a->k > kMost || a->n > kMost) { set_error("matmul_lora: M=%d K=%d N=%d, up to %d each", a->m, a->k, a->n, kMost); return RELUX_ERR_UNSUPPORTED; }
   if (rows != a->m) { set_error("matmul_lora: the requests have %lld rows, M=%d", (long long)rows, a->m); return RELUX_ERR_INVALID_ARG; }
   int32_t rc;
   if ((rc = check_dev_align(a->x, "x")) || (rc = check_dev_align(a->w, "w")) || (rc = check_dev_align(a->lora_a, "lora_a")) || (rc = check_dev_align(a->lora_b, "lora_b")) ||

@@ -428,7 +428,7 @@ int32_t do_int8_weights(Pool* p, const relux_int8_weights_args* a) {
   int32_t rc = check_codes(a->codes, a->scales, a->k);
   if (rc || (rc = check_dev_align(a->w, "w"))) return rc;
   if (a->n % 8 != 0) { set_error("int8_weights: N=%d must be a multiple of 8", a->n); return RELUX_ERR_UNSUPPORTED; }
-  const dim3 grid((unsigned)((a->n + kImpCols - 1) / kImpCols));
+  const dim3 grid((unsigned)((a->n - 1) / kImpCols + 1));
   if (a->w_dtype == RELUX_DTYPE_BF16) int8_weights_kernel<true><<<grid, 256, 0, p->dev->stream>>>(a->w, a->k, a->n, a->codes, a->scales);
   else int8_weights_kernel<false><<<grid, 256, 0, p->dev->stream>>>(a->w, a->k, a->n, a->codes, a->scales);
   RELUX_CUDA_TRY(cudaGetLastError());

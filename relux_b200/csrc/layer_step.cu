@@ -349,6 +349,7 @@ struct FinishParams {
   GemmRanges rg;
   int32_t tile_first[kMaxWeights];   // first 128-column tile of every segment
   int32_t M, n_total, S, n_segs;
+  int32_t row0;                    // first row of this launch
   ProjSeg seg[kMaxWeights];
   const int32_t* len;              // this layer's lengths BEFORE the append
   const int32_t* seq_ids;
@@ -360,7 +361,7 @@ struct FinishParams {
 };
 template <bool kTurns>   // the row blocks come in turns (GemmRanges): a tile is a column and a row
 __global__ void proj_finish_kernel(const FinishParams p) {
-  const int pair = blockIdx.x * blockDim.x + threadIdx.x, m = blockIdx.y;
+  const int pair = blockIdx.x * blockDim.x + threadIdx.x, m = p.row0 + blockIdx.y;
   const int col = 2 * pair;
   chain_release();
   chain_wait();
@@ -647,10 +648,13 @@ int32_t finish_projections(Pool* p, const SeqBatch& sb, int layer, int M, int S,
   f.rope_positions = p->rope_positions;
   f.same_pos = same_pos ? 1 : 0;
   f.status = p->d_status;
-  dim3 grid((f.n_total / 2 + 255) / 256, M);
-  RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, ranges.in_turns() ? proj_finish_kernel<true> : proj_finish_kernel<false>, grid, dim3(256),
-                                0, p->dev->stream, f));
-  count_launch(p->dev);
+  constexpr int kMostGridY = 65535;
+  for (f.row0 = 0; f.row0 < M; f.row0 += kMostGridY) {
+    const dim3 grid((f.n_total / 2 + 255) / 256, std::min(M - f.row0, kMostGridY));
+    RELUX_CUDA_TRY(launch_chained(p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0, ranges.in_turns() ? proj_finish_kernel<true> : proj_finish_kernel<false>, grid, dim3(256),
+                                  0, p->dev->stream, f));
+    count_launch(p->dev);
+  }
   return RELUX_OK;
 }
 

@@ -733,7 +733,8 @@ int32_t relux_matmul_lora(relux_pool_t pool, const relux_matmul_lora_args* args)
  * gave as x and the sum so far as residual.  The feed-forward half begins with relux_rmsnorm of out and that sum.
  * Each of the four projections has the layer's bf16 weight or, where codes are given, 8-bit weights (relux_int8_weights, relux_matmul_int8: the rows are
  * quantised one by one), and adapters of the requests beside it where lora_a is given (relux_matmul_lora; rank and slots are common to the four).  A projection with
- * codes needs no weight in layer->w.  Everything is checked before anything is written to the cache. */
+ * codes needs no weight in layer->w.  Everything is checked, and room made for the projections, before anything is written.  A call that fails later (no memory for attention's partial
+ * results) leaves the cache's lengths as they were, as the layer steps do; residual_out may hold the sum by then. */
 typedef struct relux_block_projection {
   const int8_t* codes;       /* device [n][k], or NULL: the layer's weight */
   const float* scales;       /* device [n], with codes */

@@ -300,6 +300,7 @@ int32_t do_int8_rows(Pool* p, const relux_int8_rows_args* a);
 int32_t do_int8_weights(Pool* p, const relux_int8_weights_args* a);
 int32_t do_matmul_int8(Pool* p, const relux_matmul_int8_args* a);
 int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a);
+size_t matmul_lora_scratch(const Pool* p, const relux_matmul_lora_args* a);   // bytes of layer_buf that such a call asks for; device pointers but w may be missing
 int32_t do_import_mla(Pool* p, const relux_mla_import_args* a);
 int32_t do_selftest_wait(Pool* p, int32_t polls);
 // After a fused call that counted sb's rows and failed: the lengths before it, on the host and, whatever the call had queued

@@ -740,22 +740,24 @@ int32_t layer_batch(Pool* p, int layer, int n_seqs, const int32_t* seq_ids, int 
   return RELUX_OK;
 }
 
-inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
+size_t part_bytes(int M, int max_n, bool few_pieces) {
+  const size_t piece = (size_t)M * max_n * 4, most = (size_t)64 << 20;
+  return pad256(std::max<size_t>(few_pieces ? std::min(most, 8 * piece) : most, piece * 4));
+}
 
 }  // namespace
 
+size_t layer_scratch_bytes(int M, int max_k, int max_n, size_t rest_bytes, bool few_pieces) {
+  return pad256((size_t)M * max_k * 2) + part_bytes(M, max_n, few_pieces) + rest_bytes;
+}
 int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, LayerScratch* out, bool few_pieces) {
-  const size_t piece = (size_t)M * max_n * 4, most = (size_t)64 << 20;
-  const size_t part_cap = pad256(std::max<size_t>(few_pieces ? std::min(most, 8 * piece) : most, piece * 4));
-  const size_t off_part = ((size_t)M * max_k * 2 + 255) & ~(size_t)255;
-  const size_t off_rest = off_part + part_cap;
-  int32_t rc = grow(p->dev, p->layer_buf, off_rest + rest_bytes);
+  int32_t rc = grow(p->dev, p->layer_buf, layer_scratch_bytes(M, max_k, max_n, rest_bytes, few_pieces));
   if (rc) return rc;
+  out->part_cap = part_bytes(M, max_n, few_pieces);
   char* base = (char*)p->layer_buf.p;
   out->a_bf16 = (uint16_t*)base;
-  out->part = (float*)(base + off_part);
-  out->part_cap = part_cap;
-  out->rest = base + off_rest;
+  out->part = (float*)(base + pad256((size_t)M * max_k * 2));
+  out->rest = (char*)out->part + out->part_cap;
   return RELUX_OK;
 }
 
@@ -849,12 +851,10 @@ int32_t do_mla_layer(Pool* p, const relux_mla_layer_args* a) {
   const bool o_bf16 = mma && mla_writes_bf16(p, sb, aa);   // the output projection's operand, rounded by the kernel that makes it
   rc = fast ? launch_mla_decode_fast(p, sb, aa, d_qc, d_qr, o_bf16 ? (void*)sc.a_bf16 : d_attn, o_bf16, fused_append ? &step : nullptr)
             : launch_attn_reference_mla(p, sb, aa, (const float*)d_qc, (const float*)d_qr, d_attn);
-  if (rc) {
-    if (fused_append) take_rows_back(p, sb, a->layer);   // nobody appended them
-    return rc;
-  }
   // 5. output projection
-  return output_projection(p, o_bf16 ? nullptr : d_attn, M, H * Dh, w.w_o, D, mma, sc.a_bf16, sc.part, sc.part_cap, a->out, a->out_mem);
+  if (!rc) rc = output_projection(p, o_bf16 ? nullptr : d_attn, M, H * Dh, w.w_o, D, mma, sc.a_bf16, sc.part, sc.part_cap, a->out, a->out_mem);
+  if (rc) take_rows_back(p, sb, a->layer);   // a call that fails leaves the lengths as they were
+  return rc;
 }
 
 // ---- the attention half of a block: what relux_gqa_block_cached adds to a layer step ----
@@ -925,6 +925,52 @@ int32_t check_block(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_bloc
   return RELUX_OK;
 }
 
+relux_matmul_lora_args block_adapters(int M, int K, int N, const relux_gqa_block_args* b, const relux_block_projection& q, const void* w, const void* y, bool y_f32, int n_seqs,
+                                      const int32_t* rows_each, float* dst) {
+  relux_matmul_lora_args l;
+  memset(&l, 0, sizeof(l));
+  l.m = M;
+  l.k = K;
+  l.n = N;
+  l.rank = b->rank;
+  l.n_slots = b->n_slots;
+  l.n_seqs = n_seqs;
+  l.x_dtype = y_f32 ? RELUX_DTYPE_F32 : RELUX_DTYPE_BF16;
+  l.out_dtype = RELUX_DTYPE_F32;
+  l.accumulate = q.codes != nullptr;
+  l.x = y;
+  l.w = q.codes ? nullptr : w;
+  l.lora_a = q.lora_a;
+  l.lora_b = q.lora_b;
+  l.factors = q.factors;
+  l.adapter = b->adapter;
+  l.n_rows = rows_each;
+  l.out = dst;
+  return l;
+}
+
+// Room for all that a block's projections ask for, before anything of the call is launched: none of them allocates on its way.  attn_f32: attention's rows come as float32.
+int32_t reserve_projections(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b, int M, const WeightRef* proj, const WeightRef& outp, int n_total, bool attn_f32,
+                            int n_seqs, const int32_t* rows_each) {
+  const int D = a->d_model;
+  const relux_block_projection* q[4] = {&b->q, &b->k, &b->v, &b->o};
+  const WeightRef w[4] = {proj[0], proj[1], proj[2], outp};
+  bool joint = true;
+  for (int j = 0; j < 3; j++) joint = joint && !q[j]->codes && !q[j]->lora_a;
+  size_t most = joint ? layer_scratch_bytes(M, D, n_total, 0) : 0;
+  for (int j = joint ? 3 : 0; j < 4; j++) {
+    if (q[j]->lora_a) {
+      const relux_matmul_lora_args l = block_adapters(M, D, w[j].n, b, *q[j], w[j].w, nullptr, j == 3 && attn_f32, n_seqs, rows_each, nullptr);
+      most = std::max(most, matmul_lora_scratch(p, &l));
+    } else if (!q[j]->codes) {
+      most = std::max(most, layer_scratch_bytes(M, D, w[j].n, 0));
+    }
+  }
+  int32_t rc = grow(p->dev, p->layer_buf, most);
+  if (!rc && a->out_mem != RELUX_MEM_DEVICE) rc = grow(p->dev, p->out_buf, (size_t)M * D * 4);
+  return rc;
+}
+
 // dst [M][N] f32 = rows x one projection of a block: its 8-bit or bf16 weights, and its adapters.  y: the rows as bf16 or (y_f32) float32, codes: in 8 bits, each
 // where it is needed.
 int32_t project_one(Pool* p, int M, int K, int N, const relux_gqa_block_args* b, const relux_block_projection& q, const void* w, const void* y, bool y_f32,
@@ -933,25 +979,7 @@ int32_t project_one(Pool* p, int M, int K, int N, const relux_gqa_block_args* b,
   if (q.codes)
     if ((rc = launch_matmul_int8(p, M, K, N, bs.codes, bs.scales, q.codes, q.scales, dst, false))) return rc;
   if (q.lora_a) {
-    relux_matmul_lora_args l;
-    memset(&l, 0, sizeof(l));
-    l.m = M;
-    l.k = K;
-    l.n = N;
-    l.rank = b->rank;
-    l.n_slots = b->n_slots;
-    l.n_seqs = n_seqs;
-    l.x_dtype = y_f32 ? RELUX_DTYPE_F32 : RELUX_DTYPE_BF16;
-    l.out_dtype = RELUX_DTYPE_F32;
-    l.accumulate = q.codes != nullptr;
-    l.x = y;
-    l.w = q.codes ? nullptr : w;
-    l.lora_a = q.lora_a;
-    l.lora_b = q.lora_b;
-    l.factors = q.factors;
-    l.adapter = b->adapter;
-    l.n_rows = rows_each;
-    l.out = dst;
+    const relux_matmul_lora_args l = block_adapters(M, K, N, b, q, w, y, y_f32, n_seqs, rows_each, dst);
     return do_matmul_lora(p, &l);
   }
   if (q.codes) return RELUX_OK;
@@ -1082,18 +1110,6 @@ static int32_t gqa_layer(Pool* p, const relux_gqa_layer_args* a, const relux_gqa
   float* d_k = (float*)(sc.rest + b_q);
   float* d_v = (float*)(sc.rest + b_q + b_kv);
   float* d_attn = (float*)(sc.rest + b_q + 2 * b_kv);
-  const int rd = a->rope ? hd : 0;
-  ProjSeg segs[3] = {{H * hd, rd, d_q, fast ? 1 : 0, S > 1}, {Hkv * hd, rd, d_k, 0, 0}, {Hkv * hd, 0, d_v, 0, 0}};
-  std::vector<int32_t> rows_each;
-  if (b) {
-    rows_each.assign((size_t)sb.n_seqs, S);
-    rc = block_projections(p, sb, a, b, dx, M, proj, segs, bs, rows_each.data());
-  } else {
-    rc = project_and_finish(p, sb, a->layer, (const float*)dx, M, D, S, proj, segs, 3, mma, sc.a_bf16, sc.part, sc.part_cap, faithful);
-  }
-  if (rc) return rc;
-  // append: the GEMM rows are token-major [row][Hkv][hd]; advance = 0 leaves the rows past the cursor (verify).  A short
-  // step leaves the append to the attention launch.
   relux_attn_args aa;
   memset(&aa, 0, sizeof(aa));
   aa.mode = a->mode;
@@ -1101,6 +1117,20 @@ static int32_t gqa_layer(Pool* p, const relux_gqa_layer_args* a, const relux_gqa
   aa.q_tokens = S;
   aa.extra_tokens = a->advance ? 0 : S;
   const bool fused_append = fast && gqa_append_fusable(p, aa, S, a->advance != 0);
+  const bool o_bf16 = mma && fused_append;   // the output projection's operand, rounded by the kernel that makes it
+  const int rd = a->rope ? hd : 0;
+  ProjSeg segs[3] = {{H * hd, rd, d_q, fast ? 1 : 0, S > 1}, {Hkv * hd, rd, d_k, 0, 0}, {Hkv * hd, 0, d_v, 0, 0}};
+  std::vector<int32_t> rows_each;
+  if (b) {
+    rows_each.assign((size_t)sb.n_seqs, S);
+    rc = reserve_projections(p, a, b, M, proj, outp[0], n_total, !o_bf16, sb.n_seqs, rows_each.data());
+    if (!rc) rc = block_projections(p, sb, a, b, dx, M, proj, segs, bs, rows_each.data());
+  } else {
+    rc = project_and_finish(p, sb, a->layer, (const float*)dx, M, D, S, proj, segs, 3, mma, sc.a_bf16, sc.part, sc.part_cap, faithful);
+  }
+  if (rc) return rc;
+  // append: the GEMM rows are token-major [row][Hkv][hd]; advance = 0 leaves the rows past the cursor (verify).  A short
+  // step leaves the append to the attention launch.
   if (!fused_append) {
     rc = launch_gqa_append(p, sb, a->layer, d_k, d_v, RELUX_DTYPE_F32, RELUX_LAYOUT_TOKEN_MAJOR, a->advance);
     if (rc) return rc;
@@ -1120,16 +1150,14 @@ static int32_t gqa_layer(Pool* p, const relux_gqa_layer_args* a, const relux_gqa
   aa.q_dtype = fast ? RELUX_DTYPE_BF16 : RELUX_DTYPE_F32;
   aa.q_layout = RELUX_LAYOUT_TOKEN_MAJOR;
   const GqaAppend app{d_k, d_v, RELUX_DTYPE_F32, RELUX_LAYOUT_TOKEN_MAJOR, a->advance ? 1 : 0, sb.rows.data()};
-  const bool o_bf16 = mma && fused_append;   // the output projection's operand, rounded by the kernel that makes it
   rc = fused_append ? launch_gqa_stream(p, sb, aa, d_q, o_bf16 ? (void*)sc.a_bf16 : d_attn, o_bf16, &app)
        : fast       ? launch_gqa_decode_fast(p, sb, aa, d_q, d_attn)
                     : launch_attn_reference_gqa(p, sb, aa, (const float*)d_q, d_attn);
-  if (rc) {
-    if (fused_append && a->advance) take_rows_back(p, sb, a->layer);   // nobody appended them
-    return rc;
-  }
-  if (b) return block_output(p, a, b, o_bf16 ? (const void*)sc.a_bf16 : d_attn, o_bf16, M, H * hd, bs, rows_each.data());
-  return output_projection(p, o_bf16 ? nullptr : d_attn, M, H * hd, w.w_o, D, mma, sc.a_bf16, sc.part, sc.part_cap, a->out, a->out_mem);
+  if (!rc)
+    rc = b ? block_output(p, a, b, o_bf16 ? (const void*)sc.a_bf16 : d_attn, o_bf16, M, H * hd, bs, rows_each.data())
+           : output_projection(p, o_bf16 ? nullptr : d_attn, M, H * hd, w.w_o, D, mma, sc.a_bf16, sc.part, sc.part_cap, a->out, a->out_mem);
+  if (rc && a->advance) take_rows_back(p, sb, a->layer);   // a call that fails leaves the lengths as they were
+  return rc;
 }
 int32_t do_gqa_layer(Pool* p, const relux_gqa_layer_args* a) { return gqa_layer(p, a, nullptr); }
 int32_t do_gqa_block(Pool* p, const relux_gqa_layer_args* a, const relux_gqa_block_args* b) {

@@ -584,6 +584,50 @@ bool make_tiles(int M, const std::vector<Request>& requests, LoraTiles* tiles) {
   return true;
 }
 
+// The form of a call, by its sizes (and, for tiles, by how its rows are spread over requests), and what it takes of the layers' scratch.
+enum class Form { kOneLaunch, kFewRows, kTiles, kColumns, kGroups };
+struct LoraPlan {
+  Form form;
+  std::vector<Request> requests;
+  LoraTiles tiles;
+  int t_parts;      // kColumns
+  size_t t_bytes, bytes;
+};
+void plan_lora(const Pool* p, const relux_matmul_lora_args* a, LoraPlan* plan) {
+  const bool x_bf16 = a->x_dtype == RELUX_DTYPE_BF16;
+  const int sms = p->dev->sm_count;
+  plan->requests = merged_requests(a->n_seqs, a->n_rows, a->adapter);
+  plan->t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
+  // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16, with lora_down_kernel in eight parts of K both: one row 11.6 us so and
+  // 13.3 with lora_up_kernel, 16 rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with most of
+  // their rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
+  if (a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256)) {
+    // In one launch, every CTA of which takes t over its part of K: of so few sums, and so few tiles that read the same pieces of an adapter at once (one row, rank 16, x 4096 x 1024
+    // 6.6 us so, 7.9 in two; x 256 x 4096 4.4 and 5.6; x 4096 x 4096 10.3 and 10.5; rank 32 10.9 and 10.75; rank 16 x 4096 x 14336 27.9 and 21.9).
+    const bool one = a->m * a->rank <= kOneT && (a->n - 1) / kRowsOp + 1 <= sms / 4;
+    plan->form = one ? Form::kOneLaunch : Form::kFewRows;
+    plan->bytes = one ? 0 : plan->t_bytes;
+    return;
+  }
+  if (a->w && (int64_t)a->n_slots * std::max(a->n, a->rank) < (int64_t)1 << 31 && make_tiles(a->m, plan->requests, &plan->tiles)) {
+    plan->form = Form::kTiles;
+    plan->bytes = (x_bf16 ? 0 : pad256((size_t)a->m * a->k * 2)) + plan->t_bytes;
+    return;
+  }
+  // Of up to 128 rows t may be further columns of the projection, all rows with every adapter in use (AdapterColumns): their bytes are the adapters', read once, and a launch less.  It
+  // pays where they are few, or large: of small rank a step of adapters is more boxes than a step of W (bf16 rows x 4096 x 4096: 64 rows, 16 slots of rank 16 15.6 us so, 18.1 by
+  // lora_down_kernel; 32 rows, rank 128 29.9 and 36.3; 64 float32 rows, 48 slots of rank 64 29.2 and 31.2; 20, rank 16, 20 slots 15.2 and 15.7; 64 rows x 6144, 48 slots, rank 16 24.6
+  // and 19.5, rank 32 25.3 and 22.7; 40 rows x 1024 x 1024, 8 slots of rank 8 13.4 and 9.7).  Parts of K by the call's sizes alone, so that a row's sums do not depend on the
+  // adapters of the others.
+  const int most = std::min(a->m, a->n_slots);
+  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 320 || (a->rank >= 64 && most * a->rank >= 2048));
+  const int tiles_of_t = (std::min(most, kFewRows) * a->rank + 127) / 128;
+  plan->form = columns ? Form::kColumns : Form::kGroups;
+  plan->t_parts = std::min({8, 2 * sms / tiles_of_t, (a->k + 63) / 64 / 4});
+  plan->t_bytes *= columns ? (size_t)most * plan->t_parts : 1;
+  plan->bytes = layer_scratch_bytes(a->m, a->k, a->w ? a->n : 0, plan->t_bytes, true);
+}
+
 }  // namespace
 
 int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
@@ -616,7 +660,9 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     set_error("matmul_lora: K=%d and N=%d must be multiples of 8, rank=%d one of 8, 16, 32, 64, 128", a->k, a->n, a->rank);
     return RELUX_ERR_UNSUPPORTED;
   }
-  const std::vector<Request> requests = merged_requests(a->n_seqs, a->n_rows, a->adapter);
+  LoraPlan plan;
+  plan_lora(p, a, &plan);
+  const std::vector<Request>& requests = plan.requests;
   const bool x_bf16 = a->x_dtype == RELUX_DTYPE_BF16;
   DownParams down{};
   down.x = a->x;
@@ -624,36 +670,24 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   down.M = a->m;
   down.K = a->k;
   down.rank = a->rank;
-  const size_t t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
-
-  // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16, with lora_down_kernel in eight parts of K both: one row 11.6 us so and
-  // 13.3 with lora_up_kernel, 16 rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with most of
-  // their rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
-  const bool narrow = a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256);
-  LoraTiles tiles;
-  const bool wide = a->w && !narrow && (int64_t)a->n_slots * std::max(a->n, a->rank) < (int64_t)1 << 31 && make_tiles(a->m, requests, &tiles);
-  if (wide) {
-    const size_t x_bytes = x_bf16 ? 0 : ((size_t)a->m * a->k * 2 + 255) & ~(size_t)255;
-    if ((rc = grow(p->dev, p->layer_buf, x_bytes + t_bytes))) return rc;
+  if (plan.form == Form::kTiles) {
+    if ((rc = grow(p->dev, p->layer_buf, plan.bytes))) return rc;
     uint16_t* const rounded = x_bf16 ? nullptr : (uint16_t*)p->layer_buf.p;
-    uint16_t* const t_hi = (uint16_t*)((char*)p->layer_buf.p + x_bytes);
+    uint16_t* const t_hi = (uint16_t*)((char*)p->layer_buf.p + plan.bytes - plan.t_bytes);
     uint16_t* const t_lo = t_hi + (size_t)a->m * a->rank;
     const uint16_t* x = (const uint16_t*)(x_bf16 ? a->x : nullptr);   // nullptr: lora_rows_kernel rounds
     // so few tiles that even in eight parts of K they leave half of the SMs idle: float32 rows are rounded by a launch of their own, but for short K (rank 16, 4096 x 4096: 256
     // rows 28.1 us so and 32.9 without, 1024 rows 45.5 and 46.8, 1536 66.3 and 64.4; 1024 rows of K 8192 48 to 62 and 62, of K 1024 22.6 and 21.3)
-    if (!x_bf16 && tiles.n * 16 <= p->dev->sm_count && a->k >= 2048) {
+    if (!x_bf16 && plan.tiles.n * 16 <= p->dev->sm_count && a->k >= 2048) {
       if ((rc = launch_cast(p, (const float*)a->x, rounded, (size_t)a->m * a->k))) return rc;
       x = rounded;
     }
-    if ((rc = launch_lora_rows(p, a, tiles, x, rounded, t_hi, t_lo))) return rc;
-    return launch_lora_gemm(p, a, x_bf16 ? x : rounded, nullptr, &tiles, nullptr, t_hi, t_lo);
+    if ((rc = launch_lora_rows(p, a, plan.tiles, x, rounded, t_hi, t_lo))) return rc;
+    return launch_lora_gemm(p, a, x_bf16 ? x : rounded, nullptr, &plan.tiles, nullptr, t_hi, t_lo);
   }
-  if (narrow) {
-    // In one launch, every CTA of which takes t over its part of K: of so few sums, and so few tiles that read the same pieces of an adapter at once (one row, rank 16, x 4096 x 1024
-    // 6.6 us so, 7.9 in two; x 256 x 4096 4.4 and 5.6; x 4096 x 4096 10.3 and 10.5; rank 32 10.9 and 10.75; rank 16 x 4096 x 14336 27.9 and 21.9).
-    const bool one = a->m * a->rank <= kOneT && (a->n - 1) / kRowsOp + 1 <= p->dev->sm_count / 4;
-    if (!one) {
-      if ((rc = grow(p->dev, p->layer_buf, t_bytes))) return rc;
+  if (plan.form == Form::kOneLaunch || plan.form == Form::kFewRows) {
+    if (plan.form == Form::kFewRows) {
+      if ((rc = grow(p->dev, p->layer_buf, plan.bytes))) return rc;
       down.t = (float*)p->layer_buf.p;
       if ((rc = run_down(p, x_bf16, down, requests, true))) return rc;
     }
@@ -661,21 +695,11 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, r.slot);
     return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : nullptr, row_slots, nullptr, down.t, nullptr, nullptr);
   }
-
-  // Of up to 128 rows t may be further columns of the projection, all rows with every adapter in use (AdapterColumns): their bytes are the adapters', read once, and a launch less.  It
-  // pays where they are few, or large: of small rank a step of adapters is more boxes than a step of W (bf16 rows x 4096 x 4096: 64 rows, 16 slots of rank 16 15.6 us so, 18.1 by
-  // lora_down_kernel; 32 rows, rank 128 29.9 and 36.3; 64 float32 rows, 48 slots of rank 64 29.2 and 31.2; 20, rank 16, 20 slots 15.2 and 15.7; 64 rows x 6144, 48 slots, rank 16 24.6
-  // and 19.5, rank 32 25.3 and 22.7; 40 rows x 1024 x 1024, 8 slots of rank 8 13.4 and 9.7).  Parts of K by the call's sizes alone, so that a row's sums do not depend on the
-  // adapters of the others.
-  const int most = std::min(a->m, a->n_slots);
-  const bool columns = a->w && a->m <= kFewRows && a->k >= 2048 && (most * a->rank <= 320 || (a->rank >= 64 && most * a->rank >= 2048));
-  const int tiles_of_t = (std::min(most, kFewRows) * a->rank + 127) / 128;
-  const int t_parts = std::min({8, 2 * p->dev->sm_count / tiles_of_t, (a->k + 63) / 64 / 4});
   LayerScratch sc;
-  if ((rc = layer_scratch(p, a->m, a->k, a->w ? a->n : 0, columns ? t_bytes * most * t_parts : t_bytes, &sc, true))) return rc;
+  if ((rc = layer_scratch(p, a->m, a->k, a->w ? a->n : 0, plan.t_bytes, &sc, true))) return rc;
   UpParams up{};
-  if (columns) {
-    AdapterColumns cols{a->lora_a, a->n_slots, a->rank, 0, t_parts, (float*)sc.rest, {}};
+  if (plan.form == Form::kColumns) {
+    AdapterColumns cols{a->lora_a, a->n_slots, a->rank, 0, plan.t_parts, (float*)sc.rest, {}};
     std::vector<int32_t> ids;
     for (const Request& r : requests)
       if (r.slot >= 0) ids.push_back(r.slot);
@@ -686,7 +710,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg, TimeStamp{nullptr, nullptr}, &cols, x_bf16)))
       return rc;
     up.part = sc.part;
-    up.t_parts = t_parts;
+    up.t_parts = plan.t_parts;
     up.t_cols = cols.n_used * a->rank;
     up.t = cols.t;
   } else {
@@ -710,6 +734,12 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   return with_rank(a->rank, [&](auto r) {
     return for_lists(a->m, requests, [&](const auto& list, int groups) { return launch_up<decltype(r)::value>(p, up, list, groups); });
   });
+}
+
+size_t matmul_lora_scratch(const Pool* p, const relux_matmul_lora_args* a) {
+  LoraPlan plan;
+  plan_lora(p, a, &plan);
+  return plan.bytes;
 }
 
 }  // namespace relux

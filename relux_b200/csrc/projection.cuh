@@ -98,6 +98,8 @@ struct LayerScratch {
 // [activations as bf16 (M x max_k) | split partials | caller's buffers (rest_bytes)].  few_pieces: room for eight pieces of the result, or four where that is over 64 MB,
 // and not for 64 MB of them.
 int32_t layer_scratch(Pool* p, int M, int max_k, int max_n, size_t rest_bytes, LayerScratch* out, bool few_pieces = false);
+size_t layer_scratch_bytes(int M, int max_k, int max_n, size_t rest_bytes, bool few_pieces = false);   // what it makes room for
+inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
 // n float32 values, a multiple of 8, rounded to bf16 by the reference's rule.
 int32_t launch_cast(Pool* p, const float* src, uint16_t* dst, size_t n);
 bool gemm_sm100_eligible(int K, const WeightRef* ws, int nw);

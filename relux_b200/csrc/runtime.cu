@@ -1335,7 +1335,11 @@ void relux::take_rows_back(Pool* p, const SeqBatch& sb, int layer) {
   relux_cuda_last_error(why, sizeof(why));
   int32_t* hl = &p->h_len[(size_t)layer * p->prm.max_seqs];
   std::vector<int32_t> len(sb.n_seqs);
-  for (int i = 0; i < sb.n_seqs; i++) len[i] = hl[sb.seq[i]] -= sb.rows[i];
+  for (int i = 0; i < sb.n_seqs; i++) {
+    len[i] = hl[sb.seq[i]] - sb.rows[i];
+    note_set_len(p, layer, sb.seq[i], hl[sb.seq[i]], len[i]);
+    hl[sb.seq[i]] = len[i];
+  }
   (void)launch_set_len(p, sb, layer, 1, len.data());
   set_error("%s", why);
 }

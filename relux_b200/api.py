@@ -607,29 +607,46 @@ class Pool:
         n_slots and adapter [n_seqs].  x and out as for forward_cached (x may be bf16), residual and residual_out on the device."""
         ids = None if seq_ids is None else np.ascontiguousarray(seq_ids, dtype=np.int32)
         slots = None if adapter is None else np.ascontiguousarray(adapter, dtype=np.int32)
-        if slots is not None and slots.shape != (n_seqs,):
-            raise ValueError("block_cached: adapters of shape %s for %d sequences" % (slots.shape, n_seqs))
-        for name, a in (("residual", residual), ("residual_out", residual_out), ("norm_weight", norm_weight)):
-            if a is not None and not isinstance(a, (DeviceBuffer, int)):
-                raise TypeError("block_cached: %s must be device memory" % name)
-        names = ("w_q", "w_k", "w_v", "w_o")
-        for given in (weights, int8 or {}, lora or {}):
+        for what, given in (("adapters", slots), ("seq_ids", ids)):
+            if given is not None and given.shape != (n_seqs,):
+                raise ValueError("block_cached: %s of shape %s for %d sequences" % (what, given.shape, n_seqs))
+        kv = self.prm.gqa_num_kv_heads * self.prm.gqa_head_dim
+        cols = {"w_q": d_model, "w_k": kv, "w_v": kv, "w_o": d_model}
+        int8, lora = int8 or {}, lora or {}
+        for given in (weights, int8, lora):
             for n in given:
-                if n not in names:
+                if n not in cols:
                     raise ValueError("block_cached: no projection %s" % n)
-        w = L.GqaLayerWeights(**{n: _ptr(weights.get(n)) for n in names})
         xt = _dtype_flag(x, x_dtype)
-        args = L.GqaLayerArgs(layer=layer, n_seqs=n_seqs, seq_ids=_ptr(ids), q_tokens=q_tokens, causal=int(causal), d_model=d_model, num_heads=num_heads,
-                              rope=int(rope), rope_base=float(rope_base), advance=int(advance), mode=L.ATTN_FAST, x=_ptr(x), x_dtype=xt, x_mem=_mem(x),
-                              out=_ptr(out), out_mem=_mem(out), w=C.pointer(w))
+        rt, size = _flag_or(residual, residual_dtype, xt), n_seqs * q_tokens * d_model
+        sums = n_slots * rank if rank in (8, 16, 32, 64, 128) else 0   # the library refuses other ranks by itself
+
+        def at(name, a, need):
+            return self._at("block_cached", name, a, need) or None
+
+        def activations(name, a, flag):   # the device's, or a host array
+            if not isinstance(a, np.ndarray):
+                return at(name, a, size * _size(flag))
+            if a.dtype != (np.uint16 if flag == L.DTYPE_BF16 else np.float32):
+                raise TypeError("block_cached: %s of %s" % (name, a.dtype))
+            if a.size != size or not a.flags.c_contiguous:
+                raise ValueError("block_cached: %s of shape %s, %d neighbouring values needed" % (name, a.shape, size))
+            return _ptr(a)
 
         def projection(n):
-            codes, scales = (int8 or {}).get(n, (None, None))
-            a, b, f = (lora or {}).get(n, (None, None, None))
-            return L.BlockProjection(codes=_ptr(codes), scales=_ptr(scales), lora_a=_ptr(a), lora_b=_ptr(b), factors=_ptr(f))
-        block = L.GqaBlockArgs(residual=_ptr(residual), residual_out=_ptr(residual_out), norm_weight=_ptr(norm_weight),
-                               residual_dtype=_flag_or(residual, residual_dtype, xt), norm_dtype=_flag_or(norm_weight, norm_dtype, L.DTYPE_BF16), eps=float(eps), rank=rank,
-                               n_slots=n_slots, adapter=_ptr(slots), **{n[2]: projection(n) for n in names})
+            codes, scales = int8.get(n, (None, None))
+            a, b, f = lora.get(n, (None, None, None))
+            return L.BlockProjection(codes=at("codes of " + n, codes, d_model * cols[n]), scales=at("scales of " + n, scales, 4 * cols[n]),
+                                     lora_a=at("lora_a of " + n, a, 2 * sums * d_model), lora_b=at("lora_b of " + n, b, 2 * sums * cols[n]),
+                                     factors=at("factors of " + n, f, 4 * n_slots))
+        w = L.GqaLayerWeights(**{n: at(n, weights.get(n), 2 * d_model * c) for n, c in cols.items()})
+        args = L.GqaLayerArgs(layer=layer, n_seqs=n_seqs, seq_ids=_ptr(ids), q_tokens=q_tokens, causal=int(causal), d_model=d_model, num_heads=num_heads,
+                              rope=int(rope), rope_base=float(rope_base), advance=int(advance), mode=L.ATTN_FAST, x=activations("x", x, xt), x_dtype=xt, x_mem=_mem(x),
+                              out=activations("out", out, L.DTYPE_F32), out_mem=_mem(out), w=C.pointer(w))
+        nt = _flag_or(norm_weight, norm_dtype, L.DTYPE_BF16)
+        block = L.GqaBlockArgs(residual=at("residual", residual, size * _size(rt)), residual_out=at("residual_out", residual_out, size * _size(rt)),
+                               norm_weight=at("norm_weight", norm_weight, d_model * _size(nt)), residual_dtype=rt, norm_dtype=nt, eps=float(eps), rank=rank,
+                               n_slots=n_slots, adapter=_ptr(slots), **{n[2]: projection(n) for n in cols})
         L.check(self.lib.relux_gqa_block_cached(self.h, C.byref(args), C.byref(block)))
 
     def _mla_forward_cached(self, layer, n_seqs, x, out, weights, d_model, num_heads, q_tokens=1, causal=True, rope_base=0.0,

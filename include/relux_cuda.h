@@ -611,7 +611,8 @@ int32_t relux_pool_kernel_ms_list(relux_pool_t pool, int32_t last_n, float* ms_o
 
 /* Same for the input-projection launch (x . [W_Q | W_QR | W_DKV | W_KR], or x . [W_Q | W_K | W_V]) of the most recent
  * relux_*_forward_cached calls on this pool; its blocks stamp their begin before they wait for the rounded x, when their
- * weights begin to load.  Measurement aid: no counterpart in the reference. */
+ * weights begin to load.  relux_gqa_block_cached counts as such a call; with adapters or 8-bit weights its projections are launches of their own and are not timed (`counted` says how
+ * many of the calls were).  Measurement aid: no counterpart in the reference. */
 int32_t relux_pool_projection_ms_mean(relux_pool_t pool, int32_t last_n, float* mean_ms, int32_t* counted);
 
 /* ---- the matmul of the compute backend ---------------------------------------------------------

@@ -105,13 +105,15 @@ struct PipeCalls {
 };
 
 // Times of the last kCalls calls.  A call is timed by stamps its kernel writes (one launch: time_stamp_next), or by an
-// event pair around several launches (time_events_begin / _end).
+// event pair around several launches (time_events_begin / _end), or not at all (time_none).
 struct TimeRing {
-  static constexpr int kCalls = 8192, kSlots = kCalls + 1;   // a call clears the slot of the one after it
+  static constexpr int kCalls = 8192, kSlots = kCalls + 1;   // a stamped call clears the slot of the next one
+  static constexpr int32_t kEvents = -1, kNone = -2;
   TimeSlot* slots = nullptr;                                 // device [kSlots], zero-filled
   cudaEvent_t ev[kCalls][2] = {};
-  uint8_t stamped[kCalls] = {};
-  uint64_t calls = 0;
+  int32_t slot_of[kCalls] = {};   // of a stamped call, or how else it was timed
+  uint64_t calls = 0, stamped = 0;
+  int32_t next_slot() const { return (int32_t)(stamped % kSlots); }
 };
 
 struct Pool {
@@ -336,6 +338,7 @@ TimeStamp time_stamp_next(Pool* p, TimeRing& r);
 void time_stamp_done(TimeRing& r, const TimeStamp& ts);
 int32_t time_events_begin(Pool* p, TimeRing& r);
 int32_t time_events_end(Pool* p, TimeRing& r);
+inline void time_none(TimeRing& r) { r.slot_of[r.calls++ % TimeRing::kCalls] = TimeRing::kNone; }   // a call whose time is not taken: no older one stands in for it
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and context, not per launch.
 int32_t allow_smem(Device* dev, const void* kernel, size_t bytes);

@@ -1018,6 +1018,7 @@ int32_t block_projections(Pool* p, const SeqBatch& sb, const relux_gqa_layer_arg
     segs[j].src = dst;
     dst += (size_t)M * proj[j].n;
   }
+  time_none(p->proj_times);
   return finish_projections(p, sb, a->layer, M, a->q_tokens, segs, 3, nullptr, GemmRanges{}, false);
 }
 

@@ -84,10 +84,12 @@ TimeStamp time_stamp_next(Pool* p, TimeRing& r) {
     }
     cudaMemsetAsync(r.slots, 0, sizeof(TimeSlot) * TimeRing::kSlots, p->dev->stream);
   }
-  return TimeStamp{r.slots + r.calls % TimeRing::kSlots, r.slots + (r.calls + 1) % TimeRing::kSlots};
+  return TimeStamp{r.slots + r.next_slot(), r.slots + (r.stamped + 1) % TimeRing::kSlots};
 }
 void time_stamp_done(TimeRing& r, const TimeStamp& ts) {
-  if (ts.slot) r.stamped[r.calls++ % TimeRing::kCalls] = 1;
+  if (!ts.slot) return;
+  r.slot_of[r.calls++ % TimeRing::kCalls] = r.next_slot();
+  r.stamped++;
 }
 static int32_t time_event(Pool* p, TimeRing& r, int which) {
   cudaEvent_t& e = r.ev[r.calls % TimeRing::kCalls][which];
@@ -99,9 +101,7 @@ int32_t time_events_begin(Pool* p, TimeRing& r) { return time_event(p, r, 0); }
 int32_t time_events_end(Pool* p, TimeRing& r) {
   int32_t rc = time_event(p, r, 1);
   if (rc) return rc;
-  r.stamped[r.calls++ % TimeRing::kCalls] = 0;
-  if (r.slots)   // the slot of the call after this one
-    RELUX_CUDA_TRY(cudaMemsetAsync(r.slots + r.calls % TimeRing::kSlots, 0, sizeof(TimeSlot), p->dev->stream));
+  r.slot_of[r.calls++ % TimeRing::kCalls] = TimeRing::kEvents;
   return RELUX_OK;
 }
 
@@ -1750,8 +1750,10 @@ static int32_t ring_list(Pool* p, TimeRing& r, int32_t last_n, float* out, int32
   int32_t k = 0;
   for (uint64_t i = n; i-- > 0;) {
     const uint64_t c = r.calls - 1 - i;
-    if (r.stamped[c % TimeRing::kCalls]) {
-      const TimeSlot& t = slots[c % TimeRing::kSlots];
+    const int32_t slot = r.slot_of[c % TimeRing::kCalls];
+    if (slot == TimeRing::kNone) continue;
+    if (slot >= 0) {
+      const TimeSlot& t = slots[slot];
       if (t.begin_inv && t.end) out[k++] = (float)((double)(t.end - ~t.begin_inv) * 1e-6);
       continue;
     }

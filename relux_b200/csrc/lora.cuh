@@ -7,6 +7,7 @@
 namespace relux {
 
 constexpr int kNarrowRows = 16;     // calls of up to so many rows: one block of rows, float32 ones split by lora_gemm_kernel, adapters on the CUDA cores
+constexpr int kNarrowSums = 512;    // rows x rank of them, of float32 ones half as many
 constexpr int kOneT = 16;           // rows x rank of calls in one launch
 constexpr int kMaxLoraTiles = 1024; // row tiles of a longer call
 
@@ -18,18 +19,15 @@ struct LoraTiles {
 };
 
 // f v as two bf16 halves, 16 bits of it.  Both have its sign and neither is zero where it is not: the first is the largest of smaller magnitude, the second the rest.  So an infinity that
-// they are multiplied with comes out as the formula has it (with the nearest value first the rest is zero or of the other sign, and the sum of both products NaN).  An infinity, a NaN, a
-// zero are both halves themselves.  The rest is up to 2^-7 of the value, rounded by 2^-9 of itself.
+// they are multiplied with comes out as the formula has it (with the nearest value first the rest is zero or of the other sign, and the sum of both products NaN).  Of an infinity the
+// first half is the largest number and the rest the infinity; a NaN's rest is NaN.  The rest is up to 2^-7 of the value, rounded by 2^-9 of itself.
 __device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2& lo) {
-  auto first = [](float x) {
-    const uint32_t u = __float_as_uint(x), m = u & 0x7FFFFFFFu;
-    return m - 1u < 0x7F7FFFFFu ? __uint_as_float((u & 0x80000000u) | ((m - 1u) & 0xFFFF0000u)) : x;
-  };
-  auto rest = [](float x, float h) { return h == x || x != x ? x : x - h; };
-  v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-  const float4 h = make_float4(first(v.x), first(v.y), first(v.z), first(v.w));
-  hi = make_uint2(round_bf16x2(h.x, h.y), round_bf16x2(h.z, h.w));
-  lo = make_uint2(round_bf16x2(rest(v.x, h.x), rest(v.y, h.y)), round_bf16x2(rest(v.z, h.z), rest(v.w, h.w)));
+  auto times = [f](float x) { return __fadd_rn(__fmul_rn(x, f), 0.f); };   // never -0, of which there is no smaller magnitude
+  auto first = [](float x) { return (max(__float_as_uint(x), 1u) - 1u) & 0xFFFF0000u; };
+  v = make_float4(times(v.x), times(v.y), times(v.z), times(v.w));
+  const uint32_t x = first(v.x), y = first(v.y), z = first(v.z), w = first(v.w);
+  hi = make_uint2(__byte_perm(x, y, 0x7632), __byte_perm(z, w, 0x7632));
+  lo = make_uint2(round_bf16x2(v.x - __uint_as_float(x), v.y - __uint_as_float(y)), round_bf16x2(v.z - __uint_as_float(z), v.w - __uint_as_float(w)));
 }
 
 // out = x W (+ out) + t B_s^T.  x: bf16 [M][K], the caller's or what the launch before this one has rounded; nullptr: up to kNarrowRows float32 rows of the

@@ -116,3 +116,21 @@ def test_rows_of_an_infinity(dev, pool, rows, adapter, K, rank, x_bf16):  # noqa
     assert (got[row] == out[row]).all()
     assert (np.abs(got - out)[other] <= bound[other]).all()
     c.free()
+
+
+@pytest.mark.parametrize("rows,adapter,K,rank", FORMS)
+def test_products_that_vanish(dev, pool, rows, adapter, K, rank):  # noqa: F811
+    """Values and factors whose product is below the smallest float32, of both signs, and zeros of both signs: the adapter's part is nothing, and not NaN."""
+    rng = np.random.default_rng(sum(rows) + K + rank + 3)
+    c = Case(dev, rng, rows, adapter, K, N, rank, 3, False)
+    c.factors[:] = 1e-20, -1e-20, 1e-20
+    c.df.upload(c.factors)
+    c.x *= np.float32(1e-28)
+    c.x[:, ::5], c.x[:, 1::5] = 0.0, -0.0
+    c.dx.upload(c.x)
+    c.call(pool)
+    got = c.get()
+    out, _ = c.plain()
+    size = np.abs(c.x).astype(np.float64) @ np.abs(c.w).astype(np.float64)
+    assert np.isfinite(got).all() and (np.abs(got - out) <= size * 2.0 ** -8).all()
+    c.free()

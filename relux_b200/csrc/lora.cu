@@ -25,6 +25,7 @@ namespace {
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
 constexpr int kUpCols = 32 * kLoraWarps;   // columns of a block of lora_up_kernel, 32 a warp
 constexpr int kGroupRows = 16;
+constexpr int kMostParts = 4;              // of K, of lora_down_kernel
 constexpr int kMost = 1 << 30;                       // rows, k, n: counted in 32 bits, a tile past the last
 constexpr int kMostGridY = 65535;
 constexpr int kFewRows = 128, kSomeRows = 512;       // of up to so many rows a list names each
@@ -99,7 +100,7 @@ struct DownParams {
 
 // t[row][r] = sum over k of x[row][k] A_s[r][k].  grid (groups, parts of K, kSlice-th parts of the rank), the parts of K a cluster, 8 warps that take 32 k each in turn.  mma.sync: a group is a
 // handful of rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
-enum Rows { kBf16, kRounded, kSplit };   // x: bf16; float32, rounded, for the projection too where it asks; float32, in two halves
+enum Rows { kBf16, kRounded, kSplit };   // x: bf16; float32, rounded, for the projection too; float32, in two halves
 template <int kSlice, Rows kX, class List>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
   constexpr int kTiles = kSlice / 8;
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
   const int r0 = blockIdx.z * kSlice;
   const uint16_t* const a = p.a + ((size_t)max(slot, 0) * p.rank + r0) * p.K;
-  const bool rounds = kX == kRounded && p.x_bf16 && r0 == 0;
+  const bool rounds = kX == kRounded && r0 == 0;
   if (slot >= 0)   // the adapter's first pieces to L2, while the launch before this one ends (a prefetch returns no data, so it may be early)
     for (int s = s0 + warp; s < min(s1, s0 + 4 * kLoraWarps); s += kLoraWarps) {
       const int k = s * 32 + 8 * t;
@@ -465,9 +466,8 @@ int make_list(std::vector<Request> r, RunList<kCap>* list) {
 template <int kSlice, class List>
 int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int parts, bool x_bf16) {
   const size_t smem = (size_t)(kLoraWarps + parts - 1) * kGroupRows * kSlice * sizeof(float);
+  static_assert((kLoraWarps + kMostParts - 1) * kGroupRows * kSlice * sizeof(float) <= 48 << 10, "more shared memory than a launch has without asking");
   auto go = [&](auto kernel) -> int32_t {
-    if (smem > 48 << 10)
-      if (int32_t rc = allow_smem(p->dev, kernel, smem)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)groups, (unsigned)parts, (unsigned)(prm.rank / kSlice));
     cfg.blockDim = dim3(kLoraThreads);
@@ -498,13 +498,10 @@ int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups) {
       return RELUX_OK;
     };
     int32_t rc;
-    if (prm.part && prm.rg.in_turns()) {
-      rc = go(lora_up_kernel<kRank, kInTurns, List>);
-    } else if constexpr (std::is_same_v<List, RowList<kFewRows>>) {
+    if constexpr (std::is_same_v<List, RowList<kFewRows>>)   // one block of rows
       rc = prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
-    } else {
-      rc = go(lora_up_kernel<kRank, kPlain, List>);
-    }
+    else
+      rc = prm.part && prm.rg.in_turns() ? go(lora_up_kernel<kRank, kInTurns, List>) : go(lora_up_kernel<kRank, kPlain, List>);
     if (rc) return rc;
     count_launch(p->dev);
   }
@@ -554,7 +551,7 @@ int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<
     // parts of K: two blocks an SM where groups are full, of 1024 k at least, four at most and beside another launch two: larger clusters start late (64 bf16 rows x 4096 x 6144, rank
     // 16: 23.3 us in one part, 19.5 in four, 20.7 in eight; 300 rows x 4096: 29.5 in four, 35.0 in eight; beside lora_gemm_kernel, 12 rows x 4096: 12.0 in two, 13.2 in four, 13.8 in eight).
     // By the call's sizes alone: a row's sums do not depend on the adapters of the others.
-    const int parts = std::max(1, std::min({beside ? 2 : 4, 2 * p->dev->sm_count / ((prm.M + kGroupRows - 1) / kGroupRows), prm.K / 1024}));
+    const int parts = std::max(1, std::min({beside ? 2 : kMostParts, 2 * p->dev->sm_count / ((prm.M + kGroupRows - 1) / kGroupRows), prm.K / 1024}));
     // slices of the rank: of few rows 16, so that more SMs read an adapter (one row of rank 128 x 4096 x 4096: 23 us with the whole rank a block); of many 64, since
     // every slice reads x again
     if (prm.rank == 8) return launch_down<8>(p, prm, list, groups, parts, x_bf16);
@@ -601,7 +598,7 @@ void plan_lora(const Pool* p, const relux_matmul_lora_args* a, LoraPlan* plan) {
   // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16, with lora_down_kernel in eight parts of K both: one row 11.6 us so and
   // 13.3 with lora_up_kernel, 16 rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with most of
   // their rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
-  if (a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? 512 : 256)) {
+  if (a->w && a->m <= (x_bf16 ? kNarrowRows : 8) && a->m * a->rank <= (x_bf16 ? kNarrowSums : kNarrowSums / 2)) {
     // In one launch, every CTA of which takes t over its part of K: of so few sums, and so few tiles that read the same pieces of an adapter at once (one row, rank 16, x 4096 x 1024
     // 6.6 us so, 7.9 in two; x 256 x 4096 4.4 and 5.6; x 4096 x 4096 10.3 and 10.5; rank 32 10.9 and 10.75; rank 16 x 4096 x 14336 27.9 and 21.9).
     const bool one = a->m * a->rank <= kOneT && (a->n - 1) / kRowsOp + 1 <= sms / 4;

@@ -32,7 +32,7 @@ struct NormParams {
   int8_t* codes;
   float* scales;
   int32_t n_rows, d;
-  int32_t weight_bf16, out_bf16, by_tma;   // by_tma: the next launch reads codes or out by TMA
+  int32_t weight_bf16, out_bf16;
   float eps, inv_d;
 };
 
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTeam == kLanes ? 256 : kMaxRowThreads) norm_r
       }
     }
   }
-  if (p.by_tma) fence_chained_writes();
+  fence_chained_writes();   // codes, and bf16 rows, are a projection's operands
 }
 
 template <bool kXBf16, bool kRBf16, int kNV, Team kTeam, bool kNorm>
@@ -286,11 +286,9 @@ int32_t launch_typed(Pool* p, const NormParams& prm) {
     while (nv < 4 && each > 256 * nv) nv *= 2;
   const int threads = ((each + nv - 1) / nv + 31) / 32 * 32;
   const dim3 grid((unsigned)prm.n_rows * (unsigned)parts), block((unsigned)threads);
-  if (parts > 1) {
-    return nv == 1 ? launch_one<kXBf16, kRBf16, 1, kCluster, kNorm>(p, prm, grid, block, parts)
-         : nv == 2 ? launch_one<kXBf16, kRBf16, 2, kCluster, kNorm>(p, prm, grid, block, parts)
-                   : launch_one<kXBf16, kRBf16, 4, kCluster, kNorm>(p, prm, grid, block, parts);
-  }
+  static_assert(kMaxNormDim / 8 / 2 <= 2 * kMaxRowThreads, "half of a row takes more than two chunks a thread");
+  if (parts > 1)
+    return nv == 1 ? launch_one<kXBf16, kRBf16, 1, kCluster, kNorm>(p, prm, grid, block, parts) : launch_one<kXBf16, kRBf16, 2, kCluster, kNorm>(p, prm, grid, block, parts);
   return nv == 1 ? launch_one<kXBf16, kRBf16, 1, kBlock, kNorm>(p, prm, grid, block)
        : nv == 2 ? launch_one<kXBf16, kRBf16, 2, kBlock, kNorm>(p, prm, grid, block)
                  : launch_one<kXBf16, kRBf16, 4, kBlock, kNorm>(p, prm, grid, block);
@@ -395,7 +393,6 @@ int32_t do_rmsnorm(Pool* p, const relux_rmsnorm_args* a) {
   prm.d = a->d;
   prm.weight_bf16 = a->weight_dtype == RELUX_DTYPE_BF16;
   prm.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
-  prm.by_tma = 1;   // codes, and bf16 rows, are a projection's operands
   prm.eps = a->eps;
   prm.inv_d = 1.f / (float)a->d;
   return launch_rows<true>(p, prm, a->x_dtype == RELUX_DTYPE_BF16, a->residual_dtype == RELUX_DTYPE_BF16);
@@ -415,7 +412,6 @@ int32_t do_int8_rows(Pool* p, const relux_int8_rows_args* a) {
   prm.scales = a->scales;
   prm.n_rows = a->n_rows;
   prm.d = a->d;
-  prm.by_tma = 1;
   const bool bf16 = a->x_dtype == RELUX_DTYPE_BF16;
   return launch_rows<false>(p, prm, bf16, bf16);
 }

@@ -25,8 +25,8 @@ constexpr int kGroup = 16;                  // row blocks that share the columns
 constexpr int kOutRow = 128;                // bytes of a row of the epilogue's staging tiles
 
 // NC: rows of the N operand; wide tiles have 256.  kMore: bytes that the epilogue needs beside.  kSliceRows: columns of slices that there is room for.
-// kHalves: N operands of a step, where rows are two halves.
-template <int NC, int kMoreBytes, int kSliceRows = NC < 32 ? 32 : NC, int kHalves = 1>
+// kHalves: N operands of a step, where rows are two halves.  kMost: stages.
+template <int NC, int kMoreBytes, int kSliceRows = NC < 32 ? 32 : NC, int kHalves = 1, int kMost = 12>
 struct TileShape {
   static constexpr bool kWide = NC == 256;
   static constexpr int kMaxCluster = kWide ? 4 : 8;
@@ -36,7 +36,7 @@ struct TileShape {
   static constexpr int kOut = kWide ? 4 * 2 * 32 * kOutRow : 0;                              // two staging tiles of 32 rows a warp
   static constexpr int kSlices = kWide ? 0 : kSliceRows * kRowsOp * 4;                      // the slices from the cluster (wide: in the stages, which are free then)
   static constexpr int kRoom = 232448 - kBars - kMore - kOut - kSlices;
-  static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
+  static constexpr int kStages = kRoom / kStage < kMost ? kRoom / kStage : kMost;
   static constexpr int kSmem = kStages * kStage + kOut + kSlices + kMore + kBars;
   static constexpr int kAcc = NC < 32 ? 32 : NC;
 };

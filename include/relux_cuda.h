@@ -702,7 +702,7 @@ int32_t relux_matmul_int8(relux_pool_t pool, const relux_matmul_int8_args* args)
 /* C [m][n] = x [m][k] w + the low-rank adapter of each row's request: f_s (x A_s^T) B_s^T, s the request's slot.  relux_matmul_f32_bf16 for a batch
  * whose requests have adapters of their own, in as many launches; rows of requests without one (-1) are the shared projection alone.
  * bf16 x is taken as it is.  float32 x is rounded to bf16, as in relux_matmul_f32_bf16's FAST mode; it keeps 16 bits where w is NULL, or m is up to 8 and m * rank up
- * to 256.  x A_s^T is summed in float32 and keeps 16 bits.  Sums are float32 up to the one rounding of the result.  A request's rows depend on its own adapter alone, whatever
+ * to 256, and with x_halves (for twice the operations of the projection) in every call, so that a row's bits do not depend on how many there are.  x A_s^T is summed in float32 and keeps 16 bits.  Sums are float32 up to the one rounding of the result.  A request's rows depend on its own adapter alone, whatever
  * other slots hold (the order of the sums may go by how the batch's rows are spread over requests).  Infinities and NaN, in x, w, or an adapter, come out where the formula has them and
  * with its sign.
  * w NULL: no shared projection (it came from relux_matmul_int8, say: with accumulate the adapters are added to what out holds).
@@ -715,7 +715,8 @@ typedef struct relux_matmul_lora_args {
   int32_t rank, n_slots, n_seqs;
   int32_t x_dtype, out_dtype;
   int32_t accumulate;
-  int32_t reserved[3];
+  int32_t x_halves;          /* 1: float32 x keeps 16 bits whatever m is (up to 2^29 rows); of bf16 x no matter */
+  int32_t reserved[2];
   const void* x;             /* device [m][k] */
   const void* w;             /* device bf16 [k][n], or NULL */
   const void* lora_a;        /* device bf16 [n_slots][rank][k] */

@@ -347,10 +347,10 @@ class Pool:
             L.check(rc)
 
     def matmul_lora(self, m, k, n, x, w, out, lora_a, lora_b, rank, n_slots, adapter, rows=None, factors=None, accumulate=False, x_dtype=None,
-                    out_dtype=None):
+                    out_dtype=None, x_halves=False):
         """out [m, n] = x [m, k] w + each request's low-rank adapter (relux_matmul_lora): adapter [requests], slots or -1; rows [requests], None: one
         each; lora_a [n_slots, rank, k], lora_b [n_slots, n, rank], factors float32 [n_slots] or None.  w None: no shared projection; accumulate: added to
-        what out holds."""
+        what out holds; x_halves: float32 x keeps 16 bits in calls of every size."""
         ids = np.ascontiguousarray(adapter, dtype=np.int32)
         nr = None if rows is None else np.ascontiguousarray(rows, dtype=np.int32)
         if ids.ndim != 1 or (nr is not None and nr.shape != ids.shape):
@@ -359,7 +359,7 @@ class Pool:
         ot = out_dtype if out_dtype is not None else _dtype_flag(out)
         at = self._at
         rc = L.packed["matmul_lora"](self.h, L.pack_matmul_lora(
-            m, k, n, rank, n_slots, ids.size, xt, ot, 1 if accumulate else 0, x if x.__class__ is int else at("matmul_lora", "x", x, m * k * _size(xt)),
+            m, k, n, rank, n_slots, ids.size, xt, ot, 1 if accumulate else 0, 1 if x_halves else 0, x if x.__class__ is int else at("matmul_lora", "x", x, m * k * _size(xt)),
             0 if w is None else w if w.__class__ is int else at("matmul_lora", "w", w, 2 * k * n),
             lora_a if lora_a.__class__ is int else at("matmul_lora", "lora_a", lora_a, 2 * n_slots * rank * k),
             lora_b if lora_b.__class__ is int else at("matmul_lora", "lora_b", lora_b, 2 * n_slots * rank * n),

@@ -92,7 +92,7 @@ __device__ __forceinline__ int group_rows(const RunList<kCap>& list, int group, 
 
 struct DownParams {
   const void* x;
-  uint16_t* x_bf16;       // float32 x: the projection's operand, or nullptr: x in two halves
+  uint16_t* x_bf16;       // float32 x: the projection's operand [M][K], in halves [2][M][K]; or nullptr: there is no projection
   const uint16_t* a;      // [slots][rank][K]
   float* t;               // [M][rank], without factors
   int32_t M, K, rank;
@@ -100,7 +100,7 @@ struct DownParams {
 
 // t[row][r] = sum over k of x[row][k] A_s[r][k].  grid (groups, parts of K, kSlice-th parts of the rank), the parts of K a cluster, 8 warps that take 32 k each in turn.  mma.sync: a group is a
 // handful of rows, and the bound is reading A_s and x.  A thread's eight neighbouring k of a row are the pairs of two k-slices, in the same order for x and A_s.
-enum Rows { kBf16, kRounded, kSplit };   // x: bf16; float32, rounded, for the projection too; float32, in two halves
+enum Rows { kBf16, kRounded, kSplit };   // x: bf16; float32, rounded; float32, in two halves; each for the projection too where there is one
 template <int kSlice, Rows kX, class List>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownParams p, const __grid_constant__ List list) {
   constexpr int kTiles = kSlice / 8;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   const int steps = (p.K + 31) / 32, s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
   const int r0 = blockIdx.z * kSlice;
   const uint16_t* const a = p.a + ((size_t)max(slot, 0) * p.rank + r0) * p.K;
-  const bool rounds = kX == kRounded && r0 == 0;
+  const bool rounds = kX != kBf16 && p.x_bf16 && r0 == 0;
   if (slot >= 0)   // the adapter's first pieces to L2, while the launch before this one ends (a prefetch returns no data, so it may be early)
     for (int s = s0 + warp; s < min(s1, s0 + 4 * kLoraWarps); s += kLoraWarps) {
       const int k = s * 32 + 8 * t;
@@ -160,7 +160,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
           x[h] = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
           low[h] = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
         }
-        if (there && rounds) *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[h];
+        if (there && rounds) {
+          *reinterpret_cast<uint4*>(p.x_bf16 + at) = x[h];
+          if constexpr (kX == kSplit) *reinterpret_cast<uint4*>(p.x_bf16 + (size_t)p.M * p.K + at) = low[h];
+        }
       }
     }
     if (slot >= 0) {
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
       if constexpr (kX == kSplit) multiply(low);
     }
   }
-  if constexpr (kX == kRounded) fence_chained_writes();
+  if constexpr (kX != kBf16) fence_chained_writes();
   if (slot < 0) return;
   // the warps' sums, then the parts', in their order
   const int parts = gridDim.y, part = blockIdx.y;
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   }
 }
 
-enum Up { kPlain, kInTurns, kTInPieces };   // the GEMM's blocks of rows come in turns; t comes in pieces, from the GEMM
+enum Up { kPlain, kInTurns, kTInPieces, kHalves };   // the GEMM's blocks of rows come in turns; t comes in pieces, from the GEMM; every row is two of the GEMM's, M apart (in turns or not)
 struct UpParams {
   const float* part;      // the GEMM's pieces [piece][M][N]; nullptr: no shared projection
   int32_t first_block;    // of 256 columns, of this launch
@@ -259,7 +262,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
   constexpr int kStride = kRank + 8, kSlices = (kRank + 31) / 32;   // k slices of 32 (one, of 8 or 16, for small ranks)
   __shared__ __align__(16) uint16_t t_hi[kGroupRows * kStride], t_lo[kGroupRows * kStride];
   __shared__ int32_t rows[kGroupRows];
-  constexpr bool kTurns = kUp == kInTurns, kFew = kUp == kTInPieces;
+  constexpr bool kTurns = kUp == kInTurns || kUp == kHalves, kFew = kUp == kTInPieces;
+  constexpr int kOf = kUp == kHalves ? 2 : 1;   // the GEMM's rows of a row
   chain_release();
   const int slot = group_rows(list, blockIdx.x, rows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -321,9 +325,12 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
     const int row = rows[8 * h + g];
     if (row < 0 || n >= p.N) continue;
     const size_t at = (size_t)row * p.N + n;
-    const int pieces = !p.part ? 1 : kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row)) : same;
+#pragma unroll
+    for (int o = 0; o < kOf; o++) {
+      const int pieces = !p.part ? 1 : kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row + o * p.M)) : same;
 #pragma unroll 2
-    for (int s = 1; s < pieces; s++) add_f32(h, p.part + (size_t)s * p.M * p.N + at);
+      for (int s = o ? 0 : 1; s < pieces; s++) add_f32(h, p.part + ((size_t)s * kOf + o) * p.M * p.N + at);
+    }
     if (p.adds) {
       if (p.out_bf16) {
         const uint4 a = load_chained(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.out) + at));
@@ -464,7 +471,7 @@ int make_list(std::vector<Request> r, RunList<kCap>* list) {
 }
 
 template <int kSlice, class List>
-int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int parts, bool x_bf16) {
+int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups, int parts, Rows kind) {
   const size_t smem = (size_t)(kLoraWarps + parts - 1) * kGroupRows * kSlice * sizeof(float);
   static_assert((kLoraWarps + kMostParts - 1) * kGroupRows * kSlice * sizeof(float) <= 48 << 10, "more shared memory than a launch has without asking");
   auto go = [&](auto kernel) -> int32_t {
@@ -485,10 +492,10 @@ int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups
     count_launch(p->dev);
     return RELUX_OK;
   };
-  return x_bf16 ? go(lora_down_kernel<kSlice, kBf16, List>) : prm.x_bf16 ? go(lora_down_kernel<kSlice, kRounded, List>) : go(lora_down_kernel<kSlice, kSplit, List>);
+  return kind == kBf16 ? go(lora_down_kernel<kSlice, kBf16, List>) : kind == kRounded ? go(lora_down_kernel<kSlice, kRounded, List>) : go(lora_down_kernel<kSlice, kSplit, List>);
 }
 template <int kRank, class List>
-int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups) {
+int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups, bool halves) {
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
   const int blocks = (prm.N + kUpCols - 1) / kUpCols;
   for (prm.first_block = 0; prm.first_block < blocks; prm.first_block += kMostGridY) {
@@ -499,9 +506,10 @@ int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups) {
     };
     int32_t rc;
     if constexpr (std::is_same_v<List, RowList<kFewRows>>)   // one block of rows
-      rc = prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
+      rc = halves ? go(lora_up_kernel<kRank, kHalves, List>) : prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
     else
-      rc = prm.part && prm.rg.in_turns() ? go(lora_up_kernel<kRank, kInTurns, List>) : go(lora_up_kernel<kRank, kPlain, List>);
+      rc = halves ? go(lora_up_kernel<kRank, kHalves, List>)
+                  : prm.part && prm.rg.in_turns() ? go(lora_up_kernel<kRank, kInTurns, List>) : go(lora_up_kernel<kRank, kPlain, List>);
     if (rc) return rc;
     count_launch(p->dev);
   }
@@ -545,7 +553,7 @@ int32_t with_rank(int rank, F f) {
   }
 }
 // beside: the launch behind it streams W meanwhile.
-int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<Request>& requests, bool beside) {
+int32_t run_down(Pool* p, Rows kind, const DownParams& prm, const std::vector<Request>& requests, bool beside) {
   return for_lists(prm.M, requests, [&](const auto& list, int groups) {
     using List = std::decay_t<decltype(list)>;
     // parts of K: two blocks an SM where groups are full, of 1024 k at least, four at most and beside another launch two: larger clusters start late (64 bf16 rows x 4096 x 6144, rank
@@ -554,13 +562,13 @@ int32_t run_down(Pool* p, bool x_bf16, const DownParams& prm, const std::vector<
     const int parts = std::max(1, std::min({beside ? 2 : kMostParts, 2 * p->dev->sm_count / ((prm.M + kGroupRows - 1) / kGroupRows), prm.K / 1024}));
     // slices of the rank: of few rows 16, so that more SMs read an adapter (one row of rank 128 x 4096 x 4096: 23 us with the whole rank a block); of many 64, since
     // every slice reads x again
-    if (prm.rank == 8) return launch_down<8>(p, prm, list, groups, parts, x_bf16);
+    if (prm.rank == 8) return launch_down<8>(p, prm, list, groups, parts, kind);
     if constexpr (List::kNamesRows) {
-      return launch_down<16>(p, prm, list, groups, parts, x_bf16);
+      return launch_down<16>(p, prm, list, groups, parts, kind);
     } else {
-      if (prm.rank == 16) return launch_down<16>(p, prm, list, groups, parts, x_bf16);
-      if (prm.rank == 32) return launch_down<32>(p, prm, list, groups, parts, x_bf16);
-      return launch_down<64>(p, prm, list, groups, parts, x_bf16);
+      if (prm.rank == 16) return launch_down<16>(p, prm, list, groups, parts, kind);
+      if (prm.rank == 32) return launch_down<32>(p, prm, list, groups, parts, kind);
+      return launch_down<64>(p, prm, list, groups, parts, kind);
     }
   });
 }
@@ -585,6 +593,7 @@ bool make_tiles(int M, const std::vector<Request>& requests, LoraTiles* tiles) {
 enum class Form { kOneLaunch, kFewRows, kTiles, kColumns, kGroups };
 struct LoraPlan {
   Form form;
+  bool halves;      // kGroups: the projection is of rows in two halves, one behind the others
   std::vector<Request> requests;
   LoraTiles tiles;
   int t_parts;      // kColumns
@@ -595,6 +604,7 @@ void plan_lora(const Pool* p, const relux_matmul_lora_args* a, LoraPlan* plan) {
   const int sms = p->dev->sm_count;
   plan->requests = merged_requests(a->n_seqs, a->n_rows, a->adapter);
   plan->t_bytes = (size_t)a->m * a->rank * sizeof(float);   // or two halves of two bytes
+  plan->halves = false;
   // few rows of small rank: what the epilogue's warps can do while W streams (bf16 rows x 4096 x 4096, rank 16, with lora_down_kernel in eight parts of K both: one row 11.6 us so and
   // 13.3 with lora_up_kernel, 16 rows 13.1 and 15.5; rank 64, 16 rows: 22.4 and 19.5).  float32 rows are split there, by every CTA for itself: one row 13.2 and 13.2, with most of
   // their rounding less; 16 rows x 4096 x 14336 31.4 and 26.0.
@@ -604,6 +614,14 @@ void plan_lora(const Pool* p, const relux_matmul_lora_args* a, LoraPlan* plan) {
     const bool one = a->m * a->rank <= kOneT && (a->n - 1) / kRowsOp + 1 <= sms / 4;
     plan->form = one ? Form::kOneLaunch : Form::kFewRows;
     plan->bytes = one ? 0 : plan->t_bytes;
+    return;
+  }
+  // float32 rows in two halves, as twice as many rows of the projection: what it is for is the bits (bf16 results, against 64 bits: 1.65e-3 off, rounded rows 2.4e-3).  No form of its own:
+  // rank 16, 9 rows x 4096 x 4096 22.3 us (rounded 17.7), 64 x 4096 x 6144 31.5 (25.9), 700 x 4096 x 4096 62 (43); 8192 rows, rank 8, 560 (239).
+  if (a->w && !x_bf16 && a->x_halves) {
+    plan->form = Form::kGroups;
+    plan->halves = true;
+    plan->bytes = layer_scratch_bytes(2 * a->m, a->k, a->n, plan->t_bytes, true);
     return;
   }
   if (a->w && (int64_t)a->n_slots * std::max(a->n, a->rank) < (int64_t)1 << 31 && make_tiles(a->m, plan->requests, &plan->tiles)) {
@@ -635,8 +653,9 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   }
   auto dtype_ok = [](int32_t t) { return t == RELUX_DTYPE_F32 || t == RELUX_DTYPE_BF16; };
   if (!dtype_ok(a->x_dtype) || !dtype_ok(a->out_dtype)) { set_error("bad dtype flag"); return RELUX_ERR_INVALID_ARG; }
-  for (int i = 0; i < 3; i++)
+  for (int i = 0; i < 2; i++)
     if (a->reserved[i]) { set_error("reserved fields must be zero"); return RELUX_ERR_INVALID_ARG; }
+  if (a->x_halves != 0 && a->x_halves != 1) { set_error("matmul_lora: x_halves=%d must be 0 or 1", a->x_halves); return RELUX_ERR_INVALID_ARG; }
   int64_t rows = 0;
   for (int i = 0; i < a->n_seqs; i++) {
     const int n = a->n_rows ? a->n_rows[i] : 1;
@@ -648,6 +667,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     rows += n;
   }
   if (a->m > kMost || a->k > kMost || a->n > kMost) { set_error("matmul_lora: M=%d K=%d N=%d, up to %d each", a->m, a->k, a->n, kMost); return RELUX_ERR_UNSUPPORTED; }
+  if (a->x_halves && a->x_dtype == RELUX_DTYPE_F32 && a->m > kMost / 2) { set_error("matmul_lora: M=%d above %d with x_halves", a->m, kMost / 2); return RELUX_ERR_UNSUPPORTED; }
   if (rows != a->m) { set_error("matmul_lora: the requests have %lld rows, M=%d", (long long)rows, a->m); return RELUX_ERR_INVALID_ARG; }
   int32_t rc;
   if ((rc = check_dev_align(a->x, "x")) || (rc = check_dev_align(a->w, "w")) || (rc = check_dev_align(a->lora_a, "lora_a")) || (rc = check_dev_align(a->lora_b, "lora_b")) ||
@@ -686,14 +706,15 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
     if (plan.form == Form::kFewRows) {
       if ((rc = grow(p->dev, p->layer_buf, plan.bytes))) return rc;
       down.t = (float*)p->layer_buf.p;
-      if ((rc = run_down(p, x_bf16, down, requests, true))) return rc;
+      if ((rc = run_down(p, x_bf16 ? kBf16 : kSplit, down, requests, true))) return rc;
     }
     int32_t row_slots[kNarrowRows];
     for (const Request& r : requests) std::fill(row_slots + r.row, row_slots + r.row + r.n, r.slot);
     return launch_lora_gemm(p, a, x_bf16 ? (const uint16_t*)a->x : nullptr, row_slots, nullptr, down.t, nullptr, nullptr);
   }
   LayerScratch sc;
-  if ((rc = layer_scratch(p, a->m, a->k, a->w ? a->n : 0, plan.t_bytes, &sc, true))) return rc;
+  const int gemm_rows = plan.halves ? 2 * a->m : a->m;
+  if ((rc = layer_scratch(p, gemm_rows, a->k, a->w ? a->n : 0, plan.t_bytes, &sc, true))) return rc;
   UpParams up{};
   if (plan.form == Form::kColumns) {
     AdapterColumns cols{a->lora_a, a->n_slots, a->rank, 0, plan.t_parts, (float*)sc.rest, {}};
@@ -713,10 +734,10 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   } else {
     if (a->w && !x_bf16) down.x_bf16 = sc.a_bf16;
     down.t = (float*)sc.rest;
-    if ((rc = run_down(p, x_bf16, down, requests, false))) return rc;
+    if ((rc = run_down(p, x_bf16 ? kBf16 : a->w && !plan.halves ? kRounded : kSplit, down, requests, false))) return rc;
     if (a->w) {
       const WeightRef w{a->w, a->n};
-      if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, a->m, a->k, &w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
+      if ((rc = launch_skinny_gemm(p, x_bf16 ? (const uint16_t*)a->x : sc.a_bf16, gemm_rows, a->k, &w, 1, sc.part, sc.part_cap, &up.rg))) return rc;
       up.part = sc.part;
     }
     up.t = down.t;
@@ -729,7 +750,7 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   up.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
   up.adds = a->accumulate != 0;
   return with_rank(a->rank, [&](auto r) {
-    return for_lists(a->m, requests, [&](const auto& list, int groups) { return launch_up<decltype(r)::value>(p, up, list, groups); });
+    return for_lists(a->m, requests, [&](const auto& list, int groups) { return launch_up<decltype(r)::value>(p, up, list, groups, plan.halves); });
   });
 }
 

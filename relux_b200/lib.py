@@ -119,7 +119,7 @@ class MatmulInt8Args(C.Structure):
 
 class MatmulLoraArgs(C.Structure):
     _fields_ = [("m", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("rank", C.c_int32), ("n_slots", C.c_int32), ("n_seqs", C.c_int32),
-                ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("accumulate", C.c_int32), ("reserved", C.c_int32 * 3), ("x", C.c_void_p),
+                ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("accumulate", C.c_int32), ("x_halves", C.c_int32), ("reserved", C.c_int32 * 2), ("x", C.c_void_p),
                 ("w", C.c_void_p), ("lora_a", C.c_void_p), ("lora_b", C.c_void_p), ("factors", C.c_void_p), ("adapter", C.c_void_p),
                 ("n_rows", C.c_void_p), ("out", C.c_void_p)]
 

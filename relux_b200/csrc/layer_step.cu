@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(192, 1) skinny_gemm_sm100_kernel(const __grid_
           }
         const int n0 = (walk.col - prm.tile_first[j]) * kTileN;
         if (!in_items(walk)) {
-        mbar_expect_tx(&bars->full[s], SH::kStage);   // out-of-range parts of a box are zero-filled and still counted
-        tma_load_2d_hint(sw, &maps.w[j], n0, k * kTileK, &bars->full[s], policy);
-        tma_load_2d_hint(sw + kStageW / 2, &maps.w[j], n0 + 64, k * kTileK, &bars->full[s], policy);
+          mbar_expect_tx(&bars->full[s], SH::kStage);   // out-of-range parts of a box are zero-filled and still counted
+          tma_load_2d_hint(sw, &maps.w[j], n0, k * kTileK, &bars->full[s], policy);
+          tma_load_2d_hint(sw + kStageW / 2, &maps.w[j], n0 + 64, k * kTileK, &bars->full[s], policy);
         }
       }
       __syncwarp();

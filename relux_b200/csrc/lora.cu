@@ -241,10 +241,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_down_kernel(const DownPa
   }
 }
 
-enum Up { kPlain, kInTurns, kTInPieces, kHalves };   // the GEMM's blocks of rows come in turns; t comes in pieces, from the GEMM; every row is two of the GEMM's, M apart (in turns or not)
+// The GEMM's blocks of rows come in turns; t comes in pieces, from the GEMM; any of these, every row may be two of the GEMM's, M apart, and the columns those of a further launch (of its own: one sum more
+// for the first column took six registers, and 64 rows x 4096 x 6144, rank 16, 23.7 us for 22.4).
+enum Up { kPlain, kInTurns, kTInPieces, kAny };
 struct UpParams {
   const float* part;      // the GEMM's pieces [piece][M][N]; nullptr: no shared projection
-  int32_t first_block;    // of 256 columns, of this launch
+  int32_t halves, first_block;   // kAny: the GEMM's rows of a row less one; block of 256 columns that this launch begins with
   GemmRanges rg;
   const float* t;         // [M][rank], or (t_parts) in as many pieces [M][t_cols], of every adapter in use for every row
   int32_t t_parts, t_cols;
@@ -262,12 +264,11 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
   constexpr int kStride = kRank + 8, kSlices = (kRank + 31) / 32;   // k slices of 32 (one, of 8 or 16, for small ranks)
   __shared__ __align__(16) uint16_t t_hi[kGroupRows * kStride], t_lo[kGroupRows * kStride];
   __shared__ int32_t rows[kGroupRows];
-  constexpr bool kTurns = kUp == kInTurns || kUp == kHalves, kFew = kUp == kTInPieces;
-  constexpr int kOf = kUp == kHalves ? 2 : 1;   // the GEMM's rows of a row
+  constexpr bool kTurns = kUp == kInTurns || kUp == kAny, kFew = kUp == kTInPieces || kUp == kAny;
   chain_release();
   const int slot = group_rows(list, blockIdx.x, rows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = (p.first_block + (int)blockIdx.y) * kUpCols + warp * 32, n = n0 + 8 * t;
+  const int n0 = ((kUp == kAny ? p.first_block : 0) + (int)blockIdx.y) * kUpCols + warp * 32, n = n0 + 8 * t;
   // adapters were complete before the chain's head began: read ahead of the launches before this one
   uint4 w[kSlices][4];
   float factor = 1.f;
@@ -325,11 +326,15 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
     const int row = rows[8 * h + g];
     if (row < 0 || n >= p.N) continue;
     const size_t at = (size_t)row * p.N + n;
-#pragma unroll
-    for (int o = 0; o < kOf; o++) {
-      const int pieces = !p.part ? 1 : kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row + o * p.M)) : same;
+    if constexpr (kUp == kAny) {
+      for (int o = 0; o <= p.halves; o++) {
+        const int pieces = p.part ? p.rg.pieces(p.rg.tile_of(col_tile, row + o * p.M)) : 1;
+        for (int s = o ? 0 : 1; s < pieces; s++) add_f32(h, p.part + ((size_t)s * (1 + p.halves) + o) * p.M * p.N + at);
+      }
+    } else {
+      const int pieces = !p.part ? 1 : kTurns ? p.rg.pieces(p.rg.tile_of(col_tile, row)) : same;
 #pragma unroll 2
-      for (int s = o ? 0 : 1; s < pieces; s++) add_f32(h, p.part + ((size_t)s * kOf + o) * p.M * p.N + at);
+      for (int s = 1; s < pieces; s++) add_f32(h, p.part + (size_t)s * p.M * p.N + at);
     }
     if (p.adds) {
       if (p.out_bf16) {
@@ -345,8 +350,10 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
     for (int i = threadIdx.x; i < kGroupRows * kRank / 4; i += kLoraThreads) {
       const int at = 4 * i / kRank, r = 4 * i % kRank, row = rows[at];
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      bool whole = true;
       if constexpr (List::kNamesRows && kFew) {
-        if (row >= 0) {
+        whole = kUp == kAny && !p.t_parts;
+        if (row >= 0 && !whole) {
           const float* src = p.t + (size_t)row * p.t_cols + used_of(list, blockIdx.x) * kRank + r;
 #pragma unroll 8
           for (int s = 0; s < p.t_parts; s++) {
@@ -354,9 +361,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const UpParams p,
             v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
           }
         }
-      } else {
-        if (row >= 0) v = load_chained(reinterpret_cast<const float4*>(p.t + (size_t)row * kRank + r));
       }
+      if (row >= 0 && whole) v = load_chained(reinterpret_cast<const float4*>(p.t + (size_t)row * kRank + r));
       uint2 hi, lo;
       split_halves(v, factor, hi, lo);
       *reinterpret_cast<uint2*>(t_hi + at * kStride + r) = hi;
@@ -495,7 +501,7 @@ int32_t launch_down(Pool* p, const DownParams& prm, const List& list, int groups
   return kind == kBf16 ? go(lora_down_kernel<kSlice, kBf16, List>) : kind == kRounded ? go(lora_down_kernel<kSlice, kRounded, List>) : go(lora_down_kernel<kSlice, kSplit, List>);
 }
 template <int kRank, class List>
-int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups, bool halves) {
+int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups) {
   const bool chained = p->tune.get(RELUX_TUNE_CHAINED_LAUNCHES) != 0;
   const int blocks = (prm.N + kUpCols - 1) / kUpCols;
   for (prm.first_block = 0; prm.first_block < blocks; prm.first_block += kMostGridY) {
@@ -505,11 +511,12 @@ int32_t launch_up(Pool* p, UpParams prm, const List& list, int groups, bool halv
       return RELUX_OK;
     };
     int32_t rc;
-    if constexpr (std::is_same_v<List, RowList<kFewRows>>)   // one block of rows
-      rc = halves ? go(lora_up_kernel<kRank, kHalves, List>) : prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
+    if (prm.halves || blocks > kMostGridY)
+      rc = go(lora_up_kernel<kRank, kAny, List>);
+    else if constexpr (std::is_same_v<List, RowList<kFewRows>>)   // one block of rows
+      rc = prm.t_parts ? go(lora_up_kernel<kRank, kTInPieces, List>) : go(lora_up_kernel<kRank, kPlain, List>);
     else
-      rc = halves ? go(lora_up_kernel<kRank, kHalves, List>)
-                  : prm.part && prm.rg.in_turns() ? go(lora_up_kernel<kRank, kInTurns, List>) : go(lora_up_kernel<kRank, kPlain, List>);
+      rc = prm.part && prm.rg.in_turns() ? go(lora_up_kernel<kRank, kInTurns, List>) : go(lora_up_kernel<kRank, kPlain, List>);
     if (rc) return rc;
     count_launch(p->dev);
   }
@@ -617,7 +624,7 @@ void plan_lora(const Pool* p, const relux_matmul_lora_args* a, LoraPlan* plan) {
     return;
   }
   // float32 rows in two halves, as twice as many rows of the projection: what it is for is the bits (bf16 results, against 64 bits: 1.65e-3 off, rounded rows 2.4e-3).  No form of its own:
-  // rank 16, 9 rows x 4096 x 4096 22.3 us (rounded 17.7), 64 x 4096 x 6144 31.5 (25.9), 700 x 4096 x 4096 62 (43); 8192 rows, rank 8, 560 (239).
+  // rank 16, 9 rows x 4096 x 4096 22.8 us (rounded 17.7), 64 x 4096 x 6144 34.0 (25.4), 700 x 4096 x 4096 64 (43); 8192 rows, rank 8, 565 (239).
   if (a->w && !x_bf16 && a->x_halves) {
     plan->form = Form::kGroups;
     plan->halves = true;
@@ -745,12 +752,13 @@ int32_t do_matmul_lora(Pool* p, const relux_matmul_lora_args* a) {
   up.b = (const uint16_t*)a->lora_b;
   up.factors = a->factors;
   up.out = a->out;
+  up.halves = plan.halves;
   up.M = a->m;
   up.N = a->n;
   up.out_bf16 = a->out_dtype == RELUX_DTYPE_BF16;
   up.adds = a->accumulate != 0;
   return with_rank(a->rank, [&](auto r) {
-    return for_lists(a->m, requests, [&](const auto& list, int groups) { return launch_up<decltype(r)::value>(p, up, list, groups, plan.halves); });
+    return for_lists(a->m, requests, [&](const auto& list, int groups) { return launch_up<decltype(r)::value>(p, up, list, groups); });
   });
 }
 

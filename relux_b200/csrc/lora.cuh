@@ -18,7 +18,7 @@ struct LoraTiles {
   int16_t rows[kMaxLoraTiles];
 };
 
-// f v as two bf16 halves, 16 bits of it.  Both have its sign and neither is zero where it is not: the first is the largest of smaller magnitude, the second the rest.  So an infinity that
+// f v as two bf16 halves, 16 bits of it.  Both have its sign, and not both are zero where it is not (down to 2^-133): the first is the largest of smaller magnitude, the second the rest.  So an infinity that
 // they are multiplied with comes out as the formula has it (with the nearest value first the rest is zero or of the other sign, and the sum of both products NaN).  Of an infinity the
 // first half is the largest number and the rest the infinity; a NaN's rest is NaN.  The rest is up to 2^-7 of the value, rounded by 2^-9 of itself.
 __device__ __forceinline__ void split_halves(float4 v, float f, uint2& hi, uint2& lo) {
